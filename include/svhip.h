@@ -28,6 +28,9 @@ enum svhip_dtype { SVHIP_F32 = 0, SVHIP_BF16 = 1, SVHIP_FP8_E4M3 = 3, SVHIP_FP8_
 
 enum svhip_status { SVHIP_OK = 0, SVHIP_EINVAL = -1, SVHIP_ELAUNCH = -2, SVHIP_EWORKSPACE = -3 };
 
+/* How the pairs of a head turn: element i with i + pairs, 2 i with 2 i + 1, or the three axes of svhip_axial_rope. */
+enum svhip_rotary_layout { SVHIP_ROTARY_NONE = 0, SVHIP_ROTARY_HALF = 1, SVHIP_ROTARY_INTERLEAVED = 2, SVHIP_ROTARY_AXIAL = 3 };
+
 enum svhip_lel_mode { SVHIP_LEL_LAYER = 0, SVHIP_LEL_BAND = 1, SVHIP_LEL_COLUMN = 2 };
 
 /* Library version (major * 10000 + minor * 100 + patch) and the last error of the calling thread. */
@@ -415,6 +418,73 @@ int svhip_sample_chosen(const void* logits, int dtype, int64_t classes, int64_t 
                         int64_t stride_c, int64_t stride_n, const uint8_t* chosen, int64_t* tokens, int16_t* values,
                         const int64_t* seed, const int64_t* step, int* err, int64_t batch, int64_t Y, int64_t Z,
                         int64_t X, void* stream);
+
+/*
+ * Rotary positions: out[b, h, n] = x[b, h, n] with its first 2 `pairs` elements turned, the rest kept. Pair i turns by
+ * p freq[i] radians, p = positions[b, n] (int32, or int64 when positions_wide; any sign), and is scaled by `amplitude`:
+ *   y_a = amplitude (x_a cos - x_b sin), y_b = amplitude (x_b cos + x_a sin),
+ * (a, b) = (i, i + pairs) for SVHIP_ROTARY_HALF, (2 i, 2 i + 1) for SVHIP_ROTARY_INTERLEAVED. The turns are formed in 64
+ * bits, the rest is fp32, rounded once to the type. `inverse`: the transposed rotation, which takes the gradient of out
+ * to the gradient of x. x, out: bf16 or fp32 (dtype), element (b, h, n, d) at b*s_b + h*s_h + n*s_n + d; out may be x
+ * with the same strides. freq: fp64 [pairs], pairs <= 128.
+ * Beside svhip_axial_rope; no counterpart in the reference, whose positions have three axes.
+ */
+int svhip_rotary(const void* x, void* out, int dtype, const void* positions, int positions_wide, const double* freq,
+                 int64_t pairs, int layout, float amplitude, int inverse, int64_t B, int64_t H, int64_t N, int64_t D,
+                 int64_t sx_b, int64_t sx_h, int64_t sx_n, int64_t so_b, int64_t so_h, int64_t so_n, int64_t sp_b,
+                 int64_t sp_n, void* stream);
+
+/*
+ * A paged cache: pools k_pages, v_pages of `pages` pages, element (page, h, r, d) at page*s_p + h*s_h + r*s_r + d, rows r in
+ * [0, page_size), page_size a power of two from 16 to 1024; key j of window b is row j % page_size of page
+ * page_table[b*st_b + j / page_size] (int32, max_pages numbers a window). kv_dtype SVHIP_BF16, or SVHIP_FP8_E4M3: OCP
+ * e4m3fn codes with one power of two for each row and head, value = code 2^(exponent - 127), exponent bytes (page, h, r)
+ * at page*se_p + h*se_h + r. Windows may share pages that are only read.
+ *
+ * svhip_paged_append writes the new tokens' keys and values. Window b has N tokens, element (b, h, n, d) at b*s_b + h*s_h +
+ * n*s_n + d, or with cu_tokens (int32 [B + 1], ascending) the packed tokens [cu[b], cu[b + 1]) of N in all (s_b unused;
+ * tokens outside every window are left alone). lengths[b] (int32) counts the window's keys with these: token i of n goes
+ * to key lengths[b] - before - n + i, so `before` keys behind them are left to another call. `layout` rotates the keys on
+ * the way: SVHIP_ROTARY_HALF / _INTERLEAVED as svhip_rotary (freq fp64 [pairs]; positions int32 / int64 at b*sp_b + n*sp_n,
+ * or null: the key's index), SVHIP_ROTARY_AXIAL with svhip_axial_rope's arithmetic (positions fp32, three a token; freq
+ * fp32 [head_dim / 6]; pairs = head_dim / 2). e4m3: a row's exponent is the least with bound <= 448 2^(exponent - 127),
+ * bound = its largest magnitude, for rotated keys 1.5 max(1, |amplitude|) times it before the rotation.
+ * `bad` (int32, may be null) is set to 1 when a token's key lies outside the window's row of the table or its page outside
+ * the pool; such a token is not written. Key and value rows bf16, 16-byte aligned; rows of a page 16-byte aligned (e4m3:
+ * 8). head_dim a multiple of 8 up to 128.
+ * Beside svhip_kv_write (FastSlotForward.encode + _write, streamvoxel/stream/fast_ops.py:228-250), which rewrites a
+ * window's slab whole; no counterpart in the reference.
+ */
+int svhip_paged_append(const void* key, const void* value, int64_t sk_b, int64_t sk_h, int64_t sk_n, int64_t sv_b,
+                       int64_t sv_h, int64_t sv_n, int64_t B, int64_t H, int64_t N, int64_t D, const int32_t* cu_tokens,
+                       int64_t before, void* k_pages, void* v_pages, uint8_t* k_exponents, uint8_t* v_exponents,
+                       int kv_dtype, int64_t pages, int64_t page_size, int64_t sck_p, int64_t sck_h, int64_t sck_r,
+                       int64_t scv_p, int64_t scv_h, int64_t scv_r, int64_t sek_p, int64_t sek_h, int64_t sev_p,
+                       int64_t sev_h, const int32_t* page_table, int64_t st_b, int64_t max_pages, const int32_t* lengths,
+                       int layout, const void* positions, int positions_wide, int64_t sp_b, int64_t sp_n,
+                       const void* freq, int64_t pairs, float amplitude, int32_t* bad, void* stream);
+
+/*
+ * Attention of the windows' new tokens over a paged cache: out[b, h, i] = softmax_j(scale q[b, h, i] . k_j) v_j over the keys
+ * j < lengths[b] of key head h / (H / Hkv), with `causal` only j <= lengths[b] - n + i (n tokens of window b, its last
+ * keys); no key: zeros. Queries and out bf16, N a window or packed by cu_queries, as in svhip_paged_append (rows outside
+ * every window are left as they are). Products in bf16 on the matrix cores with fp32 sums, softmax weights rounded to
+ * bf16. `bad` is set to 1 when a page lies outside the pool (its keys and values then read as zeros) or lengths[b] passes
+ * the window's row of the table (and is cut to it). scale > 0. Query rows 16-byte aligned, rows of out 8, rows of a page as
+ * in svhip_paged_append. workspace: svhip_paged_attention_workspace_bytes with max_keys = max_pages * page_size (0: none
+ * needed), N and packed (cu_queries or not) as in the call; 16-byte aligned.
+ * Beside svhip_xattn_fwd (streamvoxel/stream/fast_ops.py:104-108); no counterpart in the reference.
+ */
+size_t svhip_paged_attention_workspace_bytes(int64_t B, int64_t H, int64_t Hkv, int64_t N, int packed, int64_t D,
+                                             int64_t max_keys);
+int svhip_paged_attention(const void* q, const void* k_pages, const void* v_pages, const uint8_t* k_exponents,
+                          const uint8_t* v_exponents, void* out, int kv_dtype, int64_t B, int64_t H, int64_t Hkv,
+                          int64_t N, int64_t D, const int32_t* cu_queries, int64_t pages, int64_t page_size,
+                          const int32_t* page_table, int64_t st_b, int64_t max_pages, const int32_t* lengths,
+                          int64_t sq_b, int64_t sq_h, int64_t sq_n, int64_t sk_p, int64_t sk_h, int64_t sk_r,
+                          int64_t sv_p, int64_t sv_h, int64_t sv_r, int64_t sek_p, int64_t sek_h, int64_t sev_p,
+                          int64_t sev_h, int64_t so_b, int64_t so_h, int64_t so_n, int causal, float scale, int32_t* bad,
+                          void* workspace, size_t workspace_bytes, void* stream);
 
 #ifdef __cplusplus
 }

@@ -5,6 +5,7 @@ call fails, a RuntimeError is raised.
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import os
 import threading
@@ -15,6 +16,7 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(HERE, 'libsvhip.so')
 
 SVHIP_F32, SVHIP_BF16, SVHIP_FP8_E4M3, SVHIP_FP8_E4M3_PFP8 = 0, 1, 3, 5
+SVHIP_ROTARY_NONE, SVHIP_ROTARY_HALF, SVHIP_ROTARY_INTERLEAVED, SVHIP_ROTARY_AXIAL = 0, 1, 2, 3
 SVHIP_LEL_LAYER, SVHIP_LEL_BAND, SVHIP_LEL_COLUMN = 0, 1, 2
 
 _c_i64, _c_i32, _c_p, _c_sz, _c_f, _c_d = (ctypes.c_int64, ctypes.c_int32, ctypes.c_void_p, ctypes.c_size_t,
@@ -81,6 +83,15 @@ SIGNATURES = {
                             + [_c_i64] * 12 + [_c_f, _c_p]),
     'svhip_patch_embed': (ctypes.c_int, [_c_p] * 5 + [_c_i64] * 10 + [_c_p]),
     'svhip_sample_chosen': (ctypes.c_int, [_c_p, ctypes.c_int] + [_c_i64] * 5 + [_c_p] * 6 + [_c_i64] * 4 + [_c_p]),
+    'svhip_rotary': (ctypes.c_int, [_c_p, _c_p, ctypes.c_int, _c_p, ctypes.c_int, _c_p, _c_i64, ctypes.c_int, _c_f,
+                                    ctypes.c_int] + [_c_i64] * 12 + [_c_p]),
+    'svhip_paged_append': (ctypes.c_int, [_c_p, _c_p] + [_c_i64] * 10 + [_c_p, _c_i64] + [_c_p] * 4 + [ctypes.c_int]
+                           + [_c_i64] * 12 + [_c_p, _c_i64, _c_i64, _c_p, ctypes.c_int, _c_p, ctypes.c_int, _c_i64,
+                                              _c_i64, _c_p, _c_i64, _c_f, _c_p, _c_p]),
+    'svhip_paged_attention_workspace_bytes': (_c_sz, [_c_i64] * 4 + [ctypes.c_int] + [_c_i64] * 2),
+    'svhip_paged_attention': (ctypes.c_int, [_c_p] * 6 + [ctypes.c_int] + [_c_i64] * 5 + [_c_p, _c_i64, _c_i64, _c_p,
+                                                                                      _c_i64, _c_i64, _c_p]
+                              + [_c_i64] * 16 + [ctypes.c_int, _c_f, _c_p, _c_p, _c_sz, _c_p]),
 }
 
 _lib = None
@@ -128,6 +139,19 @@ def require_gpu(*tensors):
         if t is not None and (not torch.is_tensor(t) or not t.is_cuda):
             raise RuntimeError('streamvoxel_amd kernels take GPU tensors (got %s); there is no CPU path'
                                % (t.device if torch.is_tensor(t) else type(t).__name__))
+
+
+def require_same_device(first, *tensors):
+    for t in tensors:
+        if t is not None and t.device != first.device:
+            raise ValueError(f'tensors on {first.device} and {t.device}: one call takes one device')
+
+
+def device_of(t):
+    """A context in which launches go to the tensor's device, whatever the current one is."""
+    if t.device.index == torch.cuda.current_device():
+        return contextlib.nullcontext()
+    return torch.cuda.device(t.device)
 
 
 def dtype_code(dtype):

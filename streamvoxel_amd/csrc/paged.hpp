@@ -1,0 +1,91 @@
+// A paged cache of keys and values: key j of window b is row j % S of page table[b][j / S] of a pool [pages, H, S, D], S a
+// power of two. bf16 rows, or OCP e4m3fn rows with one power of two for each row and head, held as its exponent's byte
+// (value = code 2^(byte - 127)): scaling by it is exact, so an e4m3 row decodes to bf16 without a second rounding and the
+// row's scale takes part in neither product of the attention.
+#pragma once
+
+#include "common.hpp"
+
+namespace svhip {
+
+constexpr int kMinPage = 16;
+constexpr int kMaxPage = 1024;
+
+struct Pages {
+  const int32_t* table;   // [B, max_pages], rows st_b apart
+  int64_t st_b, max_pages, pages;
+  int shift;              // log2 of the page size
+  const int32_t* lengths;
+  int32_t* bad;           // set to 1 where a page lies outside the pool or a window outside its row of the table; or null
+};
+
+__device__ __forceinline__ void set_bad(const Pages& p) {
+  if (p.bad) *p.bad = 1;
+}
+
+// Page of key j of window b, or -1 (and the flag) for a number outside the pool. j lies inside the table's row.
+__device__ __forceinline__ int64_t page_of(const Pages& p, int64_t b, int64_t j) {
+  const int32_t page = p.table[b * p.st_b + (j >> p.shift)];
+  if (page >= 0 && page < p.pages) return page;
+  set_bad(p);
+  return -1;
+}
+
+// Keys of window b: its length, cut to what its row of the table can name.
+__device__ __forceinline__ int64_t held_keys(const Pages& p, int64_t b) {
+  const int64_t L = p.lengths[b], most = p.max_pages << p.shift;
+  if (L > most) set_bad(p);
+  return L < 0 ? 0 : (L > most ? most : L);
+}
+
+// The windows' new tokens: N of each, or packed [0, T) with the windows' borders.
+struct Tokens {
+  const int32_t* cu;  // [B + 1] or null
+  int64_t B, N;       // N: tokens of a window, or T
+};
+
+// Border i of the packed windows, inside [0, T].
+__device__ __forceinline__ int64_t border(const Tokens& t, int64_t i) {
+  const int64_t c = t.cu[i];
+  return c < 0 ? 0 : (c > t.N ? t.N : c);
+}
+
+// First token and count of window b.
+__device__ __forceinline__ void window_tokens(const Tokens& t, int64_t b, int64_t& first, int64_t& count) {
+  if (!t.cu) {
+    first = b * t.N;
+    count = t.N;
+    return;
+  }
+  first = border(t, b);
+  const int64_t end = border(t, b + 1);
+  count = end > first ? end - first : 0;
+}
+
+// Window of packed token i (borders ascending), or -1 for one in front of the first border or behind the last.
+__device__ __forceinline__ int64_t window_of(const Tokens& t, int64_t i) {
+  if (i < t.cu[0] || i >= t.cu[t.B]) return -1;
+  int64_t lo = 0, hi = t.B;  // cu[lo] <= i < cu[hi]
+  while (hi - lo > 1) {
+    const int64_t mid = (lo + hi) >> 1;
+    (t.cu[mid] <= i ? lo : hi) = mid;
+  }
+  return lo;
+}
+
+// Exponent byte of a row whose magnitudes are at most `bound`: of the least power of two with bound <= 448 2^e.
+__device__ __forceinline__ int row_exponent(float bound) {
+  const uint32_t u = __float_as_uint(bound);
+  const int e = static_cast<int>(u >> 23) - ((u & 0x7fffffu) <= 0x600000u ? 8 : 7);
+  return e < 1 ? 1 : (e > 254 ? 254 : e);
+}
+
+__device__ __forceinline__ float exponent_value(int code) { return __uint_as_float(static_cast<uint32_t>(code) << 23); }
+
+inline int page_shift(int64_t page) {
+  int s = 0;
+  while ((1ll << s) < page) ++s;
+  return s;
+}
+
+}  // namespace svhip

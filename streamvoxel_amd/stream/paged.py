@@ -1,0 +1,176 @@
+"""A paged cache of keys and values on the HIP kernels: the append that fills it, the attention over it, and the context
+that stands in `CachedContext`'s place with its windows in one pool of pages.
+
+`step.CachedContext` (PackedKeys, streamvoxel/stream/fast_ops.py:122-159) keeps a slab of the longest condition for every
+slot and rewrites it whole; here a window holds the pages that its keys fill, and new keys go behind the ones that are
+there. No counterpart in the reference.
+"""
+from __future__ import annotations
+
+import math
+
+import torch
+
+from streamvoxel_amd import _lib
+
+__all__ = ['paged_append', 'paged_attention', 'PagedContext']
+
+LAYOUTS = {None: _lib.SVHIP_ROTARY_NONE, 'half': _lib.SVHIP_ROTARY_HALF, 'interleaved': _lib.SVHIP_ROTARY_INTERLEAVED,
+           'axial': _lib.SVHIP_ROTARY_AXIAL}
+
+
+def _check_pool(k_pages, v_pages, page_table, lengths, k_exponents, v_exponents, bad):
+    """The pool's type code; ValueError / TypeError for what the kernels do not take."""
+    if k_pages.dim() != 4 or v_pages.shape != k_pages.shape or v_pages.dtype != k_pages.dtype:
+        raise ValueError('k_pages and v_pages must be [pages, heads, page, head_dim] alike')
+    if k_pages.stride(-1) != 1 or v_pages.stride(-1) != 1:
+        raise ValueError('rows of a page need a contiguous head_dim')
+    if page_table.dtype != torch.int32 or page_table.dim() != 2 or page_table.stride(-1) != 1:
+        raise ValueError('page_table must be int32 [B, pages of a window] with contiguous rows')
+    if lengths.dtype != torch.int32 or lengths.shape != page_table.shape[:1] or not lengths.is_contiguous():
+        raise ValueError('lengths must be a contiguous int32 [B]')
+    if bad is not None and (bad.dtype != torch.int32 or bad.numel() != 1):
+        raise ValueError('bad must be one int32')
+    if k_pages.dtype == torch.bfloat16:
+        if k_exponents is not None or v_exponents is not None:
+            raise TypeError('bf16 pages take no exponents')
+        return _lib.SVHIP_BF16
+    if k_pages.dtype != torch.float8_e4m3fn:
+        raise TypeError(f'pages of {k_pages.dtype} unsupported (bfloat16 or float8_e4m3fn)')
+    for e in (k_exponents, v_exponents):
+        if e is None or e.dtype != torch.uint8 or e.shape != k_pages.shape[:3] or e.stride(-1) != 1:
+            raise ValueError('e4m3 pages need k_exponents and v_exponents, uint8 [pages, heads, page] with contiguous rows')
+    return _lib.SVHIP_FP8_E4M3
+
+
+def _windows(t, cu, B, what):
+    """(heads, tokens, (stride of a window, of a head, of a token)) of [B,H,n,D], or packed [H,T,D] with borders cu."""
+    if cu is None:
+        if t.dim() != 4 or t.shape[0] != B:
+            raise ValueError(f'{what} must be [B, heads, n, head_dim] with the B windows of the table, or packed '
+                             '[heads, T, head_dim] with their borders')
+        return t.shape[1], t.shape[2], (t.stride(0), t.stride(1), t.stride(2))
+    if cu.dtype != torch.int32 or cu.shape != (B + 1,) or not cu.is_contiguous():
+        raise ValueError('the borders must be a contiguous int32 [B + 1]')
+    if t.dim() != 3:
+        raise ValueError(f'packed {what} must be [heads, T, head_dim]')
+    return t.shape[0], t.shape[1], (0, t.stride(0), t.stride(1))
+
+
+def _rows16(t):
+    """bf16 rows on 16-byte boundaries: the tensor itself, or a contiguous copy."""
+    if t.stride(-1) == 1 and t.data_ptr() % 16 == 0 and all(s % 8 == 0 for s in t.stride()[:-1]):
+        return t
+    return t.contiguous() if not t.is_contiguous() or t.data_ptr() % 16 else t.clone()
+
+
+def _exponents(e):
+    return (0, 0) if e is None else (e.stride(0), e.stride(1))
+
+
+def paged_append(key, value, k_pages, v_pages, page_table, lengths, cu_tokens=None, before=0, positions=None,
+                 frequencies=None, layout='half', amplitude=1.0, k_exponents=None, v_exponents=None, bad=None):
+    """The windows' new keys and values into their rows of a paged cache, the keys rotated on the way.
+
+    key, value bf16 [B,H,n,D] (head_dim contiguous, any other strides), or packed [H,T,D] with the windows' borders
+    `cu_tokens` int32 [B+1] (device, ascending; tokens outside every window are left alone). k_pages, v_pages
+    [pages,H,page,D] in bf16, or float8_e4m3fn with `k_exponents` / `v_exponents` uint8 [pages,H,page], one power of two
+    2^(exponent - 127) for each row (written too); page a power of two from 16 to 1024. page_table int32 [B, m]: key j of
+    window b is row j % page of page page_table[b, j // page]. `lengths` int32 [B] (device) counts each window's keys with
+    the new ones: they are its last n keys, or the n in front of its last `before`. Two tokens must not share a row.
+    `frequencies` rotates the keys: with layout 'half' / 'interleaved' as `rotary` does (fp64; `positions` int32 / int64 [B,n]
+    or [T], or None: each key's index in its window; `amplitude`), with 'axial' as `producer.axial_rope` does (its fp32
+    buffer and fp32 positions [B,n,3] or [T,3]). `bad` (optional int32 [1], device) becomes 1 when a key lies outside
+    its window's row of the table or a page outside the pool; such keys are not written."""
+    _lib.require_gpu(key, value, k_pages, v_pages, page_table, lengths, cu_tokens, positions, frequencies, k_exponents,
+                     v_exponents, bad)
+    _lib.require_same_device(key, value, k_pages, v_pages, page_table, lengths, cu_tokens, positions, frequencies,
+                             k_exponents, v_exponents, bad)
+    code = _check_pool(k_pages, v_pages, page_table, lengths, k_exponents, v_exponents, bad)
+    if key.dtype != torch.bfloat16 or value.dtype != torch.bfloat16:
+        raise TypeError('key and value must be bfloat16')
+    key, value = _rows16(key), _rows16(value)
+    B = page_table.shape[0]
+    H, n, sk = _windows(key, cu_tokens, B, 'key')
+    sv = _windows(value, cu_tokens, B, 'value')[2]
+    P, Hp, S, D = k_pages.shape
+    if value.shape != key.shape or H != Hp or key.shape[-1] != D:
+        raise ValueError('key and value must be alike, with the heads and the head_dim of the pages')
+    if before < 0:
+        raise ValueError('before counts keys')
+    wide, pairs, sp, turn = 0, 0, (0, 0), _lib.SVHIP_ROTARY_NONE
+    if frequencies is not None:
+        if layout not in ('half', 'interleaved', 'axial'):
+            raise ValueError("layout is 'half', 'interleaved' or 'axial'")
+        turn, tokens = LAYOUTS[layout], (n,) if cu_tokens is not None else (B, n)
+        if layout == 'axial':
+            if frequencies.dtype != torch.float32 or frequencies.numel() * 6 != D or not frequencies.is_contiguous():
+                raise ValueError('frequencies must be the fp32 [head_dim / 6] buffer')
+            if positions is None or positions.dtype != torch.float32 or tuple(positions.shape) != (*tokens, 3) or (
+                    positions.stride(-1) != 1):
+                raise ValueError("the 'axial' layout needs fp32 positions, three a token")
+            pairs = D // 2
+        else:
+            if frequencies.dtype != torch.float64 or frequencies.dim() != 1 or not frequencies.is_contiguous():
+                raise ValueError('frequencies must be a contiguous fp64 vector')
+            pairs = frequencies.numel()
+            if not 1 <= pairs <= D // 2:
+                raise ValueError(f'{pairs} frequencies do not fit head_dim {D}')
+            if positions is not None and (positions.dtype not in (torch.int32, torch.int64)
+                                          or tuple(positions.shape) != tokens):
+                raise ValueError('positions must be int32 or int64, one a token')
+        if positions is not None:
+            wide = int(positions.dtype == torch.int64)
+            sp = (0, positions.stride(0)) if cu_tokens is not None else (positions.stride(0), positions.stride(1))
+    elif positions is not None:
+        raise ValueError('rotating the keys needs frequencies')
+    with _lib.device_of(key):
+        _lib.check(_lib.load().svhip_paged_append(
+            _lib.ptr(key), _lib.ptr(value), *sk, *sv, B, H, n, D, _lib.ptr(cu_tokens), before, _lib.ptr(k_pages),
+            _lib.ptr(v_pages), _lib.ptr(k_exponents), _lib.ptr(v_exponents), code, P, S, *k_pages.stride()[:3],
+            *v_pages.stride()[:3], *_exponents(k_exponents), *_exponents(v_exponents), _lib.ptr(page_table),
+            page_table.stride(0), page_table.shape[1], _lib.ptr(lengths), turn, _lib.ptr(positions), wide, *sp,
+            _lib.ptr(frequencies), pairs, float(amplitude), _lib.ptr(bad), _lib.stream_of(key)), 'svhip_paged_append')
+
+
+def paged_attention(query, k_pages, v_pages, page_table, lengths, cu_queries=None, causal=False, scale=None,
+                    k_exponents=None, v_exponents=None, out=None, bad=None):
+    """softmax(scale * Q K^T) V of the windows' new tokens over the first lengths[b] keys of their pages.
+
+    query bf16 [B,H,n,D] (head_dim contiguous, any other strides), or packed [H,T,D] with the windows' borders `cu_queries`
+    int32 [B+1] (device, ascending). k_pages, v_pages, page_table, lengths and the exponents as `paged_append` fills them;
+    the H heads share the pages' heads evenly, head h reads head h // (H / heads). `causal`: the n tokens are the window's
+    last n keys, and token i sees keys up to its own, lengths[b] - n + i; without it every token sees all of them. A token
+    with no key gets zeros. `out` (optional) bf16 like query with a contiguous head_dim; its rows outside every window are
+    left as they are (a fresh one has them undefined). `bad` (optional int32 [1], device) becomes 1 when a page lies
+    outside the pool (its keys and values read as zeros) or a length passes the window's row of the table (and is cut).
+    Returns out."""
+    _lib.require_gpu(query, k_pages, v_pages, page_table, lengths, cu_queries, k_exponents, v_exponents, out, bad)
+    _lib.require_same_device(query, k_pages, v_pages, page_table, lengths, cu_queries, k_exponents, v_exponents, out, bad)
+    code = _check_pool(k_pages, v_pages, page_table, lengths, k_exponents, v_exponents, bad)
+    if query.dtype != torch.bfloat16:
+        raise TypeError('query must be bfloat16')
+    query = _rows16(query)
+    B = page_table.shape[0]
+    H, n, sq = _windows(query, cu_queries, B, 'query')
+    P, Hkv, S, D = k_pages.shape
+    if query.shape[-1] != D or Hkv == 0 or H % Hkv:
+        raise ValueError("query needs the pages' head_dim, and heads that share theirs evenly")
+    if out is None:
+        out = torch.empty(query.shape, dtype=torch.bfloat16, device=query.device)
+    if out.shape != query.shape or out.dtype != torch.bfloat16 or out.stride(-1) != 1:
+        raise ValueError('out must be bf16 like query with a contiguous head_dim')
+    so = _windows(out, cu_queries, B, 'out')[2]
+    scale = 1.0 / math.sqrt(D) if scale is None else float(scale)
+    lib = _lib.load()
+    m = page_table.shape[1]
+    nbytes = int(lib.svhip_paged_attention_workspace_bytes(B, H, Hkv, n, cu_queries is not None, D, m * S))
+    with _lib.device_of(query):
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=query.device) if nbytes else None
+        _lib.check(lib.svhip_paged_attention(
+            _lib.ptr(query), _lib.ptr(k_pages), _lib.ptr(v_pages), _lib.ptr(k_exponents), _lib.ptr(v_exponents),
+            _lib.ptr(out), code, B, H, Hkv, n, D, _lib.ptr(cu_queries), P, S, _lib.ptr(page_table), page_table.stride(0), m,
+            _lib.ptr(lengths), *sq, *k_pages.stride()[:3], *v_pages.stride()[:3], *_exponents(k_exponents),
+            *_exponents(v_exponents), *so, int(causal), scale, _lib.ptr(bad), _lib.ptr(ws), nbytes, _lib.stream_of(query)),
+            'svhip_paged_attention')
+    return out

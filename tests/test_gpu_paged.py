@@ -1,0 +1,525 @@
+"""The append to a paged cache and the attention over it on the GPU, against plain float64 on the host.
+
+Tolerances. Append, bf16: exact for values and unrotated keys; a rotated key is off by the fp32 rotation's 8 * 2^-24 of
+|x_a| + |x_b| (test_gpu_rotary.py) and half a step of bf16. e4m3: exponents exact, codes off by half a step, 2^-4 of the
+value or 2^-10 of the row's power of two below its normal range.
+Attention: the weights are rounded to bf16 (half a step, 2^-8, of each) for the second product, and the sum of them may or
+may not be: with A = softmax |v| both together are off by at most 2 * 2^-8 A. A score is an fp32 sum of exact products,
+off by D 2^-24 of scale sum |q k|, and the exponent's argument and the exponential by 4 * 2^-24 (1 + |score|) more, which
+moves the weights of a row by at most twice that, relatively. The result is rounded to bf16, 2^-8 of it."""
+import math
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+DEV = 'cuda:0'
+
+
+def _case(msg):
+    print(f'[gpu-case] {msg}', flush=True)
+
+
+class Pool:
+    """Pages in a scattered order, filled with values (NaN where no window's keys lie, unless `clean`)."""
+
+    def __init__(self, lengths, heads, D, page, seed, kv_dtype='bf16', spare=3, token_major=False, clean=False, spread=1.0):
+        g = torch.Generator().manual_seed(seed)
+        self.lengths, self.heads, self.D, self.page, self.fp8 = lengths, heads, D, page, kv_dtype == 'fp8'
+        need = [-(-max(L, 0) // page) for L in lengths]
+        self.pages = sum(need) + spare
+        order = torch.randperm(self.pages, generator=g).to(torch.int32)
+        self.table = torch.full((len(lengths), max(max(need, default=0), 1)), 0, dtype=torch.int32)
+        used = torch.zeros(self.pages, page, dtype=torch.bool)
+        at = 0
+        for b, n in enumerate(need):
+            self.table[b, :n] = order[at:at + n]
+            for j in range(n):
+                used[self.table[b, j], :min(page, lengths[b] - j * page)] = True
+            at += n
+        shape = (self.pages, heads, page, D)
+        k, v = torch.randn(shape, generator=g) * spread, torch.randn(shape, generator=g)
+        if not clean:
+            k[~used[:, None].expand(-1, heads, -1)] = math.nan
+            v[~used[:, None].expand(-1, heads, -1)] = math.nan
+        self.ke = self.ve = None
+        if self.fp8:
+            self.k, self.v = [(t * 64).clamp(-448, 448).to(torch.float8_e4m3fn) for t in (k, v)]
+            self.ke, self.ve = [torch.randint(119, 123, shape[:3], generator=g).to(torch.uint8) for _ in 'kv']
+        else:
+            self.k, self.v = k.to(torch.bfloat16), v.to(torch.bfloat16)
+        self.token_major = token_major
+
+    def device(self, t):
+        """On the GPU, as [pages, heads, page, D] of dense pages or of pages with a token's heads together."""
+        if t is None:
+            return None
+        if not self.token_major or t.dim() != 4:
+            return t.to(DEV)
+        return t.transpose(1, 2).contiguous().to(DEV).transpose(1, 2)
+
+    def args(self):
+        return (self.device(self.k), self.device(self.v), self.table.to(DEV),
+                torch.tensor(self.lengths, dtype=torch.int32, device=DEV))
+
+    def exponents(self):
+        return dict(k_exponents=self.device(self.ke), v_exponents=self.device(self.ve)) if self.fp8 else {}
+
+    def rows(self, b):
+        """Keys and values of window b in float64 [heads, L, D]."""
+        L = max(self.lengths[b], 0)
+        page = self.table[b, :-(-L // self.page)].long()
+        out = []
+        for t, e in ((self.k, self.ke), (self.v, self.ve)):
+            x = t.view(torch.uint8)[page].view(t.dtype).float().double() if self.fp8 else t[page].double()
+            if e is not None:
+                x = x * 2.0 ** (e[page].double() - 127)[..., None]
+            out.append(x.transpose(0, 1).reshape(self.heads, -1, self.D)[:, :L])
+        return out
+
+
+def attend64(q, k, v, causal, scale):
+    """(out, allowed error) of one window: q [H, n, D], k, v [heads, L, D] float64."""
+    H, n, D = q.shape
+    L, G = k.shape[1], H // k.shape[0]
+    if L == 0 or n == 0:
+        return torch.zeros_like(q), torch.zeros_like(q)
+    k, v = k.repeat_interleave(G, 0), v.repeat_interleave(G, 0)
+    s = scale * q @ k.transpose(1, 2)
+    off = 2.0 ** -24 * (D * scale * (q.abs() @ k.abs().transpose(1, 2)) + 4 * (1 + s.abs()))
+    if causal:
+        seen = torch.arange(L) <= (L - n + torch.arange(n))[:, None]
+        s = s.masked_fill(~seen, -math.inf)
+        off = off.masked_fill(~seen, 0.0)
+    w = (s - s.amax(-1, keepdim=True).clamp(min=-1e300)).exp()
+    total = w.sum(-1, keepdim=True)
+    w = torch.where(total > 0, w / total.clamp(min=1e-300), torch.zeros_like(w))
+    out, A = w @ v, w @ v.abs()
+    err = (2 * 2.0 ** -8 + 2 * off.amax(-1, keepdim=True)) * A
+    return out, err + 2.0 ** -8 * (out.abs() + err)
+
+
+def check(got, q, pool, causal, cu=None, scale=None):
+    """got, q [B, H, n, D] or packed [H, T, D]."""
+    scale = 1 / math.sqrt(pool.D) if scale is None else scale
+    got, q = got.cpu().double(), q.cpu().double()
+    for b in range(len(pool.lengths)):
+        cut = (lambda t: t[b]) if cu is None else (lambda t: t[:, cu[b]:cu[b + 1]])
+        out, err = attend64(cut(q), *pool.rows(b), causal, scale)
+        off = (cut(got) - out).abs()
+        assert not torch.isnan(off).any(), b
+        assert (off <= err).all(), (b, (off - err).max().item(), off.max().item())
+
+
+def queries(B, H, n, D, seed, spread=1.5):
+    g = torch.Generator().manual_seed(seed)
+    return (torch.randn(B, n, H, D, generator=g) * spread).to(torch.bfloat16).to(DEV).transpose(1, 2)
+
+
+LENGTHS = [[0, 1, 15, 16, 17], [63, 64, 65, 31, 33], [500, 129, 0, 700, 128], [3000], [1537, 40, 9000]]
+
+
+@pytest.mark.parametrize('kv_dtype', ['bf16', 'fp8'])
+@pytest.mark.parametrize('lengths', LENGTHS, ids=lambda x: '-'.join(map(str, x)))
+@pytest.mark.parametrize('n, causal', [(1, False), (1, True), (2, True), (7, False), (40, True), (130, True), (130, False)])
+@pytest.mark.parametrize('D, H, heads, page', [(64, 4, 4, 64), (48, 6, 2, 16), (128, 8, 1, 32), (96, 3, 3, 128),
+                                               (8, 2, 1, 1024), (72, 4, 2, 16)])
+def test_attention_against_float64(lengths, n, causal, D, H, heads, page, kv_dtype):
+    """Lengths around the tiles' and the pages' ends, empty windows, windows shorter than their tokens (rows that see
+    nothing), NaN in every row that holds no key."""
+    from streamvoxel_amd.stream.paged import paged_attention
+    _case(f'paged attention {lengths} n={n} causal={causal} D={D} H={H}/{heads} page={page} {kv_dtype}')
+    pool = Pool(lengths, heads, D, page, sum(lengths) + n, kv_dtype)
+    q = queries(len(lengths), H, n, D, n + D)
+    bad = torch.zeros(1, dtype=torch.int32, device=DEV)
+    got = paged_attention(q, *pool.args(), causal=causal, bad=bad, **pool.exponents())
+    assert int(bad) == 0
+    check(got, q, pool, causal)
+
+
+@pytest.mark.parametrize('kv_dtype', ['bf16', 'fp8'])
+@pytest.mark.parametrize('counts', [[1, 0, 5, 1, 1, 200, 33], [0, 0, 3], [1, 1, 1, 1], [129, 1]], ids=str)
+@pytest.mark.parametrize('D, H, heads, page', [(64, 4, 1, 16), (128, 4, 4, 64), (96, 8, 2, 32)])
+def test_packed_queries(counts, D, H, heads, page, kv_dtype):
+    """Windows of different token counts, none among them; rows in front of the first border and behind the last stay."""
+    from streamvoxel_amd.stream.paged import paged_attention
+    _case(f'packed {counts} D={D} H={H}/{heads} page={page} {kv_dtype}')
+    lengths = [n + 37 * i for i, n in enumerate(counts)]
+    pool = Pool(lengths, heads, D, page, 3, kv_dtype)
+    front, behind = 2, 5
+    cu = torch.tensor([0] + counts).cumsum(0) + front
+    T = int(cu[-1]) + behind
+    q = queries(1, H, T, D, 11)[0]
+    for causal in (True, False):
+        out = torch.full((T, H, D), 3.0, dtype=torch.bfloat16, device=DEV).transpose(0, 1)
+        got = paged_attention(q, *pool.args(), cu_queries=cu.to(torch.int32).to(DEV), causal=causal, out=out,
+                              **pool.exponents())
+        assert got is out
+        check(got, q, pool, causal, cu=cu.tolist())
+        assert (out[:, :front] == 3).all() and (out[:, T - behind:] == 3).all()
+
+
+@pytest.mark.parametrize('n', [1, 100])
+def test_attention_of_views(n):
+    """Pages with a token's heads together, queries and out in wider buffers, a table row wider than the windows need."""
+    from streamvoxel_amd.stream.paged import paged_attention
+    pool = Pool([300, 77, 1000], 2, 64, 32, 8, token_major=True)
+    k, v, table, lengths = pool.args()
+    wide = torch.full((3, 99), -7, dtype=torch.int32, device=DEV)
+    wide[:, :table.shape[1]] = table
+    q = torch.randn(3, n, 3, 6, 72, generator=torch.Generator().manual_seed(2)).to(torch.bfloat16).to(DEV)[:, :, 1, :, 8:]
+    q = q.transpose(1, 2)
+    out = torch.zeros(3, n, 6, 68, dtype=torch.bfloat16, device=DEV)
+    paged_attention(q, k, v, wide, lengths, out=out[..., 4:].transpose(1, 2), causal=True)
+    check(out[..., 4:].transpose(1, 2), q, pool, True)
+    assert (out[..., :4] == 0).all()
+    odd = torch.randn(3, n, 6, 65, generator=torch.Generator().manual_seed(2)).to(torch.bfloat16).to(DEV)[..., 1:]
+    odd = odd.transpose(1, 2)                                       # rows off the 16-byte boundaries: copied
+    check(paged_attention(odd, k, v, wide, lengths), odd, pool, False)
+
+
+@pytest.mark.parametrize('n', [1, 3, 64])
+def test_sharp_rows_and_score_jumps(n):
+    """Scores of standard deviation 30 and 10, one hot key in any place, scale given."""
+    from streamvoxel_amd.stream.paged import paged_attention
+    pool = Pool([2000, 65, 700], 2, 64, 16, 4, clean=True)
+    for hot in (0, 31, 32, 63, 64, 699):
+        pool.k[pool.table[2, hot // 16].long(), :, hot % 16] *= 8
+    q = queries(3, 4, n, 64, 6, spread=4.0)
+    check(paged_attention(q, *pool.args(), scale=0.9), q, pool, False, scale=0.9)
+    check(paged_attention(q, *pool.args(), scale=0.3, causal=True), q, pool, True, scale=0.3)
+
+
+@pytest.mark.parametrize('n', [1, 50])
+def test_infinite_and_nan_keys_touch_their_window_alone(n):
+    from streamvoxel_amd.stream.paged import paged_attention
+    pool = Pool([400, 400, 400], 1, 64, 64, 4, clean=True)
+    pool.k[pool.table[1, 3].long(), :, 7] = math.nan
+    q = queries(3, 2, n, 64, 6)
+    got = paged_attention(q, *pool.args())
+    assert torch.isnan(got[1]).all()
+    keep = Pool([400, 400, 400], 1, 64, 64, 4, clean=True)
+    same = paged_attention(q, *keep.args())
+    assert torch.equal(got[0], same[0]) and torch.equal(got[2], same[2])
+    check(same, q, keep, False)
+
+
+def test_windows_share_pages():
+    from streamvoxel_amd.stream.paged import paged_attention
+    pool = Pool([200, 260], 2, 64, 64, 4)
+    pool.table[0, :3] = pool.table[1, :3]
+    pool.lengths = [192, 260]
+    q = queries(2, 4, 5, 64, 1)
+    check(paged_attention(q, *pool.args(), causal=True), q, pool, True)
+
+
+@pytest.mark.parametrize('n', [1, 70])
+@pytest.mark.parametrize('kv_dtype', ['bf16', 'fp8'])
+def test_bad_pages_read_as_zeros_and_set_the_flag(n, kv_dtype):
+    from streamvoxel_amd.stream.paged import paged_attention
+    pool = Pool([300, 128, 64], 2, 64, 32, 4, kv_dtype, clean=True)
+    q = queries(3, 2, n, 64, 1)
+    k, v, table, lengths = pool.args()
+    for number in (-1, pool.pages, 2 ** 31 - 1, -2 ** 31):
+        bad = torch.zeros(1, dtype=torch.int32, device=DEV)
+        broken = table.clone()
+        broken[0, 2] = number
+        got = paged_attention(q, k, v, broken, lengths, bad=bad, **pool.exponents())
+        assert int(bad) == 1
+        zeroed = Pool([300, 128, 64], 2, 64, 32, 4, kv_dtype, clean=True)
+        zeroed.k.view(torch.uint8)[zeroed.table[0, 2].long()] = 0
+        zeroed.v.view(torch.uint8)[zeroed.table[0, 2].long()] = 0
+        check(got, q, zeroed, False)
+    bad = torch.zeros(1, dtype=torch.int32, device=DEV)
+    got = paged_attention(q, k, v, table, lengths + torch.tensor([1000, 0, 0], device=DEV, dtype=torch.int32), bad=bad,
+                          **pool.exponents())
+    assert int(bad) == 1
+    check(got[1:], q[1:], _tail(pool), False)
+
+
+def _tail(pool):
+    rest = Pool.__new__(Pool)
+    rest.__dict__.update(pool.__dict__, lengths=pool.lengths[1:], table=pool.table[1:])
+    return rest
+
+
+def test_negative_lengths_count_as_empty():
+    from streamvoxel_amd.stream.paged import paged_attention
+    pool = Pool([-5, 40], 1, 64, 16, 4)
+    for n in (1, 40):
+        q = queries(2, 1, n, 64, 1)
+        got = paged_attention(q, *pool.args(), causal=True)
+        assert (got[0] == 0).all()
+        check(got, q, pool, True)
+
+
+@pytest.mark.parametrize('kv_dtype', ['bf16', 'fp8'])
+def test_pools_past_32_bit_offsets(kv_dtype):
+    """Pages more than 2^32 bytes into the pool, written by the append and read by the attention."""
+    from streamvoxel_amd.stream.paged import paged_append, paged_attention
+    heads, D, page = 8, 128, 64
+    pages = (1 << 32) // (heads * D * page * (1 if kv_dtype == 'fp8' else 2)) + 40
+    dtype = torch.float8_e4m3fn if kv_dtype == 'fp8' else torch.bfloat16
+    k, v = [torch.empty(pages, heads, page, D, dtype=dtype, device=DEV) for _ in 'kv']
+    e = {}
+    if kv_dtype == 'fp8':
+        e = {n: torch.empty(pages, heads, page, dtype=torch.uint8, device=DEV) for n in ('k_exponents', 'v_exponents')}
+    table = torch.tensor([[pages - 1, 0, pages - 20], [pages - 2, pages - 3, 1]], dtype=torch.int32, device=DEV)
+    lengths = torch.tensor([180, 129], dtype=torch.int32, device=DEV)
+    g = torch.Generator().manual_seed(0)
+    key, value = [torch.randn(2, heads, 180, D, generator=g).to(torch.bfloat16).to(DEV) for _ in 'kv']
+    for b, n in ((0, 180), (1, 129)):
+        paged_append(key[b:b + 1, :, :n], value[b:b + 1, :, :n], k, v, table[b:b + 1], lengths[b:b + 1], **e)
+    small = Pool([180, 129], heads, D, page, 0, kv_dtype)
+    used = table.cpu().long()
+    small.table = torch.arange(6, dtype=torch.int32).view(2, 3)
+    take = lambda t: t.view(torch.uint8)[used.flatten().to(DEV)].cpu().view(t.dtype)
+    small.k, small.v = take(k), take(v)
+    if e:
+        small.ke, small.ve = take(e['k_exponents']), take(e['v_exponents'])
+    for n in (1, 90):
+        q = queries(2, heads, n, D, n)
+        check(paged_attention(q, k, v, table, lengths, causal=True, **e), q, small, True)
+
+
+# -------------------------------------------------------------------------------------------------------- append
+
+def turned64(x, positions, freq, layout, amplitude):
+    """(y, fp32 error) of keys [T, H, D] in float64."""
+    angle = positions.double()[:, None] * freq
+    c, s = (amplitude * angle.cos())[:, None], (amplitude * angle.sin())[:, None]
+    half = freq.numel()
+    i = torch.arange(half)
+    a, b = (i, i + half) if layout == 'half' else (2 * i, 2 * i + 1)
+    y, err = x.clone(), torch.zeros_like(x)
+    y[..., a], y[..., b] = x[..., a] * c - x[..., b] * s, x[..., b] * c + x[..., a] * s
+    err[..., a] = err[..., b] = 8 * 2.0 ** -24 * amplitude * (x[..., a].abs() + x[..., b].abs())
+    return y, err
+
+
+def exponent64(bound):
+    e = torch.ceil(torch.log2(bound.double() / 448)) + 127
+    return e.clamp(1, 254)
+
+
+def check_rows(got, code, want, err, bound):
+    """Rows [T, H, D] of the cache against want (float64) within err before rounding."""
+    if code is None:
+        assert ((got.double() - want).abs() <= err + 2.0 ** -8 * (want.abs() + err)).all()
+        return
+    assert torch.equal(code.double(), exponent64(bound))
+    scale = 2.0 ** (code.double() - 127)[..., None]
+    off = (got.float().double() * scale - want).abs()
+    assert (off <= err + torch.maximum(2.0 ** -4 * (want.abs() + err), 2.0 ** -10 * scale)).all()
+
+
+@pytest.mark.parametrize('kv_dtype', ['bf16', 'fp8'])
+@pytest.mark.parametrize('layout, part', [(None, 0), ('half', 1.0), ('half', 0.6), ('interleaved', 1.0), ('interleaved', 0.3)])
+@pytest.mark.parametrize('D, H, page', [(64, 4, 64), (48, 3, 16), (128, 1, 256), (8, 2, 32), (104, 5, 16)])
+@pytest.mark.parametrize('counts, packed, before', [([1, 1, 1], False, 0), ([40, 40, 40], False, 7), ([3, 0, 70, 1], True, 0)])
+def test_append_against_float64(counts, packed, before, D, H, page, layout, part, kv_dtype):
+    from streamvoxel_amd.stream.paged import paged_append
+    _case(f'append {counts} packed={packed} before={before} D={D} H={H} page={page} {layout} {part} {kv_dtype}')
+    held = [5, 100, 0, 64][:len(counts)]
+    lengths = [h + n + before for h, n in zip(held, counts)]
+    pool = Pool(lengths, H, D, page, 5, kv_dtype, clean=True)
+    k, v, table, dev_lengths = pool.args()
+    k0, v0 = k.clone(), v.clone()
+    g = torch.Generator().manual_seed(1)
+    T = sum(counts)
+    extra = 3 if packed else 0                                      # tokens behind the last window
+    key, value = [torch.randn(T + extra, H, D, generator=g).to(torch.bfloat16) for _ in 'kv']
+    if kv_dtype == 'fp8':
+        key[0], value[T // 2] = 0, 0
+        key[T - 1] *= 2.0 ** 100
+        value[T - 1] *= 2.0 ** -90
+    kw, amplitude = dict(pool.exponents()), 1.0
+    explicit = page == 16
+    where = torch.cat([torch.arange(L - before - n, L - before) for L, n in zip(lengths, counts)])
+    b = torch.cat([torch.full((n,), i) for i, n in enumerate(counts)])
+    positions = where
+    if layout:
+        pairs = max(1, int(D * part) // 2)
+        freq = 10000.0 ** (-torch.arange(pairs, dtype=torch.float64) / pairs)
+        amplitude = 1.2
+        kw.update(frequencies=freq.to(DEV), layout=layout, amplitude=amplitude)
+        if explicit:
+            positions = torch.randint(0, 5000, (T + extra,), generator=g)
+            kw['positions'] = positions.to(DEV) if packed else positions.view(len(counts), -1).to(torch.int32).to(DEV)
+            positions = positions[:T]
+    bad = torch.zeros(1, dtype=torch.int32, device=DEV)
+    dev = lambda t: t.to(DEV).transpose(0, 1) if packed else t.view(len(counts), -1, H, D).to(DEV).transpose(1, 2)
+    if packed:
+        kw['cu_tokens'] = torch.tensor([0] + counts).cumsum(0).to(torch.int32).to(DEV)
+    paged_append(dev(key), dev(value), k, v, table, dev_lengths, before=before, bad=bad, **kw)
+    assert int(bad) == 0
+    page_no, row = table.cpu().long()[b, where // page], where % page
+    x, y = key[:T].double(), value[:T].double()
+    err = torch.zeros_like(x)
+    reach = 1.0
+    if layout:
+        x, err = turned64(x, positions, freq, layout, amplitude)
+        reach = torch.tensor(1.5 * 1.2, dtype=torch.float32)
+    at = lambda t: t.view(torch.uint8).cpu().view(t.dtype)[page_no, :, row] if t.dtype != torch.float8_e4m3fn else (
+        t.view(torch.uint8).cpu()[page_no, :, row].view(torch.float8_e4m3fn))
+    code = (lambda t: t.cpu()[page_no, :, row]) if kv_dtype == 'fp8' else (lambda t: None)
+    check_rows(at(k), code(kw.get('k_exponents')) if kv_dtype == 'fp8' else None, x, err,
+               key[:T].float().abs().amax(-1) * reach)
+    check_rows(at(v), code(kw.get('v_exponents')) if kv_dtype == 'fp8' else None, y, torch.zeros_like(y),
+               value[:T].float().abs().amax(-1))
+    # Every other row stays.
+    mine = torch.zeros(pool.pages, page, dtype=torch.bool)
+    mine[page_no, row] = True
+    for now, then in ((k, k0), (v, v0)):
+        same = (now.view(torch.uint8) == then.view(torch.uint8)).view(pool.pages, H, page, -1).all(-1).cpu()
+        assert same[~mine[:, None].expand(-1, H, -1)].all()
+
+
+@pytest.mark.parametrize('kv_dtype', ['bf16', 'fp8'])
+def test_axial_append_has_the_bits_of_the_axial_rotation(kv_dtype):
+    from streamvoxel_amd.stream.paged import paged_append
+    from streamvoxel_amd.stream.producer import axial_rope, rope_frequencies
+    H, D, n = 3, 48, 77
+    g = torch.Generator().manual_seed(2)
+    key, value = [torch.randn(2, n, H, D, generator=g).to(torch.bfloat16).to(DEV).transpose(1, 2) for _ in 'kv']
+    positions = (torch.rand(2, n, 3, generator=g) * 64 - 8).to(DEV)
+    freq = rope_frequencies(D, device=DEV)
+    turned = axial_rope(key, positions, freq)
+    results = []
+    for how in (dict(positions=positions, frequencies=freq, layout='axial'), {}):
+        pool = Pool([n, n + 20], H, D, 32, 1, kv_dtype, clean=True)
+        k, v, table, lengths = pool.args()
+        e = pool.exponents()
+        paged_append(key if how else turned, value, k, v, table, lengths, **how, **e)
+        results.append((k, v, e))
+    (k, v, e), (k2, v2, e2) = results
+    if kv_dtype == 'bf16':
+        assert torch.equal(k, k2) and torch.equal(v, v2)
+    else:                                # the exponents of rotated keys are chosen before the rotation, and one larger
+        value_of = lambda t, x: t.float() * 2.0 ** (x.float() - 127)[..., None]
+        a, c = value_of(k, e['k_exponents']), value_of(k2, e2['k_exponents'])
+        step = 2.0 ** (e['k_exponents'].float() - 127)[..., None]
+        assert ((a - c).abs() <= torch.maximum(2 * 2.0 ** -4 * c.abs(), 2 * 2.0 ** -10 * step)).all()
+        assert torch.equal(v.view(torch.uint8), v2.view(torch.uint8))
+
+
+def test_append_outside_the_table_or_the_pool_writes_nothing():
+    from streamvoxel_amd.stream.paged import paged_append
+    pool = Pool([64, 64], 2, 64, 32, 1, clean=True)
+    k, v, table, lengths = pool.args()
+    key = torch.randn(2, 2, 4, 64, generator=torch.Generator().manual_seed(0)).to(torch.bfloat16).to(DEV)
+    for b, number in ((0, -1), (1, pool.pages), (0, 2 ** 31 - 1), (1, -2 ** 31)):
+        k1, v1, broken, bad = k.clone(), v.clone(), table.clone(), torch.zeros(1, dtype=torch.int32, device=DEV)
+        broken[b, 1] = number
+        paged_append(key, key, k1, v1, broken, lengths, bad=bad)
+        assert int(bad) == 1
+        where = table[b, 1].long()
+        assert torch.equal(k1[where], k[where]) and torch.equal(v1[where], v[where])
+        other = table[1 - b, 1].long()
+        assert torch.equal(k1[other][:, 28:], key[1 - b])
+    for off in (40, -64, -62):                                      # past the row's end, and in front of its first key
+        k1, v1, bad = k.clone(), v.clone(), torch.zeros(1, dtype=torch.int32, device=DEV)
+        paged_append(key, key, k1, v1, table, lengths + off, bad=bad)
+        assert int(bad) == 1
+        assert off == -62 or (torch.equal(k1, k) and torch.equal(v1, v))
+
+
+def test_append_of_views_and_odd_alignments():
+    from streamvoxel_amd.stream.paged import paged_append
+    g = torch.Generator().manual_seed(3)
+    rows = torch.randn(2, 30, 2, 3, 65, generator=g).to(torch.bfloat16).to(DEV)
+    for cut in (slice(0, 64), slice(1, 65)):
+        key, value = rows[:, :, 0, :, cut].transpose(1, 2), rows[:, :, 1, :, cut].transpose(1, 2)
+        pool = Pool([40, 30], 3, 64, 16, 1, token_major=True, clean=True)
+        k, v, table, lengths = pool.args()
+        paged_append(key, value, k, v, table, lengths)
+        for b, L in ((0, 40), (1, 30)):
+            at = torch.arange(L - 30, L, device=DEV)
+            page = table[b].long()[at // 16]
+            assert torch.equal(k[page, :, at % 16], key[b].transpose(0, 1))
+            assert torch.equal(v[page, :, at % 16], value[b].transpose(0, 1))
+
+
+def test_paged_refusals_on_the_gpu():
+    from streamvoxel_amd.stream.paged import paged_append, paged_attention
+    pool = Pool([40, 30], 2, 64, 16, 1, clean=True)
+    k, v, table, lengths = pool.args()
+    key, q = queries(2, 2, 3, 64, 0), queries(2, 4, 3, 64, 0)
+    f = torch.ones(32, dtype=torch.float64, device=DEV)
+    cu = torch.tensor([0, 3, 6], dtype=torch.int32, device=DEV)
+    e8 = dict(k_exponents=torch.zeros(k.shape[:3], dtype=torch.uint8, device=DEV),
+              v_exponents=torch.zeros(k.shape[:3], dtype=torch.uint8, device=DEV))
+    append = lambda **kw: paged_append(**{**dict(key=key, value=key, k_pages=k, v_pages=v, page_table=table,
+                                                 lengths=lengths), **kw})
+    attend = lambda **kw: paged_attention(**{**dict(query=q, k_pages=k, v_pages=v, page_table=table, lengths=lengths), **kw})
+    for kw in (dict(v_pages=v[:1]), dict(k_pages=k[0], v_pages=v[0]), dict(page_table=table.long()),
+               dict(page_table=table.t().contiguous().t()), dict(lengths=lengths.long()), dict(lengths=lengths[:1]),
+               dict(bad=torch.zeros(2, dtype=torch.int32, device=DEV)),
+               dict(k_pages=k.to(torch.float8_e4m3fn), v_pages=v.to(torch.float8_e4m3fn)),
+               dict(k_pages=k.transpose(2, 3), v_pages=v.transpose(2, 3))):
+        for call in (append, attend):
+            with pytest.raises(ValueError):
+                call(**kw)
+    for kw in (e8, dict(k_pages=k.float(), v_pages=v.float())):
+        for call in (append, attend):
+            with pytest.raises(TypeError):
+                call(**kw)
+    for kw in (dict(value=key[:, :, :2]), dict(key=key[:1], value=key[:1]), dict(key=key[0], value=key[0]), dict(before=-1),
+               dict(key=key[:, :1], value=key[:, :1]), dict(cu_tokens=cu), dict(key=key[0], value=key[0], cu_tokens=cu[:2]),
+               dict(positions=torch.zeros(2, 3, dtype=torch.int32, device=DEV)), dict(frequencies=f.float()),
+               dict(frequencies=f, layout='diagonal'), dict(frequencies=torch.cat((f, f))), dict(frequencies=f[:0]),
+               dict(frequencies=f, positions=torch.zeros(2, 4, dtype=torch.int32, device=DEV)),
+               dict(frequencies=f, positions=torch.zeros(2, 3, device=DEV)),
+               dict(frequencies=f[:10].float(), layout='axial')):
+        with pytest.raises(ValueError):
+            append(**kw)
+    for kw in (dict(query=q[:1]), dict(query=q[..., :48]), dict(query=q[:, :3]), dict(query=q[0]), dict(cu_queries=cu),
+               dict(query=q[0], cu_queries=cu.long()), dict(out=q[:, :2]), dict(out=q.float())):
+        with pytest.raises(ValueError):
+            attend(**kw)
+    with pytest.raises(TypeError):
+        attend(query=q.float())
+    with pytest.raises(TypeError):
+        append(key=key.float(), value=key.float())
+    with pytest.raises(RuntimeError, match='scale'):
+        attend(scale=0.0)
+
+
+@pytest.mark.parametrize('n', [1, 60])
+def test_calls_on_two_streams_and_in_a_graph(n):
+    """Two streams at once, and a captured append and attention replayed between eager calls of other sizes."""
+    from streamvoxel_amd.stream.paged import paged_append, paged_attention
+    g = torch.Generator().manual_seed(6)
+    pool = Pool([3000, 200, 1500], 2, 64, 64, 4, clean=True)
+    k, v, table, lengths = pool.args()
+    q, key = queries(3, 4, n, 64, 1), queries(3, 2, n, 64, 2)
+    f = torch.ones(32, dtype=torch.float64, device=DEV) / 100
+
+    def step():
+        paged_append(key, key, k, v, table, lengths, frequencies=f)
+        return paged_attention(q, k, v, table, lengths, causal=True)
+    want = step().clone()
+    torch.cuda.synchronize()
+    streams, results = [torch.cuda.Stream() for _ in range(2)], []
+    for _ in range(3):
+        for s in streams:
+            s.wait_stream(torch.cuda.current_stream())
+            with torch.cuda.stream(s):
+                results.append(paged_attention(q, k, v, table, lengths, causal=True))
+    torch.cuda.synchronize()
+    assert all(torch.equal(r, want) for r in results)
+    graphs = []
+    for _ in range(2):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = step()
+        graphs.append((graph, out))
+    for i in range(4):
+        key.copy_(queries(3, 2, n, 64, 20 + i))
+        lengths.copy_(torch.tensor([3000 - 100 * i, 200 - i, 1500 + i], dtype=torch.int32))
+        for graph, out in graphs:
+            graph.replay()
+            torch.cuda.synchronize()
+            got = out.clone()
+            paged_attention(queries(2, 2, 9, 64, i), k, v, table[:2], lengths[:2])
+            assert torch.equal(got, step())

@@ -1,0 +1,137 @@
+"""CPU checks of the rotary positions and the paged cache: the frequencies, the refusals of the C ABI (no launch) and of the
+Python entry points."""
+import ctypes
+import math
+
+import pytest
+import torch
+
+from streamvoxel_amd import _lib
+from streamvoxel_amd.stream.rotary import rotary, rotary_frequencies
+
+
+@pytest.fixture(scope='module')
+def lib():
+    import os
+    if not os.path.exists(_lib.LIB_PATH):
+        from streamvoxel_amd.build import build
+        build()
+    return _lib.load()
+
+
+def test_rotary_frequencies():
+    f, a = rotary_frequencies(8, base=100.0)
+    assert a == 1.0 and f.dtype == torch.float64
+    assert torch.allclose(f, torch.tensor([1.0, 100 ** -0.25, 0.1, 100 ** -0.75], dtype=torch.float64), rtol=1e-14, atol=0)
+    assert torch.equal(rotary_frequencies(8, base=100.0, scaling='linear', factor=4.0)[0], f / 4)
+    g, a = rotary_frequencies(64, scaling='wavelength', factor=8.0, original_length=2048)
+    f = rotary_frequencies(64)[0]
+    assert abs(a - (0.1 * math.log(8) + 1)) < 1e-15
+    turns = 2048 * f / (2 * math.pi)
+    assert torch.equal(g[turns > 32], f[turns > 32])
+    assert torch.allclose(g[turns < 1], f[turns < 1] / 8, rtol=1e-14, atol=0)
+    assert (g[1:] < g[:-1]).all() and (g <= f).all() and (g >= f / 8 * (1 - 1e-14)).all()
+    assert torch.equal(rotary_frequencies(64, scaling='wavelength', original_length=2048)[0], f)     # factor 1
+
+
+@pytest.mark.parametrize('args', [dict(rotary_dim=7), dict(rotary_dim=0), dict(rotary_dim=8, scaling='cubic'),
+                                  dict(rotary_dim=8, scaling='linear', factor=0.5),
+                                  dict(rotary_dim=8, scaling='wavelength', factor=2.0),
+                                  dict(rotary_dim=8, scaling='wavelength', original_length=100, low=4.0, high=4.0)])
+def test_rotary_frequencies_refusals(args):
+    with pytest.raises(ValueError):
+        rotary_frequencies(**args)
+
+
+def test_host_tensors_are_refused():
+    from streamvoxel_amd.stream.paged import paged_append, paged_attention
+    x = torch.zeros(1, 2, 3, 8, dtype=torch.bfloat16)
+    pages, table, n = torch.zeros(2, 2, 16, 8, dtype=torch.bfloat16), torch.zeros(1, 1, dtype=torch.int32), torch.ones(
+        1, dtype=torch.int32)
+    with pytest.raises(RuntimeError, match='GPU'):
+        rotary(x, torch.zeros(3, dtype=torch.int32), torch.ones(4, dtype=torch.float64))
+    with pytest.raises(RuntimeError, match='GPU'):
+        paged_append(x, x, pages, pages, table, n)
+    with pytest.raises(RuntimeError, match='GPU'):
+        paged_attention(x, pages, pages, table, n)
+
+
+FAKE = ctypes.c_void_p(0x1000)      # never dereferenced: every call below fails its host checks, or launches nothing
+
+
+def test_rotary_argument_errors(lib):
+    def call(x=FAKE, dtype=1, freq=FAKE, pairs=4, layout=1, sizes=(1, 2, 3, 8)):
+        return lib.svhip_rotary(x, FAKE, dtype, FAKE, 0, freq, pairs, layout, 1.0, 0, *sizes, *[8] * 6, 0, 1, None)
+    assert call(x=None) == -1 and b'null' in lib.svhip_last_error()
+    assert call(freq=None) == -1 and b'null' in lib.svhip_last_error()
+    assert call(dtype=3) == -1 and b'dtype' in lib.svhip_last_error()
+    for layout in (0, 3, 9):
+        assert call(layout=layout) == -1 and b'layout' in lib.svhip_last_error()
+    for pairs, D in ((5, 8), (0, 8), (129, 512)):
+        assert call(pairs=pairs, sizes=(1, 2, 3, D)) == -1 and b'pairs' in lib.svhip_last_error()
+    assert call(sizes=(1, 2, -3, 8)) == -1 and b'sizes' in lib.svhip_last_error()
+    for sizes in ((0, 2, 3, 8), (1, 0, 3, 8), (1, 2, 0, 8)):
+        assert call(sizes=sizes) == 0
+
+
+def append_call(lib, key=FAKE, sk=(768, 64, 128), B=2, H=2, N=3, D=64, cu=None, before=0, kp=FAKE, ke=None, dtype=1, pages=4,
+                page=64, srow=64, table=FAKE, m=2, lengths=FAKE, layout=0, positions=None, freq=None, pairs=0, amplitude=1.0):
+    return lib.svhip_paged_append(key, FAKE, *sk, 768, 64, 128, B, H, N, D, cu, before, kp, FAKE, ke, ke, dtype, pages, page,
+                                  8192, 4096, srow, 8192, 4096, srow, 128, 64, 128, 64, table, m, m, lengths, layout,
+                                  positions, 0, 6, 1, freq, pairs, amplitude, None, None)
+
+
+def test_append_argument_errors(lib):
+    error = lib.svhip_last_error
+    for D in (0, 60, 136):
+        assert append_call(lib, D=D) == -1 and b'head_dim' in error()
+    for page in (0, 8, 48, 2048):
+        assert append_call(lib, page=page) == -1 and b'page size' in error()
+    assert append_call(lib, dtype=0) == -1 and b'dtype' in error()
+    assert append_call(lib, before=-1) == -1 and b'sizes' in error()
+    assert append_call(lib, B=-1) == -1 and b'sizes' in error()
+    assert append_call(lib, pages=-1) == -1 and b'page counts' in error()
+    assert append_call(lib, layout=4) == -1 and b'layout' in error()
+    assert append_call(lib, layout=1, freq=FAKE, pairs=33) == -1 and b'pairs' in error()
+    assert append_call(lib, layout=2, freq=FAKE, pairs=0) == -1 and b'pairs' in error()
+    assert append_call(lib, layout=1, pairs=32) == -1 and b'frequencies' in error()
+    assert append_call(lib, layout=3, freq=FAKE, positions=FAKE, pairs=32) == -1 and b'three-axis' in error()
+    assert append_call(lib, layout=3, freq=FAKE, pairs=24, D=48) == -1 and b'positions' in error()
+    for name in ('key', 'kp', 'table', 'lengths'):
+        assert append_call(lib, **{name: None}) == -1 and b'null' in error()
+    assert append_call(lib, dtype=3) == -1 and b'exponents' in error()
+    assert append_call(lib, sk=(768, 60, 128)) == -1 and b'16-byte' in error()
+    assert append_call(lib, srow=68) == -1 and b'16-byte' in error()
+    assert append_call(lib, dtype=3, ke=FAKE, srow=68) == -1 and b'8-byte' in error()
+    for empty in (dict(B=0), dict(H=0), dict(N=0)):
+        assert append_call(lib, **empty) == 0
+
+
+def attend_call(lib, q=FAKE, kp=FAKE, ke=None, dtype=1, B=2, H=4, Hkv=2, N=3, D=64, cu=None, pages=4, page=64, table=FAKE,
+                m=2, lengths=FAKE, sq=64, srow=64, so=64, scale=0.125, ws=None, nbytes=0):
+    return lib.svhip_paged_attention(q, kp, FAKE, ke, ke, FAKE, dtype, B, H, Hkv, N, D, cu, pages, page, table, m, m, lengths,
+                                     768, 192, sq, 8192, 4096, srow, 8192, 4096, srow, 128, 64, 128, 64, 768, 192, so, 0,
+                                     scale, None, ws, nbytes, None)
+
+
+def test_attention_argument_errors(lib):
+    error = lib.svhip_last_error
+    for D in (0, 60, 136):
+        assert attend_call(lib, D=D) == -1 and b'head_dim' in error()
+    for page in (0, 8, 48, 2048):
+        assert attend_call(lib, page=page) == -1 and b'page size' in error()
+    for Hkv in (0, 3):
+        assert attend_call(lib, Hkv=Hkv) == -1 and b'share' in error()
+    for scale in (0.0, -1.0, math.inf, math.nan):
+        assert attend_call(lib, scale=scale) == -1 and b'scale' in error()
+    assert attend_call(lib, dtype=0) == -1 and b'dtype' in error()
+    assert attend_call(lib, N=-1) == -1 and b'sizes' in error()
+    assert attend_call(lib, m=1 << 26) == -1 and b'page counts' in error()
+    for name in ('q', 'kp', 'table', 'lengths'):
+        assert attend_call(lib, **{name: None}) == -1 and b'null' in error()
+    assert attend_call(lib, dtype=3) == -1 and b'exponents' in error()
+    assert attend_call(lib, sq=68) == -1 and b'query rows' in error()
+    assert attend_call(lib, so=66) == -1 and b'rows of out' in error()
+    assert attend_call(lib, srow=68) == -1 and b'16-byte' in error()
+    for empty in (dict(B=0), dict(H=0), dict(N=0)):
+        assert attend_call(lib, **empty) == 0
