@@ -1,13 +1,36 @@
-// svhip_paged_attention: attention of the windows' new tokens over their keys and values in a paged cache (paged.hpp).
+// svhip_paged_attention: attention of the windows' new tokens over their keys and values in a paged cache (paged.hpp), bf16
+// matrix cores, fp32 sums.
 //
-// Simple form: one wave per (token, head) with the running maximum and sum of the softmax, 64 keys at a time: a lane scores
-// one key, then holds head_dim elements of the output.
+// A key head's queries are its G heads' rows of every token, row r = token r / G, head r % G; a wave takes 32 of them as the
+// columns of S^T = K Q^T and O^T = V^T P^T (v_mfma_f32_32x32x16_bf16), so that the softmax of a row stays in two lanes and
+// P^T leaves the first product in the second one's operand layout (K rows lie in LDS under sigma_row; xattn_kernel.hpp). V
+// rows lie as they come and are read transposed (ds_read_b64_tr_b16). Two forms of work:
+//   * windows of more than kRows rows (tile): a workgroup takes 128 rows, 32 a wave; the 4 waves stage each block of 64 keys
+//     together, the next one in flight while the current one is computed. Bound: the matrix cores and the exponentials.
+//   * windows of up to kRows rows, single tokens among them (row): the 4 waves share the rows and split the keys, each
+//     staging its own blocks of 32 keys in its own LDS; no barrier until the waves' sums are joined. Bound: HBM.
+// Either form may cut a window's keys into parts for several workgroups; a part leaves O, its running maximum and its sum in
+// fp32 and paged_join_kernel joins them in order.
+//
+// Staging: 16 keys lie in one page (pages are of 16 keys or more), so the wave's load of 8 rows has one base, a scalar buffer
+// descriptor whose bound is the number of its keys that exist: keys past the window's end, bad pages and the chunks past
+// head_dim read as zeros and nothing is read outside a page.
 #include "paged.hpp"
+#include "xattn_kernel.hpp"
 
 namespace svhip {
 
 constexpr int kPagedMaxDim = 128;
 constexpr int kPagedThreads = 256;
+constexpr int kRows = 32;          // rows of a wave
+constexpr int kTileRows = 128;     // rows of a tile workgroup
+constexpr int kRowKeys = 32;       // keys of a row-form wave's block
+constexpr int kTileTarget = 512;   // workgroups that a launch of tiles is cut into at least where its keys allow
+constexpr int kRowTarget = 512;    // the same of the row form
+constexpr int kRowLeast = 256;     // least keys of a row-form part
+constexpr int kTileLeast = 6;      // least key blocks of a tile part
+constexpr float kNoMax = -3.0e38f; // running maximum before any key: finite, so that a row that sees nothing stays finite
+constexpr uint32_t kOutside = 0x7ffffff0u;  // byte offset past every descriptor's bound
 
 struct PagedArgs {
   const uint16_t* q;
@@ -16,93 +39,729 @@ struct PagedArgs {
   uint16_t* o;
   Tokens tokens;
   Pages pages;
-  int64_t H, G, D;  // G: heads of a key head
+  int64_t H, Hkv, G, D;  // G: heads of a key head
   int64_t sq_b, sq_h, sq_n, sk_p, sk_h, sk_r, sv_p, sv_h, sv_r, sek_p, sek_h, sev_p, sev_h, so_b, so_h, so_n;
   bool causal;
   float scale_log2;
+  // The plan.
+  int64_t q_tiles, tiles;  // tiles of a window (even windows), and of all (packed: at most)
+  int parts;               // of a tile's keys, at most
+  int64_t row_slots;       // row-form workgroups at most
+  int slot_rows;           // rows of a row-form slot
+  float *row_part, *tile_part;
+  int4* plan;              // a window's first slot or tile, its parts (0: nothing to join), form and part length
 };
 
-template <bool FP8>
-__device__ __forceinline__ float page_element(const void* p, int64_t i) {
+// The window as a workgroup sees it.
+struct Window {
+  int64_t first, count;  // its tokens
+  int64_t last;          // the last key that its first token sees (causal), or its last key
+  int keys;              // keys that any of its tokens sees
+};
+
+__device__ __forceinline__ Window window_at(const PagedArgs& a, int64_t b) {
+  Window w;
+  window_tokens(a.tokens, b, w.first, w.count);
+  const int64_t L = held_keys(a.pages, b);
+  w.keys = static_cast<int>(L);
+  w.last = a.causal ? a.pages.lengths[b] - w.count : L - 1;
+  return w;
+}
+
+// Last key that token i sees (below 0: none).
+__device__ __forceinline__ int last_key(const PagedArgs& a, const Window& w, int64_t i) {
+  const int64_t j = a.causal ? w.last + i : w.last;
+  return static_cast<int>(j < w.keys - 1 ? (j < -1 ? -1 : j) : w.keys - 1);
+}
+
+__device__ __forceinline__ bool row_form(const PagedArgs& a, int64_t count) { return count * a.G <= kRows; }
+
+__device__ __forceinline__ int64_t wave_sum(int64_t v) {
+#pragma unroll
+  for (int off = 32; off >= 1; off >>= 1) v += __shfl_xor(v, off, 64);
+  return v;
+}
+
+// Exclusive prefix over the wave's lanes; `total` the sum.
+__device__ __forceinline__ int wave_prefix(int v, int& total) {
+  int incl = v;
+#pragma unroll
+  for (int off = 1; off < 64; off <<= 1) {
+    const int up = __shfl_up(incl, off, 64);
+    if ((threadIdx.x & 63) >= off) incl += up;
+  }
+  total = __builtin_amdgcn_readlane(incl, 63);
+  return incl - v;
+}
+
+// Page of the 16 keys at j (a multiple of 16) of the window whose table row this is, through the scalar cache; the number
+// as it stands in the table (j may lie past the window's keys: its last entry then).
+__device__ __forceinline__ int page_number(const PagedArgs& a, const int32_t* row, int j) {
+  typedef const __attribute__((address_space(4))) int32_t* table_t;
+  const int64_t at = j >> a.pages.shift;
+  return __builtin_amdgcn_readfirstlane(((table_t)row)[at < a.pages.max_pages ? at : a.pages.max_pages - 1]);
+}
+
+#if defined(__HIP_DEVICE_COMPILE__)
+
+// Descriptor of 16 keys' rows at key j in `page`: the first `valid` of them, D elements of ES bytes each.
+template <int ES>
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t rows_of(const void* pool, int64_t page, int64_t in_page, int64_t sp,
+                                                         int64_t head, int64_t sr, int valid, int D) {
+  const char* base = static_cast<const char*>(pool) + (page * sp + head + in_page * sr) * ES;
+  const uint32_t bytes = valid > 0 ? static_cast<uint32_t>(((valid - 1) * sr + D) * ES) : 0u;
+  return __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(base), 0, bytes, kRsrcFlags);
+}
+
+// Keys of the 16 at j that exist: inside the window and on a page of the pool.
+__device__ __forceinline__ int valid_keys(const PagedArgs& a, int keys, int j, int& page) {
+  int valid = keys - j;
+  valid = valid < 0 ? 0 : (valid > 16 ? 16 : valid);
+  if (static_cast<uint32_t>(page) >= static_cast<uint32_t>(a.pages.pages)) {
+    if (valid > 0) set_bad(a.pages);
+    valid = 0;
+    page = 0;
+  }
+  return valid;
+}
+
+// A wave's 32 rows: the queries as B operands, O^T, running maximum (log2 units) and sum.
+template <int DT>
+struct Rows {
+  bf16x8_t qf[2 * DT];
+  f32x16_t o[DT];
+  f32x4_t l;   // four equal entries: the lane's share of its row's sum
+  float m;
+  int last;    // last key that the lane's row sees
+};
+
+template <int DT>
+__device__ __forceinline__ void load_rows(const PagedArgs& a, const Window& w, int64_t b, int64_t kvh, int64_t r,
+                                          Rows<DT>& s) {
+  const int hh = (threadIdx.x & 63) >> 5;
+  const int64_t i = r / a.G, g = r - i * a.G;
+  const bool ok = i < w.count;
+  const uint16_t* q = a.q + (a.tokens.cu ? 0 : b * a.sq_b) + (kvh * a.G + g) * a.sq_h +
+                      (a.tokens.cu ? w.first + i : i) * a.sq_n;
+#pragma unroll
+  for (int k = 0; k < 2 * DT; ++k) {
+    const int d0 = 16 * k + 8 * hh;
+    uint4 raw = make_uint4(0u, 0u, 0u, 0u);
+    if (ok && d0 < a.D) raw = *reinterpret_cast<const uint4*>(q + d0);
+    s.qf[k] = __builtin_bit_cast(bf16x8_t, raw);
+  }
+#pragma unroll
+  for (int j = 0; j < DT; ++j) s.o[j] = f32x16_t{0};
+  s.l = f32x4_t{0.f, 0.f, 0.f, 0.f};
+  s.m = kNoMax;
+  s.last = ok ? last_key(a, w, i) : -1;
+}
+
+// 32 keys, `key0` the first, staged at row 0 of kp (K rows under sigma_row) and vp (V rows): sub-tiles of 64 head_dim elements
+// kSubBytes apart. The running maximum moves only for a score more than kMaxHigh above it (P then stays below 2^20, which
+// fp32 sums and bf16 weights hold alike); the row's sum is taken over the bf16 weights that the second product reads, by
+// v_mfma_f32_4x4x4_16b_bf16 with ones in A, whose columns are single lanes: no row's NaN reaches another's sum.
+template <int DT, int kSubBytes>
+__device__ __forceinline__ void attend_half(Rows<DT>& s, const char* kp, const char* vp, const uint32_t (&rd)[4],
+                                            const uint32_t (&rvt)[DT], int ksteps, float sl2, bool masked, int key0) {
+  const int hh = (threadIdx.x & 63) >> 5;
+  f32x16_t x;
+#pragma unroll
+  for (int k = 0; k < 2 * DT; ++k) {
+    if (k == 0 || k < ksteps) {
+      const bf16x8_t ka = *reinterpret_cast<const bf16x8_t*>(kp + (k >> 2) * kSubBytes + rd[k & 3]);
+      x = __builtin_amdgcn_mfma_f32_32x32x16_bf16(ka, s.qf[k], k == 0 ? f32x16_t{0} : x, 0, 0, 0);
+    }
+  }
+  if (masked) {
+    const int seen = s.last - key0 - 8 * hh;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      if ((i < 8 ? i : i + 8) > seen) x[i] = -INFINITY;
+    }
+  }
+  float mx = __builtin_amdgcn_fmed3f(x[0], x[1], kFltMax);
+#pragma unroll
+  for (int i = 2; i < 16; i += 2) mx = max3(mx, x[i], x[i + 1]);
+  if (__builtin_amdgcn_ballot_w64(__builtin_fmaf(mx, sl2, -s.m) > kMaxHigh) != 0ull) {
+    const auto sw = __builtin_amdgcn_permlane32_swap(__float_as_int(mx), __float_as_int(mx), false, false);
+    const float cand = __builtin_amdgcn_fmed3f(__int_as_float(sw[0]), __int_as_float(sw[1]), kFltMax) * sl2;
+    const float mn = cand > s.m ? cand : s.m;
+    const float alpha = __builtin_amdgcn_exp2f(s.m - mn);
+    s.m = mn;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) s.l[i] *= alpha;
+#pragma unroll
+    for (int j = 0; j < DT; ++j) {
+#pragma unroll
+      for (int i = 0; i < 16; ++i) s.o[j][i] *= alpha;
+    }
+  }
+  bf16x8_t pb[2];
+#pragma unroll
+  for (int ks = 0; ks < 2; ++ks) {
+#pragma unroll
+    for (int j = 0; j < 8; j += 2) {
+      const f32x2_t two = {__builtin_amdgcn_exp2f(__builtin_fmaf(x[8 * ks + j], sl2, -s.m)),
+                           __builtin_amdgcn_exp2f(__builtin_fmaf(x[8 * ks + j + 1], sl2, -s.m))};
+      const bf16x2_t c = __builtin_convertvector(two, bf16x2_t);
+      pb[ks][j] = c[0];
+      pb[ks][j + 1] = c[1];
+    }
+  }
+  typedef short i16x4_t __attribute__((ext_vector_type(4)));
+  typedef short i16x8_t __attribute__((ext_vector_type(8)));
+  const i16x4_t ones = {0x3F80, 0x3F80, 0x3F80, 0x3F80};
+#pragma unroll
+  for (int ks = 0; ks < 2; ++ks) {
+    const i16x8_t p8 = __builtin_bit_cast(i16x8_t, pb[ks]);
+    s.l = __builtin_amdgcn_mfma_f32_4x4x4bf16_1k(ones, __builtin_shufflevector(p8, p8, 0, 1, 2, 3), s.l, 0, 0, 0);
+    s.l = __builtin_amdgcn_mfma_f32_4x4x4bf16_1k(ones, __builtin_shufflevector(p8, p8, 4, 5, 6, 7), s.l, 0, 0, 0);
+  }
+#pragma unroll
+  for (int ks = 0; ks < 2; ++ks) {
+    bf16x8_t va[DT];
+#pragma unroll
+    for (int j = 0; j < DT; ++j) {
+      typedef __bf16 bf16x4_t __attribute__((ext_vector_type(4)));
+      typedef __attribute__((address_space(3))) bf16x4_t lds_bf16x4_t;
+      char* at = const_cast<char*>(vp) + (j >> 1) * kSubBytes + rvt[j] + 16 * ks * kRow * 2;
+      const bf16x4_t lo = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((lds_bf16x4_t*)(at));
+      const bf16x4_t hi = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((lds_bf16x4_t*)(at + 4 * kRow * 2));
+      va[j] = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+    }
+#pragma unroll
+    for (int j = 0; j < DT; ++j) s.o[j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(va[j], pb[ks], s.o[j], 0, 0, 0);
+  }
+}
+
+// Byte offsets of the operand reads: K rows (rd) and V rows read transposed (rvt, of output tile j inside its sub-tile).
+template <int DT>
+__device__ __forceinline__ void read_offsets(uint32_t (&rd)[4], uint32_t (&rvt)[DT]) {
+  const int lane = threadIdx.x & 63, col = lane & 31, hh = lane >> 5;
+#pragma unroll
+  for (int k = 0; k < 4; ++k) rd[k] = static_cast<uint32_t>(col * kRow * 2 + swz(col, 2 * k + hh) * 16);
+  const int row = 8 * hh + ((lane & 15) >> 2), flip = (row >> 1) & 1;
+  const int c = 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1);
+#pragma unroll
+  for (int j = 0; j < DT; ++j) {
+    rvt[j] = static_cast<uint32_t>(row * kRow * 2 + 16 * (4 * ((j & 1) ^ flip) + c) + 8 * (lane & 1));
+  }
+}
+
+// The lane's sum of its row, both lanes' shares.
+__device__ __forceinline__ float row_sum(float l) {
+  const auto sw = __builtin_amdgcn_permlane32_swap(__float_as_int(l), __float_as_int(l), false, false);
+  return __int_as_float(sw[0]) + __int_as_float(sw[1]);
+}
+
+// A wave's staging of `kLoads` groups of 8 rows, load i of sub-tile u into rows 8 * group(i) of it.
+template <bool FP8, int DT, int kLoads>
+struct Staged {
+  uint2 k[FP8 ? kLoads * Width<DT>::kSubTiles : 1], v[FP8 ? kLoads * Width<DT>::kSubTiles : 1];
+  uint32_t ek[FP8 ? kLoads : 1], ev[FP8 ? kLoads : 1];
+};
+
+// Per-lane offsets: row lane / 8 of a load and its chunk; K under sigma_row and swz, V under swzv. A load's rows are 8 rows of
+// 16, `odd` the second 8.
+struct Lanes {
+  uint32_t k[2], v[2];   // byte offsets from the 16 keys' first row, loads of the first and the second 8 rows
+  int ck[2], cv[2];      // logical chunks
+  uint32_t rk[2];        // e4m3: the key's place among the 16
+};
+
+template <int ES>
+__device__ __forceinline__ Lanes staging_lanes(const PagedArgs& a) {
+  Lanes n;
+  const int lane = threadIdx.x & 63;
+#pragma unroll
+  for (int odd = 0; odd < 2; ++odd) {
+    const int R = 8 * odd + (lane >> 3), key = sigma_row(R);
+    n.ck[odd] = swz(R, lane & 7);
+    n.cv[odd] = swzv(R, lane & 7);
+    n.rk[odd] = static_cast<uint32_t>(key);
+    n.k[odd] = static_cast<uint32_t>((key * a.sk_r + 8 * n.ck[odd]) * ES);
+    n.v[odd] = static_cast<uint32_t>((R * a.sv_r + 8 * n.cv[odd]) * ES);
+  }
+  return n;
+}
+
+// Issues the loads of 8 rows (odd: the second 8 of the 16 keys at key j) of K and V: bf16 straight into LDS at row `row` of the
+// sub-tiles at sK and sV, e4m3 into registers at index i.
+template <bool FP8, int DT, int kSubBytes, int kLoads>
+__device__ __forceinline__ void stage_rows8(const PagedArgs& a, const Lanes& n, int page, int j, int keys, int64_t hk,
+                                            int64_t hv, int64_t hek, int64_t hev, int odd, int row, int i, char* sK,
+                                            char* sV, Staged<FP8, DT, kLoads>& st) {
+  constexpr int ES = FP8 ? 1 : 2;
+  const int valid = valid_keys(a, keys, j, page);
+  const int64_t in_page = j & ((1 << a.pages.shift) - 1);
+  const int D = static_cast<int>(a.D);
+  const auto kr = rows_of<ES>(a.k, page, in_page, a.sk_p, hk, a.sk_r, valid, D);
+  const auto vr = rows_of<ES>(a.v, page, in_page, a.sv_p, hv, a.sv_r, valid, D);
+#pragma unroll
+  for (int u = 0; u < Width<DT>::kSubTiles; ++u) {
+    const uint32_t ko = 64 * u + 8 * n.ck[odd] < D ? n.k[odd] + 64 * ES * u : kOutside;
+    const uint32_t vo = 64 * u + 8 * n.cv[odd] < D ? n.v[odd] + 64 * ES * u : kOutside;
+    if constexpr (FP8) {
+      st.k[i * Width<DT>::kSubTiles + u] = __builtin_bit_cast(uint2, __builtin_amdgcn_raw_buffer_load_b64(kr, ko, 0, 0));
+      st.v[i * Width<DT>::kSubTiles + u] = __builtin_bit_cast(uint2, __builtin_amdgcn_raw_buffer_load_b64(vr, vo, 0, 0));
+    } else {
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(kr, (lds_ptr_t)(sK + u * kSubBytes + row * kRow * 2), 16, ko, 0, 0, 0);
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(vr, (lds_ptr_t)(sV + u * kSubBytes + row * kRow * 2), 16, vo, 0, 0, 0);
+    }
+  }
   if constexpr (FP8) {
-    return __builtin_amdgcn_cvt_f32_fp8(static_cast<const uint8_t*>(p)[i], 0);
+    const auto er = rows_of<1>(a.ek, page, in_page, a.sek_p, hek, 1, valid, 1);
+    const auto fr = rows_of<1>(a.ev, page, in_page, a.sev_p, hev, 1, valid, 1);
+    st.ek[i] = __builtin_amdgcn_raw_buffer_load_b8(er, n.rk[odd], 0, 0);
+    st.ev[i] = __builtin_amdgcn_raw_buffer_load_b8(fr, 8 * odd + ((threadIdx.x & 63) >> 3), 0, 0);
+  }
+}
+
+// 8 e4m3 codes times 2^(exponent - 127) as bf16, exact.
+__device__ __forceinline__ uint4 decode8(uint2 w, uint32_t exponent) {
+  const float f = exponent_value(static_cast<int>(exponent));
+  const bf16x2_t a = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w.x, f, false);
+  const bf16x2_t b = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w.x, f, true);
+  const bf16x2_t c = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w.y, f, false);
+  const bf16x2_t d = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w.y, f, true);
+  return make_uint4(__builtin_bit_cast(uint32_t, a), __builtin_bit_cast(uint32_t, b), __builtin_bit_cast(uint32_t, c),
+                    __builtin_bit_cast(uint32_t, d));
+}
+
+// e4m3: load i of `st` into its 8 rows at `row`.
+template <int DT, int kSubBytes, int kLoads>
+__device__ __forceinline__ void commit_rows8(const Staged<true, DT, kLoads>& st, int row, int i, char* sK, char* sV) {
+  const uint32_t at = row * kRow * 2 + 16 * (threadIdx.x & 63);
+#pragma unroll
+  for (int u = 0; u < Width<DT>::kSubTiles; ++u) {
+    *reinterpret_cast<uint4*>(sK + u * kSubBytes + at) = decode8(st.k[i * Width<DT>::kSubTiles + u], st.ek[i]);
+    *reinterpret_cast<uint4*>(sV + u * kSubBytes + at) = decode8(st.v[i * Width<DT>::kSubTiles + u], st.ev[i]);
+  }
+}
+
+#endif  // __HIP_DEVICE_COMPILE__
+
+// ------------------------------------------------------------------------------------------------------- tile form
+
+template <bool FP8, int DT>
+__global__ __launch_bounds__(kPagedThreads, 2) void paged_tile_kernel(PagedArgs a) {
+#if defined(__HIP_DEVICE_COMPILE__)
+  constexpr int kSubBytes = kKB * kRow * 2, kTileBytes = Width<DT>::kSubTiles * kSubBytes;
+  __shared__ __attribute__((aligned(16))) char sK0[kTileBytes], sK1[kTileBytes], sV0[kTileBytes], sV1[kTileBytes];
+  // Workgroup -> (tile, key head, part): XCD id % 8 takes every 8th unit (window, key head, part) with all its tiles, so that
+  // its L2 reads the unit's keys once.
+  const int64_t seq = blockIdx.x >> 3;
+  const int64_t q_tiles = a.tokens.cu ? 1 : a.q_tiles;
+  int64_t qt = seq % q_tiles, unit = (seq / q_tiles) * kXcds + (blockIdx.x & 7);
+  const int part = static_cast<int>(unit % a.parts);
+  unit /= a.parts;
+  const int64_t kvh = unit % a.Hkv;
+  int64_t b = unit / a.Hkv, tile;
+  if (a.tokens.cu) {
+    // The window of tile number b, of the windows with more than kRows rows.
+    tile = b;
+    int64_t left = b;
+    b = -1;
+    for (int64_t b0 = 0; b0 < a.tokens.B; b0 += 64) {
+      const int64_t c = b0 + (threadIdx.x & 63);
+      int n = 0, total;
+      if (c < a.tokens.B) {
+        int64_t first, count;
+        window_tokens(a.tokens, c, first, count);
+        if (!row_form(a, count)) n = static_cast<int>(cdiv(count * a.G, kTileRows));
+      }
+      const int before = wave_prefix(n, total);
+      if (left < total) {
+        const int at = __builtin_ctzll(__builtin_amdgcn_ballot_w64(before <= left && left < before + n));
+        b = b0 + at;
+        qt = left - __builtin_amdgcn_readlane(before, at);
+        break;
+      }
+      left -= total;
+    }
+    if (b < 0 || tile >= a.tiles) return;
   } else {
-    return bf16_bits_to_float(static_cast<const uint16_t*>(p)[i]);
+    if (b >= a.tokens.B) return;
+    tile = b * a.q_tiles + qt;
+  }
+  b = __builtin_amdgcn_readfirstlane(static_cast<int>(b));
+  qt = __builtin_amdgcn_readfirstlane(static_cast<int>(qt));
+  const Window w = window_at(a, b);
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int lane = threadIdx.x & 63, col = lane & 31, hh = lane >> 5;
+  const int64_t r0 = qt * kTileRows, r = r0 + wave * kRows + col;
+  // Keys that the tile's last row sees, and this part's blocks of them.
+  const int64_t rows = w.count * a.G;
+  const int64_t r1 = r0 + kTileRows < rows ? r0 + kTileRows : rows;
+  const int keys = __builtin_amdgcn_readfirstlane(last_key(a, w, (r1 - 1) / a.G) + 1);
+  const int blocks = (keys + kKB - 1) / kKB;
+  int each = (blocks + a.parts - 1) / a.parts;
+  if (each < kTileLeast) each = kTileLeast;
+  const int count = blocks > each ? (blocks + each - 1) / each : 1;
+  if (part >= count) return;
+  if (a.plan && part == 0 && kvh == 0 && qt == 0 && threadIdx.x == 0) a.plan[b] = make_int4(static_cast<int>(tile), 0, 1, 0);
+  const int blk0 = part * each, blk1 = blk0 + each < blocks ? blk0 + each : blocks;
+
+  Rows<DT> s;
+  load_rows<DT>(a, w, b, kvh, r, s);
+  uint32_t rd[4], rvt[DT];
+  read_offsets<DT>(rd, rvt);
+  const Lanes lanes = staging_lanes<FP8 ? 1 : 2>(a);
+  const int ksteps = __builtin_amdgcn_readfirstlane(static_cast<int>((a.D + 15) / 16));
+  const int64_t hk = kvh * a.sk_h, hv = kvh * a.sv_h, hek = kvh * a.sek_h, hev = kvh * a.sev_h;
+  const int32_t* row = a.pages.table + b * a.pages.st_b;
+  // The wave's rows see every key up to `all` and none past `any`.
+  const int64_t wr0 = r0 + wave * kRows, wr1 = wr0 + kRows < rows ? wr0 + kRows : rows;
+  const int all = __builtin_amdgcn_readfirstlane(wr0 < rows ? last_key(a, w, wr0 / a.G) : -1);
+  const int any = __builtin_amdgcn_readfirstlane(wr0 < rows ? last_key(a, w, (wr1 - 1) / a.G) : -1);
+
+  // The wave stages rows 8 wave .. and 8 (wave + 4) .. of a block: 16 keys at 16 (wave / 2) and at 32 + 16 (wave / 2).
+  Staged<FP8, DT, 2> st;
+  const int g0 = 16 * (wave >> 1), odd = wave & 1;
+  auto issue = [&](int kv0, int p0, int p1, char* sK, char* sV) __attribute__((always_inline)) {
+    stage_rows8<FP8, DT, kSubBytes>(a, lanes, p0, kv0 + g0, keys, hk, hv, hek, hev, odd, 8 * wave, 0, sK, sV, st);
+    stage_rows8<FP8, DT, kSubBytes>(a, lanes, p1, kv0 + 32 + g0, keys, hk, hv, hek, hev, odd, 8 * wave + 32, 1, sK, sV, st);
+  };
+  auto commit = [&](char* sK, char* sV) __attribute__((always_inline)) {
+    if constexpr (FP8) {
+      commit_rows8<DT, kSubBytes>(st, 8 * wave, 0, sK, sV);
+      commit_rows8<DT, kSubBytes>(st, 8 * wave + 32, 1, sK, sV);
+    }
+  };
+  auto compute = [&](int kv0, const char* sK, const char* sV) __attribute__((always_inline)) {
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      const int key0 = kv0 + 32 * t;
+      if (key0 > any) break;
+      attend_half<DT, kSubBytes>(s, sK + 32 * t * kRow * 2, sV + 32 * t * kRow * 2, rd, rvt, ksteps, a.scale_log2,
+                                 key0 + 31 > all, key0);
+    }
+  };
+  if (blk0 < blk1) {
+    int p0 = page_number(a, row, kKB * blk0 + g0), p1 = page_number(a, row, kKB * blk0 + 32 + g0);
+    issue(kKB * blk0, p0, p1, sK0, sV0);
+    p0 = page_number(a, row, kKB * (blk0 + 1) + g0);
+    p1 = page_number(a, row, kKB * (blk0 + 1) + 32 + g0);
+    commit(sK0, sV0);
+    wait_vmem();
+    __syncthreads();
+    auto step = [&](int blk, char* cK, char* cV, char* nK, char* nV) __attribute__((always_inline)) {
+      const bool more = blk + 1 < blk1;
+      if (more) issue(kKB * (blk + 1), p0, p1, nK, nV);
+      p0 = page_number(a, row, kKB * (blk + 2) + g0);
+      p1 = page_number(a, row, kKB * (blk + 2) + 32 + g0);
+      compute(kKB * blk, cK, cV);
+      if (more) {
+        commit(nK, nV);
+        wait_vmem();
+        __syncthreads();
+      }
+    };
+    for (int blk = blk0; blk < blk1; blk += 2) {
+      step(blk, sK0, sV0, sK1, sV1);
+      if (blk + 1 < blk1) step(blk + 1, sK1, sV1, sK0, sV0);
+    }
+  }
+  const float l = row_sum(s.l[0]);
+  if (r >= rows) return;
+  if (count > 1) {
+    float* slot = a.tile_part + ((tile * a.Hkv + kvh) * a.parts + part) * (kTileRows * (a.D + 2)) +
+                  (wave * kRows + col) * (a.D + 2);
+#pragma unroll
+    for (int j = 0; j < DT; ++j) {
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        const int d0 = 32 * j + 8 * g + 4 * hh;
+        if (d0 < a.D) {
+          *reinterpret_cast<float2*>(slot + d0) = make_float2(s.o[j][4 * g], s.o[j][4 * g + 1]);
+          *reinterpret_cast<float2*>(slot + d0 + 2) = make_float2(s.o[j][4 * g + 2], s.o[j][4 * g + 3]);
+        }
+      }
+    }
+    if (hh == 0) *reinterpret_cast<float2*>(slot + a.D) = make_float2(s.m, l);
+    return;
+  }
+  const int64_t i = r / a.G, g0q = r - i * a.G;
+  uint16_t* out = a.o + (a.tokens.cu ? 0 : b * a.so_b) + (kvh * a.G + g0q) * a.so_h + (a.tokens.cu ? w.first + i : i) * a.so_n;
+  const float inv = s.last >= 0 ? 1.f / l : 0.f;
+#pragma unroll
+  for (int j = 0; j < DT; ++j) {
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      const int d0 = 32 * j + 8 * g + 4 * hh;
+      if (d0 < a.D) {
+        *reinterpret_cast<uint2*>(out + d0) = make_uint2(bf16_pack2(s.o[j][4 * g] * inv, s.o[j][4 * g + 1] * inv),
+                                                         bf16_pack2(s.o[j][4 * g + 2] * inv, s.o[j][4 * g + 3] * inv));
+      }
+    }
+  }
+#endif
+}
+
+// -------------------------------------------------------------------------------------------------------- row form
+
+// The windows' parts, a workgroup's worth each: an equal share of all keys for kRowTarget workgroups, at least kRowLeast, a
+// multiple of 4 waves' blocks. The lengths are on the device, so every workgroup forms the plan for itself.
+__device__ __forceinline__ int row_part_keys(const PagedArgs& a) {
+  int64_t sum = 0;
+  for (int64_t c = threadIdx.x & 63; c < a.tokens.B; c += 64) {
+    int64_t first, count;
+    window_tokens(a.tokens, c, first, count);
+    if (count > 0 && row_form(a, count)) sum += held_keys(a.pages, c);
+  }
+  const int64_t share = cdiv(wave_sum(sum) * a.Hkv, kRowTarget);
+  const int64_t each = cdiv(share, 4 * kRowKeys) * (4 * kRowKeys);
+  return static_cast<int>(each < kRowLeast ? kRowLeast : each);
+}
+
+template <bool FP8, int DT>
+__global__ __launch_bounds__(kPagedThreads, 2) void paged_row_kernel(PagedArgs a) {
+#if defined(__HIP_DEVICE_COMPILE__)
+  constexpr int kSubBytes = kRowKeys * kRow * 2, kTileBytes = Width<DT>::kSubTiles * kSubBytes;
+  __shared__ __attribute__((aligned(16))) char sK0[4 * kTileBytes], sK1[4 * kTileBytes], sV0[4 * kTileBytes],
+      sV1[4 * kTileBytes];
+  __shared__ float s_ml[4][2][kRows];
+  const int lane = threadIdx.x & 63, col = lane & 31, hh = lane >> 5;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  // Workgroup -> (window, part, key head).
+  const int each = __builtin_amdgcn_readfirstlane(row_part_keys(a));
+  const int id = static_cast<int>(blockIdx.x);
+  int64_t b = -1;
+  int part = 0, kvh = 0, parts = 0, before_b = 0;
+  int left = id;
+  for (int64_t b0 = 0; b0 < a.tokens.B; b0 += 64) {
+    const int64_t c = b0 + lane;
+    int n = 0, total;
+    if (c < a.tokens.B) {
+      int64_t first, count;
+      window_tokens(a.tokens, c, first, count);
+      if (count > 0 && row_form(a, count)) {
+        const int64_t L = held_keys(a.pages, c);
+        n = static_cast<int>(L > each ? cdiv(L, each) : 1) * static_cast<int>(a.Hkv);
+      }
+    }
+    const int before = wave_prefix(n, total);
+    if (left < total) {
+      const int at = __builtin_ctzll(__builtin_amdgcn_ballot_w64(before <= left && left < before + n));
+      b = b0 + at;
+      const int in = left - __builtin_amdgcn_readlane(before, at);
+      parts = __builtin_amdgcn_readlane(n, at) / static_cast<int>(a.Hkv);
+      kvh = in / parts;
+      part = in - kvh * parts;
+      before_b = id - in;
+      break;
+    }
+    left -= total;
+  }
+  if (b < 0) return;
+  b = __builtin_amdgcn_readfirstlane(static_cast<int>(b));
+  kvh = __builtin_amdgcn_readfirstlane(kvh);
+  part = __builtin_amdgcn_readfirstlane(part);
+  if (part == 0 && kvh == 0 && threadIdx.x == 0) a.plan[b] = make_int4(before_b, parts, 0, 0);
+  const Window w = window_at(a, b);
+  const int rows = static_cast<int>(w.count * a.G);
+  const int keys = __builtin_amdgcn_readfirstlane(w.keys);
+  const int k0 = part * each, k1 = k0 + each < keys ? k0 + each : keys;
+
+  Rows<DT> s;
+  load_rows<DT>(a, w, b, kvh, col, s);
+  uint32_t rd[4], rvt[DT];
+  read_offsets<DT>(rd, rvt);
+  const Lanes lanes = staging_lanes<FP8 ? 1 : 2>(a);
+  const int ksteps = __builtin_amdgcn_readfirstlane(static_cast<int>((a.D + 15) / 16));
+  const int64_t hk = kvh * a.sk_h, hv = kvh * a.sv_h, hek = kvh * a.sek_h, hev = kvh * a.sev_h;
+  const int32_t* row = a.pages.table + b * a.pages.st_b;
+  const int all = __builtin_amdgcn_readfirstlane(last_key(a, w, 0));
+  char *cK0 = sK0 + wave * kTileBytes, *cV0 = sV0 + wave * kTileBytes;
+  char *cK1 = sK1 + wave * kTileBytes, *cV1 = sV1 + wave * kTileBytes;
+  Staged<FP8, DT, 4> st;
+  auto issue = [&](int kv0, int p0, int p1, char* sK, char* sV) __attribute__((always_inline)) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      stage_rows8<FP8, DT, kSubBytes>(a, lanes, i < 2 ? p0 : p1, kv0 + 16 * (i >> 1), k1, hk, hv, hek, hev, i & 1, 8 * i, i,
+                                      sK, sV, st);
+    }
+  };
+  auto commit = [&](char* sK, char* sV) __attribute__((always_inline)) {
+    if constexpr (FP8) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) commit_rows8<DT, kSubBytes>(st, 8 * i, i, sK, sV);
+    }
+  };
+  const int stride = 4 * kRowKeys;
+  int kv = k0 + wave * kRowKeys;
+  if (kv < k1) {
+    int p0 = page_number(a, row, kv), p1 = page_number(a, row, kv + 16);
+    issue(kv, p0, p1, cK0, cV0);
+    p0 = page_number(a, row, kv + stride);
+    p1 = page_number(a, row, kv + stride + 16);
+    commit(cK0, cV0);
+    wait_vmem();
+    auto step = [&](char* xK, char* xV, char* nK, char* nV) __attribute__((always_inline)) {
+      const bool more = kv + stride < k1;
+      if (more) issue(kv + stride, p0, p1, nK, nV);
+      p0 = page_number(a, row, kv + 2 * stride);
+      p1 = page_number(a, row, kv + 2 * stride + 16);
+      attend_half<DT, kSubBytes>(s, xK, xV, rd, rvt, ksteps, a.scale_log2, kv + 31 > all, kv);
+      if (more) {
+        commit(nK, nV);
+        wait_vmem();
+      }
+      kv += stride;
+    };
+    while (kv < k1) {
+      step(cK0, cV0, cK1, cV1);
+      if (kv < k1) step(cK1, cV1, cK0, cV0);
+    }
+  }
+  // The waves' sums joined, in order: O of wave w at its tile, [head_dim][row].
+  const float l = row_sum(s.l[0]);
+  __syncthreads();
+  float* so = reinterpret_cast<float*>(wave < 2 ? sK0 : sK1) + (wave & 1) * 2 * kTileBytes / 4;
+  static_assert(2 * kTileBytes >= 32 * DT * kRows * 4, "O of a wave fits its two buffers' part");
+  if (hh == 0) {
+    s_ml[wave][0][col] = s.m;
+    s_ml[wave][1][col] = l;
+  }
+#pragma unroll
+  for (int j = 0; j < DT; ++j) {
+#pragma unroll
+    for (int e = 0; e < 16; ++e) so[(32 * j + 8 * (e >> 2) + 4 * hh + (e & 3)) * kRows + col] = s.o[j][e];
+  }
+  __syncthreads();
+  const int D = static_cast<int>(a.D);
+  for (int e = threadIdx.x; e < rows * (D / 2); e += kPagedThreads) {
+    const int rr = e / (D / 2), d = 2 * (e - rr * (D / 2));
+    float m = s_ml[0][0][rr];
+#pragma unroll
+    for (int x = 1; x < 4; ++x) m = fmaxf(m, s_ml[x][0][rr]);
+    float sum = 0.f, o0 = 0.f, o1 = 0.f;
+#pragma unroll
+    for (int x = 0; x < 4; ++x) {
+      const float f = __builtin_amdgcn_exp2f(s_ml[x][0][rr] - m);
+      const float* from = reinterpret_cast<const float*>(x < 2 ? sK0 : sK1) + (x & 1) * 2 * kTileBytes / 4;
+      sum = __builtin_fmaf(s_ml[x][1][rr], f, sum);
+      o0 = __builtin_fmaf(from[d * kRows + rr], f, o0);
+      o1 = __builtin_fmaf(from[(d + 1) * kRows + rr], f, o1);
+    }
+    if (parts > 1) {
+      float* slot = a.row_part + (static_cast<int64_t>(id) * a.slot_rows + rr) * (D + 2);
+      *reinterpret_cast<float2*>(slot + d) = make_float2(o0, o1);
+      if (d == 0) *reinterpret_cast<float2*>(slot + D) = make_float2(m, sum);
+    } else {
+      const int64_t i = rr / a.G, g = rr - i * a.G;
+      uint16_t* out = a.o + (a.tokens.cu ? 0 : b * a.so_b) + (kvh * a.G + g) * a.so_h + (a.tokens.cu ? w.first + i : i) * a.so_n;
+      const float inv = last_key(a, w, i) >= 0 ? 1.f / sum : 0.f;
+      *reinterpret_cast<uint32_t*>(out + d) = bf16_pack2(o0 * inv, o1 * inv);
+    }
+  }
+#endif
+}
+
+// The parts of a row joined in order. 32 lanes a row, 4 elements a lane.
+__global__ __launch_bounds__(kPagedThreads) void paged_join_kernel(PagedArgs a) {
+  const int64_t id = static_cast<int64_t>(blockIdx.x) * (kPagedThreads / 32) + threadIdx.x / 32;
+  const int d0 = 4 * (threadIdx.x % 32);
+  const int64_t total = (a.tokens.cu ? a.tokens.N : a.tokens.B * a.tokens.N);
+  const int64_t token = id / a.H, h = id - token * a.H;
+  if (token >= total || d0 >= a.D) return;
+  const int64_t b = a.tokens.cu ? window_of(a.tokens, token) : token / a.tokens.N;
+  if (b < 0) return;
+  const Window w = window_at(a, b);
+  if (w.count <= 0) return;
+  const int64_t i = token - w.first, kvh = h / a.G, r = i * a.G + (h - kvh * a.G);
+  const int4 plan = a.plan[b];
+  const float* slot;
+  int64_t step;
+  int count;
+  if (row_form(a, w.count)) {
+    count = plan.y;
+    if (plan.x < 0 || count < 0 || plan.x + a.Hkv * count > a.row_slots) return set_bad(a.pages);  // borders not ascending
+    slot = a.row_part + ((plan.x + kvh * count) * a.slot_rows + r) * (a.D + 2);
+    step = a.slot_rows * (a.D + 2);
+  } else {
+    const int64_t r0 = r / kTileRows * kTileRows, rows = w.count * a.G;
+    const int64_t r1 = r0 + kTileRows < rows ? r0 + kTileRows : rows;
+    const int blocks = (last_key(a, w, (r1 - 1) / a.G) + kKB) / kKB;
+    int each = (blocks + a.parts - 1) / a.parts;
+    if (each < kTileLeast) each = kTileLeast;
+    count = blocks > each ? (blocks + each - 1) / each : 1;
+    if (plan.x < 0 || plan.x + r / kTileRows >= a.tiles) return set_bad(a.pages);
+    slot = a.tile_part + ((plan.x + r / kTileRows) * a.Hkv + kvh) * a.parts * (kTileRows * (a.D + 2)) + (r - r0) * (a.D + 2);
+    step = kTileRows * (a.D + 2);
+  }
+  if (count < 2) return;
+  float m = kNoMax, l = 0.f, o[4] = {0.f, 0.f, 0.f, 0.f};
+  for (int p = 0; p < count; ++p, slot += step) {
+    const float mi = slot[a.D], li = slot[a.D + 1];
+    const float mn = fmaxf(m, mi), x = __builtin_amdgcn_exp2f(m - mn), y = __builtin_amdgcn_exp2f(mi - mn);
+    m = mn;
+    l = join_value(l, li, x, y);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) o[e] = join_value(o[e], slot[d0 + e], x, y);
+  }
+  const float inv = last_key(a, w, i) >= 0 ? 1.f / l : 0.f;
+  uint16_t* out = a.o + (a.tokens.cu ? 0 : b * a.so_b) + h * a.so_h + (a.tokens.cu ? token : i) * a.so_n;
+  *reinterpret_cast<uint2*>(out + d0) = make_uint2(bf16_pack2(o[0] * inv, o[1] * inv), bf16_pack2(o[2] * inv, o[3] * inv));
+}
+
+// What a call launches, by its sizes alone.
+struct PagedPlan {
+  bool rows, tiles;        // the forms that its windows may take
+  int64_t q_tiles, tile_count;
+  int parts;
+  int64_t row_slots;
+  int slot_rows;
+  int64_t row_floats, tile_floats, plan_windows;
+  size_t bytes() const { return static_cast<size_t>(row_floats + tile_floats) * 4 + static_cast<size_t>(plan_windows) * 16; }
+};
+
+inline PagedPlan paged_plan(int64_t B, int64_t H, int64_t Hkv, int64_t N, bool packed, int64_t D, int64_t max_keys) {
+  PagedPlan p{};
+  const int64_t G = H / Hkv;
+  p.rows = packed || N * G <= kRows;
+  p.tiles = N * G > kRows;
+  p.parts = 1;
+  if (p.tiles) {
+    p.q_tiles = packed ? 1 : cdiv(N * G, kTileRows);
+    p.tile_count = packed ? N * G / kTileRows + (N * G / (kRows + 1) < B ? N * G / (kRows + 1) : B) : B * p.q_tiles;
+    const int64_t most = cdiv(cdiv(max_keys, kKB), kTileLeast), want = kTileTarget / (p.tile_count * Hkv);
+    p.parts = static_cast<int>(want < 1 ? 1 : (want < most ? want : (most < 1 ? 1 : most)));
+    if (p.parts > 1) p.tile_floats = p.tile_count * Hkv * p.parts * kTileRows * (D + 2);
+  }
+  if (p.rows) {
+    p.row_slots = kRowTarget + B * Hkv;
+    p.slot_rows = static_cast<int>(packed ? (N * G < kRows ? N * G : kRows) : N * G);
+    p.row_floats = p.row_slots * p.slot_rows * (D + 2);
+    p.row_floats += p.row_floats & 1;
+  }
+  p.tile_floats = (p.tile_floats + 3) / 4 * 4;
+  p.row_floats = (p.row_floats + 3) / 4 * 4;
+  p.plan_windows = p.rows || p.parts > 1 ? B : 0;
+  return p;
+}
+
+template <bool FP8, int DT>
+void launch_paged(const PagedArgs& a, const PagedPlan& p, hipStream_t s) {
+  if (p.rows) {
+    paged_row_kernel<FP8, DT><<<static_cast<unsigned>(p.row_slots), kPagedThreads, 0, s>>>(a);
+  }
+  if (p.tiles) {
+    const int64_t units = p.tile_count / p.q_tiles * a.Hkv * p.parts;
+    paged_tile_kernel<FP8, DT><<<static_cast<unsigned>(cdiv(units, kXcds) * kXcds * p.q_tiles), kPagedThreads, 0, s>>>(a);
   }
 }
 
 template <bool FP8>
-__global__ __launch_bounds__(kPagedThreads) void paged_simple_kernel(PagedArgs a) {
-  __shared__ float s_q[4][kPagedMaxDim];
-  __shared__ float s_p[4][64];
-  __shared__ int64_t s_row[4][64];
-  const int w = threadIdx.x >> 6, lane = threadIdx.x & 63, D = static_cast<int>(a.D);
-  const int64_t total = (a.tokens.cu ? a.tokens.N : a.tokens.B * a.tokens.N) * a.H;
-  const int64_t id = static_cast<int64_t>(blockIdx.x) * 4 + w;
-  int64_t b = -1, h = 0, n = 0, bb = 0, keys = 0;
-  if (id < total) {
-    const int64_t i = id / a.H;
-    h = id - i * a.H;
-    b = a.tokens.cu ? window_of(a.tokens, i) : i / a.tokens.N;
-    if (b >= 0) {
-      int64_t first, count;
-      window_tokens(a.tokens, b, first, count);
-      n = a.tokens.cu ? i : i - first;
-      bb = a.tokens.cu ? 0 : b;
-      keys = held_keys(a.pages, b);
-      if (a.causal) keys = a.pages.lengths[b] - count + (i - first) + 1 < keys ? a.pages.lengths[b] - count + (i - first) + 1 : keys;
-    }
+void launch_width(const PagedArgs& a, const PagedPlan& p, hipStream_t s) {
+  if (a.D <= 64) {
+    launch_paged<FP8, 2>(a, p, s);
+  } else if (a.D <= 96) {
+    launch_paged<FP8, 3>(a, p, s);
+  } else {
+    launch_paged<FP8, 4>(a, p, s);
   }
-  if (b >= 0) {
-    for (int d = lane; d < D; d += 64) s_q[w][d] = bf16_bits_to_float(a.q[bb * a.sq_b + h * a.sq_h + n * a.sq_n + d]);
-  }
-  __syncthreads();
-  if (b < 0) return;
-  const int64_t kvh = h / a.G;
-  float m = -INFINITY, l = 0.f, o[2] = {0.f, 0.f};
-  for (int64_t j0 = 0; j0 < keys; j0 += 64) {
-    const int64_t j = j0 + lane;
-    float s = -INFINITY;
-    int64_t row = -1;
-    if (j < keys) {
-      s = 0.f;
-      const int64_t page = page_of(a.pages, b, j);
-      const int64_t r = j & ((1ll << a.pages.shift) - 1);
-      if (page >= 0) {
-        const int64_t at = page * a.sk_p + kvh * a.sk_h + r * a.sk_r;
-        for (int d = 0; d < D; ++d) s += s_q[w][d] * page_element<FP8>(a.k, at + d);
-        if constexpr (FP8) s *= exponent_value(a.ek[page * a.sek_p + kvh * a.sek_h + r]);
-        s *= a.scale_log2;
-        row = (page << 16) | r;
-      }
-    }
-    float mx = s;
-    for (int off = 32; off >= 1; off >>= 1) mx = fmaxf(mx, __shfl_xor(mx, off));
-    const float mn = fmaxf(m, mx);
-    const float alpha = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - mn);
-    float p = s == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(s - mn);
-    m = mn;
-    s_p[w][lane] = p;
-    s_row[w][lane] = row;
-    for (int off = 32; off >= 1; off >>= 1) p += __shfl_xor(p, off);
-    l = l * alpha + p;
-    o[0] *= alpha;
-    o[1] *= alpha;
-    const int count = static_cast<int>(keys - j0 < 64 ? keys - j0 : 64);
-    for (int t = 0; t < count; ++t) {
-      const int64_t at = s_row[w][t];
-      if (at < 0) continue;
-      const int64_t page = at >> 16, r = at & 0xffff;
-      const float x = FP8 ? s_p[w][t] * exponent_value(a.ev[page * a.sev_p + kvh * a.sev_h + r]) : s_p[w][t];
-      const int64_t vat = page * a.sv_p + kvh * a.sv_h + r * a.sv_r;
-      if (lane < D) o[0] += x * page_element<FP8>(a.v, vat + lane);
-      if (lane + 64 < D) o[1] += x * page_element<FP8>(a.v, vat + lane + 64);
-    }
-  }
-  uint16_t* out = a.o + bb * a.so_b + h * a.so_h + n * a.so_n;
-  const float inv = keys > 0 ? 1.f / l : 0.f;
-  if (lane < D) out[lane] = bf16_bits(o[0] * inv);
-  if (lane + 64 < D) out[lane + 64] = bf16_bits(o[1] * inv);
 }
 
 }  // namespace svhip
@@ -111,7 +770,8 @@ using namespace svhip;
 
 extern "C" size_t svhip_paged_attention_workspace_bytes(int64_t B, int64_t H, int64_t Hkv, int64_t N, int packed,
                                                         int64_t D, int64_t max_keys) {
-  return 0;
+  if (B < 1 || H < 1 || Hkv < 1 || H % Hkv != 0 || N < 1 || D < 1 || max_keys < 0) return 0;
+  return paged_plan(B, H, Hkv, N, packed != 0, D, max_keys).bytes();
 }
 
 extern "C" int svhip_paged_attention(const void* q, const void* k_pages, const void* v_pages, const uint8_t* k_exponents,
@@ -149,20 +809,33 @@ extern "C" int svhip_paged_attention(const void* q, const void* k_pages, const v
   SVHIP_REQUIRE(runs(out, so_b, so_h, so_n, 8, 4), "%s: rows of out must start on 8-byte boundaries", name);
   SVHIP_REQUIRE(runs(k_pages, sk_p, sk_h, sk_r, fp8 ? 8 : 16, 8) && runs(v_pages, sv_p, sv_h, sv_r, fp8 ? 8 : 16, 8),
                 "%s: rows of a page must start on %d-byte boundaries", name, fp8 ? 8 : 16);
-  const PagedArgs a{static_cast<const uint16_t*>(q), k_pages, v_pages, k_exponents, v_exponents,
-                    static_cast<uint16_t*>(out), Tokens{cu_queries, B, N},
-                    Pages{page_table, st_b, max_pages, pages, page_shift(page_size), lengths, bad}, H, H / Hkv, D, sq_b,
-                    sq_h, sq_n, sk_p, sk_h, sk_r, sv_p, sv_h, sv_r, sek_p, sek_h, sev_p, sev_h, so_b, so_h, so_n,
-                    causal != 0, scale * kLog2e};
-  const int64_t rows = (cu_queries ? N : B * N) * H;
-  SVHIP_REQUIRE(cdiv(rows, 4) < (1ll << 31), "%s: grid too large", name);
-  const unsigned grid = static_cast<unsigned>(cdiv(rows, 4));
+  PagedArgs a{static_cast<const uint16_t*>(q), k_pages, v_pages, k_exponents, v_exponents, static_cast<uint16_t*>(out),
+              Tokens{cu_queries, B, N}, Pages{page_table, st_b, max_pages, pages, page_shift(page_size), lengths, bad}, H,
+              Hkv, H / Hkv, D, sq_b, sq_h, sq_n, sk_p, sk_h, sk_r, sv_p, sv_h, sv_r, sek_p, sek_h, sev_p, sev_h, so_b,
+              so_h, so_n, causal != 0, scale * kLog2e};
+  const PagedPlan p = paged_plan(B, H, Hkv, N, cu_queries != nullptr, D, max_pages * page_size);
+  SVHIP_REQUIRE(p.bytes() == 0 || (workspace && workspace_bytes >= p.bytes() &&
+                                   reinterpret_cast<uintptr_t>(workspace) % 16 == 0),
+                "%s: workspace too small or misaligned (%zu < %zu bytes)", name, workspace_bytes, p.bytes());
+  SVHIP_REQUIRE(sk_r >= 0 && sk_r < (1 << 26) && sv_r >= 0 && sv_r < (1 << 26), "%s: rows of a page too far apart", name);
+  const int64_t rows = (cu_queries ? N : B * N) * H, join = cdiv(rows, kPagedThreads / 32);
+  SVHIP_REQUIRE(p.row_slots < (1ll << 31) && p.tile_count * Hkv * p.parts < (1ll << 30) && join < (1ll << 31),
+                "%s: grid too large", name);
+  a.q_tiles = p.q_tiles;
+  a.tiles = p.tile_count;
+  a.parts = p.parts;
+  a.row_slots = p.row_slots;
+  a.slot_rows = p.slot_rows;
+  a.row_part = static_cast<float*>(workspace);
+  a.tile_part = a.row_part + p.row_floats;
+  a.plan = p.plan_windows ? reinterpret_cast<int4*>(a.tile_part + p.tile_floats) : nullptr;
   hipStream_t s = as_stream(stream);
   if (fp8) {
-    paged_simple_kernel<true><<<grid, kPagedThreads, 0, s>>>(a);
+    launch_width<true>(a, p, s);
   } else {
-    paged_simple_kernel<false><<<grid, kPagedThreads, 0, s>>>(a);
+    launch_width<false>(a, p, s);
   }
+  if (p.plan_windows) paged_join_kernel<<<static_cast<unsigned>(join), kPagedThreads, 0, s>>>(a);
   SVHIP_LAUNCHED(name);
   return SVHIP_OK;
 }
