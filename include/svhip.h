@@ -29,7 +29,12 @@ enum svhip_dtype { SVHIP_F32 = 0, SVHIP_BF16 = 1, SVHIP_FP8_E4M3 = 3, SVHIP_FP8_
 enum svhip_status { SVHIP_OK = 0, SVHIP_EINVAL = -1, SVHIP_ELAUNCH = -2, SVHIP_EWORKSPACE = -3 };
 
 /* How the pairs of a head turn: element i with i + pairs, 2 i with 2 i + 1, or the three axes of svhip_axial_rope. */
-enum svhip_rotary_layout { SVHIP_ROTARY_NONE = 0, SVHIP_ROTARY_HALF = 1, SVHIP_ROTARY_INTERLEAVED = 2, SVHIP_ROTARY_AXIAL = 3 };
+enum svhip_rotary_layout {
+  SVHIP_ROTARY_NONE = 0,
+  SVHIP_ROTARY_HALF = 1,
+  SVHIP_ROTARY_INTERLEAVED = 2,
+  SVHIP_ROTARY_AXIAL = 3
+};
 
 enum svhip_lel_mode { SVHIP_LEL_LAYER = 0, SVHIP_LEL_BAND = 1, SVHIP_LEL_COLUMN = 2 };
 
@@ -426,65 +431,83 @@ int svhip_sample_chosen(const void* logits, int dtype, int64_t classes, int64_t 
  * (a, b) = (i, i + pairs) for SVHIP_ROTARY_HALF, (2 i, 2 i + 1) for SVHIP_ROTARY_INTERLEAVED. The turns are formed in 64
  * bits, the rest is fp32, rounded once to the type. `inverse`: the transposed rotation, which takes the gradient of out
  * to the gradient of x. x, out: bf16 or fp32 (dtype), element (b, h, n, d) at b*s_b + h*s_h + n*s_n + d; out may be x
- * with the same strides. freq: fp64 [pairs], pairs <= 128.
+ * with the same strides. freq: fp64 [pairs], pairs <= 128. The arguments stand in a struct (a host pointer, read before
+ * the call returns), here and below: a call from Python then costs one packing, not a conversion for each.
  * Beside svhip_axial_rope; no counterpart in the reference, whose positions have three axes.
  */
-int svhip_rotary(const void* x, void* out, int dtype, const void* positions, int positions_wide, const double* freq,
-                 int64_t pairs, int layout, float amplitude, int inverse, int64_t B, int64_t H, int64_t N, int64_t D,
-                 int64_t sx_b, int64_t sx_h, int64_t sx_n, int64_t so_b, int64_t so_h, int64_t so_n, int64_t sp_b,
-                 int64_t sp_n, void* stream);
+typedef struct svhip_rotary_args {
+  const void* x;
+  void* out;
+  const void* positions;
+  const double* freq;
+  int64_t dtype, positions_wide, pairs, layout, inverse;
+  int64_t B, H, N, D, sx_b, sx_h, sx_n, so_b, so_h, so_n, sp_b, sp_n;
+  double amplitude;
+} svhip_rotary_args;
+int svhip_rotary(const svhip_rotary_args* args, void* stream);
 
 /*
- * A paged cache: pools k_pages, v_pages of `pages` pages, element (page, h, r, d) at page*s_p + h*s_h + r*s_r + d, rows r in
- * [0, page_size), page_size a power of two from 16 to 1024; key j of window b is row j % page_size of page
- * page_table[b*st_b + j / page_size] (int32, max_pages numbers a window). kv_dtype SVHIP_BF16, or SVHIP_FP8_E4M3: OCP
- * e4m3fn codes with one power of two for each row and head, value = code 2^(exponent - 127), exponent bytes (page, h, r)
- * at page*se_p + h*se_h + r. Windows may share pages that are only read.
- *
- * svhip_paged_append writes the new tokens' keys and values. Window b has N tokens, element (b, h, n, d) at b*s_b + h*s_h +
- * n*s_n + d, or with cu_tokens (int32 [B + 1], ascending) the packed tokens [cu[b], cu[b + 1]) of N in all (s_b unused;
- * tokens outside every window are left alone). lengths[b] (int32) counts the window's keys with these: token i of n goes
- * to key lengths[b] - before - n + i, so `before` keys behind them are left to another call. `layout` rotates the keys on
- * the way: SVHIP_ROTARY_HALF / _INTERLEAVED as svhip_rotary (freq fp64 [pairs]; positions int32 / int64 at b*sp_b + n*sp_n,
- * or null: the key's index), SVHIP_ROTARY_AXIAL with svhip_axial_rope's arithmetic (positions fp32, three a token; freq
- * fp32 [head_dim / 6]; pairs = head_dim / 2). e4m3: a row's exponent is the least with bound <= 448 2^(exponent - 127),
- * bound = its largest magnitude, for rotated keys 1.5 max(1, |amplitude|) times it before the rotation.
- * `bad` (int32, may be null) is set to 1 when a token's key lies outside the window's row of the table or its page outside
- * the pool; such a token is not written. Key and value rows bf16, 16-byte aligned; rows of a page 16-byte aligned (e4m3:
- * 8). head_dim a multiple of 8 up to 128.
+ * A paged cache: pools k_pages, v_pages of `pages` pages, element (page, h, r, d) at page*s_p + h*s_h + r*s_r + d, rows r
+ * in [0, page_size), page_size a power of two from 16 to 1024, head_dim a multiple of 8 up to 128, rows 16-byte aligned
+ * (e4m3: 8). Key j of window b is row j % page_size of page page_table[b*table_stride + j / page_size] (int32, max_pages
+ * numbers a window); lengths[b] (int32) counts the window's keys. kv_dtype SVHIP_BF16, or SVHIP_FP8_E4M3: OCP e4m3fn
+ * codes with one power of two for each row and head, value = code 2^(exponent - 127), exponent bytes (page, h, r) at
+ * page*se_p + h*se_h + r. Windows may share pages that are only read. `bad` (int32, may be null) is set to 1 by a call
+ * that meets a page outside the pool or a key outside its window's row of the table.
+ */
+typedef struct svhip_paged_cache {
+  void *k_pages, *v_pages;
+  uint8_t *k_exponents, *v_exponents;
+  const int32_t *page_table, *lengths;
+  int32_t* bad;
+  int64_t kv_dtype, windows, heads, head_dim, pages, page_size, max_pages, table_stride;
+  int64_t sk_p, sk_h, sk_r, sv_p, sv_h, sv_r, sek_p, sek_h, sev_p, sev_h;
+} svhip_paged_cache;
+
+/*
+ * Writes the new tokens' keys and values into a paged cache. Window b has N tokens, element (b, h, n, d) at b*s_b + h*s_h
+ * + n*s_n + d, or with cu_tokens (int32 [windows + 1], ascending) the packed tokens [cu[b], cu[b + 1]) of N in all (s_b
+ * unused; tokens outside every window are left alone). The window's length counts them: token i of n goes to key
+ * lengths[b] - before - n + i, so `before` keys behind them are left to another call. `layout` rotates the keys on the
+ * way: SVHIP_ROTARY_HALF / _INTERLEAVED as svhip_rotary (freq fp64 [pairs]; positions int32 / int64 at b*sp_b + n*sp_n, or
+ * null: the key's index), SVHIP_ROTARY_AXIAL with svhip_axial_rope's arithmetic (positions fp32, three a token; freq fp32
+ * [head_dim / 6]; pairs = head_dim / 2). e4m3: a row's exponent is the least with bound <= 448 2^(exponent - 127), bound =
+ * its largest magnitude, for rotated keys 1.5 max(1, |amplitude|) times it before the rotation. A token whose key or page
+ * is bad is not written. Key and value rows bf16, 16-byte aligned.
  * Beside svhip_kv_write (FastSlotForward.encode + _write, streamvoxel/stream/fast_ops.py:228-250), which rewrites a
  * window's slab whole; no counterpart in the reference.
  */
-int svhip_paged_append(const void* key, const void* value, int64_t sk_b, int64_t sk_h, int64_t sk_n, int64_t sv_b,
-                       int64_t sv_h, int64_t sv_n, int64_t B, int64_t H, int64_t N, int64_t D, const int32_t* cu_tokens,
-                       int64_t before, void* k_pages, void* v_pages, uint8_t* k_exponents, uint8_t* v_exponents,
-                       int kv_dtype, int64_t pages, int64_t page_size, int64_t sck_p, int64_t sck_h, int64_t sck_r,
-                       int64_t scv_p, int64_t scv_h, int64_t scv_r, int64_t sek_p, int64_t sek_h, int64_t sev_p,
-                       int64_t sev_h, const int32_t* page_table, int64_t st_b, int64_t max_pages, const int32_t* lengths,
-                       int layout, const void* positions, int positions_wide, int64_t sp_b, int64_t sp_n,
-                       const void* freq, int64_t pairs, float amplitude, int32_t* bad, void* stream);
+typedef struct svhip_paged_append_args {
+  const void *key, *value;
+  const int32_t* cu_tokens;
+  const void *positions, *freq;
+  int64_t N, before, sk_b, sk_h, sk_n, sv_b, sv_h, sv_n;
+  int64_t layout, positions_wide, sp_b, sp_n, pairs;
+  double amplitude;
+} svhip_paged_append_args;
+int svhip_paged_append(const svhip_paged_cache* cache, const svhip_paged_append_args* args, void* stream);
 
 /*
- * Attention of the windows' new tokens over a paged cache: out[b, h, i] = softmax_j(scale q[b, h, i] . k_j) v_j over the keys
- * j < lengths[b] of key head h / (H / Hkv), with `causal` only j <= lengths[b] - n + i (n tokens of window b, its last
- * keys); no key: zeros. Queries and out bf16, N a window or packed by cu_queries, as in svhip_paged_append (rows outside
- * every window are left as they are). Products in bf16 on the matrix cores with fp32 sums, softmax weights rounded to
- * bf16. `bad` is set to 1 when a page lies outside the pool (its keys and values then read as zeros) or lengths[b] passes
- * the window's row of the table (and is cut to it). scale > 0. Query rows 16-byte aligned, rows of out 8, rows of a page as
- * in svhip_paged_append. workspace: svhip_paged_attention_workspace_bytes with max_keys = max_pages * page_size (0: none
- * needed), N and packed (cu_queries or not) as in the call; 16-byte aligned.
+ * Attention of the windows' new tokens over a paged cache: out[b, h, i] = softmax_j(scale q[b, h, i] . k_j) v_j over the
+ * keys j < lengths[b] of key head h / (H / heads), with `causal` only j <= lengths[b] - n + i (n tokens of window b, its
+ * last keys); no key: zeros. Queries and out bf16, N a window or packed by cu_queries, as in svhip_paged_append (rows
+ * outside every window are left as they are). Products in bf16 on the matrix cores with fp32 sums, softmax weights rounded
+ * to bf16. Keys and values of a bad page read as zeros; a length past the window's row of the table is cut to it. scale >
+ * 0. Query rows 16-byte aligned, rows of out 8. workspace: svhip_paged_attention_workspace_bytes with max_keys = max_pages
+ * * page_size (0: none needed), N and packed (cu_queries or not) as in the call; 16-byte aligned.
  * Beside svhip_xattn_fwd (streamvoxel/stream/fast_ops.py:104-108); no counterpart in the reference.
  */
+typedef struct svhip_paged_attention_args {
+  const void* q;
+  void* out;
+  const int32_t* cu_queries;
+  void* workspace;
+  int64_t workspace_bytes, H, N, sq_b, sq_h, sq_n, so_b, so_h, so_n, causal;
+  double scale;
+} svhip_paged_attention_args;
 size_t svhip_paged_attention_workspace_bytes(int64_t B, int64_t H, int64_t Hkv, int64_t N, int packed, int64_t D,
                                              int64_t max_keys);
-int svhip_paged_attention(const void* q, const void* k_pages, const void* v_pages, const uint8_t* k_exponents,
-                          const uint8_t* v_exponents, void* out, int kv_dtype, int64_t B, int64_t H, int64_t Hkv,
-                          int64_t N, int64_t D, const int32_t* cu_queries, int64_t pages, int64_t page_size,
-                          const int32_t* page_table, int64_t st_b, int64_t max_pages, const int32_t* lengths,
-                          int64_t sq_b, int64_t sq_h, int64_t sq_n, int64_t sk_p, int64_t sk_h, int64_t sk_r,
-                          int64_t sv_p, int64_t sv_h, int64_t sv_r, int64_t sek_p, int64_t sek_h, int64_t sev_p,
-                          int64_t sev_h, int64_t so_b, int64_t so_h, int64_t so_n, int causal, float scale, int32_t* bad,
-                          void* workspace, size_t workspace_bytes, void* stream);
+int svhip_paged_attention(const svhip_paged_cache* cache, const svhip_paged_attention_args* args, void* stream);
 
 #ifdef __cplusplus
 }

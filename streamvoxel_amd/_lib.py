@@ -21,6 +21,7 @@ SVHIP_LEL_LAYER, SVHIP_LEL_BAND, SVHIP_LEL_COLUMN = 0, 1, 2
 
 _c_i64, _c_i32, _c_p, _c_sz, _c_f, _c_d = (ctypes.c_int64, ctypes.c_int32, ctypes.c_void_p, ctypes.c_size_t,
                                              ctypes.c_float, ctypes.c_double)
+_c_b = ctypes.c_char_p   # a struct of arguments, packed into bytes
 
 # name -> (restype, argtypes); mirrors include/svhip.h
 SIGNATURES = {
@@ -83,15 +84,10 @@ SIGNATURES = {
                             + [_c_i64] * 12 + [_c_f, _c_p]),
     'svhip_patch_embed': (ctypes.c_int, [_c_p] * 5 + [_c_i64] * 10 + [_c_p]),
     'svhip_sample_chosen': (ctypes.c_int, [_c_p, ctypes.c_int] + [_c_i64] * 5 + [_c_p] * 6 + [_c_i64] * 4 + [_c_p]),
-    'svhip_rotary': (ctypes.c_int, [_c_p, _c_p, ctypes.c_int, _c_p, ctypes.c_int, _c_p, _c_i64, ctypes.c_int, _c_f,
-                                    ctypes.c_int] + [_c_i64] * 12 + [_c_p]),
-    'svhip_paged_append': (ctypes.c_int, [_c_p, _c_p] + [_c_i64] * 10 + [_c_p, _c_i64] + [_c_p] * 4 + [ctypes.c_int]
-                           + [_c_i64] * 12 + [_c_p, _c_i64, _c_i64, _c_p, ctypes.c_int, _c_p, ctypes.c_int, _c_i64,
-                                              _c_i64, _c_p, _c_i64, _c_f, _c_p, _c_p]),
+    'svhip_rotary': (ctypes.c_int, [_c_b, _c_p]),
+    'svhip_paged_append': (ctypes.c_int, [_c_b, _c_b, _c_p]),
     'svhip_paged_attention_workspace_bytes': (_c_sz, [_c_i64] * 4 + [ctypes.c_int] + [_c_i64] * 2),
-    'svhip_paged_attention': (ctypes.c_int, [_c_p] * 6 + [ctypes.c_int] + [_c_i64] * 5 + [_c_p, _c_i64, _c_i64, _c_p,
-                                                                                      _c_i64, _c_i64, _c_p]
-                              + [_c_i64] * 16 + [ctypes.c_int, _c_f, _c_p, _c_p, _c_sz, _c_p]),
+    'svhip_paged_attention': (ctypes.c_int, [_c_b, _c_b, _c_p]),
 }
 
 _lib = None
@@ -141,10 +137,15 @@ def require_gpu(*tensors):
                                % (t.device if torch.is_tensor(t) else type(t).__name__))
 
 
-def require_same_device(first, *tensors):
+def require_one_gpu(first, *tensors):
+    """require_gpu, and all of them on one device."""
+    device = first.device if torch.is_tensor(first) else None
     for t in tensors:
-        if t is not None and t.device != first.device:
-            raise ValueError(f'tensors on {first.device} and {t.device}: one call takes one device')
+        if t is not None and not (torch.is_tensor(t) and t.device == device):
+            require_gpu(first, *tensors)
+            raise ValueError(f'tensors on {device} and {t.device}: one call takes one device')
+    if device is None or device.type != 'cuda':
+        require_gpu(first, *tensors)
 
 
 def device_of(t):

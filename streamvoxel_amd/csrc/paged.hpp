@@ -10,6 +10,7 @@ namespace svhip {
 
 constexpr int kMinPage = 16;
 constexpr int kMaxPage = 1024;
+constexpr int kMaxPagedDim = 128;
 
 struct Pages {
   const int32_t* table;   // [B, max_pages], rows st_b apart
@@ -86,6 +87,47 @@ inline int page_shift(int64_t page) {
   int s = 0;
   while ((1ll << s) < page) ++s;
   return s;
+}
+
+// What both calls ask of a cache; the status of the first check that fails.
+inline int check_cache(const char* name, const svhip_paged_cache* cache) {
+  SVHIP_REQUIRE(cache, "%s: null cache", name);
+  const svhip_paged_cache& c = *cache;
+  SVHIP_REQUIRE(c.windows >= 0 && c.heads >= 0, "%s: bad sizes", name);
+  SVHIP_REQUIRE(c.head_dim >= 8 && c.head_dim <= kMaxPagedDim && c.head_dim % 8 == 0,
+                "%s: head_dim %lld unsupported (a multiple of 8 up to %d)", name, (long long)c.head_dim, kMaxPagedDim);
+  SVHIP_REQUIRE(c.kv_dtype == SVHIP_BF16 || c.kv_dtype == SVHIP_FP8_E4M3, "%s: kv dtype %d unsupported", name,
+                (int)c.kv_dtype);
+  SVHIP_REQUIRE(c.page_size >= kMinPage && c.page_size <= kMaxPage && (c.page_size & (c.page_size - 1)) == 0,
+                "%s: page size %lld unsupported (a power of two, %d to %d)", name, (long long)c.page_size, kMinPage,
+                kMaxPage);
+  SVHIP_REQUIRE(c.pages >= 0 && c.pages < (1ll << 31) && c.max_pages >= 0 && c.max_pages < (1ll << 31) / c.page_size,
+                "%s: bad page counts", name);
+  return SVHIP_OK;
+}
+
+// The checks of a cache that a call touches.
+inline int check_pool(const char* name, const svhip_paged_cache& c) {
+  const bool fp8 = c.kv_dtype == SVHIP_FP8_E4M3;
+  SVHIP_REQUIRE(c.lengths && (c.max_pages == 0 || c.page_table) && (c.pages == 0 || (c.k_pages && c.v_pages)),
+                "%s: null pointer", name);
+  SVHIP_REQUIRE(!fp8 || c.pages == 0 || (c.k_exponents && c.v_exponents), "%s: e4m3 pages need the rows' exponents", name);
+  const uintptr_t bytes = fp8 ? 8 : 16;
+  SVHIP_REQUIRE(reinterpret_cast<uintptr_t>(c.k_pages) % bytes == 0 && reinterpret_cast<uintptr_t>(c.v_pages) % bytes == 0 &&
+                    (c.sk_p | c.sk_h | c.sk_r | c.sv_p | c.sv_h | c.sv_r) % 8 == 0,
+                "%s: rows of a page must start on %d-byte boundaries", name, (int)bytes);
+  SVHIP_REQUIRE(c.sk_r >= 0 && c.sk_r < (1 << 26) && c.sv_r >= 0 && c.sv_r < (1 << 26), "%s: rows of a page too far apart",
+                name);
+  return SVHIP_OK;
+}
+
+// Rows of 8 bf16 values that start on 16-byte boundaries.
+inline bool rows16(const void* p, int64_t x, int64_t y, int64_t z) {
+  return reinterpret_cast<uintptr_t>(p) % 16 == 0 && (x | y | z) % 8 == 0;
+}
+
+inline Pages pages_of(const svhip_paged_cache& c) {
+  return Pages{c.page_table, c.table_stride, c.max_pages, c.pages, page_shift(c.page_size), c.lengths, c.bad};
 }
 
 }  // namespace svhip

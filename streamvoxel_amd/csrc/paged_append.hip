@@ -13,7 +13,6 @@ namespace svhip {
 constexpr int kAppendThreads = 256;
 constexpr int kAppendTokens = 8;
 constexpr int kAppendLanes = 16;
-constexpr int kAppendMaxDim = 128;
 
 enum AppendTurn { kTurnNone = 0, kTurnRotary = 1, kTurnAxial = 2 };
 
@@ -53,7 +52,7 @@ __device__ __forceinline__ float turned_element(const AppendArgs& a, int turn, c
 
 template <int TURN, bool FP8>
 __global__ __launch_bounds__(kAppendThreads) void paged_append_kernel(AppendArgs a) {
-  __shared__ float2 table[kAppendTokens * kAppendMaxDim / 2];
+  __shared__ float2 table[kAppendTokens * kMaxPagedDim / 2];
   __shared__ int64_t s_src[kAppendTokens][2], s_page[kAppendTokens], s_pos[kAppendTokens];
   __shared__ int s_row[kAppendTokens];
   const int64_t total = a.tokens.cu ? a.tokens.N : a.tokens.B * a.tokens.N;
@@ -160,56 +159,41 @@ void launch_append(const AppendArgs& a, unsigned grid, bool fp8, hipStream_t s) 
 
 using namespace svhip;
 
-extern "C" int svhip_paged_append(const void* key, const void* value, int64_t sk_b, int64_t sk_h, int64_t sk_n,
-                                  int64_t sv_b, int64_t sv_h, int64_t sv_n, int64_t B, int64_t H, int64_t N, int64_t D,
-                                  const int32_t* cu_tokens, int64_t before, void* k_pages, void* v_pages,
-                                  uint8_t* k_exponents, uint8_t* v_exponents, int kv_dtype, int64_t pages,
-                                  int64_t page_size, int64_t sck_p, int64_t sck_h, int64_t sck_r, int64_t scv_p,
-                                  int64_t scv_h, int64_t scv_r, int64_t sek_p, int64_t sek_h, int64_t sev_p,
-                                  int64_t sev_h, const int32_t* page_table, int64_t st_b, int64_t max_pages,
-                                  const int32_t* lengths, int layout, const void* positions, int positions_wide,
-                                  int64_t sp_b, int64_t sp_n, const void* freq, int64_t pairs, float amplitude,
-                                  int32_t* bad, void* stream) {
+extern "C" int svhip_paged_append(const svhip_paged_cache* cache, const svhip_paged_append_args* args, void* stream) {
   const char* name = "svhip_paged_append";
   clear_error();
-  SVHIP_REQUIRE(B >= 0 && H >= 0 && N >= 0 && before >= 0, "%s: bad sizes", name);
-  SVHIP_REQUIRE(D >= 8 && D <= kAppendMaxDim && D % 8 == 0, "%s: head_dim %lld unsupported (a multiple of 8 up to %d)",
-                name, (long long)D, kAppendMaxDim);
-  SVHIP_REQUIRE(kv_dtype == SVHIP_BF16 || kv_dtype == SVHIP_FP8_E4M3, "%s: kv dtype %d unsupported", name, kv_dtype);
-  SVHIP_REQUIRE(page_size >= kMinPage && page_size <= kMaxPage && (page_size & (page_size - 1)) == 0,
-                "%s: page size %lld unsupported (a power of two, %d to %d)", name, (long long)page_size, kMinPage,
-                kMaxPage);
-  SVHIP_REQUIRE(pages >= 0 && pages < (1ll << 31) && max_pages >= 0 && max_pages < (1ll << 31), "%s: bad page counts", name);
-  const bool turns = layout != SVHIP_ROTARY_NONE, axial = layout == SVHIP_ROTARY_AXIAL;
-  SVHIP_REQUIRE(layout >= SVHIP_ROTARY_NONE && layout <= SVHIP_ROTARY_AXIAL, "%s: layout %d unsupported", name, layout);
-  SVHIP_REQUIRE(!turns || (pairs >= 1 && 2 * pairs <= D), "%s: %lld pairs do not fit head_dim %lld", name, (long long)pairs,
-                (long long)D);
-  SVHIP_REQUIRE(!axial || (2 * pairs == D && D % 6 == 0),
+  if (const int rc = check_cache(name, cache)) return rc;
+  SVHIP_REQUIRE(args, "%s: null arguments", name);
+  const svhip_paged_cache& p = *cache;
+  const svhip_paged_append_args& c = *args;
+  const int64_t D = p.head_dim;
+  SVHIP_REQUIRE(c.N >= 0 && c.before >= 0, "%s: bad sizes", name);
+  const bool turns = c.layout != SVHIP_ROTARY_NONE, axial = c.layout == SVHIP_ROTARY_AXIAL;
+  SVHIP_REQUIRE(c.layout >= SVHIP_ROTARY_NONE && c.layout <= SVHIP_ROTARY_AXIAL, "%s: layout %d unsupported", name,
+                (int)c.layout);
+  SVHIP_REQUIRE(!turns || (c.pairs >= 1 && 2 * c.pairs <= D), "%s: %lld pairs do not fit head_dim %lld", name,
+                (long long)c.pairs, (long long)D);
+  SVHIP_REQUIRE(!axial || (2 * c.pairs == D && D % 6 == 0),
                 "%s: the three-axis rotation takes the whole head, a multiple of 6", name);
-  const bool fp8 = kv_dtype == SVHIP_FP8_E4M3;
-  if (B == 0 || H == 0 || N == 0) return SVHIP_OK;
-  SVHIP_REQUIRE(key && value && k_pages && v_pages && page_table && lengths, "%s: null pointer", name);
-  SVHIP_REQUIRE(!turns || freq, "%s: the rotation needs frequencies", name);
-  SVHIP_REQUIRE(!axial || positions, "%s: the three-axis rotation needs positions", name);
-  SVHIP_REQUIRE(!fp8 || (k_exponents && v_exponents), "%s: e4m3 pages need the rows' exponents", name);
-  SVHIP_REQUIRE(H <= 1 << 20, "%s: sizes too large", name);
-  auto runs = [](const void* p, int64_t x, int64_t y, int64_t z, uintptr_t bytes, int64_t elems) {
-    return reinterpret_cast<uintptr_t>(p) % bytes == 0 && x % elems == 0 && y % elems == 0 && z % elems == 0;
-  };
-  SVHIP_REQUIRE(runs(key, sk_b, sk_h, sk_n, 16, 8) && runs(value, sv_b, sv_h, sv_n, 16, 8),
+  if (p.windows == 0 || p.heads == 0 || c.N == 0) return SVHIP_OK;
+  if (const int rc = check_pool(name, p)) return rc;
+  SVHIP_REQUIRE(c.key && c.value, "%s: null pointer", name);
+  SVHIP_REQUIRE(!turns || c.freq, "%s: the rotation needs frequencies", name);
+  SVHIP_REQUIRE(!axial || c.positions, "%s: the three-axis rotation needs positions", name);
+  SVHIP_REQUIRE(p.heads <= 1 << 20, "%s: sizes too large", name);
+  SVHIP_REQUIRE(rows16(c.key, c.sk_b, c.sk_h, c.sk_n) && rows16(c.value, c.sv_b, c.sv_h, c.sv_n),
                 "%s: key and value rows must start on 16-byte boundaries", name);
-  SVHIP_REQUIRE(runs(k_pages, sck_p, sck_h, sck_r, fp8 ? 8 : 16, 8) && runs(v_pages, scv_p, scv_h, scv_r, fp8 ? 8 : 16, 8),
-                "%s: rows of a page must start on %d-byte boundaries", name, fp8 ? 8 : 16);
-  const int64_t total = cu_tokens ? N : B * N;
+  const int64_t total = c.cu_tokens ? c.N : p.windows * c.N;
   const int64_t grid = cdiv(total, kAppendTokens);
   SVHIP_REQUIRE(grid < (1ll << 31), "%s: grid too large", name);
-  const float most = amplitude < 0.f ? -amplitude : amplitude;
-  const AppendArgs a{static_cast<const uint16_t*>(key), static_cast<const uint16_t*>(value), sk_b, sk_h, sk_n, sv_b, sv_h,
-                     sv_n, Tokens{cu_tokens, B, N}, before, H, D, k_pages, v_pages, sck_p, sck_h, sck_r, scv_p, scv_h,
-                     scv_r, k_exponents, v_exponents, sek_p, sek_h, sev_p, sev_h,
-                     Pages{page_table, st_b, max_pages, pages, page_shift(page_size), lengths, bad}, positions, sp_b, sp_n,
-                     freq, turns ? static_cast<int>(pairs) : 0, axial || layout == SVHIP_ROTARY_INTERLEAVED,
-                     positions_wide != 0, amplitude, turns ? 1.5f * (axial || most < 1.f ? 1.f : most) : 1.f};
+  const float amplitude = static_cast<float>(c.amplitude), most = amplitude < 0.f ? -amplitude : amplitude;
+  const bool fp8 = p.kv_dtype == SVHIP_FP8_E4M3;
+  const AppendArgs a{static_cast<const uint16_t*>(c.key), static_cast<const uint16_t*>(c.value), c.sk_b, c.sk_h, c.sk_n,
+                     c.sv_b, c.sv_h, c.sv_n, Tokens{c.cu_tokens, p.windows, c.N}, c.before, p.heads, D, p.k_pages,
+                     p.v_pages, p.sk_p, p.sk_h, p.sk_r, p.sv_p, p.sv_h, p.sv_r, p.k_exponents, p.v_exponents, p.sek_p,
+                     p.sek_h, p.sev_p, p.sev_h, pages_of(p), c.positions, c.sp_b, c.sp_n, c.freq,
+                     turns ? static_cast<int>(c.pairs) : 0, axial || c.layout == SVHIP_ROTARY_INTERLEAVED,
+                     c.positions_wide != 0, amplitude, turns ? 1.5f * (axial || most < 1.f ? 1.f : most) : 1.f};
   hipStream_t s = as_stream(stream);
   if (axial) {
     launch_append<kTurnAxial>(a, static_cast<unsigned>(grid), fp8, s);

@@ -20,7 +20,6 @@
 
 namespace svhip {
 
-constexpr int kPagedMaxDim = 128;
 constexpr int kPagedThreads = 256;
 constexpr int kRows = 32;          // rows of a wave
 constexpr int kTileRows = 128;     // rows of a tile workgroup
@@ -774,63 +773,42 @@ extern "C" size_t svhip_paged_attention_workspace_bytes(int64_t B, int64_t H, in
   return paged_plan(B, H, Hkv, N, packed != 0, D, max_keys).bytes();
 }
 
-extern "C" int svhip_paged_attention(const void* q, const void* k_pages, const void* v_pages, const uint8_t* k_exponents,
-                                     const uint8_t* v_exponents, void* out, int kv_dtype, int64_t B, int64_t H,
-                                     int64_t Hkv, int64_t N, int64_t D, const int32_t* cu_queries, int64_t pages,
-                                     int64_t page_size, const int32_t* page_table, int64_t st_b, int64_t max_pages,
-                                     const int32_t* lengths, int64_t sq_b, int64_t sq_h, int64_t sq_n, int64_t sk_p,
-                                     int64_t sk_h, int64_t sk_r, int64_t sv_p, int64_t sv_h, int64_t sv_r, int64_t sek_p,
-                                     int64_t sek_h, int64_t sev_p, int64_t sev_h, int64_t so_b, int64_t so_h,
-                                     int64_t so_n, int causal, float scale, int32_t* bad, void* workspace,
-                                     size_t workspace_bytes, void* stream) {
+extern "C" int svhip_paged_attention(const svhip_paged_cache* cache, const svhip_paged_attention_args* args,
+                                     void* stream) {
   const char* name = "svhip_paged_attention";
   clear_error();
-  SVHIP_REQUIRE(B >= 0 && H >= 0 && N >= 0, "%s: bad sizes", name);
-  SVHIP_REQUIRE(D >= 8 && D <= kPagedMaxDim && D % 8 == 0, "%s: head_dim %lld unsupported (a multiple of 8 up to %d)",
-                name, (long long)D, kPagedMaxDim);
+  if (const int rc = check_cache(name, cache)) return rc;
+  SVHIP_REQUIRE(args, "%s: null arguments", name);
+  const svhip_paged_cache& pc = *cache;
+  const svhip_paged_attention_args& c = *args;
+  const int64_t B = pc.windows, H = c.H, Hkv = pc.heads, N = c.N, D = pc.head_dim;
+  SVHIP_REQUIRE(H >= 0 && N >= 0, "%s: bad sizes", name);
   SVHIP_REQUIRE(Hkv >= 1 && H % Hkv == 0, "%s: %lld heads do not share %lld key heads evenly", name, (long long)H,
                 (long long)Hkv);
-  SVHIP_REQUIRE(kv_dtype == SVHIP_BF16 || kv_dtype == SVHIP_FP8_E4M3, "%s: kv dtype %d unsupported", name, kv_dtype);
+  const float scale = static_cast<float>(c.scale);
   SVHIP_REQUIRE(scale > 0.f && scale < INFINITY, "%s: scale must be positive and finite", name);
-  SVHIP_REQUIRE(page_size >= kMinPage && page_size <= kMaxPage && (page_size & (page_size - 1)) == 0,
-                "%s: page size %lld unsupported (a power of two, %d to %d)", name, (long long)page_size, kMinPage,
-                kMaxPage);
-  SVHIP_REQUIRE(pages >= 0 && pages < (1ll << 31) && max_pages >= 0 && max_pages * page_size < (1ll << 31),
-                "%s: bad page counts", name);
-  const bool fp8 = kv_dtype == SVHIP_FP8_E4M3;
   if (B == 0 || H == 0 || N == 0) return SVHIP_OK;
-  SVHIP_REQUIRE(q && out && lengths && (max_pages == 0 || page_table) && (pages == 0 || (k_pages && v_pages)),
-                "%s: null pointer", name);
-  SVHIP_REQUIRE(!fp8 || (k_exponents && v_exponents), "%s: e4m3 pages need the rows' exponents", name);
-  auto runs = [](const void* p, int64_t x, int64_t y, int64_t z, uintptr_t bytes, int64_t elems) {
-    return reinterpret_cast<uintptr_t>(p) % bytes == 0 && x % elems == 0 && y % elems == 0 && z % elems == 0;
-  };
-  SVHIP_REQUIRE(runs(q, sq_b, sq_h, sq_n, 16, 8), "%s: query rows must start on 16-byte boundaries", name);
-  SVHIP_REQUIRE(runs(out, so_b, so_h, so_n, 8, 4), "%s: rows of out must start on 8-byte boundaries", name);
-  SVHIP_REQUIRE(runs(k_pages, sk_p, sk_h, sk_r, fp8 ? 8 : 16, 8) && runs(v_pages, sv_p, sv_h, sv_r, fp8 ? 8 : 16, 8),
-                "%s: rows of a page must start on %d-byte boundaries", name, fp8 ? 8 : 16);
-  PagedArgs a{static_cast<const uint16_t*>(q), k_pages, v_pages, k_exponents, v_exponents, static_cast<uint16_t*>(out),
-              Tokens{cu_queries, B, N}, Pages{page_table, st_b, max_pages, pages, page_shift(page_size), lengths, bad}, H,
-              Hkv, H / Hkv, D, sq_b, sq_h, sq_n, sk_p, sk_h, sk_r, sv_p, sv_h, sv_r, sek_p, sek_h, sev_p, sev_h, so_b,
-              so_h, so_n, causal != 0, scale * kLog2e};
-  const PagedPlan p = paged_plan(B, H, Hkv, N, cu_queries != nullptr, D, max_pages * page_size);
-  SVHIP_REQUIRE(p.bytes() == 0 || (workspace && workspace_bytes >= p.bytes() &&
-                                   reinterpret_cast<uintptr_t>(workspace) % 16 == 0),
-                "%s: workspace too small or misaligned (%zu < %zu bytes)", name, workspace_bytes, p.bytes());
-  SVHIP_REQUIRE(sk_r >= 0 && sk_r < (1 << 26) && sv_r >= 0 && sv_r < (1 << 26), "%s: rows of a page too far apart", name);
-  const int64_t rows = (cu_queries ? N : B * N) * H, join = cdiv(rows, kPagedThreads / 32);
+  if (const int rc = check_pool(name, pc)) return rc;
+  SVHIP_REQUIRE(c.q && c.out, "%s: null pointer", name);
+  SVHIP_REQUIRE(rows16(c.q, c.sq_b, c.sq_h, c.sq_n), "%s: query rows must start on 16-byte boundaries", name);
+  SVHIP_REQUIRE(reinterpret_cast<uintptr_t>(c.out) % 8 == 0 && (c.so_b | c.so_h | c.so_n) % 4 == 0,
+                "%s: rows of out must start on 8-byte boundaries", name);
+  const PagedPlan p = paged_plan(B, H, Hkv, N, c.cu_queries != nullptr, D, pc.max_pages * pc.page_size);
+  SVHIP_REQUIRE(p.bytes() == 0 || (c.workspace && c.workspace_bytes >= static_cast<int64_t>(p.bytes()) &&
+                                   reinterpret_cast<uintptr_t>(c.workspace) % 16 == 0),
+                "%s: workspace too small or misaligned (%lld < %zu bytes)", name, (long long)c.workspace_bytes, p.bytes());
+  const int64_t rows = (c.cu_queries ? N : B * N) * H, join = cdiv(rows, kPagedThreads / 32);
   SVHIP_REQUIRE(p.row_slots < (1ll << 31) && p.tile_count * Hkv * p.parts < (1ll << 30) && join < (1ll << 31),
                 "%s: grid too large", name);
-  a.q_tiles = p.q_tiles;
-  a.tiles = p.tile_count;
-  a.parts = p.parts;
-  a.row_slots = p.row_slots;
-  a.slot_rows = p.slot_rows;
-  a.row_part = static_cast<float*>(workspace);
-  a.tile_part = a.row_part + p.row_floats;
-  a.plan = p.plan_windows ? reinterpret_cast<int4*>(a.tile_part + p.tile_floats) : nullptr;
+  float* const part = static_cast<float*>(c.workspace);
+  const PagedArgs a{static_cast<const uint16_t*>(c.q), pc.k_pages, pc.v_pages, pc.k_exponents, pc.v_exponents,
+                    static_cast<uint16_t*>(c.out), Tokens{c.cu_queries, B, N}, pages_of(pc), H, Hkv, H / Hkv, D, c.sq_b,
+                    c.sq_h, c.sq_n, pc.sk_p, pc.sk_h, pc.sk_r, pc.sv_p, pc.sv_h, pc.sv_r, pc.sek_p, pc.sek_h, pc.sev_p,
+                    pc.sev_h, c.so_b, c.so_h, c.so_n, c.causal != 0, scale * kLog2e, p.q_tiles, p.tile_count, p.parts,
+                    p.row_slots, p.slot_rows, part, part + p.row_floats,
+                    p.plan_windows ? reinterpret_cast<int4*>(part + p.row_floats + p.tile_floats) : nullptr};
   hipStream_t s = as_stream(stream);
-  if (fp8) {
+  if (pc.kv_dtype == SVHIP_FP8_E4M3) {
     launch_width<true>(a, p, s);
   } else {
     launch_width<false>(a, p, s);

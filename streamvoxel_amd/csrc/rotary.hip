@@ -69,29 +69,28 @@ __global__ __launch_bounds__(kRotaryThreads) void rotary_kernel(RotaryArgs a) {
 
 using namespace svhip;
 
-extern "C" int svhip_rotary(const void* x, void* out, int dtype, const void* positions, int positions_wide,
-                            const double* freq, int64_t pairs, int layout, float amplitude, int inverse, int64_t B,
-                            int64_t H, int64_t N, int64_t D, int64_t sx_b, int64_t sx_h, int64_t sx_n, int64_t so_b,
-                            int64_t so_h, int64_t so_n, int64_t sp_b, int64_t sp_n, void* stream) {
+extern "C" int svhip_rotary(const svhip_rotary_args* args, void* stream) {
   const char* name = "svhip_rotary";
   clear_error();
-  SVHIP_REQUIRE(B >= 0 && H >= 0 && N >= 0 && D >= 1, "%s: bad sizes", name);
-  SVHIP_REQUIRE(dtype == SVHIP_F32 || dtype == SVHIP_BF16, "%s: dtype %d unsupported", name, dtype);
-  SVHIP_REQUIRE(layout == SVHIP_ROTARY_HALF || layout == SVHIP_ROTARY_INTERLEAVED, "%s: layout %d unsupported", name,
-                layout);
-  SVHIP_REQUIRE(pairs >= 1 && pairs <= kMaxRotaryPairs && 2 * pairs <= D,
-                "%s: %lld pairs do not fit head_dim %lld (at most %d)", name, (long long)pairs, (long long)D,
+  SVHIP_REQUIRE(args, "%s: null arguments", name);
+  const svhip_rotary_args& c = *args;
+  SVHIP_REQUIRE(c.B >= 0 && c.H >= 0 && c.N >= 0 && c.D >= 1, "%s: bad sizes", name);
+  SVHIP_REQUIRE(c.dtype == SVHIP_F32 || c.dtype == SVHIP_BF16, "%s: dtype %d unsupported", name, (int)c.dtype);
+  SVHIP_REQUIRE(c.layout == SVHIP_ROTARY_HALF || c.layout == SVHIP_ROTARY_INTERLEAVED, "%s: layout %d unsupported", name,
+                (int)c.layout);
+  SVHIP_REQUIRE(c.pairs >= 1 && c.pairs <= kMaxRotaryPairs && 2 * c.pairs <= c.D,
+                "%s: %lld pairs do not fit head_dim %lld (at most %d)", name, (long long)c.pairs, (long long)c.D,
                 kMaxRotaryPairs);
-  SVHIP_REQUIRE(D <= 1 << 20 && H <= 1 << 20, "%s: sizes too large", name);
-  if (B == 0 || H == 0 || N == 0) return SVHIP_OK;
-  SVHIP_REQUIRE(x && out && positions && freq, "%s: null pointer", name);
-  const int64_t grid = B * cdiv(N, kRotaryTokens);
+  SVHIP_REQUIRE(c.D <= 1 << 20 && c.H <= 1 << 20, "%s: sizes too large", name);
+  if (c.B == 0 || c.H == 0 || c.N == 0) return SVHIP_OK;
+  SVHIP_REQUIRE(c.x && c.out && c.positions && c.freq, "%s: null pointer", name);
+  const int64_t grid = c.B * cdiv(c.N, kRotaryTokens);
   SVHIP_REQUIRE(grid < (1ll << 31), "%s: grid too large", name);
-  const RotaryArgs a{x, out, positions, freq, B, H, N, D, static_cast<int>(pairs), positions_wide != 0,
-                     layout == SVHIP_ROTARY_INTERLEAVED, amplitude, inverse ? -1.f : 1.f, sx_b, sx_h, sx_n, so_b, so_h,
-                     so_n, sp_b, sp_n};
+  const RotaryArgs a{c.x, c.out, c.positions, c.freq, c.B, c.H, c.N, c.D, static_cast<int>(c.pairs),
+                     c.positions_wide != 0, c.layout == SVHIP_ROTARY_INTERLEAVED, static_cast<float>(c.amplitude),
+                     c.inverse ? -1.f : 1.f, c.sx_b, c.sx_h, c.sx_n, c.so_b, c.so_h, c.so_n, c.sp_b, c.sp_n};
   hipStream_t s = as_stream(stream);
-  if (dtype == SVHIP_F32) {
+  if (c.dtype == SVHIP_F32) {
     rotary_kernel<float><<<static_cast<unsigned>(grid), kRotaryThreads, 0, s>>>(a);
   } else {
     rotary_kernel<uint16_t><<<static_cast<unsigned>(grid), kRotaryThreads, 0, s>>>(a);

@@ -8,6 +8,7 @@ there. No counterpart in the reference.
 from __future__ import annotations
 
 import math
+import struct
 
 import torch
 
@@ -64,8 +65,24 @@ def _rows16(t):
     return t.contiguous() if not t.is_contiguous() or t.data_ptr() % 16 else t.clone()
 
 
-def _exponents(e):
-    return (0, 0) if e is None else (e.stride(0), e.stride(1))
+_CACHE = struct.Struct('7P18q')    # svhip_paged_cache
+_APPEND = struct.Struct('5P13qd')  # svhip_paged_append_args
+_ATTEND = struct.Struct('4P10qd')  # svhip_paged_attention_args
+
+
+def _address(t):
+    return 0 if t is None else t.data_ptr()
+
+
+def _packed(code, k_pages, v_pages, page_table, lengths, k_exponents, v_exponents, bad):
+    """The svhip_paged_cache of checked tensors."""
+    P, H, S, D = k_pages.shape
+    ke, ve = (0, 0), (0, 0)
+    if k_exponents is not None:
+        ke, ve = k_exponents.stride()[:2], v_exponents.stride()[:2]
+    return _CACHE.pack(k_pages.data_ptr(), v_pages.data_ptr(), _address(k_exponents), _address(v_exponents),
+                       page_table.data_ptr(), lengths.data_ptr(), _address(bad), code, page_table.shape[0], H, D, P, S,
+                       page_table.shape[1], page_table.stride(0), *k_pages.stride()[:3], *v_pages.stride()[:3], *ke, *ve)
 
 
 def paged_append(key, value, k_pages, v_pages, page_table, lengths, cu_tokens=None, before=0, positions=None,
@@ -82,10 +99,8 @@ def paged_append(key, value, k_pages, v_pages, page_table, lengths, cu_tokens=No
     or [T], or None: each key's index in its window; `amplitude`), with 'axial' as `producer.axial_rope` does (its fp32
     buffer and fp32 positions [B,n,3] or [T,3]). `bad` (optional int32 [1], device) becomes 1 when a key lies outside
     its window's row of the table or a page outside the pool; such keys are not written."""
-    _lib.require_gpu(key, value, k_pages, v_pages, page_table, lengths, cu_tokens, positions, frequencies, k_exponents,
-                     v_exponents, bad)
-    _lib.require_same_device(key, value, k_pages, v_pages, page_table, lengths, cu_tokens, positions, frequencies,
-                             k_exponents, v_exponents, bad)
+    _lib.require_one_gpu(key, value, k_pages, v_pages, page_table, lengths, cu_tokens, positions, frequencies, k_exponents,
+                         v_exponents, bad)
     code = _check_pool(k_pages, v_pages, page_table, lengths, k_exponents, v_exponents, bad)
     if key.dtype != torch.bfloat16 or value.dtype != torch.bfloat16:
         raise TypeError('key and value must be bfloat16')
@@ -124,13 +139,11 @@ def paged_append(key, value, k_pages, v_pages, page_table, lengths, cu_tokens=No
             sp = (0, positions.stride(0)) if cu_tokens is not None else (positions.stride(0), positions.stride(1))
     elif positions is not None:
         raise ValueError('rotating the keys needs frequencies')
+    args = _APPEND.pack(key.data_ptr(), value.data_ptr(), _address(cu_tokens), _address(positions), _address(frequencies),
+                        n, before, *sk, *sv, turn, wide, *sp, pairs, amplitude)
+    cache = _packed(code, k_pages, v_pages, page_table, lengths, k_exponents, v_exponents, bad)
     with _lib.device_of(key):
-        _lib.check(_lib.load().svhip_paged_append(
-            _lib.ptr(key), _lib.ptr(value), *sk, *sv, B, H, n, D, _lib.ptr(cu_tokens), before, _lib.ptr(k_pages),
-            _lib.ptr(v_pages), _lib.ptr(k_exponents), _lib.ptr(v_exponents), code, P, S, *k_pages.stride()[:3],
-            *v_pages.stride()[:3], *_exponents(k_exponents), *_exponents(v_exponents), _lib.ptr(page_table),
-            page_table.stride(0), page_table.shape[1], _lib.ptr(lengths), turn, _lib.ptr(positions), wide, *sp,
-            _lib.ptr(frequencies), pairs, float(amplitude), _lib.ptr(bad), _lib.stream_of(key)), 'svhip_paged_append')
+        _lib.check(_lib.load().svhip_paged_append(cache, args, _lib.stream_of(key)), 'svhip_paged_append')
 
 
 def paged_attention(query, k_pages, v_pages, page_table, lengths, cu_queries=None, causal=False, scale=None,
@@ -145,8 +158,7 @@ def paged_attention(query, k_pages, v_pages, page_table, lengths, cu_queries=Non
     left as they are (a fresh one has them undefined). `bad` (optional int32 [1], device) becomes 1 when a page lies
     outside the pool (its keys and values read as zeros) or a length passes the window's row of the table (and is cut).
     Returns out."""
-    _lib.require_gpu(query, k_pages, v_pages, page_table, lengths, cu_queries, k_exponents, v_exponents, out, bad)
-    _lib.require_same_device(query, k_pages, v_pages, page_table, lengths, cu_queries, k_exponents, v_exponents, out, bad)
+    _lib.require_one_gpu(query, k_pages, v_pages, page_table, lengths, cu_queries, k_exponents, v_exponents, out, bad)
     code = _check_pool(k_pages, v_pages, page_table, lengths, k_exponents, v_exponents, bad)
     if query.dtype != torch.bfloat16:
         raise TypeError('query must be bfloat16')
@@ -165,12 +177,10 @@ def paged_attention(query, k_pages, v_pages, page_table, lengths, cu_queries=Non
     lib = _lib.load()
     m = page_table.shape[1]
     nbytes = int(lib.svhip_paged_attention_workspace_bytes(B, H, Hkv, n, cu_queries is not None, D, m * S))
+    cache = _packed(code, k_pages, v_pages, page_table, lengths, k_exponents, v_exponents, bad)
     with _lib.device_of(query):
         ws = torch.empty(nbytes, dtype=torch.uint8, device=query.device) if nbytes else None
-        _lib.check(lib.svhip_paged_attention(
-            _lib.ptr(query), _lib.ptr(k_pages), _lib.ptr(v_pages), _lib.ptr(k_exponents), _lib.ptr(v_exponents),
-            _lib.ptr(out), code, B, H, Hkv, n, D, _lib.ptr(cu_queries), P, S, _lib.ptr(page_table), page_table.stride(0), m,
-            _lib.ptr(lengths), *sq, *k_pages.stride()[:3], *v_pages.stride()[:3], *_exponents(k_exponents),
-            *_exponents(v_exponents), *so, int(causal), scale, _lib.ptr(bad), _lib.ptr(ws), nbytes, _lib.stream_of(query)),
-            'svhip_paged_attention')
+        args = _ATTEND.pack(query.data_ptr(), out.data_ptr(), _address(cu_queries), _address(ws), nbytes, H, n, *sq, *so,
+                            causal, scale)
+        _lib.check(lib.svhip_paged_attention(cache, args, _lib.stream_of(query)), 'svhip_paged_attention')
     return out

@@ -7,6 +7,7 @@ reference's positions with the reference's bf16 roundings; no counterpart in the
 from __future__ import annotations
 
 import math
+import struct
 
 import torch
 
@@ -46,14 +47,16 @@ def rotary_frequencies(rotary_dim, base=10000.0, scaling=None, factor=1.0, origi
     return (freq if device is None else freq.to(device)), amplitude
 
 
+_ARGS = struct.Struct('4P17qd')   # svhip_rotary_args
+
+
 def _launch(x, out, positions, frequencies, layout, amplitude, inverse):
-    B, H, N, D = x.shape
+    args = _ARGS.pack(x.data_ptr(), out.data_ptr(), positions.data_ptr(), frequencies.data_ptr(),
+                      _lib.dtype_code(x.dtype), positions.dtype == torch.int64, frequencies.numel(), LAYOUTS[layout],
+                      inverse, *x.shape, *x.stride()[:3], *out.stride()[:3],
+                      positions.stride(0) if positions.dim() == 2 else 0, positions.stride(-1), amplitude)
     with _lib.device_of(x):
-        _lib.check(_lib.load().svhip_rotary(
-            _lib.ptr(x), _lib.ptr(out), _lib.dtype_code(x.dtype), _lib.ptr(positions), positions.dtype == torch.int64,
-            _lib.ptr(frequencies), frequencies.numel(), LAYOUTS[layout], amplitude, inverse, B, H, N, D, x.stride(0),
-            x.stride(1), x.stride(2), out.stride(0), out.stride(1), out.stride(2),
-            positions.stride(0) if positions.dim() == 2 else 0, positions.stride(-1), _lib.stream_of(x)), 'svhip_rotary')
+        _lib.check(_lib.load().svhip_rotary(args, _lib.stream_of(x)), 'svhip_rotary')
     return out
 
 
@@ -80,7 +83,7 @@ def rotary(x, positions, frequencies, layout='half', amplitude=1.0, out=None):
     128 pairs. The turns are formed in 64 bits (far positions keep their angle), the rest in fp32, rounded once to x's type.
     Differentiable in x. `out` (optional, no gradient through it; x itself, or memory that x does not share) receives the
     result; returns it."""
-    _lib.require_gpu(x, positions, frequencies, out)
+    _lib.require_one_gpu(x, positions, frequencies, out)
     if layout not in LAYOUTS:
         raise ValueError("layout is 'half' or 'interleaved'")
     if x.dtype not in (torch.bfloat16, torch.float32):
@@ -94,7 +97,6 @@ def rotary(x, positions, frequencies, layout='half', amplitude=1.0, out=None):
         raise ValueError('frequencies must be a contiguous fp64 vector')
     if not 1 <= frequencies.numel() <= min(D // 2, 128):
         raise ValueError(f'{frequencies.numel()} frequencies do not fit head_dim {D} (at most 128)')
-    _lib.require_same_device(x, positions, frequencies, out)
     if out is None:
         if torch.is_grad_enabled() and x.requires_grad:
             return _Rotary.apply(x, positions, frequencies, layout, float(amplitude))

@@ -1,6 +1,6 @@
 """CPU checks of the rotary positions and the paged cache: the frequencies, the refusals of the C ABI (no launch) and of the
 Python entry points."""
-import ctypes
+import struct
 import math
 
 import pytest
@@ -56,14 +56,15 @@ def test_host_tensors_are_refused():
         paged_attention(x, pages, pages, table, n)
 
 
-FAKE = ctypes.c_void_p(0x1000)      # never dereferenced: every call below fails its host checks, or launches nothing
+FAKE = 0x1000      # never dereferenced: every call below fails its host checks, or launches nothing
 
 
 def test_rotary_argument_errors(lib):
     def call(x=FAKE, dtype=1, freq=FAKE, pairs=4, layout=1, sizes=(1, 2, 3, 8)):
-        return lib.svhip_rotary(x, FAKE, dtype, FAKE, 0, freq, pairs, layout, 1.0, 0, *sizes, *[8] * 6, 0, 1, None)
-    assert call(x=None) == -1 and b'null' in lib.svhip_last_error()
-    assert call(freq=None) == -1 and b'null' in lib.svhip_last_error()
+        args = struct.pack('4P17qd', x, FAKE, FAKE, freq, dtype, 0, pairs, layout, 0, *sizes, *[8] * 6, 0, 1, 1.0)
+        return lib.svhip_rotary(args, None)
+    assert call(x=0) == -1 and b'null' in lib.svhip_last_error()
+    assert call(freq=0) == -1 and b'null' in lib.svhip_last_error()
     assert call(dtype=3) == -1 and b'dtype' in lib.svhip_last_error()
     for layout in (0, 3, 9):
         assert call(layout=layout) == -1 and b'layout' in lib.svhip_last_error()
@@ -72,66 +73,89 @@ def test_rotary_argument_errors(lib):
     assert call(sizes=(1, 2, -3, 8)) == -1 and b'sizes' in lib.svhip_last_error()
     for sizes in ((0, 2, 3, 8), (1, 0, 3, 8), (1, 2, 0, 8)):
         assert call(sizes=sizes) == 0
+    assert lib.svhip_rotary(None, None) == -1 and b'null' in lib.svhip_last_error()
 
 
-def append_call(lib, key=FAKE, sk=(768, 64, 128), B=2, H=2, N=3, D=64, cu=None, before=0, kp=FAKE, ke=None, dtype=1, pages=4,
-                page=64, srow=64, table=FAKE, m=2, lengths=FAKE, layout=0, positions=None, freq=None, pairs=0, amplitude=1.0):
-    return lib.svhip_paged_append(key, FAKE, *sk, 768, 64, 128, B, H, N, D, cu, before, kp, FAKE, ke, ke, dtype, pages, page,
-                                  8192, 4096, srow, 8192, 4096, srow, 128, 64, 128, 64, table, m, m, lengths, layout,
-                                  positions, 0, 6, 1, freq, pairs, amplitude, None, None)
+def cache_of(B=2, H=2, D=64, kp=FAKE, ke=0, dtype=1, pages=4, page=64, srow=64, table=FAKE, m=2, lengths=FAKE):
+    return struct.pack('7P18q', kp, FAKE, ke, ke, table, lengths, 0, dtype, B, H, D, pages, page, m, m, 8192, 4096, srow,
+                       8192, 4096, srow, 128, 64, 128, 64)
+
+
+def append_call(lib, key=FAKE, sk=(768, 64, 128), N=3, before=0, layout=0, positions=0, freq=0, pairs=0, **cache):
+    args = struct.pack('5P13qd', key, FAKE, 0, positions, freq, N, before, *sk, 768, 64, 128, layout, 0, 6, 1, pairs, 1.0)
+    return lib.svhip_paged_append(cache_of(**cache), args, None)
+
+
+def attend_call(lib, q=FAKE, H=4, N=3, sq=64, so=64, scale=0.125, ws=0, nbytes=0, **cache):
+    args = struct.pack('4P10qd', q, FAKE, 0, ws, nbytes, H, N, 768, 192, sq, 768, 192, so, 0, scale)
+    return lib.svhip_paged_attention(cache_of(**cache), args, None)
+
+
+@pytest.mark.parametrize('call', [append_call, attend_call])
+def test_cache_errors(lib, call):
+    error = lib.svhip_last_error
+    for D in (0, 60, 136):
+        assert call(lib, D=D) == -1 and b'head_dim' in error()
+    for page in (0, 8, 48, 2048):
+        assert call(lib, page=page) == -1 and b'page size' in error()
+    assert call(lib, dtype=0) == -1 and b'dtype' in error()
+    assert call(lib, B=-1) == -1 and b'sizes' in error()
+    for kw in (dict(pages=-1), dict(m=-1), dict(m=1 << 25), dict(pages=1 << 31)):
+        assert call(lib, **kw) == -1 and b'page counts' in error()
+    for name in ('kp', 'table', 'lengths'):
+        assert call(lib, **{name: 0}) == -1 and b'null' in error()
+    assert call(lib, dtype=3) == -1 and b'exponents' in error()
+    assert call(lib, srow=68) == -1 and b'16-byte' in error()
+    assert call(lib, dtype=3, ke=FAKE, srow=68) == -1 and b'8-byte' in error()
+    for srow in (-64, 1 << 26):
+        assert call(lib, srow=srow) == -1 and b'too far' in error()
+    for empty in (dict(B=0), dict(N=0)):
+        assert call(lib, **empty) == 0
 
 
 def test_append_argument_errors(lib):
     error = lib.svhip_last_error
-    for D in (0, 60, 136):
-        assert append_call(lib, D=D) == -1 and b'head_dim' in error()
-    for page in (0, 8, 48, 2048):
-        assert append_call(lib, page=page) == -1 and b'page size' in error()
-    assert append_call(lib, dtype=0) == -1 and b'dtype' in error()
     assert append_call(lib, before=-1) == -1 and b'sizes' in error()
-    assert append_call(lib, B=-1) == -1 and b'sizes' in error()
-    assert append_call(lib, pages=-1) == -1 and b'page counts' in error()
     assert append_call(lib, layout=4) == -1 and b'layout' in error()
     assert append_call(lib, layout=1, freq=FAKE, pairs=33) == -1 and b'pairs' in error()
     assert append_call(lib, layout=2, freq=FAKE, pairs=0) == -1 and b'pairs' in error()
     assert append_call(lib, layout=1, pairs=32) == -1 and b'frequencies' in error()
     assert append_call(lib, layout=3, freq=FAKE, positions=FAKE, pairs=32) == -1 and b'three-axis' in error()
     assert append_call(lib, layout=3, freq=FAKE, pairs=24, D=48) == -1 and b'positions' in error()
-    for name in ('key', 'kp', 'table', 'lengths'):
-        assert append_call(lib, **{name: None}) == -1 and b'null' in error()
-    assert append_call(lib, dtype=3) == -1 and b'exponents' in error()
+    assert append_call(lib, key=0) == -1 and b'null' in error()
     assert append_call(lib, sk=(768, 60, 128)) == -1 and b'16-byte' in error()
-    assert append_call(lib, srow=68) == -1 and b'16-byte' in error()
-    assert append_call(lib, dtype=3, ke=FAKE, srow=68) == -1 and b'8-byte' in error()
-    for empty in (dict(B=0), dict(H=0), dict(N=0)):
-        assert append_call(lib, **empty) == 0
-
-
-def attend_call(lib, q=FAKE, kp=FAKE, ke=None, dtype=1, B=2, H=4, Hkv=2, N=3, D=64, cu=None, pages=4, page=64, table=FAKE,
-                m=2, lengths=FAKE, sq=64, srow=64, so=64, scale=0.125, ws=None, nbytes=0):
-    return lib.svhip_paged_attention(q, kp, FAKE, ke, ke, FAKE, dtype, B, H, Hkv, N, D, cu, pages, page, table, m, m, lengths,
-                                     768, 192, sq, 8192, 4096, srow, 8192, 4096, srow, 128, 64, 128, 64, 768, 192, so, 0,
-                                     scale, None, ws, nbytes, None)
+    assert append_call(lib, H=0) == 0
+    assert lib.svhip_paged_append(None, None, None) == -1 and b'null' in error()
+    assert lib.svhip_paged_append(cache_of(), None, None) == -1 and b'null' in error()
 
 
 def test_attention_argument_errors(lib):
     error = lib.svhip_last_error
-    for D in (0, 60, 136):
-        assert attend_call(lib, D=D) == -1 and b'head_dim' in error()
-    for page in (0, 8, 48, 2048):
-        assert attend_call(lib, page=page) == -1 and b'page size' in error()
-    for Hkv in (0, 3):
-        assert attend_call(lib, Hkv=Hkv) == -1 and b'share' in error()
+    for heads in (0, 3):
+        assert _attend_heads(lib, heads) == -1 and b'share' in error()
     for scale in (0.0, -1.0, math.inf, math.nan):
         assert attend_call(lib, scale=scale) == -1 and b'scale' in error()
-    assert attend_call(lib, dtype=0) == -1 and b'dtype' in error()
     assert attend_call(lib, N=-1) == -1 and b'sizes' in error()
-    assert attend_call(lib, m=1 << 26) == -1 and b'page counts' in error()
-    for name in ('q', 'kp', 'table', 'lengths'):
-        assert attend_call(lib, **{name: None}) == -1 and b'null' in error()
-    assert attend_call(lib, dtype=3) == -1 and b'exponents' in error()
+    assert attend_call(lib, q=0) == -1 and b'null' in error()
     assert attend_call(lib, sq=68) == -1 and b'query rows' in error()
     assert attend_call(lib, so=66) == -1 and b'rows of out' in error()
-    assert attend_call(lib, srow=68) == -1 and b'16-byte' in error()
-    for empty in (dict(B=0), dict(H=0), dict(N=0)):
-        assert attend_call(lib, **empty) == 0
+    need = lib.svhip_paged_attention_workspace_bytes(2, 4, 2, 3, 0, 64, 128)
+    assert need > 0
+    for ws, nbytes in ((0, need), (FAKE, need - 1), (FAKE + 8, need)):
+        assert attend_call(lib, ws=ws, nbytes=nbytes) == -1 and b'workspace' in error()
+    assert lib.svhip_paged_attention(None, None, None) == -1 and b'null' in error()
+    assert lib.svhip_paged_attention(cache_of(), None, None) == -1 and b'null' in error()
+
+
+def _attend_heads(lib, heads):
+    args = struct.pack('4P10qd', FAKE, FAKE, 0, 0, 0, 4, 3, 768, 192, 64, 768, 192, 64, 0, 0.125)
+    return lib.svhip_paged_attention(cache_of(H=heads), args, None)
+
+
+def test_workspace_query():
+    """Bytes for what a call may launch; nothing for sizes that no call takes."""
+    need = _lib.load().svhip_paged_attention_workspace_bytes
+    assert need(0, 4, 2, 3, 0, 64, 128) == need(2, 4, 3, 3, 0, 64, 128) == need(2, 4, 2, 0, 0, 64, 128) == 0
+    assert need(8, 12, 12, 1024, 0, 64, 9744) == 0           # tiles that fill the chip
+    assert need(1, 12, 12, 1024, 0, 64, 9744) > 0
+    assert need(64, 16, 16, 1, 0, 64, 9744) > 0
