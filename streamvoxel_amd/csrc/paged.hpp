@@ -109,15 +109,15 @@ inline int check_cache(const char* name, const svhip_paged_cache* cache) {
 // The checks of a cache that a call touches.
 inline int check_pool(const char* name, const svhip_paged_cache& c) {
   const bool fp8 = c.kv_dtype == SVHIP_FP8_E4M3;
-  SVHIP_REQUIRE(c.lengths && (c.max_pages == 0 || c.page_table) && (c.pages == 0 || (c.k_pages && c.v_pages)),
-                "%s: null pointer", name);
-  SVHIP_REQUIRE(!fp8 || c.pages == 0 || (c.k_exponents && c.v_exponents), "%s: e4m3 pages need the rows' exponents", name);
+  SVHIP_REQUIRE(c.pages >= 1, "%s: a pool needs a page", name);
+  SVHIP_REQUIRE(c.lengths && (c.max_pages == 0 || c.page_table) && c.k_pages && c.v_pages, "%s: null pointer", name);
+  SVHIP_REQUIRE(!fp8 || (c.k_exponents && c.v_exponents), "%s: e4m3 pages need the rows' exponents", name);
   const uintptr_t bytes = fp8 ? 8 : 16;
   SVHIP_REQUIRE(reinterpret_cast<uintptr_t>(c.k_pages) % bytes == 0 && reinterpret_cast<uintptr_t>(c.v_pages) % bytes == 0 &&
                     (c.sk_p | c.sk_h | c.sk_r | c.sv_p | c.sv_h | c.sv_r) % 8 == 0,
                 "%s: rows of a page must start on %d-byte boundaries", name, (int)bytes);
   SVHIP_REQUIRE(c.sk_r >= 0 && c.sk_r < (1 << 26) && c.sv_r >= 0 && c.sv_r < (1 << 26), "%s: rows of a page too far apart",
-                name);
+                name);  // 16 rows within a descriptor's 32-bit offsets
   return SVHIP_OK;
 }
 

@@ -26,10 +26,10 @@ constexpr int kTileRows = 128;     // rows of a tile workgroup
 constexpr int kRowKeys = 32;       // keys of a row-form wave's block
 constexpr int kTileTarget = 512;   // workgroups that a launch of tiles is cut into at least where its keys allow
 constexpr int kRowTarget = 512;    // the same of the row form
-constexpr int kRowLeast = 256;     // least keys of a row-form part
+constexpr int kRowLeast = 256;     // keys that a row-form part has a multiple of
 constexpr int kTileLeast = 6;      // least key blocks of a tile part
 constexpr float kNoMax = -3.0e38f; // running maximum before any key: finite, so that a row that sees nothing stays finite
-constexpr uint32_t kOutside = 0x7ffffff0u;  // byte offset past every descriptor's bound
+[[maybe_unused]] constexpr uint32_t kOutside = 0x7ffffff0u;  // byte offset past every descriptor's bound
 
 struct PagedArgs {
   const uint16_t* q;
@@ -103,12 +103,13 @@ __device__ __forceinline__ int page_number(const PagedArgs& a, const int32_t* ro
 
 #if defined(__HIP_DEVICE_COMPILE__)
 
-// Descriptor of 16 keys' rows at key j in `page`: the first `valid` of them, D elements of ES bytes each.
+// Descriptor of the rows of 16 keys, row in_page of `page` the first, from a head's part of a pool: `valid` of them, D
+// elements of ES bytes each.
 template <int ES>
-__device__ __forceinline__ __amdgpu_buffer_rsrc_t rows_of(const void* pool, int64_t page, int64_t in_page, int64_t sp,
-                                                         int64_t head, int64_t sr, int valid, int D) {
-  const char* base = static_cast<const char*>(pool) + (page * sp + head + in_page * sr) * ES;
-  const uint32_t bytes = valid > 0 ? static_cast<uint32_t>(((valid - 1) * sr + D) * ES) : 0u;
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t rows_of(const char* head, int page, int in_page, int64_t sp, int64_t sr,
+                                                         int valid, int D) {
+  const char* base = head + (page * sp + in_page * sr) * ES;
+  const uint32_t bytes = valid > 0 ? static_cast<uint32_t>(((valid - 1) * static_cast<int>(sr) + D) * ES) : 0u;
   return __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(base), 0, bytes, kRsrcFlags);
 }
 
@@ -124,54 +125,62 @@ __device__ __forceinline__ int valid_keys(const PagedArgs& a, int keys, int j, i
   return valid;
 }
 
+// Head widths: KS steps of 16 head_dim elements in the score product, and output tiles of 32.
+constexpr int tiles_of(int KS) { return (KS + 1) / 2; }
+
 // A wave's 32 rows: the queries as B operands, O^T, running maximum (log2 units) and sum.
-template <int DT>
+template <int KS>
 struct Rows {
-  bf16x8_t qf[2 * DT];
-  f32x16_t o[DT];
+  bf16x8_t qf[KS];
+  f32x16_t o[tiles_of(KS)];
   f32x4_t l;   // four equal entries: the lane's share of its row's sum
   float m;
   int last;    // last key that the lane's row sees
 };
 
-template <int DT>
+template <int KS>
 __device__ __forceinline__ void load_rows(const PagedArgs& a, const Window& w, int64_t b, int64_t kvh, int64_t r,
-                                          Rows<DT>& s) {
+                                          Rows<KS>& s) {
   const int hh = (threadIdx.x & 63) >> 5;
   const int64_t i = r / a.G, g = r - i * a.G;
   const bool ok = i < w.count;
   const uint16_t* q = a.q + (a.tokens.cu ? 0 : b * a.sq_b) + (kvh * a.G + g) * a.sq_h +
                       (a.tokens.cu ? w.first + i : i) * a.sq_n;
 #pragma unroll
-  for (int k = 0; k < 2 * DT; ++k) {
+  for (int k = 0; k < KS; ++k) {
     const int d0 = 16 * k + 8 * hh;
     uint4 raw = make_uint4(0u, 0u, 0u, 0u);
     if (ok && d0 < a.D) raw = *reinterpret_cast<const uint4*>(q + d0);
     s.qf[k] = __builtin_bit_cast(bf16x8_t, raw);
   }
 #pragma unroll
-  for (int j = 0; j < DT; ++j) s.o[j] = f32x16_t{0};
+  for (int j = 0; j < tiles_of(KS); ++j) s.o[j] = f32x16_t{0};
   s.l = f32x4_t{0.f, 0.f, 0.f, 0.f};
   s.m = kNoMax;
   s.last = ok ? last_key(a, w, i) : -1;
 }
 
-// 32 keys, `key0` the first, staged at row 0 of kp (K rows under sigma_row) and vp (V rows): sub-tiles of 64 head_dim elements
-// kSubBytes apart. The running maximum moves only for a score more than kMaxHigh above it (P then stays below 2^20, which
-// fp32 sums and bf16 weights hold alike); the row's sum is taken over the bf16 weights that the second product reads, by
-// v_mfma_f32_4x4x4_16b_bf16 with ones in A, whose columns are single lanes: no row's NaN reaches another's sum.
-template <int DT, int kSubBytes>
-__device__ __forceinline__ void attend_half(Rows<DT>& s, const char* kp, const char* vp, const uint32_t (&rd)[4],
-                                            const uint32_t (&rvt)[DT], int ksteps, float sl2, bool masked, int key0) {
-  const int hh = (threadIdx.x & 63) >> 5;
+// S^T of 32 keys: ka the K rows as A operands, row R of the tile key sigma_row(R).
+template <int KS>
+__device__ __forceinline__ f32x16_t scores(const Rows<KS>& s, const bf16x8_t (&ka)[KS]) {
   f32x16_t x;
 #pragma unroll
-  for (int k = 0; k < 2 * DT; ++k) {
-    if (k == 0 || k < ksteps) {
-      const bf16x8_t ka = *reinterpret_cast<const bf16x8_t*>(kp + (k >> 2) * kSubBytes + rd[k & 3]);
-      x = __builtin_amdgcn_mfma_f32_32x32x16_bf16(ka, s.qf[k], k == 0 ? f32x16_t{0} : x, 0, 0, 0);
-    }
+  for (int k = 0; k < KS; ++k) {
+    x = __builtin_amdgcn_mfma_f32_32x32x16_bf16(ka[k], s.qf[k], k == 0 ? f32x16_t{0} : x, 0, 0, 0);
   }
+  return x;
+}
+
+// The rest of 32 keys, `key0` the first, from their scores x: weights, sum, and O^T += V^T P^T with V rows staged at row 0 of
+// vp (sub-tiles of 64 head_dim elements kSubBytes apart). The running maximum moves only for a score more than kMaxHigh
+// above it (P then stays below 2^20, which fp32 sums and bf16 weights hold alike); the row's sum is taken over the bf16
+// weights that the second product reads, by v_mfma_f32_4x4x4_16b_bf16 with ones in A, whose columns are single lanes: no
+// row's NaN reaches another's sum.
+template <int KS, int kSubBytes>
+__device__ __forceinline__ void attend_half(Rows<KS>& s, f32x16_t x, const char* vp,
+                                            const uint32_t (&rvt)[tiles_of(KS)], float sl2, bool masked, int key0) {
+  constexpr int DT = tiles_of(KS);
+  const int hh = (threadIdx.x & 63) >> 5;
   if (masked) {
     const int seen = s.last - key0 - 8 * hh;
 #pragma unroll
@@ -234,12 +243,10 @@ __device__ __forceinline__ void attend_half(Rows<DT>& s, const char* kp, const c
   }
 }
 
-// Byte offsets of the operand reads: K rows (rd) and V rows read transposed (rvt, of output tile j inside its sub-tile).
+// Byte offsets of the reads of V rows, transposed: output tile j inside its sub-tile (xattn_kernel.hpp).
 template <int DT>
-__device__ __forceinline__ void read_offsets(uint32_t (&rd)[4], uint32_t (&rvt)[DT]) {
-  const int lane = threadIdx.x & 63, col = lane & 31, hh = lane >> 5;
-#pragma unroll
-  for (int k = 0; k < 4; ++k) rd[k] = static_cast<uint32_t>(col * kRow * 2 + swz(col, 2 * k + hh) * 16);
+__device__ __forceinline__ void v_offsets(uint32_t (&rvt)[DT]) {
+  const int lane = threadIdx.x & 63, hh = lane >> 5;
   const int row = 8 * hh + ((lane & 15) >> 2), flip = (row >> 1) & 1;
   const int c = 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1);
 #pragma unroll
@@ -254,66 +261,76 @@ __device__ __forceinline__ float row_sum(float l) {
   return __int_as_float(sw[0]) + __int_as_float(sw[1]);
 }
 
-// A wave's staging of `kLoads` groups of 8 rows, load i of sub-tile u into rows 8 * group(i) of it.
-template <bool FP8, int DT, int kLoads>
+// e4m3 rows on their way to LDS: a wave's kLoads loads of 8 rows, and the rows' exponents.
+template <int DT, int kLoads>
 struct Staged {
-  uint2 k[FP8 ? kLoads * Width<DT>::kSubTiles : 1], v[FP8 ? kLoads * Width<DT>::kSubTiles : 1];
-  uint32_t ek[FP8 ? kLoads : 1], ev[FP8 ? kLoads : 1];
+  uint2 w[kLoads * Width<DT>::kSubTiles];
+  uint32_t e[kLoads];
 };
 
-// Per-lane offsets: row lane / 8 of a load and its chunk; K under sigma_row and swz, V under swzv. A load's rows are 8 rows of
-// 16, `odd` the second 8.
-struct Lanes {
-  uint32_t k[2], v[2];   // byte offsets from the 16 keys' first row, loads of the first and the second 8 rows
-  int ck[2], cv[2];      // logical chunks
-  uint32_t rk[2];        // e4m3: the key's place among the 16
+// A lane's place in a load of 8 rows, the first or the second (odd) 8 of 16 keys: row lane / 8 and its chunk, K under
+// sigma_row and swz, V under swzv.
+struct Lane8 {
+  uint32_t at[2];   // byte offset from the 16 keys' first row in each sub-tile, or kOutside past head_dim
+  uint32_t key;     // the key's place among the 16
 };
 
 template <int ES>
-__device__ __forceinline__ Lanes staging_lanes(const PagedArgs& a) {
-  Lanes n;
-  const int lane = threadIdx.x & 63;
+__device__ __forceinline__ Lane8 lane_of_load(int64_t sr, int64_t D, int key, int chunk) {
+  Lane8 n;
+  n.key = static_cast<uint32_t>(key);
 #pragma unroll
-  for (int odd = 0; odd < 2; ++odd) {
-    const int R = 8 * odd + (lane >> 3), key = sigma_row(R);
-    n.ck[odd] = swz(R, lane & 7);
-    n.cv[odd] = swzv(R, lane & 7);
-    n.rk[odd] = static_cast<uint32_t>(key);
-    n.k[odd] = static_cast<uint32_t>((key * a.sk_r + 8 * n.ck[odd]) * ES);
-    n.v[odd] = static_cast<uint32_t>((R * a.sv_r + 8 * n.cv[odd]) * ES);
+  for (int u = 0; u < 2; ++u) {
+    const int d = 64 * u + 8 * chunk;
+    n.at[u] = d < D ? static_cast<uint32_t>((key * sr + d) * ES) : kOutside;
   }
   return n;
 }
+template <int ES>
+__device__ __forceinline__ Lane8 k_lane(const PagedArgs& a, int odd) {
+  const int lane = threadIdx.x & 63, R = 8 * odd + (lane >> 3);
+  return lane_of_load<ES>(a.sk_r, a.D, sigma_row(R), swz(R, lane & 7));
+}
+template <int ES>
+__device__ __forceinline__ Lane8 v_lane(const PagedArgs& a, int odd) {
+  const int lane = threadIdx.x & 63, R = 8 * odd + (lane >> 3);
+  return lane_of_load<ES>(a.sv_r, a.D, R, swzv(R, lane & 7));
+}
 
-// Issues the loads of 8 rows (odd: the second 8 of the 16 keys at key j) of K and V: bf16 straight into LDS at row `row` of the
-// sub-tiles at sK and sV, e4m3 into registers at index i.
+// One key head's part of a pool (of keys or of values).
+struct Source {
+  const char* rows;
+  const uint8_t* exponents;
+  int64_t sp, sr, se;  // elements from page to page and row to row, exponents from page to page
+};
+template <int ES>
+__device__ __forceinline__ Source k_source(const PagedArgs& a, int64_t kvh) {
+  return Source{static_cast<const char*>(a.k) + kvh * a.sk_h * ES, ES == 1 ? a.ek + kvh * a.sek_h : nullptr, a.sk_p,
+                a.sk_r, a.sek_p};
+}
+template <int ES>
+__device__ __forceinline__ Source v_source(const PagedArgs& a, int64_t kvh) {
+  return Source{static_cast<const char*>(a.v) + kvh * a.sv_h * ES, ES == 1 ? a.ev + kvh * a.sev_h : nullptr, a.sv_p,
+                a.sv_r, a.sev_p};
+}
+
+// Issues the loads of 8 of the 16 keys at row in_page of `page`, `valid` of which exist: bf16 straight into LDS at `to` (row 0
+// of the 8 in sub-tile 0), e4m3 into registers at index i.
 template <bool FP8, int DT, int kSubBytes, int kLoads>
-__device__ __forceinline__ void stage_rows8(const PagedArgs& a, const Lanes& n, int page, int j, int keys, int64_t hk,
-                                            int64_t hv, int64_t hek, int64_t hev, int odd, int row, int i, char* sK,
-                                            char* sV, Staged<FP8, DT, kLoads>& st) {
-  constexpr int ES = FP8 ? 1 : 2;
-  const int valid = valid_keys(a, keys, j, page);
-  const int64_t in_page = j & ((1 << a.pages.shift) - 1);
-  const int D = static_cast<int>(a.D);
-  const auto kr = rows_of<ES>(a.k, page, in_page, a.sk_p, hk, a.sk_r, valid, D);
-  const auto vr = rows_of<ES>(a.v, page, in_page, a.sv_p, hv, a.sv_r, valid, D);
+__device__ __forceinline__ void stage_rows8(const Source& src, const Lane8& n, int page, int in_page, int valid, int D,
+                                            int i, char* to, Staged<DT, kLoads>& st) {
+  const auto r = rows_of<FP8 ? 1 : 2>(src.rows, page, in_page, src.sp, src.sr, valid, D);
 #pragma unroll
   for (int u = 0; u < Width<DT>::kSubTiles; ++u) {
-    const uint32_t ko = 64 * u + 8 * n.ck[odd] < D ? n.k[odd] + 64 * ES * u : kOutside;
-    const uint32_t vo = 64 * u + 8 * n.cv[odd] < D ? n.v[odd] + 64 * ES * u : kOutside;
     if constexpr (FP8) {
-      st.k[i * Width<DT>::kSubTiles + u] = __builtin_bit_cast(uint2, __builtin_amdgcn_raw_buffer_load_b64(kr, ko, 0, 0));
-      st.v[i * Width<DT>::kSubTiles + u] = __builtin_bit_cast(uint2, __builtin_amdgcn_raw_buffer_load_b64(vr, vo, 0, 0));
+      st.w[i * Width<DT>::kSubTiles + u] = __builtin_bit_cast(uint2, __builtin_amdgcn_raw_buffer_load_b64(r, n.at[u], 0, 0));
     } else {
-      __builtin_amdgcn_raw_ptr_buffer_load_lds(kr, (lds_ptr_t)(sK + u * kSubBytes + row * kRow * 2), 16, ko, 0, 0, 0);
-      __builtin_amdgcn_raw_ptr_buffer_load_lds(vr, (lds_ptr_t)(sV + u * kSubBytes + row * kRow * 2), 16, vo, 0, 0, 0);
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (lds_ptr_t)(to + u * kSubBytes), 16, n.at[u], 0, 0, 0);
     }
   }
   if constexpr (FP8) {
-    const auto er = rows_of<1>(a.ek, page, in_page, a.sek_p, hek, 1, valid, 1);
-    const auto fr = rows_of<1>(a.ev, page, in_page, a.sev_p, hev, 1, valid, 1);
-    st.ek[i] = __builtin_amdgcn_raw_buffer_load_b8(er, n.rk[odd], 0, 0);
-    st.ev[i] = __builtin_amdgcn_raw_buffer_load_b8(fr, 8 * odd + ((threadIdx.x & 63) >> 3), 0, 0);
+    const auto er = rows_of<1>(reinterpret_cast<const char*>(src.exponents), page, in_page, src.se, 1, valid, 1);
+    st.e[i] = __builtin_amdgcn_raw_buffer_load_b8(er, n.key, 0, 0);
   }
 }
 
@@ -328,14 +345,13 @@ __device__ __forceinline__ uint4 decode8(uint2 w, uint32_t exponent) {
                     __builtin_bit_cast(uint32_t, d));
 }
 
-// e4m3: load i of `st` into its 8 rows at `row`.
+// e4m3: load i of `st` into its 8 rows at `to`.
 template <int DT, int kSubBytes, int kLoads>
-__device__ __forceinline__ void commit_rows8(const Staged<true, DT, kLoads>& st, int row, int i, char* sK, char* sV) {
-  const uint32_t at = row * kRow * 2 + 16 * (threadIdx.x & 63);
+__device__ __forceinline__ void commit_rows8(const Staged<DT, kLoads>& st, int i, char* to) {
 #pragma unroll
   for (int u = 0; u < Width<DT>::kSubTiles; ++u) {
-    *reinterpret_cast<uint4*>(sK + u * kSubBytes + at) = decode8(st.k[i * Width<DT>::kSubTiles + u], st.ek[i]);
-    *reinterpret_cast<uint4*>(sV + u * kSubBytes + at) = decode8(st.v[i * Width<DT>::kSubTiles + u], st.ev[i]);
+    *reinterpret_cast<uint4*>(to + u * kSubBytes + 16 * (threadIdx.x & 63)) =
+        decode8(st.w[i * Width<DT>::kSubTiles + u], st.e[i]);
   }
 }
 
@@ -343,9 +359,10 @@ __device__ __forceinline__ void commit_rows8(const Staged<true, DT, kLoads>& st,
 
 // ------------------------------------------------------------------------------------------------------- tile form
 
-template <bool FP8, int DT>
+template <bool FP8, int KS>
 __global__ __launch_bounds__(kPagedThreads, 2) void paged_tile_kernel(PagedArgs a) {
 #if defined(__HIP_DEVICE_COMPILE__)
+  constexpr int DT = tiles_of(KS);
   constexpr int kSubBytes = kKB * kRow * 2, kTileBytes = Width<DT>::kSubTiles * kSubBytes;
   __shared__ __attribute__((aligned(16))) char sK0[kTileBytes], sK1[kTileBytes], sV0[kTileBytes], sV1[kTileBytes];
   // Workgroup -> (tile, key head, part): XCD id % 8 takes every 8th unit (window, key head, part) with all its tiles, so that
@@ -402,13 +419,15 @@ __global__ __launch_bounds__(kPagedThreads, 2) void paged_tile_kernel(PagedArgs 
   if (a.plan && part == 0 && kvh == 0 && qt == 0 && threadIdx.x == 0) a.plan[b] = make_int4(static_cast<int>(tile), 0, 1, 0);
   const int blk0 = part * each, blk1 = blk0 + each < blocks ? blk0 + each : blocks;
 
-  Rows<DT> s;
-  load_rows<DT>(a, w, b, kvh, r, s);
+  Rows<KS> s;
+  load_rows<KS>(a, w, b, kvh, r, s);
+  // K rows: lane (col, hh) takes logical chunk 2 k + hh of rows col and 32 + col, which share their swizzle.
   uint32_t rd[4], rvt[DT];
-  read_offsets<DT>(rd, rvt);
-  const Lanes lanes = staging_lanes<FP8 ? 1 : 2>(a);
-  const int ksteps = __builtin_amdgcn_readfirstlane(static_cast<int>((a.D + 15) / 16));
-  const int64_t hk = kvh * a.sk_h, hv = kvh * a.sv_h, hek = kvh * a.sek_h, hev = kvh * a.sev_h;
+#pragma unroll
+  for (int k = 0; k < 4; ++k) rd[k] = static_cast<uint32_t>(col * kRow * 2 + swz(col, 2 * k + hh) * 16);
+  v_offsets<DT>(rvt);
+  constexpr int ES = FP8 ? 1 : 2;
+  const Source ks = k_source<ES>(a, kvh), vs = v_source<ES>(a, kvh);
   const int32_t* row = a.pages.table + b * a.pages.st_b;
   // The wave's rows see every key up to `all` and none past `any`.
   const int64_t wr0 = r0 + wave * kRows, wr1 = wr0 + kRows < rows ? wr0 + kRows : rows;
@@ -416,16 +435,26 @@ __global__ __launch_bounds__(kPagedThreads, 2) void paged_tile_kernel(PagedArgs 
   const int any = __builtin_amdgcn_readfirstlane(wr0 < rows ? last_key(a, w, (wr1 - 1) / a.G) : -1);
 
   // The wave stages rows 8 wave .. and 8 (wave + 4) .. of a block: 16 keys at 16 (wave / 2) and at 32 + 16 (wave / 2).
-  Staged<FP8, DT, 2> st;
-  const int g0 = 16 * (wave >> 1), odd = wave & 1;
+  Staged<DT, FP8 ? 2 : 1> kst, vst;
+  const int g0 = 16 * (wave >> 1), in_mask = (1 << a.pages.shift) - 1, D = static_cast<int>(a.D);
+  const Lane8 kl = k_lane<ES>(a, wave & 1), vl = v_lane<ES>(a, wave & 1);
   auto issue = [&](int kv0, int p0, int p1, char* sK, char* sV) __attribute__((always_inline)) {
-    stage_rows8<FP8, DT, kSubBytes>(a, lanes, p0, kv0 + g0, keys, hk, hv, hek, hev, odd, 8 * wave, 0, sK, sV, st);
-    stage_rows8<FP8, DT, kSubBytes>(a, lanes, p1, kv0 + 32 + g0, keys, hk, hv, hek, hev, odd, 8 * wave + 32, 1, sK, sV, st);
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const int j = kv0 + 32 * i + g0, to = (8 * wave + 32 * i) * kRow * 2;
+      int page = i ? p1 : p0;
+      const int valid = valid_keys(a, keys, j, page);
+      stage_rows8<FP8, DT, kSubBytes>(ks, kl, page, j & in_mask, valid, D, i, sK + to, kst);
+      stage_rows8<FP8, DT, kSubBytes>(vs, vl, page, j & in_mask, valid, D, i, sV + to, vst);
+    }
   };
   auto commit = [&](char* sK, char* sV) __attribute__((always_inline)) {
     if constexpr (FP8) {
-      commit_rows8<DT, kSubBytes>(st, 8 * wave, 0, sK, sV);
-      commit_rows8<DT, kSubBytes>(st, 8 * wave + 32, 1, sK, sV);
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        commit_rows8<DT, kSubBytes>(kst, i, sK + (8 * wave + 32 * i) * kRow * 2);
+        commit_rows8<DT, kSubBytes>(vst, i, sV + (8 * wave + 32 * i) * kRow * 2);
+      }
     }
   };
   auto compute = [&](int kv0, const char* sK, const char* sV) __attribute__((always_inline)) {
@@ -433,8 +462,12 @@ __global__ __launch_bounds__(kPagedThreads, 2) void paged_tile_kernel(PagedArgs 
     for (int t = 0; t < 2; ++t) {
       const int key0 = kv0 + 32 * t;
       if (key0 > any) break;
-      attend_half<DT, kSubBytes>(s, sK + 32 * t * kRow * 2, sV + 32 * t * kRow * 2, rd, rvt, ksteps, a.scale_log2,
-                                 key0 + 31 > all, key0);
+      bf16x8_t ka[KS];
+#pragma unroll
+      for (int k = 0; k < KS; ++k) {
+        ka[k] = *reinterpret_cast<const bf16x8_t*>(sK + (k >> 2) * kSubBytes + rd[k & 3] + 32 * t * kRow * 2);
+      }
+      attend_half<KS, kSubBytes>(s, scores<KS>(s, ka), sV + 32 * t * kRow * 2, rvt, a.scale_log2, key0 + 31 > all, key0);
     }
   };
   if (blk0 < blk1) {
@@ -500,8 +533,8 @@ __global__ __launch_bounds__(kPagedThreads, 2) void paged_tile_kernel(PagedArgs 
 
 // -------------------------------------------------------------------------------------------------------- row form
 
-// The windows' parts, a workgroup's worth each: an equal share of all keys for kRowTarget workgroups, at least kRowLeast, a
-// multiple of 4 waves' blocks. The lengths are on the device, so every workgroup forms the plan for itself.
+// The windows' parts, a workgroup's worth each: an equal share of all keys for kRowTarget workgroups, a multiple of kRowLeast
+// (4 waves' blocks). The lengths are on the device, so every workgroup forms the plan for itself.
 __device__ __forceinline__ int row_part_keys(const PagedArgs& a) {
   int64_t sum = 0;
   for (int64_t c = threadIdx.x & 63; c < a.tokens.B; c += 64) {
@@ -510,16 +543,23 @@ __device__ __forceinline__ int row_part_keys(const PagedArgs& a) {
     if (count > 0 && row_form(a, count)) sum += held_keys(a.pages, c);
   }
   const int64_t share = cdiv(wave_sum(sum) * a.Hkv, kRowTarget);
-  const int64_t each = cdiv(share, 4 * kRowKeys) * (4 * kRowKeys);
-  return static_cast<int>(each < kRowLeast ? kRowLeast : each);
+  const int64_t each = cdiv(share, kRowLeast) * kRowLeast;
+  return static_cast<int>(each < kRowLeast ? kRowLeast : (each < (1 << 30) ? each : (1 << 30)));
 }
 
-template <bool FP8, int DT>
+// A wave takes every 4th block of 32 keys of its part (e4m3: 64). K rows go straight from memory to the A operands, a lane its
+// own key's chunks, the next block's while the current one's softmax and second product run; V rows go through the wave's LDS,
+// since they are read transposed.
+template <bool FP8, int KS>
 __global__ __launch_bounds__(kPagedThreads, 2) void paged_row_kernel(PagedArgs a) {
 #if defined(__HIP_DEVICE_COMPILE__)
-  constexpr int kSubBytes = kRowKeys * kRow * 2, kTileBytes = Width<DT>::kSubTiles * kSubBytes;
-  __shared__ __attribute__((aligned(16))) char sK0[4 * kTileBytes], sK1[4 * kTileBytes], sV0[4 * kTileBytes],
-      sV1[4 * kTileBytes];
+  constexpr int DT = tiles_of(KS), ES = FP8 ? 1 : 2;
+  constexpr int kHalves = FP8 ? 2 : 1, kKeys = kRowKeys * kHalves;  // of a wave's block
+  constexpr int kSubBytes = kKeys * kRow * 2, kTileBytes = Width<DT>::kSubTiles * kSubBytes;
+  // V of the four waves, bf16 two blocks of each; O of them at the end, 32 DT x 32 floats each.
+  constexpr int kWaveO = 32 * DT * kRows, kFirst = FP8 ? 4 : 2;  // waves whose O goes to sV0
+  constexpr int kBuffer = 4 * kTileBytes > kFirst * kWaveO * 4 ? 4 * kTileBytes : kFirst * kWaveO * 4;
+  __shared__ __attribute__((aligned(16))) char sV0[kBuffer], sV1[FP8 ? 16 : kBuffer];
   __shared__ float s_ml[4][2][kRows];
   const int lane = threadIdx.x & 63, col = lane & 31, hh = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -563,62 +603,140 @@ __global__ __launch_bounds__(kPagedThreads, 2) void paged_row_kernel(PagedArgs a
   const int keys = __builtin_amdgcn_readfirstlane(w.keys);
   const int k0 = part * each, k1 = k0 + each < keys ? k0 + each : keys;
 
-  Rows<DT> s;
-  load_rows<DT>(a, w, b, kvh, col, s);
-  uint32_t rd[4], rvt[DT];
-  read_offsets<DT>(rd, rvt);
-  const Lanes lanes = staging_lanes<FP8 ? 1 : 2>(a);
-  const int ksteps = __builtin_amdgcn_readfirstlane(static_cast<int>((a.D + 15) / 16));
-  const int64_t hk = kvh * a.sk_h, hv = kvh * a.sv_h, hek = kvh * a.sek_h, hev = kvh * a.sev_h;
+  Rows<KS> s;
+  load_rows<KS>(a, w, b, kvh, col, s);
+  uint32_t rvt[DT];
+  v_offsets<DT>(rvt);
+  const Source ks = k_source<ES>(a, kvh), vs = v_source<ES>(a, kvh);
+  const Lane8 vl[2] = {v_lane<ES>(a, 0), v_lane<ES>(a, 1)};
   const int32_t* row = a.pages.table + b * a.pages.st_b;
   const int all = __builtin_amdgcn_readfirstlane(last_key(a, w, 0));
-  char *cK0 = sK0 + wave * kTileBytes, *cV0 = sV0 + wave * kTileBytes;
-  char *cK1 = sK1 + wave * kTileBytes, *cV1 = sV1 + wave * kTileBytes;
-  Staged<FP8, DT, 4> st;
-  auto issue = [&](int kv0, int p0, int p1, char* sK, char* sV) __attribute__((always_inline)) {
+  const int in_mask = (1 << a.pages.shift) - 1, D = static_cast<int>(a.D);
+  // The lane's key among 16, and its offsets in a K row (the last step's chunk may lie past head_dim, where Q is zero: any
+  // chunk of the row then).
+  const int own = sigma_row(col) & 15;
+  const int64_t k_own = (own * ks.sr + 8 * hh) * ES;
+  const int k_last = 16 * (KS - 1) + 8 * hh < D ? 16 * (KS - 1) * ES : -8 * hh * ES;
+
+  using KWord = typename std::conditional<FP8, uint2, uint4>::type;
+  KWord kw[kHalves][KS];
+  uint32_t ke[FP8 ? kHalves : 1];
+  Staged<DT, FP8 ? 4 * kHalves : 1> vst;
+  int page[2 * kHalves], valid[2 * kHalves];   // of the 16-key groups of the block to load
+  bool broken = false;                         // the block in kw has keys on a bad page
+  auto find = [&](int kv) __attribute__((always_inline)) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      stage_rows8<FP8, DT, kSubBytes>(a, lanes, i < 2 ? p0 : p1, kv0 + 16 * (i >> 1), k1, hk, hv, hek, hev, i & 1, 8 * i, i,
-                                      sK, sV, st);
+    for (int g = 0; g < 2 * kHalves; ++g) page[g] = page_number(a, row, kv + 16 * g);
+  };
+  auto check = [&](int kv) __attribute__((always_inline)) {
+#pragma unroll
+    for (int g = 0; g < 2 * kHalves; ++g) valid[g] = valid_keys(a, k1, kv + 16 * g, page[g]);
+  };
+  auto load_v = [&](int kv, char* to) __attribute__((always_inline)) {
+#pragma unroll
+    for (int i = 0; i < 4 * kHalves; ++i) {
+      stage_rows8<FP8, DT, kSubBytes>(vs, vl[i & 1], page[i >> 1], (kv + 8 * i) & in_mask & ~15, valid[i >> 1], D, i,
+                                      to + 8 * i * kRow * 2, vst);
     }
   };
-  auto commit = [&](char* sK, char* sV) __attribute__((always_inline)) {
-    if constexpr (FP8) {
+  // Keys that do not exist are never loaded (the block's first one is read instead, or page 0 where its page is bad; pools
+  // have a page wherever a window has keys): their scores are masked, but for bad pages, which count as zeros.
+  auto load_k = [&](int kv) __attribute__((always_inline)) {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) commit_rows8<DT, kSubBytes>(st, 8 * i, i, sK, sV);
-    }
-  };
-  const int stride = 4 * kRowKeys;
-  int kv = k0 + wave * kRowKeys;
-  if (kv < k1) {
-    int p0 = page_number(a, row, kv), p1 = page_number(a, row, kv + 16);
-    issue(kv, p0, p1, cK0, cV0);
-    p0 = page_number(a, row, kv + stride);
-    p1 = page_number(a, row, kv + stride + 16);
-    commit(cK0, cV0);
-    wait_vmem();
-    auto step = [&](char* xK, char* xV, char* nK, char* nV) __attribute__((always_inline)) {
-      const bool more = kv + stride < k1;
-      if (more) issue(kv + stride, p0, p1, nK, nV);
-      p0 = page_number(a, row, kv + 2 * stride);
-      p1 = page_number(a, row, kv + 2 * stride + 16);
-      attend_half<DT, kSubBytes>(s, xK, xV, rd, rvt, ksteps, a.scale_log2, kv + 31 > all, kv);
-      if (more) {
-        commit(nK, nV);
-        wait_vmem();
+    for (int t = 0; t < kHalves; ++t) {
+      const bool second = col >= 16;
+      const int g0 = 2 * t, in0 = (kv + 32 * t) & in_mask, in1 = (kv + 32 * t + 16) & in_mask;
+      const char* b0 = ks.rows + (page[g0] * ks.sp + in0 * ks.sr) * ES;
+      const char* b1 = ks.rows + (page[g0 + 1] * ks.sp + in1 * ks.sr) * ES;
+      const uint8_t *e0 = ks.exponents + page[g0] * ks.se + in0, *e1 = ks.exponents + page[g0 + 1] * ks.se + in1;
+      const bool here = own < (second ? valid[g0 + 1] : valid[g0]);
+      const char* first = valid[0] > 0 ? ks.rows + (page[0] * ks.sp + (kv & in_mask) * ks.sr) * ES : ks.rows;
+      const char* at = here ? (second ? b1 : b0) + k_own : first + 8 * hh * ES;
+#pragma unroll
+      for (int k = 0; k < KS; ++k) {
+        kw[t][k] = *reinterpret_cast<const KWord*>(at + (k < KS - 1 ? 16 * k * ES : k_last));
       }
-      kv += stride;
+      if constexpr (FP8) ke[t] = *(here ? (second ? e1 : e0) + own : ks.exponents);
+    }
+    broken = false;
+#pragma unroll
+    for (int g = 0; g < 2 * kHalves; ++g) broken |= valid[g] == 0 && kv + 16 * g < k1;
+  };
+  const int stride = 4 * kKeys;
+  int kv = k0 + wave * kKeys;
+  char *c0 = sV0 + wave * kTileBytes, *c1 = FP8 ? c0 : sV1 + wave * kTileBytes;
+  if (kv < k1) {
+    find(kv);
+    check(kv);
+    load_v(kv, c0);
+    load_k(kv);
+    int kvn = kv + stride;
+    find(kvn);
+    auto step = [&](char* cur, char* next) __attribute__((always_inline)) {
+      const bool more = kvn < k1;
+      if constexpr (FP8) {
+#pragma unroll
+        for (int i = 0; i < 4 * kHalves; ++i) commit_rows8<DT, kSubBytes>(vst, i, cur + 8 * i * kRow * 2);
+      }
+      if (more) {
+        check(kvn);
+        load_v(kvn, next);
+      }
+      f32x16_t x[kHalves];
+#pragma unroll
+      for (int t = 0; t < kHalves; ++t) {
+        bf16x8_t ka[KS];
+#pragma unroll
+        for (int k = 0; k < KS; ++k) {
+          if constexpr (FP8) {
+            ka[k] = __builtin_bit_cast(bf16x8_t, decode8(kw[t][k], ke[t]));
+          } else {
+            ka[k] = __builtin_bit_cast(bf16x8_t, kw[t][k]);
+          }
+        }
+        x[t] = scores<KS>(s, ka);
+        if (broken) {
+          // (The pages' numbers are the next block's by now: looked up again.)
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            const int g = kv + 32 * t + (i < 8 ? 0 : 16);
+            if (static_cast<uint32_t>(page_number(a, row, g)) >= static_cast<uint32_t>(a.pages.pages)) x[t][i] = 0.f;
+          }
+        }
+      }
+      if (more) {
+        load_k(kvn);
+        find(kvn + stride);
+      } else {
+        broken = false;
+      }
+      // V of this block was on its way before K of this block, which has arrived: at most the next block's loads are left.
+      if constexpr (!FP8) {
+        if (more) {
+          asm volatile("s_waitcnt vmcnt(%0)" ::"n"(4 * Width<DT>::kSubTiles + KS) : "memory");
+        } else {
+          wait_vmem();
+        }
+      }
+#pragma unroll
+      for (int t = 0; t < kHalves; ++t) {
+        if (t == 0 || kv + 32 * t < k1) {
+          attend_half<KS, kSubBytes>(s, x[t], cur + 32 * t * kRow * 2, rvt, a.scale_log2, kv + 32 * t + 31 > all,
+                                     kv + 32 * t);
+        }
+      }
+      kv = kvn;
+      kvn += stride;
     };
     while (kv < k1) {
-      step(cK0, cV0, cK1, cV1);
-      if (kv < k1) step(cK1, cV1, cK0, cV0);
+      step(c0, c1);
+      if (!FP8 && kv < k1) step(c1, c0);
     }
   }
-  // The waves' sums joined, in order: O of wave w at its tile, [head_dim][row].
+  // The waves' sums joined, in order: O of wave w [head_dim][row].
   const float l = row_sum(s.l[0]);
   __syncthreads();
-  float* so = reinterpret_cast<float*>(wave < 2 ? sK0 : sK1) + (wave & 1) * 2 * kTileBytes / 4;
-  static_assert(2 * kTileBytes >= 32 * DT * kRows * 4, "O of a wave fits its two buffers' part");
+  float* so = reinterpret_cast<float*>(wave < kFirst ? sV0 : sV1) + (wave % kFirst) * kWaveO;
   if (hh == 0) {
     s_ml[wave][0][col] = s.m;
     s_ml[wave][1][col] = l;
@@ -629,7 +747,6 @@ __global__ __launch_bounds__(kPagedThreads, 2) void paged_row_kernel(PagedArgs a
     for (int e = 0; e < 16; ++e) so[(32 * j + 8 * (e >> 2) + 4 * hh + (e & 3)) * kRows + col] = s.o[j][e];
   }
   __syncthreads();
-  const int D = static_cast<int>(a.D);
   for (int e = threadIdx.x; e < rows * (D / 2); e += kPagedThreads) {
     const int rr = e / (D / 2), d = 2 * (e - rr * (D / 2));
     float m = s_ml[0][0][rr];
@@ -639,7 +756,7 @@ __global__ __launch_bounds__(kPagedThreads, 2) void paged_row_kernel(PagedArgs a
 #pragma unroll
     for (int x = 0; x < 4; ++x) {
       const float f = __builtin_amdgcn_exp2f(s_ml[x][0][rr] - m);
-      const float* from = reinterpret_cast<const float*>(x < 2 ? sK0 : sK1) + (x & 1) * 2 * kTileBytes / 4;
+      const float* from = reinterpret_cast<const float*>(x < kFirst ? sV0 : sV1) + (x % kFirst) * kWaveO;
       sum = __builtin_fmaf(s_ml[x][1][rr], f, sum);
       o0 = __builtin_fmaf(from[d * kRows + rr], f, o0);
       o1 = __builtin_fmaf(from[(d + 1) * kRows + rr], f, o1);
@@ -658,7 +775,9 @@ __global__ __launch_bounds__(kPagedThreads, 2) void paged_row_kernel(PagedArgs a
 #endif
 }
 
-// The parts of a row joined in order. 32 lanes a row, 4 elements a lane.
+// The parts of a row joined in order. 32 lanes a row, 4 elements a lane, kAhead parts in flight.
+constexpr int kAhead = 8;
+
 __global__ __launch_bounds__(kPagedThreads) void paged_join_kernel(PagedArgs a) {
   const int64_t id = static_cast<int64_t>(blockIdx.x) * (kPagedThreads / 32) + threadIdx.x / 32;
   const int d0 = 4 * (threadIdx.x % 32);
@@ -692,13 +811,26 @@ __global__ __launch_bounds__(kPagedThreads) void paged_join_kernel(PagedArgs a) 
   }
   if (count < 2) return;
   float m = kNoMax, l = 0.f, o[4] = {0.f, 0.f, 0.f, 0.f};
-  for (int p = 0; p < count; ++p, slot += step) {
-    const float mi = slot[a.D], li = slot[a.D + 1];
-    const float mn = fmaxf(m, mi), x = __builtin_amdgcn_exp2f(m - mn), y = __builtin_amdgcn_exp2f(mi - mn);
-    m = mn;
-    l = join_value(l, li, x, y);
+  for (int p0 = 0; p0 < count; p0 += kAhead, slot += kAhead * step) {
+    float2 ml[kAhead], oa[kAhead], ob[kAhead];
 #pragma unroll
-    for (int e = 0; e < 4; ++e) o[e] = join_value(o[e], slot[d0 + e], x, y);
+    for (int p = 0; p < kAhead; ++p) {  // the last part again behind the end: no branch around the loads
+      const float* at = slot + (p0 + p < count ? p : count - 1 - p0) * step;
+      ml[p] = *reinterpret_cast<const float2*>(at + a.D);
+      oa[p] = *reinterpret_cast<const float2*>(at + d0);
+      ob[p] = *reinterpret_cast<const float2*>(at + d0 + 2);
+    }
+#pragma unroll
+    for (int p = 0; p < kAhead; ++p) {
+      if (p0 + p >= count) break;
+      const float mn = fmaxf(m, ml[p].x), x = __builtin_amdgcn_exp2f(m - mn), y = __builtin_amdgcn_exp2f(ml[p].x - mn);
+      m = mn;
+      l = join_value(l, ml[p].y, x, y);
+      o[0] = join_value(o[0], oa[p].x, x, y);
+      o[1] = join_value(o[1], oa[p].y, x, y);
+      o[2] = join_value(o[2], ob[p].x, x, y);
+      o[3] = join_value(o[3], ob[p].y, x, y);
+    }
   }
   const float inv = last_key(a, w, i) >= 0 ? 1.f / l : 0.f;
   uint16_t* out = a.o + (a.tokens.cu ? 0 : b * a.so_b) + h * a.so_h + (a.tokens.cu ? token : i) * a.so_n;
@@ -741,25 +873,29 @@ inline PagedPlan paged_plan(int64_t B, int64_t H, int64_t Hkv, int64_t N, bool p
   return p;
 }
 
-template <bool FP8, int DT>
+template <bool FP8, int KS>
 void launch_paged(const PagedArgs& a, const PagedPlan& p, hipStream_t s) {
   if (p.rows) {
-    paged_row_kernel<FP8, DT><<<static_cast<unsigned>(p.row_slots), kPagedThreads, 0, s>>>(a);
+    paged_row_kernel<FP8, KS><<<static_cast<unsigned>(p.row_slots), kPagedThreads, 0, s>>>(a);
   }
   if (p.tiles) {
     const int64_t units = p.tile_count / p.q_tiles * a.Hkv * p.parts;
-    paged_tile_kernel<FP8, DT><<<static_cast<unsigned>(cdiv(units, kXcds) * kXcds * p.q_tiles), kPagedThreads, 0, s>>>(a);
+    paged_tile_kernel<FP8, KS><<<static_cast<unsigned>(cdiv(units, kXcds) * kXcds * p.q_tiles), kPagedThreads, 0, s>>>(a);
   }
 }
 
+// By the steps that head_dim takes.
 template <bool FP8>
 void launch_width(const PagedArgs& a, const PagedPlan& p, hipStream_t s) {
-  if (a.D <= 64) {
-    launch_paged<FP8, 2>(a, p, s);
-  } else if (a.D <= 96) {
-    launch_paged<FP8, 3>(a, p, s);
-  } else {
-    launch_paged<FP8, 4>(a, p, s);
+  switch (static_cast<int>(cdiv(a.D, 16))) {
+    case 8: return launch_paged<FP8, 8>(a, p, s);
+    case 7: return launch_paged<FP8, 7>(a, p, s);
+    case 6: return launch_paged<FP8, 6>(a, p, s);
+    case 5: return launch_paged<FP8, 5>(a, p, s);
+    case 4: return launch_paged<FP8, 4>(a, p, s);
+    case 3: return launch_paged<FP8, 3>(a, p, s);
+    case 2: return launch_paged<FP8, 2>(a, p, s);
+    default: return launch_paged<FP8, 1>(a, p, s);
   }
 }
 

@@ -102,6 +102,7 @@ def test_cache_errors(lib, call):
     assert call(lib, B=-1) == -1 and b'sizes' in error()
     for kw in (dict(pages=-1), dict(m=-1), dict(m=1 << 25), dict(pages=1 << 31)):
         assert call(lib, **kw) == -1 and b'page counts' in error()
+    assert call(lib, pages=0) == -1 and b'needs a page' in error()
     for name in ('kp', 'table', 'lengths'):
         assert call(lib, **{name: 0}) == -1 and b'null' in error()
     assert call(lib, dtype=3) == -1 and b'exponents' in error()
