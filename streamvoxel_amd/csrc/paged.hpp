@@ -116,8 +116,8 @@ inline int check_pool(const char* name, const svhip_paged_cache& c) {
   SVHIP_REQUIRE(reinterpret_cast<uintptr_t>(c.k_pages) % bytes == 0 && reinterpret_cast<uintptr_t>(c.v_pages) % bytes == 0 &&
                     (c.sk_p | c.sk_h | c.sk_r | c.sv_p | c.sv_h | c.sv_r) % 8 == 0,
                 "%s: rows of a page must start on %d-byte boundaries", name, (int)bytes);
-  SVHIP_REQUIRE(c.sk_r >= 0 && c.sk_r < (1 << 26) && c.sv_r >= 0 && c.sv_r < (1 << 26), "%s: rows of a page too far apart",
-                name);  // 16 rows within a descriptor's 32-bit offsets
+  SVHIP_REQUIRE(c.sk_r >= 0 && c.sv_r >= 0 && c.sk_r < (1 << 29) / c.page_size && c.sv_r < (1 << 29) / c.page_size,
+                "%s: rows of a page too far apart", name);  // a head's rows in a page within 2^31 bytes
   return SVHIP_OK;
 }
 

@@ -97,8 +97,8 @@ __device__ __forceinline__ int wave_prefix(int v, int& total) {
 // as it stands in the table (j may lie past the window's keys: its last entry then).
 __device__ __forceinline__ int page_number(const PagedArgs& a, const int32_t* row, int j) {
   typedef const __attribute__((address_space(4))) int32_t* table_t;
-  const int64_t at = j >> a.pages.shift;
-  return __builtin_amdgcn_readfirstlane(((table_t)row)[at < a.pages.max_pages ? at : a.pages.max_pages - 1]);
+  const int at = j >> a.pages.shift, last = static_cast<int>(a.pages.max_pages) - 1;
+  return __builtin_amdgcn_readfirstlane(((table_t)row)[at < last ? at : last]);
 }
 
 #if defined(__HIP_DEVICE_COMPILE__)
@@ -108,16 +108,16 @@ __device__ __forceinline__ int page_number(const PagedArgs& a, const int32_t* ro
 template <int ES>
 __device__ __forceinline__ __amdgpu_buffer_rsrc_t rows_of(const char* head, int page, int in_page, int64_t sp, int64_t sr,
                                                          int valid, int D) {
-  const char* base = head + (page * sp + in_page * sr) * ES;
-  const uint32_t bytes = valid > 0 ? static_cast<uint32_t>(((valid - 1) * static_cast<int>(sr) + D) * ES) : 0u;
+  const int row = static_cast<int>(sr) * ES;  // a page spans less than 2^31 bytes
+  const char* base = head + static_cast<uint32_t>(page) * (sp * ES) + in_page * row;
+  const uint32_t bytes = valid > 0 ? static_cast<uint32_t>((valid - 1) * row + D * ES) : 0u;
   return __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(base), 0, bytes, kRsrcFlags);
 }
 
 // Keys of the 16 at j that exist: inside the window and on a page of the pool.
 __device__ __forceinline__ int valid_keys(const PagedArgs& a, int keys, int j, int& page) {
-  int valid = keys - j;
-  valid = valid < 0 ? 0 : (valid > 16 ? 16 : valid);
-  if (static_cast<uint32_t>(page) >= static_cast<uint32_t>(a.pages.pages)) {
+  int valid = j + 16 <= keys ? 16 : (j < keys ? keys - j : 0);
+  if (__builtin_expect(static_cast<uint32_t>(page) >= static_cast<uint32_t>(a.pages.pages), 0)) {
     if (valid > 0) set_bad(a.pages);
     valid = 0;
     page = 0;
@@ -188,12 +188,15 @@ __device__ __forceinline__ void attend_half(Rows<KS>& s, f32x16_t x, const char*
       if ((i < 8 ? i : i + 8) > seen) x[i] = -INFINITY;
     }
   }
-  float mx = __builtin_amdgcn_fmed3f(x[0], x[1], kFltMax);
-#pragma unroll
-  for (int i = 2; i < 16; i += 2) mx = max3(mx, x[i], x[i + 1]);
-  if (__builtin_amdgcn_ballot_w64(__builtin_fmaf(mx, sl2, -s.m) > kMaxHigh) != 0ull) {
+  const auto max3 = [](float p, float q, float r) __attribute__((always_inline)) {
+    return __builtin_elementwise_maximum(__builtin_elementwise_maximum(p, q), r);
+  };
+  const float mx = max3(max3(max3(x[0], x[1], x[2]), max3(x[3], x[4], x[5]), max3(x[6], x[7], x[8])),
+                        max3(x[9], x[10], x[11]), max3(max3(x[12], x[13], x[14]), x[15], x[15]));
+  if (__builtin_expect(__builtin_amdgcn_ballot_w64(__builtin_fmaf(mx, sl2, -s.m) > kMaxHigh) != 0ull, 0)) {
     const auto sw = __builtin_amdgcn_permlane32_swap(__float_as_int(mx), __float_as_int(mx), false, false);
-    const float cand = __builtin_amdgcn_fmed3f(__int_as_float(sw[0]), __int_as_float(sw[1]), kFltMax) * sl2;
+    const float top = fmaxf(__int_as_float(sw[0]), __int_as_float(sw[1]));
+    const float cand = (top < kFltMax ? top : kFltMax) * sl2;
     const float mn = cand > s.m ? cand : s.m;
     const float alpha = __builtin_amdgcn_exp2f(s.m - mn);
     s.m = mn;
@@ -547,14 +550,14 @@ __device__ __forceinline__ int row_part_keys(const PagedArgs& a) {
   return static_cast<int>(each < kRowLeast ? kRowLeast : (each < (1 << 30) ? each : (1 << 30)));
 }
 
-// A wave takes every 4th block of 32 keys of its part (e4m3: 64). K rows go straight from memory to the A operands, a lane its
+// A wave takes every 4th block of 32 keys of its part (e4m3 up to head_dim 64: of 64 keys, as many bytes). K rows go straight from memory to the A operands, a lane its
 // own key's chunks, the next block's while the current one's softmax and second product run; V rows go through the wave's LDS,
 // since they are read transposed.
 template <bool FP8, int KS>
 __global__ __launch_bounds__(kPagedThreads, 2) void paged_row_kernel(PagedArgs a) {
 #if defined(__HIP_DEVICE_COMPILE__)
   constexpr int DT = tiles_of(KS), ES = FP8 ? 1 : 2;
-  constexpr int kHalves = FP8 ? 2 : 1, kKeys = kRowKeys * kHalves;  // of a wave's block
+  constexpr int kHalves = FP8 && KS <= 4 ? 2 : 1, kKeys = kRowKeys * kHalves;  // of a wave's block
   constexpr int kSubBytes = kKeys * kRow * 2, kTileBytes = Width<DT>::kSubTiles * kSubBytes;
   // V of the four waves, bf16 two blocks of each; O of them at the end, 32 DT x 32 floats each.
   constexpr int kWaveO = 32 * DT * kRows, kFirst = FP8 ? 4 : 2;  // waves whose O goes to sV0
