@@ -116,8 +116,13 @@ inline int check_pool(const char* name, const svhip_paged_cache& c) {
   SVHIP_REQUIRE(reinterpret_cast<uintptr_t>(c.k_pages) % bytes == 0 && reinterpret_cast<uintptr_t>(c.v_pages) % bytes == 0 &&
                     (c.sk_p | c.sk_h | c.sk_r | c.sv_p | c.sv_h | c.sv_r) % 8 == 0,
                 "%s: rows of a page must start on %d-byte boundaries", name, (int)bytes);
+  // A head's rows of a page lie within 2^31 bytes, pages start less than 2^32 bytes apart.
   SVHIP_REQUIRE(c.sk_r >= 0 && c.sv_r >= 0 && c.sk_r < (1 << 29) / c.page_size && c.sv_r < (1 << 29) / c.page_size,
-                "%s: rows of a page too far apart", name);  // a head's rows in a page within 2^31 bytes
+                "%s: rows of a page too far apart", name);
+  const int64_t most = 1ll << 31;
+  SVHIP_REQUIRE(c.sk_p >= 0 && c.sk_p < most && c.sv_p >= 0 && c.sv_p < most && c.sek_p >= 0 && c.sek_p < most &&
+                    c.sev_p >= 0 && c.sev_p < most,
+                "%s: pages too far apart", name);
   return SVHIP_OK;
 }
 

@@ -1,0 +1,428 @@
+// What the kernels of svhip_paged_attention share (paged_attention.hip describes them).
+#pragma once
+
+#include "paged.hpp"
+#include "xattn_kernel.hpp"
+
+namespace svhip {
+
+constexpr int kPagedThreads = 256;
+constexpr int kRows = 32;          // rows of a wave
+constexpr int kTileRows = 128;     // rows of a tile workgroup
+constexpr int kTileTarget = 512;   // tile workgroups below which keys are split: two for every CU
+constexpr int kTileLeast = 6;      // least key blocks of a tile's part
+constexpr int kRowTarget = 512;    // row-form workgroups that all keys are shared out to
+constexpr int kRowLeast = 256;     // keys that a row-form part has a multiple of
+constexpr int kWholePages = 64;    // pages from this size on hold whole blocks of keys
+constexpr int kUncut = 0x40000000; // a part length that cuts nothing
+constexpr float kNoMax = -3.0e38f; // running maximum before any key: finite, so that a row that sees nothing stays finite
+[[maybe_unused]] constexpr uint32_t kOutside = 0x7ffffff0u;  // byte offset past every descriptor's bound
+
+struct PagedArgs {
+  const uint16_t* q;
+  const void *k, *v;
+  const uint8_t *ek, *ev;
+  uint16_t* o;
+  Tokens tokens;
+  Pages pages;
+  int64_t H, Hkv, G, D;  // G: heads of a key head
+  int64_t sq_b, sq_h, sq_n, sk_h, sv_h, sek_h, sev_h, so_b, so_h, so_n;
+  uint32_t sk_p, sk_r, sv_p, sv_r, sek_p, sev_p;  // bytes from page to page and row to row
+  bool causal;
+  float scale_log2;
+  // The plan.
+  int q_tiles;          // tiles of a window (even windows)
+  bool split;           // tiles: whether parts of keys may be dealt out
+  int row_slots, tile_slots;  // slots of parts at most
+  int slot_rows;        // rows of a row-form slot
+  float *row_part, *tile_part;
+  int4* plan;           // a window's first slot, its parts, a part's length (tiles: blocks) and its tiles
+};
+
+// The window as a workgroup sees it.
+struct Window {
+  int64_t first, count;  // its tokens
+  int64_t last;          // the last key that its first token sees (causal), or its last key
+  int keys;              // its keys
+};
+
+__device__ __forceinline__ Window window_at(const PagedArgs& a, int64_t b) {
+  Window w;
+  window_tokens(a.tokens, b, w.first, w.count);
+  const int64_t L = held_keys(a.pages, b);
+  w.keys = static_cast<int>(L);
+  w.last = a.causal ? a.pages.lengths[b] - w.count : L - 1;
+  return w;
+}
+
+// Last key that token i sees (below 0: none).
+__device__ __forceinline__ int last_key(const PagedArgs& a, const Window& w, int64_t i) {
+  const int64_t j = a.causal ? w.last + i : w.last;
+  return static_cast<int>(j < w.keys - 1 ? (j < -1 ? -1 : j) : w.keys - 1);
+}
+
+__device__ __forceinline__ bool row_form(const PagedArgs& a, int64_t count) { return count * a.G <= kRows; }
+
+// Keys that the rows of tile qt see, the last of them the most.
+__device__ __forceinline__ int tile_keys(const PagedArgs& a, const Window& w, int64_t qt) {
+  const int64_t r1 = (qt + 1) * kTileRows, rows = w.count * a.G;
+  return last_key(a, w, ((r1 < rows ? r1 : rows) - 1) / a.G) + 1;
+}
+
+// Row of `out` (or, with its strides, of the queries) that token i and head h have.
+__device__ __forceinline__ int64_t row_at(const PagedArgs& a, const Window& w, int64_t b, int64_t h, int64_t i, int64_t sb,
+                                          int64_t sh, int64_t sn) {
+  return a.tokens.cu ? h * sh + (w.first + i) * sn : b * sb + h * sh + i * sn;
+}
+
+__device__ __forceinline__ int64_t wave_sum(int64_t v) {
+#pragma unroll
+  for (int off = 32; off >= 1; off >>= 1) v += __shfl_xor(v, off, 64);
+  return v;
+}
+
+// Exclusive prefix over the wave's lanes; `total` the sum.
+__device__ __forceinline__ int wave_prefix(int v, int& total) {
+  int incl = v;
+#pragma unroll
+  for (int off = 1; off < 64; off <<= 1) {
+    const int up = __shfl_up(incl, off, 64);
+    if ((threadIdx.x & 63) >= off) incl += up;
+  }
+  total = __builtin_amdgcn_readlane(incl, 63);
+  return incl - v;
+}
+
+// What a workgroup takes: part `part` of `parts` of key head kvh of window b (tiles: of tile qt), at place `at` of all, the
+// window's first being `before`. b < 0: nothing.
+struct PagedItem {
+  int b, kvh, part, parts, qt, tiles, at, before;
+};
+
+// The item at place `at` of the windows' lists, one after the other: window c has tiles(c) * Hkv * parts(c) of them, for every
+// key head its parts, for every part its tiles.
+template <typename Count>
+__device__ __forceinline__ PagedItem item_at(const PagedArgs& a, int at, Count count) {
+  const int lane = threadIdx.x & 63, Hkv = static_cast<int>(a.Hkv);
+  PagedItem item{-1, 0, 0, 1, 0, 1, at, 0};
+  int left = at;
+  for (int b0 = 0; b0 < a.tokens.B; b0 += 64) {
+    int tiles = 0, parts = 1, total;
+    if (b0 + lane < a.tokens.B) count(b0 + lane, tiles, parts);
+    const int n = tiles * Hkv * parts;
+    const int before = wave_prefix(n, total);
+    if (left < total) {
+      const int c = __builtin_ctzll(__builtin_amdgcn_ballot_w64(before <= left && left < before + n));
+      const int in = left - __builtin_amdgcn_readlane(before, c);
+      item.b = b0 + c;
+      item.tiles = __builtin_amdgcn_readlane(tiles, c);
+      item.parts = __builtin_amdgcn_readlane(parts, c);
+      item.before = at - in;
+      item.qt = in % item.tiles;
+      const int u = in / item.tiles;
+      item.kvh = u / item.parts;
+      item.part = u - item.kvh * item.parts;
+      return item;
+    }
+    left -= total;
+  }
+  return item;
+}
+
+// Page of the keys at j of the window whose table row this is, through the scalar cache; the number as it stands in the
+// table (j may lie past the window's keys: its last entry then).
+__device__ __forceinline__ int page_number(const PagedArgs& a, const int32_t* row, int j) {
+  typedef const __attribute__((address_space(4))) int32_t* table_t;
+  const int at = j >> a.pages.shift, last = static_cast<int>(a.pages.max_pages) - 1;
+  return __builtin_amdgcn_readfirstlane(((table_t)row)[at < last ? at : last]);
+}
+
+// Keys of the kGroup at j that exist: inside the window and on a page of the pool.
+template <int kGroup>
+__device__ __forceinline__ int valid_keys(const PagedArgs& a, int keys, int j, int& page) {
+  int valid = j + kGroup <= keys ? kGroup : (j < keys ? keys - j : 0);
+  if (__builtin_expect(static_cast<uint32_t>(page) >= static_cast<uint32_t>(a.pages.pages), 0)) {
+    if (valid > 0) set_bad(a.pages);
+    valid = 0;
+    page = 0;
+  }
+  return valid;
+}
+
+#if defined(__HIP_DEVICE_COMPILE__)
+
+// One key head's part of a pool (of keys or of values): bytes from page to page and row to row.
+struct Source {
+  const char* rows;
+  const uint8_t* exponents;
+  uint32_t sp, sr, se;
+};
+template <int ES>
+__device__ __forceinline__ Source k_source(const PagedArgs& a, int64_t kvh) {
+  return Source{static_cast<const char*>(a.k) + kvh * a.sk_h * ES, ES == 1 ? a.ek + kvh * a.sek_h : nullptr, a.sk_p,
+                a.sk_r, a.sek_p};
+}
+template <int ES>
+__device__ __forceinline__ Source v_source(const PagedArgs& a, int64_t kvh) {
+  return Source{static_cast<const char*>(a.v) + kvh * a.sv_h * ES, ES == 1 ? a.ev + kvh * a.sev_h : nullptr, a.sv_p,
+                a.sv_r, a.sev_p};
+}
+
+// Descriptor of the rows of a group of keys, row in_page of `page` the first: `valid` of them, `bytes` of each. A read past
+// them gives zeros.
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t rows_of(const char* head, uint32_t sp, uint32_t sr, int page, int in_page,
+                                                         int valid, int bytes) {
+  const char* base = head + static_cast<uint64_t>(static_cast<uint32_t>(page)) * sp + static_cast<uint32_t>(in_page) * sr;
+  const uint32_t bound = valid > 0 ? static_cast<uint32_t>(valid - 1) * sr + bytes : 0u;
+  return __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(base), 0, bound, kRsrcFlags);
+}
+
+// Head widths: KS steps of 16 head_dim elements in the score product, and output tiles of 32.
+constexpr int tiles_of(int KS) { return (KS + 1) / 2; }
+
+// A wave's 32 rows: the queries as B operands, O^T, running maximum (log2 units) and sum.
+template <int KS>
+struct Rows {
+  bf16x8_t qf[KS];
+  f32x16_t o[tiles_of(KS)];
+  f32x4_t l;   // four equal entries: the lane's share of its row's sum
+  float m;
+  int last;    // last key that the lane's row sees
+};
+
+template <int KS>
+__device__ __forceinline__ void load_rows(const PagedArgs& a, const Window& w, int64_t b, int64_t kvh, int64_t r,
+                                          Rows<KS>& s) {
+  const int hh = (threadIdx.x & 63) >> 5;
+  const int64_t i = r / a.G, g = r - i * a.G;
+  const bool ok = i < w.count;
+  const uint16_t* q = a.q + row_at(a, w, b, kvh * a.G + g, i, a.sq_b, a.sq_h, a.sq_n);
+#pragma unroll
+  for (int k = 0; k < KS; ++k) {
+    const int d0 = 16 * k + 8 * hh;
+    uint4 raw = make_uint4(0u, 0u, 0u, 0u);
+    if (ok && d0 < a.D) raw = *reinterpret_cast<const uint4*>(q + d0);
+    s.qf[k] = __builtin_bit_cast(bf16x8_t, raw);
+  }
+#pragma unroll
+  for (int j = 0; j < tiles_of(KS); ++j) s.o[j] = f32x16_t{0};
+  s.l = f32x4_t{0.f, 0.f, 0.f, 0.f};
+  s.m = kNoMax;
+  s.last = ok ? last_key(a, w, i) : -1;
+}
+
+// S^T of 32 keys: ka the K rows as A operands, row R of the tile key sigma_row(R).
+template <int KS>
+__device__ __forceinline__ f32x16_t scores(const Rows<KS>& s, const bf16x8_t (&ka)[KS]) {
+  f32x16_t x;
+#pragma unroll
+  for (int k = 0; k < KS; ++k) {
+    x = __builtin_amdgcn_mfma_f32_32x32x16_bf16(ka[k], s.qf[k], k == 0 ? f32x16_t{0} : x, 0, 0, 0);
+  }
+  return x;
+}
+
+// The rest of 32 keys, `key0` the first, from their scores x: weights, sum, and O^T += V^T P^T with V rows staged at row 0 of
+// vp (sub-tiles of 64 head_dim elements kSubBytes apart). The running maximum moves only for a score more than kMaxHigh
+// above it (P then stays below 2^20, which fp32 sums and bf16 weights hold alike); the row's sum is taken over the bf16
+// weights that the second product reads, by v_mfma_f32_4x4x4_16b_bf16 with ones in A, whose columns are single lanes: no
+// row's NaN reaches another's sum.
+template <int KS, int kSubBytes>
+__device__ __forceinline__ void attend_half(Rows<KS>& s, f32x16_t x, const char* vp,
+                                            const uint32_t (&rvt)[tiles_of(KS)], float sl2, bool masked, int key0) {
+  constexpr int DT = tiles_of(KS);
+  const int hh = (threadIdx.x & 63) >> 5;
+  if (masked) {
+    const int seen = s.last - key0 - 8 * hh;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      if ((i < 8 ? i : i + 8) > seen) x[i] = -INFINITY;
+    }
+  }
+  const auto max3 = [](float p, float q, float r) __attribute__((always_inline)) {
+    return __builtin_elementwise_maximum(__builtin_elementwise_maximum(p, q), r);
+  };
+  const float mx = max3(max3(max3(x[0], x[1], x[2]), max3(x[3], x[4], x[5]), max3(x[6], x[7], x[8])),
+                        max3(x[9], x[10], x[11]), max3(max3(x[12], x[13], x[14]), x[15], x[15]));
+  if (__builtin_expect(__builtin_amdgcn_ballot_w64(__builtin_fmaf(mx, sl2, -s.m) > kMaxHigh) != 0ull, 0)) {
+    const auto sw = __builtin_amdgcn_permlane32_swap(__float_as_int(mx), __float_as_int(mx), false, false);
+    const float top = fmaxf(__int_as_float(sw[0]), __int_as_float(sw[1]));
+    const float cand = (top < kFltMax ? top : kFltMax) * sl2;
+    const float mn = cand > s.m ? cand : s.m;
+    const float alpha = __builtin_amdgcn_exp2f(s.m - mn);
+    s.m = mn;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) s.l[i] *= alpha;
+#pragma unroll
+    for (int j = 0; j < DT; ++j) {
+#pragma unroll
+      for (int i = 0; i < 16; ++i) s.o[j][i] *= alpha;
+    }
+  }
+  bf16x8_t pb[2];
+#pragma unroll
+  for (int ks = 0; ks < 2; ++ks) {
+#pragma unroll
+    for (int j = 0; j < 8; j += 2) {
+      const f32x2_t two = {__builtin_amdgcn_exp2f(__builtin_fmaf(x[8 * ks + j], sl2, -s.m)),
+                           __builtin_amdgcn_exp2f(__builtin_fmaf(x[8 * ks + j + 1], sl2, -s.m))};
+      const bf16x2_t c = __builtin_convertvector(two, bf16x2_t);
+      pb[ks][j] = c[0];
+      pb[ks][j + 1] = c[1];
+    }
+  }
+  typedef short i16x4_t __attribute__((ext_vector_type(4)));
+  typedef short i16x8_t __attribute__((ext_vector_type(8)));
+  const i16x4_t ones = {0x3F80, 0x3F80, 0x3F80, 0x3F80};
+#pragma unroll
+  for (int ks = 0; ks < 2; ++ks) {
+    const i16x8_t p8 = __builtin_bit_cast(i16x8_t, pb[ks]);
+    s.l = __builtin_amdgcn_mfma_f32_4x4x4bf16_1k(ones, __builtin_shufflevector(p8, p8, 0, 1, 2, 3), s.l, 0, 0, 0);
+    s.l = __builtin_amdgcn_mfma_f32_4x4x4bf16_1k(ones, __builtin_shufflevector(p8, p8, 4, 5, 6, 7), s.l, 0, 0, 0);
+  }
+#pragma unroll
+  for (int ks = 0; ks < 2; ++ks) {
+    bf16x8_t va[DT];
+#pragma unroll
+    for (int j = 0; j < DT; ++j) {
+      typedef __bf16 bf16x4_t __attribute__((ext_vector_type(4)));
+      typedef __attribute__((address_space(3))) bf16x4_t lds_bf16x4_t;
+      char* at = const_cast<char*>(vp) + (j >> 1) * kSubBytes + rvt[j] + 16 * ks * kRow * 2;
+      const bf16x4_t lo = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((lds_bf16x4_t*)(at));
+      const bf16x4_t hi = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((lds_bf16x4_t*)(at + 4 * kRow * 2));
+      va[j] = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+    }
+#pragma unroll
+    for (int j = 0; j < DT; ++j) s.o[j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(va[j], pb[ks], s.o[j], 0, 0, 0);
+  }
+}
+
+// Byte offsets of the reads of V rows, transposed: output tile j inside its sub-tile (xattn_kernel.hpp).
+template <int DT>
+__device__ __forceinline__ void v_offsets(uint32_t (&rvt)[DT]) {
+  const int lane = threadIdx.x & 63, hh = lane >> 5;
+  const int row = 8 * hh + ((lane & 15) >> 2), flip = (row >> 1) & 1;
+  const int c = 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1);
+#pragma unroll
+  for (int j = 0; j < DT; ++j) {
+    rvt[j] = static_cast<uint32_t>(row * kRow * 2 + 16 * (4 * ((j & 1) ^ flip) + c) + 8 * (lane & 1));
+  }
+}
+
+// The lane's sum of its row, both lanes' shares.
+__device__ __forceinline__ float row_sum(float l) {
+  const auto sw = __builtin_amdgcn_permlane32_swap(__float_as_int(l), __float_as_int(l), false, false);
+  return __int_as_float(sw[0]) + __int_as_float(sw[1]);
+}
+
+// e4m3 rows on their way to LDS: a wave's kLoads loads of 8 rows, and the rows' exponents.
+template <int DT, int kLoads>
+struct Staged {
+  uint2 w[kLoads * Width<DT>::kSubTiles];
+  uint32_t e[kLoads];
+};
+
+// A lane's place in a load of 8 rows whose first is row `first` of a block's tile (a multiple of 8), `base` being the tile row
+// of the descriptor's first key: row lane / 8 and its chunk; K under sigma_row and swz, V under swzv.
+struct Lane8 {
+  uint32_t at[2];   // byte offset in the descriptor in each sub-tile, or kOutside past head_dim
+  uint32_t key;     // the key's place in the descriptor
+};
+
+template <int ES>
+__device__ __forceinline__ Lane8 lane_of_load(uint32_t sr, int64_t D, int key, int chunk) {
+  Lane8 n;
+  n.key = static_cast<uint32_t>(key);
+#pragma unroll
+  for (int u = 0; u < 2; ++u) {
+    const int d = 64 * u + 8 * chunk;
+    n.at[u] = d < D ? n.key * sr + static_cast<uint32_t>(d * ES) : kOutside;
+  }
+  return n;
+}
+template <int ES>
+__device__ __forceinline__ Lane8 k_lane(const PagedArgs& a, int first, int base) {
+  const int lane = threadIdx.x & 63, R = first + (lane >> 3);
+  return lane_of_load<ES>(a.sk_r, a.D, sigma_row(R) - base, swz(R, lane & 7));
+}
+template <int ES>
+__device__ __forceinline__ Lane8 v_lane(const PagedArgs& a, int first, int base) {
+  const int lane = threadIdx.x & 63, R = first + (lane >> 3);
+  return lane_of_load<ES>(a.sv_r, a.D, R - base, swzv(R, lane & 7));
+}
+
+// Issues a load of 8 rows: bf16 straight into LDS at `to` (row 0 of the 8 in sub-tile 0), e4m3 into registers at index i.
+template <bool FP8, int DT, int kSubBytes, int kLoads>
+__device__ __forceinline__ void stage_rows8(const __amdgpu_buffer_rsrc_t r, const __amdgpu_buffer_rsrc_t er, const Lane8& n,
+                                            int i, char* to, Staged<DT, kLoads>& st) {
+#pragma unroll
+  for (int u = 0; u < Width<DT>::kSubTiles; ++u) {
+    if constexpr (FP8) {
+      st.w[i * Width<DT>::kSubTiles + u] = __builtin_bit_cast(uint2, __builtin_amdgcn_raw_buffer_load_b64(r, n.at[u], 0, 0));
+    } else {
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (lds_ptr_t)(to + u * kSubBytes), 16, n.at[u], 0, 0, 0);
+    }
+  }
+  if constexpr (FP8) st.e[i] = __builtin_amdgcn_raw_buffer_load_b8(er, n.key, 0, 0);
+}
+
+// 8 e4m3 codes times 2^(exponent - 127) as bf16, exact.
+__device__ __forceinline__ uint4 decode8(uint2 w, uint32_t exponent) {
+  const float f = exponent_value(static_cast<int>(exponent));
+  const bf16x2_t a = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w.x, f, false);
+  const bf16x2_t b = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w.x, f, true);
+  const bf16x2_t c = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w.y, f, false);
+  const bf16x2_t d = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w.y, f, true);
+  return make_uint4(__builtin_bit_cast(uint32_t, a), __builtin_bit_cast(uint32_t, b), __builtin_bit_cast(uint32_t, c),
+                    __builtin_bit_cast(uint32_t, d));
+}
+
+// e4m3: load i of `st` into its 8 rows at `to`.
+template <int DT, int kSubBytes, int kLoads>
+__device__ __forceinline__ void commit_rows8(const Staged<DT, kLoads>& st, int i, char* to) {
+#pragma unroll
+  for (int u = 0; u < Width<DT>::kSubTiles; ++u) {
+    *reinterpret_cast<uint4*>(to + u * kSubBytes + 16 * (threadIdx.x & 63)) =
+        decode8(st.w[i * Width<DT>::kSubTiles + u], st.e[i]);
+  }
+}
+
+#endif  // __HIP_DEVICE_COMPILE__
+
+// What a call launches, by its sizes alone.
+struct PagedPlan {
+  bool rows, tiles, split;  // the forms that its windows may take, and whether tiles may be split
+  int q_tiles;
+  int64_t tile_grid, tile_slots, row_slots, slot_rows, row_floats, tile_floats, plan_windows;
+  size_t bytes() const { return static_cast<size_t>(row_floats + tile_floats) * 4 + static_cast<size_t>(plan_windows) * 16; }
+};
+
+// FP8, KS: steps of 16 head_dim elements; whole: pages of kWholePages keys or more.
+void launch_paged_rows(const PagedArgs& a, const PagedPlan& p, bool fp8, bool whole, hipStream_t s);
+void launch_paged_tiles(const PagedArgs& a, const PagedPlan& p, bool fp8, bool whole, hipStream_t s);
+
+// The instantiations of `launch` by type, page size and head width.
+#define SVHIP_PAGED_WIDTH(launch, FP8, WHOLE)                      \
+  switch (static_cast<int>(cdiv(a.D, 16))) {                       \
+    case 8: return launch<FP8, WHOLE, 8>(a, p, s);                 \
+    case 7: return launch<FP8, WHOLE, 7>(a, p, s);                 \
+    case 6: return launch<FP8, WHOLE, 6>(a, p, s);                 \
+    case 5: return launch<FP8, WHOLE, 5>(a, p, s);                 \
+    case 4: return launch<FP8, WHOLE, 4>(a, p, s);                 \
+    case 3: return launch<FP8, WHOLE, 3>(a, p, s);                 \
+    case 2: return launch<FP8, WHOLE, 2>(a, p, s);                 \
+    default: return launch<FP8, WHOLE, 1>(a, p, s);                \
+  }
+#define SVHIP_PAGED_LAUNCH(launch)           \
+  if (fp8) {                                 \
+    if (whole) {                             \
+      SVHIP_PAGED_WIDTH(launch, true, true)  \
+    }                                        \
+    SVHIP_PAGED_WIDTH(launch, true, false)   \
+  }                                          \
+  if (whole) {                               \
+    SVHIP_PAGED_WIDTH(launch, false, true)   \
+  }                                          \
+  SVHIP_PAGED_WIDTH(launch, false, false)
+
+}  // namespace svhip
