@@ -125,8 +125,7 @@ inline PagedPlan paged_plan(int64_t B, int64_t H, int64_t Hkv, int64_t N, bool p
       p.tile_grid = cdiv(B * Hkv, kXcds) * kXcds * p.q_tiles;
       p.tile_slots = p.tile_grid;
     } else {
-      // Parts only where there are fewer than kTileTarget tiles: an equal share each and one more for every tile.
-      p.tile_slots = kTileTarget + (units < kTileTarget ? units : kTileTarget);
+      p.tile_slots = kTileTarget;  // parts only where there are fewer tiles than that
       p.tile_grid = cdiv(units > p.tile_slots ? units : p.tile_slots, kXcds) * kXcds;
       p.tile_floats = p.tile_slots * kTileRows * (D + 2);
     }

@@ -129,6 +129,31 @@ __device__ __forceinline__ PagedItem item_at(const PagedArgs& a, int at, Count c
   return item;
 }
 
+// The least length of a part, a multiple of `grain` and `least` at least, for which the windows' parts are at most `target`:
+// they then run side by side, and none longer than it must. places(c, length): parts of window c, all key heads and tiles.
+template <typename Places>
+__device__ __forceinline__ int part_length(const PagedArgs& a, int64_t work, int target, int grain, int least,
+                                           Places places) {
+  // An equal share is too short, or all but; twice as long again and again until it fits, then halves between.
+  int low = static_cast<int>(work / target / grain);
+  if (low * grain < least) low = least / grain - 1;
+  int high = low + 1;
+  auto fits = [&](int length) __attribute__((always_inline)) {
+    int64_t n = 0;
+    for (int64_t c = threadIdx.x & 63; c < a.tokens.B; c += 64) n += places(static_cast<int>(c), length * grain);
+    return wave_sum(n) <= target;
+  };
+  while (high < kUncut / grain / 2 && !fits(high)) {
+    low = high;
+    high += high;
+  }
+  while (high - low > 1) {
+    const int mid = low + (high - low) / 2;
+    (fits(mid) ? high : low) = mid;
+  }
+  return high * grain;
+}
+
 // Page of the keys at j of the window whose table row this is, through the scalar cache; the number as it stands in the
 // table (j may lie past the window's keys: its last entry then).
 __device__ __forceinline__ int page_number(const PagedArgs& a, const int32_t* row, int j) {
@@ -180,13 +205,13 @@ __device__ __forceinline__ __amdgpu_buffer_rsrc_t rows_of(const char* head, uint
 // Head widths: KS steps of 16 head_dim elements in the score product, and output tiles of 32.
 constexpr int tiles_of(int KS) { return (KS + 1) / 2; }
 
-// A wave's 32 rows: the queries as B operands, O^T, running maximum (log2 units) and sum.
+// A wave's 32 rows: the queries as B operands, O^T, running maximum and sum.
 template <int KS>
 struct Rows {
   bf16x8_t qf[KS];
   f32x16_t o[tiles_of(KS)];
   f32x4_t l;   // four equal entries: the lane's share of its row's sum
-  float m;
+  float m;     // running maximum, log2 units
   int last;    // last key that the lane's row sees
 };
 
@@ -222,29 +247,39 @@ __device__ __forceinline__ f32x16_t scores(const Rows<KS>& s, const bf16x8_t (&k
   return x;
 }
 
-// The rest of 32 keys, `key0` the first, from their scores x: weights, sum, and O^T += V^T P^T with V rows staged at row 0 of
-// vp (sub-tiles of 64 head_dim elements kSubBytes apart). The running maximum moves only for a score more than kMaxHigh
-// above it (P then stays below 2^20, which fp32 sums and bf16 weights hold alike); the row's sum is taken over the bf16
-// weights that the second product reads, by v_mfma_f32_4x4x4_16b_bf16 with ones in A, whose columns are single lanes: no
-// row's NaN reaches another's sum.
-template <int KS, int kSubBytes>
-__device__ __forceinline__ void attend_half(Rows<KS>& s, f32x16_t x, const char* vp,
-                                            const uint32_t (&rvt)[tiles_of(KS)], float sl2, bool masked, int key0) {
+// The rest of a block of 32 kHalves keys, `key0` the first, from their scores x: weights, sum, and O^T += V^T P^T with V rows
+// staged at row 0 of vp (sub-tiles of 64 head_dim elements kSubBytes apart). The running maximum moves only for a score more
+// than kMaxHigh above it (the weights then stay below 2^20, which fp32 sums and bf16 hold alike). One such branch a block: a
+// second one in a loop makes the compiler merge two register sets of O behind it, a copy that the common path pays. The row's
+// sum is taken over the bf16 weights that the second product reads, by v_mfma_f32_4x4x4_16b_bf16 with ones in A, whose
+// columns are single lanes: no row's NaN reaches another's sum.
+template <int KS, int kSubBytes, int kHalves>
+__device__ __forceinline__ void attend_block(Rows<KS>& s, f32x16_t (&x)[kHalves], const char* vp,
+                                             const uint32_t (&rvt)[tiles_of(KS)], float sl2, bool masked, int key0) {
   constexpr int DT = tiles_of(KS);
   const int hh = (threadIdx.x & 63) >> 5;
   if (masked) {
-    const int seen = s.last - key0 - 8 * hh;
 #pragma unroll
-    for (int i = 0; i < 16; ++i) {
-      if ((i < 8 ? i : i + 8) > seen) x[i] = -INFINITY;
+    for (int t = 0; t < kHalves; ++t) {
+      const int seen = s.last - key0 - 32 * t - 8 * hh;
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        if ((i < 8 ? i : i + 8) > seen) x[t][i] = -INFINITY;
+      }
     }
   }
   const auto max3 = [](float p, float q, float r) __attribute__((always_inline)) {
     return __builtin_elementwise_maximum(__builtin_elementwise_maximum(p, q), r);
   };
-  const float mx = max3(max3(max3(x[0], x[1], x[2]), max3(x[3], x[4], x[5]), max3(x[6], x[7], x[8])),
-                        max3(x[9], x[10], x[11]), max3(max3(x[12], x[13], x[14]), x[15], x[15]));
-  if (__builtin_expect(__builtin_amdgcn_ballot_w64(__builtin_fmaf(mx, sl2, -s.m) > kMaxHigh) != 0ull, 0)) {
+  float mx = 0.f;
+#pragma unroll
+  for (int t = 0; t < kHalves; ++t) {
+    const f32x16_t& y = x[t];
+    const float h = max3(max3(max3(y[0], y[1], y[2]), max3(y[3], y[4], y[5]), max3(y[6], y[7], y[8])),
+                         max3(y[9], y[10], y[11]), max3(max3(y[12], y[13], y[14]), y[15], y[15]));
+    mx = t == 0 ? h : __builtin_elementwise_maximum(mx, h);
+  }
+  if (__builtin_amdgcn_ballot_w64(__builtin_fmaf(mx, sl2, -s.m) > kMaxHigh) != 0ull) {
     const auto sw = __builtin_amdgcn_permlane32_swap(__float_as_int(mx), __float_as_int(mx), false, false);
     const float top = fmaxf(__int_as_float(sw[0]), __int_as_float(sw[1]));
     const float cand = (top < kFltMax ? top : kFltMax) * sl2;
@@ -259,41 +294,45 @@ __device__ __forceinline__ void attend_half(Rows<KS>& s, f32x16_t x, const char*
       for (int i = 0; i < 16; ++i) s.o[j][i] *= alpha;
     }
   }
-  bf16x8_t pb[2];
+  const float nm = -s.m;
 #pragma unroll
-  for (int ks = 0; ks < 2; ++ks) {
+  for (int t = 0; t < kHalves; ++t) {
+    bf16x8_t pb[2];
 #pragma unroll
-    for (int j = 0; j < 8; j += 2) {
-      const f32x2_t two = {__builtin_amdgcn_exp2f(__builtin_fmaf(x[8 * ks + j], sl2, -s.m)),
-                           __builtin_amdgcn_exp2f(__builtin_fmaf(x[8 * ks + j + 1], sl2, -s.m))};
-      const bf16x2_t c = __builtin_convertvector(two, bf16x2_t);
-      pb[ks][j] = c[0];
-      pb[ks][j + 1] = c[1];
+    for (int ks = 0; ks < 2; ++ks) {
+#pragma unroll
+      for (int j = 0; j < 8; j += 2) {
+        const f32x2_t two = {__builtin_amdgcn_exp2f(__builtin_fmaf(x[t][8 * ks + j], sl2, nm)),
+                             __builtin_amdgcn_exp2f(__builtin_fmaf(x[t][8 * ks + j + 1], sl2, nm))};
+        const bf16x2_t c = __builtin_convertvector(two, bf16x2_t);
+        pb[ks][j] = c[0];
+        pb[ks][j + 1] = c[1];
+      }
     }
-  }
-  typedef short i16x4_t __attribute__((ext_vector_type(4)));
-  typedef short i16x8_t __attribute__((ext_vector_type(8)));
-  const i16x4_t ones = {0x3F80, 0x3F80, 0x3F80, 0x3F80};
+    typedef short i16x4_t __attribute__((ext_vector_type(4)));
+    typedef short i16x8_t __attribute__((ext_vector_type(8)));
+    const i16x4_t ones = {0x3F80, 0x3F80, 0x3F80, 0x3F80};
 #pragma unroll
-  for (int ks = 0; ks < 2; ++ks) {
-    const i16x8_t p8 = __builtin_bit_cast(i16x8_t, pb[ks]);
-    s.l = __builtin_amdgcn_mfma_f32_4x4x4bf16_1k(ones, __builtin_shufflevector(p8, p8, 0, 1, 2, 3), s.l, 0, 0, 0);
-    s.l = __builtin_amdgcn_mfma_f32_4x4x4bf16_1k(ones, __builtin_shufflevector(p8, p8, 4, 5, 6, 7), s.l, 0, 0, 0);
-  }
-#pragma unroll
-  for (int ks = 0; ks < 2; ++ks) {
-    bf16x8_t va[DT];
-#pragma unroll
-    for (int j = 0; j < DT; ++j) {
-      typedef __bf16 bf16x4_t __attribute__((ext_vector_type(4)));
-      typedef __attribute__((address_space(3))) bf16x4_t lds_bf16x4_t;
-      char* at = const_cast<char*>(vp) + (j >> 1) * kSubBytes + rvt[j] + 16 * ks * kRow * 2;
-      const bf16x4_t lo = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((lds_bf16x4_t*)(at));
-      const bf16x4_t hi = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((lds_bf16x4_t*)(at + 4 * kRow * 2));
-      va[j] = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+    for (int ks = 0; ks < 2; ++ks) {
+      const i16x8_t p8 = __builtin_bit_cast(i16x8_t, pb[ks]);
+      s.l = __builtin_amdgcn_mfma_f32_4x4x4bf16_1k(ones, __builtin_shufflevector(p8, p8, 0, 1, 2, 3), s.l, 0, 0, 0);
+      s.l = __builtin_amdgcn_mfma_f32_4x4x4bf16_1k(ones, __builtin_shufflevector(p8, p8, 4, 5, 6, 7), s.l, 0, 0, 0);
     }
 #pragma unroll
-    for (int j = 0; j < DT; ++j) s.o[j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(va[j], pb[ks], s.o[j], 0, 0, 0);
+    for (int ks = 0; ks < 2; ++ks) {
+      bf16x8_t va[DT];
+#pragma unroll
+      for (int j = 0; j < DT; ++j) {
+        typedef __bf16 bf16x4_t __attribute__((ext_vector_type(4)));
+        typedef __attribute__((address_space(3))) bf16x4_t lds_bf16x4_t;
+        char* at = const_cast<char*>(vp) + (j >> 1) * kSubBytes + rvt[j] + (32 * t + 16 * ks) * kRow * 2;
+        const bf16x4_t lo = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((lds_bf16x4_t*)(at));
+        const bf16x4_t hi = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((lds_bf16x4_t*)(at + 4 * kRow * 2));
+        va[j] = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+      }
+#pragma unroll
+      for (int j = 0; j < DT; ++j) s.o[j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(va[j], pb[ks], s.o[j], 0, 0, 0);
+    }
   }
 }
 

@@ -21,29 +21,34 @@ __global__ __launch_bounds__(kPagedThreads, 2) void paged_row_kernel(PagedArgs a
   __shared__ float s_ml[4][2][kRows];
   const int lane = threadIdx.x & 63, col = lane & 31, hh = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  // The parts: an equal share of all keys for kRowTarget workgroups, a multiple of kRowLeast (4 waves' blocks). The lengths
-  // are on the device, so every workgroup forms the plan for itself.
+  // The parts: of the least length, a multiple of kRowLeast (4 waves' blocks), for which they are at most kRowTarget more than
+  // the (window, key head) pairs. The lengths are on the device, so every workgroup forms the plan for itself.
   auto keys_of = [&](int64_t c) __attribute__((always_inline)) -> int {  // -1: not of this form
     int64_t first, count;
     window_tokens(a.tokens, c, first, count);
     return count > 0 && row_form(a, count) ? static_cast<int>(held_keys(a.pages, c)) : -1;
   };
-  int64_t sum = 0;
+  int64_t sum = 0, units = 0;
   int mine = -1;
   for (int64_t c = lane; c < a.tokens.B; c += 64) {
     mine = keys_of(c);
     sum += mine > 0 ? mine : 0;
+    units += mine >= 0 ? 1 : 0;
   }
-  const int64_t share = cdiv(cdiv(wave_sum(sum) * a.Hkv, kRowTarget), kRowLeast) * kRowLeast;
-  const int each =
-      __builtin_amdgcn_readfirstlane(share < kUncut ? static_cast<int>(share < kRowLeast ? kRowLeast : share) : kUncut);
   const bool one = a.tokens.B <= 64;  // the lane's window is still at hand
-  auto count = [&](int c, int& tiles, int& parts) __attribute__((always_inline)) {
+  auto parts_of = [&](int c, int length) __attribute__((always_inline)) -> int {
     const int n = one ? mine : keys_of(c);
-    tiles = n >= 0 ? 1 : 0;
-    parts = n > each ? (n - 1) / each + 1 : 1;
+    return n < 0 ? 0 : (n > length ? (n - 1) / length + 1 : 1);
   };
-  const PagedItem item = item_at(a, static_cast<int>(blockIdx.x), count);
+  auto places = [&](int c, int length) __attribute__((always_inline)) { return a.Hkv * parts_of(c, length); };
+  const int target = static_cast<int>(wave_sum(units) * a.Hkv) + kRowTarget;
+  const int each = __builtin_amdgcn_readfirstlane(
+      part_length(a, wave_sum(sum) * a.Hkv, target, kRowLeast, kRowLeast, places));
+  const PagedItem item = item_at(a, static_cast<int>(blockIdx.x), [&](int c, int& tiles, int& parts)
+                                                                      __attribute__((always_inline)) {
+    parts = parts_of(c, each);
+    tiles = parts > 0 ? 1 : 0;
+  });
   const int b = __builtin_amdgcn_readfirstlane(item.b);
   if (b < 0) return;
   const int kvh = __builtin_amdgcn_readfirstlane(item.kvh), part = __builtin_amdgcn_readfirstlane(item.part);
@@ -186,13 +191,7 @@ __global__ __launch_bounds__(kPagedThreads, 2) void paged_row_kernel(PagedArgs a
           wait_vmem();
         }
       }
-#pragma unroll
-      for (int t = 0; t < kHalves; ++t) {
-        if (t == 0 || kv + 32 * t < k1) {
-          attend_half<KS, kSubBytes>(s, x[t], cur + 32 * t * kRow * 2, rvt, a.scale_log2, kv + 32 * t + 31 > all,
-                                     kv + 32 * t);
-        }
-      }
+      attend_block<KS, kSubBytes, kHalves>(s, x, cur, rvt, a.scale_log2, kv + kKeys - 1 > all, kv);
       kv = kvn;
       kvn += stride;
     };

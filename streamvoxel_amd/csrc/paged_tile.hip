@@ -41,11 +41,11 @@ __device__ __forceinline__ PagedItem whole_item(const PagedArgs& a) {
   return item;
 }
 
-// Otherwise the tiles stand one window after the other. Fewer than kTileTarget of them share out their keys: a part has the
-// blocks of an equal share of all for kTileTarget workgroups, at least kTileLeast, and an XCD takes a run of consecutive
-// places, so that the tiles of a part meet in its L2.
+// Otherwise the tiles stand one window after the other. Fewer than kTileTarget of them share out their keys: into parts of the
+// least number of blocks, kTileLeast at least, for which the parts are at most kTileTarget and run side by side. An XCD then
+// takes a run of consecutive places, so that the tiles of a part meet in its L2.
 __device__ __forceinline__ PagedItem shared_item(const PagedArgs& a, int& each) {
-  const int lane = threadIdx.x & 63;
+  const int lane = threadIdx.x & 63, Hkv = static_cast<int>(a.Hkv);
   int64_t units = 0, work = 0;
   int tiles = 0, blocks = 0;
   for (int64_t c = lane; c < a.tokens.B; c += 64) {
@@ -53,36 +53,35 @@ __device__ __forceinline__ PagedItem shared_item(const PagedArgs& a, int& each) 
     units += tiles;
     work += static_cast<int64_t>(tiles) * blocks;
   }
-  units = wave_sum(units) * a.Hkv;
-  work = wave_sum(work) * a.Hkv;
-  const bool split = units < kTileTarget;
-  const int64_t share = cdiv(work, kTileTarget);
-  each = __builtin_amdgcn_readfirstlane(
-      split && share < kUncut ? static_cast<int>(share < kTileLeast ? kTileLeast : share) : kUncut);
-  const bool one = a.tokens.B <= 64;  // the lane's window is still at hand
-  auto count = [&](int c, int& t, int& parts) __attribute__((always_inline)) {
+  units = wave_sum(units) * Hkv;
+  work = wave_sum(work) * Hkv;
+  const bool split = units < kTileTarget, one = a.tokens.B <= 64;  // one: the lane's window is still at hand
+  auto count = [&](int c, int length, int& t, int& parts) __attribute__((always_inline)) {
     int nb = blocks;
     t = tiles;
     if (!one) tiles_of_window(a, c, t, nb);
-    parts = nb > each ? (nb - 1) / each + 1 : 1;
+    parts = nb > length ? (nb - 1) / length + 1 : 1;
   };
+  auto places = [&](int c, int length) __attribute__((always_inline)) {
+    int t, parts;
+    count(c, length, t, parts);
+    return static_cast<int64_t>(t) * Hkv * parts;
+  };
+  each = split ? part_length(a, work, kTileTarget, 1, kTileLeast, places) : kUncut;
+  each = __builtin_amdgcn_readfirstlane(each);
   int at = static_cast<int>(blockIdx.x);
   if (split) {
     int64_t total = 0;
-    for (int64_t c = lane; c < a.tokens.B; c += 64) {
-      int t, parts;
-      count(static_cast<int>(c), t, parts);
-      total += t * parts;
-    }
-    const int run = static_cast<int>(cdiv(wave_sum(total) * a.Hkv, kXcds));
+    for (int64_t c = lane; c < a.tokens.B; c += 64) total += places(static_cast<int>(c), each);
+    const int run = static_cast<int>(cdiv(wave_sum(total), kXcds));
     if ((at >> 3) >= run) return PagedItem{-1, 0, 0, 1, 0, 1, 0, 0};
     at = (at & 7) * run + (at >> 3);
   }
-  return item_at(a, at, count);
+  return item_at(a, at, [&](int c, int& t, int& parts) __attribute__((always_inline)) { count(c, each, t, parts); });
 }
 
 template <bool FP8, bool WHOLE, int KS>
-__global__ __launch_bounds__(kPagedThreads, KS <= 4 ? 3 : 2) void paged_tile_kernel(PagedArgs a) {
+__global__ __launch_bounds__(kPagedThreads, FP8 || KS > 4 ? 2 : 4) void paged_tile_kernel(PagedArgs a) {
 #if defined(__HIP_DEVICE_COMPILE__)
   constexpr int DT = tiles_of(KS), ES = FP8 ? 1 : 2;
   constexpr int kSubBytes = kKB * kRow * 2, kTileBytes = Width<DT>::kSubTiles * kSubBytes;
@@ -165,17 +164,18 @@ __global__ __launch_bounds__(kPagedThreads, KS <= 4 ? 3 : 2) void paged_tile_ker
     }
   };
   auto compute = [&](int kv0, const char* sK, const char* sV) __attribute__((always_inline)) {
+    if (kv0 > any) return;
+    f32x16_t x[2];
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
-      const int key0 = kv0 + 32 * t;
-      if (key0 > any) break;
       bf16x8_t ka[KS];
 #pragma unroll
       for (int k = 0; k < KS; ++k) {
         ka[k] = *reinterpret_cast<const bf16x8_t*>(sK + (k >> 2) * kSubBytes + rd[k & 3] + 32 * t * kRow * 2);
       }
-      attend_half<KS, kSubBytes>(s, scores<KS>(s, ka), sV + 32 * t * kRow * 2, rvt, a.scale_log2, key0 + 31 > all, key0);
+      x[t] = scores<KS>(s, ka);
     }
+    attend_block<KS, kSubBytes, 2>(s, x, sV, rvt, a.scale_log2, kv0 + kKB - 1 > all, kv0);
   };
   if (blk0 < blk1) {
     find(kKB * blk0);
