@@ -11,7 +11,7 @@ constexpr int kRows = 32;          // rows of a wave
 constexpr int kTileRows = 128;     // rows of a tile workgroup
 constexpr int kTileTarget = 512;   // tile workgroups below which keys are split: two for every CU
 constexpr int kTileLeast = 6;      // least key blocks of a tile's part
-constexpr int kRowTarget = 512;    // row-form workgroups that all keys are shared out to
+constexpr int kRowTarget = 2048;   // row-form parts beyond one for each (window, key head)
 constexpr int kRowLeast = 256;     // keys that a row-form part has a multiple of
 constexpr int kWholePages = 64;    // pages from this size on hold whole blocks of keys
 constexpr int kUncut = 0x40000000; // a part length that cuts nothing

@@ -1,26 +1,54 @@
 // svhip_rotary: rotary positions of activations [B, H, N, D] (rotary.hpp), and with `inverse` the gradient: the transposed
 // rotation, sin negated.
 //
-// Bound: HBM, every element read and written once (3 operations each). Workgroup = (window, kRotaryTokens tokens), all
+// Bound: HBM, every element read and written once (3 operations each). Workgroup = (window, up to kRotaryTokens tokens), all
 // heads: the tile's (cos, sin) of every (token, pair) go to LDS once, since they are the same for every head, and a thread
-// then turns runs of 16 bytes; its first loads are in flight while the table is formed.
+// then turns pairs of 16-byte runs, kRotaryAhead of them in flight before the table is formed. Rows that are not made of such
+// runs (odd numbers of pairs, unaligned rows) go pair by pair.
 #include "rotary.hpp"
 
 namespace svhip {
 
 constexpr int kRotaryThreads = 256;
 constexpr int kRotaryTokens = 8;
+constexpr int kRotaryAhead = 2;
 
 struct RotaryArgs {
   const void* x;
   void* out;
   const void* positions;
   const double* freq;
-  int64_t B, H, N, D;
-  int half;
+  int64_t B, N, sx_b, sx_h, sx_n, so_b, so_h, so_n, sp_b, sp_n;
+  int H, D, half, tokens;  // tokens: of a workgroup
   bool wide, interleaved;
   float amplitude, sign;
-  int64_t sx_b, sx_h, sx_n, so_b, so_h, so_n, sp_b, sp_n;
+};
+
+// Elements of T in 16 bytes, as fp32.
+template <typename T>
+struct Run {
+  static constexpr int n = 16 / sizeof(T);
+  uint4 w;
+  __device__ __forceinline__ void load(const T* p) { w = *reinterpret_cast<const uint4*>(p); }
+  __device__ __forceinline__ void store(T* p) const { *reinterpret_cast<uint4*>(p) = w; }
+  __device__ __forceinline__ void get(float (&x)[n]) const {
+    const uint32_t u[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if constexpr (n == 4) {
+        x[i] = __uint_as_float(u[i]);
+      } else {
+        x[2 * i] = __uint_as_float(u[i] << 16);
+        x[2 * i + 1] = __uint_as_float(u[i] & 0xffff0000u);
+      }
+    }
+  }
+  __device__ __forceinline__ void set(const float (&x)[n]) {
+    uint32_t u[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) u[i] = n == 4 ? __float_as_uint(x[i]) : bf16_pack2(x[2 * i], x[2 * i + 1]);
+    w = make_uint4(u[0], u[1], u[2], u[3]);
+  }
 };
 
 template <typename T>
@@ -32,36 +60,118 @@ __device__ __forceinline__ void store_as(T* p, float v) {
   }
 }
 
-// An item is one pair, or one element past the pairs.
-template <typename T>
+// VEC: an item is Run::n pairs (two runs), or one run past the pairs; else one pair, or one element.
+template <typename T, bool VEC>
 __global__ __launch_bounds__(kRotaryThreads) void rotary_kernel(RotaryArgs a) {
   __shared__ float2 table[kRotaryTokens * kMaxRotaryPairs];
-  const int64_t tiles = cdiv(a.N, kRotaryTokens);
-  const int64_t b = blockIdx.x / tiles, n0 = (blockIdx.x % tiles) * kRotaryTokens;
-  const int tokens = static_cast<int>(a.N - n0 < kRotaryTokens ? a.N - n0 : kRotaryTokens);
+  constexpr int E = VEC ? Run<T>::n : 1, kAhead = VEC ? kRotaryAhead : 1;
+  const int64_t tiles = cdiv(a.N, a.tokens);
+  const int64_t b = blockIdx.x / tiles, n0 = (blockIdx.x - b * tiles) * a.tokens;
+  const int tokens = static_cast<int>(a.N - n0 < a.tokens ? a.N - n0 : a.tokens);
+  const T* x = static_cast<const T*>(a.x) + b * a.sx_b + n0 * a.sx_n;
+  T* out = static_cast<T*>(a.out) + b * a.so_b + n0 * a.so_n;
+  const int turning = a.half / E, per_row = turning + (a.D - 2 * a.half) / E;
+  // Item e of (token, head) row th = t H + h; kRotaryThreads items further on without a division.
+  int th = static_cast<int>(threadIdx.x) / per_row, e = static_cast<int>(threadIdx.x) - th * per_row;
+  int t = th / a.H, h = th - t * a.H;
+  const int step_th = kRotaryThreads / per_row, step_e = kRotaryThreads - step_th * per_row;
+  const int step_t = step_th / a.H, step_h = step_th - step_t * a.H;
+  auto advance = [&]() __attribute__((always_inline)) {
+    e += step_e;
+    h += step_h;
+    t += step_t;
+    if (e >= per_row) {
+      e -= per_row;
+      ++h;
+    }
+    if (h >= a.H) {
+      h -= a.H;
+      ++t;
+    }
+  };
+  struct Item {
+    int t, h, first, second, pair;  // elements of the two runs; pair < 0: one run, kept
+    Run<T> u, v;
+    float p, q;
+  };
+  Item items[kAhead];
+  auto load = [&](Item& it) __attribute__((always_inline)) {
+    it.t = t;
+    it.h = h;
+    it.pair = e < turning ? E * e : -1;
+    it.first = e < turning ? (a.interleaved ? 2 * E * e : E * e) : 2 * a.half + E * (e - turning);
+    it.second = e < turning ? (a.interleaved ? it.first + E : a.half + E * e) : it.first;
+    if (t < tokens) {
+      const T* row = x + h * a.sx_h + t * a.sx_n;
+      if constexpr (VEC) {
+        it.u.load(row + it.first);
+        it.v.load(row + it.second);
+      } else {
+        it.p = to_float<T>(row[it.first]);
+        it.q = to_float<T>(row[it.second]);
+      }
+    }
+    advance();
+  };
+#pragma unroll
+  for (int i = 0; i < kAhead; ++i) load(items[i]);
   for (int i = threadIdx.x; i < tokens * a.half; i += kRotaryThreads) {
-    const int t = i / a.half, pr = i - t * a.half;
-    const double p = rotary_position(a.positions, a.wide, b * a.sp_b + (n0 + t) * a.sp_n);
-    float2 r = rotary_phase(p, a.freq[pr], a.amplitude);
+    const int row = i / a.half, pr = i - row * a.half;
+    float2 r = rotary_phase(rotary_position(a.positions, a.wide, b * a.sp_b + (n0 + row) * a.sp_n), a.freq[pr], a.amplitude);
     r.y *= a.sign;
     table[i] = r;
   }
   __syncthreads();
-  const int per_row = static_cast<int>(a.D) - a.half, H = static_cast<int>(a.H);
-  for (int64_t i = threadIdx.x; i < static_cast<int64_t>(tokens) * H * per_row; i += kRotaryThreads) {
-    const int e = static_cast<int>(i % per_row), th = static_cast<int>(i / per_row);
-    const int h = th % H, t = th / H;
-    const T* src = static_cast<const T*>(a.x) + b * a.sx_b + h * a.sx_h + (n0 + t) * a.sx_n;
-    T* dst = static_cast<T*>(a.out) + b * a.so_b + h * a.so_h + (n0 + t) * a.so_n;
-    if (e < a.half) {
-      const int i0 = a.interleaved ? 2 * e : e, i1 = a.interleaved ? 2 * e + 1 : e + a.half;
-      float u = to_float<T>(src[i0]), v = to_float<T>(src[i1]);
-      rotary_turn(u, v, table[t * a.half + e]);
-      store_as<T>(dst + i0, u);
-      store_as<T>(dst + i1, v);
-    } else {
-      dst[e + a.half] = src[e + a.half];
+  while (items[0].t < tokens) {
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) {
+      Item& it = items[i];
+      if (it.t >= tokens) break;
+      T* row = out + it.h * a.so_h + it.t * a.so_n;
+      const float2* angle = table + it.t * a.half + it.pair;
+      if constexpr (VEC) {
+        if (it.pair < 0) {
+          it.u.store(row + it.first);
+          continue;
+        }
+        float p[E], q[E];
+        it.u.get(p);
+        it.v.get(q);
+        if (a.interleaved) {
+#pragma unroll
+          for (int j = 0; j < E; j += 2) {
+            rotary_turn(p[j], p[j + 1], angle[j / 2]);
+            rotary_turn(q[j], q[j + 1], angle[(E + j) / 2]);
+          }
+        } else {
+#pragma unroll
+          for (int j = 0; j < E; ++j) rotary_turn(p[j], q[j], angle[j]);
+        }
+        it.u.set(p);
+        it.v.set(q);
+        it.u.store(row + it.first);
+        it.v.store(row + it.second);
+      } else {
+        float p = it.p, q = it.q;
+        if (it.pair >= 0) {
+          rotary_turn(p, q, angle[0]);
+          store_as<T>(row + it.second, q);
+        }
+        store_as<T>(row + it.first, p);
+      }
     }
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) load(items[i]);
+  }
+}
+
+template <typename T>
+void launch_rotary(const RotaryArgs& a, bool vec, hipStream_t s) {
+  const unsigned grid = static_cast<unsigned>(a.B * cdiv(a.N, a.tokens));
+  if (vec) {
+    rotary_kernel<T, true><<<grid, kRotaryThreads, 0, s>>>(a);
+  } else {
+    rotary_kernel<T, false><<<grid, kRotaryThreads, 0, s>>>(a);
   }
 }
 
@@ -84,16 +194,22 @@ extern "C" int svhip_rotary(const svhip_rotary_args* args, void* stream) {
   SVHIP_REQUIRE(c.D <= 1 << 20 && c.H <= 1 << 20, "%s: sizes too large", name);
   if (c.B == 0 || c.H == 0 || c.N == 0) return SVHIP_OK;
   SVHIP_REQUIRE(c.x && c.out && c.positions && c.freq, "%s: null pointer", name);
-  const int64_t grid = c.B * cdiv(c.N, kRotaryTokens);
-  SVHIP_REQUIRE(grid < (1ll << 31), "%s: grid too large", name);
-  const RotaryArgs a{c.x, c.out, c.positions, c.freq, c.B, c.H, c.N, c.D, static_cast<int>(c.pairs),
-                     c.positions_wide != 0, c.layout == SVHIP_ROTARY_INTERLEAVED, static_cast<float>(c.amplitude),
-                     c.inverse ? -1.f : 1.f, c.sx_b, c.sx_h, c.sx_n, c.so_b, c.so_h, c.so_n, c.sp_b, c.sp_n};
+  // Few tokens: one for each workgroup, so that they fill the chip.
+  const int64_t tokens = c.B * c.N <= 2 * 256 ? 1 : kRotaryTokens;
+  SVHIP_REQUIRE(c.B * cdiv(c.N, tokens) < (1ll << 31), "%s: grid too large", name);
+  const RotaryArgs a{c.x, c.out, c.positions, c.freq, c.B, c.N, c.sx_b, c.sx_h, c.sx_n, c.so_b, c.so_h, c.so_n, c.sp_b,
+                     c.sp_n, static_cast<int>(c.H), static_cast<int>(c.D), static_cast<int>(c.pairs),
+                     static_cast<int>(tokens), c.positions_wide != 0, c.layout == SVHIP_ROTARY_INTERLEAVED,
+                     static_cast<float>(c.amplitude), c.inverse ? -1.f : 1.f};
+  const int64_t run = c.dtype == SVHIP_F32 ? 4 : 8;
+  const bool vec = c.pairs % run == 0 && c.D % run == 0 && reinterpret_cast<uintptr_t>(c.x) % 16 == 0 &&
+                   reinterpret_cast<uintptr_t>(c.out) % 16 == 0 &&
+                   (c.sx_b | c.sx_h | c.sx_n | c.so_b | c.so_h | c.so_n) % run == 0;
   hipStream_t s = as_stream(stream);
   if (c.dtype == SVHIP_F32) {
-    rotary_kernel<float><<<static_cast<unsigned>(grid), kRotaryThreads, 0, s>>>(a);
+    launch_rotary<float>(a, vec, s);
   } else {
-    rotary_kernel<uint16_t><<<static_cast<unsigned>(grid), kRotaryThreads, 0, s>>>(a);
+    launch_rotary<uint16_t>(a, vec, s);
   }
   SVHIP_LAUNCHED(name);
   return SVHIP_OK;
