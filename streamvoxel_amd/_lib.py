@@ -5,7 +5,6 @@ call fails, a RuntimeError is raised.
 """
 from __future__ import annotations
 
-import contextlib
 import ctypes
 import os
 import threading
@@ -148,11 +147,18 @@ def require_one_gpu(first, *tensors):
         require_gpu(first, *tensors)
 
 
-def device_of(t):
-    """A context in which launches go to the tensor's device, whatever the current one is."""
-    if t.device.index == torch.cuda.current_device():
-        return contextlib.nullcontext()
-    return torch.cuda.device(t.device)
+def launch(name, t, *args):
+    """The entry point `name` with args and the current stream of the tensor's device, launched on that device whatever the
+    current one is; RuntimeError for a status."""
+    fn, index = getattr(load(), name), t.get_device()
+    stream = torch._C._cuda_getCurrentRawStream(index)   # what current_stream(index).cuda_stream is, in a tenth of the time
+    if index == torch.cuda.current_device():
+        rc = fn(*args, stream)
+    else:
+        with torch.cuda.device(index):
+            rc = fn(*args, stream)
+    if rc:
+        check(rc, name)
 
 
 def dtype_code(dtype):

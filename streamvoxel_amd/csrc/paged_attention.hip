@@ -131,11 +131,14 @@ inline PagedPlan paged_plan(int64_t B, int64_t H, int64_t Hkv, int64_t N, bool p
     }
   }
   if (p.rows) {
-    p.row_slots = kRowTarget + B * Hkv;
+    // One for each (window, key head), and the parts: at most kRowTarget more, and no shorter than kRowLeast.
+    const int64_t more = B * Hkv * (cdiv(max_keys, kRowLeast) - 1);
+    p.row_parts = more > 0;
+    p.row_slots = (more < 0 ? 0 : (more < kRowTarget ? more : kRowTarget)) + B * Hkv;
     p.slot_rows = packed ? (N * G < kRows ? N * G : kRows) : N * G;
-    p.row_floats = (p.row_slots * p.slot_rows * (D + 2) + 3) / 4 * 4;
+    if (p.row_parts) p.row_floats = (p.row_slots * p.slot_rows * (D + 2) + 3) / 4 * 4;
   }
-  p.plan_windows = p.rows || p.split ? B : 0;
+  p.plan_windows = p.row_parts || p.split ? B : 0;
   return p;
 }
 

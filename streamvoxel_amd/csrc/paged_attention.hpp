@@ -36,7 +36,7 @@ struct PagedArgs {
   int row_slots, tile_slots;  // slots of parts at most
   int slot_rows;        // rows of a row-form slot
   float *row_part, *tile_part;
-  int4* plan;           // a window's first slot, its parts, a part's length (tiles: blocks) and its tiles
+  int4* plan;           // (null: no parts) a window's first slot, its parts, a part's length (tiles: blocks) and its tiles
 };
 
 // The window as a workgroup sees it.
@@ -430,7 +430,7 @@ __device__ __forceinline__ void commit_rows8(const Staged<DT, kLoads>& st, int i
 
 // What a call launches, by its sizes alone.
 struct PagedPlan {
-  bool rows, tiles, split;  // the forms that its windows may take, and whether tiles may be split
+  bool rows, tiles, row_parts, split;  // the forms that its windows may take, and which may be cut into parts
   int q_tiles;
   int64_t tile_grid, tile_slots, row_slots, slot_rows, row_floats, tile_floats, plan_windows;
   size_t bytes() const { return static_cast<size_t>(row_floats + tile_floats) * 4 + static_cast<size_t>(plan_windows) * 16; }

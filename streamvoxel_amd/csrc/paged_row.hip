@@ -53,7 +53,7 @@ __global__ __launch_bounds__(kPagedThreads, 2) void paged_row_kernel(PagedArgs a
   if (b < 0) return;
   const int kvh = __builtin_amdgcn_readfirstlane(item.kvh), part = __builtin_amdgcn_readfirstlane(item.part);
   const int parts = __builtin_amdgcn_readfirstlane(item.parts);
-  if (part == 0 && kvh == 0 && threadIdx.x == 0) a.plan[b] = make_int4(item.before, parts, each, 1);
+  if (a.plan && part == 0 && kvh == 0 && threadIdx.x == 0) a.plan[b] = make_int4(item.before, parts, each, 1);
   const Window w = window_at(a, b);
   const int rows = static_cast<int>(w.count * a.G);
   const int keys = __builtin_amdgcn_readfirstlane(w.keys);

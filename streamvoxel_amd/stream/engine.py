@@ -25,9 +25,11 @@ from typing import NamedTuple
 import torch
 
 from streamvoxel_amd.stream.forward import StepForward
+from streamvoxel_amd.stream.paged import PagedContext
 from streamvoxel_amd.stream.step import CachedContext
 
-__all__ = ['Encoded', 'StepGraphs', 'SlotEngine', 'condition_widths', 'write_condition', 'RECOMMENDED']
+__all__ = ['Encoded', 'StepGraphs', 'SlotEngine', 'condition_widths', 'write_condition', 'extend_condition',
+           'RECOMMENDED']
 
 # The reference's recommended options (fast_ops.py:35); every combination runs the same kernels here.
 RECOMMENDED = dict(patchify='gather', attention='flex', compile='emulate')
@@ -86,19 +88,32 @@ def write_condition(model, context, index, enc):
     """Every layer's cache entry of slot `index` of `context` (FastSlotForward.encode + _write, fast_ops.py:228-250):
     local K / V = the layer's key_value projection of `enc.local` (bf16 autocast, as the reference's), local K
     rotated at `enc.positions` by `svhip_kv_write`, the prefix rows first, zeros to the capacity."""
-    dev = context.lengths.device
-    local = enc.local.to(dev)
-    positions = enc.positions.to(device=dev, dtype=torch.float32)[0]
+    positions = enc.positions.to(device=context.lengths.device, dtype=torch.float32)[0]
+    for j, (cross, key, value) in enumerate(_local_kv(model, context, enc.local)):
+        pk, pv = enc.prefix[j]
+        context.write(j, index, key, value, prefix=(pk, pv), positions=positions, frequencies=cross.rope.frequencies)
+
+
+def _local_kv(model, context, local):
+    """(layer, K, V) of every cross-attention layer, [H, L, D] views of its key_value projection of `local` [1, L, W]."""
+    local = local.to(context.lengths.device)
     L = local.shape[1]
-    with torch.autocast('cuda', dtype=torch.bfloat16):
-        for j, cross in enumerate(model.cross):
-            H = int(cross.heads)
-            D = int(cross.width) // H
-            kv = cross.key_value(local[0]).to(torch.bfloat16).view(L, 2, H, D)
-            key, value = kv[:, 0].transpose(0, 1), kv[:, 1].transpose(0, 1)      # [H, L, D] views
-            pk, pv = enc.prefix[j]
-            context.write(j, index, key, value, prefix=(pk, pv), positions=positions,
-                          frequencies=cross.rope.frequencies)
+    for cross in model.cross:
+        H = int(cross.heads)
+        with torch.autocast('cuda', dtype=torch.bfloat16):
+            kv = cross.key_value(local[0]).to(torch.bfloat16).view(L, 2, H, int(cross.width) // H)
+        yield cross, kv[:, 0].transpose(0, 1), kv[:, 1].transpose(0, 1)
+
+
+def extend_condition(model, context, index, local, positions):
+    """Further local context of slot `index` behind what a PagedContext holds of it: `local` [1, L, W] projected by every layer,
+    the keys rotated at `positions` [1, L, 3]; nothing that is there is written again."""
+    L = local.shape[1]
+    positions = positions.to(device=context.lengths.device, dtype=torch.float32)[0].contiguous()
+    context.resize(index, context.host_lengths[index] + L)
+    for j, (cross, key, value) in enumerate(_local_kv(model, context, local)):
+        freq = cross.rope.frequencies.to(device=positions.device, dtype=torch.float32)
+        context.append(j, key, value, index=index, positions=positions, frequencies=freq, layout='axial')
 
 
 class StepGraphs:
@@ -181,7 +196,9 @@ class SlotEngine:
     item into the condition (for the reference's model: `lambda item: encode_item(model, item, spec, device)`, which
     `default_encoder` supplies when none is passed and the reference's package is importable); without one,
     `load_slot` takes an `Encoded` (or a (prefix, local, positions) tuple) itself.
-    `kv_dtype` 'bf16' (the reference's cache) or 'fp8' (e4m3 with per-(window, head) scales). `concurrent` runs the
+    `kv_dtype` 'bf16' (the reference's cache) or 'fp8' (e4m3 with per-(window, head) scales). `pages`: the slots share a pool
+    of that many pages of `page_size` keys (a `PagedContext`, e4m3 with a scale a row) in place of a slab of the longest
+    condition each; a slot's context can then grow (`extend_slot`). `concurrent` runs the
     control branch on its own stream inside the step. `patchify`, `attention` and `compile` are the reference's
     option names (fast_ops.py:168-171): 'gather' and 'conv' both run the HIP gather patchify, bit for bit the
     reference's embedding-bag form, which computes the one-hot Conv3d's sum (the reference's own test,
@@ -190,7 +207,8 @@ class SlotEngine:
     changes nothing (the blocks run on HIP kernels that round where eager autocast does)."""
 
     def __init__(self, model, spec, device, batch, l1_cap, l2_cap, *, patchify='gather', attention='flex',
-                 compile=False, capture=True, encoder=None, kv_dtype='bf16', concurrent=True):
+                 compile=False, capture=True, encoder=None, kv_dtype='bf16', concurrent=True, pages=None,
+                 page_size=64):
         check_engine_options(patchify, attention, compile, kv_dtype)
         self.device = torch.device(device)
         if self.device.type != 'cuda':
@@ -211,8 +229,13 @@ class SlotEngine:
         cross = model.cross[0]
         heads = int(cross.heads)
         dev = self.device
-        self.context = CachedContext(len(model.cross), self.batch, heads, int(cross.width) // heads,
-                                     self.prefix_len + self.local_len, dev, kv_dtype)
+        capacity = self.prefix_len + self.local_len
+        if pages is None:
+            self.context = CachedContext(len(model.cross), self.batch, heads, int(cross.width) // heads, capacity, dev,
+                                         kv_dtype)
+        else:
+            self.context = PagedContext(len(model.cross), self.batch, heads, int(cross.width) // heads, int(pages), dev,
+                                        page_size, max(1, -(-capacity // page_size)), kv_dtype)
         self.forward_fn = StepForward(model, self.context, concurrent=concurrent)
         self.tokens = torch.full((self.batch, *self.shape), self.classes, dtype=torch.int64, device=dev)
         self.timestep = torch.ones(self.batch, dtype=torch.float32, device=dev)
@@ -275,6 +298,25 @@ class SlotEngine:
                     t.record_stream(self.side)
             write_condition(self.model, self.context, index, enc)
             self.tokens[index].fill_(self.classes)
+
+    @torch.inference_mode()
+    def extend_slot(self, index, local, positions):
+        """Slot `index` of a paged engine takes further local context (`local` [1, L, W], `positions` [1, L, 3]) behind the
+        condition that it holds, on the side stream like `load_slot`: a neighbour that has come in costs its own keys, not
+        the window's. The slot's tokens stay."""
+        index = int(index)
+        if not isinstance(self.context, PagedContext):
+            raise ValueError('extending a slot needs an engine with pages')
+        if not 0 <= index < self.batch:
+            raise IndexError(f'slot {index} of {self.batch}')
+        if local.dim() != 3 or local.shape[0] != 1 or positions.shape != (1, local.shape[1], 3):
+            raise ValueError('local must be [1, L, W] with positions [1, L, 3]')
+        self.side.wait_stream(torch.cuda.current_stream(self.device))
+        with torch.cuda.stream(self.side):
+            for t in (local, positions):
+                if t.is_cuda:
+                    t.record_stream(self.side)
+            extend_condition(self.model, self.context, index, local, positions)
 
     def wait_loads(self):
         torch.cuda.current_stream(self.device).wait_stream(self.side)

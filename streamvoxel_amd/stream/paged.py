@@ -142,8 +142,7 @@ def paged_append(key, value, k_pages, v_pages, page_table, lengths, cu_tokens=No
     args = _APPEND.pack(key.data_ptr(), value.data_ptr(), _address(cu_tokens), _address(positions), _address(frequencies),
                         n, before, *sk, *sv, turn, wide, *sp, pairs, amplitude)
     cache = _packed(code, k_pages, v_pages, page_table, lengths, k_exponents, v_exponents, bad)
-    with _lib.device_of(key):
-        _lib.check(_lib.load().svhip_paged_append(cache, args, _lib.stream_of(key)), 'svhip_paged_append')
+    _lib.launch('svhip_paged_append', key, cache, args)
 
 
 def paged_attention(query, k_pages, v_pages, page_table, lengths, cu_queries=None, causal=False, scale=None,
@@ -169,18 +168,166 @@ def paged_attention(query, k_pages, v_pages, page_table, lengths, cu_queries=Non
     if query.shape[-1] != D or Hkv == 0 or H % Hkv:
         raise ValueError("query needs the pages' head_dim, and heads that share theirs evenly")
     if out is None:
-        out = torch.empty(query.shape, dtype=torch.bfloat16, device=query.device)
-    if out.shape != query.shape or out.dtype != torch.bfloat16 or out.stride(-1) != 1:
+        out = torch.empty_like(query)
+    elif out.shape != query.shape or out.dtype != torch.bfloat16 or out.stride(-1) != 1:
         raise ValueError('out must be bf16 like query with a contiguous head_dim')
     so = _windows(out, cu_queries, B, 'out')[2]
     scale = 1.0 / math.sqrt(D) if scale is None else float(scale)
-    lib = _lib.load()
-    m = page_table.shape[1]
-    nbytes = int(lib.svhip_paged_attention_workspace_bytes(B, H, Hkv, n, cu_queries is not None, D, m * S))
+    nbytes = _lib.load().svhip_paged_attention_workspace_bytes(B, H, Hkv, n, cu_queries is not None, D,
+                                                               page_table.shape[1] * S)
     cache = _packed(code, k_pages, v_pages, page_table, lengths, k_exponents, v_exponents, bad)
-    with _lib.device_of(query):
-        ws = torch.empty(nbytes, dtype=torch.uint8, device=query.device) if nbytes else None
-        args = _ATTEND.pack(query.data_ptr(), out.data_ptr(), _address(cu_queries), _address(ws), nbytes, H, n, *sq, *so,
-                            causal, scale)
-        _lib.check(lib.svhip_paged_attention(cache, args, _lib.stream_of(query)), 'svhip_paged_attention')
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=query.device) if nbytes else None
+    args = _ATTEND.pack(query.data_ptr(), out.data_ptr(), _address(cu_queries), _address(ws), nbytes, H, n, *sq, *so, causal,
+                        scale)
+    _lib.launch('svhip_paged_attention', query, cache, args)
     return out
+
+
+class PagedContext:
+    """The cached keys and values of `batch` windows in one pool of `pages` pages a layer (each `page_size` keys of every head),
+    in `CachedContext`'s place: `write`, `attend`, `lengths` as there, and windows that grow (`grow`, `append`) and give
+    their pages back (`release`). A window holds as many pages as its keys need, at most `max_pages` of them (default: all).
+    kv_dtype 'bf16' or 'fp8' (OCP e4m3fn with one power of two for each row and head).
+
+    The host keeps the books: `resize` and `grow` take and free pages and send table and lengths to the device on the current
+    stream without waiting for it; calls that touch a window's pages must be ordered after them, as usual. A replayed graph
+    reads the table and the lengths as they stand. `bad` (device int32 [1]) becomes non-zero when a call meets a page outside
+    the pool, which these books never name."""
+
+    def __init__(self, layers, batch, heads, head_dim, pages, device, page_size=64, max_pages=None, kv_dtype='bf16'):
+        if kv_dtype not in ('bf16', 'fp8'):
+            raise ValueError("kv_dtype must be 'bf16' or 'fp8'")
+        if page_size not in (16, 32, 64, 128, 256, 512, 1024):
+            raise ValueError('page_size must be a power of two from 16 to 1024')
+        if head_dim < 8 or head_dim > 128 or head_dim % 8:
+            raise ValueError('head_dim must be a multiple of 8 up to 128')
+        if layers < 1 or batch < 1 or heads < 1 or pages < 1 or (max_pages is not None and max_pages < 1):
+            raise ValueError('layers, batch, heads, pages and max_pages must be positive')
+        self.layers, self.batch, self.heads, self.head_dim = layers, batch, heads, head_dim
+        self.pages, self.page_size, self.kv_dtype = pages, page_size, kv_dtype
+        self.max_pages = pages if max_pages is None else max_pages
+        dt = torch.bfloat16 if kv_dtype == 'bf16' else torch.float8_e4m3fn
+        pool = lambda dtype, *shape: [torch.empty(pages, heads, page_size, *shape, dtype=dtype, device=device)
+                                      for _ in range(layers)]
+        self.k, self.v = pool(dt, head_dim), pool(dt, head_dim)
+        none = [None] * layers
+        self.k_exponents, self.v_exponents = (pool(torch.uint8), pool(torch.uint8)) if kv_dtype == 'fp8' else (none, none)
+        self.table = torch.zeros(batch, self.max_pages, dtype=torch.int32, device=device)
+        self.lengths = torch.zeros(batch, dtype=torch.int32, device=device)
+        self.bad = torch.zeros(1, dtype=torch.int32, device=device)
+        self.host_lengths = [0] * batch
+        self._owned = [[] for _ in range(batch)]
+        self._free = list(range(pages - 1, -1, -1))
+
+    @property
+    def free_pages(self):
+        return len(self._free)
+
+    def _pages_for(self, length):
+        return -(-length // self.page_size)
+
+    def _set(self, wanted):
+        """The windows' lengths {index: length}: pages taken and freed, table and lengths sent. Nothing changes on error."""
+        need = 0
+        for index, length in wanted.items():
+            if not 0 <= index < self.batch:
+                raise IndexError(f'window {index} of {self.batch}')
+            if length < 0:
+                raise ValueError('a window holds 0 keys or more')
+            if self._pages_for(length) > self.max_pages:
+                raise ValueError('Condition exceeds the slot capacity')
+            need += self._pages_for(length) - len(self._owned[index])
+        if need > len(self._free):
+            raise RuntimeError(f'the pool has {len(self._free)} pages left, {need} more are needed')
+        moved = []
+        for index, length in wanted.items():          # freed pages first: another window may take them
+            own, n = self._owned[index], self._pages_for(length)
+            if n != len(own):
+                moved.append(index)
+            self._free.extend(reversed(own[n:]))
+            del own[n:]
+        for index, length in wanted.items():
+            own, n = self._owned[index], self._pages_for(length)
+            own.extend(self._free.pop() for _ in range(n - len(own)))
+            self.host_lengths[index] = length
+        for index in moved:
+            self._send(self.table[index, :len(self._owned[index])], self._owned[index])
+        self._send(self.lengths, self.host_lengths)
+
+    @staticmethod
+    def _send(to, values):
+        """Host numbers to the device on the current stream, not waited for: one by a fill, more from pinned memory (which
+        the allocator keeps until the copy is done)."""
+        if len(values) == 1:
+            to.fill_(values[0])
+        elif values:
+            to.copy_(torch.tensor(values, dtype=torch.int32, pin_memory=True), non_blocking=True)
+
+    def resize(self, index, length):
+        """Window `index` holds `length` keys: pages taken or given back at its end (the keys below both lengths stay)."""
+        self._set({int(index): int(length)})
+
+    def release(self, index):
+        """Window `index` gives its pages back."""
+        self.resize(index, 0)
+
+    def grow(self, counts):
+        """Every window grows by counts[b] keys (or all by one number), to be written by `append`."""
+        counts = [int(counts)] * self.batch if isinstance(counts, int) else [int(c) for c in counts]
+        if len(counts) != self.batch or min(counts) < 0:
+            raise ValueError(f'counts must be {self.batch} numbers, 0 or more')
+        self._set({b: self.host_lengths[b] + c for b, c in enumerate(counts)})
+
+    def _rows(self, t):
+        t = t.to(device=self.lengths.device, dtype=torch.bfloat16)
+        return t if t.stride(-1) == 1 else t.contiguous()
+
+    def append(self, layer, key, value, index=None, n=None, cu_tokens=None, **how):
+        """`paged_append` into layer `layer` of the first n windows (all by default), or of window `index` alone (key, value
+        [heads, L, head_dim] then); `how`: its before, positions, frequencies, layout, amplitude."""
+        at = slice(0, self.batch if n is None else n)
+        if index is not None:
+            at, key, value = slice(index, index + 1), key[None], value[None]
+            if how.get('positions') is not None:
+                how['positions'] = how['positions'][None]
+        paged_append(key, value, self.k[layer], self.v[layer], self.table[at], self.lengths[at], cu_tokens=cu_tokens,
+                     k_exponents=self.k_exponents[layer], v_exponents=self.v_exponents[layer], bad=self.bad, **how)
+
+    def write(self, layer, index, key, value, prefix=None, positions=None, frequencies=None):
+        """Window `index` of `layer` anew, as `CachedContext.write`: keys [0, P) from `prefix` = (prefix_k, prefix_v) [H, P, D]
+        (already rotated), keys [P, P + L) from key, value [H, L, D] (K rotated by AxialRoPE at fp32 positions [L, 3] with
+        the fp32 `frequencies` buffer when given). Sets the window's length and pages."""
+        _lib.require_gpu(key, value)
+        key, value = self._rows(key), self._rows(value)
+        H, L, D = key.shape
+        if H != self.heads or D != self.head_dim or value.shape != key.shape:
+            raise ValueError('key / value must be [heads, L, head_dim] like the cache')
+        P = 0
+        if prefix is not None:
+            pk, pv = self._rows(prefix[0]), self._rows(prefix[1])
+            if pk.shape[0] != H or pk.shape[2] != D or pv.shape != pk.shape:
+                raise ValueError('prefix K / V must be [heads, P, head_dim]')
+            P = pk.shape[1]
+        how = {}
+        if positions is not None:
+            if frequencies is None:
+                raise ValueError('rotating the local keys needs the AxialRoPE frequencies')
+            dev = self.lengths.device
+            how = dict(positions=positions.to(device=dev, dtype=torch.float32).contiguous(), layout='axial',
+                       frequencies=frequencies.to(device=dev, dtype=torch.float32).contiguous())
+            if how['positions'].shape != (L, 3):
+                raise ValueError('positions must be [L, 3]')
+        if self.host_lengths[index] != P + L:
+            self.resize(index, P + L)
+        if P:
+            self.append(layer, pk, pv, index=index, before=L)
+        if L:
+            self.append(layer, key, value, index=index, **how)
+
+    def attend(self, layer, query, out=None, n=None, cu_queries=None, causal=False):
+        """Attention of `query` [n,H,Q,D] bf16 (H a multiple of the cache's heads; packed [H,T,D] with cu_queries) over the keys
+        of the first n windows."""
+        n = self.batch if n is None else n
+        return paged_attention(query, self.k[layer], self.v[layer], self.table[:n], self.lengths[:n], cu_queries=cu_queries,
+                               causal=causal, out=out, k_exponents=self.k_exponents[layer],
+                               v_exponents=self.v_exponents[layer], bad=self.bad)

@@ -55,8 +55,7 @@ def _launch(x, out, positions, frequencies, layout, amplitude, inverse):
                       _lib.dtype_code(x.dtype), positions.dtype == torch.int64, frequencies.numel(), LAYOUTS[layout],
                       inverse, *x.shape, *x.stride()[:3], *out.stride()[:3],
                       positions.stride(0) if positions.dim() == 2 else 0, positions.stride(-1), amplitude)
-    with _lib.device_of(x):
-        _lib.check(_lib.load().svhip_rotary(args, _lib.stream_of(x)), 'svhip_rotary')
+    _lib.launch('svhip_rotary', x, args)
     return out
 
 

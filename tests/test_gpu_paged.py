@@ -523,3 +523,171 @@ def test_calls_on_two_streams_and_in_a_graph(n):
             got = out.clone()
             paged_attention(queries(2, 2, 9, 64, i), k, v, table[:2], lengths[:2])
             assert torch.equal(got, step())
+
+
+# ------------------------------------------------------------------------------------------------ together, in use
+
+@pytest.mark.parametrize('kv_dtype', ['bf16', 'fp8'])
+@pytest.mark.parametrize('layout', ['half', 'interleaved'])
+def test_a_sequence_in_chunks_and_tokens(kv_dtype, layout):
+    """Rotated queries over a cache that grows by chunks and single tokens, against float64 attention of the whole sequences.
+    On top of the attention's own error: rotated queries and keys are rounded once (bf16 2^-8; an e4m3 key and value 2^-4 of
+    itself or 2^-10 of its row's power of two). A score is then off by scale times the queries' and keys' errors against
+    each other, which moves the weights of a row by twice the largest of its row, and a value enters with its own."""
+    from streamvoxel_amd.stream.paged import PagedContext
+    from streamvoxel_amd.stream.rotary import rotary, rotary_frequencies
+    H, heads, D, lengths = 4, 2, 64, [90, 33]
+    freq, amplitude = rotary_frequencies(48, scaling='wavelength', factor=4.0, original_length=64, device=DEV)
+    ctx = PagedContext(1, 2, heads, D, pages=12, device=DEV, page_size=16, kv_dtype=kv_dtype)
+    g = torch.Generator().manual_seed(8)
+    q, k, v = [torch.randn(2, n, 90, D, generator=g).to(torch.bfloat16) for n in (H, heads, heads)]
+    chunks = [(30, 10), (1, 1), (40, 0), (1, 1), (1, 1), (16, 19), (1, 1)]
+    done = [0, 0]
+    got = [[], []]
+    for counts in chunks:
+        ctx.grow(counts)
+        cut = lambda t, b: t[b, :, done[b]:done[b] + counts[b]]
+        pack = lambda t: torch.cat([cut(t, 0), cut(t, 1)], 1).to(DEV)
+        cu = torch.tensor([0, counts[0], sum(counts)], dtype=torch.int32, device=DEV)
+        where = torch.cat([torch.arange(done[b], done[b] + counts[b]) for b in range(2)]).to(DEV)
+        how = dict(frequencies=freq, layout=layout, amplitude=amplitude)
+        ctx.append(0, pack(k), pack(v), cu_tokens=cu, **how)
+        turned = rotary(pack(q)[None], where, freq, layout, amplitude)[0]
+        out = ctx.attend(0, turned, cu_queries=cu, causal=True)
+        for b, o in enumerate(out.split(list(counts), 1)):
+            got[b].append(o)
+        done = [d + c for d, c in zip(done, counts)]
+    assert ctx.host_lengths == ctx.lengths.tolist() == done and int(ctx.bad) == 0
+    for b, L in enumerate(done):
+        out = torch.cat(got[b], 1).cpu().double()
+        where = torch.arange(L)
+        tq, eq = turned64(q[b, :, :L].transpose(0, 1).double(), where, freq.cpu(), layout, amplitude)
+        tk, ek = turned64(k[b, :, :L].transpose(0, 1).double(), where, freq.cpu(), layout, amplitude)
+        value = v[b, :, :L].double()
+        eq = (eq + 2.0 ** -8 * (tq.abs() + eq)).transpose(0, 1)
+        if kv_dtype == 'bf16':
+            ek, ev = ek + 2.0 ** -8 * (tk.abs() + ek), torch.zeros_like(value)
+        else:
+            step = lambda x, reach: 2.0 ** -10 * 2.0 ** (exponent64(reach * x.float().abs().amax(-1)) - 127)[..., None]
+            ek = ek + torch.maximum(2.0 ** -4 * (tk.abs() + ek), step(k[b, :, :L].transpose(0, 1), 1.5 * amplitude))
+            ev = torch.maximum(2.0 ** -4 * value.abs(), step(v[b, :, :L], 1.0))
+        tq, tk, ek = tq.transpose(0, 1), tk.transpose(0, 1), ek.transpose(0, 1)
+        ref, err = attend64(tq, tk, value, True, D ** -0.5)
+        G = H // heads
+        wide = lambda t: t.repeat_interleave(G, 0)
+        ds = D ** -0.5 * (eq @ wide(tk).abs().transpose(1, 2) + (tq.abs() + eq) @ wide(ek).transpose(1, 2))
+        seen = torch.ones(L, L, dtype=torch.bool).tril()
+        s = (D ** -0.5 * tq @ wide(tk).transpose(1, 2)).masked_fill(~seen, -math.inf)
+        most = (ds * seen).amax(-1, keepdim=True)
+        moved = torch.expm1(2 * most)                                 # e^(2 ds) bounds a weight's change, sum and all
+        A = s.softmax(-1) @ wide(value).abs()
+        err = err * (1 + moved) + (moved * A + (1 + moved) * (s.softmax(-1) @ wide(ev))) * (1 + 2.0 ** -6)
+        assert ((out - ref).abs() <= err).all(), ((out - ref).abs() - err).max().item()
+
+
+def _contexts(kv_dtype, batch, pages, **kw):
+    from streamvoxel_amd.stream.paged import PagedContext
+    from streamvoxel_amd.stream.step import CachedContext
+    return (CachedContext(2, batch, 4, 48, 700, DEV, kv_dtype),
+            PagedContext(2, batch, 4, 48, pages, DEV, kv_dtype=kv_dtype, **kw))
+
+
+def test_paged_context_holds_what_the_cached_context_holds():
+    """Windows written through both hold the same bits (bf16), also in pages that another window gave back; the attention of
+    either is within its bar of float64 over them."""
+    from streamvoxel_amd.stream.producer import rope_frequencies
+    slab, paged = _contexts('bf16', 3, 30, page_size=16)
+    freq = rope_frequencies(48, device=DEV)
+    g = torch.Generator().manual_seed(3)
+    for P, L, index in ((100, 77, 0), (0, 130, 1), (64, 0, 2), (16, 201, 0), (0, 0, 1), (31, 40, 1)):
+        for layer in range(2):
+            rows = lambda n: torch.randn(n, 4, 48, generator=g).to(torch.bfloat16).to(DEV).transpose(0, 1)
+            pk, pv, k, v = rows(P), rows(P), rows(L), rows(L)
+            positions = (torch.rand(L, 3, generator=g) * 60 - 8).to(DEV)
+            for ctx in (slab, paged):
+                ctx.write(layer, index, k, v, prefix=(pk, pv) if P else None, positions=positions, frequencies=freq)
+    assert paged.lengths.tolist() == slab.lengths.tolist() == [217, 71, 64] and int(paged.bad) == 0
+    assert paged.free_pages == 30 - 14 - 5 - 4
+    for layer in range(2):
+        pool = Pool.__new__(Pool)
+        pool.__dict__.update(lengths=paged.lengths.tolist(), heads=4, D=48, page=16, fp8=False, ke=None, ve=None,
+                             k=paged.k[layer].cpu(), v=paged.v[layer].cpu(), table=paged.table.cpu())
+        for b, L in enumerate(pool.lengths):
+            k, v = pool.rows(b)
+            assert torch.equal(k, slab.k[layer][b, :, :L].cpu().double())
+            assert torch.equal(v, slab.vt[layer][b, :, :, :L].transpose(1, 2).cpu().double())
+        q = queries(3, 4, 70, 48, layer)
+        check(paged.attend(layer, q), q, pool, False)
+        check(slab.attend(layer, q), q, pool, False)
+        assert torch.equal(paged.attend(layer, q[:2], n=2)[0], paged.attend(layer, q[:2], n=2)[0])
+
+
+def test_paged_context_errors_leave_it_as_it_was():
+    _, paged = _contexts('bf16', 3, 10, page_size=16, max_pages=6)
+    paged.resize(0, 70)
+    paged.resize(1, 33)
+    before = (list(paged.host_lengths), [list(o) for o in paged._owned], paged.free_pages)
+    for call, error in ((lambda: paged.resize(2, 97), ValueError), (lambda: paged.resize(2, 40), RuntimeError),
+                        (lambda: paged.resize(3, 1), IndexError), (lambda: paged.resize(0, -1), ValueError),
+                        (lambda: paged.grow((0, 0)), ValueError), (lambda: paged.grow(30), ValueError),
+                        (lambda: paged.grow((0, 30, 30)), RuntimeError)):
+        with pytest.raises(error):
+            call()
+        assert before == (list(paged.host_lengths), [list(o) for o in paged._owned], paged.free_pages)
+    paged.release(0)
+    paged.resize(2, 96)
+    assert paged.lengths.tolist() == [0, 33, 96] and paged.free_pages == 1
+    used = [p for own in paged._owned for p in own] + paged._free
+    assert sorted(used) == list(range(10))
+
+
+@pytest.mark.parametrize('kv_dtype', ['bf16', 'fp8'])
+def test_engine_over_a_shared_pool(kv_dtype):
+    """The slot engine with pages gives the slab engine's step (captured and eager, over slots of different lengths) up to the
+    attention's rounding, holds the same keys, and a slot that is extended holds what a slot loaded whole holds."""
+    from streamvoxel_amd import synth
+    from streamvoxel_amd.stream.engine import Encoded, SlotEngine
+    model = synth.StepModel(classes=40, voxel_shape=(64, 16, 16), width=192, depth=4, heads=8, control_width=192,
+                            control_depth=2, seed=3)
+    for p in model.parameters():
+        p.data = p.data.to(torch.bfloat16)
+    model = model.to(DEV)
+    spec = synth.WindowSpec(height=64, tile=16, num_classes=40)
+    make = lambda **kw: SlotEngine(model, spec, DEV, 3, l1_cap=2, l2_cap=8, kv_dtype=kv_dtype, **kw)
+    slab, paged = make(), make(pages=24, page_size=64)
+    assert paged.graph_ok and paged.context.max_pages == 10
+    conds = [synth.condition(model, P, L, seed=60 + i, device=DEV) for i, (P, L) in enumerate([(32, 500), (9, 72), (0, 300)])]
+    for engine in (slab, paged):
+        for i, c in enumerate(conds):
+            engine.load_slot(i, c)
+        engine.wait_loads()
+    assert paged.packed.lengths.tolist() == slab.packed.lengths.tolist() == [532, 81, 300]
+    with torch.inference_mode():
+        want = slab.replay(0.5).patches.float()
+        for got in (paged.replay(0.5).patches.float(), paged.eager(0.5).patches.float()):
+            # The oracle's bar of the step (test_gpu_forward.py), twice: both engines are within it of the same step.
+            bar = 2e-2 if kv_dtype == 'bf16' else 5e-2
+            assert (got - want).abs().max() <= 2 * bar * want.abs().max()
+            assert (got - want).abs().mean() <= 1e-2 * want.abs().max()
+        assert torch.equal(paged.replay(0.5).patches, paged.eager(0.5).patches)
+    # The third slot again, its local context in two parts.
+    local, positions = conds[2].local, conds[2].positions
+    rows = lambda: [t[layer].view(torch.uint8)[paged.context.table[2, :5].long()].clone()
+                    for layer in range(2) for t in (paged.context.k, paged.context.v)]
+    whole = rows()
+    paged.load_slot(2, Encoded(conds[2].prefix, local[:, :111], positions[:, :111]))
+    paged.extend_slot(2, local[:, 111:], positions[:, 111:])
+    paged.wait_loads()
+    assert paged.packed.lengths.tolist() == [532, 81, 300] and int(paged.context.bad) == 0
+    # (A projection of fewer rows may round differently: one half step of bf16 against another, and of e4m3 on top.)
+    held = lambda t: t.view(torch.bfloat16).float() if kv_dtype == 'bf16' else t.view(torch.float8_e4m3fn).float()
+    for a, b in zip(whole, rows()):
+        a, b = held(a)[:4], held(b)[:4]
+        assert (a - b).abs().max() <= (2.0 ** -5 if kv_dtype == 'bf16' else 2.0 ** -2) * a.abs().max()
+        assert (a != b).float().mean() < 0.02
+    with pytest.raises(ValueError, match='pages'):
+        slab.extend_slot(0, local, positions)
+    with pytest.raises(ValueError, match='capacity'):
+        paged.extend_slot(0, torch.zeros(1, 200, 192, device=DEV), torch.zeros(1, 200, 3, device=DEV))
+    with pytest.raises(IndexError):
+        paged.extend_slot(3, local, positions)

@@ -140,10 +140,11 @@ def test_attention_argument_errors(lib):
     assert attend_call(lib, q=0) == -1 and b'null' in error()
     assert attend_call(lib, sq=68) == -1 and b'query rows' in error()
     assert attend_call(lib, so=66) == -1 and b'rows of out' in error()
-    need = lib.svhip_paged_attention_workspace_bytes(2, 4, 2, 3, 0, 64, 128)
+    assert lib.svhip_paged_attention_workspace_bytes(2, 4, 2, 3, 0, 64, 128) == 0     # too few keys for parts
+    need = lib.svhip_paged_attention_workspace_bytes(2, 4, 2, 3, 0, 64, 1280)
     assert need > 0
     for ws, nbytes in ((0, need), (FAKE, need - 1), (FAKE + 8, need)):
-        assert attend_call(lib, ws=ws, nbytes=nbytes) == -1 and b'workspace' in error()
+        assert attend_call(lib, m=20, ws=ws, nbytes=nbytes) == -1 and b'workspace' in error()
     assert lib.svhip_paged_attention(None, None, None) == -1 and b'null' in error()
     assert lib.svhip_paged_attention(cache_of(), None, None) == -1 and b'null' in error()
 
@@ -160,3 +161,41 @@ def test_workspace_query():
     assert need(8, 12, 12, 1024, 0, 64, 9744) == 0           # tiles that fill the chip
     assert need(1, 12, 12, 1024, 0, 64, 9744) > 0
     assert need(64, 16, 16, 1, 0, 64, 9744) > 0
+
+
+def test_paged_context_books(monkeypatch):
+    """The pages that windows take, keep and give back, without a device."""
+    from streamvoxel_amd.stream.paged import PagedContext
+    monkeypatch.setattr(PagedContext, '_send', staticmethod(lambda to, v: to.copy_(torch.tensor(v, dtype=torch.int32))))
+    ctx = PagedContext(2, 3, 2, 64, 8, 'cpu', page_size=16, max_pages=5)
+    assert len(ctx.k) == len(ctx.v) == 2 and ctx.k[0].shape == (8, 2, 16, 64) and ctx.k_exponents == [None, None]
+    ctx.resize(0, 33)
+    ctx.resize(1, 16)
+    assert ctx.table[0, :3].tolist() == ctx._owned[0] == [0, 1, 2] and ctx._owned[1] == [3] and ctx.free_pages == 4
+    ctx.grow((15, 0, 1))
+    assert ctx.lengths.tolist() == ctx.host_lengths == [48, 16, 1] and ctx._owned[0] == [0, 1, 2] and ctx._owned[2] == [4]
+    ctx.grow(1)
+    assert ctx._owned[0] == [0, 1, 2, 5] and ctx._owned[1] == [3, 6] and ctx.free_pages == 1
+    ctx.resize(0, 20)
+    assert ctx._owned[0] == [0, 1] and ctx.free_pages == 3 and ctx.lengths.tolist() == [20, 17, 2]
+    ctx._set({1: 0, 2: 80})                      # pages given back in the same call serve the other window
+    assert ctx.free_pages == 1 and len(ctx._owned[2]) == 5 and ctx._owned[1] == []
+    assert sorted(sum(ctx._owned, ctx._free[:])) == list(range(8))
+    assert ctx.table[2].tolist() == ctx._owned[2]
+    e = PagedContext(1, 1, 2, 64, 3, 'cpu', kv_dtype='fp8')
+    assert e.max_pages == 3 and e.k[0].dtype == torch.float8_e4m3fn and e.k_exponents[0].shape == (3, 2, 64)
+
+
+@pytest.mark.parametrize('args', [dict(kv_dtype='fp16'), dict(page_size=24), dict(page_size=8), dict(head_dim=60),
+                                  dict(head_dim=136), dict(pages=0), dict(max_pages=0), dict(batch=0)])
+def test_paged_context_refusals(args):
+    from streamvoxel_amd.stream.paged import PagedContext
+    with pytest.raises(ValueError):
+        PagedContext(**{**dict(layers=1, batch=1, heads=2, head_dim=64, pages=4, device='cpu'), **args})
+
+
+def test_pages_of_an_engine_need_its_paged_context():
+    from streamvoxel_amd.stream.engine import SlotEngine, check_engine_options
+    assert check_engine_options('gather', 'flex', False) is None
+    with pytest.raises(RuntimeError, match='HIP'):
+        SlotEngine(None, None, 'cpu', 1, 1, 1, pages=4)
