@@ -18,7 +18,7 @@ ARCH = os.environ.get('SVHIP_ARCH', 'gfx950')
 
 SOURCES = ['api.hip', 'entropy.hip', 'select.hip', 'xattn.hip', 'xattn_split.hip', 'xattn_split_wide.hip', 'xattn_f32.hip',
            'producer.hip', 'norm.hip', 'embed.hip', 'sample.hip', 'rotary.hip', 'paged_append.hip', 'paged_attention.hip',
-           'paged_tile.hip', 'paged_row.hip']
+           'paged_tile.hip', 'paged_row.hip', 'paged_mixed.hip']
 
 FLAGS = [
     '-O3', '-std=c++17', '-fPIC', '-shared', f'--offload-arch={ARCH}',

@@ -31,13 +31,24 @@ __global__ __launch_bounds__(kPagedThreads) void paged_join_kernel(PagedArgs a) 
   const int64_t id = kGroups > 1 ? blockIdx.x : static_cast<int64_t>(blockIdx.x) * (kPagedThreads / 32) + group;
   const int64_t total = (a.tokens.cu ? a.tokens.N : a.tokens.B * a.tokens.N);
   const int64_t token = id / a.H, h = id - token * a.H;
+  int64_t b = -1;
+  if (token < total) b = a.tokens.cu ? (a.tokens.B > 64 ? window_of(a.tokens, token) : -1) : token / a.tokens.N;
+  if (a.tokens.cu && a.tokens.B <= 64) {
+    // Up to 64 borders are read at once; a wave has the tokens of its two groups.
+    const int lane = threadIdx.x & 63, B = static_cast<int>(a.tokens.B);
+    const int64_t from = a.tokens.cu[0], to = lane < B ? a.tokens.cu[1 + lane] : INT64_MAX;
+    const int64_t other = __shfl(token, lane ^ 32);
+    const int n0 = __builtin_popcountll(__builtin_amdgcn_ballot_w64(to <= (lane < 32 ? token : other)));
+    const int n1 = __builtin_popcountll(__builtin_amdgcn_ballot_w64(to <= (lane < 32 ? other : token)));
+    const int n = lane < 32 ? n0 : n1;
+    if (token < total && token >= from && n < B) b = n;
+  }
   // With several groups a row every one of them takes the same way to the barrier.
-  if (token >= total) return;
-  const int64_t b = a.tokens.cu ? window_of(a.tokens, token) : token / a.tokens.N;
   if (b < 0) return;
   const int4 plan = a.plan[b];
   const Window w = window_at(a, b);
   if (w.count <= 0) return;
+  if (token < w.first || token - w.first >= w.count) return set_bad(a.pages);  // borders not ascending
   const int64_t i = token - w.first, kvh = h / a.G, r = i * a.G + (h - kvh * a.G);
   const float* slot;
   int64_t step;
@@ -177,7 +188,7 @@ extern "C" int svhip_paged_attention(const svhip_paged_cache* cache, const svhip
                                    reinterpret_cast<uintptr_t>(c.workspace) % 16 == 0),
                 "%s: workspace too small or misaligned (%lld < %zu bytes)", name, (long long)c.workspace_bytes, p.bytes());
   const int64_t rows = (c.cu_queries ? N : B * N) * H, join = cdiv(rows, kPagedThreads / 32);
-  SVHIP_REQUIRE(p.row_slots < (1ll << 31) && p.tile_grid < (1ll << 31) && join < (1ll << 31), "%s: grid too large", name);
+  SVHIP_REQUIRE(p.row_slots + p.tile_grid < (1ll << 31) && join < (1ll << 31), "%s: grid too large", name);
   const bool fp8 = pc.kv_dtype == SVHIP_FP8_E4M3;
   const int64_t es = fp8 ? 1 : 2;
   float* const part = static_cast<float*>(c.workspace);
@@ -192,8 +203,13 @@ extern "C" int svhip_paged_attention(const svhip_paged_cache* cache, const svhip
                     p.plan_windows ? reinterpret_cast<int4*>(part + p.row_floats + p.tile_floats) : nullptr};
   hipStream_t s = as_stream(stream);
   const bool whole = pc.page_size >= kWholePages;
-  if (p.rows) launch_paged_rows(a, p, fp8, whole, s);
-  if (p.tiles) launch_paged_tiles(a, p, fp8, whole, s);
+  if (p.rows && p.tiles) {
+    launch_paged_mixed(a, p, fp8, whole, s);
+  } else if (p.rows) {
+    launch_paged_rows(a, p, fp8, whole, s);
+  } else {
+    launch_paged_tiles(a, p, fp8, whole, s);
+  }
   if (p.plan_windows) {
     if (rows <= kJoinFew) {
       paged_join_kernel<8><<<static_cast<unsigned>(rows), kPagedThreads, 0, s>>>(a);

@@ -10,6 +10,7 @@ constexpr int kPagedThreads = 256;
 constexpr int kRows = 32;          // rows of a wave
 constexpr int kTileRows = 128;     // rows of a tile workgroup
 constexpr int kTileTarget = 512;   // tile workgroups below which keys are split: two for every CU
+constexpr int kTileBeside = 256;   // the same beside the row form: one for every CU
 constexpr int kTileLeast = 6;      // least key blocks of a tile's part
 constexpr int kRowTarget = 2048;   // row-form parts beyond one for each (window, key head)
 constexpr int kRowLeast = 256;     // keys that a row-form part has a multiple of
@@ -75,21 +76,30 @@ __device__ __forceinline__ int64_t row_at(const PagedArgs& a, const Window& w, i
   return a.tokens.cu ? h * sh + (w.first + i) * sn : b * sb + h * sh + i * sn;
 }
 
-__device__ __forceinline__ int64_t wave_sum(int64_t v) {
-#pragma unroll
-  for (int off = 32; off >= 1; off >>= 1) v += __shfl_xor(v, off, 64);
-  return v;
+// The wave's sum, in every lane: the plans' counts, exact up to 2^24 (a plan has far fewer places than that where the sum
+// matters). DPP steps: a shuffle through LDS takes as long as all of them.
+__device__ __forceinline__ float wave_sum(float v) {
+  v = row16_sum(v);
+  const auto at = [&](int lane) __attribute__((always_inline)) {
+    return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), lane));
+  };
+  return (at(0) + at(16)) + (at(32) + at(48));
 }
 
 // Exclusive prefix over the wave's lanes; `total` the sum.
 __device__ __forceinline__ int wave_prefix(int v, int& total) {
   int incl = v;
-#pragma unroll
-  for (int off = 1; off < 64; off <<= 1) {
-    const int up = __shfl_up(incl, off, 64);
-    if ((threadIdx.x & 63) >= off) incl += up;
-  }
-  total = __builtin_amdgcn_readlane(incl, 63);
+  incl += __builtin_amdgcn_update_dpp(0, incl, 0x111, 0xf, 0xf, true);  // row_shr 1, 2, 4, 8
+  incl += __builtin_amdgcn_update_dpp(0, incl, 0x112, 0xf, 0xf, true);
+  incl += __builtin_amdgcn_update_dpp(0, incl, 0x114, 0xf, 0xf, true);
+  incl += __builtin_amdgcn_update_dpp(0, incl, 0x118, 0xf, 0xf, true);
+  const int r0 = __builtin_amdgcn_readlane(incl, 15), r1 = __builtin_amdgcn_readlane(incl, 31);
+  const int r2 = __builtin_amdgcn_readlane(incl, 47), r3 = __builtin_amdgcn_readlane(incl, 63);
+  const int row = (threadIdx.x & 63) >> 4;
+  incl += row > 0 ? r0 : 0;
+  incl += row > 1 ? r1 : 0;
+  incl += row > 2 ? r2 : 0;
+  total = r0 + r1 + r2 + r3;
   return incl - v;
 }
 
@@ -132,16 +142,17 @@ __device__ __forceinline__ PagedItem item_at(const PagedArgs& a, int at, Count c
 // The least length of a part, a multiple of `grain` and `least` at least, for which the windows' parts are at most `target`:
 // they then run side by side, and none longer than it must. places(c, length): parts of window c, all key heads and tiles.
 template <typename Places>
-__device__ __forceinline__ int part_length(const PagedArgs& a, int64_t work, int target, int grain, int least,
+__device__ __forceinline__ int part_length(const PagedArgs& a, float work, int target, int grain, int least,
                                            Places places) {
   // An equal share is too short, or all but; twice as long again and again until it fits, then halves between.
-  int low = static_cast<int>(work / target / grain);
+  const float share = work / static_cast<float>(target) / static_cast<float>(grain);
+  int low = share < static_cast<float>(kUncut / 4) / static_cast<float>(grain) ? static_cast<int>(share) : kUncut / 4 / grain;
   if (low * grain < least) low = least / grain - 1;
   int high = low + 1;
   auto fits = [&](int length) __attribute__((always_inline)) {
-    int64_t n = 0;
+    float n = 0.f;
     for (int64_t c = threadIdx.x & 63; c < a.tokens.B; c += 64) n += places(static_cast<int>(c), length * grain);
-    return wave_sum(n) <= target;
+    return wave_sum(n) <= static_cast<float>(target);
   };
   while (high < kUncut / grain / 2 && !fits(high)) {
     low = high;
@@ -174,6 +185,9 @@ __device__ __forceinline__ int valid_keys(const PagedArgs& a, int keys, int j, i
   return valid;
 }
 
+// Head widths: KS steps of 16 head_dim elements in the score product, and output tiles of 32.
+constexpr int tiles_of(int KS) { return (KS + 1) / 2; }
+
 #if defined(__HIP_DEVICE_COMPILE__)
 
 // One key head's part of a pool (of keys or of values): bytes from page to page and row to row.
@@ -201,9 +215,6 @@ __device__ __forceinline__ __amdgpu_buffer_rsrc_t rows_of(const char* head, uint
   const uint32_t bound = valid > 0 ? static_cast<uint32_t>(valid - 1) * sr + bytes : 0u;
   return __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(base), 0, bound, kRsrcFlags);
 }
-
-// Head widths: KS steps of 16 head_dim elements in the score product, and output tiles of 32.
-constexpr int tiles_of(int KS) { return (KS + 1) / 2; }
 
 // A wave's 32 rows: the queries as B operands, O^T, running maximum and sum.
 template <int KS>
@@ -247,16 +258,12 @@ __device__ __forceinline__ f32x16_t scores(const Rows<KS>& s, const bf16x8_t (&k
   return x;
 }
 
-// The rest of a block of 32 kHalves keys, `key0` the first, from their scores x: weights, sum, and O^T += V^T P^T with V rows
-// staged at row 0 of vp (sub-tiles of 64 head_dim elements kSubBytes apart). The running maximum moves only for a score more
-// than kMaxHigh above it (the weights then stay below 2^20, which fp32 sums and bf16 hold alike). One such branch a block: a
-// second one in a loop makes the compiler merge two register sets of O behind it, a copy that the common path pays. The row's
-// sum is taken over the bf16 weights that the second product reads, by v_mfma_f32_4x4x4_16b_bf16 with ones in A, whose
-// columns are single lanes: no row's NaN reaches another's sum.
-template <int KS, int kSubBytes, int kHalves>
-__device__ __forceinline__ void attend_block(Rows<KS>& s, f32x16_t (&x)[kHalves], const char* vp,
-                                             const uint32_t (&rvt)[tiles_of(KS)], float sl2, bool masked, int key0) {
-  constexpr int DT = tiles_of(KS);
+// Scores x of a block of 32 kHalves keys, `key0` the first: those that a row does not see masked, and the running maximum
+// moved for a score more than kMaxHigh above it (the weights then stay below 2^20, which fp32 sums and bf16 hold alike). One
+// such branch a block: a second one in a loop makes the compiler merge two register sets of O behind it, a copy that the
+// common path pays.
+template <int KS, int kHalves>
+__device__ __forceinline__ void bound_scores(Rows<KS>& s, f32x16_t (&x)[kHalves], float sl2, bool masked, int key0) {
   const int hh = (threadIdx.x & 63) >> 5;
   if (masked) {
 #pragma unroll
@@ -289,50 +296,60 @@ __device__ __forceinline__ void attend_block(Rows<KS>& s, f32x16_t (&x)[kHalves]
 #pragma unroll
     for (int i = 0; i < 4; ++i) s.l[i] *= alpha;
 #pragma unroll
-    for (int j = 0; j < DT; ++j) {
+    for (int j = 0; j < tiles_of(KS); ++j) {
 #pragma unroll
       for (int i = 0; i < 16; ++i) s.o[j][i] *= alpha;
     }
   }
+}
+
+// 32 keys' weights P^T = exp2(sl2 x - m) as B operands of the second product's two steps.
+template <int KS>
+__device__ __forceinline__ void weights_of(const Rows<KS>& s, const f32x16_t& x, float sl2, bf16x8_t (&pb)[2]) {
   const float nm = -s.m;
 #pragma unroll
-  for (int t = 0; t < kHalves; ++t) {
-    bf16x8_t pb[2];
+  for (int ks = 0; ks < 2; ++ks) {
 #pragma unroll
-    for (int ks = 0; ks < 2; ++ks) {
-#pragma unroll
-      for (int j = 0; j < 8; j += 2) {
-        const f32x2_t two = {__builtin_amdgcn_exp2f(__builtin_fmaf(x[t][8 * ks + j], sl2, nm)),
-                             __builtin_amdgcn_exp2f(__builtin_fmaf(x[t][8 * ks + j + 1], sl2, nm))};
-        const bf16x2_t c = __builtin_convertvector(two, bf16x2_t);
-        pb[ks][j] = c[0];
-        pb[ks][j + 1] = c[1];
-      }
+    for (int j = 0; j < 8; j += 2) {
+      const f32x2_t two = {__builtin_amdgcn_exp2f(__builtin_fmaf(x[8 * ks + j], sl2, nm)),
+                           __builtin_amdgcn_exp2f(__builtin_fmaf(x[8 * ks + j + 1], sl2, nm))};
+      const bf16x2_t c = __builtin_convertvector(two, bf16x2_t);
+      pb[ks][j] = c[0];
+      pb[ks][j + 1] = c[1];
     }
-    typedef short i16x4_t __attribute__((ext_vector_type(4)));
-    typedef short i16x8_t __attribute__((ext_vector_type(8)));
-    const i16x4_t ones = {0x3F80, 0x3F80, 0x3F80, 0x3F80};
+  }
+}
+
+// O^T += V^T P^T and the row's sum for 32 keys whose V rows are staged at vp (sub-tiles of 64 head_dim elements kSubBytes
+// apart). The sum is taken over the bf16 weights that the product reads, by v_mfma_f32_4x4x4_16b_bf16 with ones in A, whose
+// columns are single lanes: no row's NaN reaches another's sum.
+template <int KS, int kSubBytes>
+__device__ __forceinline__ void add_values(Rows<KS>& s, const bf16x8_t (&pb)[2], const char* vp,
+                                           const uint32_t (&rvt)[tiles_of(KS)]) {
+  constexpr int DT = tiles_of(KS);
+  typedef short i16x4_t __attribute__((ext_vector_type(4)));
+  typedef short i16x8_t __attribute__((ext_vector_type(8)));
+  const i16x4_t ones = {0x3F80, 0x3F80, 0x3F80, 0x3F80};
 #pragma unroll
-    for (int ks = 0; ks < 2; ++ks) {
-      const i16x8_t p8 = __builtin_bit_cast(i16x8_t, pb[ks]);
-      s.l = __builtin_amdgcn_mfma_f32_4x4x4bf16_1k(ones, __builtin_shufflevector(p8, p8, 0, 1, 2, 3), s.l, 0, 0, 0);
-      s.l = __builtin_amdgcn_mfma_f32_4x4x4bf16_1k(ones, __builtin_shufflevector(p8, p8, 4, 5, 6, 7), s.l, 0, 0, 0);
+  for (int ks = 0; ks < 2; ++ks) {
+    const i16x8_t p8 = __builtin_bit_cast(i16x8_t, pb[ks]);
+    s.l = __builtin_amdgcn_mfma_f32_4x4x4bf16_1k(ones, __builtin_shufflevector(p8, p8, 0, 1, 2, 3), s.l, 0, 0, 0);
+    s.l = __builtin_amdgcn_mfma_f32_4x4x4bf16_1k(ones, __builtin_shufflevector(p8, p8, 4, 5, 6, 7), s.l, 0, 0, 0);
+  }
+#pragma unroll
+  for (int ks = 0; ks < 2; ++ks) {
+    bf16x8_t va[DT];
+#pragma unroll
+    for (int j = 0; j < DT; ++j) {
+      typedef __bf16 bf16x4_t __attribute__((ext_vector_type(4)));
+      typedef __attribute__((address_space(3))) bf16x4_t lds_bf16x4_t;
+      char* at = const_cast<char*>(vp) + (j >> 1) * kSubBytes + rvt[j] + 16 * ks * kRow * 2;
+      const bf16x4_t lo = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((lds_bf16x4_t*)(at));
+      const bf16x4_t hi = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((lds_bf16x4_t*)(at + 4 * kRow * 2));
+      va[j] = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
     }
 #pragma unroll
-    for (int ks = 0; ks < 2; ++ks) {
-      bf16x8_t va[DT];
-#pragma unroll
-      for (int j = 0; j < DT; ++j) {
-        typedef __bf16 bf16x4_t __attribute__((ext_vector_type(4)));
-        typedef __attribute__((address_space(3))) bf16x4_t lds_bf16x4_t;
-        char* at = const_cast<char*>(vp) + (j >> 1) * kSubBytes + rvt[j] + (32 * t + 16 * ks) * kRow * 2;
-        const bf16x4_t lo = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((lds_bf16x4_t*)(at));
-        const bf16x4_t hi = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((lds_bf16x4_t*)(at + 4 * kRow * 2));
-        va[j] = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
-      }
-#pragma unroll
-      for (int j = 0; j < DT; ++j) s.o[j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(va[j], pb[ks], s.o[j], 0, 0, 0);
-    }
+    for (int j = 0; j < DT; ++j) s.o[j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(va[j], pb[ks], s.o[j], 0, 0, 0);
   }
 }
 
@@ -439,6 +456,7 @@ struct PagedPlan {
 // FP8, KS: steps of 16 head_dim elements; whole: pages of kWholePages keys or more.
 void launch_paged_rows(const PagedArgs& a, const PagedPlan& p, bool fp8, bool whole, hipStream_t s);
 void launch_paged_tiles(const PagedArgs& a, const PagedPlan& p, bool fp8, bool whole, hipStream_t s);
+void launch_paged_mixed(const PagedArgs& a, const PagedPlan& p, bool fp8, bool whole, hipStream_t s);
 
 // The instantiations of `launch` by type, page size and head width.
 #define SVHIP_PAGED_WIDTH(launch, FP8, WHOLE)                      \
