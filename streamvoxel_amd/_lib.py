@@ -169,6 +169,11 @@ def dtype_code(dtype):
     raise TypeError(f'unsupported logits dtype {dtype} (float32 or bfloat16)')
 
 
+def stacked(t):
+    """True when elements of a tensor lie on each other (a dimension expanded with stride 0): no place for results."""
+    return 0 in t.stride() and any(s == 0 and n > 1 for n, s in zip(t.shape, t.stride()))
+
+
 def byte_span(t):
     """[first, last) device byte addresses a tensor's elements occupy (its strides taken into account)."""
     if t.numel() == 0:

@@ -93,7 +93,7 @@ inline int page_shift(int64_t page) {
 inline int check_cache(const char* name, const svhip_paged_cache* cache) {
   SVHIP_REQUIRE(cache, "%s: null cache", name);
   const svhip_paged_cache& c = *cache;
-  SVHIP_REQUIRE(c.windows >= 0 && c.heads >= 0, "%s: bad sizes", name);
+  SVHIP_REQUIRE(c.windows >= 0 && c.windows < (1ll << 31) && c.heads >= 0 && c.heads <= 1 << 20, "%s: bad sizes", name);
   SVHIP_REQUIRE(c.head_dim >= 8 && c.head_dim <= kMaxPagedDim && c.head_dim % 8 == 0,
                 "%s: head_dim %lld unsupported (a multiple of 8 up to %d)", name, (long long)c.head_dim, kMaxPagedDim);
   SVHIP_REQUIRE(c.kv_dtype == SVHIP_BF16 || c.kv_dtype == SVHIP_FP8_E4M3, "%s: kv dtype %d unsupported", name,
@@ -101,8 +101,8 @@ inline int check_cache(const char* name, const svhip_paged_cache* cache) {
   SVHIP_REQUIRE(c.page_size >= kMinPage && c.page_size <= kMaxPage && (c.page_size & (c.page_size - 1)) == 0,
                 "%s: page size %lld unsupported (a power of two, %d to %d)", name, (long long)c.page_size, kMinPage,
                 kMaxPage);
-  SVHIP_REQUIRE(c.pages >= 0 && c.pages < (1ll << 31) && c.max_pages >= 0 && c.max_pages < (1ll << 31) / c.page_size,
-                "%s: bad page counts", name);
+  SVHIP_REQUIRE(c.pages >= 0 && c.pages < (1ll << 31) && c.max_pages >= 0 && c.max_pages <= (1ll << 30) / c.page_size,
+                "%s: bad page counts", name);  // (keys and a few blocks of them further on are counted in 32 bits)
   return SVHIP_OK;
 }
 

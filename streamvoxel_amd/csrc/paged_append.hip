@@ -258,7 +258,7 @@ extern "C" int svhip_paged_append(const svhip_paged_cache* cache, const svhip_pa
   const svhip_paged_cache& p = *cache;
   const svhip_paged_append_args& c = *args;
   const int64_t D = p.head_dim;
-  SVHIP_REQUIRE(c.N >= 0 && c.before >= 0, "%s: bad sizes", name);
+  SVHIP_REQUIRE(c.N >= 0 && c.N < (1ll << 31) && c.before >= 0 && c.before < (1ll << 31), "%s: bad sizes", name);
   const bool turns = c.layout != SVHIP_ROTARY_NONE, axial = c.layout == SVHIP_ROTARY_AXIAL;
   SVHIP_REQUIRE(c.layout >= SVHIP_ROTARY_NONE && c.layout <= SVHIP_ROTARY_AXIAL, "%s: layout %d unsupported", name,
                 (int)c.layout);
@@ -271,7 +271,6 @@ extern "C" int svhip_paged_append(const svhip_paged_cache* cache, const svhip_pa
   SVHIP_REQUIRE(c.key && c.value, "%s: null pointer", name);
   SVHIP_REQUIRE(!turns || c.freq, "%s: the rotation needs frequencies", name);
   SVHIP_REQUIRE(!axial || c.positions, "%s: the three-axis rotation needs positions", name);
-  SVHIP_REQUIRE(p.heads <= 1 << 20, "%s: sizes too large", name);
   SVHIP_REQUIRE(rows16(c.key, c.sk_b, c.sk_h, c.sk_n) && rows16(c.value, c.sv_b, c.sv_h, c.sv_n),
                 "%s: key and value rows must start on 16-byte boundaries", name);
   const int64_t total = c.cu_tokens ? c.N : p.windows * c.N;

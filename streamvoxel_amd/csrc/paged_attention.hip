@@ -15,9 +15,63 @@
 // Staging: 16 keys lie in one page (pages are of 16 keys or more), so the wave's load of 8 rows has one base, a scalar buffer
 // descriptor whose bound is the number of its keys that exist: keys past the window's end, bad pages and the chunks past
 // head_dim read as zeros and nothing is read outside a page.
-#include "paged_attention.hpp"
+#include "paged_row.hpp"
+#include "paged_tile.hpp"
 
 namespace svhip {
+
+// The plan of more windows than a wave has lanes, by one workgroup: part lengths, and every window's places in the lists of
+// row-form parts and of tiles. (Up to 64 windows a workgroup's own plan is one load a lane, less than this launch.)
+__global__ __launch_bounds__(kPlanThreads) void paged_plan_kernel(PagedArgs a, bool rows, bool tiles) {
+  __shared__ float of_wave[kPlanThreads / 64];
+  __shared__ int2 counts[kPlanThreads / 64];
+  const BlockTeam team{of_wave};
+  const int tid = static_cast<int>(threadIdx.x), Hkv = static_cast<int>(a.Hkv);
+  int unused, more;
+  float total;
+  const int row_each = rows && a.row_part ? row_length(a, team, 0, unused) : kUncut;
+  const int tile_each = tiles ? tile_length(a, team, unused, more, total) : kUncut;
+  int2 at = make_int2(0, 0);
+  int cut = 0;  // 1: windows of the row form, 2: tiles
+  for (int64_t c0 = 0; c0 < a.tokens.B; c0 += kPlanThreads) {
+    const int64_t c = c0 + tid;
+    int row = 0, tile = 0, parts = 1, t = 0, blocks = 0;
+    if (c < a.tokens.B) {
+      if (tiles) tiles_of_window(a, c, t, blocks);
+      if (t > 0) {
+        parts = tile_parts(blocks, tile_each);
+        tile = t * Hkv * parts;
+      } else if (rows) {
+        parts = row_parts(row_keys(a, c), row_each);
+        row = Hkv * parts;
+      }
+    }
+    cut |= parts > 1 ? (t > 0 ? 2 : 1) : 0;
+    int row_sum, tile_sum;
+    int2 before = make_int2(wave_prefix(row, row_sum), 0);
+    before.y = wave_prefix(tile, tile_sum);
+    if ((tid & 63) == 0) counts[tid >> 6] = make_int2(row_sum, tile_sum);
+    __syncthreads();
+    int2 sum = at;
+#pragma unroll
+    for (int i = 0; i < kPlanThreads / 64; ++i) {
+      if (i == tid >> 6) {
+        before.x += sum.x;
+        before.y += sum.y;
+      }
+      sum.x += counts[i].x;
+      sum.y += counts[i].y;
+    }
+    at = sum;
+    if (c < a.tokens.B) {
+      a.plan[c] = t > 0 ? make_int4(before.y, parts, tile_each, t) : make_int4(before.x, parts, row_each, 1);
+      a.running[c] = make_int2(before.x + row, before.y + tile);
+    }
+    __syncthreads();
+  }
+  const bool row_cut = __syncthreads_or(cut & 1), tile_cut = __syncthreads_or(cut & 2);
+  if (tid == 0) a.plan[a.tokens.B] = make_int4(at.x, at.y, row_cut ? row_each : kUncut, tile_cut ? tile_each : kUncut);
+}
 
 // The parts of a row joined in order. kGroups 32-lane groups a row, 4 elements a lane: one group where the rows are many (it
 // has kAhead parts in flight), all 8 of the workgroup where they are few (every part of up to 64 in flight at once).
@@ -27,6 +81,10 @@ template <int kGroups>
 __global__ __launch_bounds__(kPagedThreads) void paged_join_kernel(PagedArgs a) {
   __shared__ float4 s_o[kGroups > 1 ? kGroups : 1][32];
   __shared__ float2 s_ml[kGroups > 1 ? kGroups : 1];
+  if (a.running) {
+    const int4 sums = a.plan[a.tokens.B];
+    if (sums.z == kUncut && sums.w == kUncut) return;  // no parts
+  }
   const int group = threadIdx.x / 32, d0 = 4 * (threadIdx.x % 32);
   const int64_t id = kGroups > 1 ? blockIdx.x : static_cast<int64_t>(blockIdx.x) * (kPagedThreads / 32) + group;
   const int64_t total = (a.tokens.cu ? a.tokens.N : a.tokens.B * a.tokens.N);
@@ -54,6 +112,7 @@ __global__ __launch_bounds__(kPagedThreads) void paged_join_kernel(PagedArgs a) 
   int64_t step;
   int count;
   if (row_form(a, w.count)) {
+    if (!a.row_part) return;
     count = plan.y;
     if (plan.x < 0 || count < 0 || plan.x + a.Hkv * count > a.row_slots) return set_bad(a.pages);  // borders not ascending
     slot = a.row_part + ((plan.x + kvh * count) * a.slot_rows + r) * (a.D + 2);
@@ -143,13 +202,15 @@ inline PagedPlan paged_plan(int64_t B, int64_t H, int64_t Hkv, int64_t N, bool p
   }
   if (p.rows) {
     // One for each (window, key head), and the parts: at most kRowTarget more, and no shorter than kRowLeast.
-    const int64_t more = B * Hkv * (cdiv(max_keys, kRowLeast) - 1);
+    // (From 2^22 pairs on there is no need, and the plan's sums stay exact.)
+    const int64_t more = B * Hkv > 1 << 22 ? 0 : B * Hkv * (cdiv(max_keys, kRowLeast) - 1);
     p.row_parts = more > 0;
     p.row_slots = (more < 0 ? 0 : (more < kRowTarget ? more : kRowTarget)) + B * Hkv;
     p.slot_rows = packed ? (N * G < kRows ? N * G : kRows) : N * G;
     if (p.row_parts) p.row_floats = (p.row_slots * p.slot_rows * (D + 2) + 3) / 4 * 4;
   }
   p.plan_windows = p.row_parts || p.split ? B : 0;
+  p.planned = p.plan_windows > 64;
   return p;
 }
 
@@ -159,7 +220,10 @@ using namespace svhip;
 
 extern "C" size_t svhip_paged_attention_workspace_bytes(int64_t B, int64_t H, int64_t Hkv, int64_t N, int packed,
                                                         int64_t D, int64_t max_keys) {
-  if (B < 1 || H < 1 || Hkv < 1 || H % Hkv != 0 || N < 1 || D < 1 || max_keys < 0) return 0;
+  if (B < 1 || B >= 1ll << 31 || Hkv < 1 || H < 1 || H > 1 << 20 || H % Hkv != 0 || N < 1 || N >= 1ll << 31 ||
+      N * H >= 1ll << 40 || D < 1 || D > kMaxPagedDim || max_keys < 0 || max_keys > 1ll << 30) {
+    return 0;
+  }
   return paged_plan(B, H, Hkv, N, packed != 0, D, max_keys).bytes();
 }
 
@@ -172,7 +236,7 @@ extern "C" int svhip_paged_attention(const svhip_paged_cache* cache, const svhip
   const svhip_paged_cache& pc = *cache;
   const svhip_paged_attention_args& c = *args;
   const int64_t B = pc.windows, H = c.H, Hkv = pc.heads, N = c.N, D = pc.head_dim;
-  SVHIP_REQUIRE(H >= 0 && N >= 0, "%s: bad sizes", name);
+  SVHIP_REQUIRE(H >= 0 && H <= 1 << 20 && N >= 0 && N < (1ll << 31) && N * H < (1ll << 40), "%s: bad sizes", name);
   SVHIP_REQUIRE(Hkv >= 1 && H % Hkv == 0, "%s: %lld heads do not share %lld key heads evenly", name, (long long)H,
                 (long long)Hkv);
   const float scale = static_cast<float>(c.scale);
@@ -192,6 +256,7 @@ extern "C" int svhip_paged_attention(const svhip_paged_cache* cache, const svhip
   const bool fp8 = pc.kv_dtype == SVHIP_FP8_E4M3;
   const int64_t es = fp8 ? 1 : 2;
   float* const part = static_cast<float*>(c.workspace);
+  int4* const plan = reinterpret_cast<int4*>(part + p.row_floats + p.tile_floats);
   const PagedArgs a{static_cast<const uint16_t*>(c.q), pc.k_pages, pc.v_pages, pc.k_exponents, pc.v_exponents,
                     static_cast<uint16_t*>(c.out), Tokens{c.cu_queries, B, N}, pages_of(pc), H, Hkv, H / Hkv, D, c.sq_b,
                     c.sq_h, c.sq_n, pc.sk_h, pc.sv_h, pc.sek_h, pc.sev_h, c.so_b, c.so_h, c.so_n,
@@ -199,9 +264,10 @@ extern "C" int svhip_paged_attention(const svhip_paged_cache* cache, const svhip
                     static_cast<uint32_t>(pc.sv_p * es), static_cast<uint32_t>(pc.sv_r * es),
                     static_cast<uint32_t>(pc.sek_p), static_cast<uint32_t>(pc.sev_p), c.causal != 0, scale * kLog2e,
                     p.q_tiles, p.split, static_cast<int>(p.row_slots), static_cast<int>(p.tile_slots),
-                    static_cast<int>(p.slot_rows), part, part + p.row_floats,
-                    p.plan_windows ? reinterpret_cast<int4*>(part + p.row_floats + p.tile_floats) : nullptr};
+                    static_cast<int>(p.slot_rows), p.row_parts ? part : nullptr, part + p.row_floats,
+                    p.plan_windows ? plan : nullptr, p.planned ? reinterpret_cast<int2*>(plan + B + 1) : nullptr};
   hipStream_t s = as_stream(stream);
+  if (p.planned) paged_plan_kernel<<<1, kPlanThreads, 0, s>>>(a, p.rows, p.tiles);
   const bool whole = pc.page_size >= kWholePages;
   if (p.rows && p.tiles) {
     launch_paged_mixed(a, p, fp8, whole, s);

@@ -36,8 +36,10 @@ struct PagedArgs {
   bool split;           // tiles: whether parts of keys may be dealt out
   int row_slots, tile_slots;  // slots of parts at most
   int slot_rows;        // rows of a row-form slot
-  float *row_part, *tile_part;
-  int4* plan;           // (null: no parts) a window's first slot, its parts, a part's length (tiles: blocks) and its tiles
+  float *row_part, *tile_part;  // row_part null: the row form's windows are not cut
+  int4* plan;           // (null: no parts) a window's first place, its parts, a part's length (tiles: blocks) and its tiles
+  int2* running;        // (null: every workgroup plans for itself) places of row form and of tiles up to and with a window;
+                        // plan[B] then has their sums and the part lengths
 };
 
 // The window as a workgroup sees it.
@@ -76,8 +78,7 @@ __device__ __forceinline__ int64_t row_at(const PagedArgs& a, const Window& w, i
   return a.tokens.cu ? h * sh + (w.first + i) * sn : b * sb + h * sh + i * sn;
 }
 
-// The wave's sum, in every lane: the plans' counts, exact up to 2^24 (a plan has far fewer places than that where the sum
-// matters). DPP steps: a shuffle through LDS takes as long as all of them.
+// The wave's sum, in every lane: the plans' counts, exact up to 2^24 (where a plan cuts, its places are fewer). DPP steps: a shuffle through LDS takes as long as all of them.
 __device__ __forceinline__ float wave_sum(float v) {
   v = row16_sum(v);
   const auto at = [&](int lane) __attribute__((always_inline)) {
@@ -109,41 +110,66 @@ struct PagedItem {
   int b, kvh, part, parts, qt, tiles, at, before;
 };
 
-// The item at place `at` of the windows' lists, one after the other: window c has tiles(c) * Hkv * parts(c) of them, for every
-// key head its parts, for every part its tiles.
-template <typename Count>
-__device__ __forceinline__ PagedItem item_at(const PagedArgs& a, int at, Count count) {
-  const int lane = threadIdx.x & 63, Hkv = static_cast<int>(a.Hkv);
-  PagedItem item{-1, 0, 0, 1, 0, 1, at, 0};
-  int left = at;
-  for (int b0 = 0; b0 < a.tokens.B; b0 += 64) {
-    int tiles = 0, parts = 1, total;
-    if (b0 + lane < a.tokens.B) count(b0 + lane, tiles, parts);
-    const int n = tiles * Hkv * parts;
-    const int before = wave_prefix(n, total);
-    if (left < total) {
-      const int c = __builtin_ctzll(__builtin_amdgcn_ballot_w64(before <= left && left < before + n));
-      const int in = left - __builtin_amdgcn_readlane(before, c);
-      item.b = b0 + c;
-      item.tiles = __builtin_amdgcn_readlane(tiles, c);
-      item.parts = __builtin_amdgcn_readlane(parts, c);
-      item.before = at - in;
-      item.qt = in % item.tiles;
-      const int u = in / item.tiles;
-      item.kvh = u / item.parts;
-      item.part = u - item.kvh * item.parts;
-      return item;
-    }
-    left -= total;
-  }
-  return item;
+// Place `in` of window b's list: for every key head its parts, for every part its tiles.
+__device__ __forceinline__ PagedItem item_of(int b, int at, int in, int parts, int tiles) {
+  const int u = in / tiles, kvh = u / parts;
+  return PagedItem{b, kvh, u - kvh * parts, parts, in - u * tiles, tiles, at, at - in};
 }
+
+// The item at place `at` of the lists of up to 64 windows, one after the other; the lane's window has `tiles` and `parts`.
+__device__ __forceinline__ PagedItem item_at(int Hkv, int at, int tiles, int parts) {
+  int total;
+  const int n = tiles * Hkv * parts, before = wave_prefix(n, total);
+  if (at >= total) return PagedItem{-1, 0, 0, 1, 0, 1, at, 0};
+  const int c = __builtin_ctzll(__builtin_amdgcn_ballot_w64(before <= at && at < before + n));
+  return item_of(c, at, at - __builtin_amdgcn_readlane(before, c), __builtin_amdgcn_readlane(parts, c),
+                 __builtin_amdgcn_readlane(tiles, c));
+}
+
+// The same from paged_plan_kernel's lists; `ends` the running sums of the form, two numbers apart. 64 windows a step.
+__device__ __forceinline__ PagedItem planned_item(const PagedArgs& a, int at, const int* ends) {
+  const int lane = threadIdx.x & 63;
+  int lo = 0, hi = static_cast<int>(a.tokens.B), c;
+  do {
+    const int step = (hi - lo + 63) / 64, end = lo + (lane + 1) * step, last = end < hi ? end : hi;
+    const uint64_t past = __builtin_amdgcn_ballot_w64(ends[2 * (last - 1)] > at);
+    if (past == 0ull) return PagedItem{-1, 0, 0, 1, 0, 1, at, 0};
+    c = __builtin_ctzll(past);
+    lo += c * step;
+    hi = hi - lo > step ? lo + step : hi;
+  } while (hi - lo > 1);
+  const int4 plan = a.plan[lo];
+  return item_of(lo, at, at - plan.x, plan.y, plan.w);
+}
+
+// Who plans: a wave, for up to 64 windows (one a lane), or a workgroup.
+struct WaveTeam {
+  static constexpr int kSize = 64;
+  __device__ __forceinline__ int id() const { return threadIdx.x & 63; }
+  __device__ __forceinline__ float sum(float v) const { return wave_sum(v); }
+};
+constexpr int kPlanThreads = 1024;
+struct BlockTeam {
+  static constexpr int kSize = kPlanThreads;
+  float* of_wave;  // LDS, one for every wave
+  __device__ __forceinline__ int id() const { return threadIdx.x; }
+  __device__ __forceinline__ float sum(float v) const {
+    v = wave_sum(v);
+    if ((threadIdx.x & 63) == 0) of_wave[threadIdx.x >> 6] = v;
+    __syncthreads();
+    float total = 0.f;
+#pragma unroll
+    for (int i = 0; i < kPlanThreads / 64; ++i) total += of_wave[i];
+    __syncthreads();
+    return total;
+  }
+};
 
 // The least length of a part, a multiple of `grain` and `least` at least, for which the windows' parts are at most `target`:
 // they then run side by side, and none longer than it must. places(c, length): parts of window c, all key heads and tiles.
-template <typename Places>
-__device__ __forceinline__ int part_length(const PagedArgs& a, float work, int target, int grain, int least,
-                                           Places places) {
+template <typename Team, typename Places>
+__device__ __forceinline__ int part_length(const PagedArgs& a, const Team& team, float work, int target, int grain,
+                                           int least, Places places) {
   // An equal share is too short, or all but; twice as long again and again until it fits, then halves between.
   const float share = work / static_cast<float>(target) / static_cast<float>(grain);
   int low = share < static_cast<float>(kUncut / 4) / static_cast<float>(grain) ? static_cast<int>(share) : kUncut / 4 / grain;
@@ -151,8 +177,8 @@ __device__ __forceinline__ int part_length(const PagedArgs& a, float work, int t
   int high = low + 1;
   auto fits = [&](int length) __attribute__((always_inline)) {
     float n = 0.f;
-    for (int64_t c = threadIdx.x & 63; c < a.tokens.B; c += 64) n += places(static_cast<int>(c), length * grain);
-    return wave_sum(n) <= static_cast<float>(target);
+    for (int64_t c = team.id(); c < a.tokens.B; c += Team::kSize) n += places(static_cast<int>(c), length * grain);
+    return team.sum(n) <= static_cast<float>(target);
   };
   while (high < kUncut / grain / 2 && !fits(high)) {
     low = high;
@@ -443,14 +469,75 @@ __device__ __forceinline__ void commit_rows8(const Staged<DT, kLoads>& st, int i
   }
 }
 
+// Values that are not finite, in a block whose keys some rows of the product see and some do not: their weight 0 times such a
+// value is NaN. So they are zeroed in LDS before the product (true: one was), a thread 16 bytes of `bytes` every `step`, and
+// added to the rows that see them at the end, from the pool.
+__device__ __forceinline__ bool clean_values(char* v, int bytes, int at, int step) {
+  bool odd = false;
+  for (; at < bytes; at += step) {
+    uint4* const p = reinterpret_cast<uint4*>(v + at);
+    const uint4 w = *p;
+    uint32_t u[4] = {w.x, w.y, w.z, w.w};
+    bool here = false;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const bool lo = (u[i] & 0x7f80u) == 0x7f80u, hi = (u[i] & 0x7f800000u) == 0x7f800000u;
+      here |= lo || hi;
+      u[i] &= (lo ? 0xffff0000u : ~0u) & (hi ? 0xffffu : ~0u);
+    }
+    if (here) *p = make_uint4(u[0], u[1], u[2], u[3]);
+    odd |= here;
+  }
+  return odd;
+}
+
+// Those of keys [from, to) to O^T of the rows that see them. (Their weights are above 0, and an infinity or NaN stays one.)
+template <bool FP8, int KS>
+__device__ __forceinline__ void add_odd_values(const PagedArgs& a, const Source& vs, const int32_t* row, int from, int to,
+                                               Rows<KS>& s) {
+  const int hh = (threadIdx.x & 63) >> 5, in_mask = (1 << a.pages.shift) - 1;
+  for (int j = from; j < to; ++j) {
+    const int page = page_number(a, row, j);
+    if (static_cast<uint32_t>(page) < static_cast<uint32_t>(a.pages.pages) && j <= s.last) {
+      const uint32_t in_page = j & in_mask;
+      const char* at = vs.rows + static_cast<uint64_t>(page) * vs.sp + in_page * vs.sr;
+      float f = 0.f;
+      if constexpr (FP8) f = exponent_value(vs.exponents[static_cast<uint64_t>(page) * vs.se + in_page]);
+#pragma unroll
+      for (int i = 0; i < 4 * tiles_of(KS); ++i) {
+        const int d0 = 8 * i + 4 * hh;
+        if (d0 >= a.D) continue;
+        uint2 w;
+        if constexpr (FP8) {
+          const uint32_t codes = *reinterpret_cast<const uint32_t*>(at + d0);
+          w = make_uint2(__builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(codes, f, false)),
+                         __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(codes, f, true)));
+        } else {
+          w = *reinterpret_cast<const uint2*>(at + 2 * d0);
+        }
+        const float v[4] = {__uint_as_float(w.x << 16), __uint_as_float(w.x & 0xffff0000u), __uint_as_float(w.y << 16),
+                            __uint_as_float(w.y & 0xffff0000u)};
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          if ((__float_as_uint(v[e]) & 0x7f800000u) == 0x7f800000u) s.o[i >> 2][4 * (i & 3) + e] += v[e];
+        }
+      }
+    }
+  }
+}
+
 #endif  // __HIP_DEVICE_COMPILE__
 
 // What a call launches, by its sizes alone.
 struct PagedPlan {
   bool rows, tiles, row_parts, split;  // the forms that its windows may take, and which may be cut into parts
   int q_tiles;
+  bool planned;                        // by paged_plan_kernel: more windows than a wave has lanes
   int64_t tile_grid, tile_slots, row_slots, slot_rows, row_floats, tile_floats, plan_windows;
-  size_t bytes() const { return static_cast<size_t>(row_floats + tile_floats) * 4 + static_cast<size_t>(plan_windows) * 16; }
+  size_t bytes() const {
+    return static_cast<size_t>(row_floats + tile_floats) * 4 +
+           static_cast<size_t>(planned ? plan_windows * 24 + 16 : plan_windows * 16);
+  }
 };
 
 // FP8, KS: steps of 16 head_dim elements; whole: pages of kWholePages keys or more.

@@ -14,9 +14,10 @@ __global__ __launch_bounds__(kPagedThreads, 2) void paged_mixed_kernel(PagedArgs
   constexpr int kTile = TileLds<KS>::kBuffer;
   __shared__ __attribute__((aligned(16))) char s0[R::k0 > kTile ? R::k0 : kTile], s1[R::k1 > kTile ? R::k1 : kTile];
   __shared__ float s_ml[4][2][kRows];
+  __shared__ int s_odd;
   const int place = static_cast<int>(blockIdx.x);
   if (place < tile_grid) {
-    tile_work<FP8, WHOLE, KS>(a, place, s0, s1);
+    tile_work<FP8, WHOLE, KS>(a, place, s0, s1, &s_odd);
   } else {
     row_work<FP8, WHOLE, KS, 2>(a, place - tile_grid, s0, s1, s_ml);
   }

@@ -7,6 +7,59 @@ namespace svhip {
 
 [[maybe_unused]] constexpr int kRowKeys = 32;  // keys of a half of a wave's block
 
+// Keys of window c, or -1: not of this form.
+__device__ __forceinline__ int row_keys(const PagedArgs& a, int64_t c) {
+  int64_t first, count;
+  window_tokens(a.tokens, c, first, count);
+  return count > 0 && row_form(a, count) ? static_cast<int>(held_keys(a.pages, c)) : -1;
+}
+__device__ __forceinline__ int row_parts(int keys, int length) {
+  return keys < 0 ? 0 : (keys > length ? (keys - 1) / length + 1 : 1);
+}
+
+// The length of a part: the least, a multiple of kRowLeast (4 waves' blocks), for which the parts are at most kRowTarget more
+// than the (window, key head) pairs; kUncut if there are no places from `place` on. `mine`: keys of the team's own window.
+template <typename Team>
+__device__ __forceinline__ int row_length(const PagedArgs& a, const Team& team, int place, int& mine) {
+  float keys = 0.f, units = 0.f;
+  mine = -1;
+  for (int64_t c = team.id(); c < a.tokens.B; c += Team::kSize) {
+    mine = row_keys(a, c);
+    keys += mine > 0 ? static_cast<float>(mine) : 0.f;
+    units += mine >= 0 ? 1.f : 0.f;
+  }
+  const float Hkv = static_cast<float>(a.Hkv);
+  keys = team.sum(keys) * Hkv;
+  units = team.sum(units) * Hkv;
+  // (At most that many parts; a little more, since the sum of the keys is rounded.)
+  if (static_cast<float>(place) > units + keys * (1.01f / kRowLeast)) return kUncut;
+  const int own = mine;
+  return part_length(a, team, keys, static_cast<int>(units) + kRowTarget, kRowLeast, kRowLeast,
+                     [&](int c, int length) __attribute__((always_inline)) {
+                       const int n = a.tokens.B <= Team::kSize ? own : row_keys(a, c);
+                       return Hkv * static_cast<float>(row_parts(n, length));
+                     });
+}
+
+// The lengths are on the device, so the workgroups form the plan themselves, or read it.
+__device__ __forceinline__ PagedItem row_item(const PagedArgs& a, int place, int& each) {
+  const int Hkv = static_cast<int>(a.Hkv);
+  if (!a.row_part) {
+    const int b = place / Hkv;
+    return PagedItem{b < a.tokens.B ? b : -1, place - b * Hkv, 0, 1, 0, 1, place, 0};
+  }
+  if (a.running) {
+    const int4 sums = a.plan[a.tokens.B];
+    each = sums.z;
+    if (place >= sums.x) return PagedItem{-1, 0, 0, 1, 0, 1, 0, 0};
+    return planned_item(a, place, &a.running->x);
+  }
+  int mine;
+  each = __builtin_amdgcn_readfirstlane(row_length(a, WaveTeam{}, place, mine));
+  const int parts = row_parts(mine, each);
+  return item_at(Hkv, place, parts > 0 ? 1 : 0, parts);
+}
+
 // A wave takes every 4th block of 32 keys of its part (e4m3 up to head_dim 64: of 64 keys, as many bytes). K rows go straight
 // from memory to the A operands, a lane its own key's chunks, the next block's while the current one's softmax and second
 // product run; V rows go through the wave's LDS, since they are read transposed.
@@ -31,43 +84,15 @@ __device__ __forceinline__ void row_work(const PagedArgs& a, int place, char* sV
   constexpr int kWaveO = L::kWaveO;
   const int lane = threadIdx.x & 63, col = lane & 31, hh = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  // The parts: of the least length, a multiple of kRowLeast (4 waves' blocks), for which they are at most kRowTarget more than
-  // the (window, key head) pairs. The lengths are on the device, so every workgroup forms the plan for itself.
-  auto keys_of = [&](int64_t c) __attribute__((always_inline)) -> int {  // -1: not of this form
-    int64_t first, count;
-    window_tokens(a.tokens, c, first, count);
-    return count > 0 && row_form(a, count) ? static_cast<int>(held_keys(a.pages, c)) : -1;
-  };
-  float sum = 0.f, units = 0.f;
-  int mine = -1;
-  for (int64_t c = lane; c < a.tokens.B; c += 64) {
-    mine = keys_of(c);
-    sum += mine > 0 ? static_cast<float>(mine) : 0.f;
-    units += mine >= 0 ? 1.f : 0.f;
-  }
-  const bool one = a.tokens.B <= 64;  // the lane's window is still at hand
-  auto parts_of = [&](int c, int length) __attribute__((always_inline)) -> int {
-    const int n = one ? mine : keys_of(c);
-    return n < 0 ? 0 : (n > length ? (n - 1) / length + 1 : 1);
-  };
-  const float Hkv = static_cast<float>(a.Hkv);
-  auto places = [&](int c, int length) __attribute__((always_inline)) {
-    return Hkv * static_cast<float>(parts_of(c, length));
-  };
-  const int target = static_cast<int>(wave_sum(units) * Hkv) + kRowTarget;
-  const int each =
-      __builtin_amdgcn_readfirstlane(part_length(a, wave_sum(sum) * Hkv, target, kRowLeast, kRowLeast, places));
-  const PagedItem item = item_at(a, place, [&](int c, int& tiles, int& parts)
-                                                                      __attribute__((always_inline)) {
-    parts = parts_of(c, each);
-    tiles = parts > 0 ? 1 : 0;
-  });
+  int each = kUncut;
+  const PagedItem item = row_item(a, place, each);
   const int b = __builtin_amdgcn_readfirstlane(item.b);
   if (b < 0) return;
   const int kvh = __builtin_amdgcn_readfirstlane(item.kvh), part = __builtin_amdgcn_readfirstlane(item.part);
   const int parts = __builtin_amdgcn_readfirstlane(item.parts);
-  if (a.plan && part == 0 && kvh == 0 && threadIdx.x == 0) a.plan[b] = make_int4(item.before, parts, each, 1);
+  if (a.row_part && !a.running && part == 0 && kvh == 0 && threadIdx.x == 0) a.plan[b] = make_int4(item.before, parts, each, 1);
   const Window w = window_at(a, b);
+  if (w.count <= 0 || !row_form(a, w.count)) return;  // (uncut windows stand by their numbers)
   const int rows = static_cast<int>(w.count * a.G);
   const int keys = __builtin_amdgcn_readfirstlane(w.keys);
   const int k0 = part * each, k1 = keys - k0 > each ? k0 + each : keys;
@@ -79,6 +104,9 @@ __device__ __forceinline__ void row_work(const PagedArgs& a, int place, char* sV
   const Source ks = k_source<ES>(a, kvh), vs = v_source<ES>(a, kvh);
   const int32_t* row = a.pages.table + b * a.pages.st_b;
   const int all = __builtin_amdgcn_readfirstlane(last_key(a, w, 0));
+  // Blocks that end past it are seen in part (clean_values), if a later token sees more.
+  const int clean_from = all + 1 < keys ? all + 1 - kKeys : kUncut;
+  bool odd = false;
   const int in_mask = (1 << a.pages.shift) - 1, D = static_cast<int>(a.D);
   // Groups of a block's keys that lie in one page for sure: all of it (WHOLE), or 16 keys.
   constexpr int kGroup = WHOLE ? kKeys : 16, kGroups = kKeys / kGroup;
@@ -204,6 +232,9 @@ __device__ __forceinline__ void row_work(const PagedArgs& a, int place, char* sV
           wait_vmem();
         }
       }
+      if (kv > clean_from) {
+        odd |= __builtin_amdgcn_ballot_w64(clean_values(cur, kTileBytes, 16 * lane, 16 * 64)) != 0ull;
+      }
       bound_scores<KS, kHalves>(s, x, a.scale_log2, kv + kKeys - 1 > all, kv);
 #pragma unroll
       for (int t = 0; t < kHalves; ++t) {
@@ -217,6 +248,11 @@ __device__ __forceinline__ void row_work(const PagedArgs& a, int place, char* sV
     while (kv < k1) {
       step(c0, c1);
       if (!FP8 && kv < k1) step(c1, c0);
+    }
+  }
+  if (odd) {
+    for (kv = k0 + wave * kKeys; kv < k1; kv += stride) {
+      if (kv > clean_from) add_odd_values<FP8, KS>(a, vs, row, kv, kv + kKeys < k1 ? kv + kKeys : k1, s);
     }
   }
   // The waves' sums joined, in order: O of wave w [head_dim][row].

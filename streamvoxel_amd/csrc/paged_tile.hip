@@ -7,7 +7,8 @@ template <bool FP8, bool WHOLE, int KS>
 __global__ __launch_bounds__(kPagedThreads, FP8 || KS > 4 ? 2 : 4) void paged_tile_kernel(PagedArgs a) {
 #if defined(__HIP_DEVICE_COMPILE__)
   __shared__ __attribute__((aligned(16))) char s0[TileLds<KS>::kBuffer], s1[TileLds<KS>::kBuffer];
-  tile_work<FP8, WHOLE, KS>(a, static_cast<int>(blockIdx.x), s0, s1);
+  __shared__ int s_odd;
+  tile_work<FP8, WHOLE, KS>(a, static_cast<int>(blockIdx.x), s0, s1, &s_odd);
 #endif
 }
 

@@ -13,6 +13,8 @@ __device__ __forceinline__ void tiles_of_window(const PagedArgs& a, int64_t c, i
   blocks = count > 0 ? static_cast<int>((held_keys(a.pages, c) + kKB - 1) / kKB) : 0;
 }
 
+__device__ __forceinline__ int tile_parts(int blocks, int length) { return blocks > length ? (blocks - 1) / length + 1 : 1; }
+
 // Even windows that fill the chip by themselves (split false): XCD id % 8 takes every 8th (window, key head) with all its
 // tiles, so that its L2 reads the keys once; the windows longest first (up to 64 of them), and every other round of an XCD's
 // CUs in reverse, which evens out the CUs' sums.
@@ -46,44 +48,57 @@ __device__ __forceinline__ PagedItem whole_item(const PagedArgs& a, int place) {
 // Otherwise the tiles stand one window after the other. Fewer than kTileTarget of them share out their keys: into parts of the
 // least number of blocks, kTileLeast at least, for which the parts are at most kTileTarget and run side by side; at most
 // kTileBeside where the row form's windows read half as many blocks or more (they then have the other half of every CU: a
-// block takes about 1 us of either's CU; 24 mixed windows 101 us for 110). An XCD then takes a run of consecutive places, so
-// that the tiles of a part meet in its L2.
-__device__ __forceinline__ PagedItem shared_item(const PagedArgs& a, int place, int& each) {
-  const int lane = threadIdx.x & 63, Hkv = static_cast<int>(a.Hkv);
+// block takes about 1 us of either's CU; 24 mixed windows 101 us for 110). kUncut: no parts. `tiles`, `blocks`: of the team's
+// own window; `total`: the tiles.
+template <typename Team>
+__device__ __forceinline__ int tile_length(const PagedArgs& a, const Team& team, int& tiles, int& blocks, float& total) {
+  const float Hkv = static_cast<float>(a.Hkv);
   float units = 0.f, work = 0.f, beside = 0.f;
-  int tiles = 0, blocks = 0;
-  for (int64_t c = lane; c < a.tokens.B; c += 64) {
+  tiles = blocks = 0;
+  for (int64_t c = team.id(); c < a.tokens.B; c += Team::kSize) {
     tiles_of_window(a, c, tiles, blocks);
     units += static_cast<float>(tiles);
     work += static_cast<float>(tiles) * static_cast<float>(blocks);
     beside += tiles == 0 ? static_cast<float>(blocks) : 0.f;
   }
-  units = wave_sum(units) * static_cast<float>(Hkv);
-  work = wave_sum(work) * static_cast<float>(Hkv);
-  const int target = wave_sum(beside) * static_cast<float>(2 * Hkv) >= work && work > 0.f ? kTileBeside : kTileTarget;
-  const bool split = units < static_cast<float>(target), one = a.tokens.B <= 64;  // one: the lane's window is still at hand
-  auto count = [&](int c, int length, int& t, int& parts) __attribute__((always_inline)) {
-    int nb = blocks;
-    t = tiles;
-    if (!one) tiles_of_window(a, c, t, nb);
-    parts = nb > length ? (nb - 1) / length + 1 : 1;
-  };
-  auto places = [&](int c, int length) __attribute__((always_inline)) {
-    int t, parts;
-    count(c, length, t, parts);
-    return static_cast<float>(t * Hkv) * static_cast<float>(parts);
-  };
-  each = split ? part_length(a, work, target, 1, kTileLeast, places) : kUncut;
-  each = __builtin_amdgcn_readfirstlane(each);
-  int at = place;
-  if (split) {
-    float total = 0.f;
-    for (int64_t c = lane; c < a.tokens.B; c += 64) total += places(static_cast<int>(c), each);
-    const int run = (static_cast<int>(wave_sum(total)) + kXcds - 1) / kXcds;
-    if ((at >> 3) >= run) return PagedItem{-1, 0, 0, 1, 0, 1, 0, 0};
-    at = (at & 7) * run + (at >> 3);
+  total = team.sum(units) * Hkv;
+  if (total == 0.f) return kUncut;
+  work = team.sum(work) * Hkv;
+  const int target = 2.f * Hkv * team.sum(beside) >= work ? kTileBeside : kTileTarget;
+  if (total >= static_cast<float>(target)) return kUncut;
+  const int own_tiles = tiles, own_blocks = blocks;
+  return part_length(a, team, work, target, 1, kTileLeast, [&](int c, int length) __attribute__((always_inline)) {
+    int t = own_tiles, n = own_blocks;
+    if (a.tokens.B > Team::kSize) tiles_of_window(a, c, t, n);
+    return Hkv * static_cast<float>(t) * static_cast<float>(tile_parts(n, length));
+  });
+}
+
+// An XCD takes a run of consecutive places of parts, so that the tiles of a part meet in its L2.
+__device__ __forceinline__ int shared_place(int place, int total, int each) {
+  if (each == kUncut) return place < total ? place : -1;
+  const int run = (total + kXcds - 1) / kXcds, at = (place & 7) * run + (place >> 3);
+  return (place >> 3) < run && at < total ? at : -1;
+}
+
+__device__ __forceinline__ PagedItem shared_item(const PagedArgs& a, int place, int& each) {
+  const PagedItem none{-1, 0, 0, 1, 0, 1, 0, 0};
+  if (a.running) {
+    const int4 sums = a.plan[a.tokens.B];
+    each = sums.w;
+    const int at = shared_place(place, sums.y, each);
+    return at < 0 ? none : planned_item(a, at, &a.running->y);
   }
-  return item_at(a, at, [&](int c, int& t, int& parts) __attribute__((always_inline)) { count(c, each, t, parts); });
+  const int Hkv = static_cast<int>(a.Hkv);
+  int tiles, blocks;
+  float total;
+  each = __builtin_amdgcn_readfirstlane(tile_length(a, WaveTeam{}, tiles, blocks, total));
+  if (total == 0.f) return none;
+  const int parts = tile_parts(blocks, each);
+  int sum;
+  wave_prefix(tiles * Hkv * parts, sum);
+  const int at = shared_place(place, sum, each);
+  return at < 0 ? none : item_at(Hkv, at, tiles, parts);
 }
 
 // Two buffers of a block of K and a block of V.
@@ -96,7 +111,7 @@ struct TileLds {
 #if defined(__HIP_DEVICE_COMPILE__)
 
 template <bool FP8, bool WHOLE, int KS>
-__device__ __forceinline__ void tile_work(const PagedArgs& a, int place, char* s0, char* s1) {
+__device__ __forceinline__ void tile_work(const PagedArgs& a, int place, char* s0, char* s1, int* s_odd) {
   constexpr int DT = tiles_of(KS), ES = FP8 ? 1 : 2;
   constexpr int kSubBytes = TileLds<KS>::kSubBytes, kTileBytes = TileLds<KS>::kTileBytes;
   char *sK0 = s0, *sV0 = s0 + kTileBytes, *sK1 = s1, *sV1 = s1 + kTileBytes;
@@ -113,7 +128,7 @@ __device__ __forceinline__ void tile_work(const PagedArgs& a, int place, char* s
   const int keys = __builtin_amdgcn_readfirstlane(tile_keys(a, w, qt));
   const int blocks = (keys + kKB - 1) / kKB;
   const int count = blocks > each ? (blocks - 1) / each + 1 : 1;
-  if (a.split && part == 0 && kvh == 0 && qt == 0 && threadIdx.x == 0) {
+  if (a.split && !a.running && part == 0 && kvh == 0 && qt == 0 && threadIdx.x == 0) {
     a.plan[b] = make_int4(item.before, item.parts, each, item.tiles);
   }
   if (part >= count || (count > 1 && item.at >= a.tile_slots)) return;  // (borders not ascending)
@@ -141,6 +156,9 @@ __device__ __forceinline__ void tile_work(const PagedArgs& a, int place, char* s
   const int64_t wr0 = r0 + wave * kRows, wr1 = wr0 + kRows < rows ? wr0 + kRows : rows;
   const int all = __builtin_amdgcn_readfirstlane(wr0 < rows ? last_key(a, w, wr0 / a.G) : -1);
   const int any = __builtin_amdgcn_readfirstlane(wr0 < rows ? last_key(a, w, (wr1 - 1) / a.G) : -1);
+  // Every row of the tile sees the keys up to `seen`; blocks past it are seen in part (clean_values).
+  const int seen = __builtin_amdgcn_readfirstlane(last_key(a, w, r0 / a.G));
+  const int clean_from = seen + 1 < keys ? (seen + 1) / kKB : kUncut;
 
   // The wave stages rows 8 wave .. and 8 wave + 32 .. of a block: of one page (WHOLE), or of the 16 keys around each.
   constexpr int kGroup = WHOLE ? 64 : 16, kGroups = WHOLE ? 1 : 2;
@@ -207,6 +225,7 @@ __device__ __forceinline__ void tile_work(const PagedArgs& a, int place, char* s
     }
   };
   if (blk0 < blk1) {
+    if (threadIdx.x == 0) *s_odd = 0;
     find(kKB * blk0);
     issue(kKB * blk0, sK0, sV0);
     find(kKB * (blk0 + 1));
@@ -217,6 +236,10 @@ __device__ __forceinline__ void tile_work(const PagedArgs& a, int place, char* s
       const bool more = blk + 1 < blk1;
       if (more) issue(kKB * (blk + 1), nK, nV);
       find(kKB * (blk + 2));
+      if (blk >= clean_from) {
+        if (clean_values(cV, kTileBytes, 16 * static_cast<int>(threadIdx.x), 16 * kPagedThreads)) *s_odd = 1;
+        __syncthreads();
+      }
       compute(kKB * blk, cK, cV);
       if (more) {
         commit(nK, nV);
@@ -227,6 +250,10 @@ __device__ __forceinline__ void tile_work(const PagedArgs& a, int place, char* s
     for (int blk = blk0; blk < blk1; blk += 2) {
       step(blk, sK0, sV0, sK1, sV1);
       if (blk + 1 < blk1) step(blk + 1, sK1, sV1, sK0, sV0);
+    }
+    if (clean_from < blk1 && *s_odd != 0) {
+      add_odd_values<FP8, KS>(a, vs, row, kKB * (clean_from > blk0 ? clean_from : blk0),
+                              kKB * blk1 < keys ? kKB * blk1 : keys, s);
     }
   }
   const float l = row_sum(s.l[0]);

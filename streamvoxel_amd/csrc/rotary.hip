@@ -184,7 +184,8 @@ extern "C" int svhip_rotary(const svhip_rotary_args* args, void* stream) {
   clear_error();
   SVHIP_REQUIRE(args, "%s: null arguments", name);
   const svhip_rotary_args& c = *args;
-  SVHIP_REQUIRE(c.B >= 0 && c.H >= 0 && c.N >= 0 && c.D >= 1, "%s: bad sizes", name);
+  SVHIP_REQUIRE(c.B >= 0 && c.B < (1ll << 31) && c.H >= 0 && c.N >= 0 && c.N < (1ll << 31) && c.D >= 1, "%s: bad sizes",
+                name);
   SVHIP_REQUIRE(c.dtype == SVHIP_F32 || c.dtype == SVHIP_BF16, "%s: dtype %d unsupported", name, (int)c.dtype);
   SVHIP_REQUIRE(c.layout == SVHIP_ROTARY_HALF || c.layout == SVHIP_ROTARY_INTERLEAVED, "%s: layout %d unsupported", name,
                 (int)c.layout);

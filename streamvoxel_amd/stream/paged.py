@@ -62,7 +62,7 @@ def _rows16(t):
     """bf16 rows on 16-byte boundaries: the tensor itself, or a contiguous copy."""
     if t.stride(-1) == 1 and t.data_ptr() % 16 == 0 and all(s % 8 == 0 for s in t.stride()[:-1]):
         return t
-    return t.contiguous() if not t.is_contiguous() or t.data_ptr() % 16 else t.clone()
+    return t.clone() if t.is_contiguous() else t.contiguous()
 
 
 _CACHE = struct.Struct('7P18q')    # svhip_paged_cache
@@ -113,6 +113,8 @@ def paged_append(key, value, k_pages, v_pages, page_table, lengths, cu_tokens=No
         raise ValueError('key and value must be alike, with the heads and the head_dim of the pages')
     if before < 0:
         raise ValueError('before counts keys')
+    if _lib.stacked(k_pages) or _lib.stacked(v_pages):
+        raise ValueError('k_pages and v_pages must have a place for every element')
     wide, pairs, sp, turn = 0, 0, (0, 0), _lib.SVHIP_ROTARY_NONE
     if frequencies is not None:
         if layout not in ('half', 'interleaved', 'axial'):
@@ -153,7 +155,8 @@ def paged_attention(query, k_pages, v_pages, page_table, lengths, cu_queries=Non
     int32 [B+1] (device, ascending). k_pages, v_pages, page_table, lengths and the exponents as `paged_append` fills them;
     the H heads share the pages' heads evenly, head h reads head h // (H / heads). `causal`: the n tokens are the window's
     last n keys, and token i sees keys up to its own, lengths[b] - n + i; without it every token sees all of them. A token
-    with no key gets zeros. `out` (optional) bf16 like query with a contiguous head_dim; its rows outside every window are
+    with no key gets zeros, and what is not finite among keys that a token does not see does not reach it. `out` (optional; query
+    itself, or memory that query does not share) bf16 like query with a contiguous head_dim; its rows outside every window are
     left as they are (a fresh one has them undefined). `bad` (optional int32 [1], device) becomes 1 when a page lies
     outside the pool (its keys and values read as zeros) or a length passes the window's row of the table (and is cut).
     Returns out."""
@@ -161,7 +164,7 @@ def paged_attention(query, k_pages, v_pages, page_table, lengths, cu_queries=Non
     code = _check_pool(k_pages, v_pages, page_table, lengths, k_exponents, v_exponents, bad)
     if query.dtype != torch.bfloat16:
         raise TypeError('query must be bfloat16')
-    query = _rows16(query)
+    given, query = query, _rows16(query)
     B = page_table.shape[0]
     H, n, sq = _windows(query, cu_queries, B, 'query')
     P, Hkv, S, D = k_pages.shape
@@ -169,8 +172,10 @@ def paged_attention(query, k_pages, v_pages, page_table, lengths, cu_queries=Non
         raise ValueError("query needs the pages' head_dim, and heads that share theirs evenly")
     if out is None:
         out = torch.empty_like(query)
-    elif out.shape != query.shape or out.dtype != torch.bfloat16 or out.stride(-1) != 1:
-        raise ValueError('out must be bf16 like query with a contiguous head_dim')
+    elif out.shape != query.shape or out.dtype != torch.bfloat16 or out.stride(-1) != 1 or _lib.stacked(out):
+        raise ValueError('out must be bf16 like query with a contiguous head_dim and a place for every element')
+    elif _lib.overlaps(given, out) and (given.data_ptr() != out.data_ptr() or given.stride() != out.stride()):
+        raise ValueError('out must be query itself or memory that query does not share')
     so = _windows(out, cu_queries, B, 'out')[2]
     scale = 1.0 / math.sqrt(D) if scale is None else float(scale)
     nbytes = _lib.load().svhip_paged_attention_workspace_bytes(B, H, Hkv, n, cu_queries is not None, D,

@@ -103,8 +103,8 @@ def rotary(x, positions, frequencies, layout='half', amplitude=1.0, out=None):
     else:
         if torch.is_grad_enabled() and (x.requires_grad or out.requires_grad):
             raise ValueError('out= takes no part in a gradient')
-        if out.shape != x.shape or out.dtype != x.dtype or out.stride(-1) != 1:
-            raise ValueError("out must have x's shape and type and a contiguous head_dim")
+        if out.shape != x.shape or out.dtype != x.dtype or out.stride(-1) != 1 or _lib.stacked(out):
+            raise ValueError("out must have x's shape and type, a contiguous head_dim and a place for every element")
         if _lib.overlaps(x, out) and (x.data_ptr() != out.data_ptr() or x.stride() != out.stride()):
             raise ValueError('out must be x itself or memory that x does not share')
     return _launch(x, out, positions, frequencies, layout, float(amplitude), 0)

@@ -691,3 +691,120 @@ def test_engine_over_a_shared_pool(kv_dtype):
         paged.extend_slot(0, torch.zeros(1, 200, 192, device=DEV), torch.zeros(1, 200, 3, device=DEV))
     with pytest.raises(IndexError):
         paged.extend_slot(3, local, positions)
+
+
+@pytest.mark.parametrize('kv_dtype', ['bf16', 'fp8'])
+@pytest.mark.parametrize('D, heads, page', [(64, 1, 64), (128, 2, 16)])
+@pytest.mark.parametrize('n, at, packed', [(3, 1, False), (16, 9, False), (40, 17, False), (200, 70, False), (200, 199, True),
+                                           (32, 1, True)])
+def test_what_a_token_does_not_see_does_not_reach_it(n, at, packed, D, heads, page, kv_dtype):
+    """A key and a value of the chunk's token `at` that are not finite: the tokens in front of it are as if it were not there,
+    it and the later ones have the formula's NaN and infinities."""
+    from streamvoxel_amd.stream.paged import paged_attention
+    _case(f'values that are not finite: n={n} at={at} packed={packed} D={D} page={page} {kv_dtype}')
+    L = 700
+    j = L - n + at
+    for what in ('v', 'k', 'inf'):
+        if what == 'inf' and kv_dtype == 'fp8':
+            continue   # (no code for it)
+        pool = Pool([900, L], heads, D, page, n + D, kv_dtype, clean=True)
+        q = queries(2, 2 * heads, n, D, n)
+        row = (pool.table[1, j // page].long(), slice(None), j % page)
+        if what == 'k':
+            pool.k[row] = torch.full((heads, D), math.nan).to(pool.k.dtype)
+        else:
+            v = torch.where(torch.arange(D) == 5, math.inf if what == 'inf' else math.nan, pool.v[row].float())
+            pool.v[row] = v.to(pool.v.dtype)
+        cu, qq = None, q
+        if packed:
+            cu = torch.tensor([0, n, 2 * n], dtype=torch.int32, device=DEV)
+            qq = torch.cat((q[0], q[1]), 1)
+        got = paged_attention(qq, *pool.args(), cu_queries=cu, causal=True, **pool.exponents())
+        if packed:
+            got = torch.stack((got[:, :n], got[:, n:]))
+        k, v = pool.rows(1)
+        want, err = attend64(q[1, :, :at].cpu().double(), k[:, :j], v[:, :j], True, D ** -0.5)
+        assert ((got[1, :, :at].cpu().double() - want).abs() <= err).all()
+        check(got[:1], q[:1], _window(pool, 0), True)
+        late = got[1, :, at:].cpu()
+        if what == 'k':
+            assert torch.isnan(late).all()
+            continue
+        assert (torch.isnan if what == 'v' else torch.isposinf)(late[..., 5]).all()
+        k, v = k, v.masked_fill(torch.arange(D) == 5, 0.0)
+        want, err = attend64(q[1].cpu().double(), k, v, True, D ** -0.5)
+        rest = torch.arange(D) != 5
+        assert ((late.double() - want[:, at:]).abs() <= err[:, at:])[..., rest].all()
+
+
+@pytest.mark.parametrize('kv_dtype', ['bf16', 'fp8'])
+@pytest.mark.parametrize('B', [65, 200, 1100])
+@pytest.mark.parametrize('kind', ['tokens', 'chunks', 'packed'])
+def test_many_windows(kind, B, kv_dtype):
+    """More windows than a workgroup plans by itself: short ones, empty ones, a few long enough for parts."""
+    from streamvoxel_amd.stream.paged import paged_attention
+    _case(f'many windows: {kind} B={B} {kv_dtype}')
+    lengths = [(0, 1, 40, 17, 64, 3, 100)[b % 7] if b % 60 != 31 else 900 + b for b in range(B)]
+    pool = Pool(lengths, 1, 16, 16, B, kv_dtype)
+    if kind != 'packed':
+        n = 1 if kind == 'tokens' else 33
+        q = queries(B, 2, n, 16, B)
+        check(paged_attention(q, *pool.args(), causal=True, **pool.exponents()), q, pool, True)
+        return
+    counts = [(1, 0, 5, 1, 40, 1, 17)[b % 7] if b % 60 != 31 else (130 if b % 120 == 31 else 1) for b in range(B)]
+    cu = [0]
+    for c in counts:
+        cu.append(cu[-1] + c)
+    g = torch.Generator().manual_seed(B)
+    q = torch.randn(2, cu[-1], 16, generator=g).to(torch.bfloat16).to(DEV)
+    got = paged_attention(q, *pool.args(), cu_queries=torch.tensor(cu, dtype=torch.int32, device=DEV), causal=True,
+                          **pool.exponents())
+    check(got, q, pool, True, cu)
+    one = paged_attention(q[:, cu[31]:cu[32]].contiguous(), *[t[31:32] if i > 1 else t for i, t in enumerate(pool.args())],
+                          cu_queries=torch.tensor([0, counts[31]], dtype=torch.int32, device=DEV), causal=True,
+                          **pool.exponents())
+    check(one, q[:, cu[31]:cu[32]], _window(pool, 31), True, [0, counts[31]])
+
+
+def _window(pool, b):
+    kept = Pool.__new__(Pool)
+    kept.__dict__.update(pool.__dict__, lengths=pool.lengths[b:b + 1], table=pool.table[b:b + 1])
+    return kept
+
+
+def test_rows_off_their_alignment_are_copied():
+    """Contiguous queries, keys and values that start between 16-byte boundaries."""
+    from streamvoxel_amd.stream.paged import paged_append, paged_attention
+    pool = Pool([40, 30], 2, 64, 16, 1, clean=True)
+    k, v, table, lengths = pool.args()
+    g = torch.Generator().manual_seed(2)
+    flat = torch.randn(2, 2 * 2 * 3 * 64 + 1, generator=g).to(torch.bfloat16).to(DEV)
+    key, value = [t[1:].view(2, 2, 3, 64) for t in flat]
+    assert key.is_contiguous() and key.data_ptr() % 16
+    check(paged_attention(key, k, v, table, lengths), key, pool, False)
+    paged_append(key, value, k, v, table, lengths)
+    for b, L in ((0, 40), (1, 30)):
+        at = torch.arange(L - 3, L, device=DEV)
+        page = table[b].long()[at // 16]
+        assert torch.equal(k[page, :, at % 16], key[b].transpose(0, 1))
+        assert torch.equal(v[page, :, at % 16], value[b].transpose(0, 1))
+
+
+@pytest.mark.parametrize('n', [1, 50])
+def test_out_over_the_query_and_refused_places(n):
+    from streamvoxel_amd.stream.paged import paged_append, paged_attention
+    pool = Pool([1500, 30], 2, 64, 16, 1, clean=True)
+    args = pool.args()
+    q = queries(2, 4, n, 64, 3)
+    want = paged_attention(q, *args, causal=True)
+    over = q.clone(memory_format=torch.preserve_format)
+    assert paged_attention(over, *args, causal=True, out=over) is over
+    assert torch.equal(over, want)
+    room = torch.zeros(2, 4, n + 1, 64, dtype=torch.bfloat16, device=DEV)
+    with pytest.raises(ValueError, match='share'):
+        paged_attention(room[:, :, :n], *args, out=room[:, :, 1:])
+    with pytest.raises(ValueError, match='place'):
+        paged_attention(q, *args, out=room[:, :1, :n].expand(2, 4, n, 64))
+    key = queries(2, 2, n, 64, 4)
+    with pytest.raises(ValueError, match='place'):
+        paged_append(key, key, args[0][:1].expand(args[0].shape), args[1], *args[2:])

@@ -164,3 +164,5 @@ def test_rotary_refuses_on_the_gpu():
     buffer = torch.zeros(1, 2, 4, 8, device=DEV)
     with pytest.raises(ValueError, match='share'):
         rotary(buffer[:, :, :3], p, f, out=buffer[:, :, 1:])
+    with pytest.raises(ValueError, match='place'):
+        rotary(buffer[:, :, :3].clone(), p, f, out=torch.zeros(1, 1, 3, 8, device=DEV).expand(1, 2, 3, 8))

@@ -199,3 +199,20 @@ def test_pages_of_an_engine_need_its_paged_context():
     assert check_engine_options('gather', 'flex', False) is None
     with pytest.raises(RuntimeError, match='HIP'):
         SlotEngine(None, None, 'cpu', 1, 1, 1, pages=4)
+
+
+def test_sizes_that_would_not_fit_the_kernels_counts(lib):
+    """Key numbers, a few blocks past the last of them, stay below 2^31; windows, tokens and heads are bounded."""
+    error = lib.svhip_last_error
+    for call in (append_call, attend_call):
+        for m, page in (((1 << 24) + 1, 64), ((1 << 20) + 1, 1024)):
+            assert call(lib, m=m, page=page) == -1 and b'page counts' in error()
+        for kw in (dict(B=1 << 31), dict(H=(1 << 20) + 1), dict(N=1 << 31)):
+            assert call(lib, **kw) == -1 and b'sizes' in error()
+    assert append_call(lib, before=1 << 31) == -1 and b'sizes' in error()
+    for sizes in ((1 << 31, 1, 1, 8), (1, 1, 1 << 31, 8)):
+        args = struct.pack('4P17qd', FAKE, FAKE, FAKE, FAKE, 1, 0, 4, 1, 0, *sizes, *[8] * 6, 0, 1, 1.0)
+        assert lib.svhip_rotary(args, None) == -1 and b'sizes' in error()
+    need = lib.svhip_paged_attention_workspace_bytes
+    assert need(2, 4, 2, 3, 0, 64, (1 << 30) + 1) == need(1 << 31, 4, 2, 3, 0, 64, 1280) == 0
+    assert need(2, 1 << 20, 2, 1 << 21, 0, 64, 1280) == 0
