@@ -122,7 +122,7 @@ __global__ __launch_bounds__(kAppendThreads) void paged_append_kernel(AppendArgs
   int64_t b = 0, n = mine;
   if (tid < tokens) {
     if (!a.tokens.cu) {
-      b = mine / a.tokens.N;
+      b = static_cast<int>(mine) / static_cast<int>(a.tokens.N);
       n = mine - b * a.tokens.N;
     }
     s_src[tid][0] = b * a.sk_b + n * a.sk_n;         // packed: b is 0 here
@@ -277,7 +277,7 @@ extern "C" int svhip_paged_append(const svhip_paged_cache* cache, const svhip_pa
   // Few tokens: one for each workgroup, so that they fill the chip.
   const int per_group = total <= 2 * 256 ? 1 : kAppendTokens;
   const int64_t groups = cdiv(total, per_group);
-  SVHIP_REQUIRE(groups < (1ll << 31), "%s: grid too large", name);
+  SVHIP_REQUIRE(total < (1ll << 31), "%s: sizes too large", name);
   const float amplitude = static_cast<float>(c.amplitude), most = amplitude < 0.f ? -amplitude : amplitude;
   const bool fp8 = p.kv_dtype == SVHIP_FP8_E4M3;
   const AppendArgs a{static_cast<const uint16_t*>(c.key), static_cast<const uint16_t*>(c.value), c.sk_b, c.sk_h, c.sk_n,

@@ -26,7 +26,7 @@ __global__ __launch_bounds__(kPlanThreads) void paged_plan_kernel(PagedArgs a, b
   __shared__ float of_wave[kPlanThreads / 64];
   __shared__ int2 counts[kPlanThreads / 64];
   const BlockTeam team{of_wave};
-  const int tid = static_cast<int>(threadIdx.x), Hkv = static_cast<int>(a.Hkv);
+  const int tid = static_cast<int>(threadIdx.x), Hkv = a.Hkv;
   int unused, more;
   float total;
   const int row_each = rows && a.row_part ? row_length(a, team, 0, unused) : kUncut;
@@ -86,16 +86,16 @@ __global__ __launch_bounds__(kPagedThreads) void paged_join_kernel(PagedArgs a) 
     if (sums.z == kUncut && sums.w == kUncut) return;  // no parts
   }
   const int group = threadIdx.x / 32, d0 = 4 * (threadIdx.x % 32);
-  const int64_t id = kGroups > 1 ? blockIdx.x : static_cast<int64_t>(blockIdx.x) * (kPagedThreads / 32) + group;
-  const int64_t total = (a.tokens.cu ? a.tokens.N : a.tokens.B * a.tokens.N);
-  const int64_t token = id / a.H, h = id - token * a.H;
+  const int id = static_cast<int>(kGroups > 1 ? blockIdx.x : blockIdx.x * (kPagedThreads / 32) + group);
+  const int total = static_cast<int>(a.tokens.cu ? a.tokens.N : a.tokens.B * a.tokens.N);
+  const int token = id / a.H, h = id - token * a.H;
   int64_t b = -1;
-  if (token < total) b = a.tokens.cu ? (a.tokens.B > 64 ? window_of(a.tokens, token) : -1) : token / a.tokens.N;
+  if (token < total) b = a.tokens.cu ? (a.tokens.B > 64 ? window_of(a.tokens, token) : -1) : token / static_cast<int>(a.tokens.N);
   if (a.tokens.cu && a.tokens.B <= 64) {
     // Up to 64 borders are read at once; a wave has the tokens of its two groups.
     const int lane = threadIdx.x & 63, B = static_cast<int>(a.tokens.B);
-    const int64_t from = a.tokens.cu[0], to = lane < B ? a.tokens.cu[1 + lane] : INT64_MAX;
-    const int64_t other = __shfl(token, lane ^ 32);
+    const int from = a.tokens.cu[0], to = lane < B ? a.tokens.cu[1 + lane] : INT_MAX;
+    const int other = __shfl(token, lane ^ 32);
     const int n0 = __builtin_popcountll(__builtin_amdgcn_ballot_w64(to <= (lane < 32 ? token : other)));
     const int n1 = __builtin_popcountll(__builtin_amdgcn_ballot_w64(to <= (lane < 32 ? other : token)));
     const int n = lane < 32 ? n0 : n1;
@@ -107,27 +107,27 @@ __global__ __launch_bounds__(kPagedThreads) void paged_join_kernel(PagedArgs a) 
   const Window w = window_at(a, b);
   if (w.count <= 0) return;
   if (token < w.first || token - w.first >= w.count) return set_bad(a.pages);  // borders not ascending
-  const int64_t i = token - w.first, kvh = h / a.G, r = i * a.G + (h - kvh * a.G);
+  const int i = static_cast<int>(token - w.first), kvh = h / a.G, r = i * a.G + (h - kvh * a.G);
   const float* slot;
   int64_t step;
   int count;
   if (row_form(a, w.count)) {
     if (!a.row_part) return;
     count = plan.y;
-    if (plan.x < 0 || count < 0 || plan.x + a.Hkv * count > a.row_slots) return set_bad(a.pages);  // borders not ascending
-    slot = a.row_part + ((plan.x + kvh * count) * a.slot_rows + r) * (a.D + 2);
-    step = a.slot_rows * (a.D + 2);
+    if (plan.x < 0 || count < 0 || plan.x + static_cast<int64_t>(a.Hkv) * count > a.row_slots) return set_bad(a.pages);  // borders not ascending
+    slot = a.row_part + (static_cast<int64_t>(plan.x + kvh * count) * a.slot_rows + r) * (a.D + 2);
+    step = static_cast<int64_t>(a.slot_rows) * (a.D + 2);
   } else {
     if (!a.split) return;
-    const int64_t qt = r / kTileRows, blocks = (tile_keys(a, w, qt) + kKB - 1) / kKB;
+    const int qt = r / kTileRows, blocks = (tile_keys(a, w, qt) + kKB - 1) / kKB;
     const int each = plan.z, tiles = plan.w;
     if (each < 1) return set_bad(a.pages);
-    count = static_cast<int>(blocks > each ? cdiv(blocks, each) : 1);
+    count = blocks > each ? (blocks - 1) / each + 1 : 1;
     if (count < 2) return;
-    if (plan.x < 0 || plan.y < count || tiles <= qt || plan.x + a.Hkv * plan.y * tiles > a.tile_slots) {
+    if (plan.x < 0 || plan.y < count || tiles <= qt || plan.x + static_cast<int64_t>(a.Hkv) * plan.y * tiles > a.tile_slots) {
       return set_bad(a.pages);
     }
-    slot = a.tile_part + ((plan.x + kvh * plan.y * tiles + qt) * kTileRows + (r - qt * kTileRows)) * (a.D + 2);
+    slot = a.tile_part + (static_cast<int64_t>(plan.x + kvh * plan.y * tiles + qt) * kTileRows + (r - qt * kTileRows)) * (a.D + 2);
     step = static_cast<int64_t>(tiles) * kTileRows * (a.D + 2);
   }
   if (count < 2) return;
@@ -252,13 +252,15 @@ extern "C" int svhip_paged_attention(const svhip_paged_cache* cache, const svhip
                                    reinterpret_cast<uintptr_t>(c.workspace) % 16 == 0),
                 "%s: workspace too small or misaligned (%lld < %zu bytes)", name, (long long)c.workspace_bytes, p.bytes());
   const int64_t rows = (c.cu_queries ? N : B * N) * H, join = cdiv(rows, kPagedThreads / 32);
-  SVHIP_REQUIRE(p.row_slots + p.tile_grid < (1ll << 31) && join < (1ll << 31), "%s: grid too large", name);
+  SVHIP_REQUIRE(p.row_slots + p.tile_grid < (1ll << 31) && rows < (1ll << 31) - kPagedThreads &&
+                    N * (H / Hkv) < (1ll << 31) - kPagedThreads, "%s: sizes too large", name);
   const bool fp8 = pc.kv_dtype == SVHIP_FP8_E4M3;
   const int64_t es = fp8 ? 1 : 2;
   float* const part = static_cast<float*>(c.workspace);
   int4* const plan = reinterpret_cast<int4*>(part + p.row_floats + p.tile_floats);
   const PagedArgs a{static_cast<const uint16_t*>(c.q), pc.k_pages, pc.v_pages, pc.k_exponents, pc.v_exponents,
-                    static_cast<uint16_t*>(c.out), Tokens{c.cu_queries, B, N}, pages_of(pc), H, Hkv, H / Hkv, D, c.sq_b,
+                    static_cast<uint16_t*>(c.out), Tokens{c.cu_queries, B, N}, pages_of(pc), static_cast<int>(H), static_cast<int>(Hkv),
+                    static_cast<int>(H / Hkv), static_cast<int>(D), c.sq_b,
                     c.sq_h, c.sq_n, pc.sk_h, pc.sv_h, pc.sek_h, pc.sev_h, c.so_b, c.so_h, c.so_n,
                     static_cast<uint32_t>(pc.sk_p * es), static_cast<uint32_t>(pc.sk_r * es),
                     static_cast<uint32_t>(pc.sv_p * es), static_cast<uint32_t>(pc.sv_r * es),

@@ -1,6 +1,8 @@
 // The row form of svhip_paged_attention (paged_attention.hip): windows of up to kRows rows, single tokens among them.
 #pragma once
 
+#include <type_traits>
+
 #include "paged_attention.hpp"
 
 namespace svhip {
@@ -11,7 +13,8 @@ namespace svhip {
 __device__ __forceinline__ int row_keys(const PagedArgs& a, int64_t c) {
   int64_t first, count;
   window_tokens(a.tokens, c, first, count);
-  return count > 0 && row_form(a, count) ? static_cast<int>(held_keys(a.pages, c)) : -1;
+  const int held = static_cast<int>(held_keys(a.pages, c));  // (read beside the borders, not after them)
+  return count > 0 && row_form(a, count) ? held : -1;
 }
 __device__ __forceinline__ int row_parts(int keys, int length) {
   return keys < 0 ? 0 : (keys > length ? (keys - 1) / length + 1 : 1);
@@ -43,7 +46,7 @@ __device__ __forceinline__ int row_length(const PagedArgs& a, const Team& team, 
 
 // The lengths are on the device, so the workgroups form the plan themselves, or read it.
 __device__ __forceinline__ PagedItem row_item(const PagedArgs& a, int place, int& each) {
-  const int Hkv = static_cast<int>(a.Hkv);
+  const int Hkv = a.Hkv;
   if (!a.row_part) {
     const int b = place / Hkv;
     return PagedItem{b < a.tokens.B ? b : -1, place - b * Hkv, 0, 1, 0, 1, place, 0};
@@ -93,7 +96,7 @@ __device__ __forceinline__ void row_work(const PagedArgs& a, int place, char* sV
   if (a.row_part && !a.running && part == 0 && kvh == 0 && threadIdx.x == 0) a.plan[b] = make_int4(item.before, parts, each, 1);
   const Window w = window_at(a, b);
   if (w.count <= 0 || !row_form(a, w.count)) return;  // (uncut windows stand by their numbers)
-  const int rows = static_cast<int>(w.count * a.G);
+  const int rows = w.count * a.G;
   const int keys = __builtin_amdgcn_readfirstlane(w.keys);
   const int k0 = part * each, k1 = keys - k0 > each ? k0 + each : keys;
 
@@ -107,7 +110,7 @@ __device__ __forceinline__ void row_work(const PagedArgs& a, int place, char* sV
   // Blocks that end past it are seen in part (clean_values), if a later token sees more.
   const int clean_from = all + 1 < keys ? all + 1 - kKeys : kUncut;
   bool odd = false;
-  const int in_mask = (1 << a.pages.shift) - 1, D = static_cast<int>(a.D);
+  const int in_mask = (1 << a.pages.shift) - 1, D = a.D;
   // Groups of a block's keys that lie in one page for sure: all of it (WHOLE), or 16 keys.
   constexpr int kGroup = WHOLE ? kKeys : 16, kGroups = kKeys / kGroup;
   Lane8 vl[4 * kHalves];
@@ -288,7 +291,7 @@ __device__ __forceinline__ void row_work(const PagedArgs& a, int place, char* sV
       *reinterpret_cast<float2*>(slot + d) = make_float2(o0, o1);
       if (d == 0) *reinterpret_cast<float2*>(slot + D) = make_float2(m, total);
     } else {
-      const int64_t i = rr / a.G, g = rr - i * a.G;
+      const int i = rr / a.G, g = rr - i * a.G;
       uint16_t* out = a.o + row_at(a, w, b, kvh * a.G + g, i, a.so_b, a.so_h, a.so_n);
       const float inv = last_key(a, w, i) >= 0 ? 1.f / total : 0.f;
       *reinterpret_cast<uint32_t*>(out + d) = bf16_pack2(o0 * inv, o1 * inv);

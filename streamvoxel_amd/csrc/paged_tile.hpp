@@ -10,7 +10,8 @@ __device__ __forceinline__ void tiles_of_window(const PagedArgs& a, int64_t c, i
   int64_t first, count;
   window_tokens(a.tokens, c, first, count);
   tiles = row_form(a, count) ? 0 : static_cast<int>(cdiv(count * a.G, kTileRows));
-  blocks = count > 0 ? static_cast<int>((held_keys(a.pages, c) + kKB - 1) / kKB) : 0;
+  const int held = static_cast<int>((held_keys(a.pages, c) + kKB - 1) / kKB);  // (read beside the borders, not after them)
+  blocks = count > 0 ? held : 0;
 }
 
 __device__ __forceinline__ int tile_parts(int blocks, int length) { return blocks > length ? (blocks - 1) / length + 1 : 1; }
@@ -29,8 +30,8 @@ __device__ __forceinline__ PagedItem whole_item(const PagedArgs& a, int place) {
   const int unit = k * kXcds + (place & 7);
   PagedItem item{-1, 0, 0, 1, seq - seq / q_tiles * q_tiles, q_tiles, 0, 0};
   if (unit >= units) return item;
-  const int rank = unit / static_cast<int>(a.Hkv);
-  item.kvh = unit - rank * static_cast<int>(a.Hkv);
+  const int rank = unit / a.Hkv;
+  item.kvh = unit - rank * a.Hkv;
   item.b = rank;
   if (a.tokens.B > 1 && a.tokens.B <= 64) {
     const int lane = threadIdx.x & 63, B = static_cast<int>(a.tokens.B);
@@ -89,7 +90,7 @@ __device__ __forceinline__ PagedItem shared_item(const PagedArgs& a, int place, 
     const int at = shared_place(place, sums.y, each);
     return at < 0 ? none : planned_item(a, at, &a.running->y);
   }
-  const int Hkv = static_cast<int>(a.Hkv);
+  const int Hkv = a.Hkv;
   int tiles, blocks;
   float total;
   each = __builtin_amdgcn_readfirstlane(tile_length(a, WaveTeam{}, tiles, blocks, total));
@@ -124,7 +125,7 @@ __device__ __forceinline__ void tile_work(const PagedArgs& a, int place, char* s
   const Window w = window_at(a, b);
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int lane = threadIdx.x & 63, col = lane & 31, hh = lane >> 5;
-  const int64_t r0 = static_cast<int64_t>(qt) * kTileRows, r = r0 + wave * kRows + col, rows = w.count * a.G;
+  const int r0 = qt * kTileRows, r = r0 + wave * kRows + col, rows = w.count * a.G;
   const int keys = __builtin_amdgcn_readfirstlane(tile_keys(a, w, qt));
   const int blocks = (keys + kKB - 1) / kKB;
   const int count = blocks > each ? (blocks - 1) / each + 1 : 1;
@@ -138,10 +139,10 @@ __device__ __forceinline__ void tile_work(const PagedArgs& a, int place, char* s
   load_rows<KS>(a, w, b, kvh, r, s);
   // Where the lane's row goes, found now: what it takes would stay in scalar registers through the loop.
   const bool cut = count > 1;
-  const int D = static_cast<int>(a.D);
+  const int D = a.D;
   void* dest = nullptr;
   if (r < rows) {
-    const int64_t i = r / a.G;
+    const int i = r / a.G;
     dest = cut ? static_cast<void*>(a.tile_part + (static_cast<int64_t>(item.at) * kTileRows + (r - r0)) * (a.D + 2))
                : static_cast<void*>(a.o + row_at(a, w, b, kvh * a.G + (r - i * a.G), i, a.so_b, a.so_h, a.so_n));
   }
@@ -153,7 +154,7 @@ __device__ __forceinline__ void tile_work(const PagedArgs& a, int place, char* s
   const Source ks = k_source<ES>(a, kvh), vs = v_source<ES>(a, kvh);
   const int32_t* row = a.pages.table + b * a.pages.st_b;
   // The wave's rows see every key up to `all` and none past `any`.
-  const int64_t wr0 = r0 + wave * kRows, wr1 = wr0 + kRows < rows ? wr0 + kRows : rows;
+  const int wr0 = r0 + wave * kRows, wr1 = wr0 + kRows < rows ? wr0 + kRows : rows;
   const int all = __builtin_amdgcn_readfirstlane(wr0 < rows ? last_key(a, w, wr0 / a.G) : -1);
   const int any = __builtin_amdgcn_readfirstlane(wr0 < rows ? last_key(a, w, (wr1 - 1) / a.G) : -1);
   // Every row of the tile sees the keys up to `seen`; blocks past it are seen in part (clean_values).
