@@ -425,14 +425,16 @@ int svhip_sample_chosen(const void* logits, int dtype, int64_t classes, int64_t 
                         int64_t X, void* stream);
 
 /*
- * Rotary positions: out[b, h, n] = x[b, h, n] with its first 2 `pairs` elements turned, the rest kept. Pair i turns by
- * p freq[i] radians, p = positions[b, n] (int32, or int64 when positions_wide; any sign), and is scaled by `amplitude`:
+ * Rotary positions: out[b, h, n] = x[b, h, n] with its first 2 `pairs` elements turned, the rest kept. Pair i turns
+ * by p freq[i] radians, p = positions[b, n] (int32, or int64 when positions_wide; any sign), and is scaled by
+ * `amplitude`:
  *   y_a = amplitude (x_a cos - x_b sin), y_b = amplitude (x_b cos + x_a sin),
- * (a, b) = (i, i + pairs) for SVHIP_ROTARY_HALF, (2 i, 2 i + 1) for SVHIP_ROTARY_INTERLEAVED. The turns are formed in 64
- * bits, the rest is fp32, rounded once to the type. `inverse`: the transposed rotation, which takes the gradient of out
- * to the gradient of x. x, out: bf16 or fp32 (dtype), element (b, h, n, d) at b*s_b + h*s_h + n*s_n + d; out may be x
- * with the same strides. freq: fp64 [pairs], pairs <= 128. The arguments stand in a struct (a host pointer, read before
- * the call returns), here and below: a call from Python then costs one packing, not a conversion for each.
+ * (a, b) = (i, i + pairs) for SVHIP_ROTARY_HALF, (2 i, 2 i + 1) for SVHIP_ROTARY_INTERLEAVED. The turns are formed
+ * in 64 bits, the rest is fp32, rounded once to the type. `inverse`: the transposed rotation, which takes the
+ * gradient of out to the gradient of x. x, out: bf16 or fp32 (dtype), element (b, h, n, d) at b*s_b + h*s_h + n*s_n
+ * + d; out may be x with the same strides. freq: fp64 [pairs], pairs <= 128. The arguments stand in a struct (a
+ * host pointer, read before the call returns), here and below: a call from Python then costs one packing, not a
+ * conversion for each.
  * Beside svhip_axial_rope; no counterpart in the reference, whose positions have three axes.
  */
 typedef struct svhip_rotary_args {
@@ -447,13 +449,14 @@ typedef struct svhip_rotary_args {
 int svhip_rotary(const svhip_rotary_args* args, void* stream);
 
 /*
- * A paged cache: pools k_pages, v_pages of `pages` pages, element (page, h, r, d) at page*s_p + h*s_h + r*s_r + d, rows r
- * in [0, page_size), page_size a power of two from 16 to 1024, head_dim a multiple of 8 up to 128, rows 16-byte aligned
- * (e4m3: 8), max_pages * page_size at most 2^30. Key j of window b is row j % page_size of page page_table[b*table_stride + j / page_size] (int32, max_pages
- * numbers a window); lengths[b] (int32) counts the window's keys. kv_dtype SVHIP_BF16, or SVHIP_FP8_E4M3: OCP e4m3fn
- * codes with one power of two for each row and head, value = code 2^(exponent - 127), exponent bytes (page, h, r) at
- * page*se_p + h*se_h + r. Windows may share pages that are only read. `bad` (int32, may be null) is set to 1 by a call
- * that meets a page outside the pool or a key outside its window's row of the table.
+ * A paged cache: pools k_pages, v_pages of `pages` pages, element (page, h, r, d) at page*s_p + h*s_h + r*s_r + d,
+ * rows r in [0, page_size), page_size a power of two from 16 to 1024, head_dim a multiple of 8 up to 128, rows
+ * 16-byte aligned (e4m3: 8), max_pages * page_size at most 2^30. Key j of window b is row j % page_size of page
+ * page_table[b*table_stride + j / page_size] (int32, max_pages numbers a window); lengths[b] (int32) counts the
+ * window's keys. kv_dtype SVHIP_BF16, or SVHIP_FP8_E4M3: OCP e4m3fn codes with one power of two for each row and
+ * head, value = code 2^(exponent - 127), exponent bytes (page, h, r) at page*se_p + h*se_h + r. Windows may share
+ * pages that are only read. `bad` (int32, may be null) is set to 1 by a call that meets a page outside the pool or
+ * a key outside its window's row of the table.
  */
 typedef struct svhip_paged_cache {
   void *k_pages, *v_pages;
@@ -465,15 +468,15 @@ typedef struct svhip_paged_cache {
 } svhip_paged_cache;
 
 /*
- * Writes the new tokens' keys and values into a paged cache. Window b has N tokens, element (b, h, n, d) at b*s_b + h*s_h
- * + n*s_n + d, or with cu_tokens (int32 [windows + 1], ascending) the packed tokens [cu[b], cu[b + 1]) of N in all (s_b
- * unused; tokens outside every window are left alone). The window's length counts them: token i of n goes to key
- * lengths[b] - before - n + i, so `before` keys behind them are left to another call. `layout` rotates the keys on the
- * way: SVHIP_ROTARY_HALF / _INTERLEAVED as svhip_rotary (freq fp64 [pairs]; positions int32 / int64 at b*sp_b + n*sp_n, or
- * null: the key's index), SVHIP_ROTARY_AXIAL with svhip_axial_rope's arithmetic (positions fp32, three a token; freq fp32
- * [head_dim / 6]; pairs = head_dim / 2). e4m3: a row's exponent is the least with bound <= 448 2^(exponent - 127), bound =
- * its largest magnitude, for rotated keys 1.5 max(1, |amplitude|) times it before the rotation. A token whose key or page
- * is bad is not written. Key and value rows bf16, 16-byte aligned.
+ * Writes the new tokens' keys and values into a paged cache. Window b has N tokens, element (b, h, n, d) at b*s_b +
+ * h*s_h + n*s_n + d, or with cu_tokens (int32 [windows + 1], ascending) the packed tokens [cu[b], cu[b + 1]) of N
+ * in all (s_b unused; tokens outside every window are left alone). The window's length counts them: token i of n
+ * goes to key lengths[b] - before - n + i, so `before` keys behind them are left to another call. `layout` rotates
+ * the keys on the way: SVHIP_ROTARY_HALF / _INTERLEAVED as svhip_rotary (freq fp64 [pairs]; positions int32 / int64
+ * at b*sp_b + n*sp_n, or null: the key's index), SVHIP_ROTARY_AXIAL with svhip_axial_rope's arithmetic (positions
+ * fp32, three a token; freq fp32 [head_dim / 6]; pairs = head_dim / 2). e4m3: a row's exponent is the least with
+ * bound <= 448 2^(exponent - 127), bound = its largest magnitude, for rotated keys 1.5 max(1, |amplitude|) times it
+ * before the rotation. A token whose key or page is bad is not written. Key and value rows bf16, 16-byte aligned.
  * Beside svhip_kv_write (FastSlotForward.encode + _write, streamvoxel/stream/fast_ops.py:228-250), which rewrites a
  * window's slab whole; no counterpart in the reference.
  */
@@ -488,13 +491,14 @@ typedef struct svhip_paged_append_args {
 int svhip_paged_append(const svhip_paged_cache* cache, const svhip_paged_append_args* args, void* stream);
 
 /*
- * Attention of the windows' new tokens over a paged cache: out[b, h, i] = softmax_j(scale q[b, h, i] . k_j) v_j over the
- * keys j < lengths[b] of key head h / (H / heads), with `causal` only j <= lengths[b] - n + i (n tokens of window b, its
- * last keys); no key: zeros; infinities and NaN reach the tokens that see them. Queries and out bf16, N a window or packed by cu_queries, as in svhip_paged_append (rows
- * outside every window are left as they are). Products in bf16 on the matrix cores with fp32 sums, softmax weights rounded
- * to bf16. Keys and values of a bad page read as zeros; a length past the window's row of the table is cut to it. scale >
- * 0. Query rows 16-byte aligned, rows of out 8. workspace: svhip_paged_attention_workspace_bytes with max_keys = max_pages
- * * page_size (0: none needed), N and packed (cu_queries or not) as in the call; 16-byte aligned.
+ * Attention of the windows' new tokens over a paged cache: out[b, h, i] = softmax_j(scale q[b, h, i] . k_j) v_j
+ * over the keys j < lengths[b] of key head h / (H / heads), with `causal` only j <= lengths[b] - n + i (n tokens of
+ * window b, its last keys); no key: zeros; infinities and NaN reach the tokens that see them. Queries and out bf16,
+ * N a window or packed by cu_queries, as in svhip_paged_append (rows outside every window are left as they are).
+ * Products in bf16 on the matrix cores with fp32 sums, softmax weights rounded to bf16. Keys and values of a bad
+ * page read as zeros; a length past the window's row of the table is cut to it. scale > 0. Query rows 16-byte
+ * aligned, rows of out 8. workspace: svhip_paged_attention_workspace_bytes with max_keys = max_pages * page_size
+ * (0: none needed), N and packed (cu_queries or not) as in the call; 16-byte aligned.
  * Beside svhip_xattn_fwd (streamvoxel/stream/fast_ops.py:104-108); no counterpart in the reference.
  */
 typedef struct svhip_paged_attention_args {

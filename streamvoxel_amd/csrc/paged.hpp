@@ -1,7 +1,7 @@
-// A paged cache of keys and values: key j of window b is row j % S of page table[b][j / S] of a pool [pages, H, S, D], S a
-// power of two. bf16 rows, or OCP e4m3fn rows with one power of two for each row and head, held as its exponent's byte
-// (value = code 2^(byte - 127)): scaling by it is exact, so an e4m3 row decodes to bf16 without a second rounding and the
-// row's scale takes part in neither product of the attention.
+// A paged cache of keys and values: key j of window b is row j % S of page table[b][j / S] of a pool [pages, H, S,
+// D], S a power of two. bf16 rows, or OCP e4m3fn rows with one power of two for each row and head, held as its
+// exponent's byte (value = code 2^(byte - 127)): scaling by it is exact, so an e4m3 row decodes to bf16 without a
+// second rounding and the row's scale takes part in neither product of the attention.
 #pragma once
 
 #include "common.hpp"

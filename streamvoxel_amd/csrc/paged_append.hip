@@ -1,11 +1,12 @@
-// svhip_paged_append: the new tokens' keys and values into their rows of a paged cache (paged.hpp), the keys rotated on the
-// way: rotary positions (rotary.hpp, fp32, rounded once to the cache's type), or the three-axis rotation of svhip_axial_rope
-// with its roundings (the phase one fp32 product; sin, cos, every product and sum rounded to bf16).
+// svhip_paged_append: the new tokens' keys and values into their rows of a paged cache (paged.hpp), the keys rotated
+// on the way: rotary positions (rotary.hpp, fp32, rounded once to the cache's type), or the three-axis rotation of
+// svhip_axial_rope with its roundings (the phase one fp32 product; sin, cos, every product and sum rounded to bf16).
 //
-// Bound: HBM, the rows read once and written once. Workgroup = up to kAppendTokens tokens, all heads: where each token goes and
-// its (cos, sin) are the same for every head and go to LDS once; a group of 8 or 16 lanes then carries a (token, head) row, 16
-// bytes of it a lane, so that an e4m3 row's largest magnitude is a reduction within the group. A thread's first rows are on
-// their way before the chain length -> page -> positions -> table, which a launch of few tokens waits for.
+// Bound: HBM, the rows read once and written once. Workgroup = up to kAppendTokens tokens, all heads: where each
+// token goes and its (cos, sin) are the same for every head and go to LDS once; a group of 8 or 16 lanes then carries
+// a (token, head) row, 16 bytes of it a lane, so that an e4m3 row's largest magnitude is a reduction within the
+// group. A thread's first rows are on their way before the chain length -> page -> positions -> table, which a launch
+// of few tokens waits for.
 #include "paged.hpp"
 #include "rotary.hpp"
 
@@ -62,8 +63,8 @@ __device__ __forceinline__ float turned(float x, float y, float2 r, bool second)
   return __builtin_fmaf(x, r.x, second ? y * r.y : -(y * r.y));
 }
 
-// 8 elements d0 .. of a key row turned: x the row's, `other` the 8 that hold their partners (half layout: half further on or
-// back; else unused).
+// 8 elements d0 .. of a key row turned: x the row's, `other` the 8 that hold their partners (half layout: half
+// further on or back; else unused).
 template <int TURN>
 __device__ __forceinline__ void turn_run(const AppendArgs& a, float (&x)[8], const uint4& other, const uint16_t* row,
                                          const float2* table, int d0) {

@@ -1,27 +1,29 @@
-// svhip_paged_attention: attention of the windows' new tokens over their keys and values in a paged cache (paged.hpp), bf16
-// matrix cores, fp32 sums.
+// svhip_paged_attention: attention of the windows' new tokens over their keys and values in a paged cache
+// (paged.hpp), bf16 matrix cores, fp32 sums.
 //
-// A key head's queries are its G heads' rows of every token, row r = token r / G, head r % G; a wave takes 32 of them as the
-// columns of S^T = K Q^T and O^T = V^T P^T (v_mfma_f32_32x32x16_bf16), so that the softmax of a row stays in two lanes and
-// P^T leaves the first product in the second one's operand layout (K rows lie in LDS under sigma_row; xattn_kernel.hpp). V
-// rows lie as they come and are read transposed (ds_read_b64_tr_b16). Two forms of work:
-//   * windows of more than kRows rows (tile): a workgroup takes 128 rows, 32 a wave; the 4 waves stage each block of 64 keys
-//     together, the next one in flight while the current one is computed. Bound: the matrix cores and the exponentials.
+// A key head's queries are its G heads' rows of every token, row r = token r / G, head r % G; a wave takes 32 of them
+// as the columns of S^T = K Q^T and O^T = V^T P^T (v_mfma_f32_32x32x16_bf16), so that the softmax of a row stays in
+// two lanes and P^T leaves the first product in the second one's operand layout (K rows lie in LDS under sigma_row;
+// xattn_kernel.hpp). V rows lie as they come and are read transposed (ds_read_b64_tr_b16). Two forms of work:
+//   * windows of more than kRows rows (tile): a workgroup takes 128 rows, 32 a wave; the 4 waves stage each block of
+//     64 keys together, the next one in flight while the current one is computed. Bound: the matrix cores and the
+//     exponentials.
 //   * windows of up to kRows rows, single tokens among them (row): the 4 waves share the rows and split the keys, each
 //     staging its own blocks of 32 keys in its own LDS; no barrier until the waves' sums are joined. Bound: HBM.
-// Either form may cut a window's keys into parts for several workgroups; a part leaves O, its running maximum and its sum in
-// fp32 and paged_join_kernel joins them in order.
+// Either form may cut a window's keys into parts for several workgroups; a part leaves O, its running maximum and its
+// sum in fp32 and paged_join_kernel joins them in order.
 //
-// Staging: 16 keys lie in one page (pages are of 16 keys or more), so the wave's load of 8 rows has one base, a scalar buffer
-// descriptor whose bound is the number of its keys that exist: keys past the window's end, bad pages and the chunks past
-// head_dim read as zeros and nothing is read outside a page.
+// Staging: 16 keys lie in one page (pages are of 16 keys or more), so the wave's load of 8 rows has one base, a
+// scalar buffer descriptor whose bound is the number of its keys that exist: keys past the window's end, bad pages
+// and the chunks past head_dim read as zeros and nothing is read outside a page.
 #include "paged_row.hpp"
 #include "paged_tile.hpp"
 
 namespace svhip {
 
-// The plan of more windows than a wave has lanes, by one workgroup: part lengths, and every window's places in the lists of
-// row-form parts and of tiles. (Up to 64 windows a workgroup's own plan is one load a lane, less than this launch.)
+// The plan of more windows than a wave has lanes, by one workgroup: part lengths, and every window's places in the
+// lists of row-form parts and of tiles. (Up to 64 windows a workgroup's own plan is one load a lane, less than this
+// launch.)
 __global__ __launch_bounds__(kPlanThreads) void paged_plan_kernel(PagedArgs a, bool rows, bool tiles) {
   __shared__ float of_wave[kPlanThreads / 64];
   __shared__ int2 counts[kPlanThreads / 64];
@@ -73,8 +75,9 @@ __global__ __launch_bounds__(kPlanThreads) void paged_plan_kernel(PagedArgs a, b
   if (tid == 0) a.plan[a.tokens.B] = make_int4(at.x, at.y, row_cut ? row_each : kUncut, tile_cut ? tile_each : kUncut);
 }
 
-// The parts of a row joined in order. kGroups 32-lane groups a row, 4 elements a lane: one group where the rows are many (it
-// has kAhead parts in flight), all 8 of the workgroup where they are few (every part of up to 64 in flight at once).
+// The parts of a row joined in order. kGroups 32-lane groups a row, 4 elements a lane: one group where the rows are
+// many (it has kAhead parts in flight), all 8 of the workgroup where they are few (every part of up to 64 in flight
+// at once).
 constexpr int kAhead = 8;
 
 template <int kGroups>
@@ -178,7 +181,9 @@ __global__ __launch_bounds__(kPagedThreads) void paged_join_kernel(PagedArgs a) 
   *reinterpret_cast<uint2*>(out + d0) = make_uint2(bf16_pack2(o[0] * inv, o[1] * inv), bf16_pack2(o[2] * inv, o[3] * inv));
 }
 
-constexpr int64_t kJoinFew = 4096;  // rows up to which a row has a workgroup of its own
+// Rows up to which a row has a workgroup of its own (one token, 12 rows: 15.8 us, 25.7 without; 64 tokens, 1024 rows:
+// 217.6 and 222.9; 32 768 rows in two parts: 323 with, 281 without; 16 304 rows 116 and 104).
+constexpr int64_t kJoinFew = 4096;
 
 inline PagedPlan paged_plan(int64_t B, int64_t H, int64_t Hkv, int64_t N, bool packed, int64_t D, int64_t max_keys) {
   PagedPlan p{};
@@ -270,13 +275,12 @@ extern "C" int svhip_paged_attention(const svhip_paged_cache* cache, const svhip
                     p.plan_windows ? plan : nullptr, p.planned ? reinterpret_cast<int2*>(plan + B + 1) : nullptr};
   hipStream_t s = as_stream(stream);
   if (p.planned) paged_plan_kernel<<<1, kPlanThreads, 0, s>>>(a, p.rows, p.tiles);
-  const bool whole = pc.page_size >= kWholePages;
   if (p.rows && p.tiles) {
-    launch_paged_mixed(a, p, fp8, whole, s);
+    launch_paged_mixed(a, p, fp8, s);
   } else if (p.rows) {
-    launch_paged_rows(a, p, fp8, whole, s);
+    launch_paged_rows(a, p, fp8, s);
   } else {
-    launch_paged_tiles(a, p, fp8, whole, s);
+    launch_paged_tiles(a, p, fp8, pc.page_size >= kWholePages, s);
   }
   if (p.plan_windows) {
     if (rows <= kJoinFew) {

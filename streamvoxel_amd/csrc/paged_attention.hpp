@@ -9,12 +9,17 @@ namespace svhip {
 constexpr int kPagedThreads = 256;
 constexpr int kRows = 32;          // rows of a wave
 constexpr int kTileRows = 128;     // rows of a tile workgroup
-constexpr int kTileTarget = 512;   // tile workgroups below which keys are split: two for every CU
-constexpr int kTileBeside = 256;   // the same beside the row form: one for every CU
-constexpr int kTileLeast = 6;      // least key blocks of a tile's part
-constexpr int kRowTarget = 2048;   // row-form parts beyond one for each (window, key head)
-constexpr int kRowLeast = 256;     // keys that a row-form part has a multiple of
-constexpr int kWholePages = 64;    // pages from this size on hold whole blocks of keys
+// Tile workgroups below which keys are split, two for every CU (one, four: a causal chunk of 4 x 512 tokens, head_dim
+// 128, 313 and 278 us for 281; the same with all keys seen 198 and 180 for 167; 1024 queries over 9744 keys 82 and 61
+// for 60).
+constexpr int kTileTarget = 512;
+constexpr int kTileBeside = 256;   // the same beside the row form: one for every CU (24 mixed windows 101 us; 512: 110)
+constexpr int kTileLeast = 6;      // least key blocks of a tile's part (1024 queries over 9744 keys 60 us; 3, 12: 61)
+// Row-form parts beyond one for each (window, key head): eight for every CU (64 tokens, four heads to a key head, 218
+// us, 512 parts: 248; over e4m3 pages 158 and 180).
+constexpr int kRowTarget = 2048;
+constexpr int kRowLeast = 256;     // keys that a row-form part has a multiple of: 2 blocks of each wave (512: no difference)
+constexpr int kWholePages = 64;    // pages from this size on hold whole blocks of keys: found once a block (tiles 1.4 % less)
 constexpr int kUncut = 0x40000000; // a part length that cuts nothing
 constexpr float kNoMax = -3.0e38f; // running maximum before any key: finite, so that a row that sees nothing stays finite
 [[maybe_unused]] constexpr uint32_t kOutside = 0x7ffffff0u;  // byte offset past every descriptor's bound
@@ -81,7 +86,8 @@ __device__ __forceinline__ int64_t row_at(const PagedArgs& a, const Window& w, i
   return a.tokens.cu ? h * sh + (w.first + i) * sn : b * sb + h * sh + i * sn;
 }
 
-// The wave's sum, in every lane: the plans' counts, exact up to 2^24 (where a plan cuts, its places are fewer). DPP steps: a shuffle through LDS takes as long as all of them.
+// The wave's sum, in every lane: the plans' counts, exact up to 2^24 (where a plan cuts, its places are fewer). DPP
+// steps: a shuffle through LDS takes as long as all of them.
 __device__ __forceinline__ float wave_sum(float v) {
   v = row16_sum(v);
   const auto at = [&](int lane) __attribute__((always_inline)) {
@@ -107,8 +113,8 @@ __device__ __forceinline__ int wave_prefix(int v, int& total) {
   return incl - v;
 }
 
-// What a workgroup takes: part `part` of `parts` of key head kvh of window b (tiles: of tile qt), at place `at` of all, the
-// window's first being `before`. b < 0: nothing.
+// What a workgroup takes: part `part` of `parts` of key head kvh of window b (tiles: of tile qt), at place `at` of
+// all, the window's first being `before`. b < 0: nothing.
 struct PagedItem {
   int b, kvh, part, parts, qt, tiles, at, before;
 };
@@ -119,7 +125,8 @@ __device__ __forceinline__ PagedItem item_of(int b, int at, int in, int parts, i
   return PagedItem{b, kvh, u - kvh * parts, parts, in - u * tiles, tiles, at, at - in};
 }
 
-// The item at place `at` of the lists of up to 64 windows, one after the other; the lane's window has `tiles` and `parts`.
+// The item at place `at` of the lists of up to 64 windows, one after the other; the lane's window has `tiles` and
+// `parts`.
 __device__ __forceinline__ PagedItem item_at(int Hkv, int at, int tiles, int parts) {
   int total;
   const int n = tiles * Hkv * parts, before = wave_prefix(n, total);
@@ -168,8 +175,9 @@ struct BlockTeam {
   }
 };
 
-// The least length of a part, a multiple of `grain` and `least` at least, for which the windows' parts are at most `target`:
-// they then run side by side, and none longer than it must. places(c, length): parts of window c, all key heads and tiles.
+// The least length of a part, a multiple of `grain` and `least` at least, for which the windows' parts are at most
+// `target`: they then run side by side, and none longer than it must. places(c, length): parts of window c, all key
+// heads and tiles.
 template <typename Team, typename Places>
 __device__ __forceinline__ int part_length(const PagedArgs& a, const Team& team, float work, int target, int grain,
                                            int least, Places places) {
@@ -236,8 +244,8 @@ __device__ __forceinline__ Source v_source(const PagedArgs& a, int64_t kvh) {
                 a.sv_r, a.sev_p};
 }
 
-// Descriptor of the rows of a group of keys, row in_page of `page` the first: `valid` of them, `bytes` of each. A read past
-// them gives zeros.
+// Descriptor of the rows of a group of keys, row in_page of `page` the first: `valid` of them, `bytes` of each. A
+// read past them gives zeros.
 __device__ __forceinline__ __amdgpu_buffer_rsrc_t rows_of(const char* head, uint32_t sp, uint32_t sr, int page, int in_page,
                                                          int valid, int bytes) {
   const char* base = head + static_cast<uint64_t>(static_cast<uint32_t>(page)) * sp + static_cast<uint32_t>(in_page) * sr;
@@ -287,10 +295,10 @@ __device__ __forceinline__ f32x16_t scores(const Rows<KS>& s, const bf16x8_t (&k
   return x;
 }
 
-// Scores x of a block of 32 kHalves keys, `key0` the first: those that a row does not see masked, and the running maximum
-// moved for a score more than kMaxHigh above it (the weights then stay below 2^20, which fp32 sums and bf16 hold alike). One
-// such branch a block: a second one in a loop makes the compiler merge two register sets of O behind it, a copy that the
-// common path pays.
+// Scores x of a block of 32 kHalves keys, `key0` the first: those that a row does not see masked, and the running
+// maximum moved for a score more than kMaxHigh above it (the weights then stay below 2^20, which fp32 sums and bf16
+// hold alike). One such branch a block: a second one in a loop makes the compiler merge two register sets of O behind
+// it, a copy that the common path pays.
 template <int KS, int kHalves>
 __device__ __forceinline__ void bound_scores(Rows<KS>& s, f32x16_t (&x)[kHalves], float sl2, bool masked, int key0) {
   const int hh = (threadIdx.x & 63) >> 5;
@@ -349,9 +357,9 @@ __device__ __forceinline__ void weights_of(const Rows<KS>& s, const f32x16_t& x,
   }
 }
 
-// O^T += V^T P^T and the row's sum for 32 keys whose V rows are staged at vp (sub-tiles of 64 head_dim elements kSubBytes
-// apart). The sum is taken over the bf16 weights that the product reads, by v_mfma_f32_4x4x4_16b_bf16 with ones in A, whose
-// columns are single lanes: no row's NaN reaches another's sum.
+// O^T += V^T P^T and the row's sum for 32 keys whose V rows are staged at vp (sub-tiles of 64 head_dim elements
+// kSubBytes apart). The sum is taken over the bf16 weights that the product reads, by v_mfma_f32_4x4x4_16b_bf16 with
+// ones in A, whose columns are single lanes: no row's NaN reaches another's sum.
 template <int KS, int kSubBytes>
 __device__ __forceinline__ void add_values(Rows<KS>& s, const bf16x8_t (&pb)[2], const char* vp,
                                            const uint32_t (&rvt)[tiles_of(KS)]) {
@@ -407,8 +415,8 @@ struct Staged {
   uint32_t e[kLoads];
 };
 
-// A lane's place in a load of 8 rows whose first is row `first` of a block's tile (a multiple of 8), `base` being the tile row
-// of the descriptor's first key: row lane / 8 and its chunk; K under sigma_row and swz, V under swzv.
+// A lane's place in a load of 8 rows whose first is row `first` of a block's tile (a multiple of 8), `base` being the
+// tile row of the descriptor's first key: row lane / 8 and its chunk; K under sigma_row and swz, V under swzv.
 struct Lane8 {
   uint32_t at[2];   // byte offset in the descriptor in each sub-tile, or kOutside past head_dim
   uint32_t key;     // the key's place in the descriptor
@@ -436,7 +444,8 @@ __device__ __forceinline__ Lane8 v_lane(const PagedArgs& a, int first, int base)
   return lane_of_load<ES>(a.sv_r, a.D, R - base, swzv(R, lane & 7));
 }
 
-// Issues a load of 8 rows: bf16 straight into LDS at `to` (row 0 of the 8 in sub-tile 0), e4m3 into registers at index i.
+// Issues a load of 8 rows: bf16 straight into LDS at `to` (row 0 of the 8 in sub-tile 0), e4m3 into registers at
+// index i.
 template <bool FP8, int DT, int kSubBytes, int kLoads>
 __device__ __forceinline__ void stage_rows8(const __amdgpu_buffer_rsrc_t r, const __amdgpu_buffer_rsrc_t er, const Lane8& n,
                                             int i, char* to, Staged<DT, kLoads>& st) {
@@ -472,9 +481,9 @@ __device__ __forceinline__ void commit_rows8(const Staged<DT, kLoads>& st, int i
   }
 }
 
-// Values that are not finite, in a block whose keys some rows of the product see and some do not: their weight 0 times such a
-// value is NaN. So they are zeroed in LDS before the product (true: one was), a thread 16 bytes of `bytes` every `step`, and
-// added to the rows that see them at the end, from the pool.
+// Values that are not finite, in a block whose keys some rows of the product see and some do not: their weight 0
+// times such a value is NaN. So they are zeroed in LDS before the product (true: one was), a thread 16 bytes of
+// `bytes` every `step`, and added to the rows that see them at the end, from the pool.
 __device__ __forceinline__ bool clean_values(char* v, int bytes, int at, int step) {
   bool odd = false;
   for (; at < bytes; at += step) {
@@ -494,7 +503,8 @@ __device__ __forceinline__ bool clean_values(char* v, int bytes, int at, int ste
   return odd;
 }
 
-// Those of keys [from, to) to O^T of the rows that see them. (Their weights are above 0, and an infinity or NaN stays one.)
+// Those of keys [from, to) to O^T of the rows that see them. (Their weights are above 0, and an infinity or NaN stays
+// one.)
 template <bool FP8, int KS>
 __device__ __forceinline__ void add_odd_values(const PagedArgs& a, const Source& vs, const int32_t* row, int from, int to,
                                                Rows<KS>& s) {
@@ -543,33 +553,22 @@ struct PagedPlan {
   }
 };
 
-// FP8, KS: steps of 16 head_dim elements; whole: pages of kWholePages keys or more.
-void launch_paged_rows(const PagedArgs& a, const PagedPlan& p, bool fp8, bool whole, hipStream_t s);
+// KS: steps of 16 head_dim elements; whole: pages of kWholePages keys or more.
+void launch_paged_rows(const PagedArgs& a, const PagedPlan& p, bool fp8, hipStream_t s);
 void launch_paged_tiles(const PagedArgs& a, const PagedPlan& p, bool fp8, bool whole, hipStream_t s);
-void launch_paged_mixed(const PagedArgs& a, const PagedPlan& p, bool fp8, bool whole, hipStream_t s);
+void launch_paged_mixed(const PagedArgs& a, const PagedPlan& p, bool fp8, hipStream_t s);
 
-// The instantiations of `launch` by type, page size and head width.
-#define SVHIP_PAGED_WIDTH(launch, FP8, WHOLE)                      \
-  switch ((a.D + 15) / 16) {                                       \
-    case 8: return launch<FP8, WHOLE, 8>(a, p, s);                 \
-    case 7: return launch<FP8, WHOLE, 7>(a, p, s);                 \
-    case 6: return launch<FP8, WHOLE, 6>(a, p, s);                 \
-    case 5: return launch<FP8, WHOLE, 5>(a, p, s);                 \
-    case 4: return launch<FP8, WHOLE, 4>(a, p, s);                 \
-    case 3: return launch<FP8, WHOLE, 3>(a, p, s);                 \
-    case 2: return launch<FP8, WHOLE, 2>(a, p, s);                 \
-    default: return launch<FP8, WHOLE, 1>(a, p, s);                \
+// The instantiations of `launch` by head width; the others of its template arguments in front.
+#define SVHIP_PAGED_WIDTH(launch, ...)                       \
+  switch ((a.D + 15) / 16) {                                 \
+    case 8: return launch<__VA_ARGS__, 8>(a, p, s);          \
+    case 7: return launch<__VA_ARGS__, 7>(a, p, s);          \
+    case 6: return launch<__VA_ARGS__, 6>(a, p, s);          \
+    case 5: return launch<__VA_ARGS__, 5>(a, p, s);          \
+    case 4: return launch<__VA_ARGS__, 4>(a, p, s);          \
+    case 3: return launch<__VA_ARGS__, 3>(a, p, s);          \
+    case 2: return launch<__VA_ARGS__, 2>(a, p, s);          \
+    default: return launch<__VA_ARGS__, 1>(a, p, s);         \
   }
-#define SVHIP_PAGED_LAUNCH(launch)           \
-  if (fp8) {                                 \
-    if (whole) {                             \
-      SVHIP_PAGED_WIDTH(launch, true, true)  \
-    }                                        \
-    SVHIP_PAGED_WIDTH(launch, true, false)   \
-  }                                          \
-  if (whole) {                               \
-    SVHIP_PAGED_WIDTH(launch, false, true)   \
-  }                                          \
-  SVHIP_PAGED_WIDTH(launch, false, false)
 
 }  // namespace svhip

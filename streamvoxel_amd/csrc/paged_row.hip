@@ -3,24 +3,27 @@
 namespace svhip {
 
 // Windows that are all of the row form.
-template <bool FP8, bool WHOLE, int KS>
+template <bool FP8, int KS>
 __global__ __launch_bounds__(kPagedThreads, 2) void paged_row_kernel(PagedArgs a) {
 #if defined(__HIP_DEVICE_COMPILE__)
   constexpr int kFirst = FP8 ? 4 : 2;
   typedef RowLds<FP8, KS, kFirst> L;
   __shared__ __attribute__((aligned(16))) char s0[L::k0], s1[L::k1];
   __shared__ float s_ml[4][2][kRows];
-  row_work<FP8, WHOLE, KS, kFirst>(a, static_cast<int>(blockIdx.x), s0, s1, s_ml);
+  row_work<FP8, KS, kFirst>(a, static_cast<int>(blockIdx.x), s0, s1, s_ml);
 #endif
 }
 
-template <bool FP8, bool WHOLE, int KS>
+template <bool FP8, int KS>
 void launch_rows(const PagedArgs& a, const PagedPlan& p, hipStream_t s) {
-  paged_row_kernel<FP8, WHOLE, KS><<<static_cast<unsigned>(p.row_slots), kPagedThreads, 0, s>>>(a);
+  paged_row_kernel<FP8, KS><<<static_cast<unsigned>(p.row_slots), kPagedThreads, 0, s>>>(a);
 }
 
-void launch_paged_rows(const PagedArgs& a, const PagedPlan& p, bool fp8, bool whole, hipStream_t s) {
-  SVHIP_PAGED_LAUNCH(launch_rows)
+void launch_paged_rows(const PagedArgs& a, const PagedPlan& p, bool fp8, hipStream_t s) {
+  if (fp8) {
+    SVHIP_PAGED_WIDTH(launch_rows, true)
+  }
+  SVHIP_PAGED_WIDTH(launch_rows, false)
 }
 
 }  // namespace svhip

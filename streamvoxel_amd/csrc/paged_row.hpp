@@ -20,8 +20,9 @@ __device__ __forceinline__ int row_parts(int keys, int length) {
   return keys < 0 ? 0 : (keys > length ? (keys - 1) / length + 1 : 1);
 }
 
-// The length of a part: the least, a multiple of kRowLeast (4 waves' blocks), for which the parts are at most kRowTarget more
-// than the (window, key head) pairs; kUncut if there are no places from `place` on. `mine`: keys of the team's own window.
+// The length of a part: the least, a multiple of kRowLeast (4 waves' blocks), for which the parts are at most
+// kRowTarget more than the (window, key head) pairs; kUncut if there are no places from `place` on. `mine`: keys of
+// the team's own window.
 template <typename Team>
 __device__ __forceinline__ int row_length(const PagedArgs& a, const Team& team, int place, int& mine) {
   float keys = 0.f, units = 0.f;
@@ -63,11 +64,11 @@ __device__ __forceinline__ PagedItem row_item(const PagedArgs& a, int place, int
   return item_at(Hkv, place, parts > 0 ? 1 : 0, parts);
 }
 
-// A wave takes every 4th block of 32 keys of its part (e4m3 up to head_dim 64: of 64 keys, as many bytes). K rows go straight
-// from memory to the A operands, a lane its own key's chunks, the next block's while the current one's softmax and second
-// product run; V rows go through the wave's LDS, since they are read transposed.
-// Its LDS: V of the four waves, bf16 two blocks of each; O of them at the end, 32 DT x 32 floats each, of the first `kFirst`
-// in the one buffer and of the others in the other.
+// A wave takes every 4th block of 32 keys of its part (e4m3 up to head_dim 64: of 64 keys, as many bytes). K rows go
+// straight from memory to the A operands, a lane its own key's chunks, the next block's while the current one's
+// softmax and second product run; V rows go through the wave's LDS, since they are read transposed. Its LDS: V of the
+// four waves, bf16 two blocks of each; O of them at the end, 32 DT x 32 floats each, of the first `kFirst` in the one
+// buffer and of the others in the other.
 template <bool FP8, int KS, int kFirst>
 struct RowLds {
   static constexpr int kHalves = FP8 && KS <= 4 ? 2 : 1, kKeys = kRowKeys * kHalves;  // of a wave's block
@@ -79,7 +80,7 @@ struct RowLds {
 
 #if defined(__HIP_DEVICE_COMPILE__)
 
-template <bool FP8, bool WHOLE, int KS, int kFirst>
+template <bool FP8, int KS, int kFirst>
 __device__ __forceinline__ void row_work(const PagedArgs& a, int place, char* sV0, char* sV1, float (*s_ml)[2][kRows]) {
   constexpr int DT = tiles_of(KS), ES = FP8 ? 1 : 2;
   typedef RowLds<FP8, KS, kFirst> L;
@@ -111,13 +112,12 @@ __device__ __forceinline__ void row_work(const PagedArgs& a, int place, char* sV
   const int clean_from = all + 1 < keys ? all + 1 - kKeys : kUncut;
   bool odd = false;
   const int in_mask = (1 << a.pages.shift) - 1, D = a.D;
-  // Groups of a block's keys that lie in one page for sure: all of it (WHOLE), or 16 keys.
-  constexpr int kGroup = WHOLE ? kKeys : 16, kGroups = kKeys / kGroup;
+  constexpr int kGroup = 16, kGroups = kKeys / kGroup;  // keys that lie in one page for sure
   Lane8 vl[4 * kHalves];
 #pragma unroll
-  for (int i = 0; i < 4 * kHalves; ++i) vl[i] = v_lane<ES>(a, 8 * i, WHOLE ? 0 : 16 * (i >> 1));
-  // The lane's key of each half and its offsets in a K row (the last step's chunk may lie past head_dim, where Q is zero:
-  // any chunk of the row then).
+  for (int i = 0; i < 4 * kHalves; ++i) vl[i] = v_lane<ES>(a, 8 * i, 16 * (i >> 1));
+  // The lane's key of each half and its offsets in a K row (the last step's chunk may lie past head_dim, where Q is
+  // zero: any chunk of the row then).
   const int own = sigma_row(col);
   const int k_last = 16 * (KS - 1) + 8 * hh < D ? 16 * (KS - 1) * ES : -8 * hh * ES;
 
@@ -150,28 +150,18 @@ __device__ __forceinline__ void row_work(const PagedArgs& a, int place, char* sV
       stage_rows8<FP8, DT, kSubBytes>(r, er, vl[i], i, to + 8 * i * kRow * 2, vst);
     }
   };
-  // Keys that do not exist are never loaded (the group's first one is read instead, or page 0 where there is none): their
-  // scores are masked, but for bad pages, which count as zeros.
+  // Keys that do not exist are never loaded (the group's first one is read instead, or page 0 where there is none):
+  // their scores are masked, but for bad pages, which count as zeros.
   auto load_k = [&](int kv) __attribute__((always_inline)) {
 #pragma unroll
     for (int t = 0; t < kHalves; ++t) {
-      const char* at;
-      if constexpr (WHOLE) {
-        const int in_page = kv & in_mask, key = 32 * t + own;
-        const uint64_t number = static_cast<uint32_t>(page[0]);
-        const char* base = ks.rows + number * ks.sp + static_cast<uint32_t>(in_page) * ks.sr;
-        const int there = key < valid[0] ? key : 0;
-        at = base + (static_cast<uint32_t>(there) * ks.sr + 8 * hh * ES);
-        if constexpr (FP8) ke[t] = ks.exponents[number * ks.se + in_page + there];
-      } else {
-        const int g = 2 * t;
-        const int in0 = (kv + 16 * g) & in_mask, in1 = (kv + 16 * g + 16) & in_mask;
-        const bool second = col >= 16;
-        const uint32_t pg = second ? page[g + 1] : page[g], in = second ? in1 : in0;
-        const int there = (own & 15) < (second ? valid[g + 1] : valid[g]) ? own & 15 : 0;
-        at = ks.rows + static_cast<uint64_t>(pg) * ks.sp + ((in + there) * ks.sr + 8 * hh * ES);
-        if constexpr (FP8) ke[t] = ks.exponents[static_cast<uint64_t>(pg) * ks.se + in + there];
-      }
+      const int g = 2 * t;
+      const int in0 = (kv + 16 * g) & in_mask, in1 = (kv + 16 * g + 16) & in_mask;
+      const bool second = col >= 16;
+      const uint32_t pg = second ? page[g + 1] : page[g], in = second ? in1 : in0;
+      const int there = (own & 15) < (second ? valid[g + 1] : valid[g]) ? own & 15 : 0;
+      const char* at = ks.rows + static_cast<uint64_t>(pg) * ks.sp + ((in + there) * ks.sr + 8 * hh * ES);
+      if constexpr (FP8) ke[t] = ks.exponents[static_cast<uint64_t>(pg) * ks.se + in + there];
 #pragma unroll
       for (int k = 0; k < KS; ++k) {
         kw[t][k] = *reinterpret_cast<const KWord*>(at + (k < KS - 1 ? 16 * k * ES : k_last));
@@ -227,7 +217,8 @@ __device__ __forceinline__ void row_work(const PagedArgs& a, int place, char* sV
         load_k(kvn);
         find(kvn + stride);
       }
-      // V of this block was on its way before K of this block, which has arrived: at most the next block's loads are left.
+      // V of this block was on its way before K of this block, which has arrived: at most the next block's loads are
+      // left.
       if constexpr (!FP8) {
         if (more) {
           asm volatile("s_waitcnt vmcnt(%0)" ::"n"(4 * Width<DT>::kSubTiles + KS) : "memory");

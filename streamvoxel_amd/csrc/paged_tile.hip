@@ -2,7 +2,9 @@
 
 namespace svhip {
 
-// Windows that are all of the tile form.
+// Windows that are all of the tile form. Up to 64 head_dim elements a bf16 pool's kernel fits 128 registers and four
+// workgroups a CU (8 windows of 1024 queries, head_dim 64: 203.6 us, 204.5 with room for two); wider or decoding ones
+// spill there.
 template <bool FP8, bool WHOLE, int KS>
 __global__ __launch_bounds__(kPagedThreads, FP8 || KS > 4 ? 2 : 4) void paged_tile_kernel(PagedArgs a) {
 #if defined(__HIP_DEVICE_COMPILE__)
@@ -18,7 +20,16 @@ void launch_tiles(const PagedArgs& a, const PagedPlan& p, hipStream_t s) {
 }
 
 void launch_paged_tiles(const PagedArgs& a, const PagedPlan& p, bool fp8, bool whole, hipStream_t s) {
-  SVHIP_PAGED_LAUNCH(launch_tiles)
+  if (fp8) {
+    if (whole) {
+      SVHIP_PAGED_WIDTH(launch_tiles, true, true)
+    }
+    SVHIP_PAGED_WIDTH(launch_tiles, true, false)
+  }
+  if (whole) {
+    SVHIP_PAGED_WIDTH(launch_tiles, false, true)
+  }
+  SVHIP_PAGED_WIDTH(launch_tiles, false, false)
 }
 
 }  // namespace svhip

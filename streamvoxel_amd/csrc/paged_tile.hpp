@@ -16,9 +16,9 @@ __device__ __forceinline__ void tiles_of_window(const PagedArgs& a, int64_t c, i
 
 __device__ __forceinline__ int tile_parts(int blocks, int length) { return blocks > length ? (blocks - 1) / length + 1 : 1; }
 
-// Even windows that fill the chip by themselves (split false): XCD id % 8 takes every 8th (window, key head) with all its
-// tiles, so that its L2 reads the keys once; the windows longest first (up to 64 of them), and every other round of an XCD's
-// CUs in reverse, which evens out the CUs' sums.
+// Even windows that fill the chip by themselves (split false): XCD id % 8 takes every 8th (window, key head) with all
+// its tiles, so that its L2 reads the keys once; the windows longest first (up to 64 of them), and every other round
+// of an XCD's CUs in reverse, which evens out the CUs' sums.
 __device__ __forceinline__ PagedItem whole_item(const PagedArgs& a, int place) {
   const int seq = place >> 3, q_tiles = a.q_tiles;
   int k = seq / q_tiles;
@@ -46,11 +46,11 @@ __device__ __forceinline__ PagedItem whole_item(const PagedArgs& a, int place) {
   return item;
 }
 
-// Otherwise the tiles stand one window after the other. Fewer than kTileTarget of them share out their keys: into parts of the
-// least number of blocks, kTileLeast at least, for which the parts are at most kTileTarget and run side by side; at most
-// kTileBeside where the row form's windows read half as many blocks or more (they then have the other half of every CU: a
-// block takes about 1 us of either's CU; 24 mixed windows 101 us for 110). kUncut: no parts. `tiles`, `blocks`: of the team's
-// own window; `total`: the tiles.
+// Otherwise the tiles stand one window after the other. Fewer than kTileTarget of them share out their keys: into
+// parts of the least number of blocks, kTileLeast at least, for which the parts are at most kTileTarget and run side
+// by side; at most kTileBeside where the row form's windows read half as many blocks or more (they then have the
+// other half of every CU: a block takes about 1 us of either's CU; 24 mixed windows 101 us for 110). kUncut: no
+// parts. `tiles`, `blocks`: of the team's own window; `total`: the tiles.
 template <typename Team>
 __device__ __forceinline__ int tile_length(const PagedArgs& a, const Team& team, int& tiles, int& blocks, float& total) {
   const float Hkv = static_cast<float>(a.Hkv);

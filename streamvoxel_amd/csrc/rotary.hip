@@ -1,10 +1,10 @@
-// svhip_rotary: rotary positions of activations [B, H, N, D] (rotary.hpp), and with `inverse` the gradient: the transposed
-// rotation, sin negated.
+// svhip_rotary: rotary positions of activations [B, H, N, D] (rotary.hpp), and with `inverse` the gradient: the
+// transposed rotation, sin negated.
 //
-// Bound: HBM, every element read and written once (3 operations each). Workgroup = (window, up to kRotaryTokens tokens), all
-// heads: the tile's (cos, sin) of every (token, pair) go to LDS once, since they are the same for every head, and a thread
-// then turns pairs of 16-byte runs, kRotaryAhead of them in flight before the table is formed. Rows that are not made of such
-// runs (odd numbers of pairs, unaligned rows) go pair by pair.
+// Bound: HBM, every element read and written once (3 operations each). Workgroup = (window, up to kRotaryTokens
+// tokens), all heads: the tile's (cos, sin) of every (token, pair) go to LDS once, since they are the same for every
+// head, and a thread then turns pairs of 16-byte runs, kRotaryAhead of them in flight before the table is formed.
+// Rows that are not made of such runs (odd numbers of pairs, unaligned rows) go pair by pair.
 #include "rotary.hpp"
 
 namespace svhip {

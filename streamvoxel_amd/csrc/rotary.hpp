@@ -1,10 +1,10 @@
 // Rotary positions: what the rotation of activations and the append to a paged cache share.
 //
-// Pair i < half of a head turns by theta = p f_i: y_a = A (x_a cos - x_b sin), y_b = A (x_b cos + x_a sin), with
-// (a, b) = (i, i + half) in the half layout and (2 i, 2 i + 1) in the interleaved one; elements from 2 half on are kept.
-// A phase in fp32 is off by p f 2^-24: a thirtieth of a radian at position 2^19. So the turns p f / 2 pi are formed in 64
-// bits and cut to half a turn there (off by 2^-52 of the turns, below fp32's step up to position 2^30), and only
-// what is left goes to fp32's sin and cos; both are shared by all heads of a token, so the table costs little.
+// Pair i < half of a head turns by theta = p f_i: y_a = A (x_a cos - x_b sin), y_b = A (x_b cos + x_a sin), with (a,
+// b) = (i, i + half) in the half layout and (2 i, 2 i + 1) in the interleaved one; elements from 2 half on are kept.
+// A phase in fp32 is off by p f 2^-24: a thirtieth of a radian at position 2^19. So the turns p f / 2 pi are formed
+// in 64 bits and cut to half a turn there (off by 2^-52 of the turns, below fp32's step up to position 2^30), and
+// only what is left goes to fp32's sin and cos; both are shared by all heads of a token, so the table costs little.
 #pragma once
 
 #include "common.hpp"

@@ -80,7 +80,7 @@ def rotary(x, positions, frequencies, layout='half', amplitude=1.0, out=None):
     positions * frequencies[i] and is scaled by `amplitude`, the other elements are kept. `layout` 'half' pairs element i
     with i + len(frequencies), 'interleaved' 2i with 2i + 1. frequencies: the fp64 buffer of `rotary_frequencies`, at most
     128 pairs. The turns are formed in 64 bits (far positions keep their angle), the rest in fp32, rounded once to x's type.
-    Differentiable in x. `out` (optional, no gradient through it; x itself, or memory that x does not share) receives the
+    Differentiable in x (captured into a graph: for leaves that no eager graph still holds). `out` (optional, no gradient through it; x itself, or memory that x does not share) receives the
     result; returns it."""
     _lib.require_one_gpu(x, positions, frequencies, out)
     if layout not in LAYOUTS:

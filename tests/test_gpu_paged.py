@@ -808,3 +808,26 @@ def test_out_over_the_query_and_refused_places(n):
     key = queries(2, 2, n, 64, 4)
     with pytest.raises(ValueError, match='place'):
         paged_append(key, key, args[0][:1].expand(args[0].shape), args[1], *args[2:])
+
+
+@pytest.mark.parametrize('kv_dtype', ['bf16', 'fp8'])
+@pytest.mark.parametrize('page', [16, 64])
+@pytest.mark.parametrize('D', range(8, 129, 8))
+def test_every_head_width(D, page, kv_dtype):
+    """Single tokens, chunks, and both packed, with windows short and long enough for parts."""
+    from streamvoxel_amd.stream.paged import paged_append, paged_attention
+    _case(f'head width D={D} page={page} {kv_dtype}')
+    pool = Pool([700, 90], 2, D, page, D, kv_dtype)
+    args, how = pool.args(), dict(causal=True, **pool.exponents())
+    for n in (1, 40):
+        q = queries(2, 4, n, D, n)
+        check(paged_attention(q, *args, **how), q, pool, True)
+    cu = [0, 1, 41]
+    q = torch.randn(4, 41, D, generator=torch.Generator().manual_seed(D)).to(torch.bfloat16).to(DEV)
+    got = paged_attention(q, *args, cu_queries=torch.tensor(cu, dtype=torch.int32, device=DEV), **how)
+    check(got, q, pool, True, cu)
+    key = queries(2, 2, 3, D, 5)
+    paged_append(key, key, *args, **pool.exponents())
+    if kv_dtype == 'bf16':
+        at = torch.arange(697, 700, device=DEV)
+        assert torch.equal(args[0][args[2][0].long()[at // page], :, at % page], key[0].transpose(0, 1))
