@@ -5,13 +5,21 @@
 // as the columns of S^T = K Q^T and O^T = V^T P^T (v_mfma_f32_32x32x16_bf16), so that the softmax of a row stays in
 // two lanes and P^T leaves the first product in the second one's operand layout (K rows lie in LDS under sigma_row;
 // xattn_kernel.hpp). V rows lie as they come and are read transposed (ds_read_b64_tr_b16). Two forms of work:
-//   * windows of more than kRows rows (tile): a workgroup takes 128 rows, 32 a wave; the 4 waves stage each block of
-//     64 keys together, the next one in flight while the current one is computed. Bound: the matrix cores and the
-//     exponentials.
-//   * windows of up to kRows rows, single tokens among them (row): the 4 waves share the rows and split the keys, each
-//     staging its own blocks of 32 keys in its own LDS; no barrier until the waves' sums are joined. Bound: HBM.
-// Either form may cut a window's keys into parts for several workgroups; a part leaves O, its running maximum and its
-// sum in fp32 and paged_join_kernel joins them in order.
+//   * windows of more than kRows rows (tile, paged_tile.hpp): a workgroup takes 128 rows, 32 a wave; the 4 waves
+//     stage each block of 64 keys together, the next one in flight while the current one is computed. Bound: the
+//     matrix cores and the exponentials, which overlap little. Measured: 8 windows x 1024 queries, 1552 to 9744 keys,
+//     12 x 64 (153 GFLOP) 200 us, 770 TFLOP/s; 4 causal chunks of 512, 16 heads to 4 of 128, up to 16 384 keys (241
+//     GFLOP) 268 us and 12 of join.
+//   * windows of up to kRows rows, single tokens among them (row, paged_row.hpp): the 4 waves share the rows and
+//     split the keys, each staging its own blocks of 32 keys in its own LDS; no barrier until the waves' sums are
+//     joined. Bound: HBM. Measured: 64 tokens over 1.18 GB of keys 216 us, 5.4 TB/s; over 754 MB of e4m3 pages 148
+//     us, 5.1 TB/s; one token over 30 MB 9.1 us, a chain of loads. One wave a row of its own, with shuffles instead
+//     of the products, took 14.9 ms.
+// Packed windows may be of both (paged_mixed.hip). Either form may cut a window's keys into parts for several
+// workgroups; a part leaves O, its running maximum and its sum in fp32 and paged_join_kernel joins them in order (4.5
+// us for one token, 12 for 34 MB of parts). What is cut is planned on the device, where the lengths are: by every
+// workgroup for up to 64 windows, one a lane, else by paged_plan_kernel (6.6 us; every workgroup for itself: 4096
+// windows of one token 2348 us for 491).
 //
 // Staging: 16 keys lie in one page (pages are of 16 keys or more), so the wave's load of 8 rows has one base, a
 // scalar buffer descriptor whose bound is the number of its keys that exist: keys past the window's end, bad pages
@@ -93,7 +101,8 @@ __global__ __launch_bounds__(kPagedThreads) void paged_join_kernel(PagedArgs a) 
   const int total = static_cast<int>(a.tokens.cu ? a.tokens.N : a.tokens.B * a.tokens.N);
   const int token = id / a.H, h = id - token * a.H;
   int64_t b = -1;
-  if (token < total) b = a.tokens.cu ? (a.tokens.B > 64 ? window_of(a.tokens, token) : -1) : token / static_cast<int>(a.tokens.N);
+  if (token < total && !a.tokens.cu) b = token / static_cast<int>(a.tokens.N);
+  if (token < total && a.tokens.cu && a.tokens.B > 64) b = window_of(a.tokens, token);
   if (a.tokens.cu && a.tokens.B <= 64) {
     // Up to 64 borders are read at once; a wave has the tokens of its two groups.
     const int lane = threadIdx.x & 63, B = static_cast<int>(a.tokens.B);
@@ -117,7 +126,9 @@ __global__ __launch_bounds__(kPagedThreads) void paged_join_kernel(PagedArgs a) 
   if (row_form(a, w.count)) {
     if (!a.row_part) return;
     count = plan.y;
-    if (plan.x < 0 || count < 0 || plan.x + static_cast<int64_t>(a.Hkv) * count > a.row_slots) return set_bad(a.pages);  // borders not ascending
+    if (plan.x < 0 || count < 0 || plan.x + static_cast<int64_t>(a.Hkv) * count > a.row_slots) {
+      return set_bad(a.pages);  // borders not ascending
+    }
     slot = a.row_part + (static_cast<int64_t>(plan.x + kvh * count) * a.slot_rows + r) * (a.D + 2);
     step = static_cast<int64_t>(a.slot_rows) * (a.D + 2);
   } else {
@@ -127,10 +138,12 @@ __global__ __launch_bounds__(kPagedThreads) void paged_join_kernel(PagedArgs a) 
     if (each < 1) return set_bad(a.pages);
     count = blocks > each ? (blocks - 1) / each + 1 : 1;
     if (count < 2) return;
-    if (plan.x < 0 || plan.y < count || tiles <= qt || plan.x + static_cast<int64_t>(a.Hkv) * plan.y * tiles > a.tile_slots) {
+    if (plan.x < 0 || plan.y < count || tiles <= qt ||
+        plan.x + static_cast<int64_t>(a.Hkv) * plan.y * tiles > a.tile_slots) {
       return set_bad(a.pages);
     }
-    slot = a.tile_part + (static_cast<int64_t>(plan.x + kvh * plan.y * tiles + qt) * kTileRows + (r - qt * kTileRows)) * (a.D + 2);
+    const int64_t first = static_cast<int64_t>(plan.x + kvh * plan.y * tiles + qt) * kTileRows;
+    slot = a.tile_part + (first + (r - qt * kTileRows)) * (a.D + 2);
     step = static_cast<int64_t>(tiles) * kTileRows * (a.D + 2);
   }
   if (count < 2) return;
@@ -264,8 +277,8 @@ extern "C" int svhip_paged_attention(const svhip_paged_cache* cache, const svhip
   float* const part = static_cast<float*>(c.workspace);
   int4* const plan = reinterpret_cast<int4*>(part + p.row_floats + p.tile_floats);
   const PagedArgs a{static_cast<const uint16_t*>(c.q), pc.k_pages, pc.v_pages, pc.k_exponents, pc.v_exponents,
-                    static_cast<uint16_t*>(c.out), Tokens{c.cu_queries, B, N}, pages_of(pc), static_cast<int>(H), static_cast<int>(Hkv),
-                    static_cast<int>(H / Hkv), static_cast<int>(D), c.sq_b,
+                    static_cast<uint16_t*>(c.out), Tokens{c.cu_queries, B, N}, pages_of(pc),
+                    static_cast<int>(H), static_cast<int>(Hkv), static_cast<int>(H / Hkv), static_cast<int>(D), c.sq_b,
                     c.sq_h, c.sq_n, pc.sk_h, pc.sv_h, pc.sek_h, pc.sev_h, c.so_b, c.so_h, c.so_n,
                     static_cast<uint32_t>(pc.sk_p * es), static_cast<uint32_t>(pc.sk_r * es),
                     static_cast<uint32_t>(pc.sv_p * es), static_cast<uint32_t>(pc.sv_r * es),

@@ -94,7 +94,9 @@ __device__ __forceinline__ void row_work(const PagedArgs& a, int place, char* sV
   if (b < 0) return;
   const int kvh = __builtin_amdgcn_readfirstlane(item.kvh), part = __builtin_amdgcn_readfirstlane(item.part);
   const int parts = __builtin_amdgcn_readfirstlane(item.parts);
-  if (a.row_part && !a.running && part == 0 && kvh == 0 && threadIdx.x == 0) a.plan[b] = make_int4(item.before, parts, each, 1);
+  if (a.row_part && !a.running && part == 0 && kvh == 0 && threadIdx.x == 0) {
+    a.plan[b] = make_int4(item.before, parts, each, 1);
+  }
   const Window w = window_at(a, b);
   if (w.count <= 0 || !row_form(a, w.count)) return;  // (uncut windows stand by their numbers)
   const int rows = w.count * a.G;

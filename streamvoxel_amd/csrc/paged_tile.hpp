@@ -14,7 +14,9 @@ __device__ __forceinline__ void tiles_of_window(const PagedArgs& a, int64_t c, i
   blocks = count > 0 ? held : 0;
 }
 
-__device__ __forceinline__ int tile_parts(int blocks, int length) { return blocks > length ? (blocks - 1) / length + 1 : 1; }
+__device__ __forceinline__ int tile_parts(int blocks, int length) {
+  return blocks > length ? (blocks - 1) / length + 1 : 1;
+}
 
 // Even windows that fill the chip by themselves (split false): XCD id % 8 takes every 8th (window, key head) with all
 // its tiles, so that its L2 reads the keys once; the windows longest first (up to 64 of them), and every other round
@@ -25,7 +27,7 @@ __device__ __forceinline__ PagedItem whole_item(const PagedArgs& a, int place) {
   const int units = static_cast<int>(a.tokens.B * a.Hkv), per_round = kCusPerXcd / q_tiles;
   if (kCusPerXcd % q_tiles == 0 && per_round > 1) {
     const int round = k / per_round;
-    if ((round & 1) && round < units / kXcds / per_round) k = round * per_round + (per_round - 1 - (k - round * per_round));
+    if ((round & 1) && round < units / kXcds / per_round) k = (2 * round + 1) * per_round - 1 - k;
   }
   const int unit = k * kXcds + (place & 7);
   PagedItem item{-1, 0, 0, 1, seq - seq / q_tiles * q_tiles, q_tiles, 0, 0};

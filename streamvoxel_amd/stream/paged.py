@@ -1,9 +1,9 @@
 """A paged cache of keys and values on the HIP kernels: the append that fills it, the attention over it, and the context
 that stands in `CachedContext`'s place with its windows in one pool of pages.
 
-`step.CachedContext` (PackedKeys, streamvoxel/stream/fast_ops.py:122-159) keeps a slab of the longest condition for every
-slot and rewrites it whole; here a window holds the pages that its keys fill, and new keys go behind the ones that are
-there. No counterpart in the reference.
+`step.CachedContext` (PackedKeys, streamvoxel/stream/fast_ops.py:122-159) keeps a slab of the longest condition for
+every slot and rewrites it whole; here a window holds the pages that its keys fill, and new keys go behind the ones
+that are there. No counterpart in the reference.
 """
 from __future__ import annotations
 
@@ -16,7 +16,7 @@ from streamvoxel_amd import _lib
 
 __all__ = ['paged_append', 'paged_attention', 'PagedContext']
 
-LAYOUTS = {None: _lib.SVHIP_ROTARY_NONE, 'half': _lib.SVHIP_ROTARY_HALF, 'interleaved': _lib.SVHIP_ROTARY_INTERLEAVED,
+LAYOUTS = {'half': _lib.SVHIP_ROTARY_HALF, 'interleaved': _lib.SVHIP_ROTARY_INTERLEAVED,
            'axial': _lib.SVHIP_ROTARY_AXIAL}
 
 
@@ -91,14 +91,15 @@ def paged_append(key, value, k_pages, v_pages, page_table, lengths, cu_tokens=No
 
     key, value bf16 [B,H,n,D] (head_dim contiguous, any other strides), or packed [H,T,D] with the windows' borders
     `cu_tokens` int32 [B+1] (device, ascending; tokens outside every window are left alone). k_pages, v_pages
-    [pages,H,page,D] in bf16, or float8_e4m3fn with `k_exponents` / `v_exponents` uint8 [pages,H,page], one power of two
-    2^(exponent - 127) for each row (written too); page a power of two from 16 to 1024. page_table int32 [B, m]: key j of
-    window b is row j % page of page page_table[b, j // page]. `lengths` int32 [B] (device) counts each window's keys with
-    the new ones: they are its last n keys, or the n in front of its last `before`. Two tokens must not share a row.
-    `frequencies` rotates the keys: with layout 'half' / 'interleaved' as `rotary` does (fp64; `positions` int32 / int64 [B,n]
-    or [T], or None: each key's index in its window; `amplitude`), with 'axial' as `producer.axial_rope` does (its fp32
-    buffer and fp32 positions [B,n,3] or [T,3]). `bad` (optional int32 [1], device) becomes 1 when a key lies outside
-    its window's row of the table or a page outside the pool; such keys are not written."""
+    [pages,H,page,D] in bf16, or float8_e4m3fn with `k_exponents` / `v_exponents` uint8 [pages,H,page], one power of
+    two 2^(exponent - 127) for each row (written too); page a power of two from 16 to 1024. page_table int32 [B, m]:
+    key j of window b is row j % page of page page_table[b, j // page]. `lengths` int32 [B] (device) counts each
+    window's keys with the new ones: they are its last n keys, or the n in front of its last `before`. Two tokens must
+    not share a row. `frequencies` rotates the keys: with layout 'half' / 'interleaved' as `rotary` does (fp64;
+    `positions` int32 / int64 [B,n] or [T], or None: each key's index in its window; `amplitude`), with 'axial' as
+    `producer.axial_rope` does (its fp32 buffer and fp32 positions [B,n,3] or [T,3]). `bad` (optional int32 [1],
+    device) becomes 1 when a key lies outside its window's row of the table or a page outside the pool; such keys are
+    not written."""
     _lib.require_one_gpu(key, value, k_pages, v_pages, page_table, lengths, cu_tokens, positions, frequencies, k_exponents,
                          v_exponents, bad)
     code = _check_pool(k_pages, v_pages, page_table, lengths, k_exponents, v_exponents, bad)
@@ -117,7 +118,7 @@ def paged_append(key, value, k_pages, v_pages, page_table, lengths, cu_tokens=No
         raise ValueError('k_pages and v_pages must have a place for every element')
     wide, pairs, sp, turn = 0, 0, (0, 0), _lib.SVHIP_ROTARY_NONE
     if frequencies is not None:
-        if layout not in ('half', 'interleaved', 'axial'):
+        if layout not in LAYOUTS:
             raise ValueError("layout is 'half', 'interleaved' or 'axial'")
         turn, tokens = LAYOUTS[layout], (n,) if cu_tokens is not None else (B, n)
         if layout == 'axial':
@@ -151,15 +152,15 @@ def paged_attention(query, k_pages, v_pages, page_table, lengths, cu_queries=Non
                     k_exponents=None, v_exponents=None, out=None, bad=None):
     """softmax(scale * Q K^T) V of the windows' new tokens over the first lengths[b] keys of their pages.
 
-    query bf16 [B,H,n,D] (head_dim contiguous, any other strides), or packed [H,T,D] with the windows' borders `cu_queries`
-    int32 [B+1] (device, ascending). k_pages, v_pages, page_table, lengths and the exponents as `paged_append` fills them;
-    the H heads share the pages' heads evenly, head h reads head h // (H / heads). `causal`: the n tokens are the window's
-    last n keys, and token i sees keys up to its own, lengths[b] - n + i; without it every token sees all of them. A token
-    with no key gets zeros, and what is not finite among keys that a token does not see does not reach it. `out` (optional; query
-    itself, or memory that query does not share) bf16 like query with a contiguous head_dim; its rows outside every window are
-    left as they are (a fresh one has them undefined). `bad` (optional int32 [1], device) becomes 1 when a page lies
-    outside the pool (its keys and values read as zeros) or a length passes the window's row of the table (and is cut).
-    Returns out."""
+    query bf16 [B,H,n,D] (head_dim contiguous, any other strides), or packed [H,T,D] with the windows' borders
+    `cu_queries` int32 [B+1] (device, ascending). k_pages, v_pages, page_table, lengths and the exponents as
+    `paged_append` fills them; the H heads share the pages' heads evenly, head h reads head h // (H / heads).
+    `causal`: the n tokens are the window's last n keys, and token i sees keys up to its own, lengths[b] - n + i;
+    without it every token sees all of them. A token with no key gets zeros, and what is not finite among keys that a
+    token does not see does not reach it. `out` (optional; query itself, or memory that query does not share) bf16
+    like query with a contiguous head_dim; its rows outside every window are left as they are (a fresh one has them
+    undefined). `bad` (optional int32 [1], device) becomes 1 when a page lies outside the pool (its keys and values
+    read as zeros) or a length passes the window's row of the table (and is cut). Returns out."""
     _lib.require_one_gpu(query, k_pages, v_pages, page_table, lengths, cu_queries, k_exponents, v_exponents, out, bad)
     code = _check_pool(k_pages, v_pages, page_table, lengths, k_exponents, v_exponents, bad)
     if query.dtype != torch.bfloat16:
@@ -189,15 +190,16 @@ def paged_attention(query, k_pages, v_pages, page_table, lengths, cu_queries=Non
 
 
 class PagedContext:
-    """The cached keys and values of `batch` windows in one pool of `pages` pages a layer (each `page_size` keys of every head),
-    in `CachedContext`'s place: `write`, `attend`, `lengths` as there, and windows that grow (`grow`, `append`) and give
-    their pages back (`release`). A window holds as many pages as its keys need, at most `max_pages` of them (default: all).
-    kv_dtype 'bf16' or 'fp8' (OCP e4m3fn with one power of two for each row and head).
+    """The cached keys and values of `batch` windows in one pool of `pages` pages a layer (each `page_size` keys of
+    every head), in `CachedContext`'s place: `write`, `attend`, `lengths` as there, and windows that grow (`grow`,
+    `append`) and give their pages back (`release`). A window holds as many pages as its keys need, at most
+    `max_pages` of them (default: all). kv_dtype 'bf16' or 'fp8' (OCP e4m3fn with one power of two for each row and
+    head).
 
-    The host keeps the books: `resize` and `grow` take and free pages and send table and lengths to the device on the current
-    stream without waiting for it; calls that touch a window's pages must be ordered after them, as usual. A replayed graph
-    reads the table and the lengths as they stand. `bad` (device int32 [1]) becomes non-zero when a call meets a page outside
-    the pool, which these books never name."""
+    The host keeps the books: `resize` and `grow` take and free pages and send table and lengths to the device on the
+    current stream without waiting for it; calls that touch a window's pages must be ordered after them, as usual. A
+    replayed graph reads the table and the lengths as they stand. `bad` (device int32 [1]) becomes non-zero when a
+    call meets a page outside the pool, which these books never name."""
 
     def __init__(self, layers, batch, heads, head_dim, pages, device, page_size=64, max_pages=None, kv_dtype='bf16'):
         if kv_dtype not in ('bf16', 'fp8'):
@@ -232,7 +234,8 @@ class PagedContext:
         return -(-length // self.page_size)
 
     def _set(self, wanted):
-        """The windows' lengths {index: length}: pages taken and freed, table and lengths sent. Nothing changes on error."""
+        """The windows' lengths {index: length}: pages taken and freed, table and lengths sent. Nothing changes on
+        error."""
         need = 0
         for index, length in wanted.items():
             if not 0 <= index < self.batch:
@@ -261,15 +264,16 @@ class PagedContext:
 
     @staticmethod
     def _send(to, values):
-        """Host numbers to the device on the current stream, not waited for: one by a fill, more from pinned memory (which
-        the allocator keeps until the copy is done)."""
+        """Host numbers to the device on the current stream, not waited for: one by a fill, more from pinned memory
+        (which the allocator keeps until the copy is done)."""
         if len(values) == 1:
             to.fill_(values[0])
         elif values:
             to.copy_(torch.tensor(values, dtype=torch.int32, pin_memory=True), non_blocking=True)
 
     def resize(self, index, length):
-        """Window `index` holds `length` keys: pages taken or given back at its end (the keys below both lengths stay)."""
+        """Window `index` holds `length` keys: pages taken or given back at its end (the keys below both lengths
+        stay)."""
         self._set({int(index): int(length)})
 
     def release(self, index):
@@ -288,8 +292,8 @@ class PagedContext:
         return t if t.stride(-1) == 1 else t.contiguous()
 
     def append(self, layer, key, value, index=None, n=None, cu_tokens=None, **how):
-        """`paged_append` into layer `layer` of the first n windows (all by default), or of window `index` alone (key, value
-        [heads, L, head_dim] then); `how`: its before, positions, frequencies, layout, amplitude."""
+        """`paged_append` into layer `layer` of the first n windows (all by default), or of window `index` alone (key,
+        value [heads, L, head_dim] then); `how`: its before, positions, frequencies, layout, amplitude."""
         at = slice(0, self.batch if n is None else n)
         if index is not None:
             at, key, value = slice(index, index + 1), key[None], value[None]
@@ -299,9 +303,9 @@ class PagedContext:
                      k_exponents=self.k_exponents[layer], v_exponents=self.v_exponents[layer], bad=self.bad, **how)
 
     def write(self, layer, index, key, value, prefix=None, positions=None, frequencies=None):
-        """Window `index` of `layer` anew, as `CachedContext.write`: keys [0, P) from `prefix` = (prefix_k, prefix_v) [H, P, D]
-        (already rotated), keys [P, P + L) from key, value [H, L, D] (K rotated by AxialRoPE at fp32 positions [L, 3] with
-        the fp32 `frequencies` buffer when given). Sets the window's length and pages."""
+        """Window `index` of `layer` anew, as `CachedContext.write`: keys [0, P) from `prefix` = (prefix_k, prefix_v)
+        [H, P, D] (already rotated), keys [P, P + L) from key, value [H, L, D] (K rotated by AxialRoPE at fp32
+        positions [L, 3] with the fp32 `frequencies` buffer when given). Sets the window's length and pages."""
         _lib.require_gpu(key, value)
         key, value = self._rows(key), self._rows(value)
         H, L, D = key.shape
@@ -330,8 +334,8 @@ class PagedContext:
             self.append(layer, key, value, index=index, **how)
 
     def attend(self, layer, query, out=None, n=None, cu_queries=None, causal=False):
-        """Attention of `query` [n,H,Q,D] bf16 (H a multiple of the cache's heads; packed [H,T,D] with cu_queries) over the keys
-        of the first n windows."""
+        """Attention of `query` [n,H,Q,D] bf16 (H a multiple of the cache's heads; packed [H,T,D] with cu_queries)
+        over the keys of the first n windows."""
         n = self.batch if n is None else n
         return paged_attention(query, self.k[layer], self.v[layer], self.table[:n], self.lengths[:n], cu_queries=cu_queries,
                                causal=causal, out=out, k_exponents=self.k_exponents[layer],

@@ -1,8 +1,8 @@
 """Rotary positions of one axis on the HIP kernels: interleaved and half layouts, part of a head, frequencies scaled for
 contexts longer than the trained one.
 
-Beside `producer.axial_rope` (AxialRoPE, streamvoxel/models/unconditional_md4.py:10-24), which turns the three axes of the
-reference's positions with the reference's bf16 roundings; no counterpart in the reference.
+Beside `producer.axial_rope` (AxialRoPE, streamvoxel/models/unconditional_md4.py:10-24), which turns the three axes of
+the reference's positions with the reference's bf16 roundings; no counterpart in the reference.
 """
 from __future__ import annotations
 
@@ -20,9 +20,9 @@ LAYOUTS = {'half': _lib.SVHIP_ROTARY_HALF, 'interleaved': _lib.SVHIP_ROTARY_INTE
 
 def rotary_frequencies(rotary_dim, base=10000.0, scaling=None, factor=1.0, original_length=None, low=1.0, high=32.0,
                        device=None):
-    """(frequencies, amplitude): the fp64 frequencies base^(-2i / rotary_dim), i < rotary_dim / 2, in radians a position, and
-    the factor of the turned pairs, 1 unless the scaling changes it. `scaling` for contexts `factor` times as long as
-    the trained one:
+    """(frequencies, amplitude): the fp64 frequencies base^(-2i / rotary_dim), i < rotary_dim / 2, in radians a
+    position, and the factor of the turned pairs, 1 unless the scaling changes it. `scaling` for contexts `factor`
+    times as long as the trained one:
       'linear': every frequency divided by `factor` (position interpolation);
       'wavelength': the pairs that make fewer than `low` turns over `original_length` trained positions divided by it,
         those that make more than `high` kept, a linear ramp in between, and the amplitude 0.1 ln(factor) + 1 (the
@@ -75,12 +75,13 @@ class _Rotary(torch.autograd.Function):
 
 
 def rotary(x, positions, frequencies, layout='half', amplitude=1.0, out=None):
-    """Rotary positions of x [B,H,N,D] bf16 or fp32 (head_dim contiguous, any other strides; packed tokens as [1,H,T,D]) at
-    integer positions [N] or [B,N] (int32 or int64, any sign): pair i of the first 2 * len(frequencies) elements turns by
-    positions * frequencies[i] and is scaled by `amplitude`, the other elements are kept. `layout` 'half' pairs element i
-    with i + len(frequencies), 'interleaved' 2i with 2i + 1. frequencies: the fp64 buffer of `rotary_frequencies`, at most
-    128 pairs. The turns are formed in 64 bits (far positions keep their angle), the rest in fp32, rounded once to x's type.
-    Differentiable in x (captured into a graph: for leaves that no eager graph still holds). `out` (optional, no gradient through it; x itself, or memory that x does not share) receives the
+    """Rotary positions of x [B,H,N,D] bf16 or fp32 (head_dim contiguous, any other strides; packed tokens as
+    [1,H,T,D]) at integer positions [N] or [B,N] (int32 or int64, any sign): pair i of the first 2 * len(frequencies)
+    elements turns by positions * frequencies[i] and is scaled by `amplitude`, the other elements are kept. `layout`
+    'half' pairs element i with i + len(frequencies), 'interleaved' 2i with 2i + 1. frequencies: the fp64 buffer of
+    `rotary_frequencies`, at most 128 pairs. The turns are formed in 64 bits (far positions keep their angle), the
+    rest in fp32, rounded once to x's type. Differentiable in x (captured into a graph: for leaves that no eager graph
+    still holds). `out` (optional, no gradient through it; x itself, or memory that x does not share) receives the
     result; returns it."""
     _lib.require_one_gpu(x, positions, frequencies, out)
     if layout not in LAYOUTS:
