@@ -454,7 +454,7 @@ int svhip_rotary(const svhip_rotary_args* args, void* stream);
  * 16-byte aligned (e4m3: 8), max_pages * page_size at most 2^30. Key j of window b is row j % page_size of page
  * page_table[b*table_stride + j / page_size] (int32, max_pages numbers a window); lengths[b] (int32) counts the
  * window's keys. kv_dtype SVHIP_BF16, or SVHIP_FP8_E4M3: OCP e4m3fn codes with one power of two for each row and
- * head, value = code 2^(exponent - 127), exponent bytes (page, h, r) at page*se_p + h*se_h + r. Windows may share
+ * head, value = code 2^(exponent - 127), exponents 1 to 254, bytes (page, h, r) at page*se_p + h*se_h + r. Windows may share
  * pages that are only read. `bad` (int32, may be null) is set to 1 by a call that meets a page outside the pool or
  * a key outside its window's row of the table.
  */

@@ -92,7 +92,7 @@ def paged_append(key, value, k_pages, v_pages, page_table, lengths, cu_tokens=No
     key, value bf16 [B,H,n,D] (head_dim contiguous, any other strides), or packed [H,T,D] with the windows' borders
     `cu_tokens` int32 [B+1] (device, ascending; tokens outside every window are left alone). k_pages, v_pages
     [pages,H,page,D] in bf16, or float8_e4m3fn with `k_exponents` / `v_exponents` uint8 [pages,H,page], one power of
-    two 2^(exponent - 127) for each row (written too); page a power of two from 16 to 1024. page_table int32 [B, m]:
+    two 2^(exponent - 127) for each row (written too, 1 to 254); page a power of two from 16 to 1024. page_table int32 [B, m]:
     key j of window b is row j % page of page page_table[b, j // page]. `lengths` int32 [B] (device) counts each
     window's keys with the new ones: they are its last n keys, or the n in front of its last `before`. Two tokens must
     not share a row. `frequencies` rotates the keys: with layout 'half' / 'interleaved' as `rotary` does (fp64;

@@ -60,18 +60,22 @@ def _launch(x, out, positions, frequencies, layout, amplitude, inverse):
 
 
 class _Rotary(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, x, positions, frequencies, layout, amplitude):
-        ctx.save_for_backward(positions, frequencies)
-        ctx.args = layout, amplitude
-        return _launch(x, torch.empty_like(x), positions, frequencies, layout, amplitude, 0)
+    """The rotation, or its transpose (inverse 1): linear, so that each is the other's gradient, as often as asked for."""
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
+    def forward(ctx, x, positions, frequencies, layout, amplitude, inverse):
+        ctx.save_for_backward(positions, frequencies)
+        ctx.args = layout, amplitude, 1 - inverse
+        return _launch(x, torch.empty_like(x), positions, frequencies, layout, amplitude, inverse)
+
+    @staticmethod
     def backward(ctx, dy):
-        positions, frequencies = ctx.saved_tensors
         dy = dy if dy.stride(-1) == 1 else dy.contiguous()
-        return _launch(dy, torch.empty_like(dy), positions, frequencies, *ctx.args, 1), None, None, None, None
+        if torch.is_grad_enabled() and dy.requires_grad:
+            dx = _Rotary.apply(dy, *ctx.saved_tensors, *ctx.args)
+        else:
+            dx = _launch(dy, torch.empty_like(dy), *ctx.saved_tensors, *ctx.args)
+        return dx, None, None, None, None, None
 
 
 def rotary(x, positions, frequencies, layout='half', amplitude=1.0, out=None):
@@ -99,7 +103,7 @@ def rotary(x, positions, frequencies, layout='half', amplitude=1.0, out=None):
         raise ValueError(f'{frequencies.numel()} frequencies do not fit head_dim {D} (at most 128)')
     if out is None:
         if torch.is_grad_enabled() and x.requires_grad:
-            return _Rotary.apply(x, positions, frequencies, layout, float(amplitude))
+            return _Rotary.apply(x, positions, frequencies, layout, float(amplitude), 0)
         out = torch.empty_like(x)
     else:
         if torch.is_grad_enabled() and (x.requires_grad or out.requires_grad):

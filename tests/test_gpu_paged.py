@@ -376,10 +376,11 @@ def test_append_against_float64(counts, packed, before, D, H, page, layout, part
 
 
 @pytest.mark.parametrize('kv_dtype', ['bf16', 'fp8'])
-def test_axial_append_has_the_bits_of_the_axial_rotation(kv_dtype):
+@pytest.mark.parametrize('D', [48, 96])
+def test_axial_append_has_the_bits_of_the_axial_rotation(D, kv_dtype):
     from streamvoxel_amd.stream.paged import paged_append
     from streamvoxel_amd.stream.producer import axial_rope, rope_frequencies
-    H, D, n = 3, 48, 77
+    H, n = 3, 77
     g = torch.Generator().manual_seed(2)
     key, value = [torch.randn(2, n, H, D, generator=g).to(torch.bfloat16).to(DEV).transpose(1, 2) for _ in 'kv']
     positions = (torch.rand(2, n, 3, generator=g) * 64 - 8).to(DEV)

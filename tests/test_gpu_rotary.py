@@ -186,3 +186,18 @@ def test_rotary_gradient_in_a_graph():
         assert torch.equal(y.detach(), rotary(x.detach(), positions, f, 'interleaved'))
         # The transposed rotation is the rotation by the negative angle, whose sines are the same numbers negated.
         assert torch.equal(dx, rotary(dy, -positions, f, 'interleaved'))
+
+
+def test_rotary_gradient_of_the_gradient():
+    """The rotation is linear: the gradient of <w, dx> by dy is the rotation of w, whatever the order."""
+    from streamvoxel_amd.stream.rotary import rotary
+    g = torch.Generator().manual_seed(9)
+    x, w = [torch.randn(2, 3, 20, 32, generator=g).to(DEV) for _ in 'xw']
+    dy = torch.randn(2, 3, 20, 32, generator=g).to(DEV).requires_grad_()
+    positions, f = torch.arange(20, device=DEV) * 7, freqs(16)
+    y = rotary(x.requires_grad_(), positions, f, amplitude=1.5)
+    dx, = torch.autograd.grad(y, x, dy, create_graph=True)
+    ddy, = torch.autograd.grad(dx, dy, w, create_graph=True)
+    assert torch.equal(ddy.detach(), rotary(w, positions, f, amplitude=1.5))
+    again, = torch.autograd.grad(y, x, dy.detach())
+    assert torch.equal(again, dx.detach())
