@@ -138,7 +138,7 @@ __global__ __launch_bounds__(kPagedThreads) void paged_join_kernel(PagedArgs a) 
     if (each < 1) return set_bad(a.pages);
     count = blocks > each ? (blocks - 1) / each + 1 : 1;
     if (count < 2) return;
-    if (plan.x < 0 || plan.y < count || tiles <= qt ||
+    if (plan.x < 0 || plan.y < count || plan.y > a.tile_slots || tiles <= qt || tiles > a.tile_slots ||
         plan.x + static_cast<int64_t>(a.Hkv) * plan.y * tiles > a.tile_slots) {
       return set_bad(a.pages);
     }

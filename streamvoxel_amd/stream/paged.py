@@ -160,7 +160,8 @@ def paged_attention(query, k_pages, v_pages, page_table, lengths, cu_queries=Non
     token does not see does not reach it. `out` (optional; query itself, or memory that query does not share) bf16
     like query with a contiguous head_dim; its rows outside every window are left as they are (a fresh one has them
     undefined). `bad` (optional int32 [1], device) becomes 1 when a page lies outside the pool (its keys and values
-    read as zeros) or a length passes the window's row of the table (and is cut). Returns out."""
+    read as zeros) or a length passes the window's row of the table (and is cut). Takes no part in a gradient. Returns
+    out."""
     _lib.require_one_gpu(query, k_pages, v_pages, page_table, lengths, cu_queries, k_exponents, v_exponents, out, bad)
     code = _check_pool(k_pages, v_pages, page_table, lengths, k_exponents, v_exponents, bad)
     if query.dtype != torch.bfloat16:

@@ -832,3 +832,31 @@ def test_every_head_width(D, page, kv_dtype):
     if kv_dtype == 'bf16':
         at = torch.arange(697, 700, device=DEV)
         assert torch.equal(args[0][args[2][0].long()[at // page], :, at % page], key[0].transpose(0, 1))
+
+
+@pytest.mark.parametrize('B', [20, 90])
+def test_a_captured_call_follows_lengths_and_borders(B):
+    """A packed call captured once: its plan is made on the device at every replay, whatever the lengths and the borders
+    are by then."""
+    from streamvoxel_amd.stream.paged import paged_attention
+    longest, T = 1200, 400
+    pool = Pool([longest] * B, 2, 32, 64, B, clean=True)
+    k, v, table, lengths = pool.args()
+    q = torch.randn(4, T, 32, generator=torch.Generator().manual_seed(B)).to(torch.bfloat16).to(DEV)
+    cu = torch.zeros(B + 1, dtype=torch.int32, device=DEV)
+    call = lambda: paged_attention(q, k, v, table, lengths, cu_queries=cu, causal=True)
+    call()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = call()
+    g = torch.Generator().manual_seed(1)
+    for most in (30, longest, 1, longest):
+        pool.lengths = torch.randint(0, most + 1, (B,), generator=g).tolist()
+        cut = sorted(torch.randint(0, T + 1, (B - 1,), generator=g).tolist())
+        borders = [0, *cut, T] if most > 1 else [0] * B + [T]
+        lengths.copy_(torch.tensor(pool.lengths, dtype=torch.int32))
+        cu.copy_(torch.tensor(borders, dtype=torch.int32))
+        graph.replay()
+        torch.cuda.synchronize()
+        check(out, q, pool, True, borders)
+        assert torch.equal(out, call())
