@@ -138,21 +138,27 @@ def require_gpu(*tensors):
 
 def require_one_gpu(first, *tensors):
     """require_gpu, and all of them on one device."""
-    device = first.device if torch.is_tensor(first) else None
-    for t in tensors:
-        if t is not None and not (torch.is_tensor(t) and t.device == device):
-            require_gpu(first, *tensors)
-            raise ValueError(f'tensors on {device} and {t.device}: one call takes one device')
-    if device is None or device.type != 'cuda':
-        require_gpu(first, *tensors)
+    try:
+        index = first.get_device()             # -1 on the host
+        if index >= 0:
+            for t in tensors:
+                if t is not None and t.get_device() != index:
+                    break
+            else:
+                return
+    except AttributeError:
+        pass
+    require_gpu(first, *tensors)
+    raise ValueError('tensors on ' + ', '.join(sorted({str(t.device) for t in (first, *tensors) if t is not None}))
+                     + ': one call takes one device')
 
 
 def launch(name, t, *args):
-    """The entry point `name` with args and the current stream of the tensor's device, launched on that device whatever the
-    current one is; RuntimeError for a status."""
-    fn, index = getattr(load(), name), t.get_device()
-    stream = torch._C._cuda_getCurrentRawStream(index)   # what current_stream(index).cuda_stream is, in a tenth of the time
-    if index == torch.cuda.current_device():
+    """The entry point `name` with args and the current stream of the tensor's device, launched on that device whatever
+    the current one is; RuntimeError for a status."""
+    fn, index = getattr(_lib or load(), name), t.get_device()
+    stream = torch._C._cuda_getCurrentRawStream(index)   # current_stream(index).cuda_stream, in a tenth of the time
+    if index == torch._C._cuda_getDevice():
         rc = fn(*args, stream)
     else:
         with torch.cuda.device(index):

@@ -7,7 +7,6 @@ that are there. No counterpart in the reference.
 """
 from __future__ import annotations
 
-import math
 import struct
 
 import torch
@@ -22,7 +21,8 @@ LAYOUTS = {'half': _lib.SVHIP_ROTARY_HALF, 'interleaved': _lib.SVHIP_ROTARY_INTE
 
 def _check_pool(k_pages, v_pages, page_table, lengths, k_exponents, v_exponents, bad):
     """The pool's type code; ValueError / TypeError for what the kernels do not take."""
-    if k_pages.dim() != 4 or v_pages.shape != k_pages.shape or v_pages.dtype != k_pages.dtype:
+    shape, dtype = k_pages.shape, k_pages.dtype
+    if len(shape) != 4 or v_pages.shape != shape or v_pages.dtype != dtype:
         raise ValueError('k_pages and v_pages must be [pages, heads, page, head_dim] alike')
     if k_pages.stride(-1) != 1 or v_pages.stride(-1) != 1:
         raise ValueError('rows of a page need a contiguous head_dim')
@@ -32,35 +32,41 @@ def _check_pool(k_pages, v_pages, page_table, lengths, k_exponents, v_exponents,
         raise ValueError('lengths must be a contiguous int32 [B]')
     if bad is not None and (bad.dtype != torch.int32 or bad.numel() != 1):
         raise ValueError('bad must be one int32')
-    if k_pages.dtype == torch.bfloat16:
+    if dtype == torch.bfloat16:
         if k_exponents is not None or v_exponents is not None:
             raise TypeError('bf16 pages take no exponents')
         return _lib.SVHIP_BF16
-    if k_pages.dtype != torch.float8_e4m3fn:
-        raise TypeError(f'pages of {k_pages.dtype} unsupported (bfloat16 or float8_e4m3fn)')
+    if dtype != torch.float8_e4m3fn:
+        raise TypeError(f'pages of {dtype} unsupported (bfloat16 or float8_e4m3fn)')
     for e in (k_exponents, v_exponents):
-        if e is None or e.dtype != torch.uint8 or e.shape != k_pages.shape[:3] or e.stride(-1) != 1:
-            raise ValueError('e4m3 pages need k_exponents and v_exponents, uint8 [pages, heads, page] with contiguous rows')
+        if e is None or e.dtype != torch.uint8 or e.shape != shape[:3] or e.stride(-1) != 1:
+            raise ValueError('e4m3 pages need k_exponents and v_exponents, uint8 [pages, heads, page] with contiguous '
+                             'rows')
     return _lib.SVHIP_FP8_E4M3
 
 
 def _windows(t, cu, B, what):
     """(heads, tokens, (stride of a window, of a head, of a token)) of [B,H,n,D], or packed [H,T,D] with borders cu."""
+    shape, stride = t.shape, t.stride()
     if cu is None:
-        if t.dim() != 4 or t.shape[0] != B:
+        if len(shape) != 4 or shape[0] != B:
             raise ValueError(f'{what} must be [B, heads, n, head_dim] with the B windows of the table, or packed '
                              '[heads, T, head_dim] with their borders')
-        return t.shape[1], t.shape[2], (t.stride(0), t.stride(1), t.stride(2))
+        return shape[1], shape[2], stride[:3]
     if cu.dtype != torch.int32 or cu.shape != (B + 1,) or not cu.is_contiguous():
         raise ValueError('the borders must be a contiguous int32 [B + 1]')
-    if t.dim() != 3:
+    if len(shape) != 3:
         raise ValueError(f'packed {what} must be [heads, T, head_dim]')
-    return t.shape[0], t.shape[1], (0, t.stride(0), t.stride(1))
+    return shape[0], shape[1], (0, *stride[:2])
 
 
 def _rows16(t):
     """bf16 rows on 16-byte boundaries: the tensor itself, or a contiguous copy."""
-    if t.stride(-1) == 1 and t.data_ptr() % 16 == 0 and all(s % 8 == 0 for s in t.stride()[:-1]):
+    *rows, last = t.stride()
+    off = t.data_ptr() >> 1
+    for s in rows:
+        off |= s
+    if last == 1 and off & 7 == 0:
         return t
     return t.clone() if t.is_contiguous() else t.contiguous()
 
@@ -179,7 +185,7 @@ def paged_attention(query, k_pages, v_pages, page_table, lengths, cu_queries=Non
     elif _lib.overlaps(given, out) and (given.data_ptr() != out.data_ptr() or given.stride() != out.stride()):
         raise ValueError('out must be query itself or memory that query does not share')
     so = _windows(out, cu_queries, B, 'out')[2]
-    scale = 1.0 / math.sqrt(D) if scale is None else float(scale)
+    scale = D ** -0.5 if scale is None else float(scale)
     nbytes = _lib.load().svhip_paged_attention_workspace_bytes(B, H, Hkv, n, cu_queries is not None, D,
                                                                page_table.shape[1] * S)
     cache = _packed(code, k_pages, v_pages, page_table, lengths, k_exponents, v_exponents, bad)

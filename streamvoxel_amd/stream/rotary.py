@@ -95,7 +95,7 @@ def rotary(x, positions, frequencies, layout='half', amplitude=1.0, out=None):
     if x.dim() != 4 or x.stride(-1) != 1:
         raise ValueError('x must be [B, H, N, D] with a contiguous head_dim')
     B, H, N, D = x.shape
-    if positions.dtype not in (torch.int32, torch.int64) or tuple(positions.shape) not in ((N,), (B, N)):
+    if positions.dtype not in (torch.int32, torch.int64) or (positions.shape != (N,) and positions.shape != (B, N)):
         raise ValueError(f'positions must be int32 or int64 [N] or [B, N], got {positions.dtype} {tuple(positions.shape)}')
     if frequencies.dtype != torch.float64 or frequencies.dim() != 1 or not frequencies.is_contiguous():
         raise ValueError('frequencies must be a contiguous fp64 vector')
