@@ -5,12 +5,12 @@
 // as the columns of S^T = K Q^T and O^T = V^T P^T (v_mfma_f32_32x32x16_bf16), so that the softmax of a row stays in
 // two lanes and P^T leaves the first product in the second one's operand layout (K rows lie in LDS under sigma_row;
 // xattn_kernel.hpp). V rows lie as they come and are read transposed (ds_read_b64_tr_b16). Two forms of work:
-//   * windows of more than kRows rows (tile, paged_tile.hpp): a workgroup takes 128 rows, 32 a wave; the 4 waves
+//   * windows of more than kRowMost rows (tile, paged_tile.hpp): a workgroup takes 128 rows, 32 a wave; the 4 waves
 //     stage each block of 64 keys together, the next one in flight while the current one is computed. Bound: the
 //     matrix cores and the exponentials, which overlap little. Measured: 8 windows x 1024 queries, 1552 to 9744 keys,
 //     12 x 64 (153 GFLOP) 200 us, 770 TFLOP/s; 4 causal chunks of 512, 16 heads to 4 of 128, up to 16 384 keys (241
 //     GFLOP) 268 us and 12 of join.
-//   * windows of up to kRows rows, single tokens among them (row, paged_row.hpp): the 4 waves share the rows and
+//   * windows of up to kRowMost rows, single tokens among them (row, paged_row.hpp): the 4 waves share the rows and
 //     split the keys, each staging its own blocks of 32 keys in its own LDS; no barrier until the waves' sums are
 //     joined. Bound: HBM. Measured: 64 tokens over 1.18 GB of keys 216 us, 5.4 TB/s; over 754 MB of e4m3 pages 148
 //     us, 5.1 TB/s; one token over 30 MB 9.1 us, a chain of loads. One wave a row of its own, with shuffles instead
@@ -34,14 +34,14 @@ namespace svhip {
 // launch.)
 __global__ __launch_bounds__(kPlanThreads) void paged_plan_kernel(PagedArgs a, bool rows, bool tiles) {
   __shared__ float of_wave[kPlanThreads / 64];
-  __shared__ int2 counts[kPlanThreads / 64];
+  __shared__ int4 counts[kPlanThreads / 64];
   const BlockTeam team{of_wave};
   const int tid = static_cast<int>(threadIdx.x), Hkv = a.Hkv;
   int unused, more;
   float total;
   const int row_each = rows && a.row_part ? row_length(a, team, 0, unused) : kUncut;
   const int tile_each = tiles ? tile_length(a, team, unused, more, total) : kUncut;
-  int2 at = make_int2(0, 0);
+  int2 at = make_int2(0, 0), slot = at;
   int cut = 0;  // 1: windows of the row form, 2: tiles
   for (int64_t c0 = 0; c0 < a.tokens.B; c0 += kPlanThreads) {
     const int64_t c = c0 + tid;
@@ -57,24 +57,29 @@ __global__ __launch_bounds__(kPlanThreads) void paged_plan_kernel(PagedArgs a, b
       }
     }
     cut |= parts > 1 ? (t > 0 ? 2 : 1) : 0;
-    int row_sum, tile_sum;
-    int2 before = make_int2(wave_prefix(row, row_sum), 0);
-    before.y = wave_prefix(tile, tile_sum);
-    if ((tid & 63) == 0) counts[tid >> 6] = make_int2(row_sum, tile_sum);
+    const int row_n = parts > 1 ? row : 0, tile_n = parts > 1 ? tile : 0;
+    int4 sums;  // of places, then of slots
+    int4 before = make_int4(wave_prefix(row, sums.x), 0, 0, 0);
+    before.y = wave_prefix(tile, sums.y);
+    before.z = wave_prefix(row_n, sums.z);
+    before.w = wave_prefix(tile_n, sums.w);
+    if ((tid & 63) == 0) counts[tid >> 6] = sums;
     __syncthreads();
-    int2 sum = at;
 #pragma unroll
     for (int i = 0; i < kPlanThreads / 64; ++i) {
       if (i == tid >> 6) {
-        before.x += sum.x;
-        before.y += sum.y;
+        before.x += at.x;
+        before.y += at.y;
+        before.z += slot.x;
+        before.w += slot.y;
       }
-      sum.x += counts[i].x;
-      sum.y += counts[i].y;
+      at.x += counts[i].x;
+      at.y += counts[i].y;
+      slot.x += counts[i].z;
+      slot.y += counts[i].w;
     }
-    at = sum;
     if (c < a.tokens.B) {
-      a.plan[c] = t > 0 ? make_int4(before.y, parts, tile_each, t) : make_int4(before.x, parts, row_each, 1);
+      a.plan[c] = t > 0 ? make_int4(before.w, parts, tile_each, t) : make_int4(before.z, parts, row_each, 1);
       a.running[c] = make_int2(before.x + row, before.y + tile);
     }
     __syncthreads();
@@ -198,23 +203,28 @@ __global__ __launch_bounds__(kPagedThreads) void paged_join_kernel(PagedArgs a) 
 // 217.6 and 222.9; 32 768 rows in two parts: 323 with, 281 without; 16 304 rows 116 and 104).
 constexpr int64_t kJoinFew = 4096;
 
-inline PagedPlan paged_plan(int64_t B, int64_t H, int64_t Hkv, int64_t N, bool packed, int64_t D, int64_t max_keys) {
+inline PagedPlan paged_plan(int64_t B, int64_t H, int64_t Hkv, int64_t N, bool packed, int64_t D, int64_t max_keys,
+                             int row_most) {
   PagedPlan p{};
   const int64_t G = H / Hkv;
-  p.rows = packed || N * G <= kRows;
-  p.tiles = N * G > kRows;
+  p.rows = packed || N * G <= row_most;
+  p.tiles = N * G > row_most;
   if (p.tiles) {
     p.q_tiles = packed ? 1 : static_cast<int>(cdiv(N * G, kTileRows));
-    // Tiles of all windows and key heads: exactly, or packed at most (a window of them has more than kRows rows).
-    const int64_t windows = N * G / (kRows + 1) < B ? N * G / (kRows + 1) : B;
+    // Tiles of all windows and key heads: exactly, or packed at most (a window of them has more than row_most rows).
+    const int64_t windows = N * G / (row_most + 1) < B ? N * G / (row_most + 1) : B;
     const int64_t units = (packed ? N * G / kTileRows + windows : B * p.q_tiles) * Hkv;
-    p.split = packed || (units < kTileTarget && max_keys > kTileLeast * kKB);
+    // Even windows that fill the chip are cut, where one is far longer than the others, if they have one wave's rows
+    // (64 windows x 8 key heads of 128, 16 heads each, 1024 keys and one of 60 000: 162 us); with more the plan and
+    // the join would cost calls of even lengths a quarter (64 windows x 8 heads, 64 queries, 512 keys: 18.4 us, 23.9
+    // planned).
+    p.split = packed || ((units < kTileTarget || N * G <= kRows) && max_keys > kTileLeast * kKB);
     if (!p.split) {
       p.tile_grid = cdiv(B * Hkv, kXcds) * kXcds * p.q_tiles;
       p.tile_slots = p.tile_grid;
     } else {
-      p.tile_slots = kTileTarget;  // parts only where there are fewer tiles than that
-      p.tile_grid = cdiv(units > p.tile_slots ? units : p.tile_slots, kXcds) * kXcds;
+      p.tile_slots = kTileTarget;
+      p.tile_grid = cdiv(units < kTileTarget ? kTileTarget : units + kTileTarget, kXcds) * kXcds;
       p.tile_floats = p.tile_slots * kTileRows * (D + 2);
     }
   }
@@ -224,7 +234,7 @@ inline PagedPlan paged_plan(int64_t B, int64_t H, int64_t Hkv, int64_t N, bool p
     const int64_t more = B * Hkv > 1 << 22 ? 0 : B * Hkv * (cdiv(max_keys, kRowLeast) - 1);
     p.row_parts = more > 0;
     p.row_slots = (more < 0 ? 0 : (more < kRowTarget ? more : kRowTarget)) + B * Hkv;
-    p.slot_rows = packed ? (N * G < kRows ? N * G : kRows) : N * G;
+    p.slot_rows = packed ? (N * G < row_most ? N * G : row_most) : N * G;
     if (p.row_parts) p.row_floats = (p.row_slots * p.slot_rows * (D + 2) + 3) / 4 * 4;
   }
   p.plan_windows = p.row_parts || p.split ? B : 0;
@@ -242,7 +252,9 @@ extern "C" size_t svhip_paged_attention_workspace_bytes(int64_t B, int64_t H, in
       N * H >= 1ll << 40 || D < 1 || D > kMaxPagedDim || max_keys < 0 || max_keys > 1ll << 30) {
     return 0;
   }
-  return paged_plan(B, H, Hkv, N, packed != 0, D, max_keys).bytes();
+  const size_t bf16 = paged_plan(B, H, Hkv, N, packed != 0, D, max_keys, kRowMost).bytes();
+  const size_t fp8 = paged_plan(B, H, Hkv, N, packed != 0, D, max_keys, kRowMostFp8).bytes();
+  return bf16 > fp8 ? bf16 : fp8;
 }
 
 extern "C" int svhip_paged_attention(const svhip_paged_cache* cache, const svhip_paged_attention_args* args,
@@ -265,14 +277,15 @@ extern "C" int svhip_paged_attention(const svhip_paged_cache* cache, const svhip
   SVHIP_REQUIRE(rows16(c.q, c.sq_b, c.sq_h, c.sq_n), "%s: query rows must start on 16-byte boundaries", name);
   SVHIP_REQUIRE(reinterpret_cast<uintptr_t>(c.out) % 8 == 0 && (c.so_b | c.so_h | c.so_n) % 4 == 0,
                 "%s: rows of out must start on 8-byte boundaries", name);
-  const PagedPlan p = paged_plan(B, H, Hkv, N, c.cu_queries != nullptr, D, pc.max_pages * pc.page_size);
+  const bool fp8 = pc.kv_dtype == SVHIP_FP8_E4M3;
+  const int row_most = fp8 ? kRowMostFp8 : kRowMost;
+  const PagedPlan p = paged_plan(B, H, Hkv, N, c.cu_queries != nullptr, D, pc.max_pages * pc.page_size, row_most);
   SVHIP_REQUIRE(p.bytes() == 0 || (c.workspace && c.workspace_bytes >= static_cast<int64_t>(p.bytes()) &&
                                    reinterpret_cast<uintptr_t>(c.workspace) % 16 == 0),
                 "%s: workspace too small or misaligned (%lld < %zu bytes)", name, (long long)c.workspace_bytes, p.bytes());
   const int64_t rows = (c.cu_queries ? N : B * N) * H, join = cdiv(rows, kPagedThreads / 32);
   SVHIP_REQUIRE(p.row_slots + p.tile_grid < (1ll << 31) && rows < (1ll << 31) - kPagedThreads &&
                     N * (H / Hkv) < (1ll << 31) - kPagedThreads, "%s: sizes too large", name);
-  const bool fp8 = pc.kv_dtype == SVHIP_FP8_E4M3;
   const int64_t es = fp8 ? 1 : 2;
   float* const part = static_cast<float*>(c.workspace);
   int4* const plan = reinterpret_cast<int4*>(part + p.row_floats + p.tile_floats);
@@ -283,7 +296,7 @@ extern "C" int svhip_paged_attention(const svhip_paged_cache* cache, const svhip
                     static_cast<uint32_t>(pc.sk_p * es), static_cast<uint32_t>(pc.sk_r * es),
                     static_cast<uint32_t>(pc.sv_p * es), static_cast<uint32_t>(pc.sv_r * es),
                     static_cast<uint32_t>(pc.sek_p), static_cast<uint32_t>(pc.sev_p), c.causal != 0, scale * kLog2e,
-                    p.q_tiles, p.split, static_cast<int>(p.row_slots), static_cast<int>(p.tile_slots),
+                    row_most, p.q_tiles, p.split, static_cast<int>(p.row_slots), static_cast<int>(p.tile_slots),
                     static_cast<int>(p.slot_rows), p.row_parts ? part : nullptr, part + p.row_floats,
                     p.plan_windows ? plan : nullptr, p.planned ? reinterpret_cast<int2*>(plan + B + 1) : nullptr};
   hipStream_t s = as_stream(stream);

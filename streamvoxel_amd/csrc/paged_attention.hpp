@@ -8,6 +8,12 @@ namespace svhip {
 
 constexpr int kPagedThreads = 256;
 constexpr int kRows = 32;          // rows of a wave
+// Rows of a window up to which it is of the row form, bf16 and e4m3. At 4, 8, 16, 32 rows a key head the row form
+// takes 47, 57, 59, 85 us and tiles 42, 46, 41, 46 (64 windows of 512 to 1024 keys, 8 key heads of 128); 16 windows
+// of 2048 to 4096 keys: 42, 50, 59, 82 and 38, 41, 44, 48; e4m3, 64 windows of 2048 to 4096 keys of 64: 51, 57, 56,
+// 71 and 72, 73, 73, 76. With one of 64 windows 60 times as long as the others, 4 rows: 113 and 160; 200 windows of
+// 1024 keys: 161 and 183.
+constexpr int kRowMost = 4, kRowMostFp8 = 16;
 constexpr int kTileRows = 128;     // rows of a tile workgroup
 // Tile workgroups below which keys are split, two for every CU (one, four: a causal chunk of 4 x 512 tokens, head_dim
 // 128, 313 and 278 us for 281; the same with all keys seen 198 and 180 for 167; 1024 queries over 9744 keys 82 and 61
@@ -37,12 +43,13 @@ struct PagedArgs {
   bool causal;
   float scale_log2;
   // The plan.
+  int row_most;         // rows of a window up to which it is of the row form
   int q_tiles;          // tiles of a window (even windows)
   bool split;           // tiles: whether parts of keys may be dealt out
   int row_slots, tile_slots;  // slots of parts at most
   int slot_rows;        // rows of a row-form slot
   float *row_part, *tile_part;  // row_part null: the row form's windows are not cut
-  int4* plan;           // (null: no parts) a window's first place, its parts, a part's length (tiles: blocks) and its tiles
+  int4* plan;           // (null: no parts) a window's first slot, its parts, a part's length (tiles: blocks) and its tiles
   int2* running;        // (null: every workgroup plans for itself) places of row form and of tiles up to and with a window;
                         // plan[B] then has their sums and the part lengths
 };
@@ -72,7 +79,7 @@ __device__ __forceinline__ int last_key(const PagedArgs& a, const Window& w, int
   return static_cast<int>(j < w.keys - 1 ? (j < -1 ? -1 : j) : w.keys - 1);
 }
 
-__device__ __forceinline__ bool row_form(const PagedArgs& a, int64_t count) { return count * a.G <= kRows; }
+__device__ __forceinline__ bool row_form(const PagedArgs& a, int64_t count) { return count * a.G <= a.row_most; }
 
 // Keys that the rows of tile qt see, the last of them the most.
 __device__ __forceinline__ int tile_keys(const PagedArgs& a, const Window& w, int qt) {
@@ -113,16 +120,17 @@ __device__ __forceinline__ int wave_prefix(int v, int& total) {
   return incl - v;
 }
 
-// What a workgroup takes: part `part` of `parts` of key head kvh of window b (tiles: of tile qt), at place `at` of
-// all, the window's first being `before`. b < 0: nothing.
+// What a workgroup takes: part `part` of `parts` of key head kvh of window b (tiles: of tile qt). The windows that
+// are cut have slots for their parts, one after the other: this one's is `slot`, its window's first `first`. b < 0:
+// nothing.
 struct PagedItem {
-  int b, kvh, part, parts, qt, tiles, at, before;
+  int b, kvh, part, parts, qt, tiles, slot, first;
 };
 
-// Place `in` of window b's list: for every key head its parts, for every part its tiles.
-__device__ __forceinline__ PagedItem item_of(int b, int at, int in, int parts, int tiles) {
+// Place `in` of window b's list: for every key head its parts, for every part its tiles; slots from `first` on.
+__device__ __forceinline__ PagedItem item_of(int b, int first, int in, int parts, int tiles) {
   const int u = in / tiles, kvh = u / parts;
-  return PagedItem{b, kvh, u - kvh * parts, parts, in - u * tiles, tiles, at, at - in};
+  return PagedItem{b, kvh, u - kvh * parts, parts, in - u * tiles, tiles, first + in, first};
 }
 
 // The item at place `at` of the lists of up to 64 windows, one after the other; the lane's window has `tiles` and
@@ -130,10 +138,12 @@ __device__ __forceinline__ PagedItem item_of(int b, int at, int in, int parts, i
 __device__ __forceinline__ PagedItem item_at(int Hkv, int at, int tiles, int parts) {
   int total;
   const int n = tiles * Hkv * parts, before = wave_prefix(n, total);
-  if (at >= total) return PagedItem{-1, 0, 0, 1, 0, 1, at, 0};
+  if (at >= total) return PagedItem{-1, 0, 0, 1, 0, 1, 0, 0};
+  int slots;
+  const int first = wave_prefix(parts > 1 ? n : 0, slots);
   const int c = __builtin_ctzll(__builtin_amdgcn_ballot_w64(before <= at && at < before + n));
-  return item_of(c, at, at - __builtin_amdgcn_readlane(before, c), __builtin_amdgcn_readlane(parts, c),
-                 __builtin_amdgcn_readlane(tiles, c));
+  return item_of(c, __builtin_amdgcn_readlane(first, c), at - __builtin_amdgcn_readlane(before, c),
+                 __builtin_amdgcn_readlane(parts, c), __builtin_amdgcn_readlane(tiles, c));
 }
 
 // The same from paged_plan_kernel's lists; `ends` the running sums of the form, two numbers apart. 64 windows a step.
@@ -143,13 +153,13 @@ __device__ __forceinline__ PagedItem planned_item(const PagedArgs& a, int at, co
   do {
     const int step = (hi - lo + 63) / 64, end = lo + (lane + 1) * step, last = end < hi ? end : hi;
     const uint64_t past = __builtin_amdgcn_ballot_w64(ends[2 * (last - 1)] > at);
-    if (past == 0ull) return PagedItem{-1, 0, 0, 1, 0, 1, at, 0};
+    if (past == 0ull) return PagedItem{-1, 0, 0, 1, 0, 1, 0, 0};
     c = __builtin_ctzll(past);
     lo += c * step;
     hi = hi - lo > step ? lo + step : hi;
   } while (hi - lo > 1);
   const int4 plan = a.plan[lo];
-  return item_of(lo, at, at - plan.x, plan.y, plan.w);
+  return item_of(lo, plan.x, at - (lo > 0 ? ends[2 * (lo - 1)] : 0), plan.y, plan.w);
 }
 
 // Who plans: a wave, for up to 64 windows (one a lane), or a workgroup.

@@ -1,4 +1,5 @@
-// The row form of svhip_paged_attention (paged_attention.hip): windows of up to kRows rows, single tokens among them.
+// The row form of svhip_paged_attention (paged_attention.hip): windows of up to row_most rows, single tokens among
+// them.
 #pragma once
 
 #include <type_traits>
@@ -50,7 +51,7 @@ __device__ __forceinline__ PagedItem row_item(const PagedArgs& a, int place, int
   const int Hkv = a.Hkv;
   if (!a.row_part) {
     const int b = place / Hkv;
-    return PagedItem{b < a.tokens.B ? b : -1, place - b * Hkv, 0, 1, 0, 1, place, 0};
+    return PagedItem{b < a.tokens.B ? b : -1, place - b * Hkv, 0, 1, 0, 1, 0, 0};
   }
   if (a.running) {
     const int4 sums = a.plan[a.tokens.B];
@@ -95,7 +96,7 @@ __device__ __forceinline__ void row_work(const PagedArgs& a, int place, char* sV
   const int kvh = __builtin_amdgcn_readfirstlane(item.kvh), part = __builtin_amdgcn_readfirstlane(item.part);
   const int parts = __builtin_amdgcn_readfirstlane(item.parts);
   if (a.row_part && !a.running && part == 0 && kvh == 0 && threadIdx.x == 0) {
-    a.plan[b] = make_int4(item.before, parts, each, 1);
+    a.plan[b] = make_int4(item.first, parts, each, 1);
   }
   const Window w = window_at(a, b);
   if (w.count <= 0 || !row_form(a, w.count)) return;  // (uncut windows stand by their numbers)
@@ -280,7 +281,7 @@ __device__ __forceinline__ void row_work(const PagedArgs& a, int place, char* sV
       o1 = __builtin_fmaf(from[(d + 1) * kRows + rr], f, o1);
     }
     if (parts > 1) {
-      float* slot = a.row_part + (static_cast<int64_t>(item.at) * a.slot_rows + rr) * (D + 2);
+      float* slot = a.row_part + (static_cast<int64_t>(item.slot) * a.slot_rows + rr) * (D + 2);
       *reinterpret_cast<float2*>(slot + d) = make_float2(o0, o1);
       if (d == 0) *reinterpret_cast<float2*>(slot + D) = make_float2(m, total);
     } else {

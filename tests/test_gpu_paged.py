@@ -696,7 +696,7 @@ def test_engine_over_a_shared_pool(kv_dtype):
 
 @pytest.mark.parametrize('kv_dtype', ['bf16', 'fp8'])
 @pytest.mark.parametrize('D, heads, page', [(64, 1, 64), (128, 2, 16)])
-@pytest.mark.parametrize('n, at, packed', [(3, 1, False), (16, 9, False), (40, 17, False), (200, 70, False), (200, 199, True),
+@pytest.mark.parametrize('n, at, packed', [(2, 1, False), (3, 1, False), (16, 9, False), (40, 17, False), (200, 70, False), (200, 199, True),
                                            (32, 1, True)])
 def test_what_a_token_does_not_see_does_not_reach_it(n, at, packed, D, heads, page, kv_dtype):
     """A key and a value of the chunk's token `at` that are not finite: the tokens in front of it are as if it were not there,
