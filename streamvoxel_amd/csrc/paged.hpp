@@ -20,7 +20,7 @@ struct Pages {
   int32_t* bad;           // set to 1 where a page lies outside the pool or a window outside its row of the table; or null
 };
 
-__device__ __forceinline__ void set_bad(const Pages& p) {
+__host__ __device__ __forceinline__ void set_bad(const Pages& p) {
   if (p.bad) *p.bad = 1;
 }
 
@@ -33,7 +33,7 @@ __device__ __forceinline__ int64_t page_of(const Pages& p, int64_t b, int64_t j)
 }
 
 // Keys of window b: its length, cut to what its row of the table can name.
-__device__ __forceinline__ int64_t held_keys(const Pages& p, int64_t b) {
+__host__ __device__ __forceinline__ int64_t held_keys(const Pages& p, int64_t b) {
   const int64_t L = p.lengths[b], most = p.max_pages << p.shift;
   if (L > most) set_bad(p);
   return L < 0 ? 0 : (L > most ? most : L);
@@ -46,13 +46,13 @@ struct Tokens {
 };
 
 // Border i of the packed windows, inside [0, T].
-__device__ __forceinline__ int64_t border(const Tokens& t, int64_t i) {
+__host__ __device__ __forceinline__ int64_t border(const Tokens& t, int64_t i) {
   const int64_t c = t.cu[i];
   return c < 0 ? 0 : (c > t.N ? t.N : c);
 }
 
 // First token and count of window b.
-__device__ __forceinline__ void window_tokens(const Tokens& t, int64_t b, int64_t& first, int64_t& count) {
+__host__ __device__ __forceinline__ void window_tokens(const Tokens& t, int64_t b, int64_t& first, int64_t& count) {
   if (!t.cu) {
     first = b * t.N;
     count = t.N;

@@ -203,45 +203,6 @@ __global__ __launch_bounds__(kPagedThreads) void paged_join_kernel(PagedArgs a) 
 // 217.6 and 222.9; 32 768 rows in two parts: 323 with, 281 without; 16 304 rows 116 and 104).
 constexpr int64_t kJoinFew = 4096;
 
-inline PagedPlan paged_plan(int64_t B, int64_t H, int64_t Hkv, int64_t N, bool packed, int64_t D, int64_t max_keys,
-                             int row_most) {
-  PagedPlan p{};
-  const int64_t G = H / Hkv;
-  p.rows = packed || N * G <= row_most;
-  p.tiles = N * G > row_most;
-  if (p.tiles) {
-    p.q_tiles = packed ? 1 : static_cast<int>(cdiv(N * G, kTileRows));
-    // Tiles of all windows and key heads: exactly, or packed at most (a window of them has more than row_most rows).
-    const int64_t windows = N * G / (row_most + 1) < B ? N * G / (row_most + 1) : B;
-    const int64_t units = (packed ? N * G / kTileRows + windows : B * p.q_tiles) * Hkv;
-    // Even windows that fill the chip are cut, where one is far longer than the others, if they have one wave's rows
-    // (64 windows x 8 key heads of 128, 16 heads each, 1024 keys and one of 60 000: 162 us); with more the plan and
-    // the join would cost calls of even lengths a quarter (64 windows x 8 heads, 64 queries, 512 keys: 18.4 us, 23.9
-    // planned).
-    p.split = packed || ((units < kTileTarget || N * G <= kRows) && max_keys > kTileLeast * kKB);
-    if (!p.split) {
-      p.tile_grid = cdiv(B * Hkv, kXcds) * kXcds * p.q_tiles;
-      p.tile_slots = p.tile_grid;
-    } else {
-      p.tile_slots = kTileTarget;
-      p.tile_grid = cdiv(units < kTileTarget ? kTileTarget : units + kTileTarget, kXcds) * kXcds;
-      p.tile_floats = p.tile_slots * kTileRows * (D + 2);
-    }
-  }
-  if (p.rows) {
-    // One for each (window, key head), and the parts: at most kRowTarget more, and no shorter than kRowLeast.
-    // (From 2^22 pairs on there is no need, and the plan's sums stay exact.)
-    const int64_t more = B * Hkv > 1 << 22 ? 0 : B * Hkv * (cdiv(max_keys, kRowLeast) - 1);
-    p.row_parts = more > 0;
-    p.row_slots = (more < 0 ? 0 : (more < kRowTarget ? more : kRowTarget)) + B * Hkv;
-    p.slot_rows = packed ? (N * G < row_most ? N * G : row_most) : N * G;
-    if (p.row_parts) p.row_floats = (p.row_slots * p.slot_rows * (D + 2) + 3) / 4 * 4;
-  }
-  p.plan_windows = p.row_parts || p.split ? B : 0;
-  p.planned = p.plan_windows > 64;
-  return p;
-}
-
 }  // namespace svhip
 
 using namespace svhip;

@@ -79,7 +79,7 @@ __device__ __forceinline__ int last_key(const PagedArgs& a, const Window& w, int
   return static_cast<int>(j < w.keys - 1 ? (j < -1 ? -1 : j) : w.keys - 1);
 }
 
-__device__ __forceinline__ bool row_form(const PagedArgs& a, int64_t count) { return count * a.G <= a.row_most; }
+__host__ __device__ __forceinline__ bool row_form(const PagedArgs& a, int64_t count) { return count * a.G <= a.row_most; }
 
 // Keys that the rows of tile qt see, the last of them the most.
 __device__ __forceinline__ int tile_keys(const PagedArgs& a, const Window& w, int qt) {
@@ -189,7 +189,7 @@ struct BlockTeam {
 // `target`: they then run side by side, and none longer than it must. places(c, length): parts of window c, all key
 // heads and tiles.
 template <typename Team, typename Places>
-__device__ __forceinline__ int part_length(const PagedArgs& a, const Team& team, float work, int target, int grain,
+__host__ __device__ __forceinline__ int part_length(const PagedArgs& a, const Team& team, float work, int target, int grain,
                                            int least, Places places) {
   // An equal share is too short, or all but; twice as long again and again until it fits, then halves between.
   const float share = work / static_cast<float>(target) / static_cast<float>(grain);
@@ -562,6 +562,49 @@ struct PagedPlan {
            static_cast<size_t>(planned ? plan_windows * 24 + 16 : plan_windows * 16);
   }
 };
+
+inline PagedPlan paged_plan(int64_t B, int64_t H, int64_t Hkv, int64_t N, bool packed, int64_t D, int64_t max_keys,
+                             int row_most) {
+  PagedPlan p{};
+  const int64_t G = H / Hkv;
+  p.rows = packed || N * G <= row_most;
+  p.tiles = N * G > row_most;
+  if (p.tiles) {
+    p.q_tiles = packed ? 1 : static_cast<int>(cdiv(N * G, kTileRows));
+    // Tiles of all windows and key heads: exactly, or packed at most (a window of them has more than row_most rows).
+    const int64_t windows = N * G / (row_most + 1) < B ? N * G / (row_most + 1) : B;
+    const int64_t units = (packed ? N * G / kTileRows + windows : B * p.q_tiles) * Hkv;
+    // Even windows that fill the chip are cut, where one is far longer than the others, if they have one wave's rows
+    // (64 windows x 8 key heads of 128, 16 heads each, 1024 keys and one of 60 000: 162 us); with more the plan and
+    // the join would cost calls of even lengths a quarter (64 windows x 8 heads, 64 queries, 512 keys: 18.4 us, 23.9
+    // planned).
+    p.split = packed || ((units < kTileTarget || N * G <= kRows) && max_keys > kTileLeast * kKB);
+    if (!p.split) {
+      p.tile_grid = cdiv(B * Hkv, kXcds) * kXcds * p.q_tiles;
+      p.tile_slots = p.tile_grid;
+    } else {
+      p.tile_slots = kTileTarget;
+      // A share of parts, or tiles that are as many and a share of parts of the long windows among them: of kTileTarget,
+      // and packed, where there may be windows of the row form, also of kTileBeside (tile_length).
+      int64_t places = units < kTileTarget ? kTileTarget : units + kTileTarget;
+      if (packed && units >= kTileBeside && places < units + kTileBeside) places = units + kTileBeside;
+      p.tile_grid = cdiv(places, kXcds) * kXcds;
+      p.tile_floats = p.tile_slots * kTileRows * (D + 2);
+    }
+  }
+  if (p.rows) {
+    // One for each (window, key head), and the parts: at most kRowTarget more, and no shorter than kRowLeast.
+    // (From 2^22 pairs on there is no need, and the plan's sums stay exact.)
+    const int64_t more = B * Hkv > 1 << 22 ? 0 : B * Hkv * (cdiv(max_keys, kRowLeast) - 1);
+    p.row_parts = more > 0;
+    p.row_slots = (more < 0 ? 0 : (more < kRowTarget ? more : kRowTarget)) + B * Hkv;
+    p.slot_rows = packed ? (N * G < row_most ? N * G : row_most) : N * G;
+    if (p.row_parts) p.row_floats = (p.row_slots * p.slot_rows * (D + 2) + 3) / 4 * 4;
+  }
+  p.plan_windows = p.row_parts || p.split ? B : 0;
+  p.planned = p.plan_windows > 64;
+  return p;
+}
 
 // KS: steps of 16 head_dim elements; whole: pages of kWholePages keys or more.
 void launch_paged_rows(const PagedArgs& a, const PagedPlan& p, bool fp8, hipStream_t s);

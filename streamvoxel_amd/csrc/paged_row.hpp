@@ -11,13 +11,13 @@ namespace svhip {
 [[maybe_unused]] constexpr int kRowKeys = 32;  // keys of a half of a wave's block
 
 // Keys of window c, or -1: not of this form.
-__device__ __forceinline__ int row_keys(const PagedArgs& a, int64_t c) {
+__host__ __device__ __forceinline__ int row_keys(const PagedArgs& a, int64_t c) {
   int64_t first, count;
   window_tokens(a.tokens, c, first, count);
   const int held = static_cast<int>(held_keys(a.pages, c));  // (read beside the borders, not after them)
   return count > 0 && row_form(a, count) ? held : -1;
 }
-__device__ __forceinline__ int row_parts(int keys, int length) {
+__host__ __device__ __forceinline__ int row_parts(int keys, int length) {
   return keys < 0 ? 0 : (keys > length ? (keys - 1) / length + 1 : 1);
 }
 
@@ -25,7 +25,7 @@ __device__ __forceinline__ int row_parts(int keys, int length) {
 // kRowTarget more than the (window, key head) pairs; kUncut if there are no places from `place` on. `mine`: keys of
 // the team's own window.
 template <typename Team>
-__device__ __forceinline__ int row_length(const PagedArgs& a, const Team& team, int place, int& mine) {
+__host__ __device__ __forceinline__ int row_length(const PagedArgs& a, const Team& team, int place, int& mine) {
   float keys = 0.f, units = 0.f;
   mine = -1;
   for (int64_t c = team.id(); c < a.tokens.B; c += Team::kSize) {

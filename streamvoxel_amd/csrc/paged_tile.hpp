@@ -6,7 +6,7 @@
 namespace svhip {
 
 // A window's tiles (0: the row form) and key blocks (0: no tokens).
-__device__ __forceinline__ void tiles_of_window(const PagedArgs& a, int64_t c, int& tiles, int& blocks) {
+__host__ __device__ __forceinline__ void tiles_of_window(const PagedArgs& a, int64_t c, int& tiles, int& blocks) {
   int64_t first, count;
   window_tokens(a.tokens, c, first, count);
   tiles = row_form(a, count) ? 0 : static_cast<int>(cdiv(count * a.G, kTileRows));
@@ -14,7 +14,7 @@ __device__ __forceinline__ void tiles_of_window(const PagedArgs& a, int64_t c, i
   blocks = count > 0 ? held : 0;
 }
 
-__device__ __forceinline__ int tile_parts(int blocks, int length) {
+__host__ __device__ __forceinline__ int tile_parts(int blocks, int length) {
   return blocks > length ? (blocks - 1) / length + 1 : 1;
 }
 
@@ -54,7 +54,7 @@ __device__ __forceinline__ PagedItem whole_item(const PagedArgs& a, int place) {
 // other half of every CU: a block takes about 1 us of either's CU; 24 mixed windows 101 us for 110). kUncut: no
 // parts. `tiles`, `blocks`: of the team's own window; `total`: the tiles.
 template <typename Team>
-__device__ __forceinline__ int tile_length(const PagedArgs& a, const Team& team, int& tiles, int& blocks, float& total) {
+__host__ __device__ __forceinline__ int tile_length(const PagedArgs& a, const Team& team, int& tiles, int& blocks, float& total) {
   const float Hkv = static_cast<float>(a.Hkv);
   float units = 0.f, work = 0.f, beside = 0.f;
   tiles = blocks = 0;
@@ -81,7 +81,7 @@ __device__ __forceinline__ int tile_length(const PagedArgs& a, const Team& team,
 }
 
 // An XCD takes a run of consecutive places of parts, so that the tiles of a part meet in its L2.
-__device__ __forceinline__ int shared_place(int place, int total, int each) {
+__host__ __device__ __forceinline__ int shared_place(int place, int total, int each) {
   if (each == kUncut) return place < total ? place : -1;
   const int run = (total + kXcds - 1) / kXcds, at = (place & 7) * run + (place >> 3);
   return (place >> 3) < run && at < total ? at : -1;

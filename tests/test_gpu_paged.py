@@ -860,3 +860,26 @@ def test_a_captured_call_follows_lengths_and_borders(B):
         torch.cuda.synchronize()
         check(out, q, pool, True, borders)
         assert torch.equal(out, call())
+
+
+@pytest.mark.parametrize('kv_dtype, n', [('bf16', 5), ('fp8', 17)])
+@pytest.mark.parametrize('times', [1, 2])
+def test_a_long_window_among_tiles_beside_single_tokens(times, kv_dtype, n):
+    """Packed windows of both forms, the tiles as many as half of the chip and one window of them cut (test_paged_plan.py: more
+    places than a full share): every row is written, by its window's keys."""
+    from streamvoxel_amd.stream.paged import paged_attention
+    _case(f'a long window beside single tokens: {times} x 60 windows {kv_dtype}')
+    heads = 8 // times
+    counts = [n] * 52 * times + [1] * 8 * times
+    lengths = [64000] + [384] * (52 * times - 1) + [8192] * 8 * times
+    pool = Pool(lengths, heads, 16, 64, times, kv_dtype)
+    cu = [0]
+    for c in counts:
+        cu.append(cu[-1] + c)
+    q = torch.randn(heads, cu[-1], 16, generator=torch.Generator().manual_seed(times)).to(torch.bfloat16).to(DEV)
+    out = torch.full_like(q, math.nan)
+    for causal in (True, False):
+        out.fill_(math.nan)
+        paged_attention(q, *pool.args(), cu_queries=torch.tensor(cu, dtype=torch.int32, device=DEV), causal=causal, out=out,
+                        **pool.exponents())
+        check(out, q, pool, causal, cu)
