@@ -203,9 +203,10 @@ class PagedContext:
     `max_pages` of them (default: all). kv_dtype 'bf16' or 'fp8' (OCP e4m3fn with one power of two for each row and
     head).
 
-    The host keeps the books: `resize` and `grow` take and free pages and send table and lengths to the device on the
-    current stream without waiting for it; calls that touch a window's pages must be ordered after them, as usual. A
-    replayed graph reads the table and the lengths as they stand. `bad` (device int32 [1]) becomes non-zero when a
+    The host keeps the books: `resize` and `grow` take and free pages and send the window's table and length to the
+    device on the current stream without waiting for it; calls that touch a window's pages must be ordered after them,
+    as usual (other windows may be in work on other streams). A replayed graph reads the table and the lengths as they
+    stand. `bad` (device int32 [1]) becomes non-zero when a
     call meets a page outside the pool, which these books never name."""
 
     def __init__(self, layers, batch, heads, head_dim, pages, device, page_size=64, max_pages=None, kv_dtype='bf16'):
@@ -264,10 +265,29 @@ class PagedContext:
         for index, length in wanted.items():
             own, n = self._owned[index], self._pages_for(length)
             own.extend(self._free.pop() for _ in range(n - len(own)))
-            self.host_lengths[index] = length
         for index in moved:
             self._send(self.table[index, :len(self._owned[index])], self._owned[index])
-        self._send(self.lengths, self.host_lengths)
+        changed = sorted(index for index, length in wanted.items() if length != self.host_lengths[index])
+        for index in changed:
+            self.host_lengths[index] = wanted[index]
+        self._send_lengths(changed)
+
+    def _send_lengths(self, windows):
+        """The lengths of these windows (ascending) alone: a call for another window may be on its way on another
+        stream."""
+        runs = []
+        for index in windows:
+            if runs and runs[-1][1] == index:
+                runs[-1][1] = index + 1
+            else:
+                runs.append([index, index + 1])
+        if len(runs) > 2:          # in one copy
+            both = torch.empty(2, len(windows), dtype=torch.int32, device=self.lengths.device)
+            self._send(both.view(-1), windows + [self.host_lengths[index] for index in windows])
+            self.lengths.index_copy_(0, both[0].long(), both[1])
+            return
+        for first, end in runs:
+            self._send(self.lengths[first:end], self.host_lengths[first:end])
 
     @staticmethod
     def _send(to, values):

@@ -883,3 +883,34 @@ def test_a_long_window_among_tiles_beside_single_tokens(times, kv_dtype, n):
         paged_attention(q, *pool.args(), cu_queries=torch.tensor(cu, dtype=torch.int32, device=DEV), causal=causal, out=out,
                         **pool.exponents())
         check(out, q, pool, causal, cu)
+
+
+def test_windows_of_one_context_on_two_streams():
+    """A window that is written on a side stream, behind other work there, while the others grow on the current one: every
+    length and every key is the last call's for its window."""
+    from streamvoxel_amd.stream.paged import PagedContext
+    ctx = PagedContext(1, 6, 2, 64, 60, DEV, page_size=16)
+    g = torch.Generator().manual_seed(5)
+    rows = lambda n: torch.randn(2, n, 64, generator=g).to(torch.bfloat16).to(DEV)
+    held = [[torch.empty(2, 0, 64, dtype=torch.bfloat16, device=DEV)] for _ in range(6)]
+    side, busy = torch.cuda.Stream(), torch.randn(4096, 4096, device=DEV)
+    for step, counts in enumerate([(0, 3, 20, 1, 1, 1), (0, 1, 0, 17, 0, 2), (0, 16, 16, 16, 16, 16)]):
+        loaded, new = rows(40 + 30 * step), [rows(n) for n in counts]
+        torch.cuda.synchronize()
+        with torch.cuda.stream(side):
+            for _ in range(20):
+                busy @ busy
+            ctx.resize(0, loaded.shape[1])
+            ctx.append(0, loaded, loaded, index=0)
+        ctx.grow(counts)
+        for b in range(1, 6):
+            ctx.append(0, new[b], new[b], index=b)
+            held[b].append(new[b])
+        held[0] = [loaded]
+        torch.cuda.synchronize()
+        assert ctx.lengths.tolist() == ctx.host_lengths == [sum(t.shape[1] for t in h) for h in held]
+        for b in range(6):
+            at = torch.arange(ctx.host_lengths[b], device=DEV)
+            page = ctx.table[b].long()[at // 16]
+            assert torch.equal(ctx.k[0][page, :, at % 16].transpose(0, 1), torch.cat(held[b], 1)), (step, b)
+    assert int(ctx.bad) == 0

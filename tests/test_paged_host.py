@@ -216,3 +216,43 @@ def test_sizes_that_would_not_fit_the_kernels_counts(lib):
     need = lib.svhip_paged_attention_workspace_bytes
     assert need(2, 4, 2, 3, 0, 64, (1 << 30) + 1) == need(1 << 31, 4, 2, 3, 0, 64, 1280) == 0
     assert need(2, 1 << 20, 2, 1 << 21, 0, 64, 1280) == 0
+
+
+class Streams:
+    """Stands in for the device of a PagedContext on the CPU: what is sent on stream `late` happens at `catch_up` alone, what
+    is sent on stream `now` at once."""
+
+    def __init__(self, monkeypatch):
+        from streamvoxel_amd.stream.paged import PagedContext
+        self.current, self.queue = 'now', []
+        monkeypatch.setattr(PagedContext, '_send', staticmethod(self.send))
+
+    def send(self, to, values):
+        values = torch.tensor(values, dtype=torch.int32)
+        if self.current == 'late':
+            self.queue.append(lambda: to.copy_(values))
+        else:
+            to.copy_(values)
+
+    def catch_up(self):
+        for work in self.queue:
+            work()
+        self.queue.clear()
+
+
+def test_a_window_in_work_on_another_stream_leaves_the_other_lengths_alone(monkeypatch):
+    from streamvoxel_amd.stream.paged import PagedContext
+    streams = Streams(monkeypatch)
+    ctx = PagedContext(1, 8, 2, 64, 40, 'cpu', page_size=16)
+    ctx.grow(10)
+    for change in (lambda: ctx.resize(1, 20), lambda: ctx.grow((0, 30, 0, 0, 0, 0, 0, 0)), lambda: ctx.release(1)):
+        streams.current = 'late'
+        change()
+        streams.current = 'now'
+        ctx.grow((1, 0, 1, 1, 0, 1, 0, 1))
+        ctx.resize(4, ctx.host_lengths[4] + 3)
+        ctx.release(6)
+        streams.catch_up()
+        assert ctx.lengths.tolist() == ctx.host_lengths
+        for b in range(8):
+            assert ctx.table[b, :len(ctx._owned[b])].tolist() == ctx._owned[b]
