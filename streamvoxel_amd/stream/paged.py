@@ -205,8 +205,8 @@ class PagedContext:
 
     The host keeps the books: `resize` and `grow` take and free pages and send the window's table and length to the
     device on the current stream without waiting for it; calls that touch a window's pages must be ordered after them,
-    as usual (other windows may be in work on other streams). A replayed graph reads the table and the lengths as they
-    stand. `bad` (device int32 [1]) becomes non-zero when a
+    as usual. Other windows may be in work on other streams: a page that changes hands is waited for. A replayed graph
+    reads the table and the lengths as they stand. `bad` (device int32 [1]) becomes non-zero when a
     call meets a page outside the pool, which these books never name."""
 
     def __init__(self, layers, batch, heads, head_dim, pages, device, page_size=64, max_pages=None, kv_dtype='bf16'):
@@ -233,10 +233,14 @@ class PagedContext:
         self.host_lengths = [0] * batch
         self._owned = [[] for _ in range(batch)]
         self._free = list(range(pages - 1, -1, -1))
+        self._left = {}        # free page -> (stream that it was given back on, event there)
 
     @property
     def free_pages(self):
         return len(self._free)
+
+    def _stream(self):
+        return torch.cuda.current_stream(self.lengths.device) if self.lengths.is_cuda else None
 
     def _pages_for(self, length):
         return -(-length // self.page_size)
@@ -255,16 +259,26 @@ class PagedContext:
             need += self._pages_for(length) - len(self._owned[index])
         if need > len(self._free):
             raise RuntimeError(f'the pool has {len(self._free)} pages left, {need} more are needed')
-        moved = []
+        stream, freed, moved = self._stream(), [], []
         for index, length in wanted.items():          # freed pages first: another window may take them
             own, n = self._owned[index], self._pages_for(length)
             if n != len(own):
                 moved.append(index)
-            self._free.extend(reversed(own[n:]))
+            freed.extend(reversed(own[n:]))
             del own[n:]
+        self._free.extend(freed)
+        if freed and stream is not None:
+            self._left.update(dict.fromkeys(freed, (stream, stream.record_event())))
+        taken = []
         for index, length in wanted.items():
             own, n = self._owned[index], self._pages_for(length)
-            own.extend(self._free.pop() for _ in range(n - len(own)))
+            new = [self._free.pop() for _ in range(n - len(own))]
+            own.extend(new)
+            taken.extend(new)
+        # A page given back on another stream may still be in work there.
+        for left, event in {self._left.pop(page) for page in taken if page in self._left}:
+            if left != stream:
+                stream.wait_event(event)
         for index in moved:
             self._send(self.table[index, :len(self._owned[index])], self._owned[index])
         changed = sorted(index for index, length in wanted.items() if length != self.host_lengths[index])

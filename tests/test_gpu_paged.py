@@ -914,3 +914,28 @@ def test_windows_of_one_context_on_two_streams():
             page = ctx.table[b].long()[at // 16]
             assert torch.equal(ctx.k[0][page, :, at % 16].transpose(0, 1), torch.cat(held[b], 1)), (step, b)
     assert int(ctx.bad) == 0
+
+
+def test_pages_that_change_hands_between_streams():
+    """A window written on a busy side stream twice, long and then short, while another takes the pages that it gave back: what
+    the first write puts there is overwritten by the other window's keys, not they by it."""
+    from streamvoxel_amd.stream.paged import PagedContext
+    ctx = PagedContext(1, 2, 2, 64, 8, DEV, page_size=16)
+    g = torch.Generator().manual_seed(6)
+    long, short, other = [torch.randn(2, n, 64, generator=g).to(torch.bfloat16).to(DEV) for n in (128, 16, 112)]
+    side, busy = torch.cuda.Stream(), torch.randn(4096, 4096, device=DEV)
+    torch.cuda.synchronize()
+    with torch.cuda.stream(side):
+        ctx.resize(0, 128)
+        for _ in range(20):
+            busy @ busy
+        ctx.append(0, long, long, index=0)
+        ctx.resize(0, 16)
+        ctx.append(0, short, short, index=0)
+    ctx.grow((0, 112))
+    ctx.append(0, other, other, index=1)
+    torch.cuda.synchronize()
+    assert ctx.lengths.tolist() == [16, 112] and int(ctx.bad) == 0
+    for b, want in ((0, short), (1, other)):
+        at = torch.arange(want.shape[1], device=DEV)
+        assert torch.equal(ctx.v[0][ctx.table[b].long()[at // 16], :, at % 16].transpose(0, 1), want)

@@ -256,3 +256,52 @@ def test_a_window_in_work_on_another_stream_leaves_the_other_lengths_alone(monke
         assert ctx.lengths.tolist() == ctx.host_lengths
         for b in range(8):
             assert ctx.table[b, :len(ctx._owned[b])].tolist() == ctx._owned[b]
+
+
+class RecordedStream:
+    """A stream that keeps a list of what is put on it."""
+
+    def __init__(self, name):
+        self.name, self.work = name, []
+
+    def record_event(self):
+        self.work.append('event')
+        return self.name, len(self.work)
+
+    def wait_event(self, event):
+        self.work.append(('wait', event))
+
+
+def test_a_page_that_changes_streams_is_waited_for(monkeypatch):
+    """The stream that takes a page waits for the one that gave it back, before it sends the table; pages that stay on a
+    stream, or were never given back, cost no wait."""
+    from streamvoxel_amd.stream.paged import PagedContext
+    side, main = RecordedStream('side'), RecordedStream('main')
+    current = [side]
+    monkeypatch.setattr(PagedContext, '_stream', lambda self: current[0])
+
+    def send(to, values):
+        if values:
+            current[0].work.append('send')
+            to.copy_(torch.tensor(values, dtype=torch.int32))
+    monkeypatch.setattr(PagedContext, '_send', staticmethod(send))
+    ctx = PagedContext(1, 3, 2, 64, 6, 'cpu', page_size=16)
+    ctx.resize(0, 64)
+    assert side.work == ['send', 'send']
+    side.work.append('keys of window 0')
+    ctx.resize(0, 10)                        # three pages back
+    assert side.work[2:] == ['keys of window 0', 'event', 'send', 'send']
+    current[0] = main
+    ctx.resize(1, 33)
+    assert ctx._owned[1] == [1, 2, 3] and main.work == [('wait', ('side', 4)), 'send', 'send']
+    main.work.clear()
+    ctx.resize(2, 30)                        # never used before
+    assert main.work == ['send', 'send']
+    main.work.clear()
+    ctx.release(1)
+    ctx.resize(2, 60)                        # given back on this stream
+    assert main.work == ['event', 'send', 'send', 'send']
+    current[0] = side
+    side.work.clear()
+    ctx.resize(0, 17)
+    assert side.work == [('wait', ('main', 1)), 'send', 'send'] and not ctx._left
