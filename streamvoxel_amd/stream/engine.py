@@ -107,13 +107,22 @@ def _local_kv(model, context, local):
 
 def extend_condition(model, context, index, local, positions):
     """Further local context of slot `index` behind what a PagedContext holds of it: `local` [1, L, W] projected by every layer,
-    the keys rotated at `positions` [1, L, 3]; nothing that is there is written again."""
-    L = local.shape[1]
-    positions = positions.to(device=context.lengths.device, dtype=torch.float32)[0].contiguous()
-    context.resize(index, context.host_lengths[index] + L)
-    for j, (cross, key, value) in enumerate(_local_kv(model, context, local)):
-        freq = cross.rope.frequencies.to(device=positions.device, dtype=torch.float32)
-        context.append(j, key, value, index=index, positions=positions, frequencies=freq, layout='axial')
+    the keys rotated at `positions` [1, L, 3]; nothing that is there is written again. The slot holds the new keys once
+    every layer's are written, and stays as it was on error."""
+    held, dev = context.host_lengths[index], context.lengths.device
+    grown = held + local.shape[1]
+    positions = positions.to(device=dev, dtype=torch.float32)[0].contiguous()
+    context.reserve(index, grown)
+    try:
+        lengths = torch.full((1,), grown, dtype=torch.int32, device=dev)
+        for j, (cross, key, value) in enumerate(_local_kv(model, context, local)):
+            freq = cross.rope.frequencies.to(device=dev, dtype=torch.float32)
+            context.append(j, key, value, index=index, lengths=lengths, positions=positions, frequencies=freq,
+                           layout='axial')
+    except BaseException:
+        context.resize(index, held)
+        raise
+    context.resize(index, grown)
 
 
 class StepGraphs:
@@ -303,7 +312,8 @@ class SlotEngine:
     def extend_slot(self, index, local, positions):
         """Slot `index` of a paged engine takes further local context (`local` [1, L, W], `positions` [1, L, 3]) behind the
         condition that it holds, on the side stream like `load_slot`: a neighbour that has come in costs its own keys, not
-        the window's. The slot's tokens stay."""
+        the window's. The slot's tokens stay; on error (a pool that has too few pages, a `local` of another width) its context
+        does too."""
         index = int(index)
         if not isinstance(self.context, PagedContext):
             raise ValueError('extending a slot needs an engine with pages')

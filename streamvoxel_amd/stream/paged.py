@@ -248,6 +248,14 @@ class PagedContext:
     def _set(self, wanted):
         """The windows' lengths {index: length}: pages taken and freed, table and lengths sent. Nothing changes on
         error."""
+        self._take(wanted)
+        changed = sorted(index for index, length in wanted.items() if length != self.host_lengths[index])
+        for index in changed:
+            self.host_lengths[index] = wanted[index]
+        self._send_lengths(changed)
+
+    def _take(self, wanted):
+        """Pages for the windows' lengths {index: length} taken and freed, and the table sent."""
         need = 0
         for index, length in wanted.items():
             if not 0 <= index < self.batch:
@@ -281,10 +289,6 @@ class PagedContext:
                 stream.wait_event(event)
         for index in moved:
             self._send(self.table[index, :len(self._owned[index])], self._owned[index])
-        changed = sorted(index for index, length in wanted.items() if length != self.host_lengths[index])
-        for index in changed:
-            self.host_lengths[index] = wanted[index]
-        self._send_lengths(changed)
 
     def _send_lengths(self, windows):
         """The lengths of these windows (ascending) alone: a call for another window may be on its way on another
@@ -317,6 +321,13 @@ class PagedContext:
         stay)."""
         self._set({int(index): int(length)})
 
+    def reserve(self, index, length):
+        """Window `index` takes the pages of `length` keys, at least as many as it holds, and holds no more for now:
+        `append` with `lengths` writes the new ones, `resize` then makes them seen."""
+        if 0 <= index < self.batch and length < self.host_lengths[index]:
+            raise ValueError(f'window {index} holds {self.host_lengths[index]} keys')
+        self._take({int(index): int(length)})
+
     def release(self, index):
         """Window `index` gives its pages back."""
         self.resize(index, 0)
@@ -332,15 +343,17 @@ class PagedContext:
         t = t.to(device=self.lengths.device, dtype=torch.bfloat16)
         return t if t.stride(-1) == 1 else t.contiguous()
 
-    def append(self, layer, key, value, index=None, n=None, cu_tokens=None, **how):
+    def append(self, layer, key, value, index=None, n=None, cu_tokens=None, lengths=None, **how):
         """`paged_append` into layer `layer` of the first n windows (all by default), or of window `index` alone (key,
-        value [heads, L, head_dim] then); `how`: its before, positions, frequencies, layout, amplitude."""
+        value [heads, L, head_dim] then); `lengths` (default: the windows') counts the keys with the new ones; `how`:
+        its before, positions, frequencies, layout, amplitude."""
         at = slice(0, self.batch if n is None else n)
         if index is not None:
             at, key, value = slice(index, index + 1), key[None], value[None]
             if how.get('positions') is not None:
                 how['positions'] = how['positions'][None]
-        paged_append(key, value, self.k[layer], self.v[layer], self.table[at], self.lengths[at], cu_tokens=cu_tokens,
+        lengths = self.lengths[at] if lengths is None else lengths
+        paged_append(key, value, self.k[layer], self.v[layer], self.table[at], lengths, cu_tokens=cu_tokens,
                      k_exponents=self.k_exponents[layer], v_exponents=self.v_exponents[layer], bad=self.bad, **how)
 
     def write(self, layer, index, key, value, prefix=None, positions=None, frequencies=None):

@@ -939,3 +939,41 @@ def test_pages_that_change_hands_between_streams():
     for b, want in ((0, short), (1, other)):
         at = torch.arange(want.shape[1], device=DEV)
         assert torch.equal(ctx.v[0][ctx.table[b].long()[at // 16], :, at % 16].transpose(0, 1), want)
+
+
+@pytest.mark.parametrize('kv_dtype', ['bf16', 'fp8'])
+def test_an_extension_that_fails_leaves_the_slot_as_it_was(kv_dtype):
+    """A local context of the wrong width, and one that fails in the last layer: lengths, pages and the step stay; a good one
+    then grows the slot."""
+    from streamvoxel_amd import synth
+    from streamvoxel_amd.stream.engine import SlotEngine
+    model = synth.StepModel(classes=40, voxel_shape=(64, 16, 16), width=192, depth=4, heads=8, control_width=192,
+                            control_depth=2, seed=3)
+    for p in model.parameters():
+        p.data = p.data.to(torch.bfloat16)
+    model = model.to(DEV)
+    spec = synth.WindowSpec(height=64, tile=16, num_classes=40)
+    engine = SlotEngine(model, spec, DEV, 2, l1_cap=2, l2_cap=8, kv_dtype=kv_dtype, pages=24)
+    conds = [synth.condition(model, P, L, seed=70 + i, device=DEV) for i, (P, L) in enumerate([(32, 100), (9, 72)])]
+    for i, c in enumerate(conds):
+        engine.load_slot(i, c)
+    engine.wait_loads()
+    want, free = engine.replay(0.5).patches.clone(), engine.context.free_pages
+    more = synth.condition(model, 0, 90, seed=80, device=DEV)
+
+    def failing(*args):
+        raise RuntimeError('the layer fails')
+    for break_it in (False, True):
+        hook = model.cross[-1].key_value.register_forward_pre_hook(failing) if break_it else None
+        with pytest.raises(RuntimeError):
+            engine.extend_slot(1, more.local if break_it else more.local[..., 8:], more.positions)
+        if hook is not None:
+            hook.remove()
+        engine.wait_loads()
+        assert engine.packed.lengths.tolist() == engine.context.host_lengths == [132, 81]
+        assert engine.context.free_pages == free and int(engine.context.bad) == 0
+        assert torch.equal(engine.replay(0.5).patches, want)
+    engine.extend_slot(1, more.local, more.positions)
+    engine.wait_loads()
+    assert engine.packed.lengths.tolist() == engine.context.host_lengths == [132, 171]
+    assert not torch.equal(engine.replay(0.5).patches, want)

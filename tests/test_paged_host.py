@@ -305,3 +305,48 @@ def test_a_page_that_changes_streams_is_waited_for(monkeypatch):
     side.work.clear()
     ctx.resize(0, 17)
     assert side.work == [('wait', ('main', 1)), 'send', 'send'] and not ctx._left
+
+
+class Layer(torch.nn.Module):
+    def __init__(self, width, context_width, heads):
+        super().__init__()
+        self.heads, self.width = heads, width
+        self.key_value = torch.nn.Linear(context_width, 2 * width)
+        self.rope = torch.nn.Module()
+        self.rope.frequencies = torch.ones(width // heads // 6)
+
+
+@pytest.mark.filterwarnings('ignore:.*autocast')
+@pytest.mark.parametrize('fails', [None, 'width', 'layer'])
+def test_a_slot_is_extended_whole_or_not_at_all(fails, monkeypatch):
+    """The new keys are written under a length of their own; the slot's stays what it was until the last layer has them, and
+    for good, its pages too, when one fails."""
+    from streamvoxel_amd.stream import paged
+    from streamvoxel_amd.stream.engine import extend_condition
+    Streams(monkeypatch)
+    model = torch.nn.Module()
+    model.cross = torch.nn.ModuleList([Layer(96, 40, 2) for _ in range(2)])
+    ctx = paged.PagedContext(2, 3, 2, 48, 12, 'cpu', page_size=16, max_pages=20)
+    ctx.resize(1, 20)
+    seen = []
+
+    def append(key, value, k, v, table, lengths, **how):
+        seen.append((key.shape, ctx.lengths.tolist(), lengths.tolist(), table[0, :4].tolist()))
+        if fails == 'layer' and len(seen) == 2:
+            raise RuntimeError('the layer fails')
+    monkeypatch.setattr(paged, 'paged_append', append)
+    extend = lambda: extend_condition(model, ctx, 1, torch.zeros(1, 30, 41 if fails == 'width' else 40), torch.zeros(1, 30, 3))
+    if fails:
+        with pytest.raises(RuntimeError):
+            extend()
+        assert ctx.host_lengths == ctx.lengths.tolist() == [0, 20, 0]
+        assert ctx._owned[1] == [0, 1] and ctx.free_pages == 10
+    else:
+        extend()
+        assert ctx.host_lengths == ctx.lengths.tolist() == [0, 50, 0] and len(ctx._owned[1]) == 4
+        assert [s[1:3] for s in seen] == [([0, 20, 0], [50])] * 2
+        assert all(s[3] == ctx._owned[1] for s in seen)
+    with pytest.raises(RuntimeError, match='pages left'):
+        extend_condition(model, ctx, 1, torch.zeros(1, 200, 40), torch.zeros(1, 200, 3))
+    with pytest.raises(ValueError, match='holds'):
+        ctx.reserve(1, 10)
