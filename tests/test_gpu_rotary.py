@@ -201,3 +201,21 @@ def test_rotary_gradient_of_the_gradient():
     assert torch.equal(ddy.detach(), rotary(w, positions, f, amplitude=1.5))
     again, = torch.autograd.grad(y, x, dy.detach())
     assert torch.equal(again, dx.detach())
+
+
+@pytest.mark.parametrize('dtype', [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize('layout', ['half', 'interleaved'])
+def test_rotary_in_forward_mode(layout, dtype):
+    """A linear map: the tangent of the result is the rotation of x's tangent, of a leaf's too."""
+    from torch.autograd import forward_ad as fw
+    from streamvoxel_amd.stream.rotary import rotary
+    g = torch.Generator().manual_seed(12)
+    x, t = [torch.randn(2, 9, 3, 40, generator=g).to(dtype).to(DEV).transpose(1, 2) for _ in range(2)]
+    positions, f = torch.randint(0, 9000, (2, 9), generator=g).to(DEV), freqs(16)
+    with fw.dual_level():
+        for leaf in (x, x.clone().requires_grad_()):
+            y = fw.unpack_dual(rotary(fw.make_dual(leaf, t), positions, f, layout, 1.5))
+            check(y.primal, x, positions, f, layout, 1.5)
+            check(y.tangent, t, positions, f, layout, 1.5)
+        with pytest.raises(ValueError, match='gradient'):
+            rotary(fw.make_dual(x, t), positions, f, out=torch.empty_like(x))

@@ -350,3 +350,47 @@ def test_a_slot_is_extended_whole_or_not_at_all(fails, monkeypatch):
         extend_condition(model, ctx, 1, torch.zeros(1, 200, 40), torch.zeros(1, 200, 3))
     with pytest.raises(ValueError, match='holds'):
         ctx.reserve(1, 10)
+
+
+def test_a_tangent_goes_through_the_rotation(monkeypatch):
+    """Forward mode, alone and over and under the gradient, with the launch replaced by the formula on the host: linear, so the
+    tangent turns as x does. No tangent is dropped silently."""
+    from torch.autograd import forward_ad as fw
+    from streamvoxel_amd.stream import rotary as module
+
+    def launch(x, out, positions, frequencies, layout, amplitude, inverse):
+        angle = positions.double()[:, None] * frequencies
+        c, s = amplitude * angle.cos(), (-1 if inverse else 1) * amplitude * angle.sin()
+        a, b = x.double().chunk(2, -1)
+        return out.copy_(torch.cat((a * c - b * s, b * c + a * s), -1))
+    monkeypatch.setattr(module, '_launch', launch)
+    monkeypatch.setattr(_lib, 'require_one_gpu', lambda *t: None)
+    g = torch.Generator().manual_seed(3)
+    x, t, dy = [torch.randn(2, 3, 5, 8, generator=g) for _ in range(3)]
+    p, f = torch.arange(5) * 3, rotary_frequencies(8)[0]
+    turn = lambda x: rotary(x, p, f, amplitude=1.5)
+    want = turn(t)
+    strange = t.transpose(2, 3).contiguous().transpose(2, 3)
+    with fw.dual_level():
+        for tangent in (t, strange):
+            y = fw.unpack_dual(turn(fw.make_dual(x, tangent)))
+            assert torch.equal(y.primal, turn(x)) and torch.equal(y.tangent, want)
+        with torch.no_grad():
+            assert torch.equal(fw.unpack_dual(turn(fw.make_dual(x, t))).tangent, want)
+        leaf = x.clone().requires_grad_()
+        y = fw.unpack_dual(turn(fw.make_dual(leaf, t)))
+        assert torch.equal(y.tangent, want)
+        back, = torch.autograd.grad(y.primal, leaf, dy)
+        assert torch.equal(back, launch(dy, torch.empty_like(dy), p, f, 'half', 1.5, 1))
+        # the tangent of the gradient: the transposed rotation of dy's
+        leaf = x.clone().requires_grad_()
+        back, = torch.autograd.grad(turn(leaf), leaf, fw.make_dual(dy, t), create_graph=True)
+        assert torch.equal(fw.unpack_dual(back).tangent, launch(t, torch.empty_like(t), p, f, 'half', 1.5, 1))
+        # the gradient of the tangent
+        moving = t.clone().requires_grad_()
+        tangent = fw.unpack_dual(turn(fw.make_dual(x, moving))).tangent
+        back, = torch.autograd.grad(tangent, moving, dy)
+        assert torch.equal(back, launch(dy, torch.empty_like(dy), p, f, 'half', 1.5, 1))
+        with pytest.raises(ValueError, match='gradient'):
+            rotary(fw.make_dual(x, t), p, f, out=torch.empty_like(x))
+    assert torch.equal(turn(x), launch(x, torch.empty_like(x), p, f, 'half', 1.5, 0))
