@@ -119,10 +119,11 @@ __device__ __forceinline__ void row_work(const PagedArgs& a, int place, char* sV
   Lane8 vl[4 * kHalves];
 #pragma unroll
   for (int i = 0; i < 4 * kHalves; ++i) vl[i] = v_lane<ES>(a, 8 * i, 16 * (i >> 1));
-  // The lane's key of each half and its offsets in a K row (the last step's chunk may lie past head_dim, where Q is
-  // zero: any chunk of the row then).
+  // The lane's key of each half and its offsets in a K row (the last step's chunk may lie past head_dim: any chunk of
+  // the row then, and zeros in its place, since an infinity there times Q's zeros would be NaN).
   const int own = sigma_row(col);
-  const int k_last = 16 * (KS - 1) + 8 * hh < D ? 16 * (KS - 1) * ES : -8 * hh * ES;
+  const bool past = 16 * (KS - 1) + 8 * hh >= D;
+  const int k_last = past ? -8 * hh * ES : 16 * (KS - 1) * ES;
 
   using KWord = typename std::conditional<FP8, uint2, uint4>::type;
   KWord kw[kHalves][KS];
@@ -206,6 +207,7 @@ __device__ __forceinline__ void row_work(const PagedArgs& a, int place, char* sV
             ka[k] = __builtin_bit_cast(bf16x8_t, kw[t][k]);
           }
         }
+        if (past) ka[KS - 1] = bf16x8_t{};
         x[t] = scores<KS>(s, ka);
         if (__builtin_expect(broken, 0)) {
           // (The pages' numbers are the next block's by now: looked up again.)

@@ -977,3 +977,32 @@ def test_an_extension_that_fails_leaves_the_slot_as_it_was(kv_dtype):
     engine.wait_loads()
     assert engine.packed.lengths.tolist() == engine.context.host_lengths == [132, 171]
     assert not torch.equal(engine.replay(0.5).patches, want)
+
+
+@pytest.mark.parametrize('kv_dtype', ['bf16', 'fp8'])
+@pytest.mark.parametrize('n', [1, 40])
+@pytest.mark.parametrize('D', [8, 24, 40, 72, 104, 120, 64])
+def test_a_key_whose_score_is_minus_infinity_has_no_weight(D, n, kv_dtype):
+    """One element of a key infinite against queries of the other sign there, in both forms and at widths whose last step is
+    half empty: the formula's finite result. (e4m3 has no code for an infinity: 448 2^127 there.)"""
+    from streamvoxel_amd.stream.paged import paged_attention
+    pool = Pool([90, 40], 2, D, 16, D, kv_dtype, clean=True)
+    q = queries(2, 4, n, D, n)
+    q[..., 3] = -q[..., 3].abs() - 0.125
+    j = 37
+    row = (pool.table[0, j // 16].long(), slice(None), j % 16)
+    key = pool.k[row].float()
+    if kv_dtype == 'bf16':
+        key[:, 3] = math.inf
+        pool.k[row] = key.to(pool.k.dtype)
+    else:
+        key[:], key[:, 3] = 0, 448
+        pool.k[row] = key.to(pool.k.dtype)
+        pool.ke[row] = 254
+    got = paged_attention(q, *pool.args(), **pool.exponents())
+    k, v = pool.rows(0)
+    keep = [i for i in range(90) if i != j]
+    want, err = attend64(q[0].cpu().double(), k[:, keep], v[:, keep], False, D ** -0.5)
+    off = (got[0].cpu().double() - want).abs()
+    assert not torch.isnan(off).any() and (off <= err).all()
+    check(got[1:], q[1:], _window(pool, 1), False)
