@@ -33,6 +33,9 @@ void clear_error();
     }                                                                                   \
   } while (0)
 
+// A stride as it counts: that of a dimension with one element, or of none (n 0: not used), may be anything.
+inline int64_t used_stride(int64_t n, int64_t stride) { return n > 1 ? stride : 0; }
+
 inline hipStream_t as_stream(void* s) { return reinterpret_cast<hipStream_t>(s); }
 
 // ----------------------------------------------------------------------------------------------- device helpers

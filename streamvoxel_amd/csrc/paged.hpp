@@ -113,22 +113,28 @@ inline int check_pool(const char* name, const svhip_paged_cache& c) {
   SVHIP_REQUIRE(c.lengths && (c.max_pages == 0 || c.page_table) && c.k_pages && c.v_pages, "%s: null pointer", name);
   SVHIP_REQUIRE(!fp8 || (c.k_exponents && c.v_exponents), "%s: e4m3 pages need the rows' exponents", name);
   const uintptr_t bytes = fp8 ? 8 : 16;
+  const int64_t sk_p = used_stride(c.pages, c.sk_p), sv_p = used_stride(c.pages, c.sv_p);
+  const int64_t sk_h = used_stride(c.heads, c.sk_h), sv_h = used_stride(c.heads, c.sv_h);
   SVHIP_REQUIRE(reinterpret_cast<uintptr_t>(c.k_pages) % bytes == 0 && reinterpret_cast<uintptr_t>(c.v_pages) % bytes == 0 &&
-                    (c.sk_p | c.sk_h | c.sk_r | c.sv_p | c.sv_h | c.sv_r) % 8 == 0,
+                    (sk_p | sk_h | c.sk_r | sv_p | sv_h | c.sv_r) % 8 == 0,
                 "%s: rows of a page must start on %d-byte boundaries", name, (int)bytes);
   // A head's rows of a page lie within 2^31 bytes, pages start less than 2^32 bytes apart.
   SVHIP_REQUIRE(c.sk_r >= 0 && c.sv_r >= 0 && c.sk_r < (1 << 29) / c.page_size && c.sv_r < (1 << 29) / c.page_size,
                 "%s: rows of a page too far apart", name);
   const int64_t most = 1ll << 31;
-  SVHIP_REQUIRE(c.sk_p >= 0 && c.sk_p < most && c.sv_p >= 0 && c.sv_p < most && c.sek_p >= 0 && c.sek_p < most &&
-                    c.sev_p >= 0 && c.sev_p < most,
+  const int64_t sek_p = used_stride(c.pages, c.sek_p), sev_p = used_stride(c.pages, c.sev_p);
+  SVHIP_REQUIRE(sk_p >= 0 && sk_p < most && sv_p >= 0 && sv_p < most && sek_p >= 0 && sek_p < most && sev_p >= 0 &&
+                    sev_p < most,
                 "%s: pages too far apart", name);
   return SVHIP_OK;
 }
 
-// Rows of 8 bf16 values that start on 16-byte boundaries.
-inline bool rows16(const void* p, int64_t x, int64_t y, int64_t z) {
-  return reinterpret_cast<uintptr_t>(p) % 16 == 0 && (x | y | z) % 8 == 0;
+// Rows of bf16 values that start on boundaries of `values` values: strides of a window, a head and a token (windows 0:
+// packed).
+inline bool rows_on(int64_t values, const void* p, int64_t windows, int64_t heads, int64_t tokens, int64_t s_b, int64_t s_h,
+                    int64_t s_n) {
+  return reinterpret_cast<uintptr_t>(p) % (2 * values) == 0 &&
+         (used_stride(windows, s_b) | used_stride(heads, s_h) | used_stride(tokens, s_n)) % values == 0;
 }
 
 inline Pages pages_of(const svhip_paged_cache& c) {

@@ -275,7 +275,9 @@ extern "C" int svhip_paged_append(const svhip_paged_cache* cache, const svhip_pa
   SVHIP_REQUIRE(c.key && c.value, "%s: null pointer", name);
   SVHIP_REQUIRE(!turns || c.freq, "%s: the rotation needs frequencies", name);
   SVHIP_REQUIRE(!axial || c.positions, "%s: the three-axis rotation needs positions", name);
-  SVHIP_REQUIRE(rows16(c.key, c.sk_b, c.sk_h, c.sk_n) && rows16(c.value, c.sv_b, c.sv_h, c.sv_n),
+  const int64_t even = c.cu_tokens ? 0 : p.windows;
+  SVHIP_REQUIRE(rows_on(8, c.key, even, p.heads, c.N, c.sk_b, c.sk_h, c.sk_n) &&
+                    rows_on(8, c.value, even, p.heads, c.N, c.sv_b, c.sv_h, c.sv_n),
                 "%s: key and value rows must start on 16-byte boundaries", name);
   const int64_t total = c.cu_tokens ? c.N : p.windows * c.N;
   const int per_group = static_cast<int>(tokens_per_group(total, kAppendTokens));

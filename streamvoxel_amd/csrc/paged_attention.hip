@@ -235,8 +235,9 @@ extern "C" int svhip_paged_attention(const svhip_paged_cache* cache, const svhip
   if (B == 0 || H == 0 || N == 0) return SVHIP_OK;
   if (const int rc = check_pool(name, pc)) return rc;
   SVHIP_REQUIRE(c.q && c.out, "%s: null pointer", name);
-  SVHIP_REQUIRE(rows16(c.q, c.sq_b, c.sq_h, c.sq_n), "%s: query rows must start on 16-byte boundaries", name);
-  SVHIP_REQUIRE(reinterpret_cast<uintptr_t>(c.out) % 8 == 0 && (c.so_b | c.so_h | c.so_n) % 4 == 0,
+  const int64_t even = c.cu_queries ? 0 : B;
+  SVHIP_REQUIRE(rows_on(8, c.q, even, H, N, c.sq_b, c.sq_h, c.sq_n), "%s: query rows must start on 16-byte boundaries", name);
+  SVHIP_REQUIRE(rows_on(4, c.out, even, H, N, c.so_b, c.so_h, c.so_n),
                 "%s: rows of out must start on 8-byte boundaries", name);
   const bool fp8 = pc.kv_dtype == SVHIP_FP8_E4M3;
   const int row_most = fp8 ? kRowMostFp8 : kRowMost;

@@ -209,7 +209,8 @@ extern "C" int svhip_rotary(const svhip_rotary_args* args, void* stream) {
   const int64_t run = c.dtype == SVHIP_F32 ? 4 : 8;
   const bool vec = c.pairs % run == 0 && c.D % run == 0 && reinterpret_cast<uintptr_t>(c.x) % 16 == 0 &&
                    reinterpret_cast<uintptr_t>(c.out) % 16 == 0 &&
-                   (c.sx_b | c.sx_h | c.sx_n | c.so_b | c.so_h | c.so_n) % run == 0;
+                   (used_stride(c.B, c.sx_b | c.so_b) | used_stride(c.H, c.sx_h | c.so_h) |
+                    used_stride(c.N, c.sx_n | c.so_n)) % run == 0;
   hipStream_t s = as_stream(stream);
   if (c.dtype == SVHIP_F32) {
     launch_rotary<float>(a, vec, s);

@@ -26,7 +26,7 @@ def _check_pool(k_pages, v_pages, page_table, lengths, k_exponents, v_exponents,
         raise ValueError('k_pages and v_pages must be [pages, heads, page, head_dim] alike')
     if k_pages.stride(-1) != 1 or v_pages.stride(-1) != 1:
         raise ValueError('rows of a page need a contiguous head_dim')
-    if page_table.dtype != torch.int32 or page_table.dim() != 2 or page_table.stride(-1) != 1:
+    if page_table.dtype != torch.int32 or page_table.dim() != 2 or (page_table.stride(1) != 1 and page_table.shape[1] > 1):
         raise ValueError('page_table must be int32 [B, pages of a window] with contiguous rows')
     if lengths.dtype != torch.int32 or lengths.shape != page_table.shape[:1] or not lengths.is_contiguous():
         raise ValueError('lengths must be a contiguous int32 [B]')
@@ -68,7 +68,10 @@ def _rows16(t):
         off |= s
     if last == 1 and off & 7 == 0:
         return t
-    return t.clone() if t.is_contiguous() else t.contiguous()
+    # (The stride of a dimension with one element is never used, and may be anything.)
+    if last == 1 and (t.data_ptr() >> 1) & 7 == 0 and all(s & 7 == 0 for n, s in zip(t.shape, rows) if n > 1):
+        return t
+    return t.clone(memory_format=torch.contiguous_format)
 
 
 _CACHE = struct.Struct('7P18q')    # svhip_paged_cache

@@ -1006,3 +1006,30 @@ def test_a_key_whose_score_is_minus_infinity_has_no_weight(D, n, kv_dtype):
     off = (got[0].cpu().double() - want).abs()
     assert not torch.isnan(off).any() and (off <= err).all()
     check(got[1:], q[1:], _window(pool, 1), False)
+
+
+@pytest.mark.parametrize('n', [1, 50])
+def test_odd_strides_of_dimensions_with_one_element(n):
+    """One window or one head whose stride, never used, is no multiple of 8: taken as it is, or copied where the rows lie
+    between 16-byte boundaries too."""
+    from streamvoxel_amd.stream.paged import paged_append, paged_attention
+    from streamvoxel_amd.stream.rotary import rotary
+    pool = Pool([400], 1, 64, 16, 1, clean=True)
+    k, v, table, lengths = pool.args()
+    buffer = torch.randn(70 * 64 + 9, generator=torch.Generator().manual_seed(n)).to(torch.bfloat16).to(DEV)
+    f = torch.ones(32, dtype=torch.float64, device=DEV) / 100
+    for start, strides in ((0, (n * 64 + 1, 3, 64, 1)), (1, (n * 64 + 1, 5, 64, 1)), (8, (7, n * 64 + 3, 64, 1))):
+        x = buffer.as_strided((1, 1, n, 64), strides, start)
+        same = x.clone(memory_format=torch.contiguous_format)
+        want = paged_attention(same, k, v, table.clone(), lengths, causal=True)
+        assert torch.equal(paged_attention(x, k, v, table, lengths, causal=True), want)
+        out = torch.zeros(n * 64 + 9, dtype=torch.bfloat16, device=DEV).as_strided((1, 1, n, 64), (n * 64 + 1, 1, 64, 1), 4)
+        assert torch.equal(paged_attention(x, k, v, table, lengths, causal=True, out=out), want)
+        check(want, same, pool, True)
+        pages = [torch.zeros(pool.pages, 16, 64, dtype=torch.bfloat16, device=DEV).as_strided(k.shape, (1024, 3, 64, 1))
+                 for _ in 'kv']
+        paged_append(x, x, *pages, table, lengths)
+        at = torch.arange(400 - n, 400, device=DEV)
+        assert torch.equal(pages[0][table[0].long()[at // 16], :, at % 16].transpose(0, 1), same[0])
+        turned = rotary(x, torch.arange(n, device=DEV), f)
+        assert torch.equal(turned, rotary(same, torch.arange(n, device=DEV), f))

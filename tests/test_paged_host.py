@@ -394,3 +394,31 @@ def test_a_tangent_goes_through_the_rotation(monkeypatch):
         with pytest.raises(ValueError, match='gradient'):
             rotary(fw.make_dual(x, t), p, f, out=torch.empty_like(x))
     assert torch.equal(turn(x), launch(x, torch.empty_like(x), p, f, 'half', 1.5, 0))
+
+
+def test_strides_of_dimensions_with_one_element_are_not_looked_at(lib):
+    """Rows are judged by the strides that a call uses: none for a dimension of one, or for the windows of packed tokens. (Calls
+    that pass their checks up to a later one, or to the workspace's.)"""
+    from streamvoxel_amd.stream.paged import _rows16
+    error = lib.svhip_last_error
+    assert append_call(lib, sk=(770, 68, 129)) == -1 and b'16-byte' in error()
+
+    def attend(B=2, Hkv=2, N=3, pages=4, cu=0, sq=(768, 192, 64), so=(768, 192, 64), sk=(8192, 4096), m=20):
+        cache = struct.pack('7P18q', FAKE, FAKE, 0, 0, FAKE, FAKE, 0, 1, B, Hkv, 64, pages, 64, m, m, *sk, 64, *sk, 64, 0, 0, 0, 0)
+        args = struct.pack('4P10qd', FAKE, FAKE, cu, 0, 0, Hkv, N, *sq, *so, 0, 0.125)
+        assert lib.svhip_paged_attention(cache, args, None) == -1
+        return error()
+    assert b'query rows' in attend(sq=(769, 192, 64)) and b'rows of out' in attend(so=(770, 192, 64))
+    assert b'rows of a page' in attend(sk=(8193, 4096)) and b'rows of a page' in attend(sk=(8192, 4097))
+    for kw in (dict(B=1, sq=(769, 192, 64), so=(770, 192, 64)), dict(Hkv=1, sq=(768, 193, 64), so=(768, 194, 64)),
+               dict(N=1, sq=(768, 192, 65), so=(768, 192, 66)), dict(pages=1, sk=(8193, 4096)), dict(Hkv=1, sk=(8192, 4097)),
+               dict(cu=FAKE, sq=(769, 192, 64), so=(770, 192, 64))):
+        assert b'workspace' in attend(**kw), kw
+    odd = torch.zeros(400, dtype=torch.bfloat16)
+    for shape, strides in (((1, 2, 3, 8), (49, 24, 8, 1)), ((2, 1, 3, 8), (24, 7, 8, 1)), ((2, 3, 1, 8), (24, 8, 5, 1))):
+        t = odd.as_strided(shape, strides)
+        assert _rows16(t) is t
+    for shape, strides in (((1, 2, 3, 8), (49, 24, 9, 1)), ((1, 1, 3, 8), (3, 5, 8, 1)), ((2, 3, 4, 8), (96, 32, 8, 1))):
+        t = odd[1:].as_strided(shape, strides, 1)
+        copy = _rows16(t)
+        assert torch.equal(copy, t) and all(s % 8 == 0 for s in copy.stride()[:-1]) and copy.data_ptr() % 16 == 0
