@@ -123,8 +123,13 @@ def paged_append(key, value, k_pages, v_pages, page_table, lengths, cu_tokens=No
         raise ValueError('key and value must be alike, with the heads and the head_dim of the pages')
     if before < 0:
         raise ValueError('before counts keys')
-    if _lib.stacked(k_pages) or _lib.stacked(v_pages):
-        raise ValueError('k_pages and v_pages must have a place for every element')
+    for k, v in ((k_pages, v_pages), (k_exponents, v_exponents)):
+        if k is None:
+            break
+        if _lib.stacked(k) or _lib.stacked(v):
+            raise ValueError('pages and their exponents must have a place for every element')
+        if P and k.data_ptr() == v.data_ptr():
+            raise ValueError('keys and values must not share their pages or exponents')
     wide, pairs, sp, turn = 0, 0, (0, 0), _lib.SVHIP_ROTARY_NONE
     if frequencies is not None:
         if layout not in LAYOUTS:

@@ -422,3 +422,26 @@ def test_strides_of_dimensions_with_one_element_are_not_looked_at(lib):
         t = odd[1:].as_strided(shape, strides, 1)
         copy = _rows16(t)
         assert torch.equal(copy, t) and all(s % 8 == 0 for s in copy.stride()[:-1]) and copy.data_ptr() % 16 == 0
+
+
+def test_an_append_has_a_place_for_every_row(monkeypatch):
+    """Pages or exponents whose elements lie on each other, or keys and values in the same ones, would be written by two rows at
+    once: refused before anything is launched. Halves of one buffer are places of their own."""
+    from streamvoxel_amd.stream import paged
+    launched = []
+    monkeypatch.setattr(_lib, 'require_one_gpu', lambda *t: None)
+    monkeypatch.setattr(_lib, 'launch', lambda *args: launched.append(args))
+    x, n = torch.zeros(1, 2, 3, 8, dtype=torch.bfloat16), torch.ones(1, dtype=torch.int32)
+    table = torch.zeros(1, 1, dtype=torch.int32)
+    both = torch.zeros(4, 2, 2, 16, 8, dtype=torch.bfloat16)
+    codes, e = torch.zeros(2, 4, 2, 16, 8).to(torch.float8_e4m3fn), torch.zeros(2, 4, 2, 16, dtype=torch.uint8)
+    append = lambda k, v, ke=None, ve=None: paged.paged_append(x, x, k, v, table, n, k_exponents=ke, v_exponents=ve)
+    append(both[:, 0], both[:, 1])
+    append(codes[0], codes[1], e[0], e[1])
+    assert len(launched) == 2
+    one = e[0, :1].expand(4, 2, 16)
+    for args in ((both[:, 0], both[:, 0]), (both[:1, 0].expand(4, 2, 16, 8), both[:, 1]), (codes[0], codes[0], e[0], e[1]),
+                 (codes[0], codes[1], e[0], e[0]), (codes[0], codes[1], one, e[1]), (codes[0], codes[1], e[1], one)):
+        with pytest.raises(ValueError, match='place|share'):
+            append(*args)
+    assert len(launched) == 2
