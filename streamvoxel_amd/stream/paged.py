@@ -214,7 +214,7 @@ class PagedContext:
     The host keeps the books: `resize` and `grow` take and free pages and send the window's table and length to the
     device on the current stream without waiting for it; calls that touch a window's pages must be ordered after them,
     as usual. Other windows may be in work on other streams: a page that changes hands is waited for. A replayed graph
-    reads the table and the lengths as they stand. `bad` (device int32 [1]) becomes non-zero when a
+    reads the table and the lengths as they stand; a capture that would change them is refused. `bad` (device int32 [1]) becomes non-zero when a
     call meets a page outside the pool, which these books never name."""
 
     def __init__(self, layers, batch, heads, head_dim, pages, device, page_size=64, max_pages=None, kv_dtype='bf16'):
@@ -250,6 +250,9 @@ class PagedContext:
     def _stream(self):
         return torch.cuda.current_stream(self.lengths.device) if self.lengths.is_cuda else None
 
+    def _capturing(self):
+        return self.lengths.is_cuda and torch.cuda.is_current_stream_capturing()
+
     def _pages_for(self, length):
         return -(-length // self.page_size)
 
@@ -276,6 +279,8 @@ class PagedContext:
         if need > len(self._free):
             raise RuntimeError(f'the pool has {len(self._free)} pages left, {need} more are needed')
         stream, freed, moved = self._stream(), [], []
+        if self._capturing():
+            raise RuntimeError('the books of a PagedContext are kept by the host: change them outside the capture')
         for index, length in wanted.items():          # freed pages first: another window may take them
             own, n = self._owned[index], self._pages_for(length)
             if n != len(own):

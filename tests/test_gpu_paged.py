@@ -1033,3 +1033,25 @@ def test_odd_strides_of_dimensions_with_one_element(n):
         assert torch.equal(pages[0][table[0].long()[at // 16], :, at % 16].transpose(0, 1), same[0])
         turned = rotary(x, torch.arange(n, device=DEV), f)
         assert torch.equal(turned, rotary(same, torch.arange(n, device=DEV), f))
+
+
+def test_books_do_not_change_in_a_capture():
+    """grow, resize and release are refused while their stream is captured; append and attend there are the graph's work."""
+    from streamvoxel_amd.stream.paged import PagedContext
+    ctx = PagedContext(1, 2, 2, 64, 6, DEV, page_size=16)
+    key, q = queries(2, 2, 5, 64, 0), queries(2, 4, 5, 64, 1)
+    ctx.grow(5)
+    ctx.append(0, key, key)
+    want = ctx.attend(0, q, causal=True)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        for change in (lambda: ctx.grow(1), lambda: ctx.release(0), lambda: ctx.resize(1, 40)):
+            with pytest.raises(RuntimeError, match='capture'):
+                change()
+        ctx.append(0, key, key)
+        out = ctx.attend(0, q, causal=True)
+    for _ in range(3):
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, want) and ctx.lengths.tolist() == ctx.host_lengths == [5, 5] and ctx.free_pages == 4
+        ctx.grow(0)

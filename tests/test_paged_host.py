@@ -445,3 +445,25 @@ def test_an_append_has_a_place_for_every_row(monkeypatch):
         with pytest.raises(ValueError, match='place|share'):
             append(*args)
     assert len(launched) == 2
+
+
+def test_a_capture_does_not_change_the_books(monkeypatch):
+    """What a capture would send is a host number of that moment, which every replay would send again: refused, and nothing
+    changes."""
+    from streamvoxel_amd.stream.paged import PagedContext
+    stream, capturing = RecordedStream('main'), [False]
+    monkeypatch.setattr(PagedContext, '_stream', lambda self: stream)
+    monkeypatch.setattr(PagedContext, '_capturing', lambda self: capturing[0], raising=False)
+    monkeypatch.setattr(PagedContext, '_send', staticmethod(lambda to, v: to.copy_(torch.tensor(v, dtype=torch.int32))))
+    ctx = PagedContext(1, 2, 2, 64, 6, 'cpu', page_size=16)
+    ctx.grow(20)
+    capturing[0] = True
+    for change in (lambda: ctx.grow(1), lambda: ctx.grow(20), lambda: ctx.release(1), lambda: ctx.resize(0, 0),
+                   lambda: ctx.reserve(1, 60)):
+        with pytest.raises(RuntimeError, match='capture'):
+            change()
+        assert ctx.lengths.tolist() == ctx.host_lengths == [20, 20] and ctx._owned == [[0, 1], [2, 3]]
+        assert ctx.free_pages == 2 and not stream.work
+    capturing[0] = False
+    ctx.grow(1)
+    assert ctx.lengths.tolist() == [21, 21]
