@@ -451,7 +451,8 @@ int svhip_rotary(const svhip_rotary_args* args, void* stream);
 /*
  * A paged cache: pools k_pages, v_pages of `pages` pages, element (page, h, r, d) at page*s_p + h*s_h + r*s_r + d,
  * rows r in [0, page_size), page_size a power of two from 16 to 1024, head_dim a multiple of 8 up to 128, rows
- * 16-byte aligned (e4m3: 8), max_pages * page_size at most 2^30. Key j of window b is row j % page_size of page
+ * 16-byte aligned (e4m3: 8; a stride counts where its dimension has more than one element, here and below), max_pages *
+ * page_size at most 2^30. Key j of window b is row j % page_size of page
  * page_table[b*table_stride + j / page_size] (int32, max_pages numbers a window); lengths[b] (int32) counts the
  * window's keys. kv_dtype SVHIP_BF16, or SVHIP_FP8_E4M3: OCP e4m3fn codes with one power of two for each row and
  * head, value = code 2^(exponent - 127), exponents 1 to 254, bytes (page, h, r) at page*se_p + h*se_h + r. Windows may share
@@ -495,7 +496,9 @@ int svhip_paged_append(const svhip_paged_cache* cache, const svhip_paged_append_
  * over the keys j < lengths[b] of key head h / (H / heads), with `causal` only j <= lengths[b] - n + i (n tokens of
  * window b, its last keys); no key: zeros; infinities and NaN reach the tokens that see them. Queries and out bf16,
  * N a window or packed by cu_queries, as in svhip_paged_append (rows outside every window are left as they are).
- * Products in bf16 on the matrix cores with fp32 sums, softmax weights rounded to bf16. Keys and values of a bad
+ * Products in bf16 on the matrix cores with fp32 sums, softmax weights rounded to bf16; scores stay below 2^30 in
+ * magnitude (a row with larger ones may be NaN). A row's last bits depend on the other windows of the call, which move
+ * the places where its keys are cut for several workgroups; the same call gives the same bits. Keys and values of a bad
  * page read as zeros; a length past the window's row of the table is cut to it. scale > 0. Query rows 16-byte
  * aligned, rows of out 8. workspace: svhip_paged_attention_workspace_bytes with max_keys = max_pages * page_size
  * (0: none needed), N and packed (cu_queries or not) as in the call; 16-byte aligned.

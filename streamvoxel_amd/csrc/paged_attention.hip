@@ -8,8 +8,9 @@
 //   * windows of more than kRowMost rows (tile, paged_tile.hpp): a workgroup takes 128 rows, 32 a wave; the 4 waves
 //     stage each block of 64 keys together, the next one in flight while the current one is computed. Bound: the
 //     matrix cores and the exponentials, which overlap little. Measured: 8 windows x 1024 queries, 1552 to 9744 keys,
-//     12 x 64 (153 GFLOP) 200 us, 770 TFLOP/s; 4 causal chunks of 512, 16 heads to 4 of 128, up to 16 384 keys (241
-//     GFLOP) 268 us and 12 of join.
+//     12 x 64 (153 GFLOP) 195 us, 785 TFLOP/s (e4m3 209); 4 causal chunks of 512, 16 heads to 4 of 128, up to 16 384
+//     keys (241 GFLOP) 279 us, 12 of them the join (e4m3 298); a causal prompt of 8192 tokens, 16 heads of 64 208 us
+//     (e4m3 235), of 128 345 (395); 32 queries of 64 windows over 2048 to 4096 keys, 8 heads of 64 86 us (e4m3 75).
 //   * windows of up to kRowMost rows, single tokens among them (row, paged_row.hpp): the 4 waves share the rows and
 //     split the keys, each staging its own blocks of 32 keys in its own LDS; no barrier until the waves' sums are
 //     joined. Bound: HBM. Measured: 64 tokens over 1.18 GB of keys 216 us, 5.4 TB/s; over 754 MB of e4m3 pages 148

@@ -19,7 +19,12 @@ constexpr int kTileRows = 128;     // rows of a tile workgroup
 // 128, 313 and 278 us for 281; the same with all keys seen 198 and 180 for 167; 1024 queries over 9744 keys 82 and 61
 // for 60).
 constexpr int kTileTarget = 512;
-constexpr int kTileBeside = 256;   // the same beside the row form: one for every CU (24 mixed windows 101 us; 512: 110)
+// The same beside the row form: one for every CU. With 512 in its place: 24 windows, 6 of them chunks (head_dim 96) 110 us
+// for 101; 8 heads of 64, 4 chunks of 512 and 60 tokens over 8192 keys 237 for 218, 32 chunks of 64 over 4096 and 8 tokens
+// over 32 768 175 for 168, 16 chunks of 256 over 2048 and 48 tokens over 4096 123 for 110, a chunk of 128 over 16 384 and
+// 63 tokens over 4096 123 for 116; 12 heads, 3 chunks of 512 over 4096 and 100 tokens over 2048 169 for 152; but 8 heads of
+// 96, 6 chunks of 300 and 18 tokens over 8192, as much of one form as of the other, 163 for 180.
+constexpr int kTileBeside = 256;
 constexpr int kTileLeast = 6;      // least key blocks of a tile's part (1024 queries over 9744 keys 60 us; 3, 12: 61)
 // Row-form parts beyond one for each (window, key head): eight for every CU (64 tokens, four heads to a key head, 218
 // us, 512 parts: 248; over e4m3 pages 158 and 180).
@@ -350,7 +355,11 @@ __device__ __forceinline__ void bound_scores(Rows<KS>& s, f32x16_t (&x)[kHalves]
   }
 }
 
-// 32 keys' weights P^T = exp2(sl2 x - m) as B operands of the second product's two steps.
+// 32 keys' weights P^T = exp2(sl2 x - m) as B operands of the second product's two steps. They are rounded to bf16, since
+// the product runs on the bf16 matrix cores, and the row's sum is taken over the rounded weights (add_values), so that
+// what a rounding adds to the one it adds to the other: 0.0022 from 64 bits, relative, where weights in
+// fp32 leave the result's own rounding, 0.0017. m is the rounded product of a score: beyond scores of
+// 2^30 what its rounding leaves of the largest weight's exponent no longer fits fp32, and the row is NaN.
 template <int KS>
 __device__ __forceinline__ void weights_of(const Rows<KS>& s, const f32x16_t& x, float sl2, bf16x8_t (&pb)[2]) {
   const float nm = -s.m;
