@@ -128,7 +128,7 @@ def paged_append(key, value, k_pages, v_pages, page_table, lengths, cu_tokens=No
             break
         if _lib.stacked(k) or _lib.stacked(v):
             raise ValueError('pages and their exponents must have a place for every element')
-        if P and k.data_ptr() == v.data_ptr():
+        if k.data_ptr() == v.data_ptr() and k.numel():
             raise ValueError('keys and values must not share their pages or exponents')
     wide, pairs, sp, turn = 0, 0, (0, 0), _lib.SVHIP_ROTARY_NONE
     if frequencies is not None:

@@ -467,3 +467,17 @@ def test_a_capture_does_not_change_the_books(monkeypatch):
     capturing[0] = False
     ctx.grow(1)
     assert ctx.lengths.tolist() == [21, 21]
+
+
+def test_an_append_to_pages_without_heads_or_of_no_pool_writes_nothing(monkeypatch):
+    """Empty pools share the null address and nothing else: not refused for it."""
+    from streamvoxel_amd.stream import paged
+    launched = []
+    monkeypatch.setattr(_lib, 'require_one_gpu', lambda *t: None)
+    monkeypatch.setattr(_lib, 'launch', lambda *args: launched.append(args))
+    n, table = torch.ones(1, dtype=torch.int32), torch.zeros(1, 1, dtype=torch.int32)
+    for shape in ((4, 0, 16, 8), (0, 2, 16, 8)):
+        k, v = [torch.zeros(shape, dtype=torch.bfloat16) for _ in 'kv']
+        x = torch.zeros(1, shape[1], 3, 8, dtype=torch.bfloat16)
+        paged.paged_append(x, x, k, v, table, n)
+    assert len(launched) == 2
