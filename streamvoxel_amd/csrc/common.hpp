@@ -147,4 +147,16 @@ __device__ __forceinline__ int lane_id() { return __lane_id(); }
 
 __host__ __device__ __forceinline__ int64_t cdiv(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
+// Workgroups of up to 256 threads in launches of at most kLaunchGroups (a launch holds fewer than 2^32 threads; a multiple
+// of the XCDs, which a workgroup's number then names as in one launch): launch(first, count).
+constexpr int64_t kLaunchGroups = 1 << 23;
+
+template <typename Launch>
+inline void in_launches(int64_t groups, Launch launch) {
+  for (int64_t first = 0; first < groups; first += kLaunchGroups) {
+    launch(static_cast<unsigned>(first),
+           static_cast<unsigned>(groups - first < kLaunchGroups ? groups - first : kLaunchGroups));
+  }
+}
+
 }  // namespace svhip

@@ -116,11 +116,11 @@ __device__ __forceinline__ uint2 e4m3_run(const float (&x)[8], float f) {
 
 // LPR: lanes of a row (8: head_dim up to 64).
 template <int TURN, bool FP8, int LPR>
-__global__ __launch_bounds__(kAppendThreads) void paged_append_kernel(AppendArgs a) {
+__global__ __launch_bounds__(kAppendThreads) void paged_append_kernel(AppendArgs a, unsigned first_group) {
   __shared__ float2 table[kAppendTokens * kMaxPagedDim / 2];
   __shared__ int64_t s_src[kAppendTokens][2], s_page[kAppendTokens], s_pos[kAppendTokens];
   __shared__ int s_row[kAppendTokens];
-  const int64_t t0 = static_cast<int64_t>(blockIdx.x) * a.per_group;
+  const int64_t t0 = static_cast<int64_t>(first_group + blockIdx.x) * a.per_group;
   const int tokens = static_cast<int>(a.total - t0 < a.per_group ? a.total - t0 : a.per_group);
   const int tid = static_cast<int>(threadIdx.x), H = a.H;
   const int64_t mine = t0 + tid;                     // threads below `tokens`: their token, its window and place there
@@ -241,14 +241,16 @@ __global__ __launch_bounds__(kAppendThreads) void paged_append_kernel(AppendArgs
 }
 
 template <int TURN>
-void launch_append(const AppendArgs& a, unsigned grid, bool fp8, hipStream_t s) {
-  if (a.D <= 64) {
-    fp8 ? paged_append_kernel<TURN, true, 8><<<grid, kAppendThreads, 0, s>>>(a)
-        : paged_append_kernel<TURN, false, 8><<<grid, kAppendThreads, 0, s>>>(a);
-  } else {
-    fp8 ? paged_append_kernel<TURN, true, 16><<<grid, kAppendThreads, 0, s>>>(a)
-        : paged_append_kernel<TURN, false, 16><<<grid, kAppendThreads, 0, s>>>(a);
-  }
+void launch_append(const AppendArgs& a, int64_t groups, bool fp8, hipStream_t s) {
+  in_launches(groups, [&](unsigned first, unsigned grid) {
+    if (a.D <= 64) {
+      fp8 ? paged_append_kernel<TURN, true, 8><<<grid, kAppendThreads, 0, s>>>(a, first)
+          : paged_append_kernel<TURN, false, 8><<<grid, kAppendThreads, 0, s>>>(a, first);
+    } else {
+      fp8 ? paged_append_kernel<TURN, true, 16><<<grid, kAppendThreads, 0, s>>>(a, first)
+          : paged_append_kernel<TURN, false, 16><<<grid, kAppendThreads, 0, s>>>(a, first);
+    }
+  });
 }
 
 }  // namespace svhip
@@ -294,12 +296,11 @@ extern "C" int svhip_paged_append(const svhip_paged_cache* cache, const svhip_pa
                      c.pairs % (c.layout == SVHIP_ROTARY_HALF ? 8 : 4) == 0, amplitude,
                      turns ? 1.5f * (axial || most < 1.f ? 1.f : most) : 1.f};
   hipStream_t s = as_stream(stream);
-  const unsigned grid = static_cast<unsigned>(groups);
   switch (c.layout) {
-    case SVHIP_ROTARY_HALF: launch_append<kTurnHalf>(a, grid, fp8, s); break;
-    case SVHIP_ROTARY_INTERLEAVED: launch_append<kTurnInterleaved>(a, grid, fp8, s); break;
-    case SVHIP_ROTARY_AXIAL: launch_append<kTurnAxial>(a, grid, fp8, s); break;
-    default: launch_append<kTurnNone>(a, grid, fp8, s);
+    case SVHIP_ROTARY_HALF: launch_append<kTurnHalf>(a, groups, fp8, s); break;
+    case SVHIP_ROTARY_INTERLEAVED: launch_append<kTurnInterleaved>(a, groups, fp8, s); break;
+    case SVHIP_ROTARY_AXIAL: launch_append<kTurnAxial>(a, groups, fp8, s); break;
+    default: launch_append<kTurnNone>(a, groups, fp8, s);
   }
   SVHIP_LAUNCHED(name);
   return SVHIP_OK;

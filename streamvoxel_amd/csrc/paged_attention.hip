@@ -95,7 +95,7 @@ __global__ __launch_bounds__(kPlanThreads) void paged_plan_kernel(PagedArgs a, b
 constexpr int kAhead = 8;
 
 template <int kGroups>
-__global__ __launch_bounds__(kPagedThreads) void paged_join_kernel(PagedArgs a) {
+__global__ __launch_bounds__(kPagedThreads) void paged_join_kernel(PagedArgs a, unsigned first_group) {
   __shared__ float4 s_o[kGroups > 1 ? kGroups : 1][32];
   __shared__ float2 s_ml[kGroups > 1 ? kGroups : 1];
   if (a.running) {
@@ -103,7 +103,8 @@ __global__ __launch_bounds__(kPagedThreads) void paged_join_kernel(PagedArgs a) 
     if (sums.z == kUncut && sums.w == kUncut) return;  // no parts
   }
   const int group = threadIdx.x / 32, d0 = 4 * (threadIdx.x % 32);
-  const int id = static_cast<int>(kGroups > 1 ? blockIdx.x : blockIdx.x * (kPagedThreads / 32) + group);
+  const unsigned place = first_group + blockIdx.x;
+  const int id = static_cast<int>(kGroups > 1 ? place : place * (kPagedThreads / 32) + group);
   const int total = static_cast<int>(a.tokens.cu ? a.tokens.N : a.tokens.B * a.tokens.N);
   const int token = id / a.H, h = id - token * a.H;
   int64_t b = -1;
@@ -273,9 +274,11 @@ extern "C" int svhip_paged_attention(const svhip_paged_cache* cache, const svhip
   }
   if (p.plan_windows) {
     if (rows <= kJoinFew) {
-      paged_join_kernel<8><<<static_cast<unsigned>(rows), kPagedThreads, 0, s>>>(a);
+      paged_join_kernel<8><<<static_cast<unsigned>(rows), kPagedThreads, 0, s>>>(a, 0u);
     } else {
-      paged_join_kernel<1><<<static_cast<unsigned>(join), kPagedThreads, 0, s>>>(a);
+      in_launches(join, [&](unsigned first, unsigned grid) {
+        paged_join_kernel<1><<<grid, kPagedThreads, 0, s>>>(a, first);
+      });
     }
   }
   SVHIP_LAUNCHED(name);

@@ -9,14 +9,14 @@ namespace svhip {
 // both forms in turn, one tile's to one, two and four of rows: 122, 112 and 125 us, since a tile with a CU to share
 // takes no less time.
 template <bool FP8, int KS>
-__global__ __launch_bounds__(kPagedThreads, 2) void paged_mixed_kernel(PagedArgs a, int tile_grid) {
+__global__ __launch_bounds__(kPagedThreads, 2) void paged_mixed_kernel(PagedArgs a, int tile_grid, unsigned first_group) {
 #if defined(__HIP_DEVICE_COMPILE__)
   typedef RowLds<FP8, KS, 2> R;
   constexpr int kTile = TileLds<KS>::kBuffer;
   __shared__ __attribute__((aligned(16))) char s0[R::k0 > kTile ? R::k0 : kTile], s1[R::k1 > kTile ? R::k1 : kTile];
   __shared__ float s_ml[4][2][kRows];
   __shared__ int s_odd;
-  const int place = static_cast<int>(blockIdx.x);
+  const int place = static_cast<int>(first_group + blockIdx.x);
   if (place < tile_grid) {
     tile_work<FP8, false, KS>(a, place, s0, s1, &s_odd);
   } else {
@@ -27,8 +27,9 @@ __global__ __launch_bounds__(kPagedThreads, 2) void paged_mixed_kernel(PagedArgs
 
 template <bool FP8, int KS>
 void launch_mixed(const PagedArgs& a, const PagedPlan& p, hipStream_t s) {
-  paged_mixed_kernel<FP8, KS><<<static_cast<unsigned>(p.tile_grid + p.row_slots), kPagedThreads, 0, s>>>(
-      a, static_cast<int>(p.tile_grid));
+  in_launches(p.tile_grid + p.row_slots, [&](unsigned first, unsigned grid) {
+    paged_mixed_kernel<FP8, KS><<<grid, kPagedThreads, 0, s>>>(a, static_cast<int>(p.tile_grid), first);
+  });
 }
 
 void launch_paged_mixed(const PagedArgs& a, const PagedPlan& p, bool fp8, hipStream_t s) {

@@ -66,12 +66,12 @@ __device__ __forceinline__ void store_as(T* p, float v) {
 
 // VEC: an item is Run::n pairs (two runs), or one run past the pairs; else one pair, or one element.
 template <typename T, bool VEC>
-__global__ __launch_bounds__(kRotaryThreads) void rotary_kernel(RotaryArgs a) {
+__global__ __launch_bounds__(kRotaryThreads) void rotary_kernel(RotaryArgs a, unsigned first_group) {
   __shared__ float2 table[kRotaryTokens * kMaxRotaryPairs];
   constexpr int E = VEC ? Run<T>::n : 1, kAhead = VEC ? kRotaryAhead : 1;
   // (In 32 bits: a 64-bit division takes 0.3 us.)
   const unsigned N = static_cast<unsigned>(a.N), per = static_cast<unsigned>(a.tokens), tiles = (N + per - 1) / per;
-  const unsigned window = blockIdx.x / tiles, from = (blockIdx.x - window * tiles) * per;
+  const unsigned group = first_group + blockIdx.x, window = group / tiles, from = (group - window * tiles) * per;
   const int64_t b = window, n0 = from;
   const int tokens = static_cast<int>(N - from < per ? N - from : per);
   const T* x = static_cast<const T*>(a.x) + b * a.sx_b + n0 * a.sx_n;
@@ -173,12 +173,13 @@ __global__ __launch_bounds__(kRotaryThreads) void rotary_kernel(RotaryArgs a) {
 
 template <typename T>
 void launch_rotary(const RotaryArgs& a, bool vec, hipStream_t s) {
-  const unsigned grid = static_cast<unsigned>(a.B * cdiv(a.N, a.tokens));
-  if (vec) {
-    rotary_kernel<T, true><<<grid, kRotaryThreads, 0, s>>>(a);
-  } else {
-    rotary_kernel<T, false><<<grid, kRotaryThreads, 0, s>>>(a);
-  }
+  in_launches(a.B * cdiv(a.N, a.tokens), [&](unsigned first, unsigned grid) {
+    if (vec) {
+      rotary_kernel<T, true><<<grid, kRotaryThreads, 0, s>>>(a, first);
+    } else {
+      rotary_kernel<T, false><<<grid, kRotaryThreads, 0, s>>>(a, first);
+    }
+  });
 }
 
 }  // namespace svhip

@@ -1055,3 +1055,52 @@ def test_books_do_not_change_in_a_capture():
         torch.cuda.synchronize()
         assert torch.equal(out, want) and ctx.lengths.tolist() == ctx.host_lengths == [5, 5] and ctx.free_pages == 4
         ctx.grow(0)
+
+
+def test_append_of_more_tokens_than_one_launch_holds():
+    """More than 2^24 workgroups, which no launch of 256 threads each holds."""
+    from streamvoxel_amd.stream.paged import paged_append
+    T = (1 << 27) + 9
+    pages = -(-T // 1024)
+    key = torch.randn(1, 1, T, 8, device=DEV, generator=torch.Generator(DEV).manual_seed(1), dtype=torch.bfloat16)
+    k, v = [torch.zeros(pages, 1, 1024, 8, dtype=torch.bfloat16, device=DEV) for _ in 'kv']
+    table = torch.arange(pages, dtype=torch.int32, device=DEV)[None]
+    paged_append(key, key, k, v, table, torch.tensor([T], dtype=torch.int32, device=DEV))
+    for t in (k, v):
+        assert torch.equal(t.view(-1, 8)[:T], key[0, 0]) and not t.view(-1, 8)[T:].any()
+
+
+@pytest.mark.parametrize('n', [1, 5])
+def test_attention_of_more_windows_than_one_launch_holds(n):
+    """More than 2^24 workgroups of either form, all windows over one page."""
+    from streamvoxel_amd.stream.paged import paged_attention
+    B, D = (1 << 24) + 3, 8
+    g = torch.Generator(DEV).manual_seed(n)
+    q = torch.randn(B, 1, n, D, device=DEV, generator=g, dtype=torch.bfloat16)
+    k, v = [torch.randn(1, 1, 16, D, device=DEV, generator=g, dtype=torch.bfloat16) for _ in 'kv']
+    lengths = torch.randint(0, 17, (B,), device=DEV, generator=g, dtype=torch.int32)
+    got = paged_attention(q, k, v, torch.zeros(1, 1, dtype=torch.int32, device=DEV).expand(B, 1), lengths)
+    for L in range(17):
+        mine = (lengths == L).nonzero()[:, 0]
+        out, err = attend64(q[mine].view(1, -1, D).double(), k[0, :, :L].double(), v[0, :, :L].double(), False, D ** -0.5)
+        assert ((got[mine].view(1, -1, D).double() - out).abs() <= err).all(), L
+
+
+def test_a_join_of_more_rows_than_one_launch_holds():
+    """2^27 rows of a window without keys, and behind them a window whose keys are cut: its parts are joined."""
+    from streamvoxel_amd.stream.paged import paged_attention
+    H, D, first, last, L = 128, 8, 1 << 20, 200, 100000
+    g = torch.Generator(DEV).manual_seed(1)
+    q = torch.randn(first + last, H, D, device=DEV, generator=g, dtype=torch.bfloat16).transpose(0, 1)
+    pages = -(-L // 1024)
+    k, v = [torch.randn(pages, 1, 1024, D, device=DEV, generator=g, dtype=torch.bfloat16) for _ in 'kv']
+    table = torch.arange(pages, dtype=torch.int32, device=DEV).expand(2, pages)
+    out = torch.full_like(q, math.nan)
+    paged_attention(q, k, v, table, torch.tensor([0, L], dtype=torch.int32, device=DEV), out=out,
+                    cu_queries=torch.tensor([0, first, first + last], dtype=torch.int32, device=DEV))
+    assert not out[:, :first].any()
+    rows = [t.reshape(1, -1, D)[:, :L].double().cpu() for t in (k, v)]
+    for at in (0, 100, last - 2):
+        cut = slice(first + at, first + at + 2)
+        want, err = attend64(q[:, cut].cpu().double(), *rows, False, D ** -0.5)
+        assert ((out[:, cut].cpu().double() - want).abs() <= err).all(), at

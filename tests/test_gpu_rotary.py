@@ -219,3 +219,20 @@ def test_rotary_in_forward_mode(layout, dtype):
             check(y.tangent, t, positions, f, layout, 1.5)
         with pytest.raises(ValueError, match='gradient'):
             rotary(fw.make_dual(x, t), positions, f, out=torch.empty_like(x))
+
+
+def test_rotary_of_more_windows_than_one_launch_holds():
+    """More than 2^24 workgroups, which no launch of 256 threads each holds; against the formula on the GPU."""
+    from streamvoxel_amd.stream.rotary import rotary
+    B = (1 << 24) + 5
+    x = torch.randn(B, 1, 1, 8, device=DEV, generator=torch.Generator(DEV).manual_seed(1))
+    positions = torch.arange(B, dtype=torch.int32, device=DEV)[:, None]
+    f = freqs(4)
+    got = rotary(x, positions, f)
+    for at in range(0, B, 1 << 22):
+        cut = slice(at, at + (1 << 22))
+        angle = (positions[cut].double() * f)[:, None, None]
+        a, b = x[cut].double().chunk(2, -1)
+        y = torch.cat((a * angle.cos() - b * angle.sin(), b * angle.cos() + a * angle.sin()), -1)
+        err = 8 * 2.0 ** -24 * (a.abs() + b.abs()).repeat(1, 1, 1, 2)
+        assert ((got[cut].double() - y).abs() <= err + 2.0 ** -24 * (y.abs() + err)).all(), at
