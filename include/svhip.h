@@ -23,8 +23,17 @@
 extern "C" {
 #endif
 
-/* SVHIP_FP8_E4M3_PFP8: e4m3 K/V whose attention rounds P to e4m3 for the fp8 matrix cores (see svhip_xattn_fwd). */
-enum svhip_dtype { SVHIP_F32 = 0, SVHIP_BF16 = 1, SVHIP_FP8_E4M3 = 3, SVHIP_FP8_E4M3_PFP8 = 5 };
+/* SVHIP_FP8_E4M3_PFP8: e4m3 K/V whose attention rounds P to e4m3 for the fp8 matrix cores (see svhip_xattn_fwd).
+ * SVHIP_INT8_BLOCK16, 32, 64: int8 pages with a power of two for every so many keys (see svhip_paged_cache). */
+enum svhip_dtype {
+  SVHIP_F32 = 0,
+  SVHIP_BF16 = 1,
+  SVHIP_FP8_E4M3 = 3,
+  SVHIP_FP8_E4M3_PFP8 = 5,
+  SVHIP_INT8_BLOCK16 = 16,
+  SVHIP_INT8_BLOCK32 = 17,
+  SVHIP_INT8_BLOCK64 = 18
+};
 
 enum svhip_status { SVHIP_OK = 0, SVHIP_EINVAL = -1, SVHIP_ELAUNCH = -2, SVHIP_EWORKSPACE = -3 };
 
@@ -449,14 +458,43 @@ typedef struct svhip_rotary_args {
 int svhip_rotary(const svhip_rotary_args* args, void* stream);
 
 /*
+ * Queries and keys normed for each head and turned, in one pass: row x of D elements becomes
+ *   R(p) (w x / sqrt(mean x^2 + eps)),
+ * R(p) the rotation of svhip_rotary by the row's position (its layouts, pairs, freq, positions and amplitude), w fp32 or
+ * bf16 [D] (weight_dtype), one for all heads of the queries and one for the keys (null: ones). fp32 throughout (squares of a
+ * row must not pass its range), rounded once to the type. q [B, H, N, D] and k [B, Hk, N, D] share the positions; element (b, h,
+ * n, d) at b*s_b + h*s_h + n*s_n + d; out_q may be q with the same strides, out_k k; H or Hk may be 0. D from 2 to 256.
+ * svhip_norm_rotary_grad: from dq, dk, the gradients of the results, those of q and k into out_q, out_k (null: not wanted)
+ * and of the weights into dq_weight, dk_weight (weight_dtype; null: not wanted), summed over the rows in an order that the sizes
+ * alone set; workspace: svhip_norm_rotary_workspace_bytes (none without the weights' gradients), 4-byte aligned. (svhip_norm_rotary
+ * reads neither.) Beside svhip_rotary; no counterpart in the reference.
+ */
+typedef struct svhip_norm_rotary_args {
+  const void *q, *k, *dq, *dk, *q_weight, *k_weight;
+  void *out_q, *out_k, *dq_weight, *dk_weight;
+  const void* positions;
+  const double* freq;
+  void* workspace;
+  int64_t workspace_bytes, dtype, weight_dtype, positions_wide, pairs, layout;
+  int64_t B, H, Hk, N, D, sq_b, sq_h, sq_n, sk_b, sk_h, sk_n, sdq_b, sdq_h, sdq_n, sdk_b, sdk_h, sdk_n;
+  int64_t soq_b, soq_h, soq_n, sok_b, sok_h, sok_n, sp_b, sp_n;
+  double amplitude, eps;
+} svhip_norm_rotary_args;
+int svhip_norm_rotary(const svhip_norm_rotary_args* args, void* stream);
+size_t svhip_norm_rotary_workspace_bytes(int64_t B, int64_t N, int64_t D);
+int svhip_norm_rotary_grad(const svhip_norm_rotary_args* args, void* stream);
+
+/*
  * A paged cache: pools k_pages, v_pages of `pages` pages, element (page, h, r, d) at page*s_p + h*s_h + r*s_r + d,
  * rows r in [0, page_size), page_size a power of two from 16 to 1024, head_dim a multiple of 8 up to 128, rows
- * 16-byte aligned (e4m3: 8; a stride counts where its dimension has more than one element, here and below), max_pages *
+ * 16-byte aligned (codes of 8 bits: 8; a stride counts where its dimension has more than one element, here and below), max_pages *
  * page_size at most 2^30. Key j of window b is row j % page_size of page
  * page_table[b*table_stride + j / page_size] (int32, max_pages numbers a window); lengths[b] (int32) counts the
  * window's keys. kv_dtype SVHIP_BF16, or SVHIP_FP8_E4M3: OCP e4m3fn codes with one power of two for each row and
- * head, value = code 2^(exponent - 127), exponents 1 to 254, bytes (page, h, r) at page*se_p + h*se_h + r. Windows may share
- * pages that are only read. `bad` (int32, may be null) is set to 1 by a call that meets a page outside the pool or
+ * head, value = code 2^(exponent - 127), exponents 1 to 254, bytes (page, h, r) at page*se_p + h*se_h + r; or
+ * SVHIP_INT8_BLOCK16 / 32 / 64: codes of -127 to 127 with one power of two, exponents 1 to 248, for each head and block of so
+ * many rows of a page (no more than a page has), bytes (page, h, r / block) at page*se_p + h*se_h + r / block. Windows may
+ * share pages that are only read. `bad` (int32, may be null) is set to 1 by a call that meets a page outside the pool or
  * a key outside its window's row of the table.
  */
 typedef struct svhip_paged_cache {
@@ -477,7 +515,12 @@ typedef struct svhip_paged_cache {
  * at b*sp_b + n*sp_n, or null: the key's index), SVHIP_ROTARY_AXIAL with svhip_axial_rope's arithmetic (positions
  * fp32, three a token; freq fp32 [head_dim / 6]; pairs = head_dim / 2). e4m3: a row's exponent is the least with
  * bound <= 448 2^(exponent - 127), bound = its largest magnitude, for rotated keys 1.5 max(1, |amplitude|) times it
- * before the rotation. A token whose key or page is bad is not written. Key and value rows bf16, 16-byte aligned.
+ * before the rotation. int8: a block's exponent is the least, 1 to 248, with every magnitude <= 127 2^(exponent - 127), of
+ * the block's new rows (rotated, in fp32), and not below the one it has if rows in front of them, of the same window, are in
+ * the block: those codes are then divided by the power of two that the exponent grew by, rounded to nearest even, as new ones
+ * are. A block's rows are written in order: what stands behind the new rows (`before`) is yet to be written. Infinities count as the
+ * largest magnitude, NaN as 0, and set `bad`. A token whose key or page is bad is not written. Key and value rows bf16,
+ * 16-byte aligned.
  * Beside svhip_kv_write (FastSlotForward.encode + _write, streamvoxel/stream/fast_ops.py:228-250), which rewrites a
  * window's slab whole; no counterpart in the reference.
  */
@@ -490,6 +533,21 @@ typedef struct svhip_paged_append_args {
   double amplitude;
 } svhip_paged_append_args;
 int svhip_paged_append(const svhip_paged_cache* cache, const svhip_paged_append_args* args, void* stream);
+
+/*
+ * Reads keys and values back as bf16 rows: of window b the N keys in front of its last `before`, or with cu_keys (int32
+ * [windows + 1], ascending) the cu[b + 1] - cu[b] in front of them, as packed rows [cu[b], cu[b + 1]) of N in all: what a
+ * svhip_paged_append with the same tokens wrote. Key lengths[b] - before - n + i goes to row i of n, element (b, h, i, d) at
+ * b*s_b + h*s_h + i*s_n + d (packed: s_b unused). Codes are decoded exactly. A key that does not exist (an index below 0, one
+ * outside the window's row of the table or on a bad page: these two set `bad`) is a row of zeros; rows outside every window
+ * are left as they are. Rows 16-byte aligned. No counterpart in the reference.
+ */
+typedef struct svhip_paged_read_args {
+  void *key, *value;
+  const int32_t* cu_keys;
+  int64_t N, before, sk_b, sk_h, sk_n, sv_b, sv_h, sv_n;
+} svhip_paged_read_args;
+int svhip_paged_read(const svhip_paged_cache* cache, const svhip_paged_read_args* args, void* stream);
 
 /*
  * Attention of the windows' new tokens over a paged cache: out[b, h, i] = softmax_j(scale q[b, h, i] . k_j) v_j
@@ -515,6 +573,14 @@ typedef struct svhip_paged_attention_args {
 size_t svhip_paged_attention_workspace_bytes(int64_t B, int64_t H, int64_t Hkv, int64_t N, int packed, int64_t D,
                                              int64_t max_keys);
 int svhip_paged_attention(const svhip_paged_cache* cache, const svhip_paged_attention_args* args, void* stream);
+
+/*
+ * svhip_paged_attention through a sliding window: the token at key p sees keys p - window + 1 to p and the first `sinks`
+ * keys (those up to p). causal must be set; window >= 1, sinks >= 0. The keys in between are not read; workspace as there. No
+ * counterpart in the reference.
+ */
+int svhip_paged_window_attention(const svhip_paged_cache* cache, const svhip_paged_attention_args* args, int64_t window,
+                                 int64_t sinks, void* stream);
 
 #ifdef __cplusplus
 }

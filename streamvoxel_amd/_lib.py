@@ -15,6 +15,7 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(HERE, 'libsvhip.so')
 
 SVHIP_F32, SVHIP_BF16, SVHIP_FP8_E4M3, SVHIP_FP8_E4M3_PFP8 = 0, 1, 3, 5
+SVHIP_INT8_BLOCK = {16: 16, 32: 17, 64: 18}    # keys that share an exponent -> the code
 SVHIP_ROTARY_NONE, SVHIP_ROTARY_HALF, SVHIP_ROTARY_INTERLEAVED, SVHIP_ROTARY_AXIAL = 0, 1, 2, 3
 SVHIP_LEL_LAYER, SVHIP_LEL_BAND, SVHIP_LEL_COLUMN = 0, 1, 2
 
@@ -87,6 +88,11 @@ SIGNATURES = {
     'svhip_paged_append': (ctypes.c_int, [_c_b, _c_b, _c_p]),
     'svhip_paged_attention_workspace_bytes': (_c_sz, [_c_i64] * 4 + [ctypes.c_int] + [_c_i64] * 2),
     'svhip_paged_attention': (ctypes.c_int, [_c_b, _c_b, _c_p]),
+    'svhip_paged_window_attention': (ctypes.c_int, [_c_b, _c_b, _c_i64, _c_i64, _c_p]),
+    'svhip_paged_read': (ctypes.c_int, [_c_b, _c_b, _c_p]),
+    'svhip_norm_rotary': (ctypes.c_int, [_c_b, _c_p]),
+    'svhip_norm_rotary_workspace_bytes': (_c_sz, [_c_i64] * 3),
+    'svhip_norm_rotary_grad': (ctypes.c_int, [_c_b, _c_p]),
 }
 
 _lib = None

@@ -17,8 +17,9 @@ LIB = os.path.join(HERE, 'libsvhip.so')
 ARCH = os.environ.get('SVHIP_ARCH', 'gfx950')
 
 SOURCES = ['api.hip', 'entropy.hip', 'select.hip', 'xattn.hip', 'xattn_split.hip', 'xattn_split_wide.hip', 'xattn_f32.hip',
-           'producer.hip', 'norm.hip', 'embed.hip', 'sample.hip', 'rotary.hip', 'paged_append.hip', 'paged_attention.hip',
-           'paged_tile.hip', 'paged_row.hip', 'paged_mixed.hip']
+           'producer.hip', 'norm.hip', 'embed.hip', 'sample.hip', 'rotary.hip', 'norm_rotary.hip', 'paged_append.hip',
+           'paged_append_int8.hip', 'paged_read.hip', 'paged_attention.hip',
+           *(f'paged_{form}{kind}.hip' for form in ('tile', 'row', 'mixed') for kind in ('', '_window', '_int8'))]
 
 FLAGS = [
     '-O3', '-std=c++17', '-fPIC', '-shared', f'--offload-arch={ARCH}',

@@ -1,7 +1,11 @@
 // A paged cache of keys and values: key j of window b is row j % S of page table[b][j / S] of a pool [pages, H, S,
 // D], S a power of two. bf16 rows, or OCP e4m3fn rows with one power of two for each row and head, held as its
 // exponent's byte (value = code 2^(byte - 127)): scaling by it is exact, so an e4m3 row decodes to bf16 without a
-// second rounding and the row's scale takes part in neither product of the attention.
+// second rounding and the row's scale takes part in neither product of the attention. Or int8 rows with one power of
+// two for every block of 16, 32 or 64 rows and head: 7 bits of magnitude, which bf16 holds as well. A power of two also
+// where a scale is shared, since a block fills as keys come: where it must grow, the codes that are there halve, and what
+// their roundings add up to stays under one step of the new scale (1/2 + 1/4 + ...); scales that grow by less leave codes
+// where they are while what they stand for grows (0.99 * 40 rounds to 40, again and again).
 #pragma once
 
 #include "common.hpp"
@@ -11,6 +15,11 @@ namespace svhip {
 constexpr int kMinPage = 16;
 constexpr int kMaxPage = 1024;
 constexpr int kMaxPagedDim = 128;
+
+// How a pool holds its rows.
+enum Store { kBf16 = 0, kE4m3 = 1, kInt8 = 2 };
+__host__ __device__ constexpr bool coded(int store) { return store != kBf16; }
+__host__ __device__ constexpr int bytes_of(int store) { return coded(store) ? 1 : 2; }
 
 struct Pages {
   const int32_t* table;   // [B, max_pages], rows st_b apart
@@ -83,24 +92,54 @@ __device__ __forceinline__ int row_exponent(float bound) {
 
 __device__ __forceinline__ float exponent_value(int code) { return __uint_as_float(static_cast<uint32_t>(code) << 23); }
 
+// int8 blocks: whole numbers of at most kInt8Most times a power of two of at most 2^(kInt8Top - 127), the largest of them
+// with 127 of it in bf16. (A larger byte is read as that: a code's value is then finite whatever stands there.)
+constexpr int kInt8Top = 248;
+constexpr float kInt8Most = 127.f;
+__device__ __forceinline__ float int8_power(uint32_t byte) {
+  return exponent_value(static_cast<int>(byte < static_cast<uint32_t>(kInt8Top) ? byte : kInt8Top));
+}
+
+// 8 int8 codes times a power of two f as bf16: 7 bits of magnitude, exact.
+__device__ __forceinline__ uint4 int8_values(uint2 w, float f) {
+  float x[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) x[i] = static_cast<float>(static_cast<int8_t>((i < 4 ? w.x : w.y) >> 8 * (i & 3))) * f;
+  return make_uint4(bf16_pack2(x[0], x[1]), bf16_pack2(x[2], x[3]), bf16_pack2(x[4], x[5]), bf16_pack2(x[6], x[7]));
+}
+
 inline int page_shift(int64_t page) {
   int s = 0;
   while ((1ll << s) < page) ++s;
   return s;
 }
 
-// What both calls ask of a cache; the status of the first check that fails.
+// The storage that a dtype code names, or -1; and log2 of the keys of an int8 block.
+inline int store_of(int64_t kv_dtype) {
+  switch (kv_dtype) {
+    case SVHIP_BF16: return kBf16;
+    case SVHIP_FP8_E4M3: return kE4m3;
+    case SVHIP_INT8_BLOCK16: case SVHIP_INT8_BLOCK32: case SVHIP_INT8_BLOCK64: return kInt8;
+    default: return -1;
+  }
+}
+inline int block_shift(int64_t kv_dtype) {
+  return kv_dtype == SVHIP_INT8_BLOCK64 ? 6 : (kv_dtype == SVHIP_INT8_BLOCK32 ? 5 : 4);
+}
+
+// What the calls ask of a cache; the status of the first check that fails.
 inline int check_cache(const char* name, const svhip_paged_cache* cache) {
   SVHIP_REQUIRE(cache, "%s: null cache", name);
   const svhip_paged_cache& c = *cache;
   SVHIP_REQUIRE(c.windows >= 0 && c.windows < (1ll << 31) && c.heads >= 0 && c.heads <= 1 << 20, "%s: bad sizes", name);
   SVHIP_REQUIRE(c.head_dim >= 8 && c.head_dim <= kMaxPagedDim && c.head_dim % 8 == 0,
                 "%s: head_dim %lld unsupported (a multiple of 8 up to %d)", name, (long long)c.head_dim, kMaxPagedDim);
-  SVHIP_REQUIRE(c.kv_dtype == SVHIP_BF16 || c.kv_dtype == SVHIP_FP8_E4M3, "%s: kv dtype %d unsupported", name,
-                (int)c.kv_dtype);
+  SVHIP_REQUIRE(store_of(c.kv_dtype) >= 0, "%s: kv dtype %d unsupported", name, (int)c.kv_dtype);
   SVHIP_REQUIRE(c.page_size >= kMinPage && c.page_size <= kMaxPage && (c.page_size & (c.page_size - 1)) == 0,
                 "%s: page size %lld unsupported (a power of two, %d to %d)", name, (long long)c.page_size, kMinPage,
                 kMaxPage);
+  SVHIP_REQUIRE(store_of(c.kv_dtype) != kInt8 || 1 << block_shift(c.kv_dtype) <= c.page_size,
+                "%s: a block of %d keys does not fit a page of %lld", name, 1 << block_shift(c.kv_dtype), (long long)c.page_size);
   SVHIP_REQUIRE(c.pages >= 0 && c.pages < (1ll << 31) && c.max_pages >= 0 && c.max_pages <= (1ll << 30) / c.page_size,
                 "%s: bad page counts", name);  // (keys and a few blocks of them further on are counted in 32 bits)
   return SVHIP_OK;
@@ -108,11 +147,11 @@ inline int check_cache(const char* name, const svhip_paged_cache* cache) {
 
 // The checks of a cache that a call touches.
 inline int check_pool(const char* name, const svhip_paged_cache& c) {
-  const bool fp8 = c.kv_dtype == SVHIP_FP8_E4M3;
+  const bool codes = coded(store_of(c.kv_dtype));
   SVHIP_REQUIRE(c.pages >= 1, "%s: a pool needs a page", name);
   SVHIP_REQUIRE(c.lengths && (c.max_pages == 0 || c.page_table) && c.k_pages && c.v_pages, "%s: null pointer", name);
-  SVHIP_REQUIRE(!fp8 || (c.k_exponents && c.v_exponents), "%s: e4m3 pages need the rows' exponents", name);
-  const uintptr_t bytes = fp8 ? 8 : 16;
+  SVHIP_REQUIRE(!codes || (c.k_exponents && c.v_exponents), "%s: e4m3 pages need the rows' exponents, int8 pages the blocks'", name);
+  const uintptr_t bytes = codes ? 8 : 16;
   const int64_t sk_p = used_stride(c.pages, c.sk_p), sv_p = used_stride(c.pages, c.sv_p);
   const int64_t sk_h = used_stride(c.heads, c.sk_h), sv_h = used_stride(c.heads, c.sv_h);
   SVHIP_REQUIRE(reinterpret_cast<uintptr_t>(c.k_pages) % bytes == 0 && reinterpret_cast<uintptr_t>(c.v_pages) % bytes == 0 &&

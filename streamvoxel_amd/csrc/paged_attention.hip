@@ -25,14 +25,14 @@
 // Staging: 16 keys lie in one page (pages are of 16 keys or more), so the wave's load of 8 rows has one base, a
 // scalar buffer descriptor whose bound is the number of its keys that exist: keys past the window's end, bad pages
 // and the chunks past head_dim read as zeros and nothing is read outside a page.
-#include "paged_row.hpp"
-#include "paged_tile.hpp"
+#include "paged_mixed.hpp"
 
 namespace svhip {
 
 // The plan of more windows than a wave has lanes, by one workgroup: part lengths, and every window's places in the
 // lists of row-form parts and of tiles. (Up to 64 windows a workgroup's own plan is one load a lane, less than this
 // launch.)
+template <bool WIN>
 __global__ __launch_bounds__(kPlanThreads) void paged_plan_kernel(PagedArgs a, bool rows, bool tiles) {
   __shared__ float of_wave[kPlanThreads / 64];
   __shared__ int4 counts[kPlanThreads / 64];
@@ -40,20 +40,20 @@ __global__ __launch_bounds__(kPlanThreads) void paged_plan_kernel(PagedArgs a, b
   const int tid = static_cast<int>(threadIdx.x), Hkv = a.Hkv;
   int unused, more;
   float total;
-  const int row_each = rows && a.row_part ? row_length(a, team, 0, unused) : kUncut;
-  const int tile_each = tiles ? tile_length(a, team, unused, more, total) : kUncut;
+  const int row_each = rows && a.row_part ? row_length<WIN>(a, team, 0, unused) : kUncut;
+  const int tile_each = tiles ? tile_length<WIN>(a, team, unused, more, total) : kUncut;
   int2 at = make_int2(0, 0), slot = at;
   int cut = 0;  // 1: windows of the row form, 2: tiles
   for (int64_t c0 = 0; c0 < a.tokens.B; c0 += kPlanThreads) {
     const int64_t c = c0 + tid;
     int row = 0, tile = 0, parts = 1, t = 0, blocks = 0;
     if (c < a.tokens.B) {
-      if (tiles) tiles_of_window(a, c, t, blocks);
+      if (tiles) tiles_of_window<WIN>(a, c, t, blocks);
       if (t > 0) {
         parts = tile_parts(blocks, tile_each);
         tile = t * Hkv * parts;
       } else if (rows) {
-        parts = row_parts(row_keys(a, c), row_each);
+        parts = row_parts(row_keys<WIN>(a, c), row_each);
         row = Hkv * parts;
       }
     }
@@ -94,7 +94,7 @@ __global__ __launch_bounds__(kPlanThreads) void paged_plan_kernel(PagedArgs a, b
 // at once).
 constexpr int kAhead = 8;
 
-template <int kGroups>
+template <int kGroups, bool WIN>
 __global__ __launch_bounds__(kPagedThreads) void paged_join_kernel(PagedArgs a, unsigned first_group) {
   __shared__ float4 s_o[kGroups > 1 ? kGroups : 1][32];
   __shared__ float2 s_ml[kGroups > 1 ? kGroups : 1];
@@ -140,7 +140,7 @@ __global__ __launch_bounds__(kPagedThreads) void paged_join_kernel(PagedArgs a, 
     step = static_cast<int64_t>(a.slot_rows) * (a.D + 2);
   } else {
     if (!a.split) return;
-    const int qt = r / kTileRows, blocks = (tile_keys(a, w, qt) + kKB - 1) / kKB;
+    const int qt = r / kTileRows, blocks = (tile_keys(a, w, qt) - tile_left_out<WIN>(a, w, qt) + kKB - 1) / kKB;
     const int each = plan.z, tiles = plan.w;
     if (each < 1) return set_bad(a.pages);
     count = blocks > each ? (blocks - 1) / each + 1 : 1;
@@ -196,7 +196,7 @@ __global__ __launch_bounds__(kPagedThreads) void paged_join_kernel(PagedArgs a, 
     }
   }
   if (d0 >= a.D) return;
-  const float inv = last_key(a, w, i) >= 0 ? 1.f / l : 0.f;
+  const float inv = sees_any<WIN>(a, w, i) ? 1.f / l : 0.f;
   uint16_t* out = a.o + row_at(a, w, b, h, i, a.so_b, a.so_h, a.so_n);
   *reinterpret_cast<uint2*>(out + d0) = make_uint2(bf16_pack2(o[0] * inv, o[1] * inv), bf16_pack2(o[2] * inv, o[3] * inv));
 }
@@ -204,6 +204,86 @@ __global__ __launch_bounds__(kPagedThreads) void paged_join_kernel(PagedArgs a, 
 // Rows up to which a row has a workgroup of its own (one token, 12 rows: 15.8 us, 25.7 without; 64 tokens, 1024 rows:
 // 217.6 and 222.9; 32 768 rows in two parts: 323 with, 281 without; 16 304 rows 116 and 104).
 constexpr int64_t kJoinFew = 4096;
+
+// The forms' kernels by storage and window.
+template <bool WIN>
+void launch_paged(const PagedArgs& a, const PagedPlan& p, int store, bool whole, int64_t rows, hipStream_t s) {
+  if (p.planned) paged_plan_kernel<WIN><<<1, kPlanThreads, 0, s>>>(a, p.rows, p.tiles);
+  if (p.rows && p.tiles) {
+    store == kInt8 ? launch_paged_mixed<kInt8, WIN>(a, p, s)
+                   : (store == kE4m3 ? launch_paged_mixed<kE4m3, WIN>(a, p, s) : launch_paged_mixed<kBf16, WIN>(a, p, s));
+  } else if (p.rows) {
+    store == kInt8 ? launch_paged_rows<kInt8, WIN>(a, p, s)
+                   : (store == kE4m3 ? launch_paged_rows<kE4m3, WIN>(a, p, s) : launch_paged_rows<kBf16, WIN>(a, p, s));
+  } else {
+    store == kInt8 ? launch_paged_tiles<kInt8, WIN>(a, p, whole, s)
+                   : (store == kE4m3 ? launch_paged_tiles<kE4m3, WIN>(a, p, whole, s)
+                                     : launch_paged_tiles<kBf16, WIN>(a, p, whole, s));
+  }
+  if (!p.plan_windows) return;
+  if (rows <= kJoinFew) {
+    paged_join_kernel<8, WIN><<<static_cast<unsigned>(rows), kPagedThreads, 0, s>>>(a, 0u);
+  } else {
+    in_launches(cdiv(rows, kPagedThreads / 32), [&](unsigned first, unsigned grid) {
+      paged_join_kernel<1, WIN><<<grid, kPagedThreads, 0, s>>>(a, first);
+    });
+  }
+}
+
+// window 0: none.
+int paged_attention(const char* name, const svhip_paged_cache* cache, const svhip_paged_attention_args* args, int64_t window,
+                    int64_t sinks, void* stream) {
+  if (const int rc = check_cache(name, cache)) return rc;
+  SVHIP_REQUIRE(args, "%s: null arguments", name);
+  const svhip_paged_cache& pc = *cache;
+  const svhip_paged_attention_args& c = *args;
+  const int64_t B = pc.windows, H = c.H, Hkv = pc.heads, N = c.N, D = pc.head_dim;
+  SVHIP_REQUIRE(H >= 0 && H <= 1 << 20 && N >= 0 && N < (1ll << 31) && N * H < (1ll << 40), "%s: bad sizes", name);
+  SVHIP_REQUIRE(Hkv >= 1 && H % Hkv == 0, "%s: %lld heads do not share %lld key heads evenly", name, (long long)H,
+                (long long)Hkv);
+  const float scale = static_cast<float>(c.scale);
+  SVHIP_REQUIRE(scale > 0.f && scale < INFINITY, "%s: scale must be positive and finite", name);
+  SVHIP_REQUIRE(window == 0 || c.causal, "%s: a window slides with the tokens: it needs causal", name);
+  if (B == 0 || H == 0 || N == 0) return SVHIP_OK;
+  if (const int rc = check_pool(name, pc)) return rc;
+  SVHIP_REQUIRE(c.q && c.out, "%s: null pointer", name);
+  const int64_t even = c.cu_queries ? 0 : B;
+  SVHIP_REQUIRE(rows_on(8, c.q, even, H, N, c.sq_b, c.sq_h, c.sq_n), "%s: query rows must start on 16-byte boundaries", name);
+  SVHIP_REQUIRE(rows_on(4, c.out, even, H, N, c.so_b, c.so_h, c.so_n),
+                "%s: rows of out must start on 8-byte boundaries", name);
+  const int store = store_of(pc.kv_dtype);
+  const int row_most = coded(store) ? kRowMostFp8 : kRowMost;
+  window = window < kUncut ? window : kUncut;  // (no more keys than that)
+  sinks = sinks < kUncut ? sinks : kUncut;
+  const int64_t held = pc.max_pages * pc.page_size;
+  const PagedPlan p = paged_plan(B, H, Hkv, N, c.cu_queries != nullptr, D, window > 0 ? window_keys(held, window, sinks) : held,
+                                 row_most);
+  SVHIP_REQUIRE(p.bytes() == 0 || (c.workspace && c.workspace_bytes >= static_cast<int64_t>(p.bytes()) &&
+                                   reinterpret_cast<uintptr_t>(c.workspace) % 16 == 0),
+                "%s: workspace too small or misaligned (%lld < %zu bytes)", name, (long long)c.workspace_bytes, p.bytes());
+  const int64_t rows = (c.cu_queries ? N : B * N) * H;
+  SVHIP_REQUIRE(p.row_slots + p.tile_grid < (1ll << 31) && rows < (1ll << 31) - kPagedThreads &&
+                    N * (H / Hkv) < (1ll << 31) - kPagedThreads, "%s: sizes too large", name);
+  const int64_t es = bytes_of(store);
+  float* const part = static_cast<float*>(c.workspace);
+  int4* const plan = reinterpret_cast<int4*>(part + p.row_floats + p.tile_floats);
+  const PagedArgs a{static_cast<const uint16_t*>(c.q), pc.k_pages, pc.v_pages, pc.k_exponents, pc.v_exponents,
+                    static_cast<uint16_t*>(c.out), Tokens{c.cu_queries, B, N}, pages_of(pc),
+                    static_cast<int>(H), static_cast<int>(Hkv), static_cast<int>(H / Hkv), static_cast<int>(D), c.sq_b,
+                    c.sq_h, c.sq_n, pc.sk_h, pc.sv_h, pc.sek_h, pc.sev_h, c.so_b, c.so_h, c.so_n,
+                    static_cast<uint32_t>(pc.sk_p * es), static_cast<uint32_t>(pc.sk_r * es),
+                    static_cast<uint32_t>(pc.sv_p * es), static_cast<uint32_t>(pc.sv_r * es),
+                    static_cast<uint32_t>(pc.sek_p), static_cast<uint32_t>(pc.sev_p), c.causal != 0,
+                    scale * kLog2e, row_most, p.q_tiles, p.split, static_cast<int>(p.row_slots), static_cast<int>(p.tile_slots),
+                    static_cast<int>(p.slot_rows), p.row_parts ? part : nullptr, part + p.row_floats,
+                    p.plan_windows ? plan : nullptr, p.planned ? reinterpret_cast<int2*>(plan + B + 1) : nullptr,
+                    block_shift(pc.kv_dtype), static_cast<int>(window), static_cast<int>(sinks)};
+  const bool whole = pc.page_size >= kWholePages;
+  hipStream_t s = as_stream(stream);
+  window > 0 ? launch_paged<true>(a, p, store, whole, rows, s) : launch_paged<false>(a, p, store, whole, rows, s);
+  SVHIP_LAUNCHED(name);
+  return SVHIP_OK;
+}
 
 }  // namespace svhip
 
@@ -222,65 +302,14 @@ extern "C" size_t svhip_paged_attention_workspace_bytes(int64_t B, int64_t H, in
 
 extern "C" int svhip_paged_attention(const svhip_paged_cache* cache, const svhip_paged_attention_args* args,
                                      void* stream) {
-  const char* name = "svhip_paged_attention";
   clear_error();
-  if (const int rc = check_cache(name, cache)) return rc;
-  SVHIP_REQUIRE(args, "%s: null arguments", name);
-  const svhip_paged_cache& pc = *cache;
-  const svhip_paged_attention_args& c = *args;
-  const int64_t B = pc.windows, H = c.H, Hkv = pc.heads, N = c.N, D = pc.head_dim;
-  SVHIP_REQUIRE(H >= 0 && H <= 1 << 20 && N >= 0 && N < (1ll << 31) && N * H < (1ll << 40), "%s: bad sizes", name);
-  SVHIP_REQUIRE(Hkv >= 1 && H % Hkv == 0, "%s: %lld heads do not share %lld key heads evenly", name, (long long)H,
-                (long long)Hkv);
-  const float scale = static_cast<float>(c.scale);
-  SVHIP_REQUIRE(scale > 0.f && scale < INFINITY, "%s: scale must be positive and finite", name);
-  if (B == 0 || H == 0 || N == 0) return SVHIP_OK;
-  if (const int rc = check_pool(name, pc)) return rc;
-  SVHIP_REQUIRE(c.q && c.out, "%s: null pointer", name);
-  const int64_t even = c.cu_queries ? 0 : B;
-  SVHIP_REQUIRE(rows_on(8, c.q, even, H, N, c.sq_b, c.sq_h, c.sq_n), "%s: query rows must start on 16-byte boundaries", name);
-  SVHIP_REQUIRE(rows_on(4, c.out, even, H, N, c.so_b, c.so_h, c.so_n),
-                "%s: rows of out must start on 8-byte boundaries", name);
-  const bool fp8 = pc.kv_dtype == SVHIP_FP8_E4M3;
-  const int row_most = fp8 ? kRowMostFp8 : kRowMost;
-  const PagedPlan p = paged_plan(B, H, Hkv, N, c.cu_queries != nullptr, D, pc.max_pages * pc.page_size, row_most);
-  SVHIP_REQUIRE(p.bytes() == 0 || (c.workspace && c.workspace_bytes >= static_cast<int64_t>(p.bytes()) &&
-                                   reinterpret_cast<uintptr_t>(c.workspace) % 16 == 0),
-                "%s: workspace too small or misaligned (%lld < %zu bytes)", name, (long long)c.workspace_bytes, p.bytes());
-  const int64_t rows = (c.cu_queries ? N : B * N) * H, join = cdiv(rows, kPagedThreads / 32);
-  SVHIP_REQUIRE(p.row_slots + p.tile_grid < (1ll << 31) && rows < (1ll << 31) - kPagedThreads &&
-                    N * (H / Hkv) < (1ll << 31) - kPagedThreads, "%s: sizes too large", name);
-  const int64_t es = fp8 ? 1 : 2;
-  float* const part = static_cast<float*>(c.workspace);
-  int4* const plan = reinterpret_cast<int4*>(part + p.row_floats + p.tile_floats);
-  const PagedArgs a{static_cast<const uint16_t*>(c.q), pc.k_pages, pc.v_pages, pc.k_exponents, pc.v_exponents,
-                    static_cast<uint16_t*>(c.out), Tokens{c.cu_queries, B, N}, pages_of(pc),
-                    static_cast<int>(H), static_cast<int>(Hkv), static_cast<int>(H / Hkv), static_cast<int>(D), c.sq_b,
-                    c.sq_h, c.sq_n, pc.sk_h, pc.sv_h, pc.sek_h, pc.sev_h, c.so_b, c.so_h, c.so_n,
-                    static_cast<uint32_t>(pc.sk_p * es), static_cast<uint32_t>(pc.sk_r * es),
-                    static_cast<uint32_t>(pc.sv_p * es), static_cast<uint32_t>(pc.sv_r * es),
-                    static_cast<uint32_t>(pc.sek_p), static_cast<uint32_t>(pc.sev_p), c.causal != 0, scale * kLog2e,
-                    row_most, p.q_tiles, p.split, static_cast<int>(p.row_slots), static_cast<int>(p.tile_slots),
-                    static_cast<int>(p.slot_rows), p.row_parts ? part : nullptr, part + p.row_floats,
-                    p.plan_windows ? plan : nullptr, p.planned ? reinterpret_cast<int2*>(plan + B + 1) : nullptr};
-  hipStream_t s = as_stream(stream);
-  if (p.planned) paged_plan_kernel<<<1, kPlanThreads, 0, s>>>(a, p.rows, p.tiles);
-  if (p.rows && p.tiles) {
-    launch_paged_mixed(a, p, fp8, s);
-  } else if (p.rows) {
-    launch_paged_rows(a, p, fp8, s);
-  } else {
-    launch_paged_tiles(a, p, fp8, pc.page_size >= kWholePages, s);
-  }
-  if (p.plan_windows) {
-    if (rows <= kJoinFew) {
-      paged_join_kernel<8><<<static_cast<unsigned>(rows), kPagedThreads, 0, s>>>(a, 0u);
-    } else {
-      in_launches(join, [&](unsigned first, unsigned grid) {
-        paged_join_kernel<1><<<grid, kPagedThreads, 0, s>>>(a, first);
-      });
-    }
-  }
-  SVHIP_LAUNCHED(name);
-  return SVHIP_OK;
+  return paged_attention("svhip_paged_attention", cache, args, 0, 0, stream);
+}
+
+extern "C" int svhip_paged_window_attention(const svhip_paged_cache* cache, const svhip_paged_attention_args* args,
+                                            int64_t window, int64_t sinks, void* stream) {
+  const char* name = "svhip_paged_window_attention";
+  clear_error();
+  SVHIP_REQUIRE(window >= 1 && sinks >= 0, "%s: a window has a key or more, and 0 first keys or more beside it", name);
+  return paged_attention(name, cache, args, window, sinks, stream);
 }

@@ -57,6 +57,8 @@ struct PagedArgs {
   int4* plan;           // (null: no parts) a window's first slot, its parts, a part's length (tiles: blocks) and its tiles
   int2* running;        // (null: every workgroup plans for itself) places of row form and of tiles up to and with a window;
                         // plan[B] then has their sums and the part lengths
+  int block_shift;      // int8: log2 of the keys that share an exponent
+  int window, sinks;    // keys that a token sees up to its own, and first keys that it sees beside them (window 0: all)
 };
 
 // The window as a workgroup sees it.
@@ -84,12 +86,46 @@ __device__ __forceinline__ int last_key(const PagedArgs& a, const Window& w, int
   return static_cast<int>(j < w.keys - 1 ? (j < -1 ? -1 : j) : w.keys - 1);
 }
 
+// First key of token i's window, the last keys that it sees.
+__host__ __device__ __forceinline__ int first_key(int window, int64_t last, int keys, int64_t i) {
+  const int64_t j = last + i - window + 1;
+  return static_cast<int>(j < 0 ? 0 : (j < keys ? j : keys));
+}
+__device__ __forceinline__ int first_key(const PagedArgs& a, const Window& w, int64_t i) {
+  return first_key(a.window, w.last, w.keys, i);
+}
+
+// The first keys that stay visible, in whole blocks of tiles; and the keys between them and the window's first block,
+// which a workgroup whose first window begins at `low` leaves out: it walks the others as if they stood one behind the
+// other (`real_key`).
+__host__ __device__ __forceinline__ int sink_keys(int sinks) { return (sinks + kKB - 1) / kKB * kKB; }
+__host__ __device__ __forceinline__ int left_out(int sinks, int low) {
+  const int n = low / kKB * kKB - sink_keys(sinks);
+  return n > 0 ? n : 0;
+}
+__device__ __forceinline__ int real_key(int j, int sink_end, int out) { return j < sink_end ? j : j + out; }
+
+// True where token i sees a key.
+template <bool WIN>
+__device__ __forceinline__ bool sees_any(const PagedArgs& a, const Window& w, int64_t i) {
+  const int last = last_key(a, w, i);
+  if constexpr (WIN) return last >= 0 && (a.sinks > 0 || first_key(a, w, i) <= last);
+  return last >= 0;
+}
+
 __host__ __device__ __forceinline__ bool row_form(const PagedArgs& a, int64_t count) { return count * a.G <= a.row_most; }
 
 // Keys that the rows of tile qt see, the last of them the most.
 __device__ __forceinline__ int tile_keys(const PagedArgs& a, const Window& w, int qt) {
   const int r1 = (qt + 1) * kTileRows, rows = w.count * a.G;
   return last_key(a, w, ((r1 < rows ? r1 : rows) - 1) / a.G) + 1;
+}
+
+// Those of them that the tile leaves out.
+template <bool WIN>
+__device__ __forceinline__ int tile_left_out(const PagedArgs& a, const Window& w, int qt) {
+  if constexpr (WIN) return left_out(a.sinks, first_key(a, w, qt * kTileRows / a.G));
+  return 0;
 }
 
 // Row of `out` (or, with its strides, of the queries) that token i and head h have.
@@ -276,9 +312,22 @@ struct Rows {
   f32x4_t l;   // four equal entries: the lane's share of its row's sum
   float m;     // running maximum, log2 units
   int last;    // last key that the lane's row sees
+  int low;     // first key of its window (WIN)
 };
 
-template <int KS>
+// True where the lane's row sees key j, or any.
+template <bool WIN, int KS>
+__device__ __forceinline__ bool sees(const PagedArgs& a, const Rows<KS>& s, int j) {
+  if constexpr (WIN) return j <= s.last && (j >= s.low || j < a.sinks);
+  return j <= s.last;
+}
+template <bool WIN, int KS>
+__device__ __forceinline__ bool sees_any(const PagedArgs& a, const Rows<KS>& s) {
+  if constexpr (WIN) return s.last >= 0 && (a.sinks > 0 || s.low <= s.last);
+  return s.last >= 0;
+}
+
+template <bool WIN, int KS>
 __device__ __forceinline__ void load_rows(const PagedArgs& a, const Window& w, int64_t b, int kvh, int r,
                                           Rows<KS>& s) {
   const int hh = (threadIdx.x & 63) >> 5;
@@ -297,6 +346,7 @@ __device__ __forceinline__ void load_rows(const PagedArgs& a, const Window& w, i
   s.l = f32x4_t{0.f, 0.f, 0.f, 0.f};
   s.m = kNoMax;
   s.last = ok ? last_key(a, w, i) : -1;
+  if constexpr (WIN) s.low = first_key(a, w, i);
 }
 
 // S^T of 32 keys: ka the K rows as A operands, row R of the tile key sigma_row(R).
@@ -314,8 +364,10 @@ __device__ __forceinline__ f32x16_t scores(const Rows<KS>& s, const bf16x8_t (&k
 // maximum moved for a score more than kMaxHigh above it (the weights then stay below 2^20, which fp32 sums and bf16
 // hold alike). One such branch a block: a second one in a loop makes the compiler merge two register sets of O behind
 // it, a copy that the common path pays.
-template <int KS, int kHalves>
-__device__ __forceinline__ void bound_scores(Rows<KS>& s, f32x16_t (&x)[kHalves], float sl2, bool masked, int key0) {
+template <bool WIN, int KS, int kHalves>
+__device__ __forceinline__ void bound_scores(const PagedArgs& a, Rows<KS>& s, f32x16_t (&x)[kHalves], bool masked,
+                                             int key0) {
+  const float sl2 = a.scale_log2;
   const int hh = (threadIdx.x & 63) >> 5;
   if (masked) {
 #pragma unroll
@@ -324,6 +376,13 @@ __device__ __forceinline__ void bound_scores(Rows<KS>& s, f32x16_t (&x)[kHalves]
 #pragma unroll
       for (int i = 0; i < 16; ++i) {
         if ((i < 8 ? i : i + 8) > seen) x[t][i] = -INFINITY;
+      }
+      if constexpr (WIN) {
+        const int low = s.low - key0 - 32 * t - 8 * hh, sinks = a.sinks - key0 - 32 * t - 8 * hh;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          if ((i < 8 ? i : i + 8) < low && (i < 8 ? i : i + 8) >= sinks) x[t][i] = -INFINITY;
+        }
       }
     }
   }
@@ -427,7 +486,7 @@ __device__ __forceinline__ float row_sum(float l) {
   return __int_as_float(sw[0]) + __int_as_float(sw[1]);
 }
 
-// e4m3 rows on their way to LDS: a wave's kLoads loads of 8 rows, and the rows' exponents.
+// Rows of codes on their way to LDS: a wave's kLoads loads of 8 rows, and the rows' exponents.
 template <int DT, int kLoads>
 struct Staged {
   uint2 w[kLoads * Width<DT>::kSubTiles];
@@ -438,49 +497,70 @@ struct Staged {
 // tile row of the descriptor's first key: row lane / 8 and its chunk; K under sigma_row and swz, V under swzv.
 struct Lane8 {
   uint32_t at[2];   // byte offset in the descriptor in each sub-tile, or kOutside past head_dim
-  uint32_t key;     // the key's place in the descriptor
+  uint32_t key;     // the place of the key's exponent in theirs
 };
 
-template <int ES>
-__device__ __forceinline__ Lane8 lane_of_load(uint32_t sr, int D, int key, int chunk) {
+// Exponents in front of that of the `key`th of a group of keys: one a key, or int8's one a block. (A group begins with a
+// block, or lies in one.)
+template <int ST>
+__device__ __forceinline__ int exponent_at(const PagedArgs& a, int key) {
+  return ST == kInt8 ? key >> a.block_shift : key;
+}
+
+template <int ST>
+__device__ __forceinline__ Lane8 lane_of_load(const PagedArgs& a, uint32_t sr, int key, int chunk) {
   Lane8 n;
-  n.key = static_cast<uint32_t>(key);
+  n.key = static_cast<uint32_t>(exponent_at<ST>(a, key));
 #pragma unroll
   for (int u = 0; u < 2; ++u) {
     const int d = 64 * u + 8 * chunk;
-    n.at[u] = d < D ? n.key * sr + static_cast<uint32_t>(d * ES) : kOutside;
+    n.at[u] = d < a.D ? static_cast<uint32_t>(key) * sr + static_cast<uint32_t>(d * bytes_of(ST)) : kOutside;
   }
   return n;
 }
-template <int ES>
+template <int ST>
 __device__ __forceinline__ Lane8 k_lane(const PagedArgs& a, int first, int base) {
   const int lane = threadIdx.x & 63, R = first + (lane >> 3);
-  return lane_of_load<ES>(a.sk_r, a.D, sigma_row(R) - base, swz(R, lane & 7));
+  return lane_of_load<ST>(a, a.sk_r, sigma_row(R) - base, swz(R, lane & 7));
 }
-template <int ES>
+template <int ST>
 __device__ __forceinline__ Lane8 v_lane(const PagedArgs& a, int first, int base) {
   const int lane = threadIdx.x & 63, R = first + (lane >> 3);
-  return lane_of_load<ES>(a.sv_r, a.D, R - base, swzv(R, lane & 7));
+  return lane_of_load<ST>(a, a.sv_r, R - base, swzv(R, lane & 7));
 }
 
-// Issues a load of 8 rows: bf16 straight into LDS at `to` (row 0 of the 8 in sub-tile 0), e4m3 into registers at
+// Descriptor of the exponents of a group of keys, as rows_of.
+template <int ST>
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t exponents_of(const PagedArgs& a, const Source& s, int page, int in_page,
+                                                              int valid) {
+  const char* e = reinterpret_cast<const char*>(s.exponents);
+  if constexpr (ST == kInt8) {
+    const int some = valid > 0 ? ((valid - 1) >> a.block_shift) + 1 : 0;
+    return rows_of(e, s.se, 1, page, in_page >> a.block_shift, some, 1);
+  }
+  return rows_of(e, s.se, 1, page, in_page, valid, 1);
+}
+
+// Issues a load of 8 rows: bf16 straight into LDS at `to` (row 0 of the 8 in sub-tile 0), codes into registers at
 // index i.
-template <bool FP8, int DT, int kSubBytes, int kLoads>
+template <int ST, int DT, int kSubBytes, int kLoads>
 __device__ __forceinline__ void stage_rows8(const __amdgpu_buffer_rsrc_t r, const __amdgpu_buffer_rsrc_t er, const Lane8& n,
                                             int i, char* to, Staged<DT, kLoads>& st) {
 #pragma unroll
   for (int u = 0; u < Width<DT>::kSubTiles; ++u) {
-    if constexpr (FP8) {
+    if constexpr (coded(ST)) {
       st.w[i * Width<DT>::kSubTiles + u] = __builtin_bit_cast(uint2, __builtin_amdgcn_raw_buffer_load_b64(r, n.at[u], 0, 0));
     } else {
       __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (lds_ptr_t)(to + u * kSubBytes), 16, n.at[u], 0, 0, 0);
     }
   }
-  if constexpr (FP8) st.e[i] = __builtin_amdgcn_raw_buffer_load_b8(er, n.key, 0, 0);
+  if constexpr (coded(ST)) st.e[i] = __builtin_amdgcn_raw_buffer_load_b8(er, n.key, 0, 0);
 }
 
-// 8 e4m3 codes times 2^(exponent - 127) as bf16, exact.
+// 8 codes times 2^(exponent - 127) as bf16, exact.
+template <int ST>
 __device__ __forceinline__ uint4 decode8(uint2 w, uint32_t exponent) {
+  if constexpr (ST == kInt8) return int8_values(w, int8_power(exponent));
   const float f = exponent_value(static_cast<int>(exponent));
   const bf16x2_t a = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w.x, f, false);
   const bf16x2_t b = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w.x, f, true);
@@ -490,17 +570,17 @@ __device__ __forceinline__ uint4 decode8(uint2 w, uint32_t exponent) {
                     __builtin_bit_cast(uint32_t, d));
 }
 
-// e4m3: load i of `st` into its 8 rows at `to`.
-template <int DT, int kSubBytes, int kLoads>
+// Codes: load i of `st` into its 8 rows at `to`.
+template <int ST, int DT, int kSubBytes, int kLoads>
 __device__ __forceinline__ void commit_rows8(const Staged<DT, kLoads>& st, int i, char* to) {
 #pragma unroll
   for (int u = 0; u < Width<DT>::kSubTiles; ++u) {
     *reinterpret_cast<uint4*>(to + u * kSubBytes + 16 * (threadIdx.x & 63)) =
-        decode8(st.w[i * Width<DT>::kSubTiles + u], st.e[i]);
+        decode8<ST>(st.w[i * Width<DT>::kSubTiles + u], st.e[i]);
   }
 }
 
-// Values that are not finite, in a block whose keys some rows of the product see and some do not: their weight 0
+// Values that are not finite (int8 has none), in a block whose keys some rows of the product see and some do not: their weight 0
 // times such a value is NaN. So they are zeroed in LDS before the product (true: one was), a thread 16 bytes of
 // `bytes` every `step`, and added to the rows that see them at the end, from the pool.
 __device__ __forceinline__ bool clean_values(char* v, int bytes, int at, int step) {
@@ -524,23 +604,23 @@ __device__ __forceinline__ bool clean_values(char* v, int bytes, int at, int ste
 
 // Those of keys [from, to) to O^T of the rows that see them. (Their weights are above 0, and an infinity or NaN stays
 // one.)
-template <bool FP8, int KS>
+template <int ST, bool WIN, int KS>
 __device__ __forceinline__ void add_odd_values(const PagedArgs& a, const Source& vs, const int32_t* row, int from, int to,
                                                Rows<KS>& s) {
   const int hh = (threadIdx.x & 63) >> 5, in_mask = (1 << a.pages.shift) - 1;
   for (int j = from; j < to; ++j) {
     const int page = page_number(a, row, j);
-    if (static_cast<uint32_t>(page) < static_cast<uint32_t>(a.pages.pages) && j <= s.last) {
+    if (static_cast<uint32_t>(page) < static_cast<uint32_t>(a.pages.pages) && sees<WIN>(a, s, j)) {
       const uint32_t in_page = j & in_mask;
       const char* at = vs.rows + static_cast<uint64_t>(page) * vs.sp + in_page * vs.sr;
       float f = 0.f;
-      if constexpr (FP8) f = exponent_value(vs.exponents[static_cast<uint64_t>(page) * vs.se + in_page]);
+      if constexpr (ST == kE4m3) f = exponent_value(vs.exponents[static_cast<uint64_t>(page) * vs.se + in_page]);
 #pragma unroll
       for (int i = 0; i < 4 * tiles_of(KS); ++i) {
         const int d0 = 8 * i + 4 * hh;
         if (d0 >= a.D) continue;
         uint2 w;
-        if constexpr (FP8) {
+        if constexpr (ST == kE4m3) {
           const uint32_t codes = *reinterpret_cast<const uint32_t*>(at + d0);
           w = make_uint2(__builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(codes, f, false)),
                          __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(codes, f, true)));
@@ -615,10 +695,19 @@ inline PagedPlan paged_plan(int64_t B, int64_t H, int64_t Hkv, int64_t N, bool p
   return p;
 }
 
-// KS: steps of 16 head_dim elements; whole: pages of kWholePages keys or more.
-void launch_paged_rows(const PagedArgs& a, const PagedPlan& p, bool fp8, hipStream_t s);
-void launch_paged_tiles(const PagedArgs& a, const PagedPlan& p, bool fp8, bool whole, hipStream_t s);
-void launch_paged_mixed(const PagedArgs& a, const PagedPlan& p, bool fp8, hipStream_t s);
+// Keys that a tile's tokens, or those of a window of the row form, see at most of `max_keys` through a window.
+inline int64_t window_keys(int64_t max_keys, int64_t window, int64_t sinks) {
+  const int64_t most = window + 2 * kTileRows + 2 * kKB + sink_keys(static_cast<int>(sinks));
+  return max_keys < most ? max_keys : most;
+}
+
+// The launches of a storage, WIN: with a window (KS: steps of 16 head_dim elements; whole: pages of kWholePages keys or more).
+template <int ST, bool WIN>
+void launch_paged_rows(const PagedArgs& a, const PagedPlan& p, hipStream_t s);
+template <int ST, bool WIN>
+void launch_paged_tiles(const PagedArgs& a, const PagedPlan& p, bool whole, hipStream_t s);
+template <int ST, bool WIN>
+void launch_paged_mixed(const PagedArgs& a, const PagedPlan& p, hipStream_t s);
 
 // The instantiations of `launch` by head width; the others of its template arguments in front.
 #define SVHIP_PAGED_WIDTH(launch, ...)                       \

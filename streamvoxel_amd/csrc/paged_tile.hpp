@@ -5,13 +5,19 @@
 
 namespace svhip {
 
-// A window's tiles (0: the row form) and key blocks (0: no tokens).
+// A window's tiles (0: the row form) and the key blocks that a tile walks at most (0: no tokens).
+template <bool WIN = false>
 __host__ __device__ __forceinline__ void tiles_of_window(const PagedArgs& a, int64_t c, int& tiles, int& blocks) {
   int64_t first, count;
   window_tokens(a.tokens, c, first, count);
   tiles = row_form(a, count) ? 0 : static_cast<int>(cdiv(count * a.G, kTileRows));
   const int held = static_cast<int>((held_keys(a.pages, c) + kKB - 1) / kKB);  // (read beside the borders, not after them)
   blocks = count > 0 ? held : 0;
+  if constexpr (WIN) {
+    // A tile's tokens see the keys from the first one's window on: window + tokens - 1 of them, and the first blocks.
+    const int most = (a.window + (kTileRows - 1) / a.G + 1 + 2 * kKB - 2) / kKB + sink_keys(a.sinks) / kKB;
+    blocks = blocks < most ? blocks : most;
+  }
 }
 
 __host__ __device__ __forceinline__ int tile_parts(int blocks, int length) {
@@ -53,13 +59,13 @@ __device__ __forceinline__ PagedItem whole_item(const PagedArgs& a, int place) {
 // by side; at most kTileBeside where the row form's windows read half as many blocks or more (they then have the
 // other half of every CU: a block takes about 1 us of either's CU; 24 mixed windows 101 us for 110). kUncut: no
 // parts. `tiles`, `blocks`: of the team's own window; `total`: the tiles.
-template <typename Team>
+template <bool WIN = false, typename Team>
 __host__ __device__ __forceinline__ int tile_length(const PagedArgs& a, const Team& team, int& tiles, int& blocks, float& total) {
   const float Hkv = static_cast<float>(a.Hkv);
   float units = 0.f, work = 0.f, beside = 0.f;
   tiles = blocks = 0;
   for (int64_t c = team.id(); c < a.tokens.B; c += Team::kSize) {
-    tiles_of_window(a, c, tiles, blocks);
+    tiles_of_window<WIN>(a, c, tiles, blocks);
     units += static_cast<float>(tiles);
     work += static_cast<float>(tiles) * static_cast<float>(blocks);
     beside += tiles == 0 ? static_cast<float>(blocks) : 0.f;
@@ -75,7 +81,7 @@ __host__ __device__ __forceinline__ int tile_length(const PagedArgs& a, const Te
   if (full) work *= 1.5f;
   return part_length(a, team, work, target, 1, kTileLeast, [&](int c, int length) __attribute__((always_inline)) {
     int t = own_tiles, n = own_blocks;
-    if (a.tokens.B > Team::kSize) tiles_of_window(a, c, t, n);
+    if (a.tokens.B > Team::kSize) tiles_of_window<WIN>(a, c, t, n);
     return full && n <= length ? 0.f : Hkv * static_cast<float>(t) * static_cast<float>(tile_parts(n, length));
   });
 }
@@ -87,6 +93,7 @@ __host__ __device__ __forceinline__ int shared_place(int place, int total, int e
   return (place >> 3) < run && at < total ? at : -1;
 }
 
+template <bool WIN>
 __device__ __forceinline__ PagedItem shared_item(const PagedArgs& a, int place, int& each) {
   const PagedItem none{-1, 0, 0, 1, 0, 1, 0, 0};
   if (a.running) {
@@ -98,7 +105,7 @@ __device__ __forceinline__ PagedItem shared_item(const PagedArgs& a, int place, 
   const int Hkv = a.Hkv;
   int tiles, blocks;
   float total;
-  each = __builtin_amdgcn_readfirstlane(tile_length(a, WaveTeam{}, tiles, blocks, total));
+  each = __builtin_amdgcn_readfirstlane(tile_length<WIN>(a, WaveTeam{}, tiles, blocks, total));
   if (total == 0.f) return none;
   const int parts = tile_parts(blocks, each);
   int sum;
@@ -116,13 +123,14 @@ struct TileLds {
 
 #if defined(__HIP_DEVICE_COMPILE__)
 
-template <bool FP8, bool WHOLE, int KS>
+template <int ST, bool WIN, bool WHOLE, int KS>
 __device__ __forceinline__ void tile_work(const PagedArgs& a, int place, char* s0, char* s1, int* s_odd) {
-  constexpr int DT = tiles_of(KS), ES = FP8 ? 1 : 2;
+  constexpr int DT = tiles_of(KS), ES = bytes_of(ST);
+  constexpr bool kCodes = coded(ST);
   constexpr int kSubBytes = TileLds<KS>::kSubBytes, kTileBytes = TileLds<KS>::kTileBytes;
   char *sK0 = s0, *sV0 = s0 + kTileBytes, *sK1 = s1, *sV1 = s1 + kTileBytes;
   int each = kUncut;
-  const PagedItem item = a.split ? shared_item(a, place, each) : whole_item(a, place);
+  const PagedItem item = a.split ? shared_item<WIN>(a, place, each) : whole_item(a, place);
   const int b = __builtin_amdgcn_readfirstlane(item.b);
   if (b < 0) return;
   const int qt = __builtin_amdgcn_readfirstlane(item.qt), kvh = __builtin_amdgcn_readfirstlane(item.kvh);
@@ -132,7 +140,11 @@ __device__ __forceinline__ void tile_work(const PagedArgs& a, int place, char* s
   const int lane = threadIdx.x & 63, col = lane & 31, hh = lane >> 5;
   const int r0 = qt * kTileRows, r = r0 + wave * kRows + col, rows = w.count * a.G;
   const int keys = __builtin_amdgcn_readfirstlane(tile_keys(a, w, qt));
-  const int blocks = (keys + kKB - 1) / kKB;
+  // From here on `blk` counts the blocks that the tile's tokens see.
+  const int out_of_sight = WIN ? __builtin_amdgcn_readfirstlane(tile_left_out<WIN>(a, w, qt)) : 0;
+  const int sink_end = WIN ? sink_keys(a.sinks) : 0;
+  auto real = [&](int kv0) __attribute__((always_inline)) { return WIN ? real_key(kv0, sink_end, out_of_sight) : kv0; };
+  const int blocks = (keys - out_of_sight + kKB - 1) / kKB;
   const int count = blocks > each ? (blocks - 1) / each + 1 : 1;
   if (a.split && !a.running && part == 0 && kvh == 0 && qt == 0 && threadIdx.x == 0) {
     a.plan[b] = make_int4(item.first, item.parts, each, item.tiles);
@@ -141,7 +153,7 @@ __device__ __forceinline__ void tile_work(const PagedArgs& a, int place, char* s
   const int blk0 = part == 0 ? 0 : part * each, blk1 = blocks - blk0 > each ? blk0 + each : blocks;
 
   Rows<KS> s;
-  load_rows<KS>(a, w, b, kvh, r, s);
+  load_rows<WIN, KS>(a, w, b, kvh, r, s);
   // Where the lane's row goes, found now: what it takes would stay in scalar registers through the loop.
   const bool cut = count > 1;
   const int D = a.D;
@@ -165,17 +177,32 @@ __device__ __forceinline__ void tile_work(const PagedArgs& a, int place, char* s
   // Every row of the tile sees the keys up to `seen`; blocks past it are seen in part (clean_values).
   const int seen = __builtin_amdgcn_readfirstlane(last_key(a, w, r0 / a.G));
   const int clean_from = seen + 1 < keys ? (seen + 1) / kKB : kUncut;
+  // First keys of the windows of the wave's first and last token, and of the tile's last.
+  int low_first = 0, low_wave = 0, low_last = 0;
+  if constexpr (WIN) {
+    const int tr1 = r0 + kTileRows < rows ? r0 + kTileRows : rows;
+    low_first = __builtin_amdgcn_readfirstlane(wr0 < rows ? first_key(a, w, wr0 / a.G) : 0);
+    low_wave = __builtin_amdgcn_readfirstlane(wr0 < rows ? first_key(a, w, (wr1 - 1) / a.G) : 0);
+    low_last = __builtin_amdgcn_readfirstlane(first_key(a, w, (tr1 - 1) / a.G));
+  }
+  // The block at kv0 is not all in sight of a token whose window begins at `low`.
+  auto past_low = [&](int kv0, int low) __attribute__((always_inline)) {
+    return WIN && kv0 < low && kv0 + kKB > a.sinks;
+  };
+  auto in_part = [&](int kv0) __attribute__((always_inline)) {
+    return ST != kInt8 && (kv0 >= kKB * static_cast<int64_t>(clean_from) || past_low(kv0, low_last));
+  };
 
   // The wave stages rows 8 wave .. and 8 wave + 32 .. of a block: of one page (WHOLE), or of the 16 keys around each.
   constexpr int kGroup = WHOLE ? 64 : 16, kGroups = WHOLE ? 1 : 2;
-  Staged<DT, FP8 ? 2 : 1> kst, vst;
+  Staged<DT, kCodes ? 2 : 1> kst, vst;
   const int in_mask = (1 << a.pages.shift) - 1, row_bytes = D * ES;
   const int g0 = WHOLE ? 0 : 16 * (wave >> 1);
   Lane8 kl[2], vl[2];
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
-    kl[i] = k_lane<ES>(a, 8 * wave + 32 * i, WHOLE ? 0 : g0 + 32 * i);
-    vl[i] = v_lane<ES>(a, 8 * wave + 32 * i, WHOLE ? 0 : g0 + 32 * i);
+    kl[i] = k_lane<ST>(a, 8 * wave + 32 * i, WHOLE ? 0 : g0 + 32 * i);
+    vl[i] = v_lane<ST>(a, 8 * wave + 32 * i, WHOLE ? 0 : g0 + 32 * i);
   }
   int page[kGroups];
   auto find = [&](int kv0) __attribute__((always_inline)) {
@@ -191,27 +218,28 @@ __device__ __forceinline__ void tile_work(const PagedArgs& a, int place, char* s
         const int valid = valid_keys<kGroup>(a, keys, j, page[i]);
         kr = rows_of(ks.rows, ks.sp, ks.sr, page[i], in_page, valid, row_bytes);
         vr = rows_of(vs.rows, vs.sp, vs.sr, page[i], in_page, valid, row_bytes);
-        if constexpr (FP8) {
-          ek = rows_of(reinterpret_cast<const char*>(ks.exponents), ks.se, 1, page[i], in_page, valid, 1);
-          ev = rows_of(reinterpret_cast<const char*>(vs.exponents), vs.se, 1, page[i], in_page, valid, 1);
+        if constexpr (kCodes) {
+          ek = exponents_of<ST>(a, ks, page[i], in_page, valid);
+          ev = exponents_of<ST>(a, vs, page[i], in_page, valid);
         }
       }
       const int to = (8 * wave + 32 * i) * kRow * 2;
-      stage_rows8<FP8, DT, kSubBytes>(kr, ek, kl[i], i, sK + to, kst);
-      stage_rows8<FP8, DT, kSubBytes>(vr, ev, vl[i], i, sV + to, vst);
+      stage_rows8<ST, DT, kSubBytes>(kr, ek, kl[i], i, sK + to, kst);
+      stage_rows8<ST, DT, kSubBytes>(vr, ev, vl[i], i, sV + to, vst);
     }
   };
   auto commit = [&](char* sK, char* sV) __attribute__((always_inline)) {
-    if constexpr (FP8) {
+    if constexpr (kCodes) {
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
-        commit_rows8<DT, kSubBytes>(kst, i, sK + (8 * wave + 32 * i) * kRow * 2);
-        commit_rows8<DT, kSubBytes>(vst, i, sV + (8 * wave + 32 * i) * kRow * 2);
+        commit_rows8<ST, DT, kSubBytes>(kst, i, sK + (8 * wave + 32 * i) * kRow * 2);
+        commit_rows8<ST, DT, kSubBytes>(vst, i, sV + (8 * wave + 32 * i) * kRow * 2);
       }
     }
   };
   auto compute = [&](int kv0, const char* sK, const char* sV) __attribute__((always_inline)) {
     if (kv0 > any) return;
+    if (WIN && kv0 + kKB <= low_first && kv0 >= a.sinks) return;
     f32x16_t x[2];
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
@@ -222,7 +250,7 @@ __device__ __forceinline__ void tile_work(const PagedArgs& a, int place, char* s
       }
       x[t] = scores<KS>(s, ka);
     }
-    bound_scores<KS, 2>(s, x, a.scale_log2, kv0 + kKB - 1 > all, kv0);
+    bound_scores<WIN, KS, 2>(a, s, x, kv0 + kKB - 1 > all || past_low(kv0, low_wave), kv0);
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
       bf16x8_t pb[2];
@@ -232,21 +260,22 @@ __device__ __forceinline__ void tile_work(const PagedArgs& a, int place, char* s
   };
   if (blk0 < blk1) {
     if (threadIdx.x == 0) *s_odd = 0;
-    find(kKB * blk0);
-    issue(kKB * blk0, sK0, sV0);
-    find(kKB * (blk0 + 1));
+    find(real(kKB * blk0));
+    issue(real(kKB * blk0), sK0, sV0);
+    find(real(kKB * (blk0 + 1)));
     commit(sK0, sV0);
     wait_vmem();
     __syncthreads();
     auto step = [&](int blk, char* cK, char* cV, char* nK, char* nV) __attribute__((always_inline)) {
       const bool more = blk + 1 < blk1;
-      if (more) issue(kKB * (blk + 1), nK, nV);
-      find(kKB * (blk + 2));
-      if (blk >= clean_from) {
+      if (more) issue(real(kKB * (blk + 1)), nK, nV);
+      find(real(kKB * (blk + 2)));
+      const int kv0 = real(kKB * blk);
+      if (WIN ? in_part(kv0) : ST != kInt8 && blk >= clean_from) {
         if (clean_values(cV, kTileBytes, 16 * static_cast<int>(threadIdx.x), 16 * kPagedThreads)) *s_odd = 1;
         __syncthreads();
       }
-      compute(kKB * blk, cK, cV);
+      compute(kv0, cK, cV);
       if (more) {
         commit(nK, nV);
         wait_vmem();
@@ -257,14 +286,21 @@ __device__ __forceinline__ void tile_work(const PagedArgs& a, int place, char* s
       step(blk, sK0, sV0, sK1, sV1);
       if (blk + 1 < blk1) step(blk + 1, sK1, sV1, sK0, sV0);
     }
-    if (clean_from < blk1 && *s_odd != 0) {
-      add_odd_values<FP8, KS>(a, vs, row, kKB * (clean_from > blk0 ? clean_from : blk0),
-                              kKB * blk1 < keys ? kKB * blk1 : keys, s);
+    if constexpr (WIN) {
+      if (ST != kInt8 && *s_odd != 0) {
+        for (int blk = blk0; blk < blk1; ++blk) {
+          const int kv0 = real(kKB * blk);
+          if (in_part(kv0)) add_odd_values<ST, WIN, KS>(a, vs, row, kv0, kv0 + kKB < keys ? kv0 + kKB : keys, s);
+        }
+      }
+    } else if (ST != kInt8 && clean_from < blk1 && *s_odd != 0) {
+      add_odd_values<ST, WIN, KS>(a, vs, row, kKB * (clean_from > blk0 ? clean_from : blk0),
+                                  kKB * blk1 < keys ? kKB * blk1 : keys, s);
     }
   }
   const float l = row_sum(s.l[0]);
   if (dest == nullptr) return;
-  const float inv = s.last >= 0 ? 1.f / l : 0.f;
+  const float inv = sees_any<WIN>(a, s) ? 1.f / l : 0.f;
 #pragma unroll
   for (int j = 0; j < DT; ++j) {
 #pragma unroll
@@ -286,5 +322,32 @@ __device__ __forceinline__ void tile_work(const PagedArgs& a, int place, char* s
 }
 
 #endif  // __HIP_DEVICE_COMPILE__
+
+// Windows that are all of the tile form. Up to 64 head_dim elements a bf16 pool's kernel fits 128 registers and four
+// workgroups a CU (8 windows of 1024 queries, head_dim 64: 203.6 us, 204.5 with room for two); wider or decoding ones
+// spill there.
+template <int ST, bool WIN, bool WHOLE, int KS>
+__global__ __launch_bounds__(kPagedThreads, coded(ST) || KS > 4 ? 2 : 4) void paged_tile_kernel(PagedArgs a, unsigned first_group) {
+#if defined(__HIP_DEVICE_COMPILE__)
+  __shared__ __attribute__((aligned(16))) char s0[TileLds<KS>::kBuffer], s1[TileLds<KS>::kBuffer];
+  __shared__ int s_odd;
+  tile_work<ST, WIN, WHOLE, KS>(a, static_cast<int>(first_group + blockIdx.x), s0, s1, &s_odd);
+#endif
+}
+
+template <int ST, bool WIN, bool WHOLE, int KS>
+void launch_tiles(const PagedArgs& a, const PagedPlan& p, hipStream_t s) {
+  in_launches(p.tile_grid, [&](unsigned first, unsigned grid) {
+    paged_tile_kernel<ST, WIN, WHOLE, KS><<<grid, kPagedThreads, 0, s>>>(a, first);
+  });
+}
+
+template <int ST, bool WIN>
+void launch_paged_tiles(const PagedArgs& a, const PagedPlan& p, bool whole, hipStream_t s) {
+  if (whole) {
+    SVHIP_PAGED_WIDTH(launch_tiles, ST, WIN, true)
+  }
+  SVHIP_PAGED_WIDTH(launch_tiles, ST, WIN, false)
+}
 
 }  // namespace svhip

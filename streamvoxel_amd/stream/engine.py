@@ -182,10 +182,10 @@ class StepGraphs:
 
 PATCHIFY = ('gather', 'conv')
 ATTENTION = ('flex', 'sdpa')
-KV_DTYPES = ('bf16', 'fp8')
+KV_DTYPES = ('bf16', 'fp8', 'int8')
 
 
-def check_engine_options(patchify, attention, compile, kv_dtype='bf16'):
+def check_engine_options(patchify, attention, compile, kv_dtype='bf16', paged=False):
     """The engine's options, validated as the reference does (fast_ops.py:170-171): ValueError for unknown ones."""
     if patchify not in PATCHIFY or attention not in ATTENTION:
         raise ValueError('patchify must be gather|conv and attention flex|sdpa')
@@ -193,6 +193,8 @@ def check_engine_options(patchify, attention, compile, kv_dtype='bf16'):
         raise ValueError("compile must be False, True or 'emulate'")
     if kv_dtype not in KV_DTYPES:
         raise ValueError(f'kv_dtype must be one of {KV_DTYPES}')
+    if kv_dtype == 'int8' and not paged:
+        raise ValueError("kv_dtype 'int8' needs pages: a slab holds bf16 or e4m3")
 
 
 class SlotEngine:
@@ -206,8 +208,8 @@ class SlotEngine:
     `default_encoder` supplies when none is passed and the reference's package is importable); without one,
     `load_slot` takes an `Encoded` (or a (prefix, local, positions) tuple) itself.
     `kv_dtype` 'bf16' (the reference's cache) or 'fp8' (e4m3 with per-(window, head) scales). `pages`: the slots share a pool
-    of that many pages of `page_size` keys (a `PagedContext`, e4m3 with a scale a row) in place of a slab of the longest
-    condition each; a slot's context can then grow (`extend_slot`). The step takes 0.6 % longer then (e4m3 1.6 %; the
+    of that many pages of `page_size` keys (a `PagedContext`, e4m3 with a scale a row; 'int8' too, with one for each block
+    of a page's keys, which `extend_slot` may round again) in place of a slab of the longest condition each; a slot's context can then grow (`extend_slot`). The step takes 0.6 % longer then (e4m3 1.6 %; the
     shipped shape, 8 slots), and where few slots step together, loading one may change the last bits of another's logits,
     which a slab keeps. `concurrent` runs the
     control branch on its own stream inside the step. `patchify`, `attention` and `compile` are the reference's
@@ -220,7 +222,7 @@ class SlotEngine:
     def __init__(self, model, spec, device, batch, l1_cap, l2_cap, *, patchify='gather', attention='flex',
                  compile=False, capture=True, encoder=None, kv_dtype='bf16', concurrent=True, pages=None,
                  page_size=64):
-        check_engine_options(patchify, attention, compile, kv_dtype)
+        check_engine_options(patchify, attention, compile, kv_dtype, pages is not None)
         self.device = torch.device(device)
         if self.device.type != 'cuda':
             raise RuntimeError('SlotEngine runs on a HIP device; there is no CPU path')
@@ -386,8 +388,9 @@ class SlotEngine:
                                  prefix_kv=stacked, local=enc.local.to(dev), local_positions=enc.positions.to(dev))
             return out, 'model_forward'
         length = (enc.prefix[0][0].shape[1] if len(enc.prefix) else 0) + enc.local.shape[1]
+        kv_dtype = self.context.kv_dtype
         ctx = CachedContext(self.context.layers, 1, self.context.heads, self.context.head_dim, max(length, 1), dev,
-                            self.context.kv_dtype)
+                            'bf16' if kv_dtype == 'int8' else kv_dtype)
         write_condition(self.model, ctx, 0, enc)
         step = StepForward(self.model, ctx, concurrent=False)
         out = step(tokens, time, self.origin[:1], self.group_origin)

@@ -1,5 +1,5 @@
-"""A paged cache of keys and values on the HIP kernels: the append that fills it, the attention over it, and the context
-that stands in `CachedContext`'s place with its windows in one pool of pages.
+"""A paged cache of keys and values on the HIP kernels: the append that fills it, the reading back, the attention over it,
+whole or through a sliding window, and the context that stands in `CachedContext`'s place with its windows in one pool of pages.
 
 `step.CachedContext` (PackedKeys, streamvoxel/stream/fast_ops.py:122-159) keeps a slab of the longest condition for
 every slot and rewrites it whole; here a window holds the pages that its keys fill, and new keys go behind the ones
@@ -13,7 +13,7 @@ import torch
 
 from streamvoxel_amd import _lib
 
-__all__ = ['paged_append', 'paged_attention', 'PagedContext']
+__all__ = ['paged_append', 'paged_read', 'paged_attention', 'PagedContext']
 
 LAYOUTS = {'half': _lib.SVHIP_ROTARY_HALF, 'interleaved': _lib.SVHIP_ROTARY_INTERLEAVED,
            'axial': _lib.SVHIP_ROTARY_AXIAL}
@@ -36,8 +36,21 @@ def _check_pool(k_pages, v_pages, page_table, lengths, k_exponents, v_exponents,
         if k_exponents is not None or v_exponents is not None:
             raise TypeError('bf16 pages take no exponents')
         return _lib.SVHIP_BF16
+    if dtype == torch.int8:
+        for e in (k_exponents, v_exponents):
+            if e is None or e.dtype != torch.uint8 or e.dim() != 3 or e.shape[:2] != shape[:2] or (
+                    e.stride(-1) != 1 and e.shape[2] > 1):
+                raise ValueError('int8 pages need k_exponents and v_exponents, uint8 [pages, heads, page / block] with '
+                                 'contiguous rows')
+        if k_exponents.shape != v_exponents.shape:
+            raise ValueError('k_exponents and v_exponents must be alike')
+        blocks = k_exponents.shape[2]
+        block = shape[2] // blocks if blocks else 0
+        if block not in _lib.SVHIP_INT8_BLOCK or blocks * block != shape[2]:
+            raise ValueError(f'{blocks} exponents for a page of {shape[2]} keys: one is for 16, 32 or 64 of them')
+        return _lib.SVHIP_INT8_BLOCK[block]
     if dtype != torch.float8_e4m3fn:
-        raise TypeError(f'pages of {dtype} unsupported (bfloat16 or float8_e4m3fn)')
+        raise TypeError(f'pages of {dtype} unsupported (bfloat16, float8_e4m3fn or int8)')
     for e in (k_exponents, v_exponents):
         if e is None or e.dtype != torch.uint8 or e.shape != shape[:3] or e.stride(-1) != 1:
             raise ValueError('e4m3 pages need k_exponents and v_exponents, uint8 [pages, heads, page] with contiguous '
@@ -77,6 +90,7 @@ def _rows16(t):
 _CACHE = struct.Struct('7P18q')    # svhip_paged_cache
 _APPEND = struct.Struct('5P13qd')  # svhip_paged_append_args
 _ATTEND = struct.Struct('4P10qd')  # svhip_paged_attention_args
+_READ = struct.Struct('3P8q')      # svhip_paged_read_args
 
 
 def _address(t):
@@ -101,14 +115,21 @@ def paged_append(key, value, k_pages, v_pages, page_table, lengths, cu_tokens=No
     key, value bf16 [B,H,n,D] (head_dim contiguous, any other strides), or packed [H,T,D] with the windows' borders
     `cu_tokens` int32 [B+1] (device, ascending; tokens outside every window are left alone). k_pages, v_pages
     [pages,H,page,D] in bf16, or float8_e4m3fn with `k_exponents` / `v_exponents` uint8 [pages,H,page], one power of
-    two 2^(exponent - 127) for each row (written too, 1 to 254); page a power of two from 16 to 1024. page_table int32 [B, m]:
+    two 2^(exponent - 127) for each row (written too, 1 to 254), or int8 with uint8 [pages,H,page / block], one for each
+    block of 16, 32 or 64 keys (1 to 248); page a power of two from 16 to 1024. page_table int32 [B, m]:
     key j of window b is row j % page of page page_table[b, j // page]. `lengths` int32 [B] (device) counts each
     window's keys with the new ones: they are its last n keys, or the n in front of its last `before`. Two tokens must
     not share a row. `frequencies` rotates the keys: with layout 'half' / 'interleaved' as `rotary` does (fp64;
     `positions` int32 / int64 [B,n] or [T], or None: each key's index in its window; `amplitude`), with 'axial' as
     `producer.axial_rope` does (its fp32 buffer and fp32 positions [B,n,3] or [T,3]). `bad` (optional int32 [1],
     device) becomes 1 when a key lies outside its window's row of the table or a page outside the pool; such keys are
-    not written."""
+    not written.
+
+    int8: a value is held as a whole number of at most 127 times its block's power of two, off by half of that at most. The
+    block's is the least that holds its new keys, and not below the one it has if keys of the window stand in front of them
+    in the block: where it grows, those are rounded to the new one (what that adds up to stays under one step of it, however the block
+    was filled). Keys behind the new ones in a block (`before`) count as yet to be written. Infinities are held as the
+    largest number and NaN as 0, and set `bad`. No two windows may write into one block."""
     _lib.require_one_gpu(key, value, k_pages, v_pages, page_table, lengths, cu_tokens, positions, frequencies, k_exponents,
                          v_exponents, bad)
     code = _check_pool(k_pages, v_pages, page_table, lengths, k_exponents, v_exponents, bad)
@@ -162,15 +183,62 @@ def paged_append(key, value, k_pages, v_pages, page_table, lengths, cu_tokens=No
     _lib.launch('svhip_paged_append', key, cache, args)
 
 
+def paged_read(k_pages, v_pages, page_table, lengths, n, cu_keys=None, before=0, k_exponents=None, v_exponents=None, out=None,
+               bad=None):
+    """(key, value) bf16: keys and values read back from a paged cache, the inverse of `paged_append`.
+
+    Of every window the `n` keys in front of its last `before`, as [B,H,n,D]; or with `cu_keys` (int32 [B+1], device, ascending)
+    window b's cu_keys[b + 1] - cu_keys[b] of them, packed [H,n,D] with n rows in all. The pool as `paged_append` fills it (bf16,
+    e4m3 or int8; the codes' values are exact in bf16). A key that does not exist, in front of the window's first, is a row of
+    zeros, and so is one on a bad page or outside the window's row of the table, which also sets `bad` (optional int32
+    [1], device). `out` (optional): the pair that receives them, of any strides with 16-byte aligned rows; its rows outside
+    every window are left as they are (fresh ones have them undefined)."""
+    _lib.require_one_gpu(k_pages, v_pages, page_table, lengths, cu_keys, k_exponents, v_exponents, bad, *(out or ()))
+    code = _check_pool(k_pages, v_pages, page_table, lengths, k_exponents, v_exponents, bad)
+    n, B = int(n), page_table.shape[0]
+    if n < 0 or before < 0:
+        raise ValueError('n and before count keys')
+    P, H, S, D = k_pages.shape
+    shape = (B, H, n, D) if cu_keys is None else (H, n, D)
+    if out is None:
+        key, value = [torch.empty(shape, dtype=torch.bfloat16, device=k_pages.device) for _ in 'kv']
+    else:
+        key, value = out
+        for t in out:
+            if t.shape != shape or t.dtype != torch.bfloat16 or t.stride(-1) != 1 or _lib.stacked(t):
+                raise ValueError(f'out must be a pair of bf16 {shape} with a contiguous head_dim and a place for every element')
+            if any(_lib.overlaps(t, pages) for pages in (k_pages, v_pages)):
+                raise ValueError('out must not share memory with the pages')
+        if _lib.overlaps(key, value) and not _side_by_side(key, value):
+            raise ValueError('the two of out must not share memory')
+    sk, sv = _windows(key, cu_keys, B, 'key')[2], _windows(value, cu_keys, B, 'value')[2]
+    cache = _packed(code, k_pages, v_pages, page_table, lengths, k_exponents, v_exponents, bad)
+    args = _READ.pack(key.data_ptr(), value.data_ptr(), _address(cu_keys), n, before, *sk, *sv)
+    _lib.launch('svhip_paged_read', key, cache, args)
+    return key, value
+
+
+def _side_by_side(a, b):
+    """True where two tensors of one shape and the same strides interleave without touching: one dimension's stride holds both."""
+    if a.stride() != b.stride():
+        return False
+    gap = abs(a.data_ptr() - b.data_ptr()) // a.element_size()
+    inner = [(s, n) for n, s in zip(a.shape, a.stride()) if n > 1 and s <= gap]
+    outer = [s for n, s in zip(a.shape, a.stride()) if n > 1 and s > gap]
+    reach = sum((n - 1) * s for s, n in inner) + 1
+    return reach <= gap and all(gap + reach <= s for s in outer)
+
+
 def paged_attention(query, k_pages, v_pages, page_table, lengths, cu_queries=None, causal=False, scale=None,
-                    k_exponents=None, v_exponents=None, out=None, bad=None):
+                    k_exponents=None, v_exponents=None, out=None, bad=None, window=None, sinks=0):
     """softmax(scale * Q K^T) V of the windows' new tokens over the first lengths[b] keys of their pages.
 
     query bf16 [B,H,n,D] (head_dim contiguous, any other strides), or packed [H,T,D] with the windows' borders
     `cu_queries` int32 [B+1] (device, ascending). k_pages, v_pages, page_table, lengths and the exponents as
     `paged_append` fills them; the H heads share the pages' heads evenly, head h reads head h // (H / heads).
     `causal`: the n tokens are the window's last n keys, and token i sees keys up to its own, lengths[b] - n + i;
-    without it every token sees all of them. A token with no key gets zeros, and what is not finite among keys that a
+    without it every token sees all of them. `window` (with causal): a token sees the last `window` keys up to its own, and
+    the first `sinks` keys; those in between are not read. A token with no key gets zeros, and what is not finite among keys that a
     token does not see does not reach it. The same call gives the same bits; other windows in the call move the places
     where a window's keys are cut for several workgroups, and with them its last bits (`attention` keeps a window's bits
     in any batch). `out` (optional; query itself, or memory that query does not share) bf16
@@ -196,13 +264,21 @@ def paged_attention(query, k_pages, v_pages, page_table, lengths, cu_queries=Non
         raise ValueError('out must be query itself or memory that query does not share')
     so = _windows(out, cu_queries, B, 'out')[2]
     scale = D ** -0.5 if scale is None else float(scale)
+    if window is None:
+        if sinks:
+            raise ValueError('sinks stay visible beside a window')
+    elif not causal or window < 1 or sinks < 0:
+        raise ValueError('a window needs causal, a key or more, and 0 sinks or more')
     nbytes = _lib.load().svhip_paged_attention_workspace_bytes(B, H, Hkv, n, cu_queries is not None, D,
                                                                page_table.shape[1] * S)
     cache = _packed(code, k_pages, v_pages, page_table, lengths, k_exponents, v_exponents, bad)
     ws = torch.empty(nbytes, dtype=torch.uint8, device=query.device) if nbytes else None
     args = _ATTEND.pack(query.data_ptr(), out.data_ptr(), _address(cu_queries), _address(ws), nbytes, H, n, *sq, *so, causal,
                         scale)
-    _lib.launch('svhip_paged_attention', query, cache, args)
+    if window is None:
+        _lib.launch('svhip_paged_attention', query, cache, args)
+    else:
+        _lib.launch('svhip_paged_window_attention', query, cache, args, min(int(window), 1 << 30), min(int(sinks), 1 << 30))
     return out
 
 
@@ -210,8 +286,9 @@ class PagedContext:
     """The cached keys and values of `batch` windows in one pool of `pages` pages a layer (each `page_size` keys of
     every head), in `CachedContext`'s place: `write`, `attend`, `lengths` as there, and windows that grow (`grow`,
     `append`) and give their pages back (`release`). A window holds as many pages as its keys need, at most
-    `max_pages` of them (default: all). kv_dtype 'bf16' or 'fp8' (OCP e4m3fn with one power of two for each row and
-    head).
+    `max_pages` of them (default: all). kv_dtype 'bf16', 'fp8' (OCP e4m3fn with one power of two for each row and
+    head) or 'int8' (with one for each `block` keys of a page, 16, 32 or 64, and head; the least of 64 and the page by
+    default).
 
     What it costs beside the slab: the attention of 1024 queries a window takes 6 to 14 % longer at head_dim 64 (a tenth
     to a fifth less at 128), and a window's last bits depend on the other windows of the call (`paged_attention`), where
@@ -223,24 +300,30 @@ class PagedContext:
     reads the table and the lengths as they stand; a capture that would change them is refused. `bad` (device int32
     [1]) becomes non-zero when a call meets a page outside the pool, which these books never name."""
 
-    def __init__(self, layers, batch, heads, head_dim, pages, device, page_size=64, max_pages=None, kv_dtype='bf16'):
-        if kv_dtype not in ('bf16', 'fp8'):
-            raise ValueError("kv_dtype must be 'bf16' or 'fp8'")
+    def __init__(self, layers, batch, heads, head_dim, pages, device, page_size=64, max_pages=None, kv_dtype='bf16',
+                 block=None):
+        if kv_dtype not in ('bf16', 'fp8', 'int8'):
+            raise ValueError("kv_dtype must be 'bf16', 'fp8' or 'int8'")
         if page_size not in (16, 32, 64, 128, 256, 512, 1024):
             raise ValueError('page_size must be a power of two from 16 to 1024')
         if head_dim < 8 or head_dim > 128 or head_dim % 8:
             raise ValueError('head_dim must be a multiple of 8 up to 128')
         if layers < 1 or batch < 1 or heads < 1 or pages < 1 or (max_pages is not None and max_pages < 1):
             raise ValueError('layers, batch, heads, pages and max_pages must be positive')
+        if block is None:
+            block = min(64, page_size)
+        elif kv_dtype != 'int8' or block not in _lib.SVHIP_INT8_BLOCK or block > page_size:
+            raise ValueError('block is 16, 32 or 64 keys of a page, for int8')
         self.layers, self.batch, self.heads, self.head_dim = layers, batch, heads, head_dim
         self.pages, self.page_size, self.kv_dtype = pages, page_size, kv_dtype
         self.max_pages = pages if max_pages is None else max_pages
-        dt = torch.bfloat16 if kv_dtype == 'bf16' else torch.float8_e4m3fn
-        pool = lambda dtype, *shape: [torch.empty(pages, heads, page_size, *shape, dtype=dtype, device=device)
-                                      for _ in range(layers)]
-        self.k, self.v = pool(dt, head_dim), pool(dt, head_dim)
+        dt = dict(bf16=torch.bfloat16, fp8=torch.float8_e4m3fn, int8=torch.int8)[kv_dtype]
+        pool = lambda dtype, *shape: [torch.empty(pages, heads, *shape, dtype=dtype, device=device) for _ in range(layers)]
+        self.k, self.v = pool(dt, page_size, head_dim), pool(dt, page_size, head_dim)
         none = [None] * layers
-        self.k_exponents, self.v_exponents = (pool(torch.uint8), pool(torch.uint8)) if kv_dtype == 'fp8' else (none, none)
+        rows = page_size if kv_dtype == 'fp8' else page_size // block
+        self.k_exponents, self.v_exponents = (none, none) if kv_dtype == 'bf16' else (pool(torch.uint8, rows),
+                                                                                      pool(torch.uint8, rows))
         self.table = torch.zeros(batch, self.max_pages, dtype=torch.int32, device=device)
         self.lengths = torch.zeros(batch, dtype=torch.int32, device=device)
         self.bad = torch.zeros(1, dtype=torch.int32, device=device)
@@ -406,10 +489,21 @@ class PagedContext:
         if L:
             self.append(layer, key, value, index=index, **how)
 
-    def attend(self, layer, query, out=None, n=None, cu_queries=None, causal=False):
+    def read(self, layer, index=None, n=None):
+        """(key, value) bf16 [heads, keys, head_dim]: what window `index` of `layer` holds (its last n keys), as `write` and
+        `append` take them; of all windows one behind the other without an index (n: of each, at most)."""
+        held = [L if n is None else min(L, n) for L in (self.host_lengths if index is None else [self.host_lengths[index]])]
+        at = slice(0, self.batch) if index is None else slice(index, index + 1)
+        borders = torch.zeros(len(held) + 1, dtype=torch.int32)
+        borders[1:] = torch.tensor(held).cumsum(0)
+        cu = borders.to(self.lengths.device)
+        return paged_read(self.k[layer], self.v[layer], self.table[at], self.lengths[at], sum(held), cu_keys=cu,
+                          k_exponents=self.k_exponents[layer], v_exponents=self.v_exponents[layer], bad=self.bad)
+
+    def attend(self, layer, query, out=None, n=None, cu_queries=None, causal=False, window=None, sinks=0):
         """Attention of `query` [n,H,Q,D] bf16 (H a multiple of the cache's heads; packed [H,T,D] with cu_queries)
-        over the keys of the first n windows."""
+        over the keys of the first n windows, through a sliding `window` beside the first `sinks` keys if given."""
         n = self.batch if n is None else n
         return paged_attention(query, self.k[layer], self.v[layer], self.table[:n], self.lengths[:n], cu_queries=cu_queries,
                                causal=causal, out=out, k_exponents=self.k_exponents[layer],
-                               v_exponents=self.v_exponents[layer], bad=self.bad)
+                               v_exponents=self.v_exponents[layer], bad=self.bad, window=window, sinks=sinks)

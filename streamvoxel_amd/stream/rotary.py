@@ -1,5 +1,5 @@
 """Rotary positions of one axis on the HIP kernels: interleaved and half layouts, part of a head, frequencies scaled for
-contexts longer than the trained one.
+contexts longer than the trained one; and the norm of each head's queries and keys in the same pass.
 
 Beside `producer.axial_rope` (AxialRoPE, streamvoxel/models/unconditional_md4.py:10-24), which turns the three axes of
 the reference's positions with the reference's bf16 roundings; no counterpart in the reference.
@@ -11,10 +11,11 @@ import struct
 
 import torch
 from torch.autograd import forward_ad
+from torch.autograd.function import once_differentiable
 
 from streamvoxel_amd import _lib
 
-__all__ = ['rotary', 'rotary_frequencies']
+__all__ = ['rotary', 'rotary_frequencies', 'norm_rotary']
 
 LAYOUTS = {'half': _lib.SVHIP_ROTARY_HALF, 'interleaved': _lib.SVHIP_ROTARY_INTERLEAVED}
 
@@ -131,3 +132,153 @@ def rotary(x, positions, frequencies, layout='half', amplitude=1.0, out=None):
         if _lib.overlaps(x, out) and (x.data_ptr() != out.data_ptr() or x.stride() != out.stride()):
             raise ValueError('out must be x itself or memory that x does not share')
     return _launch(x, out, positions, frequencies, layout, float(amplitude), 0)
+
+
+_NORM = struct.Struct('13P31q2d')   # svhip_norm_rotary_args
+
+
+def _places(t):
+    return (0, 0, 0) if t is None else t.stride()[:3]
+
+
+def _address(t):
+    return 0 if t is None else t.data_ptr()
+
+
+def _norm_args(query, key, dq, dk, weights, outs, dw, workspace, positions, frequencies, eps, layout, amplitude):
+    B, H, N, D = query.shape
+    given = weights[0] if weights[0] is not None else weights[1]
+    wide = _lib.SVHIP_F32 if given is None else _lib.dtype_code(given.dtype)
+    return _NORM.pack(_address(query), _address(key), _address(dq), _address(dk), *map(_address, weights), *map(_address, outs),
+                      *map(_address, dw), positions.data_ptr(), frequencies.data_ptr(), _address(workspace),
+                      0 if workspace is None else workspace.numel(), _lib.dtype_code(query.dtype), wide,
+                      positions.dtype == torch.int64, frequencies.numel(), LAYOUTS[layout], B, H,
+                      0 if key is None else key.shape[1], N, D, *_places(query), *_places(key), *_places(dq), *_places(dk),
+                      *_places(outs[0]), *_places(outs[1]), positions.stride(0) if positions.dim() == 2 else 0,
+                      positions.stride(-1), amplitude, eps)
+
+
+def _normed(query, key, weights, outs, *how):
+    _lib.launch('svhip_norm_rotary', query, _norm_args(query, key, None, None, weights, outs, (None, None), None, *how))
+    return outs
+
+
+def _like(t):
+    return None if t is None else torch.empty_like(t)
+
+
+def _rows(t):
+    """Rows with a contiguous head_dim: the tensor itself, or a copy."""
+    return t if t is None or t.stride(-1) == 1 else t.contiguous()
+
+
+class _NormRotary(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, query, key, query_weight, key_weight, *how):
+        positions, frequencies, *rest = how
+        ctx.save_for_backward(query, key, query_weight, key_weight, positions, frequencies)
+        ctx.rest = rest
+        q, k = _normed(query, key, (query_weight, key_weight), (_like(query), _like(key)), *how)
+        return q if k is None else (q, k)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dq, dk=None):
+        query, key, *weights, positions, frequencies = ctx.saved_tensors
+        dq, dk = _rows(dq), _rows(dk)
+        needs = ctx.needs_input_grad
+        outs = [torch.empty_like(t) if need else None for t, need in zip((query, key), needs)]
+        dw = [torch.empty_like(t) if need else None for t, need in zip(weights, needs[2:])]
+        B, _, N, D = query.shape
+        workspace = None
+        if dw[0] is not None or dw[1] is not None:
+            workspace = torch.empty(_lib.load().svhip_norm_rotary_workspace_bytes(B, N, D), dtype=torch.uint8,
+                                    device=query.device)
+        _lib.launch('svhip_norm_rotary_grad', query, _norm_args(query, key, dq, dk, weights, outs, dw, workspace, positions,
+                                                                frequencies, *ctx.rest))
+        return *outs, *dw, *[None] * (2 + len(ctx.rest))
+
+
+def norm_rotary(query, key, query_weight, key_weight, positions, frequencies, eps=1e-6, layout='half', amplitude=1.0, out=None):
+    """(query, key) normed for each head and turned by their rotary positions, in one pass: a row x becomes
+    x / sqrt(mean(x^2) + eps) * weight, and then what `rotary` makes of it.
+
+    query [B,H,N,D] and key [B,Hk,N,D] (or None: the queries alone, key_weight None too; the second result is None then),
+    both bf16 or fp32, head_dim contiguous with any other strides, 2 <= D <= 256; query_weight and key_weight [D], fp32 or
+    bf16 alike, one for all heads, or None for ones. positions, frequencies, layout and amplitude as `rotary` takes them.
+    fp32 throughout (a row's squares must not pass its range), rounded once to the rows' type. Differentiable in the rows
+    and the weights, once and backwards; the weights' gradients are the same bits from call to call. Captured into a graph:
+    for leaves that no eager graph still holds. `out` (optional, no gradient through it): the pair that receives the
+    results, each its input itself or memory that neither input shares."""
+    tensors = [t for t in (key, query_weight, key_weight) if t is not None]
+    _lib.require_one_gpu(query, *tensors, positions, frequencies, *(out or ()))
+    if layout not in LAYOUTS:
+        raise ValueError("layout is 'half' or 'interleaved'")
+    if query.dtype not in (torch.bfloat16, torch.float32):
+        raise TypeError('query must be bfloat16 or float32')
+    if query.dim() != 4 or query.stride(-1) != 1:
+        raise ValueError('query must be [B, H, N, D] with a contiguous head_dim')
+    B, H, N, D = query.shape
+    if not 2 <= D <= 256:
+        raise ValueError(f'head_dim {D} unsupported (2 to 256)')
+    if key is None:
+        if key_weight is not None:
+            raise ValueError('key_weight needs a key')
+    else:
+        if key.dtype != query.dtype:
+            raise TypeError('query and key must have one type')
+        if key.dim() != 4 or key.stride(-1) != 1 or (key.shape[0], key.shape[2], key.shape[3]) != (B, N, D):
+            raise ValueError('key must be [B, Hk, N, D] like query with a contiguous head_dim')
+    weights = [w for w in (query_weight, key_weight) if w is not None]
+    for w in weights:
+        if w.dtype not in (torch.bfloat16, torch.float32) or w.dtype != weights[0].dtype:
+            raise TypeError('weights must be bfloat16 or float32 alike')
+        if w.shape != (D,) or not w.is_contiguous():
+            raise ValueError('weights must be contiguous [head_dim] vectors')
+    if positions.dtype not in (torch.int32, torch.int64) or (positions.shape != (N,) and positions.shape != (B, N)):
+        raise ValueError(f'positions must be int32 or int64 [N] or [B, N], got {positions.dtype} {tuple(positions.shape)}')
+    if frequencies.dtype != torch.float64 or frequencies.dim() != 1 or not frequencies.is_contiguous():
+        raise ValueError('frequencies must be a contiguous fp64 vector')
+    if not 1 <= frequencies.numel() <= min(D // 2, 128):
+        raise ValueError(f'{frequencies.numel()} frequencies do not fit head_dim {D} (at most 128)')
+    eps = float(eps)
+    if not 0.0 <= eps < math.inf:
+        raise ValueError('eps must be 0 or more and finite')
+    how = positions, frequencies, eps, layout, float(amplitude)
+    leaves = [t for t in (query, key, query_weight, key_weight) if t is not None]
+    if out is None:
+        if any(map(_tracked, leaves)):
+            both = _NormRotary.apply(query, key, query_weight, key_weight, *how)
+            return (both, None) if key is None else both
+        return _normed(query, key, (query_weight, key_weight), (_like(query), _like(key)), *how)
+    if any(map(_tracked, [*leaves, *(t for t in out if t is not None)])):
+        raise ValueError('out= takes no part in a gradient')
+    if len(out) != 2 or (out[1] is None) != (key is None) or out[0] is None:
+        raise ValueError('out must be a pair like the results')
+    for x, o in zip((query, key), out):
+        if o is None:
+            continue
+        if o.shape != x.shape or o.dtype != x.dtype or o.stride(-1) != 1 or _lib.stacked(o):
+            raise ValueError("out must have its input's shape and type, a contiguous head_dim and a place for every element")
+        for other in (query, key):
+            same = other is x and o.data_ptr() == x.data_ptr() and o.stride() == x.stride()
+            if _lib.overlaps(o, other) and not same and not _apart(o, other):
+                raise ValueError('out must be its input itself or memory that neither input shares')
+    if out[1] is not None and _lib.overlaps(*out) and not _apart(*out):
+        raise ValueError('the two of out must not share memory')
+    return _normed(query, key, (query_weight, key_weight), tuple(out), *how)
+
+
+def _apart(a, b):
+    """True where two [B, H, N, D] tensors of one type lie side by side in the rows of one buffer: the same strides, and no
+    element of the one at a place of the other's."""
+    if a.stride()[0] != b.stride()[0] or a.stride()[1:] != b.stride()[1:] or a.shape[0] != b.shape[0]:
+        return False
+    # The heads of both in a token's row: [H a.., H b..] within the token's stride.
+    sb, sh, sn, _ = a.stride()
+    gap = (b.data_ptr() - a.data_ptr()) // a.element_size()
+    first, second = (a, b) if gap >= 0 else (b, a)
+    gap, D = abs(gap), a.shape[3]
+    if not D <= sh or not first.shape[1] * sh <= gap or not gap + second.shape[1] * sh <= sn:
+        return False
+    return a.shape[0] == 1 or a.shape[2] * sn <= sb
