@@ -481,7 +481,7 @@ typedef struct svhip_norm_rotary_args {
   double amplitude, eps;
 } svhip_norm_rotary_args;
 int svhip_norm_rotary(const svhip_norm_rotary_args* args, void* stream);
-size_t svhip_norm_rotary_workspace_bytes(int64_t B, int64_t N, int64_t D);
+size_t svhip_norm_rotary_workspace_bytes(int64_t B, int64_t H, int64_t Hk, int64_t N, int64_t D);
 int svhip_norm_rotary_grad(const svhip_norm_rotary_args* args, void* stream);
 
 /*

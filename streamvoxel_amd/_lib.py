@@ -91,7 +91,7 @@ SIGNATURES = {
     'svhip_paged_window_attention': (ctypes.c_int, [_c_b, _c_b, _c_i64, _c_i64, _c_p]),
     'svhip_paged_read': (ctypes.c_int, [_c_b, _c_b, _c_p]),
     'svhip_norm_rotary': (ctypes.c_int, [_c_b, _c_p]),
-    'svhip_norm_rotary_workspace_bytes': (_c_sz, [_c_i64] * 3),
+    'svhip_norm_rotary_workspace_bytes': (_c_sz, [_c_i64] * 5),
     'svhip_norm_rotary_grad': (ctypes.c_int, [_c_b, _c_p]),
 }
 

@@ -5,131 +5,117 @@
 // R(p)^T dy and c = w g: dw = sum over rows of g u, dx = (c - u mean(c u)) / sqrt(mean x^2 + eps). Sums in fp32, results rounded
 // once. The gradient forms u again from x: a pass over x is read anyway, and nothing is kept between the passes.
 //
-// Bound: HBM, every row read once and written once (gradient: x and dy read, dx written). Workgroup = up to kNormTokens
-// tokens of a window, all heads of queries and keys; their (cos, sin) go to LDS once. A group of LPR lanes carries a row, a
-// lane its pairs' 16 elements (two 8-element runs, half apart in the half layout), so that the row's sums are steps within
-// the group and a pair turns within its lane.
+// Bound: HBM, every row read once and written once (gradient: x and dy read, dx written). Workgroup = some tokens of a
+// window, all heads of the queries or of the keys; the tokens' (cos, sin) go to LDS once. A group of LPR lanes carries a
+// row, a lane its pairs' 16 elements (two 8-element runs, half apart in the half layout), so that the row's sums are steps
+// within the group, a pair turns within its lane, and a lane's weights stay in registers. A thread's first row is on its
+// way before the angles are formed, and the next one while it computes.
 #include "rotary.hpp"
 
 namespace svhip {
 
 constexpr int kNormThreads = 256;
-constexpr int kNormTokens = 8;
-constexpr int kNormAhead = 2;      // rows that a thread has in flight
+constexpr int kNormAngles = 2048;   // angles of a workgroup at most
 constexpr int kMaxNormDim = 256;
-constexpr int kNormGroups = 1024;  // workgroups of a gradient at most: each leaves its share of the weights' gradients
+constexpr int kNormGroups = 768;    // workgroups of a gradient at most: each leaves its share of a weight's gradient
 
 struct NormSide {
   const void *x, *dy, *w;
   void* out;      // y, or dx; null: not wanted
   int64_t sx_b, sx_h, sx_n, so_b, so_h, so_n, sd_b, sd_h, sd_n;
-  int H;
+  int H, tokens, tiles, groups;  // tokens: of a tile; tiles: of all windows; groups: workgroups of the gradient
 };
 
 struct NormArgs {
   NormSide side[2];
   const void* positions;
   const double* freq;
-  int64_t B, N, sp_b, sp_n, tiles;  // tiles: groups of `tokens` tokens, of every window
-  int D, half, turning, items, tokens;
-  bool wide, interleaved, wide_weights;
+  int64_t sp_b, sp_n;
+  int N;
+  RowItems row;
+  bool wide, wide_weights;
   float eps, amplitude;
-  float* partial;  // gradient: [workgroups][2][D], or null
+  float* partial;  // gradient: [workgroups][D], or null
 };
 
-// A lane's 16 elements of a row: 8 pairs, or 16 that are kept. Item e < turning has pairs 8 e ..
-template <bool VEC>
-struct Places {
-  int first, second;  // of elements 0 .. 7 and 8 .. 15
-  int n0, n1;         // how many of each there are (VEC: 0 or 8)
-  int step;           // from element to element (1; interleaved pairs lie side by side like kept ones)
-  int pair;           // first pair, or -1
-  __device__ __forceinline__ Places(const NormArgs& a, int e) {
-    if (e >= a.items) {
-      first = second = n0 = n1 = 0;
-      pair = -1;
-      return;
+// A lane's part of a row as it lies in memory.
+template <typename T, bool VEC>
+struct Part {
+  static constexpr int kWords = sizeof(T) / 2;
+  uint4 u[kWords], v[kWords];
+  __device__ __forceinline__ void load(const T* row, const Places& at) {
+#pragma unroll
+    for (int i = 0; i < kWords; ++i) u[i] = v[i] = make_uint4(0u, 0u, 0u, 0u);
+    if (at.n0) {
+#pragma unroll
+      for (int i = 0; i < kWords; ++i) u[i] = reinterpret_cast<const uint4*>(row + at.first)[i];
     }
-    const bool turns = e < a.turning;
-    pair = turns ? 8 * e : -1;
-    const int pairs = a.half - 8 * e < 8 ? a.half - 8 * e : 8;
-    if (turns && !a.interleaved) {
-      first = 8 * e;
-      second = a.half + 8 * e;
-      n0 = n1 = pairs;
+    if (at.n1) {
+#pragma unroll
+      for (int i = 0; i < kWords; ++i) v[i] = reinterpret_cast<const uint4*>(row + at.second)[i];
+    }
+  }
+  static __device__ __forceinline__ void words(const uint4 (&w)[kWords], float* x) {
+    if constexpr (kWords == 2) {
+      x[0] = __uint_as_float(w[0].x), x[1] = __uint_as_float(w[0].y), x[2] = __uint_as_float(w[0].z);
+      x[3] = __uint_as_float(w[0].w), x[4] = __uint_as_float(w[1].x), x[5] = __uint_as_float(w[1].y);
+      x[6] = __uint_as_float(w[1].z), x[7] = __uint_as_float(w[1].w);
     } else {
-      first = turns ? 16 * e : 2 * a.half + 16 * (e - a.turning);
-      second = first + 8;
-      const int n = turns ? 2 * pairs : (a.D - first < 16 ? a.D - first : 16);
-      n0 = n < 8 ? n : 8;
-      n1 = n - n0;
+      x[0] = __uint_as_float(w[0].x << 16), x[1] = __uint_as_float(w[0].x & 0xffff0000u);
+      x[2] = __uint_as_float(w[0].y << 16), x[3] = __uint_as_float(w[0].y & 0xffff0000u);
+      x[4] = __uint_as_float(w[0].z << 16), x[5] = __uint_as_float(w[0].z & 0xffff0000u);
+      x[6] = __uint_as_float(w[0].w << 16), x[7] = __uint_as_float(w[0].w & 0xffff0000u);
     }
+  }
+  __device__ __forceinline__ void get(float (&x)[16]) const {
+    words(u, x);
+    words(v, x + 8);
+  }
+  static __device__ __forceinline__ void store_words(T* p, const float* x) {
+    if constexpr (kWords == 2) {
+      reinterpret_cast<float4*>(p)[0] = make_float4(x[0], x[1], x[2], x[3]);
+      reinterpret_cast<float4*>(p)[1] = make_float4(x[4], x[5], x[6], x[7]);
+    } else {
+      *reinterpret_cast<uint4*>(p) =
+          make_uint4(bf16_pack2(x[0], x[1]), bf16_pack2(x[2], x[3]), bf16_pack2(x[4], x[5]), bf16_pack2(x[6], x[7]));
+    }
+  }
+  static __device__ __forceinline__ void store(T* row, const Places& at, const float (&x)[16]) {
+    if (at.n0) store_words(row + at.first, x);
+    if (at.n1) store_words(row + at.second, x + 8);
   }
 };
 
+// The same element by element.
 template <typename T>
-__device__ __forceinline__ void load_run(const T* p, float* x) {
-  if constexpr (sizeof(T) == 4) {
-    const float4 u = *reinterpret_cast<const float4*>(p), v = *reinterpret_cast<const float4*>(p + 4);
-    x[0] = u.x, x[1] = u.y, x[2] = u.z, x[3] = u.w, x[4] = v.x, x[5] = v.y, x[6] = v.z, x[7] = v.w;
-  } else {
-    const uint4 w = *reinterpret_cast<const uint4*>(p);
-    const uint32_t u[4] = {w.x, w.y, w.z, w.w};
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      x[2 * i] = __uint_as_float(u[i] << 16);
-      x[2 * i + 1] = __uint_as_float(u[i] & 0xffff0000u);
-    }
-  }
-}
-
-template <typename T, bool VEC>
-__device__ __forceinline__ void load_row(const T* row, const Places<VEC>& at, float (&x)[16]) {
-  if constexpr (VEC) {
-    if (at.n0) load_run<T>(row + at.first, x);
-    if (at.n1) load_run<T>(row + at.second, x + 8);
-  } else {
+struct Part<T, false> {
+  float x0[16];
+  __device__ __forceinline__ void load(const T* row, const Places& at) {
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      if (i < at.n0) x[i] = to_float<T>(row[at.first + i]);
-      if (i < at.n1) x[8 + i] = to_float<T>(row[at.second + i]);
+      x0[i] = i < at.n0 ? to_float<T>(row[at.first + i]) : 0.f;
+      x0[8 + i] = i < at.n1 ? to_float<T>(row[at.second + i]) : 0.f;
     }
   }
-}
-
-template <typename T>
-__device__ __forceinline__ void store_one(T* p, float v) {
-  if constexpr (sizeof(T) == 4) {
-    *p = v;
-  } else {
-    *p = bf16_bits(v);
+  __device__ __forceinline__ void get(float (&x)[16]) const {
+#pragma unroll
+    for (int i = 0; i < 16; ++i) x[i] = x0[i];
   }
-}
-
-template <typename T>
-__device__ __forceinline__ void store_run(T* p, const float* x) {
-  if constexpr (sizeof(T) == 4) {
-    *reinterpret_cast<float4*>(p) = make_float4(x[0], x[1], x[2], x[3]);
-    *reinterpret_cast<float4*>(p + 4) = make_float4(x[4], x[5], x[6], x[7]);
-  } else {
-    *reinterpret_cast<uint4*>(p) =
-        make_uint4(bf16_pack2(x[0], x[1]), bf16_pack2(x[2], x[3]), bf16_pack2(x[4], x[5]), bf16_pack2(x[6], x[7]));
+  static __device__ __forceinline__ void one(T* p, float v) {
+    if constexpr (sizeof(T) == 4) {
+      *p = v;
+    } else {
+      *p = bf16_bits(v);
+    }
   }
-}
-
-template <typename T, bool VEC>
-__device__ __forceinline__ void store_row(T* row, const Places<VEC>& at, const float (&x)[16]) {
-  if constexpr (VEC) {
-    if (at.n0) store_run<T>(row + at.first, x);
-    if (at.n1) store_run<T>(row + at.second, x + 8);
-  } else {
+  static __device__ __forceinline__ void store(T* row, const Places& at, const float (&x)[16]) {
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      if (i < at.n0) store_one<T>(row + at.first + i, x[i]);
-      if (i < at.n1) store_one<T>(row + at.second + i, x[8 + i]);
+      if (i < at.n0) one(row + at.first + i, x[i]);
+      if (i < at.n1) one(row + at.second + i, x[8 + i]);
     }
   }
-}
+};
 
 // Sum over the row's LPR lanes, in all of them.
 template <int LPR>
@@ -142,213 +128,199 @@ __device__ __forceinline__ float lanes_sum(float v) {
   return v;
 }
 
-// The lane's pairs turned by r = (cos, sin), sin by `sign`.
-__device__ __forceinline__ void turn_pairs(const NormArgs& a, float (&x)[16], const float2* angle, int pairs, float sign) {
+// The lane's pairs turned by `angle`'s (cos, sin), sin by `sign`.
+template <bool VEC, bool INTER>
+__device__ __forceinline__ void turn_pairs(float (&x)[16], const float2* angle, const Places& at, float sign) {
+  if (at.pairs == 0) return;
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
-    float2 r = make_float2(1.f, 0.f);
-    if (i < pairs) r = angle[i];
-    r.y *= sign;
-    if (a.interleaved) {
-      rotary_turn(x[2 * i], x[2 * i + 1], r);
-    } else {
-      rotary_turn(x[i], x[8 + i], r);
-    }
+    if (!VEC && i >= at.pairs) break;
+    const float2 r = make_float2(angle[i].x, sign * angle[i].y);
+    rotary_turn(x[INTER ? 2 * i : i], x[INTER ? 2 * i + 1 : 8 + i], r);
   }
 }
 
-// The weights of both sides into LDS as fp32 (ones where there are none).
-__device__ __forceinline__ void load_weights(const NormArgs& a, float (*weights)[kMaxNormDim]) {
-  for (int i = threadIdx.x; i < 2 * a.D; i += kNormThreads) {
-    const int side = i >= a.D, d = i - side * a.D;
-    const void* w = a.side[side].w;
-    weights[side][d] = !w ? 1.f
-                          : (a.wide_weights ? static_cast<const float*>(w)[d]
-                                            : bf16_bits_to_float(static_cast<const uint16_t*>(w)[d]));
+__device__ __forceinline__ void load_weights(const NormArgs& a, const void* w, const Places& at, float (&x)[16]) {
+#pragma unroll
+  for (int i = 0; i < 16; ++i) {
+    const int d = (i < 8 ? at.first : at.second - 8) + i;
+    const bool there = i < 8 ? i < at.n0 : i - 8 < at.n1;
+    x[i] = !there ? 0.f
+                  : (!w ? 1.f : (a.wide_weights ? static_cast<const float*>(w)[d]
+                                                : bf16_bits_to_float(static_cast<const uint16_t*>(w)[d])));
   }
 }
 
-// (cos, sin) of the tile's tokens.
-__device__ __forceinline__ void load_angles(const NormArgs& a, float2* table, int64_t b, int64_t n0, int tokens) {
-  for (int i = threadIdx.x; i < tokens * a.half; i += kNormThreads) {
-    const int row = i / a.half, pr = i - row * a.half;
+// (cos, sin) of a tile's tokens.
+__device__ __forceinline__ void form_angles(const NormArgs& a, float2* table, int64_t b, int n0, int tokens) {
+  for (int i = threadIdx.x; i < tokens * a.row.half; i += kNormThreads) {
+    const int row = i / a.row.half, pr = i - row * a.row.half;
     table[i] = rotary_phase(rotary_position(a.positions, a.wide, b * a.sp_b + (n0 + row) * a.sp_n), a.freq[pr], a.amplitude);
   }
 }
 
-template <bool VEC>
-__device__ __forceinline__ void weights_at(const float* weights, const Places<VEC>& at, float (&w)[16]) {
-#pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    w[i] = i < at.n0 ? weights[at.first + i] : 0.f;
-    w[8 + i] = i < at.n1 ? weights[at.second + i] : 0.f;
+// The rows of a tile that a thread's group carries, one after the other: token t of the tile, head h.
+template <int LPR>
+struct Walk {
+  int t, h, step_t, step_h, H;
+  __device__ __forceinline__ explicit Walk(int heads) {
+    constexpr int kStep = kNormThreads / LPR;
+    const int at = static_cast<int>(threadIdx.x) / LPR;
+    H = heads;
+    t = at / H;
+    h = at - t * H;
+    step_t = kStep / H;
+    step_h = kStep - step_t * H;
   }
-}
-
-template <typename T, bool VEC, int LPR>
-__global__ __launch_bounds__(kNormThreads) void norm_rotary_kernel(NormArgs a, unsigned first_group) {
-  __shared__ float2 table[kNormTokens * kMaxRotaryPairs];
-  __shared__ float weights[2][kMaxNormDim];
-  const unsigned per_window = static_cast<unsigned>((a.N + a.tokens - 1) / a.tokens);
-  const unsigned group = first_group + blockIdx.x, window = group / per_window;
-  const int64_t b = window, n0 = static_cast<int64_t>(group - window * per_window) * a.tokens;
-  const int tokens = static_cast<int>(a.N - n0 < a.tokens ? a.N - n0 : a.tokens);
-  const int e = static_cast<int>(threadIdx.x) % LPR, H0 = a.side[0].H, H = H0 + a.side[1].H;
-  const Places<VEC> at(a, e);
-  constexpr int kStep = kNormThreads / LPR;
-  const int step_t = kStep / H, step_h = kStep - step_t * H;
-  int t = static_cast<int>(threadIdx.x) / LPR / H, h = static_cast<int>(threadIdx.x) / LPR - t * H;
-  struct Row {
-    int t, h;
-    float x[16];
-  };
-  Row rows[kNormAhead];
-  auto load = [&](Row& r) __attribute__((always_inline)) {
-    r.t = t;
-    r.h = h;
-#pragma unroll
-    for (int i = 0; i < 16; ++i) r.x[i] = 0.f;
-    if (t < tokens) {
-      const NormSide& s = a.side[h < H0 ? 0 : 1];
-      load_row<T, VEC>(static_cast<const T*>(s.x) + b * s.sx_b + (h < H0 ? h : h - H0) * s.sx_h + (n0 + t) * s.sx_n, at, r.x);
-    }
+  __device__ __forceinline__ void next() {
     t += step_t;
     h += step_h;
     if (h >= H) {
       h -= H;
       ++t;
     }
+  }
+};
+
+template <typename T, bool VEC, bool INTER, int LPR>
+__global__ __launch_bounds__(kNormThreads) void norm_rotary_kernel(NormArgs a, unsigned first_group) {
+  __shared__ float2 table[kNormAngles];
+  const int group = static_cast<int>(first_group + blockIdx.x);
+  const bool keys = group >= a.side[0].tiles;
+  const NormSide s = keys ? a.side[1] : a.side[0];
+  const int tile = keys ? group - a.side[0].tiles : group, per_window = (a.N + s.tokens - 1) / s.tokens;
+  const int window = tile / per_window, n0 = (tile - window * per_window) * s.tokens;
+  const int tokens = a.N - n0 < s.tokens ? a.N - n0 : s.tokens;
+  const int64_t b = window;
+  const Places at = places_of<INTER>(a.row, static_cast<int>(threadIdx.x) % LPR);
+  const T* x = static_cast<const T*>(s.x) + b * s.sx_b + n0 * s.sx_n;
+  T* out = static_cast<T*>(s.out) + b * s.so_b + n0 * s.so_n;
+  Walk<LPR> walk(s.H);
+  Part<T, VEC> part;
+  auto load = [&]() __attribute__((always_inline)) {
+    if (walk.t < tokens) part.load(x + walk.h * s.sx_h + walk.t * s.sx_n, at);
   };
-#pragma unroll
-  for (int i = 0; i < kNormAhead; ++i) load(rows[i]);
-  load_weights(a, weights);
-  load_angles(a, table, b, n0, tokens);
+  load();
+  float w[16];
+  load_weights(a, s.w, at, w);
+  form_angles(a, table, b, n0, tokens);
   __syncthreads();
-  const float per = 1.f / static_cast<float>(a.D);
-  while (rows[0].t < tokens) {
+  const float per = 1.f / static_cast<float>(a.row.D);
+  while (walk.t < tokens) {  // (the same for the row's lanes)
+    const int t = walk.t, h = walk.h;
+    float y[16], sum = 0.f;
+    part.get(y);
+    walk.next();
+    load();
 #pragma unroll
-    for (int i = 0; i < kNormAhead; ++i) {
-      Row& r = rows[i];
-      if (r.t >= tokens) break;  // (the same for the row's lanes)
-      const int side = r.h < H0 ? 0 : 1;
-      const NormSide& s = a.side[side];
-      float sum = 0.f, w[16];
+    for (int j = 0; j < 16; ++j) sum = __builtin_fmaf(y[j], y[j], sum);
+    const float unit = rsqrtf(__builtin_fmaf(lanes_sum<LPR>(sum), per, a.eps));
 #pragma unroll
-      for (int j = 0; j < 16; ++j) sum = __builtin_fmaf(r.x[j], r.x[j], sum);
-      const float unit = rsqrtf(__builtin_fmaf(lanes_sum<LPR>(sum), per, a.eps));
-      weights_at<VEC>(weights[side], at, w);
-#pragma unroll
-      for (int j = 0; j < 16; ++j) r.x[j] = r.x[j] * unit * w[j];
-      if (at.pair >= 0) turn_pairs(a, r.x, table + r.t * a.half + at.pair, a.half - at.pair, 1.f);
-      store_row<T, VEC>(static_cast<T*>(s.out) + b * s.so_b + (side ? r.h - H0 : r.h) * s.so_h + (n0 + r.t) * s.so_n, at, r.x);
-    }
-#pragma unroll
-    for (int i = 0; i < kNormAhead; ++i) load(rows[i]);
+    for (int j = 0; j < 16; ++j) y[j] = y[j] * unit * w[j];
+    turn_pairs<VEC, INTER>(y, table + t * a.row.half + at.pair, at, 1.f);
+    Part<T, VEC>::store(out + h * s.so_h + t * s.so_n, at, y);
   }
 }
 
-template <typename T, bool VEC, int LPR>
+template <typename T, bool VEC, bool INTER, int LPR>
 __global__ __launch_bounds__(kNormThreads) void norm_rotary_grad_kernel(NormArgs a) {
-  __shared__ float2 table[kNormTokens * kMaxRotaryPairs];
-  __shared__ float weights[2][kMaxNormDim];
+  __shared__ float2 table[kNormAngles];
   __shared__ float sums[kNormThreads / 64][LPR][16];
-  const unsigned per_window = static_cast<unsigned>((a.N + a.tokens - 1) / a.tokens);
-  const int e = static_cast<int>(threadIdx.x) % LPR;
-  const Places<VEC> at(a, e);
-  constexpr int kStep = kNormThreads / LPR;
-  const float per = 1.f / static_cast<float>(a.D);
-  load_weights(a, weights);
-  float dw[2][16];
+  const int group = static_cast<int>(blockIdx.x);
+  const bool keys = group >= a.side[0].groups;
+  const NormSide s = keys ? a.side[1] : a.side[0];
+  const int per_window = (a.N + s.tokens - 1) / s.tokens;
+  const Places at = places_of<INTER>(a.row, static_cast<int>(threadIdx.x) % LPR);
+  const float per = 1.f / static_cast<float>(a.row.D);
+  float w[16], dw[16];
+  load_weights(a, s.w, at, w);
 #pragma unroll
-  for (int i = 0; i < 16; ++i) dw[0][i] = dw[1][i] = 0.f;
-  for (unsigned group = blockIdx.x; group < static_cast<unsigned>(a.tiles); group += gridDim.x) {
-    const unsigned window = group / per_window;
-    const int64_t b = window, n0 = static_cast<int64_t>(group - window * per_window) * a.tokens;
-    const int tokens = static_cast<int>(a.N - n0 < a.tokens ? a.N - n0 : a.tokens);
+  for (int i = 0; i < 16; ++i) dw[i] = 0.f;
+  for (int tile = keys ? group - a.side[0].groups : group; tile < s.tiles; tile += s.groups) {
+    const int window = tile / per_window, n0 = (tile - window * per_window) * s.tokens;
+    const int tokens = a.N - n0 < s.tokens ? a.N - n0 : s.tokens;
+    const int64_t b = window;
+    const T* x = static_cast<const T*>(s.x) + b * s.sx_b + n0 * s.sx_n;
+    const T* dy = static_cast<const T*>(s.dy) + b * s.sd_b + n0 * s.sd_n;
+    T* dx = static_cast<T*>(s.out) + b * s.so_b + n0 * s.so_n;
+    Walk<LPR> walk(s.H);
+    int t, h;
+    Part<T, VEC> xs, gs;
+    auto load = [&]() __attribute__((always_inline)) {
+      t = walk.t;
+      h = walk.h;
+      if (t < tokens) {
+        xs.load(x + h * s.sx_h + t * s.sx_n, at);
+        gs.load(dy + h * s.sd_h + t * s.sd_n, at);
+      }
+      walk.next();
+    };
+    load();
     __syncthreads();  // the angles are read until here
-    load_angles(a, table, b, n0, tokens);
+    form_angles(a, table, b, n0, tokens);
     __syncthreads();
+    while (t < tokens) {
+      float u[16], g[16];
+      const int head = h, now = t;
+      xs.get(u);
+      gs.get(g);
+      load();
+      turn_pairs<VEC, INTER>(g, table + now * a.row.half + at.pair, at, -1.f);
+      float sum = 0.f, dot = 0.f;
 #pragma unroll
-    for (int side = 0; side < 2; ++side) {
-      const NormSide& s = a.side[side];
-      const int H = s.H;
-      if (H == 0) continue;
-      float w[16];
-      weights_at<VEC>(weights[side], at, w);
-      const int step_t = kStep / H, step_h = kStep - step_t * H;
-      int t = static_cast<int>(threadIdx.x) / LPR / H, h = static_cast<int>(threadIdx.x) / LPR - t * H;
-      while (t < tokens) {
-        float x[16], g[16];
+      for (int i = 0; i < 16; ++i) sum = __builtin_fmaf(u[i], u[i], sum);
+      const float unit = rsqrtf(__builtin_fmaf(lanes_sum<LPR>(sum), per, a.eps));
 #pragma unroll
-        for (int i = 0; i < 16; ++i) x[i] = g[i] = 0.f;
-        load_row<T, VEC>(static_cast<const T*>(s.x) + b * s.sx_b + h * s.sx_h + (n0 + t) * s.sx_n, at, x);
-        load_row<T, VEC>(static_cast<const T*>(s.dy) + b * s.sd_b + h * s.sd_h + (n0 + t) * s.sd_n, at, g);
-        float sum = 0.f, dot = 0.f;
-        if (at.pair >= 0) turn_pairs(a, g, table + t * a.half + at.pair, a.half - at.pair, -1.f);
-#pragma unroll
-        for (int i = 0; i < 16; ++i) sum = __builtin_fmaf(x[i], x[i], sum);
-        const float unit = rsqrtf(__builtin_fmaf(lanes_sum<LPR>(sum), per, a.eps));
-#pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          x[i] *= unit;
-          dw[side][i] = __builtin_fmaf(g[i], x[i], dw[side][i]);
-          g[i] *= w[i];
-          dot = __builtin_fmaf(g[i], x[i], dot);
-        }
+      for (int i = 0; i < 16; ++i) {
+        u[i] *= unit;
+        dw[i] = __builtin_fmaf(g[i], u[i], dw[i]);
+        g[i] *= w[i];
+        dot = __builtin_fmaf(g[i], u[i], dot);
+      }
+      if (s.out) {
         dot = lanes_sum<LPR>(dot) * per;
-        if (s.out) {
 #pragma unroll
-          for (int i = 0; i < 16; ++i) g[i] = unit * __builtin_fmaf(-x[i], dot, g[i]);
-          store_row<T, VEC>(static_cast<T*>(s.out) + b * s.so_b + h * s.so_h + (n0 + t) * s.so_n, at, g);
-        }
-        t += step_t;
-        h += step_h;
-        if (h >= H) {
-          h -= H;
-          ++t;
-        }
+        for (int i = 0; i < 16; ++i) g[i] = unit * __builtin_fmaf(-u[i], dot, g[i]);
+        Part<T, VEC>::store(dx + head * s.so_h + now * s.so_n, at, g);
       }
     }
   }
   if (!a.partial) return;
   // The workgroup's sums: over a wave's rows, then over its waves, in order.
 #pragma unroll
-  for (int side = 0; side < 2; ++side) {
+  for (int i = 0; i < 16; ++i) {
+#pragma unroll
+    for (int x = LPR; x < 64; x *= 2) dw[i] += __shfl_xor(dw[i], x);
+  }
+  if ((threadIdx.x & 63) < LPR) {
+#pragma unroll
+    for (int i = 0; i < 16; ++i) sums[threadIdx.x >> 6][threadIdx.x & 63][i] = dw[i];
+  }
+  __syncthreads();
+  if (threadIdx.x < LPR) {
+    float* to = a.partial + static_cast<int64_t>(group) * a.row.D;
 #pragma unroll
     for (int i = 0; i < 16; ++i) {
-#pragma unroll
-      for (int x = LPR; x < 64; x *= 2) dw[side][i] += __shfl_xor(dw[side][i], x);
-    }
-    __syncthreads();
-    if ((threadIdx.x & 63) < LPR) {
-#pragma unroll
-      for (int i = 0; i < 16; ++i) sums[threadIdx.x >> 6][e][i] = dw[side][i];
-    }
-    __syncthreads();
-    if (threadIdx.x < LPR) {
-      float* to = a.partial + (static_cast<int64_t>(blockIdx.x) * 2 + side) * a.D;
-#pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        float v = 0.f;
-        for (int k = 0; k < kNormThreads / 64; ++k) v += sums[k][e][i];
-        if (i < 8 ? i < at.n0 : i - 8 < at.n1) to[(i < 8 ? at.first : at.second - 8) + i] = v;
-      }
+      float v = 0.f;
+      for (int k = 0; k < kNormThreads / 64; ++k) v += sums[k][threadIdx.x][i];
+      if (i < 8 ? i < at.n0 : i - 8 < at.n1) to[(i < 8 ? at.first : at.second - 8) + i] = v;
     }
   }
 }
 
 // The workgroups' shares of the weights' gradients summed in order: workgroup = 32 elements of a side, 32 threads each.
-__global__ __launch_bounds__(1024) void norm_weight_kernel(const float* partial, int groups, int D, int tiles, bool wide,
-                                                           void* dq, void* dk) {
+__global__ __launch_bounds__(1024) void norm_weight_kernel(const float* partial, int q_groups, int k_groups, int D, int blocks,
+                                                           bool wide, void* dq, void* dk) {
   __shared__ float sums[32][33];
-  const int side = blockIdx.x / tiles, d = (blockIdx.x - side * tiles) * 32 + threadIdx.x % 32, part = threadIdx.x / 32;
+  const int side = blockIdx.x / blocks, d = (blockIdx.x - side * blocks) * 32 + threadIdx.x % 32, part = threadIdx.x / 32;
   void* to = side ? dk : dq;
   if (!to) return;
+  const int first = side ? q_groups : 0, groups = side ? k_groups : q_groups;
   float v = 0.f;
   if (d < D) {
-    const float* from = partial + static_cast<int64_t>(side) * D + d;
+    const float* from = partial + static_cast<int64_t>(first) * D + d;
 #pragma unroll 8
-    for (int g = part; g < groups; g += 32) v += from[static_cast<int64_t>(g) * 2 * D];
+    for (int g = part; g < groups; g += 32) v += from[static_cast<int64_t>(g) * D];
   }
   sums[part][threadIdx.x % 32] = v;
   __syncthreads();
@@ -362,35 +334,51 @@ __global__ __launch_bounds__(1024) void norm_weight_kernel(const float* partial,
   }
 }
 
-template <typename T, bool VEC, int LPR>
-void launch_norm(const NormArgs& a, int64_t grad_groups, hipStream_t s) {
-  if (grad_groups > 0) {
-    norm_rotary_grad_kernel<T, VEC, LPR><<<static_cast<unsigned>(grad_groups), kNormThreads, 0, s>>>(a);
+template <typename T, bool VEC, bool INTER, int LPR>
+void launch_norm(const NormArgs& a, bool grad, hipStream_t s) {
+  if (grad) {
+    const int groups = a.side[0].groups + a.side[1].groups;
+    norm_rotary_grad_kernel<T, VEC, INTER, LPR><<<static_cast<unsigned>(groups), kNormThreads, 0, s>>>(a);
   } else {
-    in_launches(a.tiles, [&](unsigned first, unsigned grid) {
-      norm_rotary_kernel<T, VEC, LPR><<<grid, kNormThreads, 0, s>>>(a, first);
+    in_launches(static_cast<int64_t>(a.side[0].tiles) + a.side[1].tiles, [&](unsigned first, unsigned grid) {
+      norm_rotary_kernel<T, VEC, INTER, LPR><<<grid, kNormThreads, 0, s>>>(a, first);
     });
   }
 }
 
-template <typename T, bool VEC>
-void launch_norm(const NormArgs& a, int64_t grad_groups, hipStream_t s) {
-  if (a.items <= 4) {
-    launch_norm<T, VEC, 4>(a, grad_groups, s);
-  } else if (a.items <= 8) {
-    launch_norm<T, VEC, 8>(a, grad_groups, s);
-  } else if (a.items <= 16) {
-    launch_norm<T, VEC, 16>(a, grad_groups, s);
-  } else {
-    launch_norm<T, VEC, 32>(a, grad_groups, s);
+template <typename T, bool VEC, bool INTER>
+void launch_norm(const NormArgs& a, bool grad, hipStream_t s) {
+  switch (row_lanes(a.row)) {
+    case 4: return launch_norm<T, VEC, INTER, 4>(a, grad, s);
+    case 8: return launch_norm<T, VEC, INTER, 8>(a, grad, s);
+    case 16: return launch_norm<T, VEC, INTER, 16>(a, grad, s);
+    default: return launch_norm<T, VEC, INTER, 32>(a, grad, s);
   }
 }
 
-int64_t norm_tokens(int64_t B, int64_t N) { return tokens_per_group(B * N, kNormTokens); }
+template <typename T>
+void launch_norm(const NormArgs& a, bool vec, bool interleaved, bool grad, hipStream_t s) {
+  if (interleaved) {
+    vec ? launch_norm<T, true, true>(a, grad, s) : launch_norm<T, false, true>(a, grad, s);
+  } else {
+    vec ? launch_norm<T, true, false>(a, grad, s) : launch_norm<T, false, false>(a, grad, s);
+  }
+}
 
-int64_t norm_grad_groups(int64_t B, int64_t N) {
-  const int64_t tiles = B * cdiv(N, norm_tokens(B, N));
-  return tiles < kNormGroups ? tiles : kNormGroups;
+// Tokens of a tile: as many as give every thread kNormRows rows, if that leaves two workgroups for every CU.
+constexpr int64_t kNormRows = 4;
+int64_t norm_tokens(int64_t B, int64_t H, int64_t N, int64_t lanes, int64_t half) {
+  int64_t n = kNormRows * kNormThreads / lanes / (H > 0 ? H : 1);
+  if (n > kNormAngles / half) n = kNormAngles / half;
+  if (n > B * N / 512) n = B * N / 512;
+  if (n > N) n = N;
+  return n < 1 ? 1 : n;
+}
+
+// Workgroups of a side's gradient: its share of kNormGroups by its heads.
+int64_t norm_groups(int64_t tiles, int64_t H, int64_t all) {
+  const int64_t most = H * kNormGroups / all > 0 ? H * kNormGroups / all : 1;
+  return H == 0 ? 0 : (tiles < most ? tiles : most);
 }
 
 int norm_rotary(const char* name, const svhip_norm_rotary_args* args, bool grad, void* stream) {
@@ -408,14 +396,14 @@ int norm_rotary(const char* name, const svhip_norm_rotary_args* args, bool grad,
                 (long long)c.pairs, (long long)c.D);
   SVHIP_REQUIRE(c.eps >= 0. && c.eps < INFINITY, "%s: eps must be 0 or more and finite", name);
   const bool weighed = grad && (c.dq_weight || c.dk_weight);
-  const int64_t groups = c.B * c.N > 0 ? norm_grad_groups(c.B, c.N) : 0, bytes = groups * 2 * c.D * 4;
+  const int half = static_cast<int>(c.pairs), D = static_cast<int>(c.D);
+  const int blocks = static_cast<int>(cdiv(D, 32));
+  hipStream_t s = as_stream(stream);
   if (c.B == 0 || c.N == 0 || c.H + c.Hk == 0) {
     // No rows: the weights' gradients are zeros.
-    hipStream_t s = as_stream(stream);
-    const int tiles = static_cast<int>(cdiv(c.D, 32));
     if (weighed) {
-      norm_weight_kernel<<<2 * tiles, 1024, 0, s>>>(nullptr, 0, static_cast<int>(c.D), tiles, c.weight_dtype == SVHIP_F32,
-                                                    c.dq_weight, c.dk_weight);
+      norm_weight_kernel<<<2 * blocks, 1024, 0, s>>>(nullptr, 0, 0, D, blocks, c.weight_dtype == SVHIP_F32, c.dq_weight,
+                                                     c.dk_weight);
       SVHIP_LAUNCHED(name);
     }
     return SVHIP_OK;
@@ -423,42 +411,40 @@ int norm_rotary(const char* name, const svhip_norm_rotary_args* args, bool grad,
   SVHIP_REQUIRE((c.H == 0 || (c.q && (grad ? c.dq != nullptr : c.out_q != nullptr))) &&
                     (c.Hk == 0 || (c.k && (grad ? c.dk != nullptr : c.out_k != nullptr))) && c.positions && c.freq,
                 "%s: null pointer", name);
+  NormArgs a{{{c.q, c.dq, c.q_weight, c.out_q, c.sq_b, c.sq_h, c.sq_n, c.soq_b, c.soq_h, c.soq_n, c.sdq_b, c.sdq_h, c.sdq_n,
+               static_cast<int>(c.H), 1, 0, 0},
+              {c.k, c.dk, c.k_weight, c.out_k, c.sk_b, c.sk_h, c.sk_n, c.sok_b, c.sok_h, c.sok_n, c.sdk_b, c.sdk_h, c.sdk_n,
+               static_cast<int>(c.Hk), 1, 0, 0}},
+             c.positions, c.freq, c.sp_b, c.sp_n, static_cast<int>(c.N), row_items(D, half),
+             c.positions_wide != 0, c.weight_dtype == SVHIP_F32, static_cast<float>(c.eps), static_cast<float>(c.amplitude),
+             weighed ? static_cast<float*>(c.workspace) : nullptr};
+  const int64_t run = c.dtype == SVHIP_F32 ? 4 : 8;
+  bool vec = half % 8 == 0 && D % 8 == 0;
+  int64_t all = 0;
+  for (NormSide& side : a.side) {
+    if (side.H == 0) continue;
+    const auto on16 = [&](const void* p, int64_t b, int64_t h, int64_t n) {
+      return reinterpret_cast<uintptr_t>(p) % 16 == 0 &&
+             (used_stride(c.B, b) | used_stride(side.H, h) | used_stride(c.N, n)) % run == 0;
+    };
+    vec = vec && on16(side.x, side.sx_b, side.sx_h, side.sx_n) && on16(side.out, side.so_b, side.so_h, side.so_n) &&
+          (!grad || on16(side.dy, side.sd_b, side.sd_h, side.sd_n));
+    const int64_t tokens = norm_tokens(c.B, side.H, c.N, row_lanes(a.row), half), tiles = c.B * cdiv(c.N, tokens);
+    all += tiles;
+    SVHIP_REQUIRE(all < (1ll << 31), "%s: grid too large", name);
+    side.tokens = static_cast<int>(tokens);
+    side.tiles = static_cast<int>(tiles);
+    side.groups = static_cast<int>(norm_groups(tiles, side.H, c.H + c.Hk));
+  }
+  const int64_t bytes = (static_cast<int64_t>(a.side[0].groups) + a.side[1].groups) * D * 4;
   SVHIP_REQUIRE(!weighed || (c.workspace && c.workspace_bytes >= bytes && reinterpret_cast<uintptr_t>(c.workspace) % 4 == 0),
                 "%s: workspace too small or misaligned (%lld < %lld bytes)", name, (long long)c.workspace_bytes,
                 (long long)bytes);
-  const int64_t tokens = norm_tokens(c.B, c.N), tiles = c.B * cdiv(c.N, tokens);
-  SVHIP_REQUIRE(tiles < (1ll << 31), "%s: grid too large", name);
-  const int half = static_cast<int>(c.pairs), D = static_cast<int>(c.D), turning = (half + 7) / 8;
-  const NormArgs a{{{c.q, c.dq, c.q_weight, c.out_q, c.sq_b, c.sq_h, c.sq_n, c.soq_b, c.soq_h, c.soq_n, c.sdq_b, c.sdq_h, c.sdq_n,
-                     static_cast<int>(c.H)},
-                    {c.k, c.dk, c.k_weight, c.out_k, c.sk_b, c.sk_h, c.sk_n, c.sok_b, c.sok_h, c.sok_n, c.sdk_b, c.sdk_h, c.sdk_n,
-                     static_cast<int>(c.Hk)}},
-                   c.positions, c.freq, c.B, c.N, c.sp_b, c.sp_n, tiles, D, half, turning,
-                   turning + (D - 2 * half + 15) / 16, static_cast<int>(tokens), c.positions_wide != 0,
-                   c.layout == SVHIP_ROTARY_INTERLEAVED, c.weight_dtype == SVHIP_F32, static_cast<float>(c.eps),
-                   static_cast<float>(c.amplitude), weighed ? static_cast<float*>(c.workspace) : nullptr};
-  const int64_t run = c.dtype == SVHIP_F32 ? 4 : 8;
-  bool vec = half % 8 == 0 && D % 8 == 0;
-  for (const NormSide& s : a.side) {
-    if (s.H == 0) continue;
-    const auto on16 = [&](const void* p, int64_t b, int64_t h, int64_t n) {
-      return reinterpret_cast<uintptr_t>(p) % 16 == 0 &&
-             (used_stride(c.B, b) | used_stride(s.H, h) | used_stride(c.N, n)) % run == 0;
-    };
-    vec = vec && on16(s.x, s.sx_b, s.sx_h, s.sx_n) && on16(s.out, s.so_b, s.so_h, s.so_n) &&
-          (!grad || on16(s.dy, s.sd_b, s.sd_h, s.sd_n));
-  }
-  hipStream_t s = as_stream(stream);
-  const int64_t launched = grad ? groups : 0;
-  if (c.dtype == SVHIP_F32) {
-    vec ? launch_norm<float, true>(a, launched, s) : launch_norm<float, false>(a, launched, s);
-  } else {
-    vec ? launch_norm<uint16_t, true>(a, launched, s) : launch_norm<uint16_t, false>(a, launched, s);
-  }
+  const bool interleaved = c.layout == SVHIP_ROTARY_INTERLEAVED;
+  c.dtype == SVHIP_F32 ? launch_norm<float>(a, vec, interleaved, grad, s) : launch_norm<uint16_t>(a, vec, interleaved, grad, s);
   if (weighed) {
-    const int blocks = static_cast<int>(cdiv(c.D, 32));
-    norm_weight_kernel<<<2 * blocks, 1024, 0, s>>>(a.partial, static_cast<int>(groups), D, blocks, a.wide_weights, c.dq_weight,
-                                                   c.dk_weight);
+    norm_weight_kernel<<<2 * blocks, 1024, 0, s>>>(a.partial, a.side[0].groups, a.side[1].groups, D, blocks, a.wide_weights,
+                                                   c.dq_weight, c.dk_weight);
   }
   SVHIP_LAUNCHED(name);
   return SVHIP_OK;
@@ -472,9 +458,11 @@ extern "C" int svhip_norm_rotary(const svhip_norm_rotary_args* args, void* strea
   return norm_rotary("svhip_norm_rotary", args, false, stream);
 }
 
-extern "C" size_t svhip_norm_rotary_workspace_bytes(int64_t B, int64_t N, int64_t D) {
-  if (B < 1 || B >= 1ll << 31 || N < 1 || N >= 1ll << 31 || D < 1 || D > kMaxNormDim) return 0;
-  return static_cast<size_t>(norm_grad_groups(B, N) * 2 * D * 4);
+extern "C" size_t svhip_norm_rotary_workspace_bytes(int64_t B, int64_t H, int64_t Hk, int64_t N, int64_t D) {
+  if (B < 1 || H < 0 || Hk < 0 || H + Hk < 1 || N < 1 || D < 1 || D > kMaxNormDim) return 0;
+  // (A window of one token has a tile at least, and a side one workgroup.)
+  const int64_t most = B < kNormGroups / N + 1 ? B * N + 1 : kNormGroups;
+  return static_cast<size_t>(2 * (most < kNormGroups ? most : kNormGroups) * D * 4);
 }
 
 extern "C" int svhip_norm_rotary_grad(const svhip_norm_rotary_args* args, void* stream) {

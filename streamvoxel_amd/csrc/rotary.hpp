@@ -34,6 +34,47 @@ __device__ __forceinline__ void rotary_turn(float& a, float& b, float2 r) {
   b = __builtin_fmaf(b, r.x, x * r.y);
 }
 
+// A row of D elements, its first `half` pairs turning, as items of 16 elements each: item e < turning has pairs 8 e .., two
+// runs of 8 elements half apart (half layout) or side by side (interleaved); the others have 16 elements that are kept. A
+// lane that carries an item turns its pairs by itself.
+struct RowItems {
+  int D, half, turning, items;
+};
+inline RowItems row_items(int D, int half) {
+  const int turning = (half + 7) / 8;
+  return RowItems{D, half, turning, turning + (D - 2 * half + 15) / 16};
+}
+// Lanes of a row: a power of two that holds its items.
+inline int row_lanes(const RowItems& r) { return r.items <= 4 ? 4 : (r.items <= 8 ? 8 : (r.items <= 16 ? 16 : 32)); }
+
+struct Places {
+  int first, second;  // of elements 0 .. 7 and 8 .. 15
+  int n0, n1;         // how many of each there are (whole runs: 0 or 8)
+  int pair, pairs;    // the first pair, and how many (0: kept)
+};
+
+template <bool INTER>
+__device__ __forceinline__ Places places_of(const RowItems& r, int e) {
+  Places p{0, 0, 0, 0, 0, 0};
+  if (e >= r.items) return p;
+  if (e < r.turning) {
+    p.pair = 8 * e;
+    p.pairs = r.half - 8 * e < 8 ? r.half - 8 * e : 8;
+  }
+  if (!INTER && e < r.turning) {
+    p.first = 8 * e;
+    p.second = r.half + 8 * e;
+    p.n0 = p.n1 = p.pairs;
+  } else {
+    p.first = e < r.turning ? 16 * e : 2 * r.half + 16 * (e - r.turning);
+    p.second = p.first + 8;
+    const int n = e < r.turning ? 2 * p.pairs : (r.D - p.first < 16 ? r.D - p.first : 16);
+    p.n0 = n < 8 ? n : 8;
+    p.n1 = n - p.n0;
+  }
+  return p;
+}
+
 // Tokens of a workgroup: as many as leave two workgroups for every CU, up to `most` (1024 tokens of 16 x 128: rotation
 // 4.1 us, append 5.6; eight in every workgroup 5.4 and 8.9; 520 tokens 3.8 and 4.4, 5.1 and 8.2).
 inline int64_t tokens_per_group(int64_t total, int64_t most) {

@@ -116,13 +116,13 @@ def test_norm_rotary_refusals(lib, name):
     for sizes in ((0, 1, 1, 1, 64), (1, 0, 0, 1, 64), (1, 1, 1, 0, 64)):
         assert call(sizes=sizes) == 0
     if grad:
-        need = lib.svhip_norm_rotary_workspace_bytes(1, 3, 64)
-        assert need >= 2 * 64 * 4
-        for how in (dict(ws=0, nbytes=need), dict(ws=FAKE, nbytes=need - 1), dict(ws=FAKE + 2, nbytes=need)):
+        need = lib.svhip_norm_rotary_workspace_bytes(1, 4, 2, 3, 64)
+        assert need >= 2 * 3 * 64 * 4
+        for how in (dict(ws=0, nbytes=need), dict(ws=FAKE, nbytes=64 * 4), dict(ws=FAKE + 2, nbytes=need)):
             assert call(dwq=FAKE, **how) == -1 and b'workspace' in lib.svhip_last_error()
     assert getattr(lib, name)(None, None) == -1 and b'null' in lib.svhip_last_error()
-    assert lib.svhip_norm_rotary_workspace_bytes(0, 3, 64) == 0
-    assert lib.svhip_norm_rotary_workspace_bytes(1 << 20, 1 << 20, 256) == 1024 * 2 * 256 * 4
+    assert lib.svhip_norm_rotary_workspace_bytes(0, 1, 1, 3, 64) == lib.svhip_norm_rotary_workspace_bytes(1, 0, 0, 3, 64) == 0
+    assert lib.svhip_norm_rotary_workspace_bytes(1 << 20, 8, 8, 1 << 20, 256) == 768 * 2 * 256 * 4
 
 
 def test_host_tensors_are_refused():
