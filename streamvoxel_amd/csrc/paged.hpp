@@ -93,18 +93,24 @@ __device__ __forceinline__ int row_exponent(float bound) {
 __device__ __forceinline__ float exponent_value(int code) { return __uint_as_float(static_cast<uint32_t>(code) << 23); }
 
 // int8 blocks: whole numbers of at most kInt8Most times a power of two of at most 2^(kInt8Top - 127), the largest of them
-// with 127 of it in bf16. (A larger byte is read as that: a code's value is then finite whatever stands there.)
+// with 127 of it in bf16. (Other bytes are read as the nearest of these: a code's value is finite whatever stands there, and a
+// score of -inf stays one when it is scaled.)
 constexpr int kInt8Top = 248;
 constexpr float kInt8Most = 127.f;
 __device__ __forceinline__ float int8_power(uint32_t byte) {
-  return exponent_value(static_cast<int>(byte < static_cast<uint32_t>(kInt8Top) ? byte : kInt8Top));
+  const int e = static_cast<int>(byte);
+  return exponent_value(e < 1 ? 1 : (e < kInt8Top ? e : kInt8Top));
 }
 
-// 8 int8 codes times a power of two f as bf16: 7 bits of magnitude, exact.
-__device__ __forceinline__ uint4 int8_values(uint2 w, float f) {
+// 8 int8 codes, as they are or times a power of two f, as bf16: 7 bits of magnitude, exact.
+template <bool SCALED = true>
+__device__ __forceinline__ uint4 int8_values(uint2 w, float f = 1.f) {
   float x[8];
 #pragma unroll
-  for (int i = 0; i < 8; ++i) x[i] = static_cast<float>(static_cast<int8_t>((i < 4 ? w.x : w.y) >> 8 * (i & 3))) * f;
+  for (int i = 0; i < 8; ++i) {
+    x[i] = static_cast<float>(static_cast<int8_t>((i < 4 ? w.x : w.y) >> 8 * (i & 3)));
+    if constexpr (SCALED) x[i] *= f;
+  }
   return make_uint4(bf16_pack2(x[0], x[1]), bf16_pack2(x[2], x[3]), bf16_pack2(x[4], x[5]), bf16_pack2(x[6], x[7]));
 }
 

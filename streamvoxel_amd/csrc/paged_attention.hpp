@@ -360,13 +360,20 @@ __device__ __forceinline__ f32x16_t scores(const Rows<KS>& s, const bf16x8_t (&k
   return x;
 }
 
+// int8: a block's keys enter the score product as their codes; what 16 of them stand for, a power of two, is put to the scores
+// (an FMA's factor where the weights are formed) and not to every element of the keys: 32 kHalves keys, 16 each.
+template <int kHalves>
+struct KeyScales {
+  float of[2 * kHalves];
+};
+
 // Scores x of a block of 32 kHalves keys, `key0` the first: those that a row does not see masked, and the running
 // maximum moved for a score more than kMaxHigh above it (the weights then stay below 2^20, which fp32 sums and bf16
 // hold alike). One such branch a block: a second one in a loop makes the compiler merge two register sets of O behind
 // it, a copy that the common path pays.
-template <bool WIN, int KS, int kHalves>
-__device__ __forceinline__ void bound_scores(const PagedArgs& a, Rows<KS>& s, f32x16_t (&x)[kHalves], bool masked,
-                                             int key0) {
+template <int ST, bool WIN, int KS, int kHalves>
+__device__ __forceinline__ void bound_scores(const PagedArgs& a, Rows<KS>& s, f32x16_t (&x)[kHalves], const KeyScales<kHalves>& f,
+                                             bool masked, int key0) {
   const float sl2 = a.scale_log2;
   const int hh = (threadIdx.x & 63) >> 5;
   if (masked) {
@@ -393,6 +400,13 @@ __device__ __forceinline__ void bound_scores(const PagedArgs& a, Rows<KS>& s, f3
 #pragma unroll
   for (int t = 0; t < kHalves; ++t) {
     const f32x16_t& y = x[t];
+    if constexpr (ST == kInt8) {
+      const float lo = max3(max3(y[0], y[1], y[2]), max3(y[3], y[4], y[5]), __builtin_elementwise_maximum(y[6], y[7]));
+      const float hi = max3(max3(y[8], y[9], y[10]), max3(y[11], y[12], y[13]), __builtin_elementwise_maximum(y[14], y[15]));
+      const float h = __builtin_elementwise_maximum(lo * f.of[2 * t], hi * f.of[2 * t + 1]);
+      mx = t == 0 ? h : __builtin_elementwise_maximum(mx, h);
+      continue;
+    }
     const float h = max3(max3(max3(y[0], y[1], y[2]), max3(y[3], y[4], y[5]), max3(y[6], y[7], y[8])),
                          max3(y[9], y[10], y[11]), max3(max3(y[12], y[13], y[14]), y[15], y[15]));
     mx = t == 0 ? h : __builtin_elementwise_maximum(mx, h);
@@ -419,11 +433,13 @@ __device__ __forceinline__ void bound_scores(const PagedArgs& a, Rows<KS>& s, f3
 // what a rounding adds to the one it adds to the other: 0.0022 from 64 bits, relative, where weights in
 // fp32 leave the result's own rounding, 0.0017. m is the rounded product of a score: beyond scores of
 // 2^30 what its rounding leaves of the largest weight's exponent no longer fits fp32, and the row is NaN.
-template <int KS>
-__device__ __forceinline__ void weights_of(const Rows<KS>& s, const f32x16_t& x, float sl2, bf16x8_t (&pb)[2]) {
+template <int ST, int KS>
+__device__ __forceinline__ void weights_of(const Rows<KS>& s, const f32x16_t& x, float scale, const float* f,
+                                           bf16x8_t (&pb)[2]) {
   const float nm = -s.m;
 #pragma unroll
   for (int ks = 0; ks < 2; ++ks) {
+    const float sl2 = ST == kInt8 ? scale * f[ks] : scale;
 #pragma unroll
     for (int j = 0; j < 8; j += 2) {
       const f32x2_t two = {__builtin_amdgcn_exp2f(__builtin_fmaf(x[8 * ks + j], sl2, nm)),
@@ -542,8 +558,8 @@ __device__ __forceinline__ __amdgpu_buffer_rsrc_t exponents_of(const PagedArgs& 
 }
 
 // Issues a load of 8 rows: bf16 straight into LDS at `to` (row 0 of the 8 in sub-tile 0), codes into registers at
-// index i.
-template <int ST, int DT, int kSubBytes, int kLoads>
+// index i, with their exponents (EXPONENTS).
+template <int ST, bool EXPONENTS, int DT, int kSubBytes, int kLoads>
 __device__ __forceinline__ void stage_rows8(const __amdgpu_buffer_rsrc_t r, const __amdgpu_buffer_rsrc_t er, const Lane8& n,
                                             int i, char* to, Staged<DT, kLoads>& st) {
 #pragma unroll
@@ -554,13 +570,13 @@ __device__ __forceinline__ void stage_rows8(const __amdgpu_buffer_rsrc_t r, cons
       __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (lds_ptr_t)(to + u * kSubBytes), 16, n.at[u], 0, 0, 0);
     }
   }
-  if constexpr (coded(ST)) st.e[i] = __builtin_amdgcn_raw_buffer_load_b8(er, n.key, 0, 0);
+  if constexpr (EXPONENTS) st.e[i] = __builtin_amdgcn_raw_buffer_load_b8(er, n.key, 0, 0);
 }
 
-// 8 codes times 2^(exponent - 127) as bf16, exact.
-template <int ST>
+// 8 codes times 2^(exponent - 127) as bf16 (int8: SCALED), exact.
+template <int ST, bool SCALED>
 __device__ __forceinline__ uint4 decode8(uint2 w, uint32_t exponent) {
-  if constexpr (ST == kInt8) return int8_values(w, int8_power(exponent));
+  if constexpr (ST == kInt8) return int8_values<SCALED>(w, SCALED ? int8_power(exponent) : 1.f);
   const float f = exponent_value(static_cast<int>(exponent));
   const bf16x2_t a = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w.x, f, false);
   const bf16x2_t b = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w.x, f, true);
@@ -570,13 +586,13 @@ __device__ __forceinline__ uint4 decode8(uint2 w, uint32_t exponent) {
                     __builtin_bit_cast(uint32_t, d));
 }
 
-// Codes: load i of `st` into its 8 rows at `to`.
-template <int ST, int DT, int kSubBytes, int kLoads>
-__device__ __forceinline__ void commit_rows8(const Staged<DT, kLoads>& st, int i, char* to) {
+// Codes: load i of `st` into its 8 rows at `to`; SCALED: times their powers of two.
+template <int ST, bool SCALED, int DT, int kSubBytes, int kLoads>
+__device__ __forceinline__ void commit_rows8(const Staged<DT, kLoads>& st, int i, uint32_t exponent, char* to) {
 #pragma unroll
   for (int u = 0; u < Width<DT>::kSubTiles; ++u) {
     *reinterpret_cast<uint4*>(to + u * kSubBytes + 16 * (threadIdx.x & 63)) =
-        decode8<ST>(st.w[i * Width<DT>::kSubTiles + u], st.e[i]);
+        decode8<ST, SCALED>(st.w[i * Width<DT>::kSubTiles + u], exponent);
   }
 }
 

@@ -145,7 +145,8 @@ __device__ __forceinline__ void row_work(const PagedArgs& a, int place, char* sV
 
   using KWord = typename std::conditional<kCodes, uint2, uint4>::type;
   KWord kw[kHalves][KS];
-  uint32_t ke[kCodes ? kHalves : 1];
+  // e4m3: the exponent of the lane's key of each half (the V rows' lie beside them); int8: one of every 16 keys, K and V.
+  uint32_t ke[ST == kInt8 ? 2 * kHalves : (kCodes ? kHalves : 1)], ve[ST == kInt8 ? 2 * kHalves : 1];
   Staged<DT, kCodes ? 4 * kHalves : 1> vst;
   int page[kGroups], valid[kGroups];   // of the groups of the block to load
   bool broken = false;                 // the block in kw has keys on a bad page
@@ -165,9 +166,12 @@ __device__ __forceinline__ void row_work(const PagedArgs& a, int place, char* sV
       if (8 * i % kGroup == 0) {
         const int in_page = (real(kv) + kGroup * g) & in_mask;
         r = rows_of(vs.rows, vs.sp, vs.sr, page[g], in_page, valid[g], D * ES);
-        if constexpr (kCodes) er = exponents_of<ST>(a, vs, page[g], in_page, valid[g]);
+        if constexpr (ST == kE4m3) er = exponents_of<ST>(a, vs, page[g], in_page, valid[g]);
+        if constexpr (ST == kInt8) {
+          ve[g] = vs.exponents[static_cast<uint64_t>(static_cast<uint32_t>(page[g])) * vs.se + (in_page >> a.block_shift)];
+        }
       }
-      stage_rows8<ST, DT, kSubBytes>(r, er, vl[i], i, to + 8 * i * kRow * 2, vst);
+      stage_rows8<ST, ST == kE4m3, DT, kSubBytes>(r, er, vl[i], i, to + 8 * i * kRow * 2, vst);
     }
   };
   // Keys that do not exist are never loaded (the group's first one is read instead, or page 0 where there is none):
@@ -181,7 +185,11 @@ __device__ __forceinline__ void row_work(const PagedArgs& a, int place, char* sV
       const uint32_t pg = second ? page[g + 1] : page[g], in = second ? in1 : in0;
       const int there = (own & 15) < (second ? valid[g + 1] : valid[g]) ? own & 15 : 0;
       const char* at = ks.rows + static_cast<uint64_t>(pg) * ks.sp + ((in + there) * ks.sr + 8 * hh * ES);
-      if constexpr (kCodes) ke[t] = ks.exponents[static_cast<uint64_t>(pg) * ks.se + exponent_at<ST>(a, in + there)];
+      if constexpr (ST == kE4m3) ke[t] = ks.exponents[static_cast<uint64_t>(pg) * ks.se + in + there];
+      if constexpr (ST == kInt8) {
+        ke[2 * t] = ks.exponents[static_cast<uint64_t>(static_cast<uint32_t>(page[g])) * ks.se + (in0 >> a.block_shift)];
+        ke[2 * t + 1] = ks.exponents[static_cast<uint64_t>(static_cast<uint32_t>(page[g + 1])) * ks.se + (in1 >> a.block_shift)];
+      }
 #pragma unroll
       for (int k = 0; k < KS; ++k) {
         kw[t][k] = *reinterpret_cast<const KWord*>(at + (k < KS - 1 ? 16 * k * ES : k_last));
@@ -205,7 +213,9 @@ __device__ __forceinline__ void row_work(const PagedArgs& a, int place, char* sV
       const bool more = kvn < k1;
       if constexpr (kCodes) {
 #pragma unroll
-        for (int i = 0; i < 4 * kHalves; ++i) commit_rows8<ST, DT, kSubBytes>(vst, i, cur + 8 * i * kRow * 2);
+        for (int i = 0; i < 4 * kHalves; ++i) {
+          commit_rows8<ST, true, DT, kSubBytes>(vst, i, ST == kInt8 ? ve[8 * i / kGroup] : vst.e[i], cur + 8 * i * kRow * 2);
+        }
       }
       if (more) {
         check(kvn);
@@ -218,7 +228,7 @@ __device__ __forceinline__ void row_work(const PagedArgs& a, int place, char* sV
 #pragma unroll
         for (int k = 0; k < KS; ++k) {
           if constexpr (kCodes) {
-            ka[k] = __builtin_bit_cast(bf16x8_t, decode8<ST>(kw[t][k], ke[t]));
+            ka[k] = __builtin_bit_cast(bf16x8_t, decode8<ST, false>(kw[t][k], ke[t]));
           } else {
             ka[k] = __builtin_bit_cast(bf16x8_t, kw[t][k]);
           }
@@ -233,6 +243,11 @@ __device__ __forceinline__ void row_work(const PagedArgs& a, int place, char* sV
             if (static_cast<uint32_t>(page_number(a, row, g)) >= static_cast<uint32_t>(a.pages.pages)) x[t][i] = 0.f;
           }
         }
+      }
+      KeyScales<kHalves> f;
+      if constexpr (ST == kInt8) {
+#pragma unroll
+        for (int i = 0; i < 2 * kHalves; ++i) f.of[i] = int8_power(ke[i]);
       }
       if (more) {
         load_k(kvn);
@@ -251,11 +266,11 @@ __device__ __forceinline__ void row_work(const PagedArgs& a, int place, char* sV
       if (ST != kInt8 && (key0 > clean_from || past_low(key0))) {
         odd |= __builtin_amdgcn_ballot_w64(clean_values(cur, kTileBytes, 16 * lane, 16 * 64)) != 0ull;
       }
-      bound_scores<WIN, KS, kHalves>(a, s, x, key0 + kKeys - 1 > all || past_low(key0), key0);
+      bound_scores<ST, WIN, KS, kHalves>(a, s, x, f, key0 + kKeys - 1 > all || past_low(key0), key0);
 #pragma unroll
       for (int t = 0; t < kHalves; ++t) {
         bf16x8_t pb[2];
-        weights_of<KS>(s, x[t], a.scale_log2, pb);
+        weights_of<ST, KS>(s, x[t], a.scale_log2, f.of + 2 * t, pb);
         add_values<KS, kSubBytes>(s, pb, cur + 32 * t * kRow * 2, rvt);
       }
       kv = kvn;
@@ -319,7 +334,7 @@ __device__ __forceinline__ void row_work(const PagedArgs& a, int place, char* sV
 
 // Windows that are all of the row form.
 template <int ST, bool WIN, int KS>
-__global__ __launch_bounds__(kPagedThreads, 2) void paged_row_kernel(PagedArgs a, unsigned first_group) {
+__global__ __launch_bounds__(kPagedThreads, ST == kInt8 && KS <= 6 ? 3 : 2) void paged_row_kernel(PagedArgs a, unsigned first_group) {
 #if defined(__HIP_DEVICE_COMPILE__)
   constexpr int kFirst = coded(ST) ? 4 : 2;
   typedef RowLds<ST, KS, kFirst> L;

@@ -124,7 +124,8 @@ struct TileLds {
 #if defined(__HIP_DEVICE_COMPILE__)
 
 template <int ST, bool WIN, bool WHOLE, int KS>
-__device__ __forceinline__ void tile_work(const PagedArgs& a, int place, char* s0, char* s1, int* s_odd) {
+__device__ __forceinline__ void tile_work(const PagedArgs& a, int place, char* s0, char* s1, int* s_odd,
+                                          [[maybe_unused]] float (*s_scale)[4]) {
   constexpr int DT = tiles_of(KS), ES = bytes_of(ST);
   constexpr bool kCodes = coded(ST);
   constexpr int kSubBytes = TileLds<KS>::kSubBytes, kTileBytes = TileLds<KS>::kTileBytes;
@@ -224,20 +225,27 @@ __device__ __forceinline__ void tile_work(const PagedArgs& a, int place, char* s
         }
       }
       const int to = (8 * wave + 32 * i) * kRow * 2;
-      stage_rows8<ST, DT, kSubBytes>(kr, ek, kl[i], i, sK + to, kst);
-      stage_rows8<ST, DT, kSubBytes>(vr, ev, vl[i], i, sV + to, vst);
+      stage_rows8<ST, kCodes, DT, kSubBytes>(kr, ek, kl[i], i, sK + to, kst);
+      stage_rows8<ST, kCodes, DT, kSubBytes>(vr, ev, vl[i], i, sV + to, vst);
     }
   };
-  auto commit = [&](char* sK, char* sV) __attribute__((always_inline)) {
+  // int8: what every 16 keys of a block stand for, beside its buffer; rows 8 wave + 32 i hold keys of group wave / 2 + 2 i.
+  auto commit = [&](char* sK, char* sV, int buffer) __attribute__((always_inline)) {
+    if constexpr (ST == kInt8) {
+      if ((wave & 1) == 0 && lane == 0) {
+#pragma unroll
+        for (int i = 0; i < 2; ++i) s_scale[buffer][(wave >> 1) + 2 * i] = int8_power(kst.e[i]);
+      }
+    }
     if constexpr (kCodes) {
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
-        commit_rows8<ST, DT, kSubBytes>(kst, i, sK + (8 * wave + 32 * i) * kRow * 2);
-        commit_rows8<ST, DT, kSubBytes>(vst, i, sV + (8 * wave + 32 * i) * kRow * 2);
+        commit_rows8<ST, false, DT, kSubBytes>(kst, i, kst.e[i], sK + (8 * wave + 32 * i) * kRow * 2);
+        commit_rows8<ST, true, DT, kSubBytes>(vst, i, vst.e[i], sV + (8 * wave + 32 * i) * kRow * 2);
       }
     }
   };
-  auto compute = [&](int kv0, const char* sK, const char* sV) __attribute__((always_inline)) {
+  auto compute = [&](int kv0, const char* sK, const char* sV, int buffer) __attribute__((always_inline)) {
     if (kv0 > any) return;
     if (WIN && kv0 + kKB <= low_first && kv0 >= a.sinks) return;
     f32x16_t x[2];
@@ -250,11 +258,16 @@ __device__ __forceinline__ void tile_work(const PagedArgs& a, int place, char* s
       }
       x[t] = scores<KS>(s, ka);
     }
-    bound_scores<WIN, KS, 2>(a, s, x, kv0 + kKB - 1 > all || past_low(kv0, low_wave), kv0);
+    KeyScales<2> f;
+    if constexpr (ST == kInt8) {
+      const float4 four = *reinterpret_cast<const float4*>(s_scale[buffer]);
+      f.of[0] = four.x, f.of[1] = four.y, f.of[2] = four.z, f.of[3] = four.w;
+    }
+    bound_scores<ST, WIN, KS, 2>(a, s, x, f, kv0 + kKB - 1 > all || past_low(kv0, low_wave), kv0);
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
       bf16x8_t pb[2];
-      weights_of<KS>(s, x[t], a.scale_log2, pb);
+      weights_of<ST, KS>(s, x[t], a.scale_log2, f.of + 2 * t, pb);
       add_values<KS, kSubBytes>(s, pb, sV + 32 * t * kRow * 2, rvt);
     }
   };
@@ -263,10 +276,10 @@ __device__ __forceinline__ void tile_work(const PagedArgs& a, int place, char* s
     find(real(kKB * blk0));
     issue(real(kKB * blk0), sK0, sV0);
     find(real(kKB * (blk0 + 1)));
-    commit(sK0, sV0);
+    commit(sK0, sV0, 0);
     wait_vmem();
     __syncthreads();
-    auto step = [&](int blk, char* cK, char* cV, char* nK, char* nV) __attribute__((always_inline)) {
+    auto step = [&](int blk, char* cK, char* cV, char* nK, char* nV, int buffer) __attribute__((always_inline)) {
       const bool more = blk + 1 < blk1;
       if (more) issue(real(kKB * (blk + 1)), nK, nV);
       find(real(kKB * (blk + 2)));
@@ -275,16 +288,16 @@ __device__ __forceinline__ void tile_work(const PagedArgs& a, int place, char* s
         if (clean_values(cV, kTileBytes, 16 * static_cast<int>(threadIdx.x), 16 * kPagedThreads)) *s_odd = 1;
         __syncthreads();
       }
-      compute(kv0, cK, cV);
+      compute(kv0, cK, cV, buffer);
       if (more) {
-        commit(nK, nV);
+        commit(nK, nV, buffer ^ 1);
         wait_vmem();
         __syncthreads();
       }
     };
     for (int blk = blk0; blk < blk1; blk += 2) {
-      step(blk, sK0, sV0, sK1, sV1);
-      if (blk + 1 < blk1) step(blk + 1, sK1, sV1, sK0, sV0);
+      step(blk, sK0, sV0, sK1, sV1, 0);
+      if (blk + 1 < blk1) step(blk + 1, sK1, sV1, sK0, sV0, 1);
     }
     if constexpr (WIN) {
       if (ST != kInt8 && *s_odd != 0) {
@@ -330,8 +343,9 @@ template <int ST, bool WIN, bool WHOLE, int KS>
 __global__ __launch_bounds__(kPagedThreads, coded(ST) || KS > 4 ? 2 : 4) void paged_tile_kernel(PagedArgs a, unsigned first_group) {
 #if defined(__HIP_DEVICE_COMPILE__)
   __shared__ __attribute__((aligned(16))) char s0[TileLds<KS>::kBuffer], s1[TileLds<KS>::kBuffer];
+  __shared__ __attribute__((aligned(16))) float s_scale[coded(ST) ? 2 : 1][4];
   __shared__ int s_odd;
-  tile_work<ST, WIN, WHOLE, KS>(a, static_cast<int>(first_group + blockIdx.x), s0, s1, &s_odd);
+  tile_work<ST, WIN, WHOLE, KS>(a, static_cast<int>(first_group + blockIdx.x), s0, s1, &s_odd, s_scale);
 #endif
 }
 
