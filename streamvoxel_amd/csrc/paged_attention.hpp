@@ -25,6 +25,7 @@ constexpr int kTileTarget = 512;
 // 63 tokens over 4096 123 for 116; 12 heads, 3 chunks of 512 over 4096 and 100 tokens over 2048 169 for 152; but 8 heads of
 // 96, 6 chunks of 300 and 18 tokens over 8192, as much of one form as of the other, 163 for 180.
 constexpr int kTileBeside = 256;
+constexpr int kTileLong = 96;      // key blocks of a part beside the row form, through a window (tile_length)
 constexpr int kTileLeast = 6;      // least key blocks of a tile's part (1024 queries over 9744 keys 60 us; 3, 12: 61)
 // Row-form parts beyond one for each (window, key head): eight for every CU (64 tokens, four heads to a key head, 218
 // us, 512 parts: 248; over e4m3 pages 158 and 180).
