@@ -195,6 +195,38 @@ def byte_span(t):
     return (low, low + extent * t.element_size())
 
 
+def apart(a, b):
+    """True where two tensors of one type interleave in one buffer without touching: alike in the strides of every dimension that
+    both have, the one's elements in the gaps of the other's (queries and keys in a fused projection's rows)."""
+    if b.data_ptr() < a.data_ptr():
+        a, b = b, a
+    size = a.element_size()
+    gap, rest = divmod(b.data_ptr() - a.data_ptr(), size)
+    if rest or b.element_size() != size or a.dim() != b.dim():
+        return False
+    dims = []
+    for n, s, m, t in zip(a.shape, a.stride(), b.shape, b.stride()):
+        if n > 1 and m > 1 and s != t:
+            return False
+        if n > 1 or m > 1:
+            dims.append((s if n > 1 else t, n, m))
+    reach, other = 1, 1            # of a's and b's elements inside the gap
+    for s, n, m in sorted(dims):
+        if s <= 0:
+            return False
+        if s <= gap:
+            reach, other = reach + (n - 1) * s, other + (m - 1) * s
+    outer = gap + other
+    if reach > gap:
+        return False
+    for s, n, m in sorted(dims):
+        if s > gap:
+            if s < outer:
+                return False
+            outer += (max(n, m) - 1) * s
+    return True
+
+
 def overlaps(a, b):
     """True when the elements of two tensors may share memory (their byte spans intersect)."""
     if a is None or b is None:

@@ -23,7 +23,7 @@ struct NormSide {
   const void *x, *dy, *w;
   void* out;      // y, or dx; null: not wanted
   int64_t sx_b, sx_h, sx_n, so_b, so_h, so_n, sd_b, sd_h, sd_n;
-  int H, tokens, tiles, groups;  // tokens: of a tile; tiles: of all windows; groups: workgroups of the gradient
+  int H, tokens, per_window, tiles, groups;  // tokens: of a tile; tiles: of a window, of all; workgroups of the gradient
 };
 
 struct NormArgs {
@@ -188,8 +188,8 @@ __global__ __launch_bounds__(kNormThreads) void norm_rotary_kernel(NormArgs a, u
   const int group = static_cast<int>(first_group + blockIdx.x);
   const bool keys = group >= a.side[0].tiles;
   const NormSide s = keys ? a.side[1] : a.side[0];
-  const int tile = keys ? group - a.side[0].tiles : group, per_window = (a.N + s.tokens - 1) / s.tokens;
-  const int window = tile / per_window, n0 = (tile - window * per_window) * s.tokens;
+  const int tile = keys ? group - a.side[0].tiles : group;
+  const int window = tile / s.per_window, n0 = (tile - window * s.per_window) * s.tokens;
   const int tokens = a.N - n0 < s.tokens ? a.N - n0 : s.tokens;
   const int64_t b = window;
   const Places at = places_of<INTER>(a.row, static_cast<int>(threadIdx.x) % LPR);
@@ -229,7 +229,6 @@ __global__ __launch_bounds__(kNormThreads) void norm_rotary_grad_kernel(NormArgs
   const int group = static_cast<int>(blockIdx.x);
   const bool keys = group >= a.side[0].groups;
   const NormSide s = keys ? a.side[1] : a.side[0];
-  const int per_window = (a.N + s.tokens - 1) / s.tokens;
   const Places at = places_of<INTER>(a.row, static_cast<int>(threadIdx.x) % LPR);
   const float per = 1.f / static_cast<float>(a.row.D);
   float w[16], dw[16];
@@ -237,7 +236,7 @@ __global__ __launch_bounds__(kNormThreads) void norm_rotary_grad_kernel(NormArgs
 #pragma unroll
   for (int i = 0; i < 16; ++i) dw[i] = 0.f;
   for (int tile = keys ? group - a.side[0].groups : group; tile < s.tiles; tile += s.groups) {
-    const int window = tile / per_window, n0 = (tile - window * per_window) * s.tokens;
+    const int window = tile / s.per_window, n0 = (tile - window * s.per_window) * s.tokens;
     const int tokens = a.N - n0 < s.tokens ? a.N - n0 : s.tokens;
     const int64_t b = window;
     const T* x = static_cast<const T*>(s.x) + b * s.sx_b + n0 * s.sx_n;
@@ -412,9 +411,9 @@ int norm_rotary(const char* name, const svhip_norm_rotary_args* args, bool grad,
                     (c.Hk == 0 || (c.k && (grad ? c.dk != nullptr : c.out_k != nullptr))) && c.positions && c.freq,
                 "%s: null pointer", name);
   NormArgs a{{{c.q, c.dq, c.q_weight, c.out_q, c.sq_b, c.sq_h, c.sq_n, c.soq_b, c.soq_h, c.soq_n, c.sdq_b, c.sdq_h, c.sdq_n,
-               static_cast<int>(c.H), 1, 0, 0},
+               static_cast<int>(c.H), 1, 1, 0, 0},
               {c.k, c.dk, c.k_weight, c.out_k, c.sk_b, c.sk_h, c.sk_n, c.sok_b, c.sok_h, c.sok_n, c.sdk_b, c.sdk_h, c.sdk_n,
-               static_cast<int>(c.Hk), 1, 0, 0}},
+               static_cast<int>(c.Hk), 1, 1, 0, 0}},
              c.positions, c.freq, c.sp_b, c.sp_n, static_cast<int>(c.N), row_items(D, half),
              c.positions_wide != 0, c.weight_dtype == SVHIP_F32, static_cast<float>(c.eps), static_cast<float>(c.amplitude),
              weighed ? static_cast<float*>(c.workspace) : nullptr};
@@ -429,10 +428,12 @@ int norm_rotary(const char* name, const svhip_norm_rotary_args* args, bool grad,
     };
     vec = vec && on16(side.x, side.sx_b, side.sx_h, side.sx_n) && on16(side.out, side.so_b, side.so_h, side.so_n) &&
           (!grad || on16(side.dy, side.sd_b, side.sd_h, side.sd_n));
-    const int64_t tokens = norm_tokens(c.B, side.H, c.N, row_lanes(a.row), half), tiles = c.B * cdiv(c.N, tokens);
+    const int64_t tokens = norm_tokens(c.B, side.H, c.N, row_lanes(a.row), half), per_window = cdiv(c.N, tokens);
+    const int64_t tiles = c.B * per_window;
     all += tiles;
     SVHIP_REQUIRE(all < (1ll << 31), "%s: grid too large", name);
     side.tokens = static_cast<int>(tokens);
+    side.per_window = static_cast<int>(per_window);
     side.tiles = static_cast<int>(tiles);
     side.groups = static_cast<int>(norm_groups(tiles, side.H, c.H + c.Hk));
   }

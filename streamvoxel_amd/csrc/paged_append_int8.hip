@@ -260,7 +260,7 @@ __global__ __launch_bounds__(kAppendThreads) void paged_append_int8_kernel(Appen
       const int64_t i = mine - start, j = a.pages.lengths[b] - a.before - count + i;
       if (j < 0 || j >= a.pages.max_pages << a.pages.shift) {
         set_bad(a.pages);
-      } else if (i == 0 || (j & (kBlock - 1)) == 0) {
+      } else if (i == 0 || (i > 0 && i < count && (j & (kBlock - 1)) == 0)) {  // (i outside: borders not ascending)
         const int older = static_cast<int>(j & (kBlock - 1));
         blk.page = page_of(a.pages, b, j);
         leads = blk.page >= 0;

@@ -115,7 +115,8 @@ def extend_condition(model, context, index, local, positions):
     context.reserve(index, grown)
     try:
         lengths = torch.full((1,), grown, dtype=torch.int32, device=dev)
-        for j, (cross, key, value) in enumerate(_local_kv(model, context, local)):
+        # (All projected before the first is written: an int8 block that both old and new keys are in may change with them.)
+        for j, (cross, key, value) in enumerate(list(_local_kv(model, context, local))):
             freq = cross.rope.frequencies.to(device=dev, dtype=torch.float32)
             context.append(j, key, value, index=index, lengths=lengths, positions=positions, frequencies=freq,
                            layout='axial')
@@ -317,7 +318,8 @@ class SlotEngine:
         """Slot `index` of a paged engine takes further local context (`local` [1, L, W], `positions` [1, L, 3]) behind the
         condition that it holds, on the side stream like `load_slot`: a neighbour that has come in costs its own keys, not
         the window's. The slot's tokens stay; on error (a pool that has too few pages, a `local` of another width) its context
-        does too."""
+        does too. int8: the block that the condition ends in is rounded again where its keys share it, so a step over the slot
+        comes behind `wait_loads`."""
         index = int(index)
         if not isinstance(self.context, PagedContext):
             raise ValueError('extending a slot needs an engine with pages')

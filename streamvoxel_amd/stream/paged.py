@@ -37,18 +37,20 @@ def _check_pool(k_pages, v_pages, page_table, lengths, k_exponents, v_exponents,
             raise TypeError('bf16 pages take no exponents')
         return _lib.SVHIP_BF16
     if dtype == torch.int8:
-        for e in (k_exponents, v_exponents):
-            if e is None or e.dtype != torch.uint8 or e.dim() != 3 or e.shape[:2] != shape[:2] or (
-                    e.stride(-1) != 1 and e.shape[2] > 1):
-                raise ValueError('int8 pages need k_exponents and v_exponents, uint8 [pages, heads, page / block] with '
-                                 'contiguous rows')
+        if k_exponents is None or v_exponents is None or k_exponents.dtype != torch.uint8 or (
+                v_exponents.dtype != torch.uint8):
+            raise ValueError('int8 pages need k_exponents and v_exponents, uint8 [pages, heads, page / block]')
         if k_exponents.shape != v_exponents.shape:
             raise ValueError('k_exponents and v_exponents must be alike')
-        blocks = k_exponents.shape[2]
-        block = shape[2] // blocks if blocks else 0
-        if block not in _lib.SVHIP_INT8_BLOCK or blocks * block != shape[2]:
-            raise ValueError(f'{blocks} exponents for a page of {shape[2]} keys: one is for 16, 32 or 64 of them')
-        return _lib.SVHIP_INT8_BLOCK[block]
+        pages, heads, *blocks = k_exponents.shape if k_exponents.dim() == 3 else (-1, -1, 1)
+        if pages != shape[0] or heads != shape[1] or blocks[0] > 1 and (
+                k_exponents.stride(2) != 1 or v_exponents.stride(2) != 1):
+            raise ValueError('k_exponents and v_exponents must be [pages, heads, page / block] with contiguous rows')
+        page, blocks = shape[2], blocks[0]
+        code = _lib.SVHIP_INT8_BLOCK.get(page // blocks if blocks else 0)
+        if code is None or page % blocks:
+            raise ValueError(f'{blocks} exponents for a page of {page} keys: one is for 16, 32 or 64 of them')
+        return code
     if dtype != torch.float8_e4m3fn:
         raise TypeError(f'pages of {dtype} unsupported (bfloat16, float8_e4m3fn or int8)')
     for e in (k_exponents, v_exponents):
@@ -201,7 +203,7 @@ def paged_read(k_pages, v_pages, page_table, lengths, n, cu_keys=None, before=0,
     P, H, S, D = k_pages.shape
     shape = (B, H, n, D) if cu_keys is None else (H, n, D)
     if out is None:
-        key, value = [torch.empty(shape, dtype=torch.bfloat16, device=k_pages.device) for _ in 'kv']
+        key, value = torch.empty((2, *shape), dtype=torch.bfloat16, device=k_pages.device).unbind(0)
     else:
         key, value = out
         for t in out:
@@ -209,24 +211,14 @@ def paged_read(k_pages, v_pages, page_table, lengths, n, cu_keys=None, before=0,
                 raise ValueError(f'out must be a pair of bf16 {shape} with a contiguous head_dim and a place for every element')
             if any(_lib.overlaps(t, pages) for pages in (k_pages, v_pages)):
                 raise ValueError('out must not share memory with the pages')
-        if _lib.overlaps(key, value) and not _side_by_side(key, value):
+        if _lib.overlaps(key, value) and not _lib.apart(key, value):
             raise ValueError('the two of out must not share memory')
-    sk, sv = _windows(key, cu_keys, B, 'key')[2], _windows(value, cu_keys, B, 'value')[2]
+    sk = _windows(key, cu_keys, B, 'key')[2]
+    sv = sk if out is None else _windows(value, cu_keys, B, 'value')[2]
     cache = _packed(code, k_pages, v_pages, page_table, lengths, k_exponents, v_exponents, bad)
     args = _READ.pack(key.data_ptr(), value.data_ptr(), _address(cu_keys), n, before, *sk, *sv)
     _lib.launch('svhip_paged_read', key, cache, args)
     return key, value
-
-
-def _side_by_side(a, b):
-    """True where two tensors of one shape and the same strides interleave without touching: one dimension's stride holds both."""
-    if a.stride() != b.stride():
-        return False
-    gap = abs(a.data_ptr() - b.data_ptr()) // a.element_size()
-    inner = [(s, n) for n, s in zip(a.shape, a.stride()) if n > 1 and s <= gap]
-    outer = [s for n, s in zip(a.shape, a.stride()) if n > 1 and s > gap]
-    reach = sum((n - 1) * s for s, n in inner) + 1
-    return reach <= gap and all(gap + reach <= s for s in outer)
 
 
 def paged_attention(query, k_pages, v_pages, page_table, lengths, cu_queries=None, causal=False, scale=None,
@@ -494,10 +486,12 @@ class PagedContext:
         `append` take them; of all windows one behind the other without an index (n: of each, at most)."""
         held = [L if n is None else min(L, n) for L in (self.host_lengths if index is None else [self.host_lengths[index]])]
         at = slice(0, self.batch) if index is None else slice(index, index + 1)
-        borders = torch.zeros(len(held) + 1, dtype=torch.int32)
-        borders[1:] = torch.tensor(held).cumsum(0)
-        cu = borders.to(self.lengths.device)
-        return paged_read(self.k[layer], self.v[layer], self.table[at], self.lengths[at], sum(held), cu_keys=cu,
+        borders = [0]
+        for count in held:
+            borders.append(borders[-1] + count)
+        cu = torch.empty(len(borders), dtype=torch.int32, device=self.lengths.device)
+        self._send(cu, borders)
+        return paged_read(self.k[layer], self.v[layer], self.table[at], self.lengths[at], borders[-1], cu_keys=cu,
                           k_exponents=self.k_exponents[layer], v_exponents=self.v_exponents[layer], bad=self.bad)
 
     def attend(self, layer, query, out=None, n=None, cu_queries=None, causal=False, window=None, sinks=0):

@@ -279,24 +279,10 @@ def norm_rotary(query, key, query_weight, key_weight, positions, frequencies, ep
         if o.shape != x.shape or o.dtype != x.dtype or o.stride(-1) != 1 or _lib.stacked(o):
             raise ValueError("out must have its input's shape and type, a contiguous head_dim and a place for every element")
         for other in (query, key):
-            same = other is x and o.data_ptr() == x.data_ptr() and o.stride() == x.stride()
-            if _lib.overlaps(o, other) and not same and not _apart(o, other):
+            same = other is x and (o is x or o.data_ptr() == x.data_ptr() and o.stride() == x.stride())
+            if not same and _lib.overlaps(o, other) and not _lib.apart(o, other):
                 raise ValueError('out must be its input itself or memory that neither input shares')
-    if out[1] is not None and _lib.overlaps(*out) and not _apart(*out):
+    if out[1] is not None and out[1] is not key and _lib.overlaps(*out) and not _lib.apart(*out):
         raise ValueError('the two of out must not share memory')
     return _normed(query, key, (query_weight, key_weight), tuple(out), *how)
 
-
-def _apart(a, b):
-    """True where two [B, H, N, D] tensors of one type lie side by side in the rows of one buffer: the same strides, and no
-    element of the one at a place of the other's."""
-    if a.stride()[0] != b.stride()[0] or a.stride()[1:] != b.stride()[1:] or a.shape[0] != b.shape[0]:
-        return False
-    # The heads of both in a token's row: [H a.., H b..] within the token's stride.
-    sb, sh, sn, _ = a.stride()
-    gap = (b.data_ptr() - a.data_ptr()) // a.element_size()
-    first, second = (a, b) if gap >= 0 else (b, a)
-    gap, D = abs(gap), a.shape[3]
-    if not D <= sh or not first.shape[1] * sh <= gap or not gap + second.shape[1] * sh <= sn:
-        return False
-    return a.shape[0] == 1 or a.shape[2] * sn <= sb

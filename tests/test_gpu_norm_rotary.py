@@ -327,6 +327,9 @@ def test_refusals():
     wide = torch.zeros(1, 1, 4, 264, dtype=torch.bfloat16, device=DEV)
     with pytest.raises(ValueError, match='head_dim'):
         norm_rotary(wide, None, None, None, p, f)
+    import torch.autograd.forward_ad as fwd
+    with fwd.dual_level(), pytest.raises((RuntimeError, NotImplementedError)):      # no tangent is dropped
+        norm_rotary(fwd.make_dual(q, torch.ones_like(q)), k, wq, wk, p, f)
     leaf = q.float().detach().requires_grad_()
     y = norm_rotary(leaf, None, None, None, p, f)[0]
     dx = torch.autograd.grad(y, leaf, torch.ones_like(y).requires_grad_(), create_graph=True)[0]

@@ -155,3 +155,36 @@ def test_int8_needs_pages():
     check_engine_options('gather', 'flex', False, 'int8', paged=True)
     with pytest.raises(ValueError, match='pages'):
         check_engine_options('gather', 'flex', False, 'int8')
+
+
+def test_tensors_that_lie_apart():
+    base = torch.zeros(2, 5, 12, 64)
+    q, k, v = [base[:, :, i:j].transpose(1, 2) for i, j in ((0, 8), (8, 10), (10, 12))]
+    assert _lib.apart(q, k) and _lib.apart(k, q) and _lib.apart(q, v) and _lib.apart(k, v)
+    assert not _lib.apart(q, q) and not _lib.apart(q, base[:, :, 7:9].transpose(1, 2)) and not _lib.apart(q, q[:, 1:3])
+    first, second = torch.zeros(2, 6, 5, 8).chunk(2, 1)
+    assert _lib.apart(first, second) and not _lib.apart(first, second.transpose(1, 2))
+    pair = torch.zeros(7, 2, 3, 8)
+    assert _lib.apart(pair[:, 0], pair[:, 1]) and _lib.apart(pair[:, 0].transpose(0, 1), pair[:, 1].transpose(0, 1))
+    one = torch.zeros(1, 1, 12, 64)
+    assert _lib.apart(one[:, :, :8].transpose(1, 2), one[:, :, 8:].transpose(1, 2))
+    flat = torch.zeros(100)
+    a, b = flat.as_strided((3, 4), (10, 2)), flat.as_strided((3, 4), (10, 2), 1)
+    assert _lib.apart(a, b)                                     # every other element of each
+    assert not _lib.apart(flat.as_strided((3, 6), (10, 2)), flat.as_strided((3, 6), (10, 2), 1))     # a row's end past the next's start
+    assert not _lib.apart(flat.as_strided((3,), (0,)), flat.as_strided((3,), (0,), 1))
+    g = torch.Generator().manual_seed(1)                         # against the elements themselves
+    draw = lambda low, high: int(torch.randint(low, high, (1,), generator=g))
+    seen = [0, 0]
+    for _ in range(3000):
+        stride = (draw(1, 14), draw(1, 6))
+        shapes = [(draw(1, 4), draw(1, 5)) for _ in 'ab']
+        a, b = [flat.as_strided(shape, stride, at) for shape, at in zip(shapes, (0, draw(0, 12)))]
+        places = [set((t.storage_offset() + i * t.stride(0) + j * t.stride(1)) for i in range(t.shape[0]) for j in range(t.shape[1]))
+                  for t in (a, b)]
+        if _lib.apart(a, b):
+            seen[0] += 1
+            assert not places[0] & places[1]
+        else:
+            seen[1] += 1
+    assert min(seen) > 200
