@@ -235,8 +235,8 @@ __global__ __launch_bounds__(kNormThreads) void norm_rotary_grad_kernel(NormArgs
   load_weights(a, s.w, at, w);
 #pragma unroll
   for (int i = 0; i < 16; ++i) dw[i] = 0.f;
-  for (int tile = keys ? group - a.side[0].groups : group; tile < s.tiles; tile += s.groups) {
-    const int window = tile / s.per_window, n0 = (tile - window * s.per_window) * s.tokens;
+  for (unsigned next = keys ? group - a.side[0].groups : group; next < static_cast<unsigned>(s.tiles); next += s.groups) {
+    const int tile = static_cast<int>(next), window = tile / s.per_window, n0 = (tile - window * s.per_window) * s.tokens;
     const int tokens = a.N - n0 < s.tokens ? a.N - n0 : s.tokens;
     const int64_t b = window;
     const T* x = static_cast<const T*>(s.x) + b * s.sx_b + n0 * s.sx_n;

@@ -9,7 +9,7 @@
 namespace svhip {
 
 constexpr int kReadThreads = 256;
-constexpr int kReadTokens = 16;
+constexpr int kReadTokens = 8;
 constexpr int kReadAhead = 4;
 
 struct ReadArgs {

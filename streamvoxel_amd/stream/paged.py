@@ -484,6 +484,8 @@ class PagedContext:
     def read(self, layer, index=None, n=None):
         """(key, value) bf16 [heads, keys, head_dim]: what window `index` of `layer` holds (its last n keys), as `write` and
         `append` take them; of all windows one behind the other without an index (n: of each, at most)."""
+        if self._capturing():
+            raise RuntimeError('the lengths of a PagedContext are kept by the host: read it outside the capture (or call paged_read)')
         held = [L if n is None else min(L, n) for L in (self.host_lengths if index is None else [self.host_lengths[index]])]
         at = slice(0, self.batch) if index is None else slice(index, index + 1)
         borders = [0]

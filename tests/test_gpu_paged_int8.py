@@ -562,10 +562,77 @@ def test_a_sequence_in_chunks_and_tokens(kind):
                 held = (keys if t is new[0] else values).cpu().double()
                 scale = held.abs().amax() if kind == 'int8' else t.abs().amax(-1, keepdim=True)
                 assert ((mine.cpu().double() - t).abs() <= step * scale).all()
+    graph = torch.cuda.CUDAGraph()
+    with pytest.raises(RuntimeError, match='capture'), torch.cuda.graph(graph):
+        ctx.read(0)
     every = ctx.read(0)
     assert every[0].shape == (Hk, sum(ctx.host_lengths), D) and int(ctx.bad) == 0
     L = ctx.host_lengths[0]
     assert torch.equal(every[0][:, L:2 * L], ctx.read(0, 1)[0])
+
+
+def test_pools_past_32_bit_offsets():
+    """Pages more than 2^32 bytes into the pool, written by the append, read by the attention, with a window and without, and
+    read back."""
+    from streamvoxel_amd.stream.paged import paged_append, paged_attention, paged_read
+    heads, D, page, block = 8, 128, 64, 32
+    pages = (1 << 32) // (heads * D * page) + 40
+    k, v = [torch.empty(pages, heads, page, D, dtype=torch.int8, device=DEV) for _ in 'kv']
+    e = {n: torch.empty(pages, heads, page // block, dtype=torch.uint8, device=DEV) for n in ('k_exponents', 'v_exponents')}
+    table = torch.tensor([[pages - 1, 0, pages - 20], [pages - 2, pages - 3, 1]], dtype=torch.int32, device=DEV)
+    lengths = torch.tensor([180, 129], dtype=torch.int32, device=DEV)
+    g = torch.Generator().manual_seed(0)
+    key, value = [torch.randn(2, heads, 180, D, generator=g).to(torch.bfloat16).to(DEV) for _ in 'kv']
+    for b, n in ((0, 180), (1, 129)):
+        paged_append(key[b:b + 1, :, :n], value[b:b + 1, :, :n], k, v, table[b:b + 1], lengths[b:b + 1], **e)
+    small = Int8Pool([180, 129], heads, D, page, 0, block)
+    used = table.flatten().long()
+    small.table = torch.arange(6, dtype=torch.int32).view(2, 3)
+    small.k, small.v = k[used].cpu(), v[used].cpu()
+    small.ke, small.ve = e['k_exponents'][used].cpu(), e['v_exponents'][used].cpu()
+    for n in (1, 90):
+        q = queries(2, heads, n, D, n)
+        for how in (dict(window=None), dict(window=70, sinks=3)):
+            check(paged_attention(q, k, v, table, lengths, causal=True, **how, **e), q, small, **how)
+    got = paged_read(k, v, table, lengths, 129, **e)
+    for b in (0, 1):
+        for t, x in zip(got, small.rows(b)):
+            assert torch.equal(t[b].cpu().double(), x[:, -129:])
+    assert (got[0].float() - torch.stack([key[0, :, 51:], key[1, :, :129]]).float()).abs().max() <= 4 / 127
+
+
+def test_read_of_more_keys_than_one_launch_holds():
+    from streamvoxel_amd.stream.paged import paged_read
+    T = (1 << 27) + 9
+    pages = -(-T // 1024)
+    k, v = [torch.randint(-127, 128, (pages, 1, 1024, 8), device=DEV, dtype=torch.int8) for _ in 'kv']
+    e = torch.full((pages, 1, 16), 127, dtype=torch.uint8, device=DEV)
+    table = torch.arange(pages, dtype=torch.int32, device=DEV)[None]
+    got = paged_read(k, v, table, torch.tensor([T], dtype=torch.int32, device=DEV), T, k_exponents=e, v_exponents=e)
+    for t, pool in zip(got, (k, v)):
+        assert torch.equal(t[0, 0].to(torch.int8), pool.view(-1, 8)[:T])
+
+
+def test_append_of_more_blocks_than_one_launch_holds():
+    """More than 2^23 slots of 64 tokens."""
+    from streamvoxel_amd.stream.paged import paged_append
+    T = (1 << 29) + 70
+    pages = -(-T // 1024)
+    row = (torch.arange(T, device=DEV) % 127 + 1).to(torch.bfloat16)
+    key = row[:, None].expand(T, 8).contiguous()[None, None]
+    k, v = [torch.empty(pages, 1, 1024, 8, dtype=torch.int8, device=DEV) for _ in 'kv']
+    ke, ve = [torch.zeros(pages, 1, 16, dtype=torch.uint8, device=DEV) for _ in 'kv']
+    table = torch.arange(pages, dtype=torch.int32, device=DEV)[None]
+    paged_append(key, key, k, v, table, torch.tensor([T], dtype=torch.int32, device=DEV), k_exponents=ke, v_exponents=ve)
+    assert torch.equal(k.view(-1)[:8 * T].view(torch.int64), v.view(-1)[:8 * T].view(torch.int64)) and torch.equal(ke, ve)
+    step = 1 << 26
+    for at in list(range(0, T, step)):
+        n = min(step, T - at)
+        blocks = ke.view(-1)[at // 64:-(-(at + n) // 64)]
+        scale = ((blocks.int() << 23).view(torch.float32)).repeat_interleave(64)[:n]
+        held = k.view(-1, 8)[at:at + n]
+        assert torch.equal(held[:, 0].float() * scale, row[at:at + n].float()), at
+        assert (held == held[:, :1]).all(), at
 
 
 @pytest.mark.parametrize('kind', ['bf16', 'int8'])
