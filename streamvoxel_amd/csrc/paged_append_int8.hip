@@ -159,15 +159,15 @@ __device__ __forceinline__ int settle(const AppendArgs& a, const Block& blk, con
     } else {
       const float f = exponent_value(127 - (code - had < 30 ? code - had : 30));
       const int per_row = a.D / 8, all = blk.older * per_row;
-      constexpr int kAtOnce = 4;
+      constexpr int kAtOnce = 2;
       for (int i0 = lane; i0 < all; i0 += kAtOnce * lanes) {
         uint2 w[kAtOnce];
-        uint8_t* at[kAtOnce];
+        int at[kAtOnce];  // (a page's rows of a head lie within 2^31 bytes)
 #pragma unroll
         for (int k = 0; k < kAtOnce; ++k) {
           const int i = i0 + k * lanes, r = i / per_row;
-          at[k] = p.rows + r * p.sr + 8 * (i - r * per_row);
-          if (i < all) w[k] = *reinterpret_cast<const uint2*>(at[k]);
+          at[k] = r * static_cast<int>(p.sr) + 8 * (i - r * per_row);
+          if (i < all) w[k] = *reinterpret_cast<const uint2*>(p.rows + at[k]);
         }
 #pragma unroll
         for (int k = 0; k < kAtOnce; ++k) {
@@ -175,7 +175,7 @@ __device__ __forceinline__ int settle(const AppendArgs& a, const Block& blk, con
           float c[8];
 #pragma unroll
           for (int e = 0; e < 8; ++e) c[e] = static_cast<float>(static_cast<int8_t>((e < 4 ? w[k].x : w[k].y) >> 8 * (e & 3)));
-          *reinterpret_cast<uint2*>(at[k]) =
+          *reinterpret_cast<uint2*>(p.rows + at[k]) =
               make_uint2(int8_codes(c[0], c[1], c[2], c[3], f), int8_codes(c[4], c[5], c[6], c[7], f));
         }
       }
@@ -197,7 +197,7 @@ __device__ __forceinline__ void hold_few(const AppendArgs& a, const RowItems& it
   for (int k = 0; k < PASSES; ++k) {
     const int r = r0 + 64 / LPR * k;
     Raw raw{make_uint4(0u, 0u, 0u, 0u), make_uint4(0u, 0u, 0u, 0u)};
-    if (r < blk.rows) raw = load_item(p.from + r * p.step, at, a.runs);
+    if (r < blk.rows) raw = load_item(p.from + r * p.step, at, TURN == kTurnNone || a.runs);
     unpack16(raw, x[k]);
   }
 #pragma unroll
@@ -222,14 +222,15 @@ __device__ __forceinline__ void hold_few(const AppendArgs& a, const RowItems& it
 #pragma unroll
   for (int k = 0; k < PASSES; ++k) {
     const int r = r0 + 64 / LPR * k;
-    if (r < blk.rows) store_item(p.rows + (blk.older + r) * p.sr, at, a.runs, x[k], exponent_value(254 - code));
+    if (r < blk.rows) store_item(p.rows + (blk.older + r) * p.sr, at, TURN == kTurnNone || a.runs, x[k], exponent_value(254 - code));
   }
 }
 
 // LPR: lanes of a row. `heads`: of a slice, `slices` of them.
+// Where a wave has one row of every lane there is room for six workgroups a CU (32 chunks 30.4 us for 32.2); more spill.
 template <int TURN, int LPR, int kBlock>
-__global__ __launch_bounds__(kAppendThreads) void paged_append_int8_kernel(AppendArgs a, RowItems items, unsigned first_group,
-                                                                          int heads, int slices) {
+__global__ __launch_bounds__(kAppendThreads, kBlock > 16 && kBlock * LPR <= kAppendThreads ? 6 : 2) void
+paged_append_int8_kernel(AppendArgs a, RowItems items, unsigned first_group, int heads, int slices) {
   constexpr int kShift = kBlock == 64 ? 6 : (kBlock == 32 ? 5 : 4), kWaves = kAppendThreads / 64;
   constexpr int kFew = 64 / LPR, kPasses = kBlock > kWaves * kFew ? kBlock / (kWaves * kFew) : 1;
   constexpr int kOwn = kBlock == 16 && kFew < 16 ? 16 / kFew : 1;  // passes of a wave by itself: all of a short block
@@ -328,7 +329,7 @@ __global__ __launch_bounds__(kAppendThreads) void paged_append_int8_kernel(Appen
 #pragma unroll
       for (int k = 0; k < kPasses; ++k) {
         const int r = kFew * (wave + kWaves * k) + r0;
-        if (r < blk.rows) raw[k] = load_item(p.from + r * p.step, at, a.runs);
+        if (r < blk.rows) raw[k] = load_item(p.from + r * p.step, at, TURN == kTurnNone || a.runs);
       }
     };
     load(0);
@@ -372,7 +373,7 @@ __global__ __launch_bounds__(kAppendThreads) void paged_append_int8_kernel(Appen
 #pragma unroll
       for (int k = 0; k < kPasses; ++k) {
         const int r = kFew * (wave + kWaves * k) + r0;
-        if (r < blk.rows) store_item(p.rows + (blk.older + r) * p.sr, at, a.runs, x[k], f);
+        if (r < blk.rows) store_item(p.rows + (blk.older + r) * p.sr, at, TURN == kTurnNone || a.runs, x[k], f);
       }
     }
   }
