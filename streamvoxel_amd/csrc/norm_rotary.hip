@@ -9,7 +9,11 @@
 // window, all heads of the queries or of the keys; the tokens' (cos, sin) go to LDS once. A group of LPR lanes carries a
 // row, a lane its pairs' 16 elements (two 8-element runs, half apart in the half layout), so that the row's sums are steps
 // within the group, a pair turns within its lane, and a lane's weights stay in registers. A thread's first row is on its
-// way before the angles are formed, and the next one while it computes.
+// way before the angles are formed, and the next one while it computes. Measured: 32 768 tokens of 16 and 4 heads of 128 in
+// bf16 (336 MB) 74 us, 4.5 TB/s of a copy's 5.1, their gradient (503 MB) 117, 4.3, and 4.7 for the weights' sums; 8192 of 12
+// and 12 of 64 (50 MB) 13.3; 64 tokens 5.5. Both sides in a workgroup, the weights in LDS: 50.9 us for the 50 MB, 873 for the
+// 839 MB of a result and its gradient (197 now). Rows a thread: 2, 4, 8: 18.7, 14.5, 15.5 us for the 50 MB; workgroups of a
+// gradient: 768 (three a CU at once), 1024, 2048: 204, 219, 208 us for the pair.
 #include "rotary.hpp"
 
 namespace svhip {

@@ -16,7 +16,17 @@
 //     joined. Bound: HBM. Measured: 64 tokens over 1.18 GB of keys 216 us, 5.4 TB/s; over 754 MB of e4m3 pages 148
 //     us, 5.1 TB/s; one token over 30 MB 9.1 us, a chain of loads. One wave a row of its own, with shuffles instead
 //     of the products, took 14.9 ms.
-// Packed windows may be of both (paged_mixed.hip). Either form may cut a window's keys into parts for several
+// int8 pools (one power of two for 16 keys at least): codes decode to bf16 whole numbers, a block's keys are scaled by a
+// factor of their scores, values as they are decoded. 64 tokens over 736 MB of int8 pages 161 us, 4.6 TB/s (two waves a
+// SIMD for three, keys scaled as they are decoded: 205 for 187 on pools in turn); 4 causal chunks of 512, 16 heads to 4 of
+// 128, up to 16 384 keys 315 us, 12 of them the join, where bf16 takes 290: a code costs a conversion (four cycles a wave),
+// half a packing and, of a value, a product; e4m3 half a conversion. Values scaled in their weights, the sums' other factor
+// the inverse: no faster.
+// A sliding window (WIN) leaves out what no token of a workgroup sees: keys are walked by their place among the others, the first
+// ones in whole blocks of 64 and those from the first token's window on. A prompt of 16 384 tokens, windows of 1024 and 16
+// first keys, 16 heads of 64: 104 us, 650 TFLOP/s of what is seen, 830 of what is walked; one token, windows of 4096 11.4 us
+// and a join of 4.4; 64 tokens over int8 windows of 1024 58 us, 76 over bf16.
+// Packed windows may be of both (paged_mixed.hpp). Either form may cut a window's keys into parts for several
 // workgroups; a part leaves O, its running maximum and its sum in fp32 and paged_join_kernel joins them in order (4.5
 // us for one token, 12 for 34 MB of parts). What is cut is planned on the device, where the lengths are: by every
 // workgroup for up to 64 windows, one a lane, else by paged_plan_kernel (6.6 us; every workgroup for itself: 4096
