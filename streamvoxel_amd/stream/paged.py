@@ -40,14 +40,14 @@ def _check_pool(k_pages, v_pages, page_table, lengths, k_exponents, v_exponents,
         if k_exponents is None or v_exponents is None or k_exponents.dtype != torch.uint8 or (
                 v_exponents.dtype != torch.uint8):
             raise ValueError('int8 pages need k_exponents and v_exponents, uint8 [pages, heads, page / block]')
-        if k_exponents.shape != v_exponents.shape:
+        held = k_exponents.shape
+        if v_exponents.shape != held:
             raise ValueError('k_exponents and v_exponents must be alike')
-        pages, heads, *blocks = k_exponents.shape if k_exponents.dim() == 3 else (-1, -1, 1)
-        if pages != shape[0] or heads != shape[1] or blocks[0] > 1 and (
+        blocks, page = held[-1] if len(held) == 3 else 0, shape[2]
+        if not blocks or held[0] != shape[0] or held[1] != shape[1] or blocks > 1 and (
                 k_exponents.stride(2) != 1 or v_exponents.stride(2) != 1):
             raise ValueError('k_exponents and v_exponents must be [pages, heads, page / block] with contiguous rows')
-        page, blocks = shape[2], blocks[0]
-        code = _lib.SVHIP_INT8_BLOCK.get(page // blocks if blocks else 0)
+        code = _lib.SVHIP_INT8_BLOCK.get(page // blocks)
         if code is None or page % blocks:
             raise ValueError(f'{blocks} exponents for a page of {page} keys: one is for 16, 32 or 64 of them')
         return code

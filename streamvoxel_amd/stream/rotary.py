@@ -138,6 +138,8 @@ _NORM = struct.Struct('13P31q2d')   # svhip_norm_rotary_args
 
 
 _NONE = 0, 0, 0
+_DTYPES = {torch.float32: _lib.SVHIP_F32, torch.bfloat16: _lib.SVHIP_BF16}
+_WHOLE = torch.int32, torch.int64
 
 
 def _places(t):
@@ -148,35 +150,30 @@ def _address(t):
     return 0 if t is None else t.data_ptr()
 
 
-def _norm_args(query, key, dq, dk, weights, outs, dw, workspace, positions, frequencies, eps, layout, amplitude):
+def _norm_args(query, key, dq, dk, weights, outs, dw, workspace, positions, frequencies, dtype, weight_dtype, layout, amplitude,
+               eps):
     """The svhip_norm_rotary_args of a gradient."""
     B, H, N, D = query.shape
-    given = weights[0] if weights[0] is not None else weights[1]
-    wide = _lib.SVHIP_F32 if given is None else _lib.dtype_code(given.dtype)
     return _NORM.pack(_address(query), _address(key), _address(dq), _address(dk), *map(_address, weights), *map(_address, outs),
                       *map(_address, dw), positions.data_ptr(), frequencies.data_ptr(), _address(workspace),
-                      0 if workspace is None else workspace.numel(), _lib.dtype_code(query.dtype), wide,
-                      positions.dtype == torch.int64, frequencies.numel(), LAYOUTS[layout], B, H,
-                      0 if key is None else key.shape[1], N, D, *_places(query), *_places(key), *_places(dq), *_places(dk),
-                      *_places(outs[0]), *_places(outs[1]), positions.stride(0) if positions.dim() == 2 else 0,
-                      positions.stride(-1), amplitude, eps)
+                      0 if workspace is None else workspace.numel(), dtype, weight_dtype, positions.dtype == torch.int64,
+                      frequencies.numel(), layout, B, H, 0 if key is None else key.shape[1], N, D, *_places(query),
+                      *_places(key), *_places(dq), *_places(dk), *_places(outs[0]), *_places(outs[1]),
+                      positions.stride(0) if positions.dim() == 2 else 0, positions.stride(-1), amplitude, eps)
 
 
-def _normed(query, key, weights, outs, positions, frequencies, eps, layout, amplitude):
+def _normed(query, key, wq, wk, outs, positions, frequencies, dtype, weight_dtype, layout, amplitude, eps):
     # (Packed here: half of _norm_args' time.)
     B, H, N, D = query.shape
-    wq, wk = weights
-    given = wq if wq is not None else wk
     q, k = outs
     Hk, ka, sk, ko, so = 0, 0, _NONE, 0, _NONE
     if key is not None:
         Hk, ka, sk, ko, so = key.shape[1], key.data_ptr(), key.stride()[:3], k.data_ptr(), k.stride()[:3]
+    sp = positions.stride()
     args = _NORM.pack(query.data_ptr(), ka, 0, 0, 0 if wq is None else wq.data_ptr(), 0 if wk is None else wk.data_ptr(),
-                      q.data_ptr(), ko, 0, 0, positions.data_ptr(), frequencies.data_ptr(), 0, 0, _lib.dtype_code(query.dtype),
-                      _lib.SVHIP_F32 if given is None else _lib.dtype_code(given.dtype), positions.dtype == torch.int64,
-                      frequencies.numel(), LAYOUTS[layout], B, H, Hk, N, D, *query.stride()[:3], *sk, *_NONE, *_NONE,
-                      *q.stride()[:3], *so, positions.stride(0) if positions.dim() == 2 else 0, positions.stride(-1), amplitude,
-                      eps)
+                      q.data_ptr(), ko, 0, 0, positions.data_ptr(), frequencies.data_ptr(), 0, 0, dtype, weight_dtype,
+                      positions.dtype == torch.int64, frequencies.numel(), layout, B, H, Hk, N, D, *query.stride()[:3], *sk,
+                      *_NONE, *_NONE, *q.stride()[:3], *so, sp[0] if len(sp) == 2 else 0, sp[-1], amplitude, eps)
     _lib.launch('svhip_norm_rotary', query, args)
     return outs
 
@@ -196,7 +193,7 @@ class _NormRotary(torch.autograd.Function):
         positions, frequencies, *rest = how
         ctx.save_for_backward(query, key, query_weight, key_weight, positions, frequencies)
         ctx.rest = rest
-        q, k = _normed(query, key, (query_weight, key_weight), (_like(query), _like(key)), *how)
+        q, k = _normed(query, key, query_weight, key_weight, (_like(query), _like(key)), *how)
         return q if k is None else (q, k)
 
     @staticmethod
@@ -228,13 +225,14 @@ def norm_rotary(query, key, query_weight, key_weight, positions, frequencies, ep
     and the weights, once and backwards; the weights' gradients are the same bits from call to call. Captured into a graph:
     for leaves that no eager graph still holds. `out` (optional, no gradient through it): the pair that receives the
     results, each its input itself or memory that neither input shares."""
-    tensors = [t for t in (key, query_weight, key_weight) if t is not None]
-    _lib.require_one_gpu(query, *tensors, positions, frequencies, *(out or ()))
+    _lib.require_one_gpu(query, key, query_weight, key_weight, positions, frequencies, *(out or ()))
     if layout not in LAYOUTS:
         raise ValueError("layout is 'half' or 'interleaved'")
-    if query.dtype not in (torch.bfloat16, torch.float32):
+    dtype = _DTYPES.get(query.dtype)
+    if dtype is None:
         raise TypeError('query must be bfloat16 or float32')
-    if query.dim() != 4 or query.stride(-1) != 1:
+    stride = query.stride()
+    if len(stride) != 4 or stride[3] != 1:
         raise ValueError('query must be [B, H, N, D] with a contiguous head_dim')
     B, H, N, D = query.shape
     if not 2 <= D <= 256:
@@ -245,16 +243,22 @@ def norm_rotary(query, key, query_weight, key_weight, positions, frequencies, ep
     else:
         if key.dtype != query.dtype:
             raise TypeError('query and key must have one type')
-        if key.dim() != 4 or key.stride(-1) != 1 or (key.shape[0], key.shape[2], key.shape[3]) != (B, N, D):
+        shape = key.shape
+        if len(shape) != 4 or key.stride(3) != 1 or shape[0] != B or shape[2] != N or shape[3] != D:
             raise ValueError('key must be [B, Hk, N, D] like query with a contiguous head_dim')
-    weights = [w for w in (query_weight, key_weight) if w is not None]
-    for w in weights:
-        if w.dtype not in (torch.bfloat16, torch.float32) or w.dtype != weights[0].dtype:
+    weight_dtype = None
+    for w in (query_weight, key_weight):
+        if w is None:
+            continue
+        code = _DTYPES.get(w.dtype)
+        if code is None or weight_dtype not in (None, code):
             raise TypeError('weights must be bfloat16 or float32 alike')
+        weight_dtype = code
         if w.shape != (D,) or not w.is_contiguous():
             raise ValueError('weights must be contiguous [head_dim] vectors')
-    if positions.dtype not in (torch.int32, torch.int64) or (positions.shape != (N,) and positions.shape != (B, N)):
-        raise ValueError(f'positions must be int32 or int64 [N] or [B, N], got {positions.dtype} {tuple(positions.shape)}')
+    places = positions.shape
+    if positions.dtype not in _WHOLE or (places != (N,) and places != (B, N)):
+        raise ValueError(f'positions must be int32 or int64 [N] or [B, N], got {positions.dtype} {tuple(places)}')
     if frequencies.dtype != torch.float64 or frequencies.dim() != 1 or not frequencies.is_contiguous():
         raise ValueError('frequencies must be a contiguous fp64 vector')
     if not 1 <= frequencies.numel() <= min(D // 2, 128):
@@ -262,14 +266,16 @@ def norm_rotary(query, key, query_weight, key_weight, positions, frequencies, ep
     eps = float(eps)
     if not 0.0 <= eps < math.inf:
         raise ValueError('eps must be 0 or more and finite')
-    how = positions, frequencies, eps, layout, float(amplitude)
-    leaves = [t for t in (query, key, query_weight, key_weight) if t is not None]
+    how = positions, frequencies, dtype, weight_dtype or 0, LAYOUTS[layout], float(amplitude), eps
+    tracked = False
+    if torch.is_grad_enabled() or forward_ad._current_level >= 0:      # (once, not for each tensor)
+        tracked = any(t is not None and _tracked(t) for t in (query, key, query_weight, key_weight, *(out or ())))
     if out is None:
-        if any(map(_tracked, leaves)):
+        if tracked:
             both = _NormRotary.apply(query, key, query_weight, key_weight, *how)
             return (both, None) if key is None else both
-        return _normed(query, key, (query_weight, key_weight), (_like(query), _like(key)), *how)
-    if any(map(_tracked, [*leaves, *(t for t in out if t is not None)])):
+        return _normed(query, key, query_weight, key_weight, (torch.empty_like(query), _like(key)), *how)
+    if tracked:
         raise ValueError('out= takes no part in a gradient')
     if len(out) != 2 or (out[1] is None) != (key is None) or out[0] is None:
         raise ValueError('out must be a pair like the results')
@@ -284,5 +290,5 @@ def norm_rotary(query, key, query_weight, key_weight, positions, frequencies, ep
                 raise ValueError('out must be its input itself or memory that neither input shares')
     if out[1] is not None and out[1] is not key and _lib.overlaps(*out) and not _lib.apart(*out):
         raise ValueError('the two of out must not share memory')
-    return _normed(query, key, (query_weight, key_weight), tuple(out), *how)
+    return _normed(query, key, query_weight, key_weight, tuple(out), *how)
 
