@@ -186,6 +186,13 @@ def stacked(t):
     return 0 in t.stride() and any(s == 0 and n > 1 for n, s in zip(t.shape, t.stride()))
 
 
+def rows_like(t):
+    """A fresh tensor like t with a contiguous last dimension (rows that overlap, in a window's strides, have another order
+    in empty_like)."""
+    fresh = torch.empty_like(t)
+    return fresh if fresh.stride(-1) == 1 else torch.empty(t.shape, dtype=t.dtype, device=t.device)
+
+
 def byte_span(t):
     """[first, last) device byte addresses a tensor's elements occupy (its strides taken into account)."""
     if t.numel() == 0:

@@ -249,7 +249,7 @@ def paged_attention(query, k_pages, v_pages, page_table, lengths, cu_queries=Non
     if query.shape[-1] != D or Hkv == 0 or H % Hkv:
         raise ValueError("query needs the pages' head_dim, and heads that share theirs evenly")
     if out is None:
-        out = torch.empty_like(query)
+        out = _lib.rows_like(query)
     elif out.shape != query.shape or out.dtype != torch.bfloat16 or out.stride(-1) != 1 or _lib.stacked(out):
         raise ValueError('out must be bf16 like query with a contiguous head_dim and a place for every element')
     elif _lib.overlaps(given, out) and (given.data_ptr() != out.data_ptr() or given.stride() != out.stride()):

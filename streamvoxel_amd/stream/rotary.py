@@ -73,7 +73,7 @@ def _turn(x, positions, frequencies, layout, amplitude, inverse):
     x = x if x.stride(-1) == 1 else x.contiguous()
     if _tracked(x):
         return _Rotary.apply(x, positions, frequencies, layout, amplitude, inverse)
-    return _launch(x, torch.empty_like(x), positions, frequencies, layout, amplitude, inverse)
+    return _launch(x, _lib.rows_like(x), positions, frequencies, layout, amplitude, inverse)
 
 
 class _Rotary(torch.autograd.Function):
@@ -85,7 +85,7 @@ class _Rotary(torch.autograd.Function):
         ctx.save_for_backward(positions, frequencies)
         ctx.save_for_forward(positions, frequencies)
         ctx.args = layout, amplitude, inverse
-        return _launch(x, torch.empty_like(x), positions, frequencies, layout, amplitude, inverse)
+        return _launch(x, _lib.rows_like(x), positions, frequencies, layout, amplitude, inverse)
 
     @staticmethod
     def backward(ctx, dy):
@@ -123,7 +123,7 @@ def rotary(x, positions, frequencies, layout='half', amplitude=1.0, out=None):
     if out is None:
         if _tracked(x):
             return _Rotary.apply(x, positions, frequencies, layout, float(amplitude), 0)
-        out = torch.empty_like(x)
+        out = _lib.rows_like(x)
     else:
         if _tracked(x) or _tracked(out):
             raise ValueError('out= takes no part in a gradient')
@@ -179,7 +179,7 @@ def _normed(query, key, wq, wk, outs, positions, frequencies, dtype, weight_dtyp
 
 
 def _like(t):
-    return None if t is None else torch.empty_like(t)
+    return None if t is None else _lib.rows_like(t)
 
 
 def _rows(t):
@@ -202,7 +202,7 @@ class _NormRotary(torch.autograd.Function):
         query, key, *weights, positions, frequencies = ctx.saved_tensors
         dq, dk = _rows(dq), _rows(dk)
         needs = ctx.needs_input_grad
-        outs = [torch.empty_like(t) if need else None for t, need in zip((query, key), needs)]
+        outs = [_lib.rows_like(t) if need else None for t, need in zip((query, key), needs)]
         dw = [torch.empty_like(t) if need else None for t, need in zip(weights, needs[2:])]
         B, H, N, D = query.shape
         workspace = None
@@ -274,7 +274,7 @@ def norm_rotary(query, key, query_weight, key_weight, positions, frequencies, ep
         if tracked:
             both = _NormRotary.apply(query, key, query_weight, key_weight, *how)
             return (both, None) if key is None else both
-        return _normed(query, key, query_weight, key_weight, (torch.empty_like(query), _like(key)), *how)
+        return _normed(query, key, query_weight, key_weight, (_lib.rows_like(query), _like(key)), *how)
     if tracked:
         raise ValueError('out= takes no part in a gradient')
     if len(out) != 2 or (out[1] is None) != (key is None) or out[0] is None:

@@ -218,6 +218,31 @@ def test_broadcast_gradients_and_views():
     check(grads[2], both, 'dw of a shared weight')
 
 
+@pytest.mark.parametrize('step', [1, 5, 64])
+def test_rows_that_overlap(step):
+    """Queries and keys as windows that slide over one sequence, `step` elements a token, and the same rows rotated alone."""
+    from streamvoxel_amd.stream.rotary import norm_rotary, rotary
+    g = torch.Generator().manual_seed(step)
+    line = torch.randn(2, 3, 6 * step + 64, generator=g).to(torch.bfloat16).to(DEV)
+    q, k = line.unfold(2, 64, step), line[:, :2].unfold(2, 64, step)
+    w = (1 + 0.3 * torch.randn(64, generator=g)).to(DEV)
+    positions, freq = torch.arange(7), 50.0 ** (-torch.arange(32, dtype=torch.float64) / 32)
+    dy = [torch.randn(t.shape, generator=g).to(torch.bfloat16).to(DEV) for t in (q, k)]
+    leaves = [t.detach().requires_grad_() for t in (q, k, w)]
+    out = norm_rotary(leaves[0], leaves[1], leaves[2], None, positions.to(DEV), freq.to(DEV))
+    plain = norm_rotary(q, k, w, None, positions.to(DEV), freq.to(DEV))
+    grads = torch.autograd.grad(out, leaves, dy)
+    for i, (x, weight) in enumerate(((q, w), (k, None))):
+        ref = reference(x, weight, positions[None].expand(2, -1), freq, 'half', 1.0, 1e-6, dy[i])
+        check(out[i], ref['y'], 'y')
+        check(grads[i], ref['dx'], 'dx')
+        assert torch.equal(out[i], plain[i])
+        if i == 0:
+            check(grads[2], ref['dw'], 'dw')
+    rows, pairs = q.double().cpu(), pair_sum(q.double().cpu(), 32, 'half')
+    check(rotary(q, positions.to(DEV), freq.to(DEV)), (turn64(rows, positions[None], freq, 'half'), 8 * E * pairs), 'rotary')
+
+
 def test_in_place_in_the_projection_and_refused_places():
     from streamvoxel_amd.stream.rotary import norm_rotary
     q, k, wq, wk, *_ = inputs(2, 10, 4, 2, 64, torch.bfloat16, torch.bfloat16, 8)

@@ -279,6 +279,18 @@ def test_bad_pages_and_lengths(n, kind):
     assert not paged_attention(q, *args, causal=True, window=50, sinks=2, **pool.exponents()).any()
 
 
+def test_queries_that_overlap():
+    """Queries as windows that slide over one sequence, 8 elements a token: their copies' results."""
+    from streamvoxel_amd.stream.paged import paged_attention
+    _case('overlapping queries')
+    pool = pool_of('int8', [40, 17], 2, 64, 32, 3)
+    query = torch.randn(2, 4, 8 * 6 + 64, generator=torch.Generator().manual_seed(9)).to(torch.bfloat16).to(DEV).unfold(2, 64, 8)
+    got, want = (paged_attention(q, *pool.args(), causal=True, window=9, sinks=2, **pool.exponents())
+                 for q in (query, query.contiguous()))
+    assert torch.equal(got, want)
+    check(got, query, pool, window=9, sinks=2)
+
+
 def test_a_window_as_long_as_everything_is_no_window():
     """The same bits where every key is in sight and the kernels cut alike."""
     from streamvoxel_amd.stream.paged import paged_attention

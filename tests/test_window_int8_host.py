@@ -188,3 +188,11 @@ def test_tensors_that_lie_apart():
         else:
             seen[1] += 1
     assert min(seen) > 200
+
+
+@pytest.mark.parametrize('stride', [(24, 8, 1, 1), (1, 1, 1, 1), (100, 1, 8, 1), (64, 16, 8, 1), (0, 0, 0, 1), (96, 8, 24, 1)], ids=str)
+def test_results_of_rows_that_overlap_have_a_contiguous_head_dim(stride):
+    x = torch.empty(400).as_strided((2, 3, 4, 8), stride)
+    y = _lib.rows_like(x)
+    assert y.shape == x.shape and y.stride(-1) == 1 and not _lib.stacked(y)
+    assert len({sum(i * s for i, s in zip(at, y.stride())) for at in torch.cartesian_prod(*map(torch.arange, x.shape)).tolist()}) == 192
