@@ -518,8 +518,8 @@ typedef struct svhip_paged_cache {
  * before the rotation. int8: a block's exponent is the least, 1 to 248, with every magnitude <= 127 2^(exponent - 127), of
  * the block's new rows (rotated, in fp32), and not below the one it has if rows in front of them, of the same window, are in
  * the block: those codes are then divided by the power of two that the exponent grew by, rounded to nearest even, as new ones
- * are. A block's rows are written in order: what stands behind the new rows (`before`) is yet to be written. Infinities count as the
- * largest magnitude, NaN as 0, and set `bad`. A token whose key or page is bad is not written. Key and value rows bf16,
+ * are. A block's rows are written in order: what stands behind the new rows (`before`) is yet to be written. Infinities and NaN take no
+ * part in it and set `bad`: held as +-127 (in a block of zeros beside them under exponent 248) and 0. A token whose key or page is bad is not written. Key and value rows bf16,
  * 16-byte aligned.
  * Beside svhip_kv_write (FastSlotForward.encode + _write, streamvoxel/stream/fast_ops.py:228-250), which rewrites a
  * window's slab whole; no counterpart in the reference.

@@ -125,14 +125,21 @@ __device__ __forceinline__ uint32_t most_bits(const float (&x)[16]) {
 // The most that a block can hold, and its bits.
 __device__ __forceinline__ float int8_reach() { return kInt8Most * exponent_value(kInt8Top); }
 
-// What int8 cannot hold: NaN as 0, the rest cut.
-__device__ __forceinline__ void cut_item(float (&x)[16]) {
+// What int8 cannot hold: finite values are cut to the reach, NaN becomes 0. Infinities stay (their code is that of 0 until
+// mark_infinities) and take no part in the block's magnitude, since one would round all other rows of the block to 0, older ones
+// for good. The bits of the largest finite magnitude.
+__device__ __forceinline__ uint32_t cut_item(float (&x)[16]) {
   const float reach = int8_reach();
+  uint32_t bits = 0;
 #pragma unroll
   for (int i = 0; i < 16; ++i) {
-    const float v = x[i] == x[i] ? x[i] : 0.f;
-    x[i] = fminf(fmaxf(v, -reach), reach);
+    const float v = x[i] == x[i] ? x[i] : 0.f, w = fminf(fmaxf(v, -reach), reach);
+    const bool finite = fabsf(v) < INFINITY;
+    x[i] = finite ? w : v;
+    const uint32_t u = finite ? __float_as_uint(w) & 0x7fffffffu : 0u;
+    bits = u > bits ? u : bits;
   }
+  return bits;
 }
 
 __device__ __forceinline__ void store_item(uint8_t* row, const Places& at, bool runs, const float (&x)[16], float f) {
@@ -150,11 +157,30 @@ __device__ __forceinline__ void store_item(uint8_t* row, const Places& at, bool 
   }
 }
 
-// The exponent of a block whose new rows' largest magnitude has these bits (cut to the reach) and that had `had`. The rows
-// that are there, `first`, first + step, .. of the lane's 8-byte runs, go with it where it grows (127 2^-8 and less round to 0).
-__device__ __forceinline__ int settle(const AppendArgs& a, const Block& blk, const Piece& p, uint32_t bits, int had, int lanes,
-                                      int lane, bool writes) {
-  int code = block_exponent(__uint_as_float(bits));
+// Infinities of a row that is written: the largest number of their block, whatever it stands for.
+__device__ __forceinline__ void mark_infinities(uint8_t* row, const Places& at, const float (&x)[16]) {
+#pragma unroll
+  for (int i = 0; i < 16; ++i) {
+    const int j = i & 7;
+    if (fabsf(x[i]) == INFINITY && j < (i < 8 ? at.n0 : at.n1)) {
+      row[(i < 8 ? at.first : at.second) + j] = static_cast<uint8_t>(x[i] > 0.f ? 127 : 0x81);
+    }
+  }
+}
+
+// 0 where all lanes' bits are finite; bit 0: a lane has an infinity, bit 1: or NaN.
+constexpr uint32_t kInfinite = 0x7f800000u;
+__device__ __forceinline__ uint32_t wild_bits(uint32_t bits) {
+  return (__builtin_amdgcn_ballot_w64(bits == kInfinite) != 0ull ? 1u : 0u) |
+         (__builtin_amdgcn_ballot_w64(bits >= kInfinite) != 0ull ? 2u : 0u);
+}
+
+// The exponent of a block whose new rows' largest finite magnitude has these bits (cut to the reach) and that had `had`; a
+// block of zeros and infinities alone (`infinite`) takes the largest. The rows that are there, `first`, first + step, .. of the
+// lane's 8-byte runs, go with it where it grows (127 2^-8 and less round to 0).
+__device__ __forceinline__ int settle(const AppendArgs& a, const Block& blk, const Piece& p, uint32_t bits, bool infinite, int had,
+                                      int lanes, int lane, bool writes) {
+  int code = infinite && bits == 0 && blk.older == 0 ? kInt8Top : block_exponent(__uint_as_float(bits));
   if (blk.older > 0) {
     if (had >= code) {
       code = had < kInt8Top ? had : kInt8Top;
@@ -209,22 +235,30 @@ __device__ __forceinline__ void hold_few(const AppendArgs& a, const RowItems& it
     const uint32_t b = most_bits(x[k]);
     bits = b > bits ? b : bits;
   }
+  uint32_t wild = 0;
   if (__builtin_expect(__builtin_amdgcn_ballot_w64(bits > __float_as_uint(int8_reach())) != 0ull, 0)) {
-    if (__builtin_amdgcn_ballot_w64(bits >= 0x7f800000u) != 0ull) set_bad(a.pages);
+    wild = wild_bits(bits);
+    if (wild) set_bad(a.pages);
     bits = 0;
 #pragma unroll
     for (int k = 0; k < PASSES; ++k) {
-      cut_item(x[k]);
-      const uint32_t b = most_bits(x[k]);
+      const uint32_t b = cut_item(x[k]);
       bits = b > bits ? b : bits;
     }
   }
-  const int code = settle(a, blk, p, __float_as_uint(wave_max(__uint_as_float(bits))), __builtin_amdgcn_readfirstlane(had), 64,
-                          lane, lane == 0);
+  const int code = settle(a, blk, p, __float_as_uint(wave_max(__uint_as_float(bits))), wild & 1, __builtin_amdgcn_readfirstlane(had),
+                          64, lane, lane == 0);
 #pragma unroll
   for (int k = 0; k < PASSES; ++k) {
     const int r = r0 + 64 / LPR * k;
     if (r < blk.rows) store_item(p.rows + (blk.older + r) * p.sr, at, TURN == kTurnNone || a.runs, x[k], exponent_value(254 - code));
+  }
+  if (__builtin_expect(wild, 0)) {
+#pragma unroll
+    for (int k = 0; k < PASSES; ++k) {
+      const int r = r0 + 64 / LPR * k;
+      if (r < blk.rows) mark_infinities(p.rows + (blk.older + r) * p.sr, at, x[k]);
+    }
   }
 }
 
@@ -354,28 +388,47 @@ paged_append_int8_kernel(AppendArgs a, RowItems items, unsigned first_group, int
       }
       const int were = __builtin_amdgcn_readfirstlane(had);
       if (u + 1 < units) load(u + 1);
+      uint32_t wild = 0;
       if (__builtin_expect(__builtin_amdgcn_ballot_w64(bits > __float_as_uint(int8_reach())) != 0ull, 0)) {
-        if (__builtin_amdgcn_ballot_w64(bits >= 0x7f800000u) != 0ull) set_bad(a.pages);
+        wild = wild_bits(bits);
+        if (wild) set_bad(a.pages);
         bits = 0;
 #pragma unroll
         for (int k = 0; k < kPasses; ++k) {
-          cut_item(x[k]);
-          const uint32_t b = most_bits(x[k]);
+          const uint32_t b = cut_item(x[k]);
           bits = b > bits ? b : bits;
         }
       }
-      const uint32_t mine = __float_as_uint(wave_max(__uint_as_float(bits)));
+      uint32_t mine = __float_as_uint(wave_max(__uint_as_float(bits)));
+      if (__builtin_expect(wild & 1, 0) && mine == 0) mine = kInfinite;
       if (lane == 0) s_most[turn][wave] = mine;
       __syncthreads();
       uint32_t most = s_most[turn][0];
 #pragma unroll
       for (int w = 1; w < kWaves; ++w) most = s_most[turn][w] > most ? s_most[turn][w] : most;
+      bool infinite = false;
+      if (__builtin_expect(__builtin_amdgcn_readfirstlane(most) == kInfinite, 0)) {  // of a wave that has nothing else but zeros
+        infinite = true;
+        most = 0;
+#pragma unroll
+        for (int w = 0; w < kWaves; ++w) {
+          const uint32_t other = s_most[turn][w];
+          most = other < kInfinite && other > most ? other : most;
+        }
+      }
       turn ^= 1;  // (a wave is behind the next unit's barrier before it writes here again)
-      const float f = exponent_value(254 - settle(a, blk, p, most, were, kAppendThreads, tid, tid == 0));
+      const float f = exponent_value(254 - settle(a, blk, p, most, infinite, were, kAppendThreads, tid, tid == 0));
 #pragma unroll
       for (int k = 0; k < kPasses; ++k) {
         const int r = kFew * (wave + kWaves * k) + r0;
         if (r < blk.rows) store_item(p.rows + (blk.older + r) * p.sr, at, TURN == kTurnNone || a.runs, x[k], f);
+      }
+      if (__builtin_expect(wild, 0)) {
+#pragma unroll
+        for (int k = 0; k < kPasses; ++k) {
+          const int r = kFew * (wave + kWaves * k) + r0;
+          if (r < blk.rows) mark_infinities(p.rows + (blk.older + r) * p.sr, at, x[k]);
+        }
       }
     }
   }

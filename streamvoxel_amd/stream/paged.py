@@ -130,8 +130,9 @@ def paged_append(key, value, k_pages, v_pages, page_table, lengths, cu_tokens=No
     int8: a value is held as a whole number of at most 127 times its block's power of two, off by half of that at most. The
     block's is the least that holds its new keys, and not below the one it has if keys of the window stand in front of them
     in the block: where it grows, those are rounded to the new one (what that adds up to stays under one step of it, however the block
-    was filled). Keys behind the new ones in a block (`before`) count as yet to be written. Infinities are held as the
-    largest number and NaN as 0, and set `bad`. No two windows may write into one block."""
+    was filled). Keys behind the new ones in a block (`before`) count as yet to be written. An infinity is held as the
+    largest number of its block, 127 times the power of two that the finite values there ask for (the largest of all where
+    there are only zeros), NaN as 0; both set `bad`. No two windows may write into one block."""
     _lib.require_one_gpu(key, value, k_pages, v_pages, page_table, lengths, cu_tokens, positions, frequencies, k_exponents,
                          v_exponents, bad)
     code = _check_pool(k_pages, v_pages, page_table, lengths, k_exponents, v_exponents, bad)

@@ -1,0 +1,111 @@
+"""An int8 paged cache on the GPU where a value, a scale or a failure is out of the ordinary: infinities beside good keys.
+
+Tolerances. What is compared is the append itself on inputs that differ in the elements under test alone: equal codes."""
+import math
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+DEV = 'cuda:0'
+
+
+def _case(msg):
+    print(f'[gpu-case] {msg}', flush=True)
+
+
+def fresh(pages, H, page, D, block):
+    k, v = [torch.zeros(pages, H, page, D, dtype=torch.int8, device=DEV) for _ in 'kv']
+    e = {name: torch.zeros(pages, H, page // block, dtype=torch.uint8, device=DEV) for name in ('k_exponents', 'v_exponents')}
+    return k, v, e
+
+
+@pytest.mark.parametrize('layout, half', [(None, 0), ('half', 24), ('half', 5), ('interleaved', 24), ('interleaved', 7)])
+@pytest.mark.parametrize('D, block', [(48, 16), (64, 64), (128, 32), (128, 64)])
+@pytest.mark.parametrize('older, n', [(0, 1), (20, 1), (3, 9), (0, 64), (40, 90), (5, 200)])
+def test_an_infinity_or_nan_beside_good_keys(older, n, D, block, layout, half):
+    """The other elements, older rows among them, are held as if a zero stood in its place: it is the largest number of its
+    block (NaN 0), and sets `bad`."""
+    from streamvoxel_amd.stream.paged import paged_append
+    _case(f'infinities older={older} n={n} D={D} block={block} {layout} {half}')
+    H, page = 3, 64
+    g = torch.Generator().manual_seed(D + n)
+    total = older + n
+    pages = -(-total // page)
+    table = torch.randperm(pages, generator=g).to(torch.int32)[None].to(DEV)
+    rows = torch.randn(2, 1, H, total, D, generator=g).to(torch.bfloat16)
+    how = {}
+    if layout:
+        how = dict(layout=layout, frequencies=(1.0 / (1.3 + torch.arange(half, dtype=torch.float64))).to(DEV))
+    # (row, head, element, value): in the first, a middle and the last new row, in either half of a row.
+    marks = [(older, 0, 1, math.inf), (older + n // 2, 1, D // 2 + 3, -math.inf), (total - 1, 2, 4, math.nan),
+             (total - 1, 0, D - 2, math.inf)]
+    if layout:                       # (what an infinity is turned to depends on the signs of cos and sin alone)
+        pair = lambda d: (None if d >= 2 * half else (d % half, d % half + half) if layout == 'half' else (d & ~1, d | 1))
+    else:
+        pair = lambda d: None
+    wild, calm = rows.clone(), rows.clone()
+    for j, h, d, value in marks:
+        for e in pair(d) or (d,):
+            wild[:, 0, h, j, e] = calm[:, 0, h, j, e] = 0.0
+    for j, h, d, value in marks:
+        wild[:, 0, h, j, d] = value
+    pools = []
+    for x in (calm, wild):
+        k, v, e = fresh(pages, H, page, D, block)
+        if older:
+            paged_append(*rows[:, :, :, :older].to(DEV), k, v, table, torch.tensor([older], dtype=torch.int32, device=DEV), **e, **how)
+        bad = torch.zeros(1, dtype=torch.int32, device=DEV)
+        paged_append(*x[:, :, :, older:].to(DEV), k, v, table, torch.tensor([total], dtype=torch.int32, device=DEV), bad=bad, **e, **how)
+        at = table[0].cpu().long()
+        line = lambda t: t.cpu()[at].transpose(0, 1).reshape(H, -1, *t.shape[3:])
+        pools.append((line(k), line(v), line(e['k_exponents']), line(e['v_exponents']), int(bad)))
+    (ck, cv, cke, cve, calm_bad), (wk, wv, wke, wve, wild_bad) = pools
+    assert calm_bad == 0 and wild_bad == 1
+    assert torch.equal(cke, wke) and torch.equal(cve, wve)
+    code = lambda x: 0 if math.isnan(x) else int(math.copysign(127, x))
+    for j, h, d, value in marks:
+        cv[h, j, d] = code(value)
+        if layout and pair(d):
+            a, b = pair(d)
+            angle = j * float(how['frequencies'][d % half if layout == 'half' else d // 2])
+            c, s = math.cos(angle), math.sin(angle)
+            if d == a:
+                turned = value * c, (math.nan if s == 0 else value * s)
+            else:
+                turned = (math.nan if s == 0 else -value * s), value * c
+            ck[h, j, a], ck[h, j, b] = map(code, turned)
+        else:
+            ck[h, j, d] = code(value)
+    assert torch.equal(ck, wk) and torch.equal(cv, wv)
+
+
+@pytest.mark.parametrize('older', [0, 2])
+@pytest.mark.parametrize('n', [1, 40, 62])
+@pytest.mark.parametrize('D', [48, 128])
+def test_infinities_among_zeros(n, older, D):
+    """A block that has nothing else but zeros holds an infinity as the largest number there is; a finite value anywhere in it,
+    or a key in front, sets the block's scale in its place."""
+    from streamvoxel_amd.stream.paged import paged_append
+    H, page, block = 2, 64, 64
+    table = torch.zeros(1, 1, dtype=torch.int32, device=DEV)
+    length = lambda x: torch.tensor([x], dtype=torch.int32, device=DEV)
+    for others in (0.0, 3.0):
+        k, v, e = fresh(1, H, page, D, block)
+        old = torch.full((1, H, older, D), 0.75, dtype=torch.bfloat16, device=DEV)
+        if older:
+            paged_append(old, old, k, v, table, length(older), **e)
+        x = torch.zeros(1, H, n, D, dtype=torch.bfloat16)
+        x[0, 1, n // 2, 5], x[0, 0, n - 1, 6] = -math.inf, math.inf
+        if others:
+            x[0, :, 0, 7] = others
+        x, bad = x.to(DEV), torch.zeros(1, dtype=torch.int32, device=DEV)
+        paged_append(x, x, k, v, table, length(older + n), bad=bad, **e)
+        exponent = 122 if others else (120 if older else 248)      # 3 = 96 * 2^-5, 0.75 = 96 * 2^-7
+        want = torch.zeros(H, page, D, dtype=torch.int8)
+        want[:, :older] = 24 if others else 96
+        want[1, older + n // 2, 5], want[0, older + n - 1, 6] = -127, 127
+        if others:
+            want[:, older, 7] = 96
+        assert int(bad) == 1 and torch.equal(k[0].cpu(), want) and torch.equal(v, k)
+        assert (e['k_exponents'] == exponent).all() and (e['v_exponents'] == exponent).all()
