@@ -94,7 +94,7 @@ __device__ __forceinline__ float exponent_value(int code) { return __uint_as_flo
 
 // int8 blocks: whole numbers of at most kInt8Most times a power of two of at most 2^(kInt8Top - 127), the largest of them
 // with 127 of it in bf16. (Other bytes are read as the nearest of these: a code's value is finite whatever stands there, and a
-// score of -inf stays one when it is scaled.)
+// score of -inf stays one when it is scaled: by the call's scale too, paged_attention.hpp.)
 constexpr int kInt8Top = 248;
 constexpr float kInt8Most = 127.f;
 __device__ __forceinline__ float int8_power(uint32_t byte) {

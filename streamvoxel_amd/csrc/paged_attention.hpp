@@ -363,11 +363,26 @@ __device__ __forceinline__ f32x16_t scores(const Rows<KS>& s, const bf16x8_t (&k
 }
 
 // int8: a block's keys enter the score product as their codes; what 16 of them stand for, a power of two, is put to the scores
-// (an FMA's factor where the weights are formed) and not to every element of the keys: 32 kHalves keys, 16 each.
+// (an FMA's factor where the weights are formed) and not to every element of the keys: 32 kHalves keys, 16 each. (So a
+// query's products with codes must fit fp32: elements up to 2^114.)
 template <int kHalves>
 struct KeyScales {
   float of[2 * kHalves];
 };
+
+// That factor with the call's scale. Not 0, which would make a masked score's -inf NaN: 2^-149 in a smaller one's place adds less
+// than 2^-21 to an exponent for any finite score. Not infinite, which a score of 0 would be NaN with: with the largest number in
+// its place scores from 2^-98 on pass 2^30 either way (weights_of). The row form bounds the product, the tile form, where
+// one lane forms a block's power of two for all, that power, from its byte (the row form so: 64 tokens through windows of 1024
+// 57.4 us for 56.5; the tile form by the product: 4 chunks of 512 337 us for 334).
+__device__ __forceinline__ float bounded_scale(float scale, float f) {
+  return __builtin_amdgcn_fmed3f(scale * f, 0x1p-149f, kFltMax);
+}
+__device__ __forceinline__ float bounded_power(float scale, uint32_t byte) {
+  const int x = __builtin_amdgcn_frexp_expf(scale);  // scale in [2^(x - 1), 2^x)
+  const int low = -21 - x > 1 ? -21 - x : 1, top = 255 - x < kInt8Top ? 255 - x : kInt8Top, e = static_cast<int>(byte);
+  return exponent_value(e < low ? low : (e < top ? e : top));
+}
 
 // Scores x of a block of 32 kHalves keys, `key0` the first: those that a row does not see masked, and the running
 // maximum moved for a score more than kMaxHigh above it (the weights then stay below 2^20, which fp32 sums and bf16
@@ -435,13 +450,14 @@ __device__ __forceinline__ void bound_scores(const PagedArgs& a, Rows<KS>& s, f3
 // what a rounding adds to the one it adds to the other: 0.0022 from 64 bits, relative, where weights in
 // fp32 leave the result's own rounding, 0.0017. m is the rounded product of a score: beyond scores of
 // 2^30 what its rounding leaves of the largest weight's exponent no longer fits fp32, and the row is NaN.
-template <int ST, int KS>
+// BOUNDED: int8's factors f are bounded_power's.
+template <int ST, bool BOUNDED, int KS>
 __device__ __forceinline__ void weights_of(const Rows<KS>& s, const f32x16_t& x, float scale, const float* f,
                                            bf16x8_t (&pb)[2]) {
   const float nm = -s.m;
 #pragma unroll
   for (int ks = 0; ks < 2; ++ks) {
-    const float sl2 = ST == kInt8 ? scale * f[ks] : scale;
+    const float sl2 = ST != kInt8 ? scale : (BOUNDED ? scale * f[ks] : bounded_scale(scale, f[ks]));
 #pragma unroll
     for (int j = 0; j < 8; j += 2) {
       const f32x2_t two = {__builtin_amdgcn_exp2f(__builtin_fmaf(x[8 * ks + j], sl2, nm)),

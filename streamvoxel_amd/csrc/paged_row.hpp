@@ -270,7 +270,7 @@ __device__ __forceinline__ void row_work(const PagedArgs& a, int place, char* sV
 #pragma unroll
       for (int t = 0; t < kHalves; ++t) {
         bf16x8_t pb[2];
-        weights_of<ST, KS>(s, x[t], a.scale_log2, f.of + 2 * t, pb);
+        weights_of<ST, false, KS>(s, x[t], a.scale_log2, f.of + 2 * t, pb);
         add_values<KS, kSubBytes>(s, pb, cur + 32 * t * kRow * 2, rvt);
       }
       kv = kvn;
@@ -334,7 +334,7 @@ __device__ __forceinline__ void row_work(const PagedArgs& a, int place, char* sV
 
 // Windows that are all of the row form.
 template <int ST, bool WIN, int KS>
-__global__ __launch_bounds__(kPagedThreads, ST == kInt8 && KS <= 6 ? 3 : 2) void paged_row_kernel(PagedArgs a, unsigned first_group) {
+__global__ __launch_bounds__(kPagedThreads, ST == kInt8 && KS <= 6 ? (KS <= 2 ? 4 : 3) : 2) void paged_row_kernel(PagedArgs a, unsigned first_group) {
 #if defined(__HIP_DEVICE_COMPILE__)
   constexpr int kFirst = coded(ST) ? 4 : 2;
   typedef RowLds<ST, KS, kFirst> L;

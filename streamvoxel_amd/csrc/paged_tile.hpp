@@ -240,7 +240,7 @@ __device__ __forceinline__ void tile_work(const PagedArgs& a, int place, char* s
     if constexpr (ST == kInt8) {
       if ((wave & 1) == 0 && lane == 0) {
 #pragma unroll
-        for (int i = 0; i < 2; ++i) s_scale[buffer][(wave >> 1) + 2 * i] = int8_power(kst.e[i]);
+        for (int i = 0; i < 2; ++i) s_scale[buffer][(wave >> 1) + 2 * i] = bounded_power(a.scale_log2, kst.e[i]);
       }
     }
     if constexpr (kCodes) {
@@ -273,7 +273,7 @@ __device__ __forceinline__ void tile_work(const PagedArgs& a, int place, char* s
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
       bf16x8_t pb[2];
-      weights_of<ST, KS>(s, x[t], a.scale_log2, f.of + 2 * t, pb);
+      weights_of<ST, true, KS>(s, x[t], a.scale_log2, f.of + 2 * t, pb);
       add_values<KS, kSubBytes>(s, pb, sV + 32 * t * kRow * 2, rvt);
     }
   };

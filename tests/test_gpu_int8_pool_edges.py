@@ -1,10 +1,15 @@
-"""An int8 paged cache on the GPU where a value, a scale or a failure is out of the ordinary: infinities beside good keys.
+"""An int8 paged cache on the GPU where a value, a scale or a failure is out of the ordinary: infinities beside good keys,
+scores scaled by next to nothing or by far too much.
 
-Tolerances. What is compared is the append itself on inputs that differ in the elements under test alone: equal codes."""
+Tolerances. Append: what is compared is the append itself on inputs that differ in the elements under test alone: equal codes.
+Attention: that of test_gpu_paged_int8.py."""
 import math
 
 import pytest
 import torch
+
+from test_gpu_paged import queries
+from test_gpu_paged_int8 import Int8Pool, check
 
 pytestmark = pytest.mark.gpu
 DEV = 'cuda:0'
@@ -109,3 +114,33 @@ def test_infinities_among_zeros(n, older, D):
             want[:, older, 7] = 96
         assert int(bad) == 1 and torch.equal(k[0].cpu(), want) and torch.equal(v, k)
         assert (e['k_exponents'] == exponent).all() and (e['v_exponents'] == exponent).all()
+
+
+@pytest.mark.parametrize('n', [1, 3, 40, 200])
+@pytest.mark.parametrize('scale', [1e-2, 1e-8, 1e-25, 1e-38, 1e-42], ids=str)
+@pytest.mark.parametrize('D, H, heads, page, block', [(64, 4, 2, 64, 64), (48, 3, 3, 16, 16), (128, 8, 1, 128, 32)])
+def test_scores_scaled_by_next_to_nothing(D, H, heads, page, block, scale, n):
+    """Blocks of zeros (their power of two is 2^-126), blocks that end inside and keys masked in them: the weights are all but
+    equal, and keys that a token does not see stay out."""
+    from streamvoxel_amd.stream.paged import paged_attention
+    _case(f'int8 scale={scale} n={n} D={D} page={page} block={block}')
+    pool = Int8Pool([70, 0, 333, 1, 1000], heads, D, page, 5, block)
+    for at in (0, pool.k.shape[0] // 2):                       # every second page: codes of zero under the least exponent
+        pool.k[at::2] = 0
+        pool.ke[at::2] = 1
+    q = queries(5, H, n, D, n)
+    for how in (dict(causal=True), dict(causal=False), dict(causal=True, window=20, sinks=3)):
+        got = paged_attention(q, *pool.args(), scale=scale, **how, **pool.exponents())
+        check(got, q, pool, scale=scale, **how)
+
+
+@pytest.mark.parametrize('n', [1, 40])
+def test_queries_of_zeros_at_the_largest_scales(n):
+    """Scores of 0 times whatever is still 0: every key in sight weighs the same."""
+    from streamvoxel_amd.stream.paged import paged_attention
+    pool = Int8Pool([70, 333], 2, 64, 64, 5, 32)
+    pool.ke[:] = 248
+    q = torch.zeros(2, 4, n, 64, dtype=torch.bfloat16, device=DEV)
+    for scale in (1.0, 200.0, 1e30):
+        got = paged_attention(q, *pool.args(), scale=scale, causal=True, **pool.exponents())
+        check(got, q, pool, scale=scale)
