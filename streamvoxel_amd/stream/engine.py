@@ -107,21 +107,25 @@ def _local_kv(model, context, local):
 
 def extend_condition(model, context, index, local, positions):
     """Further local context of slot `index` behind what a PagedContext holds of it: `local` [1, L, W] projected by every layer,
-    the keys rotated at `positions` [1, L, 3]; nothing that is there is written again. The slot holds the new keys once
-    every layer's are written, and stays as it was on error."""
+    the keys rotated at `positions` [1, L, 3]; nothing that is there is written again, but for an int8 block that the slot's keys
+    end inside of, which the new ones may round again. The slot holds the new keys once every layer's are written, and stays as
+    it was on error."""
     held, dev = context.host_lengths[index], context.lengths.device
     grown = held + local.shape[1]
     positions = positions.to(device=dev, dtype=torch.float32)[0].contiguous()
     context.reserve(index, grown)
+    tails = []
     try:
         lengths = torch.full((1,), grown, dtype=torch.int32, device=dev)
-        # (All projected before the first is written: an int8 block that both old and new keys are in may change with them.)
-        for j, (cross, key, value) in enumerate(list(_local_kv(model, context, local))):
+        for j, (cross, key, value) in enumerate(_local_kv(model, context, local)):
+            tails += context.tail(j, index)
             freq = cross.rope.frequencies.to(device=dev, dtype=torch.float32)
             context.append(j, key, value, index=index, lengths=lengths, positions=positions, frequencies=freq,
                            layout='axial')
     except BaseException:
         context.resize(index, held)
+        for part, was in tails:
+            part.copy_(was)
         raise
     context.resize(index, grown)
 

@@ -310,6 +310,7 @@ class PagedContext:
         self.layers, self.batch, self.heads, self.head_dim = layers, batch, heads, head_dim
         self.pages, self.page_size, self.kv_dtype = pages, page_size, kv_dtype
         self.max_pages = pages if max_pages is None else max_pages
+        self.block = block if kv_dtype == 'int8' else None
         dt = dict(bf16=torch.bfloat16, fp8=torch.float8_e4m3fn, int8=torch.int8)[kv_dtype]
         pool = lambda dtype, *shape: [torch.empty(pages, heads, *shape, dtype=dtype, device=device) for _ in range(layers)]
         self.k, self.v = pool(dt, page_size, head_dim), pool(dt, page_size, head_dim)
@@ -450,6 +451,18 @@ class PagedContext:
         lengths = self.lengths[at] if lengths is None else lengths
         paged_append(key, value, self.k[layer], self.v[layer], self.table[at], lengths, cu_tokens=cu_tokens,
                      k_exponents=self.k_exponents[layer], v_exponents=self.v_exponents[layer], bad=self.bad, **how)
+
+    def tail(self, layer, index):
+        """What an `append` behind window `index` of `layer` may change of its keys, with a copy of it each: the codes and the
+        exponents of an int8 block that they end inside of. Nothing for the other kinds."""
+        held = self.host_lengths[index]
+        if self.block is None or held % self.block == 0:
+            return []
+        at, row = divmod(held - 1, self.page_size)
+        page, block = self._owned[index][at], row // self.block
+        parts = [t[layer][page, :, block * self.block:row + 1] for t in (self.k, self.v)]
+        parts += [t[layer][page, :, block] for t in (self.k_exponents, self.v_exponents)]
+        return [(t, t.clone()) for t in parts]
 
     def write(self, layer, index, key, value, prefix=None, positions=None, frequencies=None):
         """Window `index` of `layer` anew, as `CachedContext.write`: keys [0, P) from `prefix` = (prefix_k, prefix_v)

@@ -1,0 +1,62 @@
+"""The slot engine over int8 pools on the GPU: an extension that fails after it has written."""
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+DEV = 'cuda:0'
+
+
+def _case(msg):
+    print(f'[gpu-case] {msg}', flush=True)
+
+
+def small(kv_dtype='int8', batch=3, **how):
+    from streamvoxel_amd import synth
+    from streamvoxel_amd.stream.engine import SlotEngine
+    model = synth.StepModel(classes=40, voxel_shape=(64, 16, 16), width=192, depth=4, heads=8, control_width=192,
+                            control_depth=2, seed=3)
+    for p in model.parameters():
+        p.data = p.data.to(torch.bfloat16)
+    model = model.to(DEV)
+    spec = synth.WindowSpec(height=64, tile=16, num_classes=40)
+    engine = SlotEngine(model, spec, DEV, batch, l1_cap=2, l2_cap=8, pages=24, page_size=64, kv_dtype=kv_dtype, **how)
+    conds = [synth.condition(model, P, L, seed=60 + i, device=DEV) for i, (P, L) in enumerate([(32, 500), (9, 72), (0, 300)][:batch])]
+    return model, engine, conds
+
+
+@pytest.mark.parametrize('kv_dtype', ['bf16', 'fp8', 'int8'])
+@pytest.mark.parametrize('held', [111, 128, 1])
+def test_an_extension_that_fails_in_its_second_layer(held, kv_dtype, monkeypatch):
+    """The keys that were there read back bit for bit (int8: those that share a block with new keys 64 times as large, which the
+    first layer's append had rounded again), the slot has its length and its pages, and the extension can be made after all."""
+    from streamvoxel_amd.stream.engine import Encoded
+    _case(f'extension fails held={held} {kv_dtype}')
+    model, engine, conds = small(kv_dtype, capture=False)
+    local, positions = conds[2].local, conds[2].positions
+    engine.load_slot(2, Encoded(conds[2].prefix, local[:, :held], positions[:, :held]))
+    engine.wait_loads()
+    context = engine.context
+    before, free = [context.read(layer, 2) for layer in range(2)], context.free_pages
+    append, calls = context.append, []
+
+    def failing(layer, *args, **how):
+        append(layer, *args, **how)
+        calls.append(layer)
+        if layer == 1:
+            raise RuntimeError('the second layer fails')
+
+    monkeypatch.setattr(context, 'append', failing)
+    with pytest.raises(RuntimeError, match='second layer'):
+        engine.extend_slot(2, 64 * local[:, held:], positions[:, held:])
+    monkeypatch.undo()
+    engine.wait_loads()
+    assert calls == [0, 1] and context.host_lengths[2] == held and context.free_pages == free
+    assert context.lengths.tolist()[2] == held
+    for layer in range(2):
+        for a, b in zip(before[layer], context.read(layer, 2)):
+            assert torch.equal(a, b), layer
+    engine.extend_slot(2, 64 * local[:, held:], positions[:, held:])
+    engine.wait_loads()
+    assert context.host_lengths[2] == 300 and int(context.bad) == 0
+    if kv_dtype == 'int8' and held % 64:                # (the older keys of that block do change then)
+        assert not torch.equal(before[0][0], context.read(0, 2)[0][:, :held])
