@@ -260,6 +260,7 @@ class SlotEngine:
         self.group_origin = torch.tensor([0.0, float(getattr(spec, 'y_origin', 0.0)), 0.0], device=dev)
         self.origin = self.group_origin.expand(self.batch, 3).contiguous()
         self.side = torch.cuda.Stream(device=dev)
+        self._extended = {}    # slot -> event behind its last extension, where that changes keys in place (int8)
         self.sizes = buckets(self.batch)
         # Largest first, so the full batch's intermediates are the pool's first tenants.
         self.steps = StepGraphs(dev, self.forward, sorted(self.sizes, reverse=True), capture=capture)
@@ -322,8 +323,8 @@ class SlotEngine:
         """Slot `index` of a paged engine takes further local context (`local` [1, L, W], `positions` [1, L, 3]) behind the
         condition that it holds, on the side stream like `load_slot`: a neighbour that has come in costs its own keys, not
         the window's. The slot's tokens stay; on error (a pool that has too few pages, a `local` of another width) its context
-        does too. int8: the block that the condition ends in is rounded again where its keys share it, so a step over the slot
-        comes behind `wait_loads`."""
+        does too. int8: the block that the condition ends in may be rounded again, so the next steps over the slot wait until
+        it is (steps over bf16 and e4m3 pools, and over other slots, do not)."""
         index = int(index)
         if not isinstance(self.context, PagedContext):
             raise ValueError('extending a slot needs an engine with pages')
@@ -336,7 +337,22 @@ class SlotEngine:
             for t in (local, positions):
                 if t.is_cuda:
                     t.record_stream(self.side)
-            extend_condition(self.model, self.context, index, local, positions)
+            try:
+                extend_condition(self.model, self.context, index, local, positions)
+            finally:
+                if self.context.kv_dtype == 'int8':
+                    self._extended[index] = self.side.record_event()
+
+    def _wait_extended(self, n):
+        """The current stream waits for the extensions of the first n slots that change keys in place."""
+        if not self._extended or torch.cuda.is_current_stream_capturing():
+            return
+        stream = torch.cuda.current_stream(self.device)
+        for index, event in list(self._extended.items()):
+            if event.query():
+                del self._extended[index]
+            elif index < n:
+                stream.wait_event(event)
 
     def wait_loads(self):
         torch.cuda.current_stream(self.device).wait_stream(self.side)
@@ -356,6 +372,7 @@ class SlotEngine:
     # -- the step
     def forward(self, n):
         """The step's forward over the first n slots -> PatchLogits [n] (class head rows in patch order)."""
+        self._wait_extended(n)
         return self.forward_fn(self.tokens[:n], self.timestep[:n], self.origin[:n], self.group_origin)
 
     def _set_time(self, timestep):
@@ -371,7 +388,9 @@ class SlotEngine:
         """Logits of the first `bucket(count)` slots (all slots when count is None) at `timestep` (one per slot,
         or one for all): a graph replay, or the eager step if no graph was captured."""
         self._set_time(timestep)
-        return self.steps(self.batch if count is None else self.bucket(count))
+        n = self.batch if count is None else self.bucket(count)
+        self._wait_extended(n)
+        return self.steps(n)
 
     def eager(self, timestep):
         self._set_time(timestep)

@@ -60,3 +60,56 @@ def test_an_extension_that_fails_in_its_second_layer(held, kv_dtype, monkeypatch
     assert context.host_lengths[2] == 300 and int(context.bad) == 0
     if kv_dtype == 'int8' and held % 64:                # (the older keys of that block do change then)
         assert not torch.equal(before[0][0], context.read(0, 2)[0][:, :held])
+
+
+@pytest.mark.parametrize('step', ['replay', 'replay of two', 'eager', 'forward'])
+def test_a_step_waits_for_an_extension_that_changes_keys_in_place(step, monkeypatch):
+    """The side stream is busy when the extension is asked for, and the step over the slot is asked for at once: it sees the whole
+    extension. A step over the slots in front of it does not wait."""
+    from streamvoxel_amd.stream.engine import Encoded
+    _case(f'step behind an extension: {step}')
+    model, engine, conds = small()
+    index = 1 if step == 'replay of two' else 2
+    local, positions = conds[2].local, conds[2].positions
+    part = lambda a, b: (64 * local[:, a:b], positions[:, a:b])
+    for i in (0, 1, 2):
+        engine.load_slot(i, Encoded(conds[2].prefix, *part(0, 111)) if i == index else conds[i])
+    engine.wait_loads()
+    call = {'replay': lambda: engine.replay(0.5), 'replay of two': lambda: engine.replay(0.5, 2), 'eager': lambda: engine.eager(0.5),
+            'forward': lambda: engine.forward(3)}[step]
+    waits, wait_event = [], torch.cuda.Stream.wait_event
+    monkeypatch.setattr(torch.cuda.Stream, 'wait_event', lambda self, event: (waits.append(event), wait_event(self, event))[1])
+    with torch.inference_mode():
+        a = torch.randn(8192, 8192, device=DEV, dtype=torch.bfloat16)
+        with torch.cuda.stream(engine.side):           # (what the first calls set up)
+            a = (a @ a).clamp(-1, 1)
+        engine.extend_slot(index, *part(111, 120))
+        engine.wait_loads()
+        before = call().patches.clone()
+        first = engine.replay(0.5, 1).patches.clone()
+        torch.cuda.synchronize()
+        with torch.cuda.stream(engine.side):
+            for _ in range(100):
+                a = (a @ a).clamp(-1, 1)
+        engine.extend_slot(index, *part(120, 300))
+        event = engine._extended[index]
+        lone = engine.replay(0.5, 1).patches.clone()
+        assert event not in waits
+        got = call().patches.clone()
+        assert event in waits
+        engine.wait_loads()
+        want = call().patches
+    assert torch.equal(lone, first)
+    assert torch.equal(got, want) and not torch.equal(got, before)
+    torch.cuda.synchronize()
+    engine.replay(0.5)
+    assert not engine._extended
+
+
+@pytest.mark.parametrize('kv_dtype', ['bf16', 'fp8'])
+def test_steps_over_pools_whose_keys_stay_do_not_wait(kv_dtype):
+    model, engine, conds = small(kv_dtype, capture=False)
+    engine.load_slot(0, conds[1])
+    engine.extend_slot(0, conds[2].local, conds[2].positions)
+    assert not engine._extended
+    engine.wait_loads()
