@@ -182,8 +182,17 @@ def dtype_code(dtype):
 
 
 def stacked(t):
-    """True when elements of a tensor lie on each other (a dimension expanded with stride 0): no place for results."""
-    return 0 in t.stride() and any(s == 0 and n > 1 for n, s in zip(t.shape, t.stride()))
+    """True when elements of a tensor lie on each other (a dimension expanded with stride 0, windows that slide by less than their
+    length): no place for results. (Also where only the order of the dimensions' strides leaves it open.)"""
+    if t.is_contiguous():
+        return False
+    dims = [(s, n) for n, s in zip(t.shape, t.stride()) if n != 1]
+    reach = 1                      # elements from the first to the last one of the dimensions so far
+    for s, n in sorted(dims):
+        if s < reach:
+            return t.numel() > 0
+        reach += (n - 1) * s
+    return False
 
 
 def rows_like(t):
