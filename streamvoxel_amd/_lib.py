@@ -204,11 +204,14 @@ def rows_like(t):
 
 def byte_span(t):
     """[first, last) device byte addresses a tensor's elements occupy (its strides taken into account)."""
-    if t.numel() == 0:
-        return (t.data_ptr(), t.data_ptr())
-    extent = sum((n - 1) * abs(s) for n, s in zip(t.shape, t.stride())) + 1
-    low = t.data_ptr() + sum((n - 1) * s for n, s in zip(t.shape, t.stride()) if s < 0) * t.element_size()
-    return (low, low + extent * t.element_size())
+    at, n = t.data_ptr(), 1
+    if t.is_contiguous():
+        return at, at + t.nbytes
+    for size, stride in zip(t.shape, t.stride()):
+        if size == 0:
+            return at, at
+        n += (size - 1) * stride
+    return at, at + n * t.element_size()
 
 
 def apart(a, b):
@@ -249,3 +252,12 @@ def overlaps(a, b):
         return False
     (a0, a1), (b0, b1) = byte_span(a), byte_span(b)
     return a0 < b1 and b0 < a1
+
+
+def overlaps_any(out, *read):
+    """The same of a result and any of the tensors (or None) that are read while it is written."""
+    low, high = byte_span(out)
+    for t in read:
+        if t is not None and t.data_ptr() < high and low < byte_span(t)[1]:
+            return True
+    return False

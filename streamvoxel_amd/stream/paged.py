@@ -210,8 +210,8 @@ def paged_read(k_pages, v_pages, page_table, lengths, n, cu_keys=None, before=0,
         for t in out:
             if t.shape != shape or t.dtype != torch.bfloat16 or t.stride(-1) != 1 or _lib.stacked(t):
                 raise ValueError(f'out must be a pair of bf16 {shape} with a contiguous head_dim and a place for every element')
-            if any(_lib.overlaps(t, pages) for pages in (k_pages, v_pages)):
-                raise ValueError('out must not share memory with the pages')
+            if _lib.overlaps_any(t, k_pages, v_pages, page_table, lengths, cu_keys, k_exponents, v_exponents, bad):
+                raise ValueError('out must not share memory with the pages, their exponents, the table, lengths or borders')
         if _lib.overlaps(key, value) and not _lib.apart(key, value):
             raise ValueError('the two of out must not share memory')
     sk = _windows(key, cu_keys, B, 'key')[2]
@@ -255,6 +255,8 @@ def paged_attention(query, k_pages, v_pages, page_table, lengths, cu_queries=Non
         raise ValueError('out must be bf16 like query with a contiguous head_dim and a place for every element')
     elif _lib.overlaps(given, out) and (given.data_ptr() != out.data_ptr() or given.stride() != out.stride()):
         raise ValueError('out must be query itself or memory that query does not share')
+    elif _lib.overlaps_any(out, k_pages, v_pages, page_table, lengths, cu_queries, k_exponents, v_exponents, bad):
+        raise ValueError('out must not share memory with the pages, their exponents, the table, lengths or borders')
     so = _windows(out, cu_queries, B, 'out')[2]
     scale = D ** -0.5 if scale is None else float(scale)
     if window is None:

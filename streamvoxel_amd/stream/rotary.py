@@ -131,6 +131,8 @@ def rotary(x, positions, frequencies, layout='half', amplitude=1.0, out=None):
             raise ValueError("out must have x's shape and type, a contiguous head_dim and a place for every element")
         if _lib.overlaps(x, out) and (x.data_ptr() != out.data_ptr() or x.stride() != out.stride()):
             raise ValueError('out must be x itself or memory that x does not share')
+        if _lib.overlaps_any(out, positions, frequencies):
+            raise ValueError('out must not share memory with positions or frequencies')
     return _launch(x, out, positions, frequencies, layout, float(amplitude), 0)
 
 
@@ -288,6 +290,8 @@ def norm_rotary(query, key, query_weight, key_weight, positions, frequencies, ep
             same = other is x and (o is x or o.data_ptr() == x.data_ptr() and o.stride() == x.stride())
             if not same and _lib.overlaps(o, other) and not _lib.apart(o, other):
                 raise ValueError('out must be its input itself or memory that neither input shares')
+        if _lib.overlaps_any(o, query_weight, key_weight, positions, frequencies):
+            raise ValueError('out must not share memory with weights, positions or frequencies')
     if out[1] is not None and out[1] is not key and _lib.overlaps(*out) and not _lib.apart(*out):
         raise ValueError('the two of out must not share memory')
     return _normed(query, key, query_weight, key_weight, tuple(out), *how)

@@ -42,3 +42,55 @@ def test_rows_that_slide_over_each_other():
     with pytest.raises(ValueError, match='place for every element'):
         paged_append(k, k, torch.empty_like(pages), pages, torch.zeros(2, 1, dtype=torch.int32, device=DEV),
                      torch.full((2,), 5, dtype=torch.int32, device=DEV))
+
+
+def test_memory_that_the_call_reads():
+    """One buffer holds a result's rows and, inside of them, what a call reads beside its rows."""
+    from streamvoxel_amd.stream.paged import paged_attention, paged_read
+    from streamvoxel_amd.stream.rotary import norm_rotary, rotary
+    B, H, n, D = 2, 4, 8, 64
+
+    def inside(t):
+        """A [B, H, n, D] result whose buffer begins with what t holds, and t there."""
+        buffer = torch.zeros(B * H * n * D, dtype=torch.bfloat16, device=DEV)
+        there = buffer.view(torch.uint8)[:t.nbytes].view(t.dtype).view(t.shape)
+        there.copy_(t)
+        return buffer.view(B, H, n, D), there
+
+    x = torch.randn(B, H, n, D, device=DEV).to(torch.bfloat16)
+    p, f = torch.arange(n, device=DEV), torch.ones(32, dtype=torch.float64, device=DEV)
+    w = torch.ones(D, device=DEV)
+    for which, t in enumerate((p, f, w, w)):
+        out, there = inside(t)
+        args = [p, f, w, w]
+        args[which] = there
+        for pair in ((out, torch.empty_like(x)), (torch.empty_like(x), out)):
+            with pytest.raises(ValueError, match='share memory'):
+                norm_rotary(x, x, args[2], args[3], args[0], args[1], out=pair)
+        if which < 2:
+            with pytest.raises(ValueError, match='share memory'):
+                rotary(x, args[0], args[1], out=out)
+    pool = Int8Pool([100, 7], H, D, 64, 1, 32)
+    k, v, table, L = pool.args()
+    e = pool.exponents()
+    cu, bad = torch.tensor([0, 8, 16], dtype=torch.int32, device=DEV), torch.zeros(1, dtype=torch.int32, device=DEV)
+    names = ('page_table', 'lengths', 'k_exponents', 'v_exponents', 'bad')
+    held = dict(page_table=table, lengths=L, bad=bad, **e)
+    for name in names:
+        out, there = inside(held[name])
+        how = {**held, name: there}
+        with pytest.raises(ValueError, match='share memory'):
+            paged_attention(x, k, v, out=out, **how)
+        for pair in ((out, torch.empty_like(out)), (torch.empty_like(out), out)):
+            with pytest.raises(ValueError, match='share memory'):
+                paged_read(k, v, n=n, out=pair, **how)
+    out, there = inside(cu)
+    packed = out.view(H, B * n, D)
+    with pytest.raises(ValueError, match='share memory'):
+        paged_attention(x.view(H, B * n, D), k, v, out=packed, cu_queries=there, **held)
+    with pytest.raises(ValueError, match='share memory'):
+        paged_read(k, v, n=B * n, out=(packed, torch.empty_like(packed)), cu_keys=there, **held)
+    pages = torch.zeros(4, H, 64, D, dtype=torch.bfloat16, device=DEV)
+    for kv in ((pages, torch.zeros_like(pages)), (torch.zeros_like(pages), pages)):
+        with pytest.raises(ValueError, match='share memory'):
+            paged_attention(x, *kv, table, L, out=pages.view(-1)[:x.numel()].view(x.shape))

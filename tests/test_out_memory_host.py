@@ -36,3 +36,24 @@ def test_elements_on_each_other():
     for t in (rows[:, :1].expand(2, 7, 3, 8), torch.zeros(40).unfold(0, 8, 4), torch.zeros(40).unfold(0, 8, 7),
               rows.as_strided((2, 2, 2, 8), (4, 48, 16, 1))):
         assert _lib.stacked(t)
+
+
+def test_spans_and_what_meets_them():
+    g = torch.Generator().manual_seed(2)
+    draw = lambda low, high: int(torch.randint(low, high, (1,), generator=g))
+    flat = torch.zeros(400)
+    met = 0
+    for _ in range(2000):
+        a, b, c = [flat.as_strided([draw(0 if i else 1, 4) for _ in range(3)], [draw(0, 12) for _ in range(3)], draw(0, 300))
+                   for i in range(3)]
+        for t in (a, b, c):
+            at = places(t)
+            first, last = _lib.byte_span(t)
+            assert (last - first == 0) if not at else (first, last) == (flat.data_ptr() + 4 * min(at), flat.data_ptr() + 4 * max(at) + 4)
+        share = lambda t: _lib.byte_span(a)[0] < _lib.byte_span(t)[1] and _lib.byte_span(t)[0] < _lib.byte_span(a)[1]
+        assert _lib.overlaps(a, b) == share(b)
+        assert _lib.overlaps_any(a, b, None, c) == (share(b) or share(c))
+        if set(places(a)) & set(places(b)):
+            met += 1
+            assert _lib.overlaps_any(a, b)
+    assert met > 50 and not _lib.overlaps_any(a, None)
