@@ -286,13 +286,20 @@ def norm_rotary(query, key, query_weight, key_weight, positions, frequencies, ep
             continue
         if o.shape != x.shape or o.dtype != x.dtype or o.stride(-1) != 1 or _lib.stacked(o):
             raise ValueError("out must have its input's shape and type, a contiguous head_dim and a place for every element")
-        for other in (query, key):
-            same = other is x and (o is x or o.data_ptr() == x.data_ptr() and o.stride() == x.stride())
-            if not same and _lib.overlaps(o, other) and not _lib.apart(o, other):
-                raise ValueError('out must be its input itself or memory that neither input shares')
+        same = o is x or o.data_ptr() == x.data_ptr() and o.stride() == x.stride()
+        if not same and _lib.overlaps(o, x) and not _lib.apart(o, x):
+            raise ValueError('out must be its input itself or memory that neither input shares')
         if _lib.overlaps_any(o, query_weight, key_weight, positions, frequencies):
             raise ValueError('out must not share memory with weights, positions or frequencies')
-    if out[1] is not None and out[1] is not key and _lib.overlaps(*out) and not _lib.apart(*out):
-        raise ValueError('the two of out must not share memory')
+    # A side's result and the other side, whose rows other workgroups read and write, be it the same tensor.
+    first, second = out
+    crossed = [(first, key)]
+    if second is not key:
+        crossed.append((first, second))
+    if first is not query or second is not key:
+        crossed.append((second, query))
+    for a, b in crossed:
+        if b is not None and a is not None and _lib.overlaps(a, b) and not _lib.apart(a, b):
+            raise ValueError('out must not share memory with the other input or the other result')
     return _normed(query, key, query_weight, key_weight, tuple(out), *how)
 

@@ -94,3 +94,31 @@ def test_memory_that_the_call_reads():
     for kv in ((pages, torch.zeros_like(pages)), (torch.zeros_like(pages), pages)):
         with pytest.raises(ValueError, match='share memory'):
             paged_attention(x, *kv, table, L, out=pages.view(-1)[:x.numel()].view(x.shape))
+
+
+def test_queries_and_keys_that_are_one_tensor():
+    """Their results may be fresh or lie elsewhere, but not in the tensor that the other side still reads."""
+    from streamvoxel_amd.stream.rotary import norm_rotary
+    x = torch.randn(2, 4, 8, 64, device=DEV).to(torch.bfloat16)
+    p, f = torch.arange(8, device=DEV), torch.ones(32, dtype=torch.float64, device=DEV)
+    w, v = torch.rand(64, device=DEV), torch.rand(64, device=DEV)
+    want = norm_rotary(x, x, w, v, p, f)
+    other, again = torch.empty_like(x), x.view(2, 4, 8, 64)
+    for q, k, out in ((x, x, (x, x)), (x, x, (x, other)), (x, x, (other, x)), (x, again, (x, again)), (x, again, (x, other)),
+                      (x, again, (other, again)), (x, x, (other, other)), (x, x[:, 1:3], (x, other[:, :2])),
+                      (x[:, 1:3], x, (other[:, :2], x))):
+        with pytest.raises(ValueError, match='memory'):
+            norm_rotary(q, k, w, v, p, f, out=out)
+    got = norm_rotary(x, x, w, v, p, f, out=(other, torch.empty_like(x)))
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+    rows = torch.randn(2, 8, 6, 64, device=DEV).to(torch.bfloat16)
+    q, k = rows[:, :, :4].transpose(1, 2), rows[:, :, 4:].transpose(1, 2)
+    want = norm_rotary(q, k, w, v, p, f)
+    spare = torch.empty_like(rows)
+    for out in ((spare[:, :, :4].transpose(1, 2), k), (q, spare[:, :, 4:].transpose(1, 2)), (q, k)):
+        keep = rows.clone()
+        got = norm_rotary(q, k, w, v, p, f, out=out)
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+        rows.copy_(keep)
+    alone = norm_rotary(q, None, w, None, p, f, out=(q, None))
+    assert alone[0] is q and torch.equal(q, want[0])
