@@ -401,7 +401,8 @@ class SlotEngine:
         """Class-major logits [1, C, Y, Z, X] of `item` at timestep 1 from an independent path: the model's own
         forward over the unpadded condition when the model has one (the reference's `unpadded_logits`,
         streamvoxel/stream/engine.py:87-102), else this library's step on a one-slot cache sized to the
-        condition alone (no padding beyond the 64-key block) and captured nowhere."""
+        condition alone (no padding beyond the 64-key block; a slab of the engine's type, int8 pages for an int8 engine) and
+        captured nowhere."""
         enc = self.encode(item)
         dev = self.device
         tokens = torch.full((1, *self.shape), self.classes, dtype=torch.int64, device=dev)
@@ -413,9 +414,12 @@ class SlotEngine:
                                  prefix_kv=stacked, local=enc.local.to(dev), local_positions=enc.positions.to(dev))
             return out, 'model_forward'
         length = (enc.prefix[0][0].shape[1] if len(enc.prefix) else 0) + enc.local.shape[1]
-        kv_dtype = self.context.kv_dtype
-        ctx = CachedContext(self.context.layers, 1, self.context.heads, self.context.head_dim, max(length, 1), dev,
-                            'bf16' if kv_dtype == 'int8' else kv_dtype)
+        held = self.context
+        if held.kv_dtype == 'int8':       # (a slab holds none)
+            ctx = PagedContext(held.layers, 1, held.heads, held.head_dim, max(1, -(-length // held.page_size)), dev,
+                               held.page_size, kv_dtype='int8', block=held.block)
+        else:
+            ctx = CachedContext(held.layers, 1, held.heads, held.head_dim, max(length, 1), dev, held.kv_dtype)
         write_condition(self.model, ctx, 0, enc)
         step = StepForward(self.model, ctx, concurrent=False)
         out = step(tokens, time, self.origin[:1], self.group_origin)
@@ -426,7 +430,8 @@ class SlotEngine:
         """The reference's gate report (fast_ops.py:351-375): slot 0 (and 1) take `item` (and `other`); the eager
         step against its graph replay (bit-identical), against the independent reference logits (argmax agreement
         >= 0.999 and mean |difference| <= 0.05) and the two-slot bucket against the full batch (the same bar).
-        Slots 0 and 1 keep these conditions afterwards."""
+        Slots 0 and 1 keep these conditions afterwards. What is held in 8 bits is compared with itself where the model has no
+        forward of its own, and with what that computes in bf16 where it has one."""
         reference, source = self._reference_logits(item)
         reference = reference.float()
         self.load_slot(0, item)

@@ -113,3 +113,13 @@ def test_steps_over_pools_whose_keys_stay_do_not_wait(kv_dtype):
     engine.extend_slot(0, conds[2].local, conds[2].positions)
     assert not engine._extended
     engine.wait_loads()
+
+
+def test_the_numerical_gate_compares_one_arithmetic():
+    """A one-slot pool of the same kind: what the engine's batch and pages change, not what 8 bits cost beside bf16."""
+    _case('int8 engine: numerical_gate')
+    model, engine, conds = small()
+    report = engine.numerical_gate(conds[0], conds[1])
+    assert report['graph_used'] and report['graph_equal'] and report['bucket_close'] and report['padded_close'], report
+    assert report['reference'] == 'one_slot_exact_cache' and report['options']['kv_dtype'] == 'int8'
+    assert engine.packed.lengths.tolist()[:2] == [532, 81] and int(engine.context.bad) == 0
