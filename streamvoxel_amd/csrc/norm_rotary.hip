@@ -414,12 +414,14 @@ int norm_rotary(const char* name, const svhip_norm_rotary_args* args, bool grad,
   SVHIP_REQUIRE((c.H == 0 || (c.q && (grad ? c.dq != nullptr : c.out_q != nullptr))) &&
                     (c.Hk == 0 || (c.k && (grad ? c.dk != nullptr : c.out_k != nullptr))) && c.positions && c.freq,
                 "%s: null pointer", name);
+  // (One that fp32 rounds to 0 would make a row of zeros NaN.)
+  const float eps = c.eps > 0. && c.eps < 0x1p-149 ? 0x1p-149f : static_cast<float>(c.eps);
   NormArgs a{{{c.q, c.dq, c.q_weight, c.out_q, c.sq_b, c.sq_h, c.sq_n, c.soq_b, c.soq_h, c.soq_n, c.sdq_b, c.sdq_h, c.sdq_n,
                static_cast<int>(c.H), 1, 1, 0, 0},
               {c.k, c.dk, c.k_weight, c.out_k, c.sk_b, c.sk_h, c.sk_n, c.sok_b, c.sok_h, c.sok_n, c.sdk_b, c.sdk_h, c.sdk_n,
                static_cast<int>(c.Hk), 1, 1, 0, 0}},
              c.positions, c.freq, c.sp_b, c.sp_n, static_cast<int>(c.N), row_items(D, half),
-             c.positions_wide != 0, c.weight_dtype == SVHIP_F32, static_cast<float>(c.eps), static_cast<float>(c.amplitude),
+             c.positions_wide != 0, c.weight_dtype == SVHIP_F32, eps, static_cast<float>(c.amplitude),
              weighed ? static_cast<float*>(c.workspace) : nullptr};
   const int64_t run = c.dtype == SVHIP_F32 ? 4 : 8;
   bool vec = half % 8 == 0 && D % 8 == 0;
