@@ -144,3 +144,15 @@ def test_queries_of_zeros_at_the_largest_scales(n):
     for scale in (1.0, 200.0, 1e30):
         got = paged_attention(q, *pool.args(), scale=scale, causal=True, **pool.exponents())
         check(got, q, pool, scale=scale)
+
+
+@pytest.mark.parametrize('kind', ['bf16', 'fp8', 'int8'])
+@pytest.mark.parametrize('n', [1, 3, 100])
+def test_a_window_over_everything_has_the_bits_of_none(n, kind):
+    from streamvoxel_amd.stream.paged import paged_attention
+    from test_gpu_paged_int8 import pool_of
+    pool = pool_of(kind, [3000, 300, 500], 2, 64, 64, 3)
+    q = queries(3, 4, n, 64, n)
+    want = paged_attention(q, *pool.args(), causal=True, **pool.exponents())
+    for window, sinks in ((3000, 0), (1 << 40, 0), (1 << 62, 1 << 62)):
+        assert torch.equal(paged_attention(q, *pool.args(), causal=True, window=window, sinks=sinks, **pool.exponents()), want)
