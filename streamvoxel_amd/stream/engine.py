@@ -348,10 +348,8 @@ class SlotEngine:
         if not self._extended or torch.cuda.is_current_stream_capturing():
             return
         stream = torch.cuda.current_stream(self.device)
-        for index, event in list(self._extended.items()):
-            if event.query():
-                del self._extended[index]
-            elif index < n:
+        for index, event in list(self._extended.items()):      # (another thread may load meanwhile)
+            if index < n and not event.query():
                 stream.wait_event(event)
 
     def wait_loads(self):
