@@ -11,7 +11,9 @@
 // within the group, a pair turns within its lane, and a lane's weights stay in registers. A thread's first row is on its
 // way before the angles are formed, and the next one while it computes. Measured: 32 768 tokens of 16 and 4 heads of 128 in
 // bf16 (336 MB) 74 us, 4.5 TB/s of a copy's 5.1, their gradient (503 MB) 117, 4.3, and 4.7 for the weights' sums; 8192 of 12
-// and 12 of 64 (50 MB) 13.3; 64 tokens 5.5. Both sides in a workgroup, the weights in LDS: 50.9 us for the 50 MB, 873 for the
+// and 12 of 64 (50 MB) 13.0, gradient 22.6; 64 tokens 5.5; fp32 141 and 209 (4.8 TB/s), 23.8 and 36. Where pairs or rows are no whole runs
+// of 8 (12 pairs of 96, 10 of 80) every element is read and written by itself, 8 or 16 apart from lane to lane: 199 and 273 us,
+// 169 and 244, for 54 and 85 of 16 pairs of 96. Both sides in a workgroup, the weights in LDS: 50.9 us for the 50 MB, 873 for the
 // 839 MB of a result and its gradient (197 now). Rows a thread: 2, 4, 8: 18.7, 14.5, 15.5 us for the 50 MB; workgroups of a
 // gradient: 768 (three a CU at once), 1024, 2048: 204, 219, 208 us for the pair.
 #include "rotary.hpp"

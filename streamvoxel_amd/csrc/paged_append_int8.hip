@@ -8,9 +8,12 @@
 // the rows of a longer one and meet over the magnitude in LDS (a wave for all 64 rows held 256 registers: 32 chunks 53 us, a
 // turned one spilled: 196). The workgroups of a slot of consecutive tokens (blockIdx.y of them) find the blocks whose
 // first new token is among them and share out (block, slice of the heads); a workgroup forms a block's (cos, sin) in LDS once
-// for the heads of its slice. Bound: HBM, and for few blocks the chain length, page, rows, magnitude. Measured: 32 ragged chunks
-// of up to 1024 tokens of 8 x 128, blocks of 32 (105 MB) 28.6 us, 3.7 TB/s, turned 39; 64 chunks of 2048 (805 MB) 170 us, 4.7
-// TB/s; 64 tokens of 16 x 64 6.9 us.
+// for the heads of its slice. Bound: HBM, and for few blocks the chain length, page, rows, magnitude. Measured on
+// pools in turn: 32 ragged chunks of up to 1024 tokens of 8 x 128, blocks of 32 (105 MB) 35.1 us, 3.1 TB/s (28.6 on one pool,
+// which the caches hold in part), turned 41.4 and 41.9, blocks of 64 35.3 and 47.5: a piece's rows are asked for behind its angles and a
+// barrier; 64 chunks of 2048 (805 MB) 164 us, 4.9 TB/s, turned 169; 64 tokens of 16 x 64 6 to 7 us. Three axes: 8480 tokens of
+// 8 x 48 22.4 us, 32 chunks of 16 x 48 50 (as they are 32); where pairs are no multiple of 8 rows go element by element, which
+// lie 16 apart from lane to lane: 12 x 72 151 us (as they are 38).
 #include "paged_append.hpp"
 
 namespace svhip {
@@ -263,7 +266,7 @@ __device__ __forceinline__ void hold_few(const AppendArgs& a, const RowItems& it
 }
 
 // LPR: lanes of a row. `heads`: of a slice, `slices` of them.
-// Where a wave has one row of every lane there is room for six workgroups a CU (32 chunks 30.4 us for 32.2); more spill.
+// Where a wave has one row of every lane there is room for six workgroups a CU (32 chunks 34.3 us, five 36.2); more spill.
 template <int TURN, int LPR, int kBlock>
 __global__ __launch_bounds__(kAppendThreads, kBlock > 16 && kBlock * LPR <= kAppendThreads ? 6 : 2) void
 paged_append_int8_kernel(AppendArgs a, RowItems items, unsigned first_group, int heads, int slices) {

@@ -17,15 +17,21 @@
 //     us, 5.1 TB/s; one token over 30 MB 9.1 us, a chain of loads. One wave a row of its own, with shuffles instead
 //     of the products, took 14.9 ms.
 // int8 pools (one power of two for 16 keys at least): codes decode to bf16 whole numbers, a block's keys are scaled by a
-// factor of their scores, values as they are decoded. 64 tokens over 736 MB of int8 pages 161 us, 4.6 TB/s (two waves a
-// SIMD for three, keys scaled as they are decoded: 205 for 187 on pools in turn); 4 causal chunks of 512, 16 heads to 4 of
-// 128, up to 16 384 keys 315 us, 12 of them the join, where bf16 takes 290: a code costs a conversion (four cycles a wave),
-// half a packing and, of a value, a product; e4m3 half a conversion. Values scaled in their weights, the sums' other factor
-// the inverse: no faster.
+// factor of their scores, values as they are decoded. On pools in turn, bf16's and e4m3's times on the same card: 64 tokens
+// over 736 MB of int8 pages 157 us, 4.7 TB/s (two waves a SIMD for three, keys scaled as they are decoded: a tenth more); 4
+// causal chunks of 512, 16 heads to 4 of 128, up to 16 384 keys 323 us, 12 of them the join, for 281 and 296 (on other cards
+// 315 to 330, the first after a pause up to 350: the clock); 8 x 1024 queries of 12 x 64 over all of 1552 to 9744 keys 238
+// for 203 and 214; a mix of 12 chunks and 36 tokens, 8 heads to 4 of 96, without a window 410 for 340 and 369, through one of 2000 keys
+// 91 for 79 and 91; 5, 8 and 16 rows of 64 windows over 2048 to 4096 keys, 8 heads of 64, 65, 69, 71 us, 3 TB/s. A code costs a
+// conversion (four cycles a wave), half a packing and, of a value, a product; e4m3 half a conversion. Values scaled in their
+// weights, the sums' other factor the inverse: no faster.
 // A sliding window (WIN) leaves out what no token of a workgroup sees: keys are walked by their place among the others, the first
 // ones in whole blocks of 64 and those from the first token's window on. A prompt of 16 384 tokens, windows of 1024 and 16
-// first keys, 16 heads of 64: 104 us, 650 TFLOP/s of what is seen, 830 of what is walked; one token, windows of 4096 11.4 us
-// and a join of 4.4; 64 tokens over int8 windows of 1024 58 us, 76 over bf16.
+// first keys, 16 heads of 64: 107 us (104 to 114 from card to card; e4m3 118, int8 129), 630 TFLOP/s of what is seen, 710 of what
+// its waves compute: they skip two of the 20 blocks that a tile of 128 tokens stages. One token of 16 heads to 4 of 128, windows
+// of 4096 11.4 us and a join of 4.2, both as a graph 16.0, 13.2 where 4096 keys are all there are (12 heads over 9744 keys:
+// of 64 16.3, of 128 20.9: two blocks a wave whatever the cache, a chain that grows with the row). 64 tokens through windows of
+// 1024 of 16 x 64 in int8 58 us, e4m3 and bf16 71.
 // Packed windows may be of both (paged_mixed.hpp). Either form may cut a window's keys into parts for several
 // workgroups; a part leaves O, its running maximum and its sum in fp32 and paged_join_kernel joins them in order (4.5
 // us for one token, 12 for 34 MB of parts). What is cut is planned on the device, where the lengths are: by every

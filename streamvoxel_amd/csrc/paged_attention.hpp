@@ -8,12 +8,12 @@ namespace svhip {
 
 constexpr int kPagedThreads = 256;
 constexpr int kRows = 32;          // rows of a wave
-// Rows of a window up to which it is of the row form, bf16 and e4m3. At 4, 8, 16, 32 rows a key head the row form
+// Rows of a window up to which it is of the row form, bf16 and codes. At 4, 8, 16, 32 rows a key head the row form
 // takes 47, 57, 59, 85 us and tiles 42, 46, 41, 46 (64 windows of 512 to 1024 keys, 8 key heads of 128); 16 windows
 // of 2048 to 4096 keys: 42, 50, 59, 82 and 38, 41, 44, 48; e4m3, 64 windows of 2048 to 4096 keys of 64: 51, 57, 56,
-// 71 and 72, 73, 73, 76 (int8, 5, 8, 16 rows: 71, 72, 76 and 94, 96, 93; 8 heads of 128 123, 130, 138 and 130, 131, 128; through
-// windows of 1000 keys 43, 47, 49 and 40, 42, 38). With one of 64 windows 60 times as long as the others, 4 rows: 113 and 160; 200 windows of
-// 1024 keys: 161 and 183.
+// 71 and 72, 73, 73, 76. int8 has e4m3's limit: at 5, 8 and 16 rows 71, 72, 76 and 94, 96, 93 us, with 8 heads of 128 123, 130,
+// 138 and 130, 131, 128; through windows of 1000 keys tiles are the faster ones, 43, 47, 49 and 40, 42, 38, and a limit of its
+// own there is left. With one of 64 windows 60 times as long as the others, 4 rows: 113 and 160; 200 windows of 1024 keys: 161 and 183.
 constexpr int kRowMost = 4, kRowMostFp8 = 16;
 constexpr int kTileRows = 128;     // rows of a tile workgroup
 // Tile workgroups below which keys are split, two for every CU (one, four: a causal chunk of 4 x 512 tokens, head_dim

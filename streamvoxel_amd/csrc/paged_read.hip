@@ -2,9 +2,9 @@
 //
 // Bound: HBM, the rows read once and written once. Workgroup = up to kReadTokens keys, all heads: where each key lies is found
 // once for all heads; a group of 8 or 16 lanes then carries a (key, head) row of keys and of values, 16 bytes out a lane,
-// kReadAhead of them in flight. Measured: 8 contexts of up to 9744 keys of 12 x 64 in int8 (218 MB) 36 us from call to call on one
-// pool, 49 on pools in turn, a copy's rate 43 (16 keys a workgroup 52; 2 and 8 in flight 50 and 47, at 8 x 128 56 and 63 for
-// 60); 1552 keys (7 MB) 5.0 us.
+// kReadAhead of them in flight. Measured: 8 contexts of up to 9744 keys of 12 x 64 in int8 (218 MB) on pools in turn 45 us, a
+// copy's rate 43 (e4m3 48, bf16, 290 MB, 54; int8 53 where nothing is left in a cache, 36 on one pool, which the caches hold in
+// part); 16 keys a workgroup 52 for 49, 2 and 8 in flight 50 and 47, at 8 x 128 56 and 63 for 60; 1552 keys (7 MB) 4.4 us, bf16 and e4m3 4.2.
 #include "paged.hpp"
 #include "rotary.hpp"
 

@@ -332,9 +332,14 @@ __device__ __forceinline__ void row_work(const PagedArgs& a, int place, char* sV
 
 #endif  // __HIP_DEVICE_COMPILE__
 
+// Workgroups a CU that the registers leave room for: int8 three up to head_dim 96, four up to 32 (64 tokens through windows of
+// 1024, head_dim 32: 43 us, three 48).
+template <int ST, int KS>
+constexpr int kRowGroups = ST == kInt8 && KS <= 6 ? (KS <= 2 ? 4 : 3) : 2;
+
 // Windows that are all of the row form.
 template <int ST, bool WIN, int KS>
-__global__ __launch_bounds__(kPagedThreads, ST == kInt8 && KS <= 6 ? (KS <= 2 ? 4 : 3) : 2) void paged_row_kernel(PagedArgs a, unsigned first_group) {
+__global__ __launch_bounds__(kPagedThreads, (kRowGroups<ST, KS>)) void paged_row_kernel(PagedArgs a, unsigned first_group) {
 #if defined(__HIP_DEVICE_COMPILE__)
   constexpr int kFirst = coded(ST) ? 4 : 2;
   typedef RowLds<ST, KS, kFirst> L;

@@ -214,11 +214,11 @@ class SlotEngine:
     `load_slot` takes an `Encoded` (or a (prefix, local, positions) tuple) itself.
     `kv_dtype` 'bf16' (the reference's cache) or 'fp8' (e4m3 with per-(window, head) scales). `pages`: the slots share a pool
     of that many pages of `page_size` keys (a `PagedContext`, e4m3 with a scale a row; 'int8' too, with one for each block
-    of a page's keys, which `extend_slot` may round again) in place of a slab of the longest condition each; a slot's context can then grow (`extend_slot`). The step takes 0.6 % longer then (e4m3 1.6 %; the
+    of a page's keys, which `extend_slot` may round again) in place of a slab of the longest condition each; a slot's context
+    can then grow (`extend_slot`). The step takes up to 0.6 % longer then (e4m3 1.6 %; int8 8.6 % longer than over bf16 slabs; the
     shipped shape, 8 slots), and where few slots step together, loading one may change the last bits of another's logits,
-    which a slab keeps. `concurrent` runs the
-    control branch on its own stream inside the step. `patchify`, `attention` and `compile` are the reference's
-    option names (fast_ops.py:168-171): 'gather' and 'conv' both run the HIP gather patchify, bit for bit the
+    which a slab keeps. `concurrent` runs the control branch on its own stream inside the step. `patchify`, `attention` and
+    `compile` are the reference's option names (fast_ops.py:168-171): 'gather' and 'conv' both run the HIP gather patchify, bit for bit the
     reference's embedding-bag form, which computes the one-hot Conv3d's sum (the reference's own test,
     tests/stream/test_live_fast_ops.py:14-21, holds the two equal); 'flex' and 'sdpa' both run the HIP attention
     kernel over the slots' key lengths (each is masked attention over the valid keys); `compile` is accepted and
